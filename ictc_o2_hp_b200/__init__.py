@@ -2,14 +2,16 @@
 
 Public names mirror the reference package ``ictc_o2_hp`` (src/ictc_o2_hp/__init__.py):
 ``TensorProduct``, ``TupleTensorProduct``, ``ComponentMajorTensorProduct``,
-``UvuTensorProduct`` and ``RadialUvuTensorProduct``.  Imports are lazy so that the
-package imports without a GPU.
+``UvuTensorProduct`` and ``RadialUvuTensorProduct``.  ``LayerNorm``, ``Linear``,
+``ResidualBlock`` and ``RadialTrunk`` (module ``dense``) are the networks around them.
+Imports are lazy so that the package imports without a GPU.
 """
 
 __version__ = "0.1.0"
 __all__ = [
     "TensorProduct", "TupleTensorProduct", "ComponentMajorTensorProduct",
-    "UvuTensorProduct", "RadialUvuTensorProduct", "__version__",
+    "UvuTensorProduct", "RadialUvuTensorProduct", "LayerNorm", "Linear", "ResidualBlock",
+    "RadialTrunk", "__version__",
 ]
 
 
@@ -23,4 +25,7 @@ def __getattr__(name):
     if name == "RadialUvuTensorProduct":
         from .radial import RadialUvuTensorProduct
         return RadialUvuTensorProduct
+    if name in {"LayerNorm", "Linear", "ResidualBlock", "RadialTrunk"}:
+        from . import dense
+        return getattr(dense, name)
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

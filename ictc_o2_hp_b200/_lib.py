@@ -22,6 +22,7 @@ NORMALIZATION = {"component": 0, "norm": 1}
 _c_float_p = ctypes.POINTER(ctypes.c_float)
 _i32, _i64, _size = ctypes.c_int32, ctypes.c_int64, ctypes.c_size_t
 _vp = ctypes.c_void_p
+_float = ctypes.c_float
 
 # name -> (restype, argtypes); must mirror include/ictc_o2_b200.h
 SIGNATURES = {
@@ -59,6 +60,17 @@ SIGNATURES = {
                                         [_i32] * 8 + [_vp, _vp, _size, _vp]),
     "ictc_o2_radial_backward_gathered": (_i32, [_vp, _vp, _i64] + [_vp] * 10 + [_i64] +
                                          [_i32] * 8 + [_i32, _vp, _vp, _size, _vp]),
+    "ictc_o2_layer_norm_forward": (_i32, [_vp, _i64] + [_vp] * 5 + [_i64, _i64, _float, _i32,
+                                                                    _i32, _vp]),
+    "ictc_o2_layer_norm_workspace": (_i32, [_i64, _i64, _i32, _i32, ctypes.POINTER(_size)]),
+    "ictc_o2_layer_norm_backward": (_i32, [_vp, _i64] + [_vp] * 4 + [_i64] + [_vp] * 4 +
+                                    [_size, _i64, _i64, _i32, _i32, _vp]),
+    "ictc_o2_linear_workspace": (_i32, [_i64, _i64, _i64, _i32, _i32, _i32,
+                                        ctypes.POINTER(_size), ctypes.POINTER(_size)]),
+    "ictc_o2_linear_forward": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _size,
+                                      _i64, _i64, _i64, _i32, _i32, _vp]),
+    "ictc_o2_linear_backward": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _i64] + [_vp] * 4 +
+                                [_size, _i64, _i64, _i64, _i32, _i32, _vp]),
     "ictc_o2_gather_rows": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _vp]),
     "ictc_o2_segment_sum": (_i32, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp]),
     "ictc_o2_graph_bad_index": (_i32, [ctypes.POINTER(_i32)]),
@@ -259,6 +271,59 @@ def radial_backward(left, angular, hidden, alpha, bias, grad_output, gx, gy, gh,
         ptr(left), ptr(angular), ptr(hidden), ptr(alpha), ptr(bias), ptr(grad_output), ptr(gx),
         ptr(gy), ptr(gh), ptr(ga), ptr(gb), left.shape[0], *rconfig, int(needed), ptr(table),
         ptr(workspace), workspace.numel(), stream_of(left.device)), "radial_backward")
+
+
+# ---------------------------------------------------------------------- dense
+# dtype and activation arguments are the C ABI's integer codes; `rows`-like tensors are
+# two-dimensional with unit stride inside a row.
+
+
+def layer_norm_workspace(rows: int, width: int, dtype: int, device: int) -> int:
+    out = _size()
+    check(load().ictc_o2_layer_norm_workspace(rows, width, dtype, device, ctypes.byref(out)),
+          "layer_norm_workspace")
+    return int(out.value)
+
+
+def layer_norm_forward(x, weight, bias, y, mean, rstd, eps, dtype, param_dtype):
+    check(load().ictc_o2_layer_norm_forward(
+        x.data_ptr(), x.stride(0), ptr(weight), ptr(bias), y.data_ptr(), ptr(mean), ptr(rstd),
+        x.shape[0], x.shape[1], eps, dtype, param_dtype, stream_of(x.device)),
+        "layer_norm_forward")
+
+
+def layer_norm_backward(x, weight, mean, rstd, grad, gx, gw, gb, workspace, dtype, param_dtype):
+    check(load().ictc_o2_layer_norm_backward(
+        x.data_ptr(), x.stride(0), ptr(weight), mean.data_ptr(), rstd.data_ptr(),
+        grad.data_ptr(), grad.stride(0), ptr(gx), ptr(gw), ptr(gb), ptr(workspace),
+        workspace.numel() if workspace is not None else 0, x.shape[0], x.shape[1], dtype,
+        param_dtype, stream_of(x.device)), "layer_norm_backward")
+
+
+def linear_workspace(rows: int, inner: int, outer: int, dtype: int, activation: int,
+                     device: int) -> tuple[int, int]:
+    fwd, bwd = _size(), _size()
+    check(load().ictc_o2_linear_workspace(rows, inner, outer, dtype, activation, device,
+                                          ctypes.byref(fwd), ctypes.byref(bwd)),
+          "linear_workspace")
+    return int(fwd.value), int(bwd.value)
+
+
+def linear_forward(x, weight, bias, residual, y, preact, workspace, outer, dtype, activation):
+    check(load().ictc_o2_linear_forward(
+        x.data_ptr(), x.stride(0), weight.data_ptr(), weight.stride(0), ptr(bias), ptr(residual),
+        residual.stride(0) if residual is not None else 0, y.data_ptr(), ptr(preact),
+        ptr(workspace), workspace.numel() if workspace is not None else 0, x.shape[0], x.shape[1],
+        outer, dtype, activation, stream_of(x.device)), "linear_forward")
+
+
+def linear_backward(x, weight, preact, grad, gx, gw, gb, workspace, rows, inner, outer, dtype,
+                    activation):
+    check(load().ictc_o2_linear_backward(
+        x.data_ptr(), x.stride(0), weight.data_ptr(), weight.stride(0), ptr(preact),
+        grad.data_ptr(), grad.stride(0), ptr(gx), ptr(gw), ptr(gb), ptr(workspace),
+        workspace.numel() if workspace is not None else 0, rows, inner, outer, dtype, activation,
+        stream_of(x.device)), "linear_backward")
 
 
 # ---------------------------------------------------------------------- graph

@@ -127,7 +127,8 @@ extern "C" int32_t ictc_o2_device_error(int32_t* code) {
   if (e != cudaSuccess) return ictc::cuda_fail(e, "cudaDeviceSynchronize");
   // every unit's flag is read and cleared; the first nonzero code is reported
   int (*const units[])(int*) = {ictc::tp_take_device_error, ictc::uvu_take_device_error,
-                                ictc::radial_take_device_error, ictc::probe_take_device_error};
+                                ictc::radial_take_device_error, ictc::probe_take_device_error,
+                                ictc::dense_take_device_error};
   int first = 0;
   for (auto take : units) {
     int value = 0;

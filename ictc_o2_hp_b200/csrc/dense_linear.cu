@@ -1,0 +1,940 @@
+// The linear layer y = act(x W^T + b) + r and its gradients.
+//
+//   p = x W^T + b,  y = act(p) + r           x [M, K], W [N, K], p and y [M, N]
+//   d = g act'(p),  dx = d W,  dW = d^T x,  db = sum_rows d,  dr = g
+//
+// Every product runs on the tensor cores with float32 accumulators in TMEM.  16-bit
+// operands enter as they are.  A float32 value is cut exactly into three bf16 parts of
+// eight significant bits each (x = x1 + x2 + x3, by truncation), and six of the nine
+// partial products are summed:
+//   a b ~ a1 b1 + (a1 b2 + a2 b1 + a2 b2 + a1 b3 + a3 b1)
+// the three left out are below 2^-22 of |a b|, 2^-24 on average.  The tensor core truncates when it adds
+// to an accumulator, so the large first term and the small others have accumulators of
+// their own, and both are moved into registers and added there, rounded to nearest,
+// every 256 elements of K.  An infinity or NaN in an operand cannot be cut; it makes the
+// element NaN or infinite, and such elements are summed again one FMA at a time.
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <type_traits>
+
+#include "common.cuh"
+#include "dense_types.cuh"
+#include "tcgen05.cuh"
+
+namespace ictc {
+namespace {
+
+// Bounded-wait codes of this unit.
+constexpr int kCodeProducer = 18, kCodeMma = 19, kCodeEpilogue = 20, kCodeDrain = 21;
+
+constexpr int kBM = 128;           // rows of an output tile
+constexpr int kBK = 64;            // K elements of a stage
+constexpr int kEpilogueWarps = 8;  // warps 0-7
+constexpr int kProducerWarps = 8;  // warps 8-15
+constexpr int kMmaWarp = kEpilogueWarps + kProducerWarps;
+constexpr int kProductThreads = (kMmaWarp + 1) * 32;
+constexpr int kGroupChunks = 4;    // float32: K stages between moves into registers
+
+struct Epilogue {
+  const void* bias;      // [n] or null
+  const void* residual;  // [m, n] or null
+  int64_t residual_stride;
+  float* preact;         // [m, n] p, or null
+  void* out;             // [m, n]
+  float* partial;        // [splits][m][n] instead of out when the K axis is split
+  int activation;
+  bool vec;              // four columns per access
+};
+
+// C[m, n] = sum over k of A(m, k) B(n, k)
+struct ProductArgs {
+  const void *a, *b;
+  int64_t m, n, k;
+  int64_t lda, ldb;      // distance of rows (K-major) or of k (MN-major), in elements
+  int tiles_m, tiles_n, splits, chunks, chunks_per_split;
+  bool vec_a, vec_b;     // every 8-element chunk inside the operand is 16-byte aligned
+  Epilogue e;
+};
+
+struct TilePos {
+  int64_t m0, n0;
+  int split, c0, c1;
+};
+
+// Work item t: the splits of K outermost; tiles in bands of eight row tiles, so that the
+// CTAs that run together share rows of A and of B in L2.
+__device__ __forceinline__ TilePos tile_at(const ProductArgs& p, int64_t t, int bn) {
+  const int64_t tiles = static_cast<int64_t>(p.tiles_m) * p.tiles_n;
+  TilePos pos;
+  pos.split = static_cast<int>(t / tiles);
+  const int64_t r = t - pos.split * tiles;
+  const int64_t band = r / (8ll * p.tiles_n);
+  const int64_t first = band * 8;
+  const int64_t high = p.tiles_m - first < 8 ? p.tiles_m - first : 8;
+  const int64_t q = r - band * 8 * p.tiles_n;
+  pos.m0 = (first + q % high) * kBM;
+  pos.n0 = (q / high) * bn;
+  pos.c0 = pos.split * p.chunks_per_split;
+  pos.c1 = pos.c0 + p.chunks_per_split < p.chunks ? pos.c0 + p.chunks_per_split : p.chunks;
+  return pos;
+}
+
+template <typename T>
+constexpr int kPieces = sizeof(T) == 4 ? 3 : 1;
+
+template <typename T, int BN>
+constexpr int kStageBytes = kPieces<T> * (kBM + BN) * 128;
+
+template <typename T, int BN>
+constexpr int kStages = sizeof(T) == 4 ? 2 : 4;
+
+constexpr int kStagingBytes = kEpilogueWarps * 4096;
+
+template <typename T, int BN>
+constexpr size_t kProductSmem = 1024 + kStages<T, BN> * kStageBytes<T, BN> + kStagingBytes + 128;
+
+// ------------------------------------------------------------------ operand loading
+// 256 producer threads bring one [ROWS x 64] operand chunk: CH pieces of eight
+// consecutive elements each.  Elements outside the operand read as zero.
+
+template <typename T, int ROWS>
+struct Held {
+  Pack<T, 8> v[ROWS / 32];
+};
+
+template <typename T, bool MN, int ROWS>
+__device__ __forceinline__ void chunk_place(int tid, int i, int* row, int* c) {
+  // K-major: 8 chunks per row; MN-major: ROWS / 8 chunks per k
+  constexpr int kPerRow = MN ? ROWS / 8 : 8;
+  *c = tid % kPerRow;
+  *row = tid / kPerRow + i * (256 / kPerRow);
+}
+
+template <typename T, bool MN, int ROWS>
+__device__ __forceinline__ void load_operand(const T* base, int64_t ld, int64_t mn0,
+                                             int64_t extent, int64_t k0, int64_t k_end, bool vec,
+                                             int tid, Held<T, ROWS>& h) {
+#pragma unroll
+  for (int i = 0; i < ROWS / 32; ++i) {
+    int row, c;
+    chunk_place<T, MN, ROWS>(tid, i, &row, &c);
+    const int64_t outer = (MN ? k0 : mn0) + row;           // index along the stride
+    const int64_t inner = (MN ? mn0 : k0) + c * 8;         // first contiguous index
+    const int64_t inner_end = MN ? extent : k_end;
+    const bool in = outer < (MN ? k_end : extent);
+    const T* src = base + outer * ld + inner;
+    if (in && vec && inner + 8 <= inner_end) {
+      if constexpr (sizeof(T) == 4) {
+        const float4 lo = __ldg(reinterpret_cast<const float4*>(src));
+        const float4 hi = __ldg(reinterpret_cast<const float4*>(src) + 1);
+        h.v[i].v[0] = lo.x; h.v[i].v[1] = lo.y; h.v[i].v[2] = lo.z; h.v[i].v[3] = lo.w;
+        h.v[i].v[4] = hi.x; h.v[i].v[5] = hi.y; h.v[i].v[6] = hi.z; h.v[i].v[7] = hi.w;
+      } else {
+        *reinterpret_cast<uint4*>(&h.v[i]) = __ldg(reinterpret_cast<const uint4*>(src));
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        h.v[i].v[j] = in && inner + j < inner_end ? src[j] : T{};
+    }
+  }
+}
+
+template <typename T, bool MN, int ROWS>
+__device__ __forceinline__ void store_operand(unsigned char* dst, int tid,
+                                              const Held<T, ROWS>& h) {
+#pragma unroll
+  for (int i = 0; i < ROWS / 32; ++i) {
+    int row, c;
+    chunk_place<T, MN, ROWS>(tid, i, &row, &c);
+    // MN-major tiles wider than 64 are blocks of [64 k rows][128 bytes]
+    const uint32_t at = MN ? (c >> 3) * (kBK * 128) + swizzled(row, c & 7) : swizzled(row, c);
+    if constexpr (sizeof(T) == 4) {
+      uint32_t part[3][4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float x0 = h.v[i].v[2 * j], x1 = h.v[i].v[2 * j + 1];
+        const uint32_t u0 = __float_as_uint(x0), u1 = __float_as_uint(x1);
+        part[0][j] = __byte_perm(u0, u1, 0x7632);
+        const float r0 = x0 - __uint_as_float(u0 & 0xffff0000u);
+        const float r1 = x1 - __uint_as_float(u1 & 0xffff0000u);
+        const uint32_t v0 = __float_as_uint(r0), v1 = __float_as_uint(r1);
+        part[1][j] = __byte_perm(v0, v1, 0x7632);
+        const float s0 = r0 - __uint_as_float(v0 & 0xffff0000u);
+        const float s1 = r1 - __uint_as_float(v1 & 0xffff0000u);
+        part[2][j] = __byte_perm(__float_as_uint(s0), __float_as_uint(s1), 0x7632);
+      }
+#pragma unroll
+      for (int q = 0; q < 3; ++q)
+        *reinterpret_cast<uint4*>(dst + q * ROWS * 128 + at) =
+            make_uint4(part[q][0], part[q][1], part[q][2], part[q][3]);
+    } else {
+      *reinterpret_cast<uint4*>(dst + at) = *reinterpret_cast<const uint4*>(&h.v[i]);
+    }
+  }
+}
+
+// ------------------------------------------------------------------------ epilogue
+
+// Four columns of a row: bias, p, activation, residual and the store of y.
+template <typename T>
+__device__ __forceinline__ void finish4(const Epilogue& e, int64_t row, int64_t col, int64_t n,
+                                        float (&v)[4], const float (&bias)[4]) {
+  const int64_t at = row * n + col;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] += bias[j];
+  if (e.vec) {
+    if (e.preact) *reinterpret_cast<float4*>(e.preact + at) = make_float4(v[0], v[1], v[2], v[3]);
+    Pack<T, 4> r{};
+    if (e.residual)
+      r = *reinterpret_cast<const Pack<T, 4>*>(static_cast<const T*>(e.residual) +
+                                               row * e.residual_stride + col);
+    Pack<T, 4> o;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      o.v[j] = from_float<T>(activate(v[j], e.activation) + (e.residual ? to_float(r.v[j]) : 0.f));
+    *reinterpret_cast<Pack<T, 4>*>(static_cast<T*>(e.out) + at) = o;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (col + j < n) {
+        if (e.preact) e.preact[at + j] = v[j];
+        float y = activate(v[j], e.activation);
+        if (e.residual)
+          y += to_float(static_cast<const T*>(e.residual)[row * e.residual_stride + col + j]);
+        static_cast<T*>(e.out)[at + j] = from_float<T>(y);
+      }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void load_bias4(const Epilogue& e, int64_t col, int64_t n,
+                                           float (&bias)[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    bias[j] = e.bias && col + j < n ? to_float(static_cast<const T*>(e.bias)[col + j]) : 0.f;
+}
+
+// One element by FMAs in K order, for elements whose operands hold infinities or NaN.
+template <bool A_MN, bool B_MN>
+__device__ __noinline__ float plain_dot(const float* a, int64_t lda, const float* b, int64_t ldb,
+                                        int64_t m, int64_t n, int64_t k0, int64_t k1) {
+  float s = 0.f;
+  for (int64_t k = k0; k < k1; ++k)
+    s = fmaf(A_MN ? a[k * lda + m] : a[m * lda + k], B_MN ? b[k * ldb + n] : b[n * ldb + k], s);
+  return s;
+}
+
+// ---------------------------------------------------------------------- the product
+// One persistent CTA per SM, warps specialised: 8 producer warps load operand chunks
+// into registers, cut float32 values and store the swizzled tiles; one thread issues the
+// MMAs of a stage; 8 epilogue warps move finished accumulators out of TMEM, which holds
+// two sets, so a tile's epilogue overlaps the next tile's products.
+template <typename T, bool A_MN, bool B_MN, int BN>
+__global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const ProductArgs p) {
+  constexpr int P = kPieces<T>;
+  constexpr int S = kStages<T, BN>;
+  constexpr uint32_t kABytes = kBM * 128, kBBytes = BN * 128;
+  constexpr uint32_t kSet = (P == 3 ? 2 : 1) * BN;  // TMEM columns of one accumulator set
+  constexpr uint32_t kColumns = 2 * kSet;
+  extern __shared__ unsigned char raw[];
+  unsigned char* smem =
+      reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t{1023});
+  unsigned char* staging = smem + S * kStageBytes<T, BN>;
+  uint64_t* full = reinterpret_cast<uint64_t*>(staging + kStagingBytes);
+  uint64_t* empty = full + S;
+  uint64_t* done = empty + S;   // accumulator set ready for the epilogue
+  uint64_t* room = done + 2;    // accumulator set free for the MMAs
+  uint64_t* drain = room + 2;
+  uint32_t* tmem_at = reinterpret_cast<uint32_t*>(drain + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&full[s], kProducerWarps);
+      mbar_init(&empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&done[s], 1);
+      mbar_init(&room[s], kEpilogueWarps);
+    }
+    mbar_init(drain, 1);
+    fence_mbarrier_init();
+  }
+  if (warp == kMmaWarp) tmem_alloc(tmem_at, kColumns);
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem = *tmem_at;
+  const int64_t total = static_cast<int64_t>(p.tiles_m) * p.tiles_n * p.splits;
+
+  if (warp >= kEpilogueWarps && warp < kMmaWarp) {
+    // ---- producers
+    const int tid = threadIdx.x - kEpilogueWarps * 32;
+    const T* a = static_cast<const T*>(p.a);
+    const T* b = static_cast<const T*>(p.b);
+    int64_t t = blockIdx.x;
+    bool ok = true;
+    uint32_t it = 0;
+    Held<T, kBM> ha;
+    Held<T, BN> hb;
+    if (t < total) {
+      TilePos pos = tile_at(p, t, BN);
+      int c = pos.c0;
+      load_operand<T, A_MN, kBM>(a, p.lda, pos.m0, p.m, static_cast<int64_t>(c) * kBK, p.k,
+                                 p.vec_a, tid, ha);
+      while (ok) {
+        load_operand<T, B_MN, BN>(b, p.ldb, pos.n0, p.n, static_cast<int64_t>(c) * kBK, p.k,
+                                  p.vec_b, tid, hb);
+        const int s = it % S;
+        ok = mbar_wait(&empty[s], ((it / S) & 1) ^ 1, kCodeProducer);
+        if (!ok) break;
+        unsigned char* stage = smem + s * kStageBytes<T, BN>;
+        store_operand<T, A_MN, kBM>(stage, tid, ha);
+        // the next chunk's A is in flight while this chunk's B is cut and stored
+        bool more = true;
+        if (++c == pos.c1) {
+          t += gridDim.x;
+          more = t < total;
+          if (more) {
+            pos = tile_at(p, t, BN);
+            c = pos.c0;
+          }
+        }
+        if (more)
+          load_operand<T, A_MN, kBM>(a, p.lda, pos.m0, p.m, static_cast<int64_t>(c) * kBK, p.k,
+                                     p.vec_a, tid, ha);
+        store_operand<T, B_MN, BN>(stage + P * kABytes, tid, hb);
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full[s]);
+        ++it;
+        if (!more) break;
+      }
+    }
+  } else if (warp == kMmaWarp) {
+    // ---- MMA issue: one thread
+    if (lane == 0) {
+      constexpr bool kBf16 = !std::is_same_v<T, __half>;
+      constexpr uint32_t kDesc = mma_descriptor(kBf16, A_MN, B_MN, kBM, BN);
+      bool ok = true;
+      uint32_t it = 0, set = 0;
+      for (int64_t t = blockIdx.x; ok && t < total; t += gridDim.x) {
+        const TilePos pos = tile_at(p, t, BN);
+        for (int c = pos.c0; ok && c < pos.c1;) {
+          const int group_end = P == 3 && c + kGroupChunks < pos.c1 ? c + kGroupChunks : pos.c1;
+          ok = mbar_wait(&room[set & 1], ((set >> 1) & 1) ^ 1, kCodeMma);
+          if (!ok) break;
+          tcgen05_fence_after();
+          const uint32_t d = tmem + (set & 1) * kSet;
+          bool add = false;
+          for (; c < group_end; ++c, ++it) {
+            const int s = it % S;
+            ok = mbar_wait(&full[s], (it / S) & 1, kCodeMma);
+            if (!ok) break;
+            tcgen05_fence_after();
+            const uint32_t sa = smem_addr(smem + s * kStageBytes<T, BN>);
+            const uint32_t sb = sa + P * kABytes;
+            const int64_t left = p.k - static_cast<int64_t>(c) * kBK;
+            const int steps = left < kBK ? static_cast<int>((left + 15) / 16) : kBK / 16;
+            for (int k = 0; k < steps; ++k) {
+              // 16 elements along K: 32 bytes of a K-major row, 16 rows MN-major
+              const uint32_t ao = k * (A_MN ? 2048 : 32), bo = k * (B_MN ? 2048 : 32);
+              uint64_t da[P], db[P];
+#pragma unroll
+              for (int q = 0; q < P; ++q) {
+                da[q] = matrix_descriptor(sa + q * kABytes + ao, kBK * 128, 1024);
+                db[q] = matrix_descriptor(sb + q * kBBytes + bo, kBK * 128, 1024);
+              }
+              mma_f16(d, da[0], db[0], kDesc, add);
+              if constexpr (P == 3) {
+                mma_f16(d + BN, da[2], db[0], kDesc, add);
+                mma_f16(d + BN, da[0], db[2], kDesc, true);
+                mma_f16(d + BN, da[1], db[1], kDesc, true);
+                mma_f16(d + BN, da[1], db[0], kDesc, true);
+                mma_f16(d + BN, da[0], db[1], kDesc, true);
+              }
+              add = true;
+            }
+            mma_commit(&empty[s]);
+          }
+          if (!ok) break;
+          mma_commit(&done[set & 1]);
+          ++set;
+        }
+      }
+      if (!ok) {  // let the MMAs in flight finish before TMEM and the stages go away
+        mma_commit(drain);
+        mbar_wait(drain, 0, kCodeDrain, kDrainLimitNs);
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---- epilogue: warp w holds TMEM lanes 32 (w % 4) .. + 31, half w / 4 of the columns
+    constexpr int kHalf = BN / 2;
+    const int quad = warp & 3, half = warp >> 2;
+    float4* mine = reinterpret_cast<float4*>(staging + warp * 4096);
+    bool ok = true;
+    uint32_t set = 0;
+    for (int64_t t = blockIdx.x; ok && t < total; t += gridDim.x) {
+      const TilePos pos = tile_at(p, t, BN);
+      float acc[kHalf];
+      const int groups = P == 3 ? (pos.c1 - pos.c0 + kGroupChunks - 1) / kGroupChunks : 1;
+      for (int gi = 0; gi < groups; ++gi, ++set) {
+        ok = mbar_wait(&done[set & 1], (set >> 1) & 1, kCodeEpilogue);
+        if (!ok) break;
+        tcgen05_fence_after();
+        const uint32_t at =
+            tmem + (set & 1) * kSet + (static_cast<uint32_t>(quad * 32) << 16) + half * kHalf;
+#pragma unroll
+        for (int j = 0; j < kHalf; j += 16) {
+          float v[16];
+          tmem_load16(at + j, v);
+          if constexpr (P == 3) {
+            float w[16];
+            tmem_load16(at + BN + j, w);
+            tmem_load_wait();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] += w[i];
+          } else {
+            tmem_load_wait();
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[j + i] = gi == 0 ? v[i] : acc[j + i] + v[i];
+        }
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&room[set & 1]);
+      }
+      if (!ok) break;
+      // 32 x 32 blocks through shared memory, so that eight lanes write 32 consecutive
+      // columns of a row
+#pragma unroll
+      for (int cb = 0; cb < kHalf / 32; ++cb) {
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+          mine[lane * 8 + (c ^ (lane & 7))] =
+              make_float4(acc[cb * 32 + 4 * c], acc[cb * 32 + 4 * c + 1],
+                          acc[cb * 32 + 4 * c + 2], acc[cb * 32 + 4 * c + 3]);
+        __syncwarp();
+        const int64_t col = pos.n0 + half * kHalf + cb * 32 + (lane & 7) * 4;
+        float bias[4];
+        load_bias4<T>(p.e, col, p.n, bias);
+#pragma unroll 2
+        for (int i = 0; i < 8; ++i) {
+          const int r = i * 4 + (lane >> 3);
+          const int64_t row = pos.m0 + quad * 32 + r;
+          const float4 f = mine[r * 8 + ((lane & 7) ^ (r & 7))];
+          if (row >= p.m || col >= p.n) continue;
+          float v[4] = {f.x, f.y, f.z, f.w};
+          if constexpr (P == 3) {
+            const bool fine = isfinite(v[0]) && isfinite(v[1]) && isfinite(v[2]) && isfinite(v[3]);
+            if (!fine) {
+              const int64_t k0 = static_cast<int64_t>(pos.c0) * kBK;
+              const int64_t k1 = static_cast<int64_t>(pos.c1) * kBK < p.k
+                                     ? static_cast<int64_t>(pos.c1) * kBK : p.k;
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                if (!isfinite(v[j]) && col + j < p.n)
+                  v[j] = plain_dot<A_MN, B_MN>(static_cast<const float*>(p.a), p.lda,
+                                               static_cast<const float*>(p.b), p.ldb, row,
+                                               col + j, k0, k1);
+            }
+          }
+          if (p.e.partial) {
+            float* o = p.e.partial + (pos.split * p.m + row) * p.n + col;
+            if (p.e.vec) {
+              *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                if (col + j < p.n) o[j] = v[j];
+            }
+          } else {
+            finish4<T>(p.e, row, col, p.n, v, bias);
+          }
+        }
+        __syncwarp();
+      }
+    }
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tcgen05_fence_after();
+    tmem_free(tmem, kColumns);
+  }
+}
+
+// out = epilogue(sum of the splits' partial products), the splits added in order.
+template <typename T>
+__global__ void __launch_bounds__(256) join_splits_kernel(const Epilogue e, int64_t m, int64_t n,
+                                                          int splits) {
+  const int64_t quads = (n + 3) / 4;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * 256;
+  for (int64_t q = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; q < m * quads; q += step) {
+    const int64_t row = q / quads, col = (q - row * quads) * 4;
+    float v[4] = {0.f, 0.f, 0.f, 0.f}, bias[4];
+    load_bias4<T>(e, col, n, bias);
+    const float* at = e.partial + row * n + col;
+    for (int s = 0; s < splits; ++s, at += m * n) {
+      if (e.vec) {
+        const float4 f = *reinterpret_cast<const float4*>(at);
+        v[0] += f.x; v[1] += f.y; v[2] += f.z; v[3] += f.w;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (col + j < n) v[j] += at[j];
+      }
+    }
+    finish4<T>(e, row, col, n, v, bias);
+  }
+}
+
+// ---------------------------------------------------------------- few rows: no tiles
+// Up to four rows: W is read once at HBM speed and the products run on the FMA pipes.
+// W_ warps share one output column, each a part of K; a lane reads V consecutive
+// elements, the warps' sums are added in warp order.
+constexpr int kRowThreads = 256;
+
+template <typename T, int ROWS, int V>
+__global__ void __launch_bounds__(kRowThreads) few_rows_kernel(
+    const T* __restrict__ x, int64_t ldx, const T* __restrict__ w, int64_t ldw, int64_t rows,
+    int64_t n, int64_t k, int share, const Epilogue e) {
+  __shared__ float sums[kRowThreads / 32][ROWS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int per_cta = (kRowThreads / 32) / share;  // columns per CTA and round
+  const int part = warp % share;
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * per_cta; base < n;
+       base += static_cast<int64_t>(gridDim.x) * per_cta) {
+    const int64_t col = base + warp / share;
+    float acc[ROWS];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) acc[r] = 0.f;
+    if (col < n) {
+      const T* wr = w + col * ldw;
+#pragma unroll 4
+      for (int64_t c = (part * 32 + lane) * V; c < k; c += share * 32 * V) {
+        const Pack<T, V> pw = *reinterpret_cast<const Pack<T, V>*>(wr + c);
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+          if (r >= rows) break;
+          const Pack<T, V> px = *reinterpret_cast<const Pack<T, V>*>(x + r * ldx + c);
+#pragma unroll
+          for (int j = 0; j < V; ++j) acc[r] = fmaf(to_float(px.v[j]), to_float(pw.v[j]), acc[r]);
+        }
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) acc[r] += __shfl_xor_sync(0xffffffffu, acc[r], o);
+    if (share > 1) {
+      if (lane == 0)
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) sums[warp][r] = acc[r];
+      __syncthreads();
+      if (part == 0)
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+          acc[r] = 0.f;
+          for (int q = 0; q < share; ++q) acc[r] += sums[warp + q][r];
+        }
+      __syncthreads();
+    }
+    if (part == 0 && lane == 0 && col < n) {
+      const float bias = e.bias ? to_float(static_cast<const T*>(e.bias)[col]) : 0.f;
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) {
+        if (r >= rows) break;
+        const float v = acc[r] + bias;
+        if (e.preact) e.preact[r * n + col] = v;
+        float y = activate(v, e.activation);
+        if (e.residual)
+          y += to_float(static_cast<const T*>(e.residual)[r * e.residual_stride + col]);
+        static_cast<T*>(e.out)[r * n + col] = from_float<T>(y);
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------- d = g act'(p) and sums of d
+// Bound by HBM.  A CTA owns a strip of columns and every gridDim.y-th block of rows; each
+// thread keeps its columns' sums in registers, and the CTA's partial row of db is joined
+// over its row lanes in order.
+template <typename T, int V>
+__global__ void __launch_bounds__(256) slope_kernel(const T* __restrict__ g, int64_t ldg,
+                                                    const float* __restrict__ preact,
+                                                    T* __restrict__ d, float* __restrict__ partial,
+                                                    int64_t m, int64_t n, int lanes,
+                                                    int activation) {
+  __shared__ float sums[256 * V];
+  const int tx = threadIdx.x % lanes, ty = threadIdx.x / lanes, rows = 256 / lanes;
+  const int64_t col = (static_cast<int64_t>(blockIdx.x) * lanes + tx) * V;
+  float acc[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) acc[j] = 0.f;
+  if (col < n) {
+#pragma unroll 2
+    for (int64_t r = static_cast<int64_t>(blockIdx.y) * rows + ty; r < m;
+         r += static_cast<int64_t>(gridDim.y) * rows) {
+      const Pack<T, V> pg = *reinterpret_cast<const Pack<T, V>*>(g + r * ldg + col);
+      float v[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] = to_float(pg.v[j]);
+      if (preact != nullptr) {
+        Pack<T, V> o;
+#pragma unroll
+        for (int j = 0; j < V; j += (V >= 4 ? 4 : 1)) {
+          float q[4];
+          if constexpr (V >= 4) {
+            const float4 f = *reinterpret_cast<const float4*>(preact + r * n + col + j);
+            q[0] = f.x; q[1] = f.y; q[2] = f.z; q[3] = f.w;
+          } else {
+            q[0] = preact[r * n + col + j];
+          }
+#pragma unroll
+          for (int i = 0; i < (V >= 4 ? 4 : 1); ++i) {
+            v[j + i] *= activation_slope(q[i], activation);
+            o.v[j + i] = from_float<T>(v[j + i]);
+          }
+        }
+        if (d != nullptr) *reinterpret_cast<Pack<T, V>*>(d + r * n + col) = o;
+      }
+#pragma unroll
+      for (int j = 0; j < V; ++j) acc[j] += v[j];
+    }
+  }
+  if (partial == nullptr) return;
+#pragma unroll
+  for (int j = 0; j < V; ++j) sums[(ty * lanes + tx) * V + j] = acc[j];
+  __syncthreads();
+  for (int c = threadIdx.x; c < lanes * V; c += 256) {
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * lanes * V + c;
+    if (at >= n) break;
+    float total = 0.f;
+    for (int q = 0; q < rows; ++q) total += sums[q * lanes * V + c];
+    partial[blockIdx.y * n + at] = total;
+  }
+}
+
+// ----------------------------------------------------------------------- host side
+
+int current_device() {
+  int device = 0;
+  return cudaGetDevice(&device) == cudaSuccess ? device : 0;
+}
+
+struct Split {
+  int tiles_m, tiles_n, bn, chunks, splits, chunks_per_split;
+  bool fits;  // tile counts fit the kernel's integers
+};
+
+// The K axis is split when the output has too few tiles to fill the SMs: at least four
+// stages of K per split (the pipeline's depth), and no more splits than fill one wave.
+Split plan_product(int64_t m, int64_t n, int64_t k, int device) {
+  Split s{};
+  s.bn = n <= 64 ? 64 : 128;
+  const int64_t tm = ceil_div(m, kBM), tn = ceil_div(n, s.bn), chunks = ceil_div(k, kBK);
+  s.fits = tm < (1ll << 31) && tn < (1ll << 31) && chunks < (1ll << 31);
+  if (!s.fits) return s;
+  s.tiles_m = static_cast<int>(tm);
+  s.tiles_n = static_cast<int>(tn);
+  s.chunks = static_cast<int>(chunks);
+  const int64_t sms = sm_count(device);
+  int64_t splits = tm * tn >= sms ? 1 : sms / (tm * tn);
+  if (splits > chunks / 4) splits = chunks / 4;
+  if (splits < 1) splits = 1;
+  s.chunks_per_split = static_cast<int>(ceil_div(chunks, splits));
+  s.splits = static_cast<int>(ceil_div(chunks, s.chunks_per_split));
+  return s;
+}
+
+size_t split_bytes(const Split& s, int64_t m, int64_t n) {
+  return s.splits > 1 ? static_cast<size_t>(s.splits) * m * n * sizeof(float) : 0;
+}
+
+template <typename T, bool A_MN, bool B_MN, int BN>
+int launch_product(const ProductArgs& p, int device, cudaStream_t stream) {
+  const void* fn = reinterpret_cast<const void*>(product_kernel<T, A_MN, B_MN, BN>);
+  const int st = allow_smem(fn, kProductSmem<T, BN>);
+  if (st != ICTC_OK) return st;
+  const int64_t total = static_cast<int64_t>(p.tiles_m) * p.tiles_n * p.splits;
+  const int64_t sms = sm_count(device);
+  product_kernel<T, A_MN, B_MN, BN>
+      <<<static_cast<unsigned>(total < sms ? total : sms), kProductThreads, kProductSmem<T, BN>,
+         stream>>>(p);
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? ICTC_OK : cuda_fail(e, "linear product launch");
+}
+
+bool chunk_aligned(const void* p, int64_t ld, size_t size) {
+  return aligned(p, 16) && (ld * static_cast<int64_t>(size)) % 16 == 0;
+}
+
+// C = epilogue(A B^T); `partial` holds split_bytes() when the plan splits K.
+template <typename T, bool A_MN, bool B_MN>
+int run_product(const T* a, int64_t lda, const T* b, int64_t ldb, int64_t m, int64_t n, int64_t k,
+                Epilogue e, float* partial, cudaStream_t stream) {
+  const int device = current_device();
+  const Split s = plan_product(m, n, k, device);
+  if (!s.fits) return fail(ICTC_ERR_UNSUPPORTED, "linear: a dimension is too large");
+  ProductArgs p{};
+  p.a = a; p.b = b;
+  p.m = m; p.n = n; p.k = k;
+  p.lda = lda; p.ldb = ldb;
+  p.tiles_m = s.tiles_m; p.tiles_n = s.tiles_n;
+  p.splits = s.splits; p.chunks = s.chunks; p.chunks_per_split = s.chunks_per_split;
+  p.vec_a = chunk_aligned(a, lda, sizeof(T));
+  p.vec_b = chunk_aligned(b, ldb, sizeof(T));
+  e.vec = n % 4 == 0 && aligned(e.out, 4 * sizeof(T)) &&
+          (!e.residual || (aligned(e.residual, 4 * sizeof(T)) && e.residual_stride % 4 == 0)) &&
+          aligned(e.preact, 16) && aligned(partial, 16);
+  e.partial = s.splits > 1 ? partial : nullptr;
+  p.e = e;
+  const int st = s.bn == 64 ? launch_product<T, A_MN, B_MN, 64>(p, device, stream)
+                            : launch_product<T, A_MN, B_MN, 128>(p, device, stream);
+  if (st != ICTC_OK || s.splits == 1) return st;
+  const int64_t blocks = ceil_div(m * ceil_div(n, 4), 256);
+  const int64_t cap = static_cast<int64_t>(sm_count(device)) * 8;
+  join_splits_kernel<T><<<static_cast<unsigned>(blocks < cap ? blocks : cap), 256, 0, stream>>>(
+      e, m, n, s.splits);
+  const cudaError_t err = cudaGetLastError();
+  return err == cudaSuccess ? ICTC_OK : cuda_fail(err, "linear split join launch");
+}
+
+template <typename T, int V>
+int launch_few_rows(const T* x, int64_t ldx, const T* w, int64_t ldw, int64_t rows, int64_t n,
+                    int64_t k, const Epilogue& e, cudaStream_t stream) {
+  const int64_t sms = sm_count(current_device());
+  // all eight warps of a CTA share a column while that still gives every SM work
+  const int share = n <= sms * 16 ? 8 : 1;
+  const int64_t want = ceil_div(n, 8 / share);
+  const unsigned grid = static_cast<unsigned>(want < sms * 8 ? want : sms * 8);
+  if (rows == 1)
+    few_rows_kernel<T, 1, V><<<grid, kRowThreads, 0, stream>>>(x, ldx, w, ldw, rows, n, k, share, e);
+  else
+    few_rows_kernel<T, 4, V><<<grid, kRowThreads, 0, stream>>>(x, ldx, w, ldw, rows, n, k, share, e);
+  const cudaError_t err = cudaGetLastError();
+  return err == cudaSuccess ? ICTC_OK : cuda_fail(err, "linear few-row launch");
+}
+
+constexpr int64_t kFewRows = 4;
+
+template <typename T>
+int run_linear_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, Epilogue e,
+                       float* partial, int64_t m, int64_t n, int64_t k, cudaStream_t stream) {
+  const T* xt = static_cast<const T*>(x);
+  const T* wt = static_cast<const T*>(w);
+  if (m <= kFewRows) {
+    constexpr int kFull = 16 / sizeof(T);
+    if (k % kFull == 0 && chunk_aligned(x, ldx, sizeof(T)) && chunk_aligned(w, ldw, sizeof(T)))
+      return launch_few_rows<T, kFull>(xt, ldx, wt, ldw, m, n, k, e, stream);
+    return launch_few_rows<T, 1>(xt, ldx, wt, ldw, m, n, k, e, stream);
+  }
+  return run_product<T, false, false>(xt, ldx, wt, ldw, m, n, k, e, partial, stream);
+}
+
+struct SlopePlan {
+  int vec, lanes;
+  unsigned blocks_x, blocks_y;
+};
+
+constexpr int64_t kSlopeParts = 296;
+
+SlopePlan plan_slope(int64_t m, int64_t n, int vec) {
+  SlopePlan s{};
+  s.vec = vec;
+  const int64_t units = ceil_div(n, vec);
+  int lanes = 1;
+  while (lanes < 32 && lanes < units) lanes *= 2;
+  s.lanes = lanes;
+  s.blocks_x = static_cast<unsigned>(ceil_div(units, lanes));
+  const int64_t row_blocks = ceil_div(m, 256 / lanes);
+  int64_t y = ceil_div(148 * 8, s.blocks_x);
+  if (y > kSlopeParts) y = kSlopeParts;
+  if (y > row_blocks) y = row_blocks;
+  s.blocks_y = static_cast<unsigned>(y < 1 ? 1 : y);
+  return s;
+}
+
+struct BackwardPlan {
+  size_t d, columns, partial, total;  // byte offsets of the workspace's parts and its size
+};
+
+BackwardPlan plan_backward(int64_t m, int64_t n, int64_t k, int dtype, bool slope, int device) {
+  BackwardPlan b{};
+  const size_t d_bytes = slope ? align_up(static_cast<size_t>(m) * n * dtype_size(dtype), 256) : 0;
+  b.d = 0;
+  b.columns = d_bytes;
+  const int64_t parts = m < kSlopeParts ? m : kSlopeParts;
+  b.partial = b.columns + align_up(static_cast<size_t>(parts) * n * sizeof(float), 256);
+  size_t split = split_bytes(plan_product(m, k, n, device), m, k);
+  const size_t other = split_bytes(plan_product(n, k, m, device), n, k);
+  if (other > split) split = other;
+  b.total = b.partial + align_up(split, 256);
+  return b;
+}
+
+template <typename T>
+int run_linear_backward(const void* x, int64_t ldx, const void* w, int64_t ldw,
+                        const float* preact, const void* g, int64_t ldg, void* dx, void* dw,
+                        void* db, unsigned char* workspace, const BackwardPlan& plan, int64_t m,
+                        int64_t n, int64_t k, int activation, cudaStream_t stream) {
+  const T* d = static_cast<const T*>(g);
+  int64_t ldd = ldg;
+  const bool slope = activation != ICTC_ACT_NONE;
+  T* d_out = slope ? reinterpret_cast<T*>(workspace + plan.d) : nullptr;
+  float* columns = db ? reinterpret_cast<float*>(workspace + plan.columns) : nullptr;
+  if (slope || db) {
+    constexpr int kFull = 16 / sizeof(T);
+    const bool vec = n % kFull == 0 && chunk_aligned(g, ldg, sizeof(T)) && aligned(preact, 16);
+    const SlopePlan s = plan_slope(m, n, vec ? kFull : 1);
+    const dim3 grid(s.blocks_x, s.blocks_y);
+    if (vec)
+      slope_kernel<T, kFull><<<grid, 256, 0, stream>>>(d, ldg, slope ? preact : nullptr, d_out,
+                                                       columns, m, n, s.lanes, activation);
+    else
+      slope_kernel<T, 1><<<grid, 256, 0, stream>>>(d, ldg, slope ? preact : nullptr, d_out,
+                                                   columns, m, n, s.lanes, activation);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return cuda_fail(e, "linear slope launch");
+    if (db) {
+      column_total_kernel<T><<<dim3(static_cast<unsigned>(ceil_div(n, 32))),
+                               dim3(32, kColumnLanes), 0, stream>>>(
+          columns, columns, static_cast<T*>(db), static_cast<T*>(db), s.blocks_y, n);
+      e = cudaGetLastError();
+      if (e != cudaSuccess) return cuda_fail(e, "linear column sum launch");
+    }
+    if (slope) {
+      d = d_out;
+      ldd = n;
+    }
+  }
+  float* partial = reinterpret_cast<float*>(workspace + plan.partial);
+  Epilogue e{};
+  if (dx) {
+    e.out = dx;
+    const int st = run_product<T, false, true>(d, ldd, static_cast<const T*>(w), ldw, m, k, n, e,
+                                               partial, stream);
+    if (st != ICTC_OK) return st;
+  }
+  if (dw) {
+    e.out = dw;
+    return run_product<T, true, true>(d, ldd, static_cast<const T*>(x), ldx, n, k, m, e, partial,
+                                      stream);
+  }
+  return ICTC_OK;
+}
+
+int check_linear(int64_t m, int64_t n, int64_t k, int32_t dtype, int32_t activation) {
+  if (m < 0 || n < 1 || k < 1)
+    return fail(ICTC_ERR_INVALID,
+                "linear needs rows >= 0 and in, out >= 1, got %lld rows, in %lld, out %lld",
+                static_cast<long long>(m), static_cast<long long>(k), static_cast<long long>(n));
+  if (!known_dtype(dtype)) return fail(ICTC_ERR_INVALID, "unknown dtype code %d", dtype);
+  if (activation < ICTC_ACT_NONE || activation > ICTC_ACT_GELU_TANH)
+    return fail(ICTC_ERR_INVALID, "unknown activation code %d", activation);
+  return ICTC_OK;
+}
+
+}  // namespace
+
+int dense_take_device_error(int* code) {
+  cudaError_t e;
+  if (take_unit_device_error(code, &e) != 0) return cuda_fail(e, "linear device error flag");
+  return ICTC_OK;
+}
+
+}  // namespace ictc
+
+using namespace ictc;
+
+extern "C" int32_t ictc_o2_linear_workspace(int64_t rows, int64_t in, int64_t out, int32_t dtype,
+                                            int32_t activation, int32_t device,
+                                            size_t* forward_bytes, size_t* backward_bytes) {
+  const int st = check_linear(rows, out, in, dtype, activation);
+  if (st != ICTC_OK) return st;
+  if (!forward_bytes || !backward_bytes) return fail(ICTC_ERR_INVALID, "null output");
+  *forward_bytes =
+      rows <= kFewRows ? 0 : split_bytes(plan_product(rows, out, in, device), rows, out);
+  *backward_bytes =
+      rows == 0 ? 0
+                : plan_backward(rows, out, in, dtype, activation != ICTC_ACT_NONE, device).total;
+  return ICTC_OK;
+}
+
+extern "C" int32_t ictc_o2_linear_forward(const void* x, int64_t x_stride, const void* weight,
+                                          int64_t weight_stride, const void* bias,
+                                          const void* residual, int64_t residual_stride, void* y,
+                                          float* preact, void* workspace, size_t workspace_bytes,
+                                          int64_t rows, int64_t in, int64_t out, int32_t dtype,
+                                          int32_t activation, void* stream) {
+  const int st = check_linear(rows, out, in, dtype, activation);
+  if (st != ICTC_OK) return st;
+  if (rows == 0) return ICTC_OK;
+  if (!x || !weight || !y) return fail(ICTC_ERR_INVALID, "null pointer");
+  if (x_stride < 0 || weight_stride < 0 || residual_stride < 0)
+    return fail(ICTC_ERR_INVALID, "negative row stride");
+  const size_t need = rows <= kFewRows
+                          ? 0 : split_bytes(plan_product(rows, out, in, current_device()), rows, out);
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
+    return fail(ICTC_ERR_WORKSPACE, "workspace has %zu bytes, needs %zu (16-byte aligned)",
+                workspace ? workspace_bytes : 0, need);
+  Epilogue e{};
+  e.bias = bias;
+  e.residual = residual;
+  e.residual_stride = residual_stride;
+  e.preact = preact;
+  e.out = y;
+  e.activation = activation;
+  float* partial = static_cast<float*>(workspace);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (dtype == ICTC_DTYPE_F32)
+    return run_linear_forward<float>(x, x_stride, weight, weight_stride, e, partial, rows, out, in,
+                                     s);
+  if (dtype == ICTC_DTYPE_BF16)
+    return run_linear_forward<__nv_bfloat16>(x, x_stride, weight, weight_stride, e, partial, rows,
+                                             out, in, s);
+  return run_linear_forward<__half>(x, x_stride, weight, weight_stride, e, partial, rows, out, in,
+                                    s);
+}
+
+extern "C" int32_t ictc_o2_linear_backward(
+    const void* x, int64_t x_stride, const void* weight, int64_t weight_stride,
+    const float* preact, const void* grad_output, int64_t grad_stride, void* grad_x,
+    void* grad_weight, void* grad_bias, void* workspace, size_t workspace_bytes, int64_t rows,
+    int64_t in, int64_t out, int32_t dtype, int32_t activation, void* stream) {
+  const int st = check_linear(rows, out, in, dtype, activation);
+  if (st != ICTC_OK) return st;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (rows == 0) {
+    cudaError_t e = cudaSuccess;
+    if (grad_weight)
+      e = cudaMemsetAsync(grad_weight, 0, static_cast<size_t>(out) * in * dtype_size(dtype), s);
+    if (e == cudaSuccess && grad_bias)
+      e = cudaMemsetAsync(grad_bias, 0, static_cast<size_t>(out) * dtype_size(dtype), s);
+    return e == cudaSuccess ? ICTC_OK : cuda_fail(e, "linear gradient clear");
+  }
+  if (!grad_x && !grad_weight && !grad_bias) return ICTC_OK;
+  if (!grad_output || (grad_x && !weight) || (grad_weight && !x) ||
+      (activation != ICTC_ACT_NONE && !preact))
+    return fail(ICTC_ERR_INVALID, "null pointer");
+  if (x_stride < 0 || weight_stride < 0 || grad_stride < 0)
+    return fail(ICTC_ERR_INVALID, "negative row stride");
+  const BackwardPlan plan = plan_backward(rows, out, in, dtype, activation != ICTC_ACT_NONE,
+                                          current_device());
+  if (!workspace || workspace_bytes < plan.total || !aligned(workspace, 256))
+    return fail(ICTC_ERR_WORKSPACE, "workspace has %zu bytes, needs %zu (256-byte aligned)",
+                workspace ? workspace_bytes : 0, plan.total);
+  unsigned char* ws = static_cast<unsigned char*>(workspace);
+#define ICTC_LINEAR_BACKWARD(T)                                                               \
+  return run_linear_backward<T>(x, x_stride, weight, weight_stride, preact, grad_output,       \
+                                grad_stride, grad_x, grad_weight, grad_bias, ws, plan, rows, out, \
+                                in, activation, s)
+  if (dtype == ICTC_DTYPE_F32) ICTC_LINEAR_BACKWARD(float);
+  if (dtype == ICTC_DTYPE_BF16) ICTC_LINEAR_BACKWARD(__nv_bfloat16);
+  ICTC_LINEAR_BACKWARD(__half);
+#undef ICTC_LINEAR_BACKWARD
+}

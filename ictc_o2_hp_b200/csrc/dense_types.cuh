@@ -1,0 +1,113 @@
+// Element types, activations and the column-sum reduction shared by the dense
+// operators (layer norm, linear layer).
+//
+// Tensors are float32, bfloat16 or float16; every sum, statistic and activation is
+// computed in float32 and rounded once when a tensor of the operand type is stored.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "common.cuh"
+
+namespace ictc {
+
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+
+template <typename T>
+__device__ __forceinline__ T from_float(float v);
+template <>
+__device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) {
+  return __float2bfloat16_rn(v);
+}
+template <>
+__device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+
+// N elements moved as one aligned access (N * sizeof(T) = 4, 8 or 16 bytes, or one
+// element).
+template <typename T, int N>
+struct alignas(sizeof(T) * N) Pack {
+  T v[N];
+};
+
+// act(p) and act'(p) for the activation codes of the C ABI.  The code is a kernel
+// argument: the branch is uniform over the launch and costs nothing beside the
+// function itself.
+__device__ __forceinline__ float activate(float p, int activation) {
+  switch (activation) {
+    case ICTC_ACT_RELU:
+      return p > 0.f ? p : (p != p ? p : 0.f);
+    case ICTC_ACT_SILU:
+      return p / (1.f + expf(-p));
+    case ICTC_ACT_GELU:
+      return 0.5f * p * (1.f + erff(p * 0.70710678118654752f));
+    case ICTC_ACT_GELU_TANH:
+      return 0.5f * p * (1.f + tanhf(0.79788456080286536f * (p + 0.044715f * p * p * p)));
+    default:
+      return p;
+  }
+}
+
+__device__ __forceinline__ float activation_slope(float p, int activation) {
+  switch (activation) {
+    case ICTC_ACT_RELU:
+      return p > 0.f ? 1.f : 0.f;
+    case ICTC_ACT_SILU: {
+      const float s = 1.f / (1.f + expf(-p));
+      return s * (1.f + p * (1.f - s));
+    }
+    case ICTC_ACT_GELU:
+      return 0.5f * (1.f + erff(p * 0.70710678118654752f)) +
+             p * expf(-0.5f * p * p) * 0.39894228040143268f;
+    case ICTC_ACT_GELU_TANH: {
+      const float c = 0.79788456080286536f;
+      const float t = tanhf(c * (p + 0.044715f * p * p * p));
+      return 0.5f * (1.f + t) + 0.5f * p * (1.f - t * t) * c * (1.f + 0.134145f * p * p);
+    }
+    default:
+      return 1.f;
+  }
+}
+
+inline size_t dtype_size(int dtype) { return dtype == ICTC_DTYPE_F32 ? 4 : 2; }
+
+inline bool known_dtype(int dtype) {
+  return dtype == ICTC_DTYPE_F32 || dtype == ICTC_DTYPE_BF16 || dtype == ICTC_DTYPE_F16;
+}
+
+inline size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
+
+// out[c] = sum over p of partial[p * width + c], added in a fixed order: each of the
+// 32 row lanes adds its rows p = lane, lane + 32, ... and the lanes' sums are added in
+// lane order, so a result does not depend on scheduling.  Two column sums of one pass
+// (weight and bias gradients) go in one launch through blockIdx.y.
+constexpr int kColumnLanes = 32;
+
+template <typename T>
+static __global__ void __launch_bounds__(32 * kColumnLanes) column_total_kernel(
+    const float* __restrict__ partial0, const float* __restrict__ partial1, T* __restrict__ out0,
+    T* __restrict__ out1, int64_t parts, int64_t width) {
+  __shared__ float sums[kColumnLanes][33];
+  const float* partial = blockIdx.y ? partial1 : partial0;
+  T* out = blockIdx.y ? out1 : out0;
+  const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + threadIdx.x;
+  float s = 0.f;
+  if (c < width)
+    for (int64_t p = threadIdx.y; p < parts; p += kColumnLanes) s += partial[p * width + c];
+  sums[threadIdx.y][threadIdx.x] = s;
+  __syncthreads();
+  if (threadIdx.y == 0 && c < width) {
+    float total = 0.f;
+    for (int l = 0; l < kColumnLanes; ++l) total += sums[l][threadIdx.x];
+    out[c] = from_float<T>(total);
+  }
+}
+
+}  // namespace ictc

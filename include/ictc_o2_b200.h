@@ -52,13 +52,14 @@ ICTC_API int32_t ictc_o2_abi_version(void);
 
 /* Synchronizes with the current device, then reads and clears the kernels'
  * device-side error flags (one per compiled unit: TensorProduct, uvu, radial and
- * the wait probe below) and returns the first nonzero code in that order: 0 = none;
+ * the wait probe below, the dense operators) and returns the first nonzero code in
+ * that order: 0 = none;
  * nonzero = a bounded wait inside a kernel ran out (2 s of the GPU's global timer)
  * and that kernel stopped early, so its outputs are invalid.  Codes: 1-4
  * TensorProduct staged kernels (stage ring, drain, weight copy), 5-6 radial edge
  * tile, 7-8 shared-weight uvu tile, 9-10 per-row uvu streamed kernel, 11-12
  * per-row uvu quad kernel, 13 the wait probe; 17 is not a wait: a gathered radial
- * call met a node index out of range.  No counterpart in the reference,
+ * call met a node index out of range; 18-21 the linear layer's products.  No counterpart in the reference,
  * whose Triton kernels have no waits. */
 ICTC_API int32_t ictc_o2_device_error(int32_t* code);
 
@@ -289,6 +290,75 @@ ICTC_API int32_t ictc_o2_segment_sum(const float* values, const int64_t* offsets
 /* Synchronizes, then reads and clears the out-of-range-index flag of the two
  * kernels above on the current device (1 = some index was out of range). */
 ICTC_API int32_t ictc_o2_graph_bad_index(int32_t* flag);
+
+/* ------------------------------------------------------------------------------
+ * Dense operators for the networks around the products (radial trunks, node
+ * feed-forward blocks): layer norm and the linear layer with bias, activation and
+ * residual.  No counterpart in the reference, which leaves them to PyTorch.
+ * Operands are float32, bfloat16 or float16 (one type per call); all sums are
+ * float32.  Inputs are row-major with a row stride in elements (unit stride inside
+ * a row; 0 repeats one row); outputs are contiguous.  Results do not depend on
+ * scheduling: every sum has a fixed order.
+ * ------------------------------------------------------------------------------ */
+
+enum { ICTC_DTYPE_F32 = 0, ICTC_DTYPE_BF16 = 1, ICTC_DTYPE_F16 = 2 };
+/* gelu: p Phi(p); gelu_tanh: its tanh form with 0.044715 */
+enum {
+  ICTC_ACT_NONE = 0,
+  ICTC_ACT_RELU = 1,
+  ICTC_ACT_SILU = 2,
+  ICTC_ACT_GELU = 3,
+  ICTC_ACT_GELU_TANH = 4
+};
+
+/* y[r, :] = (x[r, :] - mean_r) rstd_r weight + bias with mean and biased variance over
+ * the `width` elements of a row, rstd = 1 / sqrt(var + eps).  weight and bias [width]
+ * may be null (1 and 0); param_dtype is theirs: `dtype` or float32.  mean and rstd
+ * [rows] receive the statistics for the backward, or are both null. */
+ICTC_API int32_t ictc_o2_layer_norm_forward(const void* x, int64_t x_stride, const void* weight,
+                                            const void* bias, void* y, float* mean, float* rstd,
+                                            int64_t rows, int64_t width, float eps,
+                                            int32_t dtype, int32_t param_dtype, void* stream);
+
+/* Bytes of workspace that the backward needs for grad_weight and grad_bias. */
+ICTC_API int32_t ictc_o2_layer_norm_workspace(int64_t rows, int64_t width, int32_t dtype,
+                                              int32_t device, size_t* bytes);
+
+/* Gradients of the layer norm; any of the three outputs may be null.  Without
+ * grad_weight and grad_bias the workspace may be null.  rows = 0 clears grad_weight
+ * and grad_bias. */
+ICTC_API int32_t ictc_o2_layer_norm_backward(
+    const void* x, int64_t x_stride, const void* weight, const float* mean, const float* rstd,
+    const void* grad_output, int64_t grad_stride, void* grad_x, void* grad_weight,
+    void* grad_bias, void* workspace, size_t workspace_bytes, int64_t rows, int64_t width,
+    int32_t dtype, int32_t param_dtype, void* stream);
+
+/* Workspace of the linear layer's two directions (256-byte aligned). */
+ICTC_API int32_t ictc_o2_linear_workspace(int64_t rows, int64_t in, int64_t out, int32_t dtype,
+                                          int32_t activation, int32_t device,
+                                          size_t* forward_bytes, size_t* backward_bytes);
+
+/* p = x weight^T + bias, y = act(p) + residual: x [rows, in], weight [out, in], bias
+ * [out] or null, residual [rows, out] or null, y [rows, out].  preact receives p in
+ * float32 for the backward (needed there unless the activation is none), or is null.
+ * float32 products run on the tensor cores with each operand cut exactly into three
+ * bf16 parts; errors are those of a float32 product. */
+ICTC_API int32_t ictc_o2_linear_forward(const void* x, int64_t x_stride, const void* weight,
+                                        int64_t weight_stride, const void* bias,
+                                        const void* residual, int64_t residual_stride, void* y,
+                                        float* preact, void* workspace, size_t workspace_bytes,
+                                        int64_t rows, int64_t in, int64_t out, int32_t dtype,
+                                        int32_t activation, void* stream);
+
+/* d = grad_output act'(p); grad_x = d weight, grad_weight = d^T x, grad_bias = sum of
+ * d's rows (the residual's gradient is grad_output itself).  16-bit types round d to
+ * their type before the products, as they would a tensor.  Any output may be null.
+ * rows = 0 clears grad_weight and grad_bias. */
+ICTC_API int32_t ictc_o2_linear_backward(
+    const void* x, int64_t x_stride, const void* weight, int64_t weight_stride,
+    const float* preact, const void* grad_output, int64_t grad_stride, void* grad_x,
+    void* grad_weight, void* grad_bias, void* workspace, size_t workspace_bytes, int64_t rows,
+    int64_t in, int64_t out, int32_t dtype, int32_t activation, void* stream);
 
 #ifdef __cplusplus
 }
