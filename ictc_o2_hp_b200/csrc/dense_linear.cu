@@ -19,14 +19,14 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "dense_epilogue.cuh"
+#include "dense_pair.cuh"
 #include "dense_types.cuh"
 #include "tcgen05.cuh"
+#include "tmap.cuh"
 
 namespace ictc {
 namespace {
-
-// Bounded-wait codes of this unit.
-constexpr int kCodeProducer = 18, kCodeMma = 19, kCodeEpilogue = 20, kCodeDrain = 21;
 
 constexpr int kBM = 128;           // rows of an output tile
 constexpr int kBK = 64;            // K elements of a stage
@@ -35,50 +35,6 @@ constexpr int kProducerWarps = 8;  // warps 8-15
 constexpr int kMmaWarp = kEpilogueWarps + kProducerWarps;
 constexpr int kProductThreads = (kMmaWarp + 1) * 32;
 constexpr int kGroupChunks = 4;    // float32: K stages between moves into registers
-
-struct Epilogue {
-  const void* bias;      // [n] or null
-  const void* residual;  // [m, n] or null
-  int64_t residual_stride;
-  float* preact;         // [m, n] p, or null
-  void* out;             // [m, n]
-  float* partial;        // [splits][m][n] instead of out when the K axis is split
-  int activation;
-  bool vec;              // four columns per access
-};
-
-// C[m, n] = sum over k of A(m, k) B(n, k)
-struct ProductArgs {
-  const void *a, *b;
-  int64_t m, n, k;
-  int64_t lda, ldb;      // distance of rows (K-major) or of k (MN-major), in elements
-  int tiles_m, tiles_n, splits, chunks, chunks_per_split;
-  bool vec_a, vec_b;     // every 8-element chunk inside the operand is 16-byte aligned
-  Epilogue e;
-};
-
-struct TilePos {
-  int64_t m0, n0;
-  int split, c0, c1;
-};
-
-// Work item t: the splits of K outermost; tiles in bands of eight row tiles, so that the
-// CTAs that run together share rows of A and of B in L2.
-__device__ __forceinline__ TilePos tile_at(const ProductArgs& p, int64_t t, int bn) {
-  const int64_t tiles = static_cast<int64_t>(p.tiles_m) * p.tiles_n;
-  TilePos pos;
-  pos.split = static_cast<int>(t / tiles);
-  const int64_t r = t - pos.split * tiles;
-  const int64_t band = r / (8ll * p.tiles_n);
-  const int64_t first = band * 8;
-  const int64_t high = p.tiles_m - first < 8 ? p.tiles_m - first : 8;
-  const int64_t q = r - band * 8 * p.tiles_n;
-  pos.m0 = (first + q % high) * kBM;
-  pos.n0 = (q / high) * bn;
-  pos.c0 = pos.split * p.chunks_per_split;
-  pos.c1 = pos.c0 + p.chunks_per_split < p.chunks ? pos.c0 + p.chunks_per_split : p.chunks;
-  return pos;
-}
 
 template <typename T>
 constexpr int kPieces = sizeof(T) == 4 ? 3 : 1;
@@ -175,47 +131,6 @@ __device__ __forceinline__ void store_operand(unsigned char* dst, int tid,
   }
 }
 
-// ------------------------------------------------------------------------ epilogue
-
-// Four columns of a row: bias, p, activation, residual and the store of y.
-template <typename T>
-__device__ __forceinline__ void finish4(const Epilogue& e, int64_t row, int64_t col, int64_t n,
-                                        float (&v)[4], const float (&bias)[4]) {
-  const int64_t at = row * n + col;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) v[j] += bias[j];
-  if (e.vec) {
-    if (e.preact) *reinterpret_cast<float4*>(e.preact + at) = make_float4(v[0], v[1], v[2], v[3]);
-    Pack<T, 4> r{};
-    if (e.residual)
-      r = *reinterpret_cast<const Pack<T, 4>*>(static_cast<const T*>(e.residual) +
-                                               row * e.residual_stride + col);
-    Pack<T, 4> o;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      o.v[j] = from_float<T>(activate(v[j], e.activation) + (e.residual ? to_float(r.v[j]) : 0.f));
-    *reinterpret_cast<Pack<T, 4>*>(static_cast<T*>(e.out) + at) = o;
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (col + j < n) {
-        if (e.preact) e.preact[at + j] = v[j];
-        float y = activate(v[j], e.activation);
-        if (e.residual)
-          y += to_float(static_cast<const T*>(e.residual)[row * e.residual_stride + col + j]);
-        static_cast<T*>(e.out)[at + j] = from_float<T>(y);
-      }
-  }
-}
-
-template <typename T>
-__device__ __forceinline__ void load_bias4(const Epilogue& e, int64_t col, int64_t n,
-                                           float (&bias)[4]) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-    bias[j] = e.bias && col + j < n ? to_float(static_cast<const T*>(e.bias)[col + j]) : 0.f;
-}
-
 // One element by FMAs in K order, for elements whose operands hold infinities or NaN.
 template <bool A_MN, bool B_MN>
 __device__ __noinline__ float plain_dot(const float* a, int64_t lda, const float* b, int64_t ldb,
@@ -280,7 +195,7 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const Produ
     Held<T, kBM> ha;
     Held<T, BN> hb;
     if (t < total) {
-      TilePos pos = tile_at(p, t, BN);
+      TilePos pos = tile_at<kBM>(p, t, BN);
       int c = pos.c0;
       load_operand<T, A_MN, kBM>(a, p.lda, pos.m0, p.m, static_cast<int64_t>(c) * kBK, p.k,
                                  p.vec_a, tid, ha);
@@ -298,7 +213,7 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const Produ
           t += gridDim.x;
           more = t < total;
           if (more) {
-            pos = tile_at(p, t, BN);
+            pos = tile_at<kBM>(p, t, BN);
             c = pos.c0;
           }
         }
@@ -321,7 +236,7 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const Produ
       bool ok = true;
       uint32_t it = 0, set = 0;
       for (int64_t t = blockIdx.x; ok && t < total; t += gridDim.x) {
-        const TilePos pos = tile_at(p, t, BN);
+        const TilePos pos = tile_at<kBM>(p, t, BN);
         for (int c = pos.c0; ok && c < pos.c1;) {
           const int group_end = P == 3 && c + kGroupChunks < pos.c1 ? c + kGroupChunks : pos.c1;
           ok = mbar_wait(&room[set & 1], ((set >> 1) & 1) ^ 1, kCodeMma);
@@ -378,7 +293,7 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const Produ
     bool ok = true;
     uint32_t set = 0;
     for (int64_t t = blockIdx.x; ok && t < total; t += gridDim.x) {
-      const TilePos pos = tile_at(p, t, BN);
+      const TilePos pos = tile_at<kBM>(p, t, BN);
       float acc[kHalf];
       const int groups = P == 3 ? (pos.c1 - pos.c0 + kGroupChunks - 1) / kGroupChunks : 1;
       for (int gi = 0; gi < groups; ++gi, ++set) {
@@ -408,55 +323,23 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const Produ
         if (lane == 0) mbar_arrive(&room[set & 1]);
       }
       if (!ok) break;
-      // 32 x 32 blocks through shared memory, so that eight lanes write 32 consecutive
-      // columns of a row
-#pragma unroll
-      for (int cb = 0; cb < kHalf / 32; ++cb) {
-#pragma unroll
-        for (int c = 0; c < 8; ++c)
-          mine[lane * 8 + (c ^ (lane & 7))] =
-              make_float4(acc[cb * 32 + 4 * c], acc[cb * 32 + 4 * c + 1],
-                          acc[cb * 32 + 4 * c + 2], acc[cb * 32 + 4 * c + 3]);
-        __syncwarp();
-        const int64_t col = pos.n0 + half * kHalf + cb * 32 + (lane & 7) * 4;
-        float bias[4];
-        load_bias4<T>(p.e, col, p.n, bias);
-#pragma unroll 2
-        for (int i = 0; i < 8; ++i) {
-          const int r = i * 4 + (lane >> 3);
-          const int64_t row = pos.m0 + quad * 32 + r;
-          const float4 f = mine[r * 8 + ((lane & 7) ^ (r & 7))];
-          if (row >= p.m || col >= p.n) continue;
-          float v[4] = {f.x, f.y, f.z, f.w};
-          if constexpr (P == 3) {
-            const bool fine = isfinite(v[0]) && isfinite(v[1]) && isfinite(v[2]) && isfinite(v[3]);
-            if (!fine) {
-              const int64_t k0 = static_cast<int64_t>(pos.c0) * kBK;
-              const int64_t k1 = static_cast<int64_t>(pos.c1) * kBK < p.k
-                                     ? static_cast<int64_t>(pos.c1) * kBK : p.k;
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                if (!isfinite(v[j]) && col + j < p.n)
-                  v[j] = plain_dot<A_MN, B_MN>(static_cast<const float*>(p.a), p.lda,
-                                               static_cast<const float*>(p.b), p.ldb, row,
-                                               col + j, k0, k1);
-            }
-          }
-          if (p.e.partial) {
-            float* o = p.e.partial + (pos.split * p.m + row) * p.n + col;
-            if (p.e.vec) {
-              *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
-            } else {
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                if (col + j < p.n) o[j] = v[j];
-            }
-          } else {
-            finish4<T>(p.e, row, col, p.n, v, bias);
+      const auto redo = [&](int64_t row, int64_t col, float v) {
+        if constexpr (P == 3) {
+          if (!isfinite(v)) {
+            const int64_t k0 = static_cast<int64_t>(pos.c0) * kBK;
+            const int64_t k1 = static_cast<int64_t>(pos.c1) * kBK < p.k
+                                   ? static_cast<int64_t>(pos.c1) * kBK : p.k;
+            if (col < p.n)
+              v = plain_dot<A_MN, B_MN>(static_cast<const float*>(p.a), p.lda,
+                                        static_cast<const float*>(p.b), p.ldb, row, col, k0, k1);
           }
         }
-        __syncwarp();
-      }
+        return v;
+      };
+#pragma unroll
+      for (int cb = 0; cb < kHalf / 32; ++cb)
+        write_block<T>(p, pos.split, acc + cb * 32, mine, pos.m0 + quad * 32,
+                       pos.n0 + half * kHalf + cb * 32, lane, redo);
     }
   }
   tcgen05_fence_before();
@@ -626,6 +509,10 @@ int current_device() {
   return cudaGetDevice(&device) == cudaSuccess ? device : 0;
 }
 
+bool chunk_aligned(const void* p, int64_t ld, size_t size) {
+  return aligned(p, 16) && (ld * static_cast<int64_t>(size)) % 16 == 0;
+}
+
 struct Split {
   int tiles_m, tiles_n, bn, chunks, splits, chunks_per_split;
   bool fits;  // tile counts fit the kernel's integers
@@ -651,8 +538,68 @@ Split plan_product(int64_t m, int64_t n, int64_t k, int device) {
   return s;
 }
 
-size_t split_bytes(const Split& s, int64_t m, int64_t n) {
-  return s.splits > 1 ? static_cast<size_t>(s.splits) * m * n * sizeof(float) : 0;
+
+// ------------------------------------------------------------ 16-bit pairs: host side
+
+struct PairPlan {
+  bool ok;
+  int bn, tiles_m, tiles_n, chunks, splits, chunks_per_split;
+};
+
+// Pairs take 16-bit products whose rows TMA can address, from one full 128 x 128 tile of
+// work on.  BN is 256 unless 128-wide tiles leave the last wave of pairs fuller by more
+// than the 5 % they lose to the operand reads (shared memory: 96 instead of 64 bytes a
+// cycle).  K is split as for the single-SM kernel, over pairs.
+PairPlan plan_pair(int64_t m, int64_t n, int64_t k, int device) {
+  PairPlan s{};
+  if (m >= (1ll << 30) || n >= (1ll << 30) || k >= (1ll << 30)) return s;
+  const int64_t pairs = sm_count(device) / 2, tm = ceil_div(m, kPairRows);
+  const auto fill = [&](int64_t bn) {
+    const int64_t tiles = tm * ceil_div(n, bn);
+    const double waves = static_cast<double>(ceil_div(tiles, pairs));
+    return static_cast<double>(m) * n / (waves * pairs * kPairRows * bn);
+  };
+  s.bn = n > 128 && fill(256) >= 0.95 * fill(128) ? 256 : 128;
+  const int64_t tn = ceil_div(n, s.bn), chunks = ceil_div(k, 64);
+  s.tiles_m = static_cast<int>(tm);
+  s.tiles_n = static_cast<int>(tn);
+  s.chunks = static_cast<int>(chunks);
+  int64_t splits = tm * tn >= pairs ? 1 : pairs / (tm * tn);
+  if (splits > chunks / 8) splits = chunks / 8;
+  if (splits < 1) splits = 1;
+  s.chunks_per_split = static_cast<int>(ceil_div(chunks, splits));
+  s.splits = static_cast<int>(ceil_div(chunks, s.chunks_per_split));
+  s.ok = true;
+  return s;
+}
+
+// The pair kernel needs a tile's worth of work to be worth its cluster start-up.
+bool use_pair(int64_t m, int64_t n, int64_t k) {
+  return static_cast<double>(m) * n * k >= static_cast<double>(1 << 21);
+}
+
+// Bytes of partial products, whichever kernel a call's pointers let it take.
+size_t split_bytes(int64_t m, int64_t n, int64_t k, int dtype, int device) {
+  int64_t splits = plan_product(m, n, k, device).splits;
+  if (dtype != ICTC_DTYPE_F32) {
+    const int64_t q = plan_pair(m, n, k, device).splits;
+    if (q > splits) splits = q;
+  }
+  return splits > 1 ? static_cast<size_t>(splits) * m * n * sizeof(float) : 0;
+}
+
+template <typename T, bool A_MN, bool B_MN, int BN>
+int launch_pair(const PairMaps& maps, const ProductArgs& p, int device, cudaStream_t stream) {
+  const void* fn = reinterpret_cast<const void*>(pair_product_kernel<T, A_MN, B_MN, BN>);
+  const int st = allow_smem(fn, kPairSmem<BN>);
+  if (st != ICTC_OK) return st;
+  const int64_t total = static_cast<int64_t>(p.tiles_m) * p.tiles_n * p.splits;
+  const int64_t pairs = sm_count(device) / 2;
+  pair_product_kernel<T, A_MN, B_MN, BN>
+      <<<static_cast<unsigned>(2 * (total < pairs ? total : pairs)), kPairThreads, kPairSmem<BN>,
+         stream>>>(maps, p);
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? ICTC_OK : cuda_fail(e, "linear pair product launch");
 }
 
 template <typename T, bool A_MN, bool B_MN, int BN>
@@ -669,15 +616,46 @@ int launch_product(const ProductArgs& p, int device, cudaStream_t stream) {
   return e == cudaSuccess ? ICTC_OK : cuda_fail(e, "linear product launch");
 }
 
-bool chunk_aligned(const void* p, int64_t ld, size_t size) {
-  return aligned(p, 16) && (ld * static_cast<int64_t>(size)) % 16 == 0;
-}
-
 // C = epilogue(A B^T); `partial` holds split_bytes() when the plan splits K.
 template <typename T, bool A_MN, bool B_MN>
 int run_product(const T* a, int64_t lda, const T* b, int64_t ldb, int64_t m, int64_t n, int64_t k,
                 Epilogue e, float* partial, cudaStream_t stream) {
   const int device = current_device();
+  e.vec = n % 4 == 0 && aligned(e.out, 4 * sizeof(T)) &&
+          (!e.residual || (aligned(e.residual, 4 * sizeof(T)) && e.residual_stride % 4 == 0)) &&
+          aligned(e.preact, 16) && aligned(partial, 16);
+  const auto join = [&](int splits) {
+    const int64_t blocks = ceil_div(m * ceil_div(n, 4), 256);
+    const int64_t cap = static_cast<int64_t>(sm_count(device)) * 8;
+    e.partial = partial;
+    join_splits_kernel<T><<<static_cast<unsigned>(blocks < cap ? blocks : cap), 256, 0, stream>>>(
+        e, m, n, splits);
+    const cudaError_t err = cudaGetLastError();
+    return err == cudaSuccess ? ICTC_OK : cuda_fail(err, "linear split join launch");
+  };
+  if constexpr (sizeof(T) == 2) {
+    const PairPlan q = plan_pair(m, n, k, device);
+    PairMaps maps;
+    if (q.ok && use_pair(m, n, k) && chunk_aligned(a, lda, 2) && chunk_aligned(b, ldb, 2)) {
+      constexpr bool kBf16 = std::is_same_v<T, __nv_bfloat16>;
+      const bool mapped =
+          encode_matrix_map(a, kBf16, A_MN ? m : k, A_MN ? k : m, lda * 2, 64, A_MN ? 64 : 128,
+                            &maps.a) == 0 &&
+          encode_matrix_map(b, kBf16, B_MN ? n : k, B_MN ? k : n, ldb * 2, 64,
+                            B_MN ? 64 : q.bn / 2, &maps.b) == 0;
+      if (mapped) {
+        ProductArgs p{};
+        p.m = m; p.n = n; p.k = k;
+        p.tiles_m = q.tiles_m; p.tiles_n = q.tiles_n;
+        p.splits = q.splits; p.chunks = q.chunks; p.chunks_per_split = q.chunks_per_split;
+        p.e = e;
+        p.e.partial = q.splits > 1 ? partial : nullptr;
+        const int st = q.bn == 256 ? launch_pair<T, A_MN, B_MN, 256>(maps, p, device, stream)
+                                   : launch_pair<T, A_MN, B_MN, 128>(maps, p, device, stream);
+        return st != ICTC_OK || q.splits == 1 ? st : join(q.splits);
+      }
+    }
+  }
   const Split s = plan_product(m, n, k, device);
   if (!s.fits) return fail(ICTC_ERR_UNSUPPORTED, "linear: a dimension is too large");
   ProductArgs p{};
@@ -688,20 +666,11 @@ int run_product(const T* a, int64_t lda, const T* b, int64_t ldb, int64_t m, int
   p.splits = s.splits; p.chunks = s.chunks; p.chunks_per_split = s.chunks_per_split;
   p.vec_a = chunk_aligned(a, lda, sizeof(T));
   p.vec_b = chunk_aligned(b, ldb, sizeof(T));
-  e.vec = n % 4 == 0 && aligned(e.out, 4 * sizeof(T)) &&
-          (!e.residual || (aligned(e.residual, 4 * sizeof(T)) && e.residual_stride % 4 == 0)) &&
-          aligned(e.preact, 16) && aligned(partial, 16);
   e.partial = s.splits > 1 ? partial : nullptr;
   p.e = e;
   const int st = s.bn == 64 ? launch_product<T, A_MN, B_MN, 64>(p, device, stream)
                             : launch_product<T, A_MN, B_MN, 128>(p, device, stream);
-  if (st != ICTC_OK || s.splits == 1) return st;
-  const int64_t blocks = ceil_div(m * ceil_div(n, 4), 256);
-  const int64_t cap = static_cast<int64_t>(sm_count(device)) * 8;
-  join_splits_kernel<T><<<static_cast<unsigned>(blocks < cap ? blocks : cap), 256, 0, stream>>>(
-      e, m, n, s.splits);
-  const cudaError_t err = cudaGetLastError();
-  return err == cudaSuccess ? ICTC_OK : cuda_fail(err, "linear split join launch");
+  return st != ICTC_OK || s.splits == 1 ? st : join(s.splits);
 }
 
 template <typename T, int V>
@@ -770,8 +739,8 @@ BackwardPlan plan_backward(int64_t m, int64_t n, int64_t k, int dtype, bool slop
   b.columns = d_bytes;
   const int64_t parts = m < kSlopeParts ? m : kSlopeParts;
   b.partial = b.columns + align_up(static_cast<size_t>(parts) * n * sizeof(float), 256);
-  size_t split = split_bytes(plan_product(m, k, n, device), m, k);
-  const size_t other = split_bytes(plan_product(n, k, m, device), n, k);
+  size_t split = split_bytes(m, k, n, dtype, device);
+  const size_t other = split_bytes(n, k, m, dtype, device);
   if (other > split) split = other;
   b.total = b.partial + align_up(split, 256);
   return b;
@@ -858,7 +827,7 @@ extern "C" int32_t ictc_o2_linear_workspace(int64_t rows, int64_t in, int64_t ou
   if (st != ICTC_OK) return st;
   if (!forward_bytes || !backward_bytes) return fail(ICTC_ERR_INVALID, "null output");
   *forward_bytes =
-      rows <= kFewRows ? 0 : split_bytes(plan_product(rows, out, in, device), rows, out);
+      rows <= kFewRows ? 0 : split_bytes(rows, out, in, dtype, device);
   *backward_bytes =
       rows == 0 ? 0
                 : plan_backward(rows, out, in, dtype, activation != ICTC_ACT_NONE, device).total;
@@ -878,7 +847,7 @@ extern "C" int32_t ictc_o2_linear_forward(const void* x, int64_t x_stride, const
   if (x_stride < 0 || weight_stride < 0 || residual_stride < 0)
     return fail(ICTC_ERR_INVALID, "negative row stride");
   const size_t need = rows <= kFewRows
-                          ? 0 : split_bytes(plan_product(rows, out, in, current_device()), rows, out);
+                          ? 0 : split_bytes(rows, out, in, dtype, current_device());
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
     return fail(ICTC_ERR_WORKSPACE, "workspace has %zu bytes, needs %zu (16-byte aligned)",
                 workspace ? workspace_bytes : 0, need);

@@ -32,6 +32,13 @@ struct alignas(64) RowTileMaps {
 int encode_row_tile_maps(const float* base, int64_t rows, int C, int M, bool full, bool cm,
                          int64_t width, int Ct, CUtensorMap* maps);
 
+// Host: a row-major matrix of 16-bit elements, `outer` rows of `inner` elements `stride`
+// bytes apart, read in boxes of box_inner x box_outer (box_inner = 64: one 128-byte
+// swizzled row), zeros outside.  Returns 0, or -1 when the driver entry point is
+// unavailable or the encoding is rejected.
+int encode_matrix_map(const void* base, bool bf16, int64_t inner, int64_t outer, int64_t stride,
+                      int box_inner, int box_outer, CUtensorMap* map);
+
 // 3-D tile load of box coordinates (x, y, z) into shared memory, completing on `bar`.
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z,
                                             uint64_t* bar) {
