@@ -121,6 +121,9 @@ def ptr(t: torch.Tensor | None) -> int | None:
 
 
 def stream_of(device: torch.device) -> int:
+    # the raw handle, without building a torch.cuda.Stream object around it (2 us a call)
+    if device.index is not None:
+        return torch._C._cuda_getCurrentRawStream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
 

@@ -147,7 +147,7 @@ extern "C" int32_t ictc_o2_device_error(int32_t* code) {
   // every unit's flag is read and cleared; the first nonzero code is reported
   int (*const units[])(int*) = {ictc::tp_take_device_error, ictc::uvu_take_device_error,
                                 ictc::radial_take_device_error, ictc::probe_take_device_error,
-                                ictc::dense_take_device_error};
+                                ictc::dense_take_device_error, ictc::norm_take_device_error};
   int first = 0;
   for (auto take : units) {
     int value = 0;

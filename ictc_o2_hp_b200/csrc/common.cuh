@@ -29,6 +29,7 @@ int uvu_take_device_error(int* code);
 int radial_take_device_error(int* code);
 int probe_take_device_error(int* code);
 int dense_take_device_error(int* code);
+int norm_take_device_error(int* code);
 
 // Opts a kernel into `bytes` of dynamic shared memory (cached per kernel).
 int allow_smem(const void* kernel, size_t bytes);

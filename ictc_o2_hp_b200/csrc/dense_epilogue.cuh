@@ -58,46 +58,11 @@ __device__ __forceinline__ TilePos tile_at(const ProductArgs& p, int64_t t, int 
 }
 
 
-// One column of a row, v with the bias in it.
+// The residual's four columns of a row (vec epilogues).
 template <typename T>
-__device__ __forceinline__ void store1(const Epilogue& e, int64_t row, int64_t col, int64_t n,
-                                       float v) {
-  if (e.preact) e.preact[row * n + col] = v;
-  float y = activate(v, e.activation);
-  if (e.residual) y += to_float(static_cast<const T*>(e.residual)[row * e.residual_stride + col]);
-  static_cast<T*>(e.out)[row * n + col] = from_float<T>(y);
-}
-
-// Four columns of a row: bias, p, activation, residual and the store of y.
-template <typename T>
-__device__ __forceinline__ void finish4(const Epilogue& e, int64_t row, int64_t col, int64_t n,
-                                        float (&v)[4], const float (&bias)[4]) {
-  const int64_t at = row * n + col;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) v[j] += bias[j];
-  if (e.vec) {
-    if (e.preact) *reinterpret_cast<float4*>(e.preact + at) = make_float4(v[0], v[1], v[2], v[3]);
-    Pack<T, 4> r{};
-    if (e.residual)
-      r = *reinterpret_cast<const Pack<T, 4>*>(static_cast<const T*>(e.residual) +
-                                               row * e.residual_stride + col);
-    Pack<T, 4> o;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      o.v[j] = from_float<T>(activate(v[j], e.activation) + (e.residual ? to_float(r.v[j]) : 0.f));
-    *reinterpret_cast<Pack<T, 4>*>(static_cast<T*>(e.out) + at) = o;
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (col + j < n) store1<T>(e, row, col + j, n, v[j]);
-  }
-}
-
-// One column of a row.
-template <typename T>
-__device__ __forceinline__ void finish1(const Epilogue& e, int64_t row, int64_t col, int64_t n,
-                                        float v, float bias) {
-  store1<T>(e, row, col, n, v + bias);
+__device__ __forceinline__ Pack<T, 4> residual4(const Epilogue& e, int64_t row, int64_t col) {
+  return *reinterpret_cast<const Pack<T, 4>*>(static_cast<const T*>(e.residual) +
+                                              row * e.residual_stride + col);
 }
 
 template <typename T>
@@ -108,59 +73,90 @@ __device__ __forceinline__ void load_bias4(const Epilogue& e, int64_t col, int64
     bias[j] = e.bias && col + j < n ? to_float(static_cast<const T*>(e.bias)[col + j]) : 0.f;
 }
 
+// One column of a row: bias, p, activation, residual and the store of y.
+template <typename T, int ACT>
+__device__ __forceinline__ void finish1(const Epilogue& e, int64_t row, int64_t col, int64_t n,
+                                        float v, float bias) {
+  v += bias;
+  if (e.preact) e.preact[row * n + col] = v;
+  float y = activate<ACT, sizeof(T) == 2>(v, e.activation);
+  if (e.residual) y += to_float(static_cast<const T*>(e.residual)[row * e.residual_stride + col]);
+  static_cast<T*>(e.out)[row * n + col] = from_float<T>(y);
+}
+
+// Four columns of a row with 16-byte (float32) or 8-byte accesses; r is the residual's, 0
+// without one.
+template <typename T, int ACT>
+__device__ __forceinline__ void finish4(const Epilogue& e, int64_t at, float (&v)[4],
+                                        const float (&bias)[4], const Pack<T, 4>& r) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] += bias[j];
+  if (e.preact) *reinterpret_cast<float4*>(e.preact + at) = make_float4(v[0], v[1], v[2], v[3]);
+  Pack<T, 4> o;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    o.v[j] = from_float<T>(activate<ACT, sizeof(T) == 2>(v[j], e.activation) + to_float(r.v[j]));
+  *reinterpret_cast<Pack<T, 4>*>(static_cast<T*>(e.out) + at) = o;
+}
 
 // One 32 x 32 block of an output tile, row-per-lane in `acc`, to memory: through the
 // warp's 4 KB of shared memory (16-byte chunks XOR-swizzled by row), so that lanes of
 // one row touch consecutive columns: eight lanes four columns each when the rows are
-// aligned for that, 32 lanes one column each otherwise.  `redo` replaces a value (row,
-// col, value) before it is used.
-template <typename T, typename Redo>
+// aligned for that, 32 lanes one column each otherwise.  The residual's loads go out
+// ahead of the stores, which could alias them.  Loops are unrolled by four and no more:
+// the code of an activation is long, and instruction fetches had been the longest stall.
+template <typename T, int ACT>
 __device__ __forceinline__ void write_block(const ProductArgs& p, int split, const float* acc,
-                                            float4* mine, int64_t row0, int64_t col0, int lane,
-                                            const Redo& redo) {
+                                            float4* mine, int64_t row0, int64_t col0, int lane) {
+  const Epilogue& e = p.e;
+  const int64_t col = col0 + (e.vec ? (lane & 7) * 4 : lane);
+  const int rows = p.m - row0 < 32 ? static_cast<int>(p.m - row0) : 32;  // <= 0: none
 #pragma unroll
   for (int c = 0; c < 8; ++c)
     mine[lane * 8 + (c ^ (lane & 7))] =
         make_float4(acc[4 * c], acc[4 * c + 1], acc[4 * c + 2], acc[4 * c + 3]);
   __syncwarp();
-  const Epilogue& e = p.e;
-  if (e.vec) {
-    const int64_t col = col0 + (lane & 7) * 4;
-    if (col < p.n) {
+  if (col < p.n && rows > 0) {
+    if (e.partial) {
+      float* out = e.partial + (split * p.m + row0) * p.n + col;
+      if (e.vec) {
+#pragma unroll 4
+        for (int r = lane >> 3; r < rows; r += 4)
+          *reinterpret_cast<float4*>(out + r * p.n) = mine[r * 8 + ((lane & 7) ^ (r & 7))];
+      } else {
+        const float* flat = reinterpret_cast<const float*>(mine);
+#pragma unroll 4
+        for (int r = 0; r < rows; ++r)
+          out[r * p.n] = flat[r * 32 + (((lane >> 2) ^ (r & 7)) << 2) + (lane & 3)];
+      }
+    } else if (e.vec) {
       float bias[4];
       load_bias4<T>(e, col, p.n, bias);
-#pragma unroll 4
-      for (int i = 0; i < 8; ++i) {
-        const int r = i * 4 + (lane >> 3);
-        const int64_t row = row0 + r;
-        if (row >= p.m) continue;
-        const float4 f = mine[r * 8 + ((lane & 7) ^ (r & 7))];
-        float v[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll 1
+      for (int r0 = lane >> 3; r0 < rows; r0 += 16) {
+        Pack<T, 4> res[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = redo(row, col + j, v[j]);
-        if (e.partial)
-          *reinterpret_cast<float4*>(e.partial + (split * p.m + row) * p.n + col) =
-              make_float4(v[0], v[1], v[2], v[3]);
-        else
-          finish4<T>(e, row, col, p.n, v, bias);
+        for (int i = 0; i < 4; ++i) {
+          res[i] = Pack<T, 4>{};
+          if (e.residual && r0 + 4 * i < rows) res[i] = residual4<T>(e, row0 + r0 + 4 * i, col);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = r0 + 4 * i;
+          if (r < rows) {
+            const float4 f = mine[r * 8 + ((lane & 7) ^ (r & 7))];
+            float v[4] = {f.x, f.y, f.z, f.w};
+            finish4<T, ACT>(e, (row0 + r) * p.n + col, v, bias, res[i]);
+          }
+        }
       }
-    }
-  } else {
-    const int64_t col = col0 + lane;
-    if (col < p.n) {
+    } else {
       const float bias = e.bias ? to_float(static_cast<const T*>(e.bias)[col]) : 0.f;
       const float* flat = reinterpret_cast<const float*>(mine);
 #pragma unroll 4
-      for (int r = 0; r < 32; ++r) {
-        const int64_t row = row0 + r;
-        if (row >= p.m) break;
-        const float v =
-            redo(row, col, flat[r * 32 + (((lane >> 2) ^ (r & 7)) << 2) + (lane & 3)]);
-        if (e.partial)
-          e.partial[(split * p.m + row) * p.n + col] = v;
-        else
-          finish1<T>(e, row, col, p.n, v, bias);
-      }
+      for (int r = 0; r < rows; ++r)
+        finish1<T, ACT>(e, row0 + r, col, p.n,
+                        flat[r * 32 + (((lane >> 2) ^ (r & 7)) << 2) + (lane & 3)], bias);
     }
   }
   __syncwarp();

@@ -32,8 +32,8 @@ constexpr int kBM = 128;           // rows of an output tile
 constexpr int kBK = 64;            // K elements of a stage
 constexpr int kEpilogueWarps = 8;  // warps 0-7
 constexpr int kProducerWarps = 8;  // warps 8-15
-constexpr int kMmaWarp = kEpilogueWarps + kProducerWarps;
-constexpr int kProductThreads = (kMmaWarp + 1) * 32;
+constexpr int kMmaWarp = kEpilogueWarps;  // the producer warp whose lane 0 issues the MMAs
+constexpr int kProductThreads = (kEpilogueWarps + kProducerWarps) * 32;
 constexpr int kGroupChunks = 4;    // float32: K stages between moves into registers
 
 template <typename T>
@@ -71,16 +71,20 @@ template <typename T, bool MN, int ROWS>
 __device__ __forceinline__ void load_operand(const T* base, int64_t ld, int64_t mn0,
                                              int64_t extent, int64_t k0, int64_t k_end, bool vec,
                                              int tid, Held<T, ROWS>& h) {
+  int row0, c;
+  chunk_place<T, MN, ROWS>(tid, 0, &row0, &c);
+  constexpr int kRowStep = 256 / (MN ? ROWS / 8 : 8);
+  const int64_t inner = (MN ? mn0 : k0) + c * 8;  // first contiguous index
+  const int64_t inner_left = (MN ? extent : k_end) - inner;
+  const int left = inner_left < 8 ? (inner_left < 0 ? 0 : static_cast<int>(inner_left)) : 8;
+  const int64_t outer_left = (MN ? k_end - k0 : extent - mn0) - row0;  // along the stride
+  const int rows_left = outer_left < ROWS ? static_cast<int>(outer_left) : ROWS;
+  const T* src = base + ((MN ? k0 : mn0) + row0) * ld + inner;
+  const int64_t step = kRowStep * ld;
 #pragma unroll
-  for (int i = 0; i < ROWS / 32; ++i) {
-    int row, c;
-    chunk_place<T, MN, ROWS>(tid, i, &row, &c);
-    const int64_t outer = (MN ? k0 : mn0) + row;           // index along the stride
-    const int64_t inner = (MN ? mn0 : k0) + c * 8;         // first contiguous index
-    const int64_t inner_end = MN ? extent : k_end;
-    const bool in = outer < (MN ? k_end : extent);
-    const T* src = base + outer * ld + inner;
-    if (in && vec && inner + 8 <= inner_end) {
+  for (int i = 0; i < ROWS / 32; ++i, src += step) {
+    const bool in = i * kRowStep < rows_left;
+    if (in && vec && left == 8) {
       if constexpr (sizeof(T) == 4) {
         const float4 lo = __ldg(reinterpret_cast<const float4*>(src));
         const float4 hi = __ldg(reinterpret_cast<const float4*>(src) + 1);
@@ -92,7 +96,7 @@ __device__ __forceinline__ void load_operand(const T* base, int64_t ld, int64_t 
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        h.v[i].v[j] = in && inner + j < inner_end ? src[j] : T{};
+        h.v[i].v[j] = in && j < left ? src[j] : T{};
     }
   }
 }
@@ -131,26 +135,68 @@ __device__ __forceinline__ void store_operand(unsigned char* dst, int tid,
   }
 }
 
-// One element by FMAs in K order, for elements whose operands hold infinities or NaN.
+// The NaN and infinite elements of the block that write_block just wrote (lane = row;
+// the values are still in `mine`) again, by FMAs in K order: an infinity or NaN among a
+// float32 product's operands has no bf16 parts to speak of.  Rare, so kept out of line.
 template <bool A_MN, bool B_MN>
-__device__ __noinline__ float plain_dot(const float* a, int64_t lda, const float* b, int64_t ldb,
-                                        int64_t m, int64_t n, int64_t k0, int64_t k1) {
-  float s = 0.f;
-  for (int64_t k = k0; k < k1; ++k)
-    s = fmaf(A_MN ? a[k * lda + m] : a[m * lda + k], B_MN ? b[k * ldb + n] : b[n * ldb + k], s);
-  return s;
+__device__ __noinline__ void repair_block(const ProductArgs& p, int split, int c0, int c1,
+                                          const float* mine, int64_t row, int64_t col0, int lane) {
+  const float* a = static_cast<const float*>(p.a);
+  const float* b = static_cast<const float*>(p.b);
+  const int64_t k0 = static_cast<int64_t>(c0) * kBK;
+  const int64_t k1 = static_cast<int64_t>(c1) * kBK < p.k ? static_cast<int64_t>(c1) * kBK : p.k;
+  for (int c = 0; c < 32; ++c) {
+    const int64_t col = col0 + c;
+    const float v = mine[lane * 32 + (((c >> 2) ^ (lane & 7)) << 2) + (c & 3)];
+    if (row >= p.m || col >= p.n || isfinite(v)) continue;
+    float s = 0.f;
+    for (int64_t k = k0; k < k1; ++k)
+      s = fmaf(A_MN ? a[k * p.lda + row] : a[row * p.lda + k],
+               B_MN ? b[k * p.ldb + col] : b[col * p.ldb + k], s);
+    if (p.e.partial)
+      p.e.partial[(split * p.m + row) * p.n + col] = s;
+    else
+      finish1<float, kAnyActivation>(p.e, row, col, p.n, s,
+                     p.e.bias ? static_cast<const float*>(p.e.bias)[col] : 0.f);
+  }
+}
+
+// One thread: the products of a stage, `steps` K steps of 16.  `add` false starts new sums.
+template <typename T, bool A_MN, bool B_MN, int BN>
+__device__ __forceinline__ void issue_stage(uint32_t sa, uint32_t d, int steps, bool add) {
+  constexpr int P = kPieces<T>;
+  constexpr uint32_t kDesc =
+      mma_descriptor(!std::is_same_v<T, __half>, A_MN, B_MN, kBM, BN);
+  // a step's 16 elements along K: 32 bytes of a K-major row, 16 rows MN-major; piece
+  // bytes and steps are multiples of 16, the unit of the descriptor's address field
+  constexpr uint64_t kA = A_MN ? 128 : 2, kB = B_MN ? 128 : 2;
+  constexpr uint64_t kPa = kBM * 8, kPb = BN * 8;
+  uint64_t a = matrix_descriptor(sa, kBK * 128, 1024);
+  uint64_t b = matrix_descriptor(sa + P * kBM * 128, kBK * 128, 1024);
+#pragma unroll 1
+  for (int k = 0; k < steps; ++k, a += kA, b += kB) {
+    mma_f16(d, a, b, kDesc, add);
+    if constexpr (P == 3) {
+      mma_f16(d + BN, a + 2 * kPa, b, kDesc, add);
+      mma_f16(d + BN, a, b + 2 * kPb, kDesc, true);
+      mma_f16(d + BN, a + kPa, b + kPb, kDesc, true);
+      mma_f16(d + BN, a + kPa, b, kDesc, true);
+      mma_f16(d + BN, a, b + kPb, kDesc, true);
+    }
+    add = true;
+  }
 }
 
 // ---------------------------------------------------------------------- the product
 // One persistent CTA per SM, warps specialised: 8 producer warps load operand chunks
-// into registers, cut float32 values and store the swizzled tiles; one thread issues the
-// MMAs of a stage; 8 epilogue warps move finished accumulators out of TMEM, which holds
+// into registers, cut float32 values and store the swizzled tiles; one of their threads
+// issues the MMAs of a stage; 8 epilogue warps move finished accumulators out of TMEM, which holds
 // two sets, so a tile's epilogue overlaps the next tile's products.
-template <typename T, bool A_MN, bool B_MN, int BN>
-__global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const ProductArgs p) {
+template <typename T, bool A_MN, bool B_MN, int BN, int ACT>
+__global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __grid_constant__ ProductArgs p) {
   constexpr int P = kPieces<T>;
   constexpr int S = kStages<T, BN>;
-  constexpr uint32_t kABytes = kBM * 128, kBBytes = BN * 128;
+  constexpr uint32_t kABytes = kBM * 128;
   constexpr uint32_t kSet = (P == 3 ? 2 : 1) * BN;  // TMEM columns of one accumulator set
   constexpr uint32_t kColumns = 2 * kSet;
   extern __shared__ unsigned char raw[];
@@ -184,107 +230,77 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const Produ
   const uint32_t tmem = *tmem_at;
   const int64_t total = static_cast<int64_t>(p.tiles_m) * p.tiles_n * p.splits;
 
-  if (warp >= kEpilogueWarps && warp < kMmaWarp) {
-    // ---- producers
+  if (warp >= kEpilogueWarps) {
+    // ---- producers; lane 0 of the first also issues each stage's MMAs.  (A warp of its
+    // own for them would cost every thread 32 of its 128 registers: registers are given
+    // out to four warps at a time.)
     const int tid = threadIdx.x - kEpilogueWarps * 32;
     const T* a = static_cast<const T*>(p.a);
     const T* b = static_cast<const T*>(p.b);
     int64_t t = blockIdx.x;
     bool ok = true;
-    uint32_t it = 0;
+    uint32_t it = 0, set = 0, in_group = 0;
     Held<T, kBM> ha;
     Held<T, BN> hb;
-    if (t < total) {
-      TilePos pos = tile_at<kBM>(p, t, BN);
-      int c = pos.c0;
-      load_operand<T, A_MN, kBM>(a, p.lda, pos.m0, p.m, static_cast<int64_t>(c) * kBK, p.k,
-                                 p.vec_a, tid, ha);
-      while (ok) {
-        load_operand<T, B_MN, BN>(b, p.ldb, pos.n0, p.n, static_cast<int64_t>(c) * kBK, p.k,
-                                  p.vec_b, tid, hb);
-        const int s = it % S;
-        ok = mbar_wait(&empty[s], ((it / S) & 1) ^ 1, kCodeProducer);
-        if (!ok) break;
-        unsigned char* stage = smem + s * kStageBytes<T, BN>;
-        store_operand<T, A_MN, kBM>(stage, tid, ha);
-        // the next chunk's A is in flight while this chunk's B is cut and stored
-        bool more = true;
-        if (++c == pos.c1) {
-          t += gridDim.x;
-          more = t < total;
-          if (more) {
-            pos = tile_at<kBM>(p, t, BN);
-            c = pos.c0;
+    TilePos pos = tile_at<kBM>(p, t, BN);
+    int c = pos.c0;
+    load_operand<T, A_MN, kBM>(a, p.lda, pos.m0, p.m, static_cast<int64_t>(c) * kBK, p.k, p.vec_a,
+                               tid, ha);
+    for (bool more = true; more; ++it) {
+      load_operand<T, B_MN, BN>(b, p.ldb, pos.n0, p.n, static_cast<int64_t>(c) * kBK, p.k,
+                                p.vec_b, tid, hb);
+      const int s = it % S;
+      ok = mbar_wait(&empty[s], ((it / S) & 1) ^ 1, kCodeProducer);
+      if (!ok) break;
+      unsigned char* stage = smem + s * kStageBytes<T, BN>;
+      store_operand<T, A_MN, kBM>(stage, tid, ha);
+      // the next chunk's A is in flight while this chunk's B is cut and stored
+      const int64_t left = p.k - static_cast<int64_t>(c) * kBK;
+      const bool last = ++c == pos.c1;
+      if (last) {
+        t += gridDim.x;
+        more = t < total;
+        if (more) {
+          pos = tile_at<kBM>(p, t, BN);
+          c = pos.c0;
+        }
+      }
+      if (more)
+        load_operand<T, A_MN, kBM>(a, p.lda, pos.m0, p.m, static_cast<int64_t>(c) * kBK, p.k,
+                                   p.vec_a, tid, ha);
+      store_operand<T, B_MN, BN>(stage + P * kABytes, tid, hb);
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&full[s]);
+      if (warp == kMmaWarp) {
+        const bool close = last || (P == 3 && in_group == kGroupChunks - 1);
+        if (lane == 0) {
+          if (in_group == 0) ok = mbar_wait(&room[set & 1], ((set >> 1) & 1) ^ 1, kCodeMma);
+          if (ok) ok = mbar_wait(&full[s], (it / S) & 1, kCodeMma);
+          if (ok) {
+            tcgen05_fence_after();
+            issue_stage<T, A_MN, B_MN, BN>(smem_addr(stage), tmem + (set & 1) * kSet,
+                                           left < kBK ? static_cast<int>((left + 15) / 16)
+                                                      : kBK / 16,
+                                           in_group > 0);
+            mma_commit(&empty[s]);
+            if (close) mma_commit(&done[set & 1]);
           }
         }
-        if (more)
-          load_operand<T, A_MN, kBM>(a, p.lda, pos.m0, p.m, static_cast<int64_t>(c) * kBK, p.k,
-                                     p.vec_a, tid, ha);
-        store_operand<T, B_MN, BN>(stage + P * kABytes, tid, hb);
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&full[s]);
-        ++it;
-        if (!more) break;
+        ok = __shfl_sync(0xffffffffu, static_cast<int>(ok), 0) != 0;
+        if (!ok) break;
+        in_group = close ? 0 : in_group + 1;
+        set += close ? 1 : 0;
       }
     }
-  } else if (warp == kMmaWarp) {
-    // ---- MMA issue: one thread
-    if (lane == 0) {
-      constexpr bool kBf16 = !std::is_same_v<T, __half>;
-      constexpr uint32_t kDesc = mma_descriptor(kBf16, A_MN, B_MN, kBM, BN);
-      bool ok = true;
-      uint32_t it = 0, set = 0;
-      for (int64_t t = blockIdx.x; ok && t < total; t += gridDim.x) {
-        const TilePos pos = tile_at<kBM>(p, t, BN);
-        for (int c = pos.c0; ok && c < pos.c1;) {
-          const int group_end = P == 3 && c + kGroupChunks < pos.c1 ? c + kGroupChunks : pos.c1;
-          ok = mbar_wait(&room[set & 1], ((set >> 1) & 1) ^ 1, kCodeMma);
-          if (!ok) break;
-          tcgen05_fence_after();
-          const uint32_t d = tmem + (set & 1) * kSet;
-          bool add = false;
-          for (; c < group_end; ++c, ++it) {
-            const int s = it % S;
-            ok = mbar_wait(&full[s], (it / S) & 1, kCodeMma);
-            if (!ok) break;
-            tcgen05_fence_after();
-            const uint32_t sa = smem_addr(smem + s * kStageBytes<T, BN>);
-            const uint32_t sb = sa + P * kABytes;
-            const int64_t left = p.k - static_cast<int64_t>(c) * kBK;
-            const int steps = left < kBK ? static_cast<int>((left + 15) / 16) : kBK / 16;
-            for (int k = 0; k < steps; ++k) {
-              // 16 elements along K: 32 bytes of a K-major row, 16 rows MN-major
-              const uint32_t ao = k * (A_MN ? 2048 : 32), bo = k * (B_MN ? 2048 : 32);
-              uint64_t da[P], db[P];
-#pragma unroll
-              for (int q = 0; q < P; ++q) {
-                da[q] = matrix_descriptor(sa + q * kABytes + ao, kBK * 128, 1024);
-                db[q] = matrix_descriptor(sb + q * kBBytes + bo, kBK * 128, 1024);
-              }
-              mma_f16(d, da[0], db[0], kDesc, add);
-              if constexpr (P == 3) {
-                mma_f16(d + BN, da[2], db[0], kDesc, add);
-                mma_f16(d + BN, da[0], db[2], kDesc, true);
-                mma_f16(d + BN, da[1], db[1], kDesc, true);
-                mma_f16(d + BN, da[1], db[0], kDesc, true);
-                mma_f16(d + BN, da[0], db[1], kDesc, true);
-              }
-              add = true;
-            }
-            mma_commit(&empty[s]);
-          }
-          if (!ok) break;
-          mma_commit(&done[set & 1]);
-          ++set;
-        }
-      }
-      if (!ok) {  // let the MMAs in flight finish before TMEM and the stages go away
+    if (!ok && warp == kMmaWarp) {
+      // let the MMAs in flight finish before TMEM and the stages go away
+      if (lane == 0) {
         mma_commit(drain);
         mbar_wait(drain, 0, kCodeDrain, kDrainLimitNs);
       }
+      __syncwarp();
     }
-    __syncwarp();
   } else {
     // ---- epilogue: warp w holds TMEM lanes 32 (w % 4) .. + 31, half w / 4 of the columns
     constexpr int kHalf = BN / 2;
@@ -306,40 +322,35 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const Produ
         for (int j = 0; j < kHalf; j += 16) {
           float v[16];
           tmem_load16(at + j, v);
-          if constexpr (P == 3) {
-            float w[16];
-            tmem_load16(at + BN + j, w);
-            tmem_load_wait();
-#pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] += w[i];
-          } else {
-            tmem_load_wait();
-          }
+          tmem_load_wait();
 #pragma unroll
           for (int i = 0; i < 16; ++i) acc[j + i] = gi == 0 ? v[i] : acc[j + i] + v[i];
+          if constexpr (P == 3) {
+            tmem_load16(at + BN + j, v);
+            tmem_load_wait();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[j + i] += v[i];
+          }
         }
         tcgen05_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&room[set & 1]);
       }
       if (!ok) break;
-      const auto redo = [&](int64_t row, int64_t col, float v) {
-        if constexpr (P == 3) {
-          if (!isfinite(v)) {
-            const int64_t k0 = static_cast<int64_t>(pos.c0) * kBK;
-            const int64_t k1 = static_cast<int64_t>(pos.c1) * kBK < p.k
-                                   ? static_cast<int64_t>(pos.c1) * kBK : p.k;
-            if (col < p.n)
-              v = plain_dot<A_MN, B_MN>(static_cast<const float*>(p.a), p.lda,
-                                        static_cast<const float*>(p.b), p.ldb, row, col, k0, k1);
-          }
-        }
-        return v;
-      };
 #pragma unroll
-      for (int cb = 0; cb < kHalf / 32; ++cb)
-        write_block<T>(p, pos.split, acc + cb * 32, mine, pos.m0 + quad * 32,
-                       pos.n0 + half * kHalf + cb * 32, lane, redo);
+      for (int cb = 0; cb < kHalf / 32; ++cb) {
+        const int64_t row0 = pos.m0 + quad * 32, col0 = pos.n0 + half * kHalf + cb * 32;
+        write_block<T, ACT>(p, pos.split, acc + cb * 32, mine, row0, col0, lane);
+        if constexpr (P == 3) {
+          float zero = 0.f;  // stays 0 unless an element is not finite
+#pragma unroll
+          for (int i = 0; i < 32; ++i) zero = fmaf(acc[cb * 32 + i], 0.f, zero);
+          if (__any_sync(0xffffffffu, zero != 0.f))
+            repair_block<A_MN, B_MN>(p, pos.split, pos.c0, pos.c1, reinterpret_cast<const float*>(mine), row0 + lane,
+                                     col0, lane);
+          __syncwarp();
+        }
+      }
     }
   }
   tcgen05_fence_before();
@@ -358,20 +369,27 @@ __global__ void __launch_bounds__(256) join_splits_kernel(const Epilogue e, int6
   const int64_t step = static_cast<int64_t>(gridDim.x) * 256;
   for (int64_t q = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; q < m * quads; q += step) {
     const int64_t row = q / quads, col = (q - row * quads) * 4;
-    float v[4] = {0.f, 0.f, 0.f, 0.f}, bias[4];
-    load_bias4<T>(e, col, n, bias);
     const float* at = e.partial + row * n + col;
-    for (int s = 0; s < splits; ++s, at += m * n) {
-      if (e.vec) {
+    if (e.vec) {
+      float v[4] = {0.f, 0.f, 0.f, 0.f}, bias[4];
+      load_bias4<T>(e, col, n, bias);
+      Pack<T, 4> r{};
+      if (e.residual) r = residual4<T>(e, row, col);
+#pragma unroll 4
+      for (int s = 0; s < splits; ++s, at += m * n) {
         const float4 f = *reinterpret_cast<const float4*>(at);
         v[0] += f.x; v[1] += f.y; v[2] += f.z; v[3] += f.w;
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (col + j < n) v[j] += at[j];
+      }
+      finish4<T, kAnyActivation>(e, row * n + col, v, bias, r);
+    } else {
+      for (int j = 0; j < 4 && col + j < n; ++j) {
+        float v = 0.f;
+        for (int s = 0; s < splits; ++s) v += at[s * m * n + j];
+        finish1<T, kAnyActivation>(
+            e, row, col + j, n, v,
+            e.bias ? to_float(static_cast<const T*>(e.bias)[col + j]) : 0.f);
       }
     }
-    finish4<T>(e, row, col, n, v, bias);
   }
 }
 
@@ -433,7 +451,7 @@ __global__ void __launch_bounds__(kRowThreads) few_rows_kernel(
         if (r >= rows) break;
         const float v = acc[r] + bias;
         if (e.preact) e.preact[r * n + col] = v;
-        float y = activate(v, e.activation);
+        float y = activate<kAnyActivation, sizeof(T) == 2>(v, e.activation);
         if (e.residual)
           y += to_float(static_cast<const T*>(e.residual)[r * e.residual_stride + col]);
         static_cast<T*>(e.out)[r * n + col] = from_float<T>(y);
@@ -446,12 +464,11 @@ __global__ void __launch_bounds__(kRowThreads) few_rows_kernel(
 // Bound by HBM.  A CTA owns a strip of columns and every gridDim.y-th block of rows; each
 // thread keeps its columns' sums in registers, and the CTA's partial row of db is joined
 // over its row lanes in order.
-template <typename T, int V>
+template <typename T, int V, int ACT>
 __global__ void __launch_bounds__(256) slope_kernel(const T* __restrict__ g, int64_t ldg,
                                                     const float* __restrict__ preact,
                                                     T* __restrict__ d, float* __restrict__ partial,
-                                                    int64_t m, int64_t n, int lanes,
-                                                    int activation) {
+                                                    int64_t m, int64_t n, int lanes) {
   __shared__ float sums[256 * V];
   const int tx = threadIdx.x % lanes, ty = threadIdx.x / lanes, rows = 256 / lanes;
   const int64_t col = (static_cast<int64_t>(blockIdx.x) * lanes + tx) * V;
@@ -459,34 +476,36 @@ __global__ void __launch_bounds__(256) slope_kernel(const T* __restrict__ g, int
 #pragma unroll
   for (int j = 0; j < V; ++j) acc[j] = 0.f;
   if (col < n) {
-#pragma unroll 2
-    for (int64_t r = static_cast<int64_t>(blockIdx.y) * rows + ty; r < m;
-         r += static_cast<int64_t>(gridDim.y) * rows) {
-      const Pack<T, V> pg = *reinterpret_cast<const Pack<T, V>*>(g + r * ldg + col);
-      float v[V];
+    constexpr int kAhead = 4;  // rows whose loads go out together, ahead of any store
+    const int64_t step = static_cast<int64_t>(gridDim.y) * rows;
+    for (int64_t r0 = static_cast<int64_t>(blockIdx.y) * rows + ty; r0 < m; r0 += kAhead * step) {
+      Pack<T, V> pg[kAhead];
+      Pack<float, V> pp[kAhead];
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[j] = to_float(pg.v[j]);
-      if (preact != nullptr) {
-        Pack<T, V> o;
-#pragma unroll
-        for (int j = 0; j < V; j += (V >= 4 ? 4 : 1)) {
-          float q[4];
-          if constexpr (V >= 4) {
-            const float4 f = *reinterpret_cast<const float4*>(preact + r * n + col + j);
-            q[0] = f.x; q[1] = f.y; q[2] = f.z; q[3] = f.w;
-          } else {
-            q[0] = preact[r * n + col + j];
-          }
-#pragma unroll
-          for (int i = 0; i < (V >= 4 ? 4 : 1); ++i) {
-            v[j + i] *= activation_slope(q[i], activation);
-            o.v[j + i] = from_float<T>(v[j + i]);
+      for (int q = 0; q < kAhead; ++q) {
+        const int64_t r = r0 + q * step;
+        pg[q] = Pack<T, V>{};
+        if (r < m) {
+          pg[q] = *reinterpret_cast<const Pack<T, V>*>(g + r * ldg + col);
+          if constexpr (ACT != ICTC_ACT_NONE) {
+            pp[q] = *reinterpret_cast<const Pack<float, V>*>(preact + r * n + col);
           }
         }
-        if (d != nullptr) *reinterpret_cast<Pack<T, V>*>(d + r * n + col) = o;
       }
 #pragma unroll
-      for (int j = 0; j < V; ++j) acc[j] += v[j];
+      for (int q = 0; q < kAhead; ++q) {
+        const int64_t r = r0 + q * step;
+        if (r >= m) break;
+        Pack<T, V> o;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          float v = to_float(pg[q].v[j]);
+          if constexpr (ACT != ICTC_ACT_NONE) v *= activation_slope<ACT, sizeof(T) == 2>(pp[q].v[j]);
+          acc[j] += v;
+          o.v[j] = from_float<T>(v);
+        }
+        if constexpr (ACT != ICTC_ACT_NONE) *reinterpret_cast<Pack<T, V>*>(d + r * n + col) = o;
+      }
     }
   }
   if (partial == nullptr) return;
@@ -548,7 +567,7 @@ struct PairPlan {
 
 // Pairs take 16-bit products whose rows TMA can address, from one full 128 x 128 tile of
 // work on.  BN is 256 unless 128-wide tiles leave the last wave of pairs fuller by more
-// than the 5 % they lose to the operand reads (shared memory: 96 instead of 64 bytes a
+// than they lose to the operand traffic in shared memory (192 instead of 128 bytes a
 // cycle).  K is split as for the single-SM kernel, over pairs.
 PairPlan plan_pair(int64_t m, int64_t n, int64_t k, int device) {
   PairPlan s{};
@@ -559,7 +578,7 @@ PairPlan plan_pair(int64_t m, int64_t n, int64_t k, int device) {
     const double waves = static_cast<double>(ceil_div(tiles, pairs));
     return static_cast<double>(m) * n / (waves * pairs * kPairRows * bn);
   };
-  s.bn = n > 128 && fill(256) >= 0.95 * fill(128) ? 256 : 128;
+  s.bn = n > 128 && fill(256) >= 0.65 * fill(128) ? 256 : 128;
   const int64_t tn = ceil_div(n, s.bn), chunks = ceil_div(k, 64);
   s.tiles_m = static_cast<int>(tm);
   s.tiles_n = static_cast<int>(tn);
@@ -588,30 +607,58 @@ size_t split_bytes(int64_t m, int64_t n, int64_t k, int dtype, int device) {
   return splits > 1 ? static_cast<size_t>(splits) * m * n * sizeof(float) : 0;
 }
 
+// Calls f with the activation code as a compile-time constant.
+template <typename F>
+void for_activation(int activation, const F& f) {
+  switch (activation) {
+    case ICTC_ACT_RELU: return f(std::integral_constant<int, ICTC_ACT_RELU>{});
+    case ICTC_ACT_SILU: return f(std::integral_constant<int, ICTC_ACT_SILU>{});
+    case ICTC_ACT_GELU: return f(std::integral_constant<int, ICTC_ACT_GELU>{});
+    case ICTC_ACT_GELU_TANH: return f(std::integral_constant<int, ICTC_ACT_GELU_TANH>{});
+    default: return f(std::integral_constant<int, ICTC_ACT_NONE>{});
+  }
+}
+
+// The epilogue that a launch needs: gradients and partial sums have no activation.
+template <bool FORWARD, typename F>
+void for_epilogue(const ProductArgs& p, const F& f) {
+  if constexpr (FORWARD)
+    for_activation(p.e.partial ? ICTC_ACT_NONE : p.e.activation, f);
+  else
+    f(std::integral_constant<int, ICTC_ACT_NONE>{});
+}
+
 template <typename T, bool A_MN, bool B_MN, int BN>
 int launch_pair(const PairMaps& maps, const ProductArgs& p, int device, cudaStream_t stream) {
-  const void* fn = reinterpret_cast<const void*>(pair_product_kernel<T, A_MN, B_MN, BN>);
-  const int st = allow_smem(fn, kPairSmem<BN>);
-  if (st != ICTC_OK) return st;
   const int64_t total = static_cast<int64_t>(p.tiles_m) * p.tiles_n * p.splits;
   const int64_t pairs = sm_count(device) / 2;
-  pair_product_kernel<T, A_MN, B_MN, BN>
-      <<<static_cast<unsigned>(2 * (total < pairs ? total : pairs)), kPairThreads, kPairSmem<BN>,
-         stream>>>(maps, p);
+  const unsigned grid = static_cast<unsigned>(2 * (total < pairs ? total : pairs));
+  int st = ICTC_OK;
+  for_epilogue<!A_MN && !B_MN>(p, [&](auto act) {
+    const auto kernel = pair_product_kernel<T, A_MN, B_MN, BN, act.value>;
+    st = allow_smem(reinterpret_cast<const void*>(kernel), kPairSmem<BN>);
+    if (st == ICTC_OK) kernel<<<grid, kPairThreads, kPairSmem<BN>, stream>>>(maps, p);
+  });
+  if (st != ICTC_OK) return st;
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? ICTC_OK : cuda_fail(e, "linear pair product launch");
 }
 
 template <typename T, bool A_MN, bool B_MN, int BN>
 int launch_product(const ProductArgs& p, int device, cudaStream_t stream) {
-  const void* fn = reinterpret_cast<const void*>(product_kernel<T, A_MN, B_MN, BN>);
-  const int st = allow_smem(fn, kProductSmem<T, BN>);
-  if (st != ICTC_OK) return st;
   const int64_t total = static_cast<int64_t>(p.tiles_m) * p.tiles_n * p.splits;
   const int64_t sms = sm_count(device);
-  product_kernel<T, A_MN, B_MN, BN>
-      <<<static_cast<unsigned>(total < sms ? total : sms), kProductThreads, kProductSmem<T, BN>,
-         stream>>>(p);
+  const unsigned grid = static_cast<unsigned>(total < sms ? total : sms);
+  int st = ICTC_OK;
+  const auto launch = [&](auto act) {
+    const auto kernel = product_kernel<T, A_MN, B_MN, BN, act.value>;
+    st = allow_smem(reinterpret_cast<const void*>(kernel), kProductSmem<T, BN>);
+    if (st == ICTC_OK) kernel<<<grid, kProductThreads, kProductSmem<T, BN>, stream>>>(p);
+  };
+  // 16-bit products come here only when small or unaligned: one kernel for every activation
+  if constexpr (sizeof(T) == 2) launch(std::integral_constant<int, kAnyActivation>{});
+  else for_epilogue<!A_MN && !B_MN>(p, launch);
+  if (st != ICTC_OK) return st;
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? ICTC_OK : cuda_fail(e, "linear product launch");
 }
@@ -761,12 +808,14 @@ int run_linear_backward(const void* x, int64_t ldx, const void* w, int64_t ldw,
     const bool vec = n % kFull == 0 && chunk_aligned(g, ldg, sizeof(T)) && aligned(preact, 16);
     const SlopePlan s = plan_slope(m, n, vec ? kFull : 1);
     const dim3 grid(s.blocks_x, s.blocks_y);
-    if (vec)
-      slope_kernel<T, kFull><<<grid, 256, 0, stream>>>(d, ldg, slope ? preact : nullptr, d_out,
-                                                       columns, m, n, s.lanes, activation);
-    else
-      slope_kernel<T, 1><<<grid, 256, 0, stream>>>(d, ldg, slope ? preact : nullptr, d_out,
-                                                   columns, m, n, s.lanes, activation);
+    for_activation(activation, [&](auto act) {
+      if (vec)
+        slope_kernel<T, kFull, act.value>
+            <<<grid, 256, 0, stream>>>(d, ldg, preact, d_out, columns, m, n, s.lanes);
+      else
+        slope_kernel<T, 1, act.value>
+            <<<grid, 256, 0, stream>>>(d, ldg, preact, d_out, columns, m, n, s.lanes);
+    });
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return cuda_fail(e, "linear slope launch");
     if (db) {

@@ -121,9 +121,9 @@ __device__ __forceinline__ void load_tile(unsigned char* dst, const CUtensorMap*
   }
 }
 
-template <typename T, bool A_MN, bool B_MN, int BN>
+template <typename T, bool A_MN, bool B_MN, int BN, int ACT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
-    pair_product_kernel(const __grid_constant__ PairMaps maps, const ProductArgs p) {
+    pair_product_kernel(const __grid_constant__ PairMaps maps, const __grid_constant__ ProductArgs p) {
   constexpr int S = kPairStages<BN>;
   constexpr uint32_t kABytes = 128 * 128;
   constexpr uint32_t kColumns = 2 * BN;  // two accumulator sets
@@ -229,7 +229,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     const int quad = warp & 3, half = warp >> 2;
     constexpr int kHalf = BN / 2;
     float4* mine = reinterpret_cast<float4*>(staging + warp * 4096);
-    const auto keep = [](int64_t, int64_t, float v) { return v; };
     bool ok = true;
     uint32_t set = 0;
     for (int64_t t = first; t < total; t += step, ++set) {
@@ -253,7 +252,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           __syncwarp();
           if (lane == 0) arrive_cluster(peer_addr(&room[set & 1], 0));
         }
-        write_block<T>(p, pos.split, acc, mine, row0, pos.n0 + half * kHalf + cb * 32, lane, keep);
+        write_block<T, ACT>(p, pos.split, acc, mine, row0, pos.n0 + half * kHalf + cb * 32, lane);
       }
     }
   }

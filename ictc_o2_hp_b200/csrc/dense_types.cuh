@@ -30,46 +30,58 @@ __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) {
 template <>
 __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 
-// N elements moved as one aligned access (N * sizeof(T) = 4, 8 or 16 bytes, or one
-// element).
+// N elements moved as one access of up to 16 bytes (more as several of them).
 template <typename T, int N>
-struct alignas(sizeof(T) * N) Pack {
+struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) Pack {
   T v[N];
 };
 
-// act(p) and act'(p) for the activation codes of the C ABI.  The code is a kernel
-// argument: the branch is uniform over the launch and costs nothing beside the
-// function itself.
-__device__ __forceinline__ float activate(float p, int activation) {
-  switch (activation) {
+// 1 / (1 + exp(-p)).  FAST (16-bit results) takes the hardware exponential, good to about
+// 2^-21 of the result for any p whose sigmoid a 16-bit type resolves; the quotient is good
+// to 2 ulp in both and exactly 0 where exp overflows.
+template <bool FAST>
+__device__ __forceinline__ float sigmoid(float p) {
+  return __fdividef(1.f, 1.f + (FAST ? __expf(-p) : expf(-p)));
+}
+
+// act(p) and act'(p) for the activation codes of the C ABI.  ACT is the code, or
+// kAnyActivation to take it from the argument (a branch that is uniform over a launch).
+// gelu_tanh is written as p s(2 u), u = c (p + 0.044715 p^3): (1 + tanh u) / 2 = s(2 u).
+constexpr int kAnyActivation = -1;
+
+template <int ACT, bool FAST>
+__device__ __forceinline__ float activate(float p, int any = ICTC_ACT_NONE) {
+  const int code = ACT == kAnyActivation ? any : ACT;
+  switch (code) {
     case ICTC_ACT_RELU:
       return p > 0.f ? p : (p != p ? p : 0.f);
     case ICTC_ACT_SILU:
-      return p / (1.f + expf(-p));
+      return p * sigmoid<FAST>(p);
     case ICTC_ACT_GELU:
       return 0.5f * p * (1.f + erff(p * 0.70710678118654752f));
     case ICTC_ACT_GELU_TANH:
-      return 0.5f * p * (1.f + tanhf(0.79788456080286536f * (p + 0.044715f * p * p * p)));
+      return p * sigmoid<FAST>(1.5957691216057308f * (p + 0.044715f * p * p * p));
     default:
       return p;
   }
 }
 
-__device__ __forceinline__ float activation_slope(float p, int activation) {
-  switch (activation) {
+template <int ACT, bool FAST>
+__device__ __forceinline__ float activation_slope(float p, int any = ICTC_ACT_NONE) {
+  const int code = ACT == kAnyActivation ? any : ACT;
+  switch (code) {
     case ICTC_ACT_RELU:
       return p > 0.f ? 1.f : 0.f;
     case ICTC_ACT_SILU: {
-      const float s = 1.f / (1.f + expf(-p));
+      const float s = sigmoid<FAST>(p);
       return s * (1.f + p * (1.f - s));
     }
     case ICTC_ACT_GELU:
       return 0.5f * (1.f + erff(p * 0.70710678118654752f)) +
-             p * expf(-0.5f * p * p) * 0.39894228040143268f;
+             p * (FAST ? __expf(-0.5f * p * p) : expf(-0.5f * p * p)) * 0.39894228040143268f;
     case ICTC_ACT_GELU_TANH: {
-      const float c = 0.79788456080286536f;
-      const float t = tanhf(c * (p + 0.044715f * p * p * p));
-      return 0.5f * (1.f + t) + 0.5f * p * (1.f - t * t) * c * (1.f + 0.134145f * p * p);
+      const float s = sigmoid<FAST>(1.5957691216057308f * (p + 0.044715f * p * p * p));
+      return s + p * s * (1.f - s) * 1.5957691216057308f * (1.f + 0.134145f * p * p);
     }
     default:
       return 1.f;

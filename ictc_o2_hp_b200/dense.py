@@ -21,7 +21,7 @@ Like the products, these raise for CPU tensors and other types instead of fallin
 from __future__ import annotations
 
 import math
-from functools import lru_cache
+from functools import lru_cache, wraps
 
 import torch
 from torch import Tensor
@@ -57,22 +57,15 @@ def _rows(t: Tensor) -> Tensor:
     return t if width == 1 or t.stride(1) == 1 else t.contiguous()
 
 
-class _on:
-    """The CUDA device guard, skipped when the device is already current."""
-
-    __slots__ = ("guard",)
-
-    def __init__(self, device):
-        self.guard = None if torch.cuda.current_device() == device.index else \
-            torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _on_device(run):
+    """`run(x, ...)` with x's device current; the guard costs nothing when it already is."""
+    @wraps(run)
+    def guarded(x, *args):
+        if torch.cuda.current_device() == x.device.index:
+            return run(x, *args)
+        with torch.cuda.device(x.device):
+            return run(x, *args)
+    return guarded
 
 
 # Workspace sizes are a function of sizes, type and device alone.
@@ -80,42 +73,42 @@ _norm_workspace = lru_cache(maxsize=4096)(_lib.layer_norm_workspace)
 _linear_workspace = lru_cache(maxsize=4096)(_lib.linear_workspace)
 
 
-def _scratch(size: int, device) -> Tensor | None:
-    return torch.empty(size, dtype=torch.uint8, device=device) if size else None
+def _scratch(size: int, like: Tensor) -> Tensor | None:
+    return like.new_empty(size, dtype=torch.uint8) if size else None
 
 
 # -------------------------------------------------------------------- layer norm
 
 
+@_on_device
 def _norm_run(x: Tensor, weight: Tensor | None, bias: Tensor | None, eps: float,
               stats: bool) -> tuple[Tensor, Tensor | None, Tensor | None]:
     rows = _rows(x)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = x.new_empty(x.shape)
     mean = rstd = None
     if stats:
-        mean = torch.empty(rows.shape[0], dtype=torch.float32, device=x.device)
+        mean = x.new_empty(rows.shape[0], dtype=torch.float32)
         rstd = torch.empty_like(mean)
     params = weight if weight is not None else bias
     pcode = _DTYPES[(x if params is None else params).dtype]
-    with _on(x.device):
-        _lib.layer_norm_forward(rows, weight, bias, y, mean, rstd, eps, _DTYPES[x.dtype], pcode)
+    _lib.layer_norm_forward(rows, weight, bias, y, mean, rstd, eps, _DTYPES[x.dtype], pcode)
     return y, mean, rstd
 
 
+@_on_device
 def _norm_grad_run(x, weight, mean, rstd, grad, pdtype, need):
     """(dx, dweight, dbias), None where `need` is false; pdtype types the last two."""
     rows, g = _rows(x), _rows(grad)
     width = x.shape[-1]
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need[0] else None
-    dw = torch.empty(width, dtype=pdtype, device=x.device) if need[1] else None
-    db = torch.empty(width, dtype=pdtype, device=x.device) if need[2] else None
+    dx = x.new_empty(x.shape) if need[0] else None
+    dw = x.new_empty(width, dtype=pdtype) if need[1] else None
+    db = x.new_empty(width, dtype=pdtype) if need[2] else None
     code = _DTYPES[x.dtype]
     size = 0
     if need[1] or need[2]:
         size = _norm_workspace(rows.shape[0], width, code, x.device.index)
-    with _on(x.device):
-        _lib.layer_norm_backward(rows, weight, mean, rstd, g, dx, dw, db,
-                                 _scratch(size, x.device), code, _DTYPES[pdtype])
+    _lib.layer_norm_backward(rows, weight, mean, rstd, g, dx, dw, db, _scratch(size, x), code,
+                             _DTYPES[pdtype])
     return dx, dw, db
 
 
@@ -226,33 +219,32 @@ def layer_norm(x: Tensor, weight: Tensor | None = None, bias: Tensor | None = No
 # ------------------------------------------------------------------------ linear
 
 
+@_on_device
 def _linear_run(x, weight, bias, residual, code, save) -> tuple[Tensor, Tensor | None]:
     """(y, p): p, the float32 value before the activation, only when `save`."""
     rows, w = _rows(x), _rows(weight)
     r = None if residual is None else _rows(residual)
     m, n = rows.shape[0], w.shape[0]
-    y = torch.empty((*x.shape[:-1], n), dtype=x.dtype, device=x.device)
-    preact = torch.empty(m, n, dtype=torch.float32, device=x.device) if save else None
+    y = x.new_empty((*x.shape[:-1], n))
+    preact = x.new_empty((m, n), dtype=torch.float32) if save else None
     dcode = _DTYPES[x.dtype]
     size = _linear_workspace(m, rows.shape[1], n, dcode, code, x.device.index)[0]
-    with _on(x.device):
-        _lib.linear_forward(rows, w, bias, r, y, preact, _scratch(size, x.device), n, dcode, code)
+    _lib.linear_forward(rows, w, bias, r, y, preact, _scratch(size, x), n, dcode, code)
     return y, preact
 
 
+@_on_device
 def _linear_grad_run(x, weight, preact, grad, code, need):
     """(dx, dweight, dbias), None where `need` is false."""
     rows, w, g = _rows(x), _rows(weight), _rows(grad)
     m, k = rows.shape
     n = w.shape[0]
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need[0] else None
-    dw = torch.empty(n, k, dtype=x.dtype, device=x.device) if need[1] else None
-    db = torch.empty(n, dtype=x.dtype, device=x.device) if need[2] else None
+    dx = x.new_empty(x.shape) if need[0] else None
+    dw = x.new_empty((n, k)) if need[1] else None
+    db = x.new_empty(n) if need[2] else None
     dcode = _DTYPES[x.dtype]
     size = _linear_workspace(m, k, n, dcode, code, x.device.index)[1]
-    with _on(x.device):
-        _lib.linear_backward(rows, w, preact, g, dx, dw, db, _scratch(size, x.device), m, k, n,
-                             dcode, code)
+    _lib.linear_backward(rows, w, preact, g, dx, dw, db, _scratch(size, x), m, k, n, dcode, code)
     return dx, dw, db
 
 

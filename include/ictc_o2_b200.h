@@ -59,7 +59,8 @@ ICTC_API int32_t ictc_o2_abi_version(void);
  * TensorProduct staged kernels (stage ring, drain, weight copy), 5-6 radial edge
  * tile, 7-8 shared-weight uvu tile, 9-10 per-row uvu streamed kernel, 11-12
  * per-row uvu quad kernel, 13 the wait probe; 17 is not a wait: a gathered radial
- * call met a node index out of range; 18-21 the linear layer's products.  No counterpart in the reference,
+ * call met a node index out of range; 18-21 the linear layer's products, 22 layer
+ * norm's row ring.  No counterpart in the reference,
  * whose Triton kernels have no waits. */
 ICTC_API int32_t ictc_o2_device_error(int32_t* code);
 
