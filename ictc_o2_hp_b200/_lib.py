@@ -65,7 +65,7 @@ SIGNATURES = {
     "ictc_o2_layer_norm_workspace": (_i32, [_i64, _i64, _i32, _i32, ctypes.POINTER(_size)]),
     "ictc_o2_layer_norm_backward": (_i32, [_vp, _i64] + [_vp] * 4 + [_i64] + [_vp] * 4 +
                                     [_size, _i64, _i64, _i32, _i32, _vp]),
-    "ictc_o2_linear_workspace": (_i32, [_i64, _i64, _i64, _i32, _i32, _i32,
+    "ictc_o2_linear_workspace": (_i32, [_i64, _i64, _i64, _i32, _i32, _i32, _i32,
                                         ctypes.POINTER(_size), ctypes.POINTER(_size)]),
     "ictc_o2_linear_forward": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _size,
                                       _i64, _i64, _i64, _i32, _i32, _vp]),
@@ -303,10 +303,10 @@ def layer_norm_backward(x, weight, mean, rstd, grad, gx, gw, gb, workspace, dtyp
         param_dtype, stream_of(x.device)), "layer_norm_backward")
 
 
-def linear_workspace(rows: int, inner: int, outer: int, dtype: int, activation: int,
+def linear_workspace(rows: int, inner: int, outer: int, dtype: int, activation: int, layout: int,
                      device: int) -> tuple[int, int]:
     fwd, bwd = _size(), _size()
-    check(load().ictc_o2_linear_workspace(rows, inner, outer, dtype, activation, device,
+    check(load().ictc_o2_linear_workspace(rows, inner, outer, dtype, activation, layout, device,
                                           ctypes.byref(fwd), ctypes.byref(bwd)),
           "linear_workspace")
     return int(fwd.value), int(bwd.value)

@@ -100,7 +100,8 @@ int encode_matrix_map(const void* base, bool bf16, int64_t inner, int64_t outer,
                       int box_inner, int box_outer, CUtensorMap* map) {
   PFN_cuTensorMapEncodeTiled_v12000 fn = tensor_map_encoder();
   if (fn == nullptr || inner < 1 || outer < 1 || stride % 16 != 0 || stride >= (1ll << 40) ||
-      inner >= (1ll << 31) || outer >= (1ll << 31))
+      inner >= (1ll << 31) || outer >= (1ll << 31) ||
+      stride < 2 * inner)  // rows that overlap or repeat are left to other kernels
     return -1;
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer)};
   const cuuint64_t strides[1] = {static_cast<cuuint64_t>(stride)};

@@ -99,15 +99,37 @@ __device__ __forceinline__ void finish4(const Epilogue& e, int64_t at, float (&v
   *reinterpret_cast<Pack<T, 4>*>(static_cast<T*>(e.out) + at) = o;
 }
 
+// The residual's part of a 32 x 32 block: rows lane / 8 + 4 i, four columns each.  Loaded
+// well before write_block needs it (ahead of the wait for the accumulators): its latency,
+// exposed, had been half of the epilogue of a tile with little K.
+template <typename T>
+struct ResidualBlock {
+  Pack<T, 4> v[8];
+};
+
+template <typename T>
+__device__ __forceinline__ void load_residual(const ProductArgs& p, int64_t row0, int64_t col0,
+                                              int lane, ResidualBlock<T>& res) {
+  const Epilogue& e = p.e;
+  if (!e.residual || !e.vec || e.partial) return;
+  const int64_t col = col0 + (lane & 7) * 4;
+  if (col >= p.n) return;
+  const T* at = static_cast<const T*>(e.residual) + (row0 + (lane >> 3)) * e.residual_stride + col;
+  const int64_t left = p.m - row0 - (lane >> 3);
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (4 * i < left)
+      res.v[i] = *reinterpret_cast<const Pack<T, 4>*>(at + 4 * i * e.residual_stride);
+}
+
 // One 32 x 32 block of an output tile, row-per-lane in `acc`, to memory: through the
 // warp's 4 KB of shared memory (16-byte chunks XOR-swizzled by row), so that lanes of
 // one row touch consecutive columns: eight lanes four columns each when the rows are
-// aligned for that, 32 lanes one column each otherwise.  The residual's loads go out
-// ahead of the stores, which could alias them.  Loops are unrolled by four and no more:
-// the code of an activation is long, and instruction fetches had been the longest stall.
+// aligned for that, 32 lanes one column each otherwise.
 template <typename T, int ACT>
 __device__ __forceinline__ void write_block(const ProductArgs& p, int split, const float* acc,
-                                            float4* mine, int64_t row0, int64_t col0, int lane) {
+                                            float4* mine, int64_t row0, int64_t col0, int lane,
+                                            const ResidualBlock<T>& res) {
   const Epilogue& e = p.e;
   const int64_t col = col0 + (e.vec ? (lane & 7) * 4 : lane);
   const int rows = p.m - row0 < 32 ? static_cast<int>(p.m - row0) : 32;  // <= 0: none
@@ -132,22 +154,15 @@ __device__ __forceinline__ void write_block(const ProductArgs& p, int split, con
     } else if (e.vec) {
       float bias[4];
       load_bias4<T>(e, col, p.n, bias);
-#pragma unroll 1
-      for (int r0 = lane >> 3; r0 < rows; r0 += 16) {
-        Pack<T, 4> res[4];
+      const int64_t at = (row0 + (lane >> 3)) * p.n + col;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          res[i] = Pack<T, 4>{};
-          if (e.residual && r0 + 4 * i < rows) res[i] = residual4<T>(e, row0 + r0 + 4 * i, col);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = r0 + 4 * i;
-          if (r < rows) {
-            const float4 f = mine[r * 8 + ((lane & 7) ^ (r & 7))];
-            float v[4] = {f.x, f.y, f.z, f.w};
-            finish4<T, ACT>(e, (row0 + r) * p.n + col, v, bias, res[i]);
-          }
+      for (int i = 0; i < 8; ++i) {
+        const int r = (lane >> 3) + 4 * i;
+        if (r < rows) {
+          const float4 f = mine[r * 8 + ((lane & 7) ^ (r & 7))];
+          float v[4] = {f.x, f.y, f.z, f.w};
+          Pack<T, 4> z{};
+          finish4<T, ACT>(e, at + 4 * i * p.n, v, bias, e.residual ? res.v[i] : z);
         }
       }
     } else {

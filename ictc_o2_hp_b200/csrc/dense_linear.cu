@@ -20,6 +20,7 @@
 
 #include "common.cuh"
 #include "dense_epilogue.cuh"
+#include "dense_narrow.cuh"
 #include "dense_pair.cuh"
 #include "dense_types.cuh"
 #include "tcgen05.cuh"
@@ -250,7 +251,7 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
       load_operand<T, B_MN, BN>(b, p.ldb, pos.n0, p.n, static_cast<int64_t>(c) * kBK, p.k,
                                 p.vec_b, tid, hb);
       const int s = it % S;
-      ok = mbar_wait(&empty[s], ((it / S) & 1) ^ 1, kCodeProducer);
+      ok = mbar_wait_warp(&empty[s], ((it / S) & 1) ^ 1, kCodeProducer);
       if (!ok) break;
       unsigned char* stage = smem + s * kStageBytes<T, BN>;
       store_operand<T, A_MN, kBM>(stage, tid, ha);
@@ -310,10 +311,13 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
     uint32_t set = 0;
     for (int64_t t = blockIdx.x; ok && t < total; t += gridDim.x) {
       const TilePos pos = tile_at<kBM>(p, t, BN);
+      const int64_t row0 = pos.m0 + quad * 32;
+      ResidualBlock<T> res;
+      load_residual(p, row0, pos.n0 + half * kHalf, lane, res);
       float acc[kHalf];
       const int groups = P == 3 ? (pos.c1 - pos.c0 + kGroupChunks - 1) / kGroupChunks : 1;
       for (int gi = 0; gi < groups; ++gi, ++set) {
-        ok = mbar_wait(&done[set & 1], (set >> 1) & 1, kCodeEpilogue);
+        ok = mbar_wait_warp(&done[set & 1], (set >> 1) & 1, kCodeEpilogue);
         if (!ok) break;
         tcgen05_fence_after();
         const uint32_t at =
@@ -339,8 +343,9 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
       if (!ok) break;
 #pragma unroll
       for (int cb = 0; cb < kHalf / 32; ++cb) {
-        const int64_t row0 = pos.m0 + quad * 32, col0 = pos.n0 + half * kHalf + cb * 32;
-        write_block<T, ACT>(p, pos.split, acc + cb * 32, mine, row0, col0, lane);
+        const int64_t col0 = pos.n0 + half * kHalf + cb * 32;
+        write_block<T, ACT>(p, pos.split, acc + cb * 32, mine, row0, col0, lane, res);
+        if (cb + 1 < kHalf / 32) load_residual(p, row0, col0 + 32, lane, res);
         if constexpr (P == 3) {
           float zero = 0.f;  // stays 0 unless an element is not finite
 #pragma unroll
@@ -467,8 +472,9 @@ __global__ void __launch_bounds__(kRowThreads) few_rows_kernel(
 template <typename T, int V, int ACT>
 __global__ void __launch_bounds__(256) slope_kernel(const T* __restrict__ g, int64_t ldg,
                                                     const float* __restrict__ preact,
-                                                    T* __restrict__ d, float* __restrict__ partial,
-                                                    int64_t m, int64_t n, int lanes) {
+                                                    T* __restrict__ d, int64_t ldd,
+                                                    float* __restrict__ partial, int64_t m,
+                                                    int64_t n, int lanes) {
   __shared__ float sums[256 * V];
   const int tx = threadIdx.x % lanes, ty = threadIdx.x / lanes, rows = 256 / lanes;
   const int64_t col = (static_cast<int64_t>(blockIdx.x) * lanes + tx) * V;
@@ -504,7 +510,7 @@ __global__ void __launch_bounds__(256) slope_kernel(const T* __restrict__ g, int
           acc[j] += v;
           o.v[j] = from_float<T>(v);
         }
-        if constexpr (ACT != ICTC_ACT_NONE) *reinterpret_cast<Pack<T, V>*>(d + r * n + col) = o;
+        if constexpr (ACT != ICTC_ACT_NONE) *reinterpret_cast<Pack<T, V>*>(d + r * ldd + col) = o;
       }
     }
   }
@@ -663,14 +669,19 @@ int launch_product(const ProductArgs& p, int device, cudaStream_t stream) {
   return e == cudaSuccess ? ICTC_OK : cuda_fail(e, "linear product launch");
 }
 
+template <typename T>
+bool vec_epilogue(const Epilogue& e, int64_t n) {
+  return n % 4 == 0 && aligned(e.out, 4 * sizeof(T)) &&
+         (!e.residual || (aligned(e.residual, 4 * sizeof(T)) && e.residual_stride % 4 == 0)) &&
+         aligned(e.preact, 16);
+}
+
 // C = epilogue(A B^T); `partial` holds split_bytes() when the plan splits K.
 template <typename T, bool A_MN, bool B_MN>
 int run_product(const T* a, int64_t lda, const T* b, int64_t ldb, int64_t m, int64_t n, int64_t k,
                 Epilogue e, float* partial, cudaStream_t stream) {
   const int device = current_device();
-  e.vec = n % 4 == 0 && aligned(e.out, 4 * sizeof(T)) &&
-          (!e.residual || (aligned(e.residual, 4 * sizeof(T)) && e.residual_stride % 4 == 0)) &&
-          aligned(e.preact, 16) && aligned(partial, 16);
+  e.vec = vec_epilogue<T>(e, n);
   const auto join = [&](int splits) {
     const int64_t blocks = ceil_div(m * ceil_div(n, 4), 256);
     const int64_t cap = static_cast<int64_t>(sm_count(device)) * 8;
@@ -738,26 +749,199 @@ int launch_few_rows(const T* x, int64_t ldx, const T* w, int64_t ldw, int64_t ro
 
 constexpr int64_t kFewRows = 4;
 
+// ------------------------------------------------------------- rows off the boundaries
+// dst[r, :] = src[r, :] with a pitch of whole 16-byte blocks.
+template <typename T>
+__global__ void __launch_bounds__(256) align_rows_kernel(const T* __restrict__ src, int64_t ld,
+                                                         T* __restrict__ dst, int64_t pitch,
+                                                         int64_t rows, int64_t width) {
+  constexpr int V = 16 / sizeof(T);
+  const int64_t blocks = pitch / V;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * 256;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < rows * blocks;
+       i += step) {
+    const int64_t r = i / blocks, c = (i - r * blocks) * V;
+    Pack<T, V> pk;
+#pragma unroll
+    for (int j = 0; j < V; ++j) pk.v[j] = c + j < width ? src[r * ld + c + j] : T{};
+    *reinterpret_cast<Pack<T, V>*>(dst + r * pitch + c) = pk;
+  }
+}
+
+int64_t aligned_pitch(int64_t width, size_t size) {
+  const int64_t v = static_cast<int64_t>(16 / size);
+  return ceil_div(width, v) * v;
+}
+
+// Element-by-element loads of unaligned rows cost the products several times their time;
+// copying the operand first costs one pass over it and a launch.
+bool worth_aligning(int64_t m, int64_t n, int64_t k) {
+  return static_cast<double>(m) * n * k >= static_cast<double>(1 << 26);
+}
+
+// An operand with aligned rows: itself, or its copy in `space`.
+template <typename T>
+int align_operand(const T** p, int64_t* ld, int64_t rows, int64_t width, unsigned char* space,
+                  cudaStream_t stream) {
+  if (chunk_aligned(*p, *ld, sizeof(T))) return ICTC_OK;
+  const int64_t pitch = aligned_pitch(width, sizeof(T));
+  T* to = reinterpret_cast<T*>(space);
+  const int64_t blocks = ceil_div(rows * pitch * static_cast<int64_t>(sizeof(T)), 256 * 16);
+  const int64_t cap = static_cast<int64_t>(sm_count(current_device())) * 8;
+  align_rows_kernel<T><<<static_cast<unsigned>(blocks < cap ? blocks : cap), 256, 0, stream>>>(
+      *p, *ld, to, pitch, rows, width);
+  *p = to;
+  *ld = pitch;
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? ICTC_OK : cuda_fail(e, "linear operand copy launch");
+}
+
+// ------------------------------------------------------------------- plan of a call
+
+// What a call's pointers and strides allow (ICTC_LINEAR_ALIGNED, ICTC_LINEAR_PACKED).
+int32_t layout_of(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* g,
+                  int64_t ldg, const void* preact, int64_t m, int64_t n, int64_t k, size_t size) {
+  int32_t flags = 0;
+  if (chunk_aligned(x, ldx, size) && chunk_aligned(w, ldw, size) &&
+      (!g || chunk_aligned(g, ldg, size)))
+    flags |= ICTC_LINEAR_ALIGNED;
+  if (aligned(x, 16) && (ldx == k || m <= 1) &&
+      (!g || (aligned(g, 16) && (ldg == n || m <= 1) && aligned(preact, 16))))
+    flags |= ICTC_LINEAR_PACKED;
+  return flags;
+}
+
+// Byte offsets of the workspace's parts, and its size.
+struct LinearPlan {
+  bool few, narrow, align;
+  size_t d, x, w, g, columns, partial, total;
+};
+
+constexpr int64_t kSlopeParts = 296;
+
+LinearPlan plan_linear(int64_t m, int64_t n, int64_t k, int dtype, int activation, int32_t layout,
+                       bool backward, int device) {
+  LinearPlan b{};
+  const size_t size = dtype_size(dtype);
+  b.few = !backward && m <= kFewRows;
+  b.narrow = !b.few && (layout & ICTC_LINEAR_PACKED) && n <= kNarrow && k <= kNarrow &&
+             m <= (1ll << 36);
+  b.align = !(layout & ICTC_LINEAR_ALIGNED) && worth_aligning(m, n, k);
+  size_t at = 0;
+  const auto take = [&](size_t bytes) {
+    const size_t here = at;
+    at += align_up(bytes, 256);
+    return here;
+  };
+  const auto rows = [&](int64_t r, int64_t width) {
+    return static_cast<size_t>(r) * aligned_pitch(width, size) * size;
+  };
+  if (b.few) return b;
+  if (b.narrow) {
+    if (backward)
+      b.partial = take(static_cast<size_t>(sm_count(device)) * (n * k + n) * sizeof(float));
+    b.total = at;
+    return b;
+  }
+  const bool slope = backward && activation != ICTC_ACT_NONE;
+  if (slope) b.d = take(rows(m, n));
+  if (b.align) {
+    b.x = take(rows(m, k));
+    b.w = take(rows(n, k));
+    if (backward && !slope) b.g = take(rows(m, n));
+  }
+  if (backward) {
+    b.columns = take(static_cast<size_t>(m < kSlopeParts ? m : kSlopeParts) * n * sizeof(float));
+    const size_t one = split_bytes(m, k, n, dtype, device);
+    const size_t other = split_bytes(n, k, m, dtype, device);
+    b.partial = take(one > other ? one : other);
+  } else {
+    b.partial = take(split_bytes(m, n, k, dtype, device));
+  }
+  b.total = at;
+  return b;
+}
+
+template <typename T>
+int run_narrow_forward(const T* x, const T* w, int64_t ldw, Epilogue e, int64_t m, int64_t n,
+                       int64_t k, cudaStream_t stream) {
+  NarrowArgs p{};
+  p.x = x; p.w = w;
+  p.m = m; p.ldw = ldw;
+  p.n = static_cast<int>(n); p.k = static_cast<int>(k);
+  p.tiles = static_cast<int>(ceil_div(m, kNarrowTile));
+  e.vec = vec_epilogue<T>(e, n);
+  p.e = e;
+  const int sms = sm_count(current_device());
+  const int grid = p.tiles < sms ? p.tiles : sms;
+  int st = ICTC_OK;
+  for_activation(e.activation, [&](auto act) {
+    const auto kernel = narrow_forward_kernel<T, act.value>;
+    st = allow_smem(reinterpret_cast<const void*>(kernel), kNarrowForwardSmem<T>);
+    if (st == ICTC_OK) kernel<<<grid, kNarrowThreadsL, kNarrowForwardSmem<T>, stream>>>(p);
+  });
+  if (st != ICTC_OK) return st;
+  const cudaError_t err = cudaGetLastError();
+  return err == cudaSuccess ? ICTC_OK : cuda_fail(err, "narrow linear forward launch");
+}
+
+template <typename T>
+int run_narrow_backward(const T* x, const T* w, int64_t ldw, const float* preact, const T* g,
+                        T* dx, T* dw, T* db, float* partial, int64_t m, int64_t n, int64_t k,
+                        int activation, cudaStream_t stream) {
+  NarrowArgs p{};
+  p.x = x; p.w = w; p.g = g; p.preact = preact;
+  p.m = m; p.ldw = ldw;
+  p.n = static_cast<int>(n); p.k = static_cast<int>(k);
+  p.tiles = static_cast<int>(ceil_div(m, kNarrowTile));
+  p.partial = dw || db ? partial : nullptr;
+  p.e.out = dx;
+  p.e.vec = vec_epilogue<T>(p.e, k);
+  const int sms = sm_count(current_device());
+  const int grid = p.tiles < sms ? p.tiles : sms;
+  int st = ICTC_OK;
+  for_activation(activation, [&](auto act) {
+    const auto kernel = narrow_backward_kernel<T, act.value>;
+    st = allow_smem(reinterpret_cast<const void*>(kernel), kNarrowBackwardSmem<T>);
+    if (st == ICTC_OK) kernel<<<grid, kNarrowThreadsL, kNarrowBackwardSmem<T>, stream>>>(p);
+  });
+  if (st != ICTC_OK) return st;
+  cudaError_t err = cudaGetLastError();
+  if (err != cudaSuccess) return cuda_fail(err, "narrow linear backward launch");
+  if (!p.partial) return ICTC_OK;
+  const int nk = p.n * p.k;
+  narrow_total_kernel<T><<<static_cast<unsigned>(ceil_div(nk + p.n, 32)), dim3(32, kColumnLanes),
+                           0, stream>>>(partial, dw, db, grid, nk, p.n);
+  err = cudaGetLastError();
+  return err == cudaSuccess ? ICTC_OK : cuda_fail(err, "narrow linear column sum launch");
+}
+
 template <typename T>
 int run_linear_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, Epilogue e,
-                       float* partial, int64_t m, int64_t n, int64_t k, cudaStream_t stream) {
+                       unsigned char* workspace, const LinearPlan& plan, int64_t m, int64_t n,
+                       int64_t k, cudaStream_t stream) {
   const T* xt = static_cast<const T*>(x);
   const T* wt = static_cast<const T*>(w);
-  if (m <= kFewRows) {
+  if (plan.few) {
     constexpr int kFull = 16 / sizeof(T);
     if (k % kFull == 0 && chunk_aligned(x, ldx, sizeof(T)) && chunk_aligned(w, ldw, sizeof(T)))
       return launch_few_rows<T, kFull>(xt, ldx, wt, ldw, m, n, k, e, stream);
     return launch_few_rows<T, 1>(xt, ldx, wt, ldw, m, n, k, e, stream);
   }
-  return run_product<T, false, false>(xt, ldx, wt, ldw, m, n, k, e, partial, stream);
+  if (plan.narrow) return run_narrow_forward<T>(xt, wt, ldw, e, m, n, k, stream);
+  if (plan.align) {
+    int st = align_operand(&xt, &ldx, m, k, workspace + plan.x, stream);
+    if (st == ICTC_OK) st = align_operand(&wt, &ldw, n, k, workspace + plan.w, stream);
+    if (st != ICTC_OK) return st;
+  }
+  return run_product<T, false, false>(xt, ldx, wt, ldw, m, n, k, e,
+                                      reinterpret_cast<float*>(workspace + plan.partial), stream);
 }
 
 struct SlopePlan {
   int vec, lanes;
   unsigned blocks_x, blocks_y;
 };
-
-constexpr int64_t kSlopeParts = 296;
 
 SlopePlan plan_slope(int64_t m, int64_t n, int vec) {
   SlopePlan s{};
@@ -775,33 +959,23 @@ SlopePlan plan_slope(int64_t m, int64_t n, int vec) {
   return s;
 }
 
-struct BackwardPlan {
-  size_t d, columns, partial, total;  // byte offsets of the workspace's parts and its size
-};
-
-BackwardPlan plan_backward(int64_t m, int64_t n, int64_t k, int dtype, bool slope, int device) {
-  BackwardPlan b{};
-  const size_t d_bytes = slope ? align_up(static_cast<size_t>(m) * n * dtype_size(dtype), 256) : 0;
-  b.d = 0;
-  b.columns = d_bytes;
-  const int64_t parts = m < kSlopeParts ? m : kSlopeParts;
-  b.partial = b.columns + align_up(static_cast<size_t>(parts) * n * sizeof(float), 256);
-  size_t split = split_bytes(m, k, n, dtype, device);
-  const size_t other = split_bytes(n, k, m, dtype, device);
-  if (other > split) split = other;
-  b.total = b.partial + align_up(split, 256);
-  return b;
-}
-
 template <typename T>
 int run_linear_backward(const void* x, int64_t ldx, const void* w, int64_t ldw,
                         const float* preact, const void* g, int64_t ldg, void* dx, void* dw,
-                        void* db, unsigned char* workspace, const BackwardPlan& plan, int64_t m,
+                        void* db, unsigned char* workspace, const LinearPlan& plan, int64_t m,
                         int64_t n, int64_t k, int activation, cudaStream_t stream) {
+  const T* xt = static_cast<const T*>(x);
+  const T* wt = static_cast<const T*>(w);
   const T* d = static_cast<const T*>(g);
+  float* partial = reinterpret_cast<float*>(workspace + plan.partial);
+  if (plan.narrow)
+    return run_narrow_backward<T>(xt, wt, ldw, preact, d, static_cast<T*>(dx),
+                                  static_cast<T*>(dw), static_cast<T*>(db), partial, m, n, k,
+                                  activation, stream);
   int64_t ldd = ldg;
   const bool slope = activation != ICTC_ACT_NONE;
   T* d_out = slope ? reinterpret_cast<T*>(workspace + plan.d) : nullptr;
+  const int64_t d_pitch = aligned_pitch(n, sizeof(T));
   float* columns = db ? reinterpret_cast<float*>(workspace + plan.columns) : nullptr;
   if (slope || db) {
     constexpr int kFull = 16 / sizeof(T);
@@ -810,11 +984,11 @@ int run_linear_backward(const void* x, int64_t ldx, const void* w, int64_t ldw,
     const dim3 grid(s.blocks_x, s.blocks_y);
     for_activation(activation, [&](auto act) {
       if (vec)
-        slope_kernel<T, kFull, act.value>
-            <<<grid, 256, 0, stream>>>(d, ldg, preact, d_out, columns, m, n, s.lanes);
+        slope_kernel<T, kFull, act.value><<<grid, 256, 0, stream>>>(d, ldg, preact, d_out, d_pitch,
+                                                                    columns, m, n, s.lanes);
       else
-        slope_kernel<T, 1, act.value>
-            <<<grid, 256, 0, stream>>>(d, ldg, preact, d_out, columns, m, n, s.lanes);
+        slope_kernel<T, 1, act.value><<<grid, 256, 0, stream>>>(d, ldg, preact, d_out, d_pitch,
+                                                                columns, m, n, s.lanes);
     });
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return cuda_fail(e, "linear slope launch");
@@ -827,21 +1001,26 @@ int run_linear_backward(const void* x, int64_t ldx, const void* w, int64_t ldw,
     }
     if (slope) {
       d = d_out;
-      ldd = n;
+      ldd = d_pitch;
     }
   }
-  float* partial = reinterpret_cast<float*>(workspace + plan.partial);
+  if (plan.align) {
+    int st = ICTC_OK;
+    if (!slope && (dx || dw)) st = align_operand(&d, &ldd, m, n, workspace + plan.g, stream);
+    if (st == ICTC_OK && dx) st = align_operand(&wt, &ldw, n, k, workspace + plan.w, stream);
+    if (st == ICTC_OK && dw) st = align_operand(&xt, &ldx, m, k, workspace + plan.x, stream);
+    if (st != ICTC_OK) return st;
+  }
   Epilogue e{};
   if (dx) {
     e.out = dx;
-    const int st = run_product<T, false, true>(d, ldd, static_cast<const T*>(w), ldw, m, k, n, e,
-                                               partial, stream);
+    const int st =
+        run_product<T, false, true>(d, ldd, wt, ldw, m, k, n, e, partial, stream);
     if (st != ICTC_OK) return st;
   }
   if (dw) {
     e.out = dw;
-    return run_product<T, true, true>(d, ldd, static_cast<const T*>(x), ldx, n, k, m, e, partial,
-                                      stream);
+    return run_product<T, true, true>(d, ldd, xt, ldx, n, k, m, e, partial, stream);
   }
   return ICTC_OK;
 }
@@ -870,16 +1049,17 @@ int dense_take_device_error(int* code) {
 using namespace ictc;
 
 extern "C" int32_t ictc_o2_linear_workspace(int64_t rows, int64_t in, int64_t out, int32_t dtype,
-                                            int32_t activation, int32_t device,
+                                            int32_t activation, int32_t layout, int32_t device,
                                             size_t* forward_bytes, size_t* backward_bytes) {
   const int st = check_linear(rows, out, in, dtype, activation);
   if (st != ICTC_OK) return st;
   if (!forward_bytes || !backward_bytes) return fail(ICTC_ERR_INVALID, "null output");
+  *forward_bytes = *backward_bytes = 0;
+  if (rows == 0) return ICTC_OK;
   *forward_bytes =
-      rows <= kFewRows ? 0 : split_bytes(rows, out, in, dtype, device);
+      plan_linear(rows, out, in, dtype, activation, layout, false, device).total;
   *backward_bytes =
-      rows == 0 ? 0
-                : plan_backward(rows, out, in, dtype, activation != ICTC_ACT_NONE, device).total;
+      plan_linear(rows, out, in, dtype, activation, layout, true, device).total;
   return ICTC_OK;
 }
 
@@ -895,11 +1075,14 @@ extern "C" int32_t ictc_o2_linear_forward(const void* x, int64_t x_stride, const
   if (!x || !weight || !y) return fail(ICTC_ERR_INVALID, "null pointer");
   if (x_stride < 0 || weight_stride < 0 || residual_stride < 0)
     return fail(ICTC_ERR_INVALID, "negative row stride");
-  const size_t need = rows <= kFewRows
-                          ? 0 : split_bytes(rows, out, in, dtype, current_device());
-  if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
-    return fail(ICTC_ERR_WORKSPACE, "workspace has %zu bytes, needs %zu (16-byte aligned)",
-                workspace ? workspace_bytes : 0, need);
+  const int32_t layout = layout_of(x, x_stride, weight, weight_stride, nullptr, 0, nullptr, rows,
+                                   out, in, dtype_size(dtype));
+  const LinearPlan plan =
+      plan_linear(rows, out, in, dtype, activation, layout, false, current_device());
+  if (plan.total > 0 &&
+      (!workspace || workspace_bytes < plan.total || !aligned(workspace, 256)))
+    return fail(ICTC_ERR_WORKSPACE, "workspace has %zu bytes, needs %zu (256-byte aligned)",
+                workspace ? workspace_bytes : 0, plan.total);
   Epilogue e{};
   e.bias = bias;
   e.residual = residual;
@@ -907,16 +1090,14 @@ extern "C" int32_t ictc_o2_linear_forward(const void* x, int64_t x_stride, const
   e.preact = preact;
   e.out = y;
   e.activation = activation;
-  float* partial = static_cast<float*>(workspace);
+  unsigned char* ws = static_cast<unsigned char*>(workspace);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype == ICTC_DTYPE_F32)
-    return run_linear_forward<float>(x, x_stride, weight, weight_stride, e, partial, rows, out, in,
-                                     s);
-  if (dtype == ICTC_DTYPE_BF16)
-    return run_linear_forward<__nv_bfloat16>(x, x_stride, weight, weight_stride, e, partial, rows,
-                                             out, in, s);
-  return run_linear_forward<__half>(x, x_stride, weight, weight_stride, e, partial, rows, out, in,
-                                    s);
+#define ICTC_LINEAR_FORWARD(T) \
+  return run_linear_forward<T>(x, x_stride, weight, weight_stride, e, ws, plan, rows, out, in, s)
+  if (dtype == ICTC_DTYPE_F32) ICTC_LINEAR_FORWARD(float);
+  if (dtype == ICTC_DTYPE_BF16) ICTC_LINEAR_FORWARD(__nv_bfloat16);
+  ICTC_LINEAR_FORWARD(__half);
+#undef ICTC_LINEAR_FORWARD
 }
 
 extern "C" int32_t ictc_o2_linear_backward(
@@ -936,14 +1117,17 @@ extern "C" int32_t ictc_o2_linear_backward(
     return e == cudaSuccess ? ICTC_OK : cuda_fail(e, "linear gradient clear");
   }
   if (!grad_x && !grad_weight && !grad_bias) return ICTC_OK;
-  if (!grad_output || (grad_x && !weight) || (grad_weight && !x) ||
-      (activation != ICTC_ACT_NONE && !preact))
+  if (!x || !weight || !grad_output || (activation != ICTC_ACT_NONE && !preact))
     return fail(ICTC_ERR_INVALID, "null pointer");
   if (x_stride < 0 || weight_stride < 0 || grad_stride < 0)
     return fail(ICTC_ERR_INVALID, "negative row stride");
-  const BackwardPlan plan = plan_backward(rows, out, in, dtype, activation != ICTC_ACT_NONE,
-                                          current_device());
-  if (!workspace || workspace_bytes < plan.total || !aligned(workspace, 256))
+  const int32_t layout =
+      layout_of(x, x_stride, weight, weight_stride, grad_output, grad_stride,
+                activation == ICTC_ACT_NONE ? nullptr : preact, rows, out, in, dtype_size(dtype));
+  const LinearPlan plan =
+      plan_linear(rows, out, in, dtype, activation, layout, true, current_device());
+  if (plan.total > 0 &&
+      (!workspace || workspace_bytes < plan.total || !aligned(workspace, 256)))
     return fail(ICTC_ERR_WORKSPACE, "workspace has %zu bytes, needs %zu (256-byte aligned)",
                 workspace ? workspace_bytes : 0, plan.total);
   unsigned char* ws = static_cast<unsigned char*>(workspace);

@@ -233,12 +233,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     uint32_t set = 0;
     for (int64_t t = first; t < total; t += step, ++set) {
       const TilePos pos = tile_at<kPairRows>(p, t, BN);
-      ok = mbar_wait(&done[set & 1], (set >> 1) & 1, kCodeEpilogue);
+      const int64_t row0 = pos.m0 + rank * 128 + quad * 32, col0 = pos.n0 + half * kHalf;
+      ResidualBlock<T> res, next;
+      load_residual(p, row0, col0, lane, next);
+      ok = mbar_wait_warp(&done[set & 1], (set >> 1) & 1, kCodeEpilogue);
       if (!ok) break;
       tcgen05_fence_after();
       const uint32_t at =
           tmem + (set & 1) * BN + (static_cast<uint32_t>(quad * 32) << 16) + half * kHalf;
-      const int64_t row0 = pos.m0 + rank * 128 + quad * 32;
 #pragma unroll 1
       for (int cb = 0; cb < kHalf / 32; ++cb) {
         float acc[32];
@@ -246,13 +248,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         float(&hi)[16] = *reinterpret_cast<float(*)[16]>(acc + 16);
         tmem_load16(at + cb * 32, lo);
         tmem_load16(at + cb * 32 + 16, hi);
+        res = next;
+        const bool last = cb == kHalf / 32 - 1;
+        if (!last) load_residual(p, row0, col0 + (cb + 1) * 32, lane, next);
         tmem_load_wait();
-        if (cb == kHalf / 32 - 1) {  // the set's last columns are in registers
+        if (last) {  // the set's last columns are in registers
           tcgen05_fence_before();
           __syncwarp();
           if (lane == 0) arrive_cluster(peer_addr(&room[set & 1], 0));
         }
-        write_block<T, ACT>(p, pos.split, acc, mine, row0, pos.n0 + half * kHalf + cb * 32, lane);
+        write_block<T, ACT>(p, pos.split, acc, mine, row0, col0 + cb * 32, lane, res);
       }
     }
   }

@@ -99,6 +99,11 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int co
   return false;
 }
 
+// The same for a converged warp: one answer for all its lanes.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, int code) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, code)) != 0;
+}
+
 // Global -> shared bulk copy completing on `bar` (bytes counted by expect_tx).
 __device__ __forceinline__ void bulk_g2s(void* dst, const void* src, uint32_t bytes,
                                          uint64_t* bar) {

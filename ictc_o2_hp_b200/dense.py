@@ -219,6 +219,23 @@ def layer_norm(x: Tensor, weight: Tensor | None = None, bias: Tensor | None = No
 # ------------------------------------------------------------------------ linear
 
 
+_ALIGNED, _PACKED = 1, 2  # layout flags of the C ABI
+
+
+def _layout(x, w, g=None) -> int:
+    """What the operands' row starts allow (all [rows, width], unit stride in a row)."""
+    block = 16 // x.element_size()
+    packed = aligned = True
+    for t in (x, g):
+        if t is not None:
+            start = t.data_ptr() % 16 == 0
+            rows = t.stride(0)
+            packed = packed and start and (rows == t.shape[1] or t.shape[0] <= 1)
+            aligned = aligned and start and rows % block == 0
+    aligned = aligned and w.data_ptr() % 16 == 0 and w.stride(0) % block == 0
+    return (_ALIGNED if aligned else 0) | (_PACKED if packed else 0)
+
+
 @_on_device
 def _linear_run(x, weight, bias, residual, code, save) -> tuple[Tensor, Tensor | None]:
     """(y, p): p, the float32 value before the activation, only when `save`."""
@@ -228,7 +245,8 @@ def _linear_run(x, weight, bias, residual, code, save) -> tuple[Tensor, Tensor |
     y = x.new_empty((*x.shape[:-1], n))
     preact = x.new_empty((m, n), dtype=torch.float32) if save else None
     dcode = _DTYPES[x.dtype]
-    size = _linear_workspace(m, rows.shape[1], n, dcode, code, x.device.index)[0]
+    size = _linear_workspace(m, rows.shape[1], n, dcode, code, _layout(rows, w),
+                             x.device.index)[0]
     _lib.linear_forward(rows, w, bias, r, y, preact, _scratch(size, x), n, dcode, code)
     return y, preact
 
@@ -243,7 +261,7 @@ def _linear_grad_run(x, weight, preact, grad, code, need):
     dw = x.new_empty((n, k)) if need[1] else None
     db = x.new_empty(n) if need[2] else None
     dcode = _DTYPES[x.dtype]
-    size = _linear_workspace(m, k, n, dcode, code, x.device.index)[1]
+    size = _linear_workspace(m, k, n, dcode, code, _layout(rows, w, g), x.device.index)[1]
     _lib.linear_backward(rows, w, preact, g, dx, dw, db, _scratch(size, x), m, k, n, dcode, code)
     return dx, dw, db
 

@@ -334,9 +334,17 @@ ICTC_API int32_t ictc_o2_layer_norm_backward(
     void* grad_bias, void* workspace, size_t workspace_bytes, int64_t rows, int64_t width,
     int32_t dtype, int32_t param_dtype, void* stream);
 
-/* Workspace of the linear layer's two directions (256-byte aligned). */
+/* What the operands of a call allow: ICTC_LINEAR_ALIGNED, every row of x, weight and (in
+ * the backward) grad_output starts on a 16-byte boundary; ICTC_LINEAR_PACKED, x and
+ * grad_output are contiguous and they and preact start on one.  Faster kernels need
+ * them; a workspace sized for fewer of them than hold is not smaller than needed, except
+ * that PACKED calls of at most 64 inputs and outputs take a kernel with its own. */
+enum { ICTC_LINEAR_ALIGNED = 1, ICTC_LINEAR_PACKED = 2 };
+
+/* Workspace of the linear layer's two directions (256-byte aligned) for operands of the
+ * given layout flags. */
 ICTC_API int32_t ictc_o2_linear_workspace(int64_t rows, int64_t in, int64_t out, int32_t dtype,
-                                          int32_t activation, int32_t device,
+                                          int32_t activation, int32_t layout, int32_t device,
                                           size_t* forward_bytes, size_t* backward_bytes);
 
 /* p = x weight^T + bias, y = act(p) + residual: x [rows, in], weight [out, in], bias

@@ -85,8 +85,8 @@ def test_linear_status_codes():
                 {"x": None}, {"w": None}, {"y": None}, {"stride": -1}):
         assert forward(**bad) == _lib.ERR_INVALID, bad
     ws = lib.ictc_o2_linear_workspace
-    assert ws(8, 16, 8, 0, 0, 0, ctypes.byref(fwd), None) == _lib.ERR_INVALID
-    assert ws(8, 16, 8, 0, 2, 0, ctypes.byref(fwd), ctypes.byref(bwd)) == _lib.OK
+    assert ws(8, 16, 8, 0, 0, 3, 0, ctypes.byref(fwd), None) == _lib.ERR_INVALID
+    assert ws(8, 16, 8, 0, 2, 3, 0, ctypes.byref(fwd), ctypes.byref(bwd)) == _lib.OK
     assert fwd.value == 0 and bwd.value > 0
 
     def backward(preact=some, g=some, x=some, w=some, dw=some, space=some, size=1 << 30, act=2,

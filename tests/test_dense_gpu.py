@@ -110,7 +110,8 @@ def check_linear(x, w, b, r, act, g, y, grads, dtype):
 LINEAR_SHAPES = [
     (1, 1, 1), (1, 64, 64), (3, 7, 5), (4, 129, 1), (5, 8, 64), (37, 8, 64), (127, 63, 65),
     (128, 64, 128), (129, 65, 127), (200, 257, 3), (255, 16, 130), (300, 1000, 72), (64, 2049, 33),
-    (1000, 33, 200), (2500, 64, 64),
+    (1000, 33, 200), (2500, 64, 64), (5000, 7, 3), (3000, 64, 1), (129, 1, 64), (513, 61, 59),
+    (6, 16, 16), (700, 1025, 769), (2053, 211, 333),
 ]
 
 
@@ -233,6 +234,34 @@ def test_linear_nonfinite(rows, dtype, cuda_device):
     base = dense.linear(x, w)
     keep = want.isfinite()
     assert torch.equal(y[keep], base[keep]) and clean.isfinite().all()
+
+
+@pytest.mark.parametrize("shape", [(700, 48, 40), (700, 48, 140)])
+def test_linear_nonfinite_gradients(shape, cuda_device):
+    """Infinities and NaN in the gradient and in x reach the sums they belong to."""
+    from ictc_o2_hp_b200 import dense
+    m, k, n = shape
+    x = rand((m, k), torch.float32, cuda_device, 55)
+    w = rand((n, k), torch.float32, cuda_device, 56)
+    g = rand((m, n), torch.float32, cuda_device, 57)
+
+    def grads(x, w, g):
+        leaves = [t.clone().requires_grad_(True) for t in (x, w)]
+        return torch.autograd.grad(dense.linear(*leaves), leaves, g)
+
+    base = grads(x, w, g)
+    x2, w2, g2 = x.clone(), w.clone(), g.clone()
+    x2[300, 5] = math.inf
+    g2[20, 7] = -math.inf
+    g2[650, 30] = math.nan
+    w2[3, 9] = math.inf
+    got = grads(x2, w2, g2)
+    want = (g2.double() @ w2.double(), g2.double().t() @ x2.double())
+    for p, q, r in zip(got, want, base):
+        assert torch.equal(p.isnan(), q.isnan()) and torch.equal(p.isinf(), q.isinf())
+        assert torch.equal(p[p.isinf()].double(), q[q.isinf()])
+        keep = q.isfinite()
+        assert keep.any() and torch.equal(p[keep], r[keep])
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
