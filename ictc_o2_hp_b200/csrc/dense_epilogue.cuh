@@ -79,7 +79,7 @@ __device__ __forceinline__ void finish1(const Epilogue& e, int64_t row, int64_t 
                                         float v, float bias) {
   v += bias;
   if (e.preact) e.preact[row * n + col] = v;
-  float y = activate<ACT, sizeof(T) == 2>(v, e.activation);
+  float y = activate<ACT>(v, e.activation);
   if (e.residual) y += to_float(static_cast<const T*>(e.residual)[row * e.residual_stride + col]);
   static_cast<T*>(e.out)[row * n + col] = from_float<T>(y);
 }
@@ -95,7 +95,7 @@ __device__ __forceinline__ void finish4(const Epilogue& e, int64_t at, float (&v
   Pack<T, 4> o;
 #pragma unroll
   for (int j = 0; j < 4; ++j)
-    o.v[j] = from_float<T>(activate<ACT, sizeof(T) == 2>(v[j], e.activation) + to_float(r.v[j]));
+    o.v[j] = from_float<T>(activate<ACT>(v[j], e.activation) + to_float(r.v[j]));
   *reinterpret_cast<Pack<T, 4>*>(static_cast<T*>(e.out) + at) = o;
 }
 
@@ -126,18 +126,21 @@ __device__ __forceinline__ void load_residual(const ProductArgs& p, int64_t row0
 // warp's 4 KB of shared memory (16-byte chunks XOR-swizzled by row), so that lanes of
 // one row touch consecutive columns: eight lanes four columns each when the rows are
 // aligned for that, 32 lanes one column each otherwise.
-template <typename T, int ACT>
-__device__ __forceinline__ void write_block(const ProductArgs& p, int split, const float* acc,
-                                            float4* mine, int64_t row0, int64_t col0, int lane,
-                                            const ResidualBlock<T>& res) {
-  const Epilogue& e = p.e;
-  const int64_t col = col0 + (e.vec ? (lane & 7) * 4 : lane);
-  const int rows = p.m - row0 < 32 ? static_cast<int>(p.m - row0) : 32;  // <= 0: none
+__device__ __forceinline__ void stage_block(const float* acc, float4* mine, int lane) {
 #pragma unroll
   for (int c = 0; c < 8; ++c)
     mine[lane * 8 + (c ^ (lane & 7))] =
         make_float4(acc[4 * c], acc[4 * c + 1], acc[4 * c + 2], acc[4 * c + 3]);
   __syncwarp();
+}
+
+template <typename T, int ACT>
+__device__ __forceinline__ void write_staged(const ProductArgs& p, int split, const float4* mine,
+                                             int64_t row0, int64_t col0, int lane,
+                                             const ResidualBlock<T>& res) {
+  const Epilogue& e = p.e;
+  const int64_t col = col0 + (e.vec ? (lane & 7) * 4 : lane);
+  const int rows = p.m - row0 < 32 ? static_cast<int>(p.m - row0) : 32;  // <= 0: none
   if (col < p.n && rows > 0) {
     if (e.partial) {
       float* out = e.partial + (split * p.m + row0) * p.n + col;
@@ -175,6 +178,14 @@ __device__ __forceinline__ void write_block(const ProductArgs& p, int split, con
     }
   }
   __syncwarp();
+}
+
+template <typename T, int ACT>
+__device__ __forceinline__ void write_block(const ProductArgs& p, int split, const float* acc,
+                                            float4* mine, int64_t row0, int64_t col0, int lane,
+                                            const ResidualBlock<T>& res) {
+  stage_block(acc, mine, lane);
+  write_staged<T, ACT>(p, split, mine, row0, col0, lane, res);
 }
 
 }  // namespace ictc

@@ -112,24 +112,13 @@ __device__ __forceinline__ void store_operand(unsigned char* dst, int tid,
     // MN-major tiles wider than 64 are blocks of [64 k rows][128 bytes]
     const uint32_t at = MN ? (c >> 3) * (kBK * 128) + swizzled(row, c & 7) : swizzled(row, c);
     if constexpr (sizeof(T) == 4) {
-      uint32_t part[3][4];
+      uint32_t part[4][3];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float x0 = h.v[i].v[2 * j], x1 = h.v[i].v[2 * j + 1];
-        const uint32_t u0 = __float_as_uint(x0), u1 = __float_as_uint(x1);
-        part[0][j] = __byte_perm(u0, u1, 0x7632);
-        const float r0 = x0 - __uint_as_float(u0 & 0xffff0000u);
-        const float r1 = x1 - __uint_as_float(u1 & 0xffff0000u);
-        const uint32_t v0 = __float_as_uint(r0), v1 = __float_as_uint(r1);
-        part[1][j] = __byte_perm(v0, v1, 0x7632);
-        const float s0 = r0 - __uint_as_float(v0 & 0xffff0000u);
-        const float s1 = r1 - __uint_as_float(v1 & 0xffff0000u);
-        part[2][j] = __byte_perm(__float_as_uint(s0), __float_as_uint(s1), 0x7632);
-      }
+      for (int j = 0; j < 4; ++j) cut_pair(h.v[i].v[2 * j], h.v[i].v[2 * j + 1], part[j]);
 #pragma unroll
       for (int q = 0; q < 3; ++q)
         *reinterpret_cast<uint4*>(dst + q * ROWS * 128 + at) =
-            make_uint4(part[q][0], part[q][1], part[q][2], part[q][3]);
+            make_uint4(part[0][q], part[1][q], part[2][q], part[3][q]);
     } else {
       *reinterpret_cast<uint4*>(dst + at) = *reinterpret_cast<const uint4*>(&h.v[i]);
     }
@@ -276,8 +265,8 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
       if (warp == kMmaWarp) {
         const bool close = last || (P == 3 && in_group == kGroupChunks - 1);
         if (lane == 0) {
-          if (in_group == 0) ok = mbar_wait(&room[set & 1], ((set >> 1) & 1) ^ 1, kCodeMma);
-          if (ok) ok = mbar_wait(&full[s], (it / S) & 1, kCodeMma);
+          if (in_group == 0) ok = mbar_wait_idle(&room[set & 1], ((set >> 1) & 1) ^ 1, kCodeMma);
+          if (ok) ok = mbar_wait_idle(&full[s], (it / S) & 1, kCodeMma);
           if (ok) {
             tcgen05_fence_after();
             issue_stage<T, A_MN, B_MN, BN>(smem_addr(stage), tmem + (set & 1) * kSet,
@@ -456,7 +445,7 @@ __global__ void __launch_bounds__(kRowThreads) few_rows_kernel(
         if (r >= rows) break;
         const float v = acc[r] + bias;
         if (e.preact) e.preact[r * n + col] = v;
-        float y = activate<kAnyActivation, sizeof(T) == 2>(v, e.activation);
+        float y = activate<kAnyActivation>(v, e.activation);
         if (e.residual)
           y += to_float(static_cast<const T*>(e.residual)[r * e.residual_stride + col]);
         static_cast<T*>(e.out)[r * n + col] = from_float<T>(y);
@@ -506,7 +495,7 @@ __global__ void __launch_bounds__(256) slope_kernel(const T* __restrict__ g, int
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           float v = to_float(pg[q].v[j]);
-          if constexpr (ACT != ICTC_ACT_NONE) v *= activation_slope<ACT, sizeof(T) == 2>(pp[q].v[j]);
+          if constexpr (ACT != ICTC_ACT_NONE) v *= activation_slope<ACT>(pp[q].v[j]);
           acc[j] += v;
           o.v[j] = from_float<T>(v);
         }
@@ -875,8 +864,10 @@ int run_narrow_forward(const T* x, const T* w, int64_t ldw, Epilogue e, int64_t 
   const int sms = sm_count(current_device());
   const int grid = p.tiles < sms ? p.tiles : sms;
   int st = ICTC_OK;
+  const bool plain = k * sizeof(T) % 16 == 0;
   for_activation(e.activation, [&](auto act) {
-    const auto kernel = narrow_forward_kernel<T, act.value>;
+    const auto kernel = plain ? narrow_forward_kernel<T, act.value, true>
+                              : narrow_forward_kernel<T, act.value, false>;
     st = allow_smem(reinterpret_cast<const void*>(kernel), kNarrowForwardSmem<T>);
     if (st == ICTC_OK) kernel<<<grid, kNarrowThreadsL, kNarrowForwardSmem<T>, stream>>>(p);
   });
@@ -900,8 +891,10 @@ int run_narrow_backward(const T* x, const T* w, int64_t ldw, const float* preact
   const int sms = sm_count(current_device());
   const int grid = p.tiles < sms ? p.tiles : sms;
   int st = ICTC_OK;
+  const bool plain = k * sizeof(T) % 16 == 0 && n * sizeof(T) % 16 == 0;
   for_activation(activation, [&](auto act) {
-    const auto kernel = narrow_backward_kernel<T, act.value>;
+    const auto kernel = plain ? narrow_backward_kernel<T, act.value, true>
+                              : narrow_backward_kernel<T, act.value, false>;
     st = allow_smem(reinterpret_cast<const void*>(kernel), kNarrowBackwardSmem<T>);
     if (st == ICTC_OK) kernel<<<grid, kNarrowThreadsL, kNarrowBackwardSmem<T>, stream>>>(p);
   });

@@ -30,8 +30,16 @@ namespace ictc {
 constexpr int kNarrow = 64;          // most inputs and outputs
 constexpr int kNarrowTile = 128;     // rows of a tile
 constexpr int kSliceRows = 32;       // rows of a bulk copy
-constexpr int kNarrowThreadsL = 512; // 8 epilogue and 8 producer warps
-constexpr int kNarrowMmaWarp = 8, kNarrowCopyWarp = 9;  // producer warps with an extra duty
+
+// Warps of a CTA: epilogue first, then producers, one that issues the MMAs and one that
+// starts the copies.  Fourteen of them leave a thread 128 registers.  (The MMA queue
+// holds its issuer back while it is full: with a producer as the issuer the next tile's
+// slices waited for it, and the float32 backward of 1,048,576 rows took 584 instead of
+// 337 us.)
+constexpr int kNarrowWarps = 14;
+constexpr int kNarrowThreadsL = kNarrowWarps * 32;
+constexpr int kNarrowMmaWarp = 12, kNarrowCopyWarp = 13;
+constexpr int kForwardEpilogue = 8, kBackwardEpilogue = 4;
 constexpr int kDwTiles = 2;          // tiles whose d^T x is summed in TMEM
 
 template <typename T>
@@ -50,7 +58,7 @@ constexpr uint32_t kNarrowOperand = kCut<T> * kNarrowTile * 128;
 constexpr int kForwardSlices = 8;
 template <typename T>
 constexpr int kBackwardSlices = sizeof(T) == 4 ? 3 : 4;
-constexpr uint32_t kNarrowStaging = 8 * 4096;
+constexpr uint32_t kNarrowStaging = 8 * 4096;  // 4 KB per epilogue warp, at most eight
 
 template <typename T>
 constexpr size_t kNarrowForwardSmem =
@@ -78,22 +86,12 @@ __device__ __forceinline__ void store_unit(unsigned char* dst, uint32_t piece, i
                                            const float (&v)[4]) {
   unsigned char* at = dst + swizzled(r, u >> 1) + (u & 1) * 8;
   if constexpr (kCut<T> == 3) {
-    uint32_t part[3][2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const uint32_t u0 = __float_as_uint(v[2 * j]), u1 = __float_as_uint(v[2 * j + 1]);
-      part[0][j] = __byte_perm(u0, u1, 0x7632);
-      const float r0 = v[2 * j] - __uint_as_float(u0 & 0xffff0000u);
-      const float r1 = v[2 * j + 1] - __uint_as_float(u1 & 0xffff0000u);
-      const uint32_t v0 = __float_as_uint(r0), v1 = __float_as_uint(r1);
-      part[1][j] = __byte_perm(v0, v1, 0x7632);
-      const float s0 = r0 - __uint_as_float(v0 & 0xffff0000u);
-      const float s1 = r1 - __uint_as_float(v1 & 0xffff0000u);
-      part[2][j] = __byte_perm(__float_as_uint(s0), __float_as_uint(s1), 0x7632);
-    }
+    uint32_t lo[3], hi[3];
+    cut_pair(v[0], v[1], lo);
+    cut_pair(v[2], v[3], hi);
 #pragma unroll
     for (int q = 0; q < 3; ++q)
-      *reinterpret_cast<uint2*>(at + q * piece) = make_uint2(part[q][0], part[q][1]);
+      *reinterpret_cast<uint2*>(at + q * piece) = make_uint2(lo[q], hi[q]);
   } else {
     Pack<T, 4> o;
 #pragma unroll
@@ -124,8 +122,6 @@ struct Slice {
   const T* global;  // the same elements in memory
   int width, rows;  // rows of the tensor in the slice
   int copied;       // elements
-
-  __device__ __forceinline__ bool whole() const { return copied == rows * width; }
 };
 
 template <typename T>
@@ -133,60 +129,86 @@ __device__ __forceinline__ uint32_t slice_bytes(int width, int rows) {
   return static_cast<uint32_t>(rows * width * sizeof(T)) & ~15u;
 }
 
-// Columns 4 u .. of row r, zeros outside the operand.
 template <typename T>
+__device__ __noinline__ float4 read_unit_edge(const T* raw, const T* global, int width, int rows,
+                                              int copied, int r, int u) {
+  float v[4];
+  const int at = r * width + 4 * u;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    v[j] = 0.f;
+    if (r < rows && 4 * u + j < width)
+      v[j] = to_float(at + j < copied ? raw[at + j] : global[at + j]);
+  }
+  return make_float4(v[0], v[1], v[2], v[3]);
+}
+
+// Columns 4 u .. of row r, zeros outside the operand.  PLAIN: rows are whole 16-byte
+// blocks, so that all of a slice is copied and a unit is one access; a kernel of its own,
+// because the general read's code between the others' cost a third of the time.
+template <bool PLAIN, typename T>
 __device__ __forceinline__ void read_unit(const Slice<T>& s, int r, int u, float (&v)[4]) {
-  const int at = r * s.width + 4 * u;
-  if (r < s.rows && s.whole() && (s.width & 3) == 0) {
-    Pack<T, 4> pk{};
-    if (4 * u < s.width) pk = *reinterpret_cast<const Pack<T, 4>*>(s.raw + at);
+  if constexpr (PLAIN) {
+    uint32_t q[4] = {0, 0, 0, 0};
+    if (r < s.rows && 4 * u < s.width) {
+      const uint32_t at = smem_addr(s.raw) + (r * s.width + 4 * u) * sizeof(T);
+      if constexpr (sizeof(T) == 4)
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3])
+                     : "r"(at));
+      else
+        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(q[0]), "=r"(q[1]) : "r"(at));
+    }
+    const Pack<T, 4>& pk = *reinterpret_cast<const Pack<T, 4>*>(q);
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] = to_float(pk.v[j]);
   } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      v[j] = 0.f;
-      if (r < s.rows && 4 * u + j < s.width)
-        v[j] = to_float(at + j < s.copied ? s.raw[at + j] : s.global[at + j]);
-    }
+    const float4 f = read_unit_edge(s.raw, s.global, s.width, s.rows, s.copied, r, u);
+    v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
   }
 }
 
-// The `steps` K steps of one product, all the parts' products of a step together; strides
-// in the descriptors' units of 16 bytes.
+// The `steps` K steps of one product with 64 columns; strides in the descriptors' units of
+// 16 bytes.  The parts of B lie behind one another as 192 columns, so that a part of A
+// meets all the parts of B that it needs in one MMA (an MMA is bound by its operands'
+// 64 bytes a cycle out of shared memory, and fetches A again every time):
+//   a1 (b1 | b2 | b3), a2 (b1 | b2), a3 b1   into sums of order 0, 1 and 2, 64 columns each.
 template <int P>
-__device__ __forceinline__ void issue_cut(uint32_t d, uint32_t small, uint64_t a, uint64_t a_step,
-                                          uint64_t a_part, uint64_t b, uint64_t b_step,
-                                          uint64_t b_part, uint32_t desc, int steps, bool add) {
+__device__ __forceinline__ void issue_cut(uint32_t d, uint64_t a, uint64_t a_step, uint64_t a_part,
+                                          uint64_t b, uint64_t b_step, bool bf16, bool a_mn,
+                                          bool b_mn, int steps, bool add) {
+  const uint32_t one = mma_descriptor(bf16, a_mn, b_mn, kNarrowTile, kNarrow);
+  const uint32_t two = mma_descriptor(bf16, a_mn, b_mn, kNarrowTile, 2 * kNarrow);
+  const uint32_t three = mma_descriptor(bf16, a_mn, b_mn, kNarrowTile, 3 * kNarrow);
 #pragma unroll 1
   for (int k = 0; k < steps; ++k, a += a_step, b += b_step) {
-    mma_f16(d, a, b, desc, add);
     if constexpr (P == 3) {
-      mma_f16(small, a + 2 * a_part, b, desc, add);
-      mma_f16(small, a, b + 2 * b_part, desc, true);
-      mma_f16(small, a + a_part, b + b_part, desc, true);
-      mma_f16(small, a + a_part, b, desc, true);
-      mma_f16(small, a, b + b_part, desc, true);
+      mma_f16(d, a, b, three, add);
+      mma_f16(d + kNarrow, a + a_part, b, two, true);
+      mma_f16(d + 2 * kNarrow, a + 2 * a_part, b, one, true);
+    } else {
+      mma_f16(d, a, b, one, add);
     }
     add = true;
   }
 }
 
-// 32 columns of the warp's TMEM lanes, large and small sums together.
+// 32 columns of the warp's TMEM lanes, the sums of all orders together, smallest first.
 template <int P>
-__device__ __forceinline__ void take_sums(uint32_t at, uint32_t small, float (&v)[32], bool add) {
+__device__ __forceinline__ void take_sums(uint32_t at, float (&v)[32], bool add) {
 #pragma unroll
   for (int j = 0; j < 32; j += 16) {
-    float w[16];
+    float w[16], y[16], z[16];
     tmem_load16(at + j, w);
+    if constexpr (P == 3) {
+      tmem_load16(at + kNarrow + j, y);
+      tmem_load16(at + 2 * kNarrow + j, z);
+    }
     tmem_load_wait();
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[j + i] = add ? v[j + i] + w[i] : w[i];
-    if constexpr (P == 3) {
-      tmem_load16(at + small + j, w);
-      tmem_load_wait();
-#pragma unroll
-      for (int i = 0; i < 16; ++i) v[j + i] += w[i];
+    for (int i = 0; i < 16; ++i) {
+      const float sum = P == 3 ? w[i] + (y[i] + z[i]) : w[i];
+      v[j + i] = add ? v[j + i] + sum : sum;
     }
   }
 }
@@ -219,6 +241,13 @@ struct SliceWalk {
   }
 };
 
+// Copies in flight land before the CTA goes away (after a wait ran out).
+__device__ __forceinline__ void settle_copies() {
+  const unsigned long long begin = global_timer_ns();
+  while (global_timer_ns() - begin < kDrainLimitNs) {
+  }
+}
+
 // ------------------------------------------------------------------------- forward
 
 // Elements of y that came out NaN or infinite, by FMAs in order (the values are in `mine`).
@@ -237,11 +266,11 @@ __device__ __noinline__ void repair_narrow_forward(const NarrowArgs& p, const fl
   }
 }
 
-template <typename T, int ACT>
+template <typename T, int ACT, bool PLAIN>
 __global__ void __launch_bounds__(kNarrowThreadsL, 1)
     narrow_forward_kernel(const __grid_constant__ NarrowArgs p) {
   constexpr int P = kCut<T>, R = kForwardSlices;
-  constexpr uint32_t kSet = (P == 3 ? 2 : 1) * kNarrow, kColumns = 2 * kSet;
+  constexpr uint32_t kSet = P * kNarrow, kColumns = P == 3 ? 512 : 2 * kSet;
   constexpr uint32_t kPiece = kNarrowTile * 128;
   extern __shared__ unsigned char raw_smem[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(
@@ -261,15 +290,16 @@ __global__ void __launch_bounds__(kNarrowThreadsL, 1)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
+    constexpr int kProducers = kNarrowMmaWarp - kForwardEpilogue;
     for (int i = 0; i < R; ++i) {
       mbar_init(&raw_full[i], 1);
-      mbar_init(&raw_empty[i], 8);
+      mbar_init(&raw_empty[i], kProducers);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&full[i], 8);
+      mbar_init(&full[i], kProducers);
       mbar_init(&empty[i], 1);
       mbar_init(&done[i], 1);
-      mbar_init(&room[i], 8);
+      mbar_init(&room[i], kForwardEpilogue);
     }
     mbar_init(drain, 1);
     fence_mbarrier_init();
@@ -282,38 +312,63 @@ __global__ void __launch_bounds__(kNarrowThreadsL, 1)
   tcgen05_fence_after();
   const uint32_t tmem = *tmem_at;
 
-  if (warp >= 8) {
-    const int tid = threadIdx.x - 256, unit = tid & 15, r0 = tid >> 4;
-    const int steps = (p.k + 15) / 16;
+  const int steps = (p.k + 15) / 16;
+  if (warp == kNarrowCopyWarp) {
+    if (lane == 0) {
+      const T* x = static_cast<const T*>(p.x);
+      SliceWalk at{static_cast<int>(blockIdx.x), 0, p.tiles, static_cast<int>(gridDim.x), p.m};
+      bool ok = true;
+      for (uint32_t n = 0; !at.done(); at.next(), ++n) {
+        const int slot = n % R;
+        ok = mbar_wait_idle(&raw_empty[slot], ((n / R) & 1) ^ 1, kCodeProducer);
+        if (!ok) break;
+        const uint32_t bytes = slice_bytes<T>(p.k, at.rows());
+        mbar_arrive_expect_tx(&raw_full[slot], bytes);
+        if (bytes)
+          bulk_g2s(slices + slot * kSliceX<T>, x + at.row() * p.k, bytes, &raw_full[slot]);
+      }
+      if (!ok) settle_copies();
+    }
+    __syncwarp();
+  } else if (warp == kNarrowMmaWarp) {
+    if (lane == 0) {
+      bool ok = true;
+      uint32_t it = 0;
+      for (int t = blockIdx.x; t < p.tiles; t += gridDim.x, ++it) {
+        const int s = it & 1;
+        ok = mbar_wait_idle(&room[s], ((it >> 1) & 1) ^ 1, kCodeMma) &&
+             mbar_wait_idle(&full[s], (it >> 1) & 1, kCodeMma);
+        if (!ok) break;
+        tcgen05_fence_after();
+        issue_cut<P>(tmem + s * kSet,
+                     matrix_descriptor(smem_addr(tiles + s * kNarrowOperand<T>), 0, 1024), 2,
+                     kPiece / 16, matrix_descriptor(smem_addr(weights), 0, 1024), 2,
+                     !std::is_same_v<T, __half>, false, false, steps, false);
+        mma_commit(&empty[s]);
+        mma_commit(&done[s]);
+      }
+      if (!ok) {  // MMAs in flight finish
+        mma_commit(drain);
+        mbar_wait(drain, 0, kCodeDrain, kDrainLimitNs);
+      }
+    }
+    __syncwarp();
+  } else if (warp >= kForwardEpilogue) {
+    const int tid = threadIdx.x - kForwardEpilogue * 32, unit = tid & 15, r0 = tid >> 4;
     const T* x = static_cast<const T*>(p.x);
-    const SliceWalk start{static_cast<int>(blockIdx.x), 0, p.tiles, static_cast<int>(gridDim.x),
-                          p.m};
-    SliceWalk ahead = start;
-    const auto copy = [&](int slot) {  // the next slice to be copied, into `slot`
-      if (ahead.done()) return;
-      const uint32_t bytes = slice_bytes<T>(p.k, ahead.rows());
-      mbar_arrive_expect_tx(&raw_full[slot], bytes);
-      if (bytes) bulk_g2s(slices + slot * kSliceX<T>, x + ahead.row() * p.k, bytes,
-                          &raw_full[slot]);
-      ahead.next();
-    };
-    const bool copies = warp == kNarrowCopyWarp && lane == 0;
-    if (copies)
-      for (int i = 0; i < R; ++i) copy(i);
-    bool ok = true;
     uint32_t it = 0, n = 0;  // tiles and slices so far
+    bool ok = true;
     for (int t = blockIdx.x; ok && t < p.tiles; t += gridDim.x, ++it) {
       const int s = it & 1;
       ok = mbar_wait_warp(&empty[s], ((it >> 1) & 1) ^ 1, kCodeProducer);
-      if (!ok) break;
       unsigned char* tile = tiles + s * kNarrowOperand<T>;
       SliceWalk at{t, 0, p.tiles, static_cast<int>(gridDim.x), p.m};
 #pragma unroll 1
-      for (int q = 0; q < kNarrowTile / kSliceRows; ++q, ++at.slice) {
+      for (int q = 0; ok && q < kNarrowTile / kSliceRows; ++q, ++at.slice) {
         Slice<T> slice{nullptr, nullptr, p.k, 0, 0};
         const bool some = at.row() < p.m;
+        const int slot = n % R;
         if (some) {
-          const int slot = n % R;
           ok = mbar_wait_warp(&raw_full[slot], (n / R) & 1, kCodeProducer);
           if (!ok) break;
           slice.raw = reinterpret_cast<const T*>(slices + slot * kSliceX<T>);
@@ -321,60 +376,23 @@ __global__ void __launch_bounds__(kNarrowThreadsL, 1)
           slice.rows = at.rows();
           slice.copied = static_cast<int>(slice_bytes<T>(p.k, slice.rows) / sizeof(T));
         }
-        float v[2][4];
+        float v[4][4];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) read_unit(slice, r0 + 16 * j, unit, v[j]);
+        for (int j = 0; j < 4; ++j) read_unit<PLAIN>(slice, r0 + 8 * j, unit, v[j]);
         if (some) {
           __syncwarp();
-          if (lane == 0) mbar_arrive(&raw_empty[n % R]);
+          if (lane == 0) mbar_arrive(&raw_empty[slot]);
+          ++n;
         }
         if (unit < 4 * steps)
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
-            store_unit<T>(tile, kPiece, q * kSliceRows + r0 + 16 * j, unit, v[j]);
-        if (some) {
-          if (copies) {
-            ok = mbar_wait(&raw_empty[n % R], (n / R) & 1, kCodeProducer);
-            if (ok) copy(n % R);
-          }
-          if (warp == kNarrowCopyWarp) ok = __shfl_sync(0xffffffffu, static_cast<int>(ok), 0) != 0;
-          if (!ok) break;
-          ++n;
-        }
+          for (int j = 0; j < 4; ++j)
+            store_unit<T>(tile, kPiece, q * kSliceRows + r0 + 8 * j, unit, v[j]);
       }
       if (!ok) break;
       fence_proxy_async();
       __syncwarp();
       if (lane == 0) mbar_arrive(&full[s]);
-      if (warp == kNarrowMmaWarp) {
-        if (lane == 0) {
-          ok = mbar_wait(&room[s], ((it >> 1) & 1) ^ 1, kCodeMma) &&
-               mbar_wait(&full[s], (it >> 1) & 1, kCodeMma);
-          if (ok) {
-            tcgen05_fence_after();
-            constexpr uint32_t kDesc =
-                mma_descriptor(!std::is_same_v<T, __half>, false, false, kNarrowTile, kNarrow);
-            const uint32_t d = tmem + s * kSet;
-            issue_cut<P>(d, d + kNarrow, matrix_descriptor(smem_addr(tile), 0, 1024), 2,
-                         kPiece / 16, matrix_descriptor(smem_addr(weights), 0, 1024), 2,
-                         kNarrow * 128 / 16, kDesc, steps, false);
-            mma_commit(&empty[s]);
-            mma_commit(&done[s]);
-          }
-        }
-        ok = __shfl_sync(0xffffffffu, static_cast<int>(ok), 0) != 0;
-      }
-    }
-    if (!ok && (warp == kNarrowMmaWarp || warp == kNarrowCopyWarp)) {
-      if (lane == 0 && warp == kNarrowMmaWarp) {  // MMAs in flight finish
-        mma_commit(drain);
-        mbar_wait(drain, 0, kCodeDrain, kDrainLimitNs);
-      } else if (lane == 0) {  // copies in flight land
-        const unsigned long long begin = global_timer_ns();
-        while (global_timer_ns() - begin < kDrainLimitNs) {
-        }
-      }
-      __syncwarp();
     }
   } else {
     const int quad = warp & 3, half = warp >> 2;
@@ -384,22 +402,28 @@ __global__ void __launch_bounds__(kNarrowThreadsL, 1)
     o.n = p.n;
     o.e = p.e;
     uint32_t it = 0;
+    // a tile's residual is loaded while the tile before it is finished
+    ResidualBlock<T> res, next;
+    load_residual(o, static_cast<int64_t>(blockIdx.x) * kNarrowTile + quad * 32, half * 32, lane,
+                  next);
     for (int t = blockIdx.x; t < p.tiles; t += gridDim.x, ++it) {
       const int s = it & 1;
       const int64_t row0 = static_cast<int64_t>(t) * kNarrowTile + quad * 32;
-      ResidualBlock<T> res;
-      load_residual(o, row0, half * 32, lane, res);
       if (!mbar_wait_warp(&done[s], (it >> 1) & 1, kCodeEpilogue)) break;
       tcgen05_fence_after();
       float acc[32];
-      take_sums<P>(tmem + s * kSet + (static_cast<uint32_t>(quad * 32) << 16) + half * 32, kNarrow,
-                   acc, false);
+      take_sums<P>(tmem + s * kSet + (static_cast<uint32_t>(quad * 32) << 16) + half * 32, acc,
+                   false);
       tcgen05_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&room[s]);
-      write_block<T, ACT>(o, 0, acc, mine, row0, half * 32, lane, res);
+      const bool bad = P == 3 && any_nonfinite(acc);
+      stage_block(acc, mine, lane);
+      res = next;
+      load_residual(o, row0 + static_cast<int64_t>(gridDim.x) * kNarrowTile, half * 32, lane, next);
+      write_staged<T, ACT>(o, 0, mine, row0, half * 32, lane, res);
       if constexpr (P == 3) {
-        if (__any_sync(0xffffffffu, any_nonfinite(acc)))
+        if (__any_sync(0xffffffffu, bad))
           repair_narrow_forward(p, reinterpret_cast<const float*>(mine), row0 + lane, half * 32,
                                 lane);
         __syncwarp();
@@ -419,7 +443,7 @@ __global__ void __launch_bounds__(kNarrowThreadsL, 1)
 template <int ACT>
 __device__ __forceinline__ float narrow_d(const NarrowArgs& p, int64_t at) {
   const float g = static_cast<const float*>(p.g)[at];
-  return ACT == ICTC_ACT_NONE ? g : g * activation_slope<ACT, false>(p.preact[at]);
+  return ACT == ICTC_ACT_NONE ? g : g * activation_slope<ACT>(p.preact[at]);
 }
 
 // As above for dx = d W.
@@ -451,12 +475,12 @@ __device__ __noinline__ float repair_narrow_dw(const NarrowArgs& p, int n, int k
   return s;
 }
 
-template <typename T, int ACT>
+template <typename T, int ACT, bool PLAIN>
 __global__ void __launch_bounds__(kNarrowThreadsL, 1)
     narrow_backward_kernel(const __grid_constant__ NarrowArgs p) {
   constexpr int P = kCut<T>, R = kBackwardSlices<T>;
-  constexpr uint32_t kSet = (P == 3 ? 2 : 1) * kNarrow;
-  constexpr uint32_t kColumns = 4 * kSet;  // two sets of dx, two of dW
+  constexpr uint32_t kSet = P * kNarrow;
+  constexpr uint32_t kColumns = P == 3 ? 512 : 2 * kSet;  // one set of dx, one of dW
   constexpr uint32_t kPiece = kNarrowTile * 128;
   extern __shared__ unsigned char raw_smem[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(
@@ -469,28 +493,29 @@ __global__ void __launch_bounds__(kNarrowThreadsL, 1)
   uint64_t* raw_full = reinterpret_cast<uint64_t*>(staging + kNarrowStaging);
   uint64_t* raw_empty = raw_full + R;
   uint64_t* full = raw_empty + R;
-  uint64_t* empty = full + 1;
-  uint64_t* done = empty + 1;     // dx sets
-  uint64_t* room = done + 2;
-  uint64_t* dw_done = room + 2;   // dW sets
-  uint64_t* dw_room = dw_done + 2;
-  uint64_t* drain = dw_room + 2;
+  uint64_t* x_empty = full + 1;   // x's tile may be written again,
+  uint64_t* d_empty = x_empty + 1;  // and d's
+  uint64_t* done = d_empty + 1;   // dx
+  uint64_t* room = done + 1;
+  uint64_t* dw_done = room + 1;   // dW
+  uint64_t* dw_room = dw_done + 1;
+  uint64_t* drain = dw_room + 1;
   uint32_t* tmem_at = reinterpret_cast<uint32_t*>(drain + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
+    constexpr int kProducers = kNarrowMmaWarp - kBackwardEpilogue;
     for (int i = 0; i < R; ++i) {
       mbar_init(&raw_full[i], 1);
-      mbar_init(&raw_empty[i], 8);
+      mbar_init(&raw_empty[i], kProducers);
     }
-    mbar_init(full, 8);
-    mbar_init(empty, 1);
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&done[i], 1);
-      mbar_init(&room[i], 8);
-      mbar_init(&dw_done[i], 1);
-      mbar_init(&dw_room[i], 4);
-    }
+    mbar_init(full, kProducers);
+    mbar_init(x_empty, 1);
+    mbar_init(d_empty, 1);
+    mbar_init(done, 1);
+    mbar_init(room, kBackwardEpilogue);
+    mbar_init(dw_done, 1);
+    mbar_init(dw_room, 2);  // the warps of lanes 0-63
     mbar_init(drain, 1);
     fence_mbarrier_init();
   }
@@ -508,26 +533,73 @@ __global__ void __launch_bounds__(kNarrowThreadsL, 1)
   const bool want_dx = p.e.out != nullptr, want_dw = p.partial != nullptr;
   float db[4] = {0.f, 0.f, 0.f, 0.f};
 
-  if (warp >= 8) {
-    const int tid = threadIdx.x - 256, unit = tid & 15, r0 = tid >> 4;
-    const T* x = static_cast<const T*>(p.x);
-    const T* g = static_cast<const T*>(p.g);
-    SliceWalk ahead{static_cast<int>(blockIdx.x), 0, p.tiles, static_cast<int>(gridDim.x), p.m};
-    const auto copy = [&](int slot) {
-      if (ahead.done()) return;
-      const uint32_t bx = slice_bytes<T>(p.k, ahead.rows());
-      const uint32_t bg = slice_bytes<T>(p.n, ahead.rows());
-      const uint32_t bp = ACT == ICTC_ACT_NONE ? 0 : slice_bytes<float>(p.n, ahead.rows());
-      unsigned char* to = slices + slot * kBackwardSlice<T>;
-      mbar_arrive_expect_tx(&raw_full[slot], bx + bg + bp);
-      if (bx) bulk_g2s(to, x + ahead.row() * p.k, bx, &raw_full[slot]);
-      if (bg) bulk_g2s(to + kSliceX<T>, g + ahead.row() * p.n, bg, &raw_full[slot]);
-      if (bp) bulk_g2s(to + 2 * kSliceX<T>, p.preact + ahead.row() * p.n, bp, &raw_full[slot]);
-      ahead.next();
-    };
-    const bool copies = warp == kNarrowCopyWarp && lane == 0;
-    if (copies)
-      for (int i = 0; i < R; ++i) copy(i);
+  const T* x = static_cast<const T*>(p.x);
+  const T* g = static_cast<const T*>(p.g);
+  if (warp == kNarrowCopyWarp) {
+    if (lane == 0) {
+      SliceWalk at{static_cast<int>(blockIdx.x), 0, p.tiles, static_cast<int>(gridDim.x), p.m};
+      bool ok = true;
+      for (uint32_t n = 0; !at.done(); at.next(), ++n) {
+        const int slot = n % R;
+        ok = mbar_wait_idle(&raw_empty[slot], ((n / R) & 1) ^ 1, kCodeProducer);
+        if (!ok) break;
+        const uint32_t bx = slice_bytes<T>(p.k, at.rows());
+        const uint32_t bg = slice_bytes<T>(p.n, at.rows());
+        const uint32_t bp = ACT == ICTC_ACT_NONE ? 0 : slice_bytes<float>(p.n, at.rows());
+        unsigned char* to = slices + slot * kBackwardSlice<T>;
+        mbar_arrive_expect_tx(&raw_full[slot], bx + bg + bp);
+        if (bx) bulk_g2s(to, x + at.row() * p.k, bx, &raw_full[slot]);
+        if (bg) bulk_g2s(to + kSliceX<T>, g + at.row() * p.n, bg, &raw_full[slot]);
+        if (bp) bulk_g2s(to + 2 * kSliceX<T>, p.preact + at.row() * p.n, bp, &raw_full[slot]);
+      }
+      if (!ok) settle_copies();
+    }
+    __syncwarp();
+  } else if (warp == kNarrowMmaWarp) {
+    if (lane == 0) {
+      constexpr bool kBf16 = !std::is_same_v<T, __half>;
+      const uint32_t da = smem_addr(d_tile), xa = smem_addr(x_tile), wa = smem_addr(weights);
+      bool ok = true;
+      uint32_t it = 0;
+      for (int t = blockIdx.x; t < p.tiles; t += gridDim.x, ++it) {
+        ok = mbar_wait_idle(full, it & 1, kCodeMma);
+        if (!ok) break;
+        // dW first: x's tile is free again while the MMAs of dx still read d's
+        if (want_dw) {
+          const uint32_t group = it / kDwTiles;
+          const bool first = it % kDwTiles == 0;
+          if (first) ok = mbar_wait_idle(dw_room, (group & 1) ^ 1, kCodeMma);
+          if (!ok) break;
+          tcgen05_fence_after();
+          // both operands MN-major over the tile's rows; M is d's 64 columns and, one
+          // operand further, x's; N is x's columns, one part of x after the other
+          issue_cut<P>(tmem + kSet, matrix_descriptor(da, kNarrowOperand<T>, 1024), 128,
+                       kPiece / 16, matrix_descriptor(xa, kPiece, 1024), 128, kBf16, true, true,
+                       kNarrowTile / 16, !first);
+          if (it % kDwTiles == kDwTiles - 1 || t + static_cast<int>(gridDim.x) >= p.tiles)
+            mma_commit(dw_done);
+        }
+        mma_commit(x_empty);
+        if (want_dx) {
+          ok = mbar_wait_idle(room, (it & 1) ^ 1, kCodeMma);
+          if (!ok) break;
+          tcgen05_fence_after();
+          // W as [n][k] is MN-major for the sum over n: 16 rows a step
+          issue_cut<P>(tmem, matrix_descriptor(da, 0, 1024), 2, kPiece / 16,
+                       matrix_descriptor(wa, kNarrow * 128, 1024), 128, kBf16, false, true,
+                       (p.n + 15) / 16, false);
+          mma_commit(done);
+        }
+        mma_commit(d_empty);
+      }
+      if (!ok) {  // MMAs in flight finish
+        mma_commit(drain);
+        mbar_wait(drain, 0, kCodeDrain, kDrainLimitNs);
+      }
+    }
+    __syncwarp();
+  } else if (warp >= kBackwardEpilogue) {
+    const int tid = threadIdx.x - kBackwardEpilogue * 32, unit = tid & 15, r0 = tid >> 4;
     bool ok = true;
     uint32_t it = 0, n = 0;
     for (int t = blockIdx.x; ok && t < p.tiles; t += gridDim.x, ++it) {
@@ -553,14 +625,14 @@ __global__ void __launch_bounds__(kNarrowThreadsL, 1)
         }
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          read_unit(sx, r0 + 16 * j, unit, xv[2 * q + j]);
+          read_unit<PLAIN>(sx, r0 + 16 * j, unit, xv[2 * q + j]);
           float(&d)[4] = dv[2 * q + j];
-          read_unit(sg, r0 + 16 * j, unit, d);
+          read_unit<PLAIN>(sg, r0 + 16 * j, unit, d);
           if constexpr (ACT != ICTC_ACT_NONE) {
             float pv[4];
-            read_unit(sp, r0 + 16 * j, unit, pv);
+            read_unit<PLAIN>(sp, r0 + 16 * j, unit, pv);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) d[i] *= activation_slope<ACT, sizeof(T) == 2>(pv[i]);
+            for (int i = 0; i < 4; ++i) d[i] *= activation_slope<ACT>(pv[i]);
           }
 #pragma unroll
           for (int i = 0; i < 4; ++i) db[i] += d[i];
@@ -568,80 +640,26 @@ __global__ void __launch_bounds__(kNarrowThreadsL, 1)
         if (some) {
           __syncwarp();
           if (lane == 0) mbar_arrive(&raw_empty[slot]);
-          if (copies && ok) {
-            ok = mbar_wait(&raw_empty[slot], (n / R) & 1, kCodeProducer);
-            if (ok) copy(slot);
-          }
-          if (warp == kNarrowCopyWarp) ok = __shfl_sync(0xffffffffu, static_cast<int>(ok), 0) != 0;
           ++n;
         }
       }
-      if (ok) ok = mbar_wait_warp(empty, (it & 1) ^ 1, kCodeProducer);
+      if (ok) ok = mbar_wait_warp(x_empty, (it & 1) ^ 1, kCodeProducer);
       if (!ok) break;
+      const auto row = [&](int i) { return (i >> 1) * kSliceRows + r0 + 16 * (i & 1); };
+      if (4 * unit < p.k)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int r = (i >> 1) * kSliceRows + r0 + 16 * (i & 1);
-        if (4 * unit < p.k) store_unit<T>(x_tile, kPiece, r, unit, xv[i]);
-        if (4 * unit < p.n) store_unit<T>(d_tile, kPiece, r, unit, dv[i]);
-      }
+        for (int i = 0; i < 8; ++i) store_unit<T>(x_tile, kPiece, row(i), unit, xv[i]);
+      ok = mbar_wait_warp(d_empty, (it & 1) ^ 1, kCodeProducer);
+      if (!ok) break;
+      if (4 * unit < p.n)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) store_unit<T>(d_tile, kPiece, row(i), unit, dv[i]);
       fence_proxy_async();
       __syncwarp();
       if (lane == 0) mbar_arrive(full);
-      if (warp == kNarrowMmaWarp) {
-        if (lane == 0) {
-          constexpr bool kBf16 = !std::is_same_v<T, __half>;
-          const uint32_t da = smem_addr(d_tile), xa = smem_addr(x_tile), wa = smem_addr(weights);
-          ok = mbar_wait(full, it & 1, kCodeMma);
-          if (ok && want_dx) {
-            const int s = it & 1;
-            ok = mbar_wait(&room[s], ((it >> 1) & 1) ^ 1, kCodeMma);
-            if (ok) {
-              tcgen05_fence_after();
-              // W as [n][k] is MN-major for the sum over n: 16 rows a step
-              constexpr uint32_t kDesc = mma_descriptor(kBf16, false, true, kNarrowTile, kNarrow);
-              const uint32_t acc = tmem + s * kSet;
-              issue_cut<P>(acc, acc + kNarrow, matrix_descriptor(da, 0, 1024), 2, kPiece / 16,
-                           matrix_descriptor(wa, 0, 1024), 128, kNarrow * 128 / 16, kDesc,
-                           (p.n + 15) / 16, false);
-              mma_commit(&done[s]);
-            }
-          }
-          if (ok && want_dw) {
-            const uint32_t group = it / kDwTiles, s = group & 1;
-            const bool first = it % kDwTiles == 0;
-            if (first) ok = mbar_wait(&dw_room[s], ((group >> 1) & 1) ^ 1, kCodeMma);
-            if (ok) {
-              tcgen05_fence_after();
-              // both operands MN-major over the tile's rows; M is d's 64 columns and, one
-              // operand further, x's
-              constexpr uint32_t kDesc = mma_descriptor(kBf16, true, true, 128, kNarrow);
-              const uint32_t acc = tmem + 2 * kSet + s * kSet;
-              issue_cut<P>(acc, acc + kNarrow, matrix_descriptor(da, kNarrowOperand<T>, 1024), 128,
-                           kPiece / 16, matrix_descriptor(xa, 0, 1024), 128, kPiece / 16, kDesc,
-                           kNarrowTile / 16, !first);
-              if (it % kDwTiles == kDwTiles - 1 ||
-                  t + static_cast<int>(gridDim.x) >= p.tiles)
-                mma_commit(&dw_done[s]);
-            }
-          }
-          if (ok) mma_commit(empty);
-        }
-        ok = __shfl_sync(0xffffffffu, static_cast<int>(ok), 0) != 0;
-      }
-    }
-    if (!ok && (warp == kNarrowMmaWarp || warp == kNarrowCopyWarp)) {
-      if (lane == 0 && warp == kNarrowMmaWarp) {
-        mma_commit(drain);
-        mbar_wait(drain, 0, kCodeDrain, kDrainLimitNs);
-      } else if (lane == 0) {
-        const unsigned long long begin = global_timer_ns();
-        while (global_timer_ns() - begin < kDrainLimitNs) {
-        }
-      }
-      __syncwarp();
     }
   } else {
-    const int quad = warp & 3, half = warp >> 2;
+    const int quad = warp;
     float4* mine = reinterpret_cast<float4*>(staging + warp * 4096);
     const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
     ProductArgs o{};
@@ -649,58 +667,66 @@ __global__ void __launch_bounds__(kNarrowThreadsL, 1)
     o.n = p.k;
     o.e = p.e;
     const ResidualBlock<T> none{};
-    float dw[32];
+    float dw[2][32];
 #pragma unroll
-    for (int i = 0; i < 32; ++i) dw[i] = 0.f;
+    for (int i = 0; i < 32; ++i) dw[0][i] = dw[1][i] = 0.f;
     bool ok = true;
     uint32_t it = 0;
     for (int t = blockIdx.x; ok && t < p.tiles; t += gridDim.x, ++it) {
-      if (want_dx) {
-        const int s = it & 1;
-        const int64_t row0 = static_cast<int64_t>(t) * kNarrowTile + quad * 32;
-        ok = mbar_wait_warp(&done[s], (it >> 1) & 1, kCodeEpilogue);
-        if (!ok) break;
-        tcgen05_fence_after();
-        float acc[32];
-        take_sums<P>(tmem + s * kSet + lanes + half * 32, kNarrow, acc, false);
-        tcgen05_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&room[s]);
-        write_block<T, ICTC_ACT_NONE>(o, 0, acc, mine, row0, half * 32, lane, none);
-        if constexpr (P == 3) {
-          if (__any_sync(0xffffffffu, any_nonfinite(acc)))
-            repair_narrow_dx<ACT>(p, reinterpret_cast<const float*>(mine), row0 + lane, half * 32,
-                                  lane);
-          __syncwarp();
-        }
-      }
       if (want_dw && quad < 2 &&
           (it % kDwTiles == kDwTiles - 1 || t + static_cast<int>(gridDim.x) >= p.tiles)) {
-        const uint32_t group = it / kDwTiles, s = group & 1;
-        ok = mbar_wait_warp(&dw_done[s], (group >> 1) & 1, kCodeEpilogue);
+        ok = mbar_wait_warp(dw_done, (it / kDwTiles) & 1, kCodeEpilogue);
         if (!ok) break;
         tcgen05_fence_after();
-        take_sums<P>(tmem + 2 * kSet + s * kSet + lanes + half * 32, kNarrow, dw, true);
+        take_sums<P>(tmem + kSet + lanes, dw[0], true);
+        take_sums<P>(tmem + kSet + lanes + 32, dw[1], true);
         tcgen05_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&dw_room[s]);
+        if (lane == 0) mbar_arrive(dw_room);
+      }
+      if (want_dx) {
+        const int64_t row0 = static_cast<int64_t>(t) * kNarrowTile + quad * 32;
+        ok = mbar_wait_warp(done, it & 1, kCodeEpilogue);
+        if (!ok) break;
+        tcgen05_fence_after();
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+          float acc[32];
+          take_sums<P>(tmem + lanes + half * 32, acc, false);
+          if (half == 1) {
+            tcgen05_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(room);
+          }
+          if (half * 32 >= p.k) continue;
+          const bool bad = P == 3 && any_nonfinite(acc);
+          stage_block(acc, mine, lane);
+          write_staged<T, ICTC_ACT_NONE>(o, 0, mine, row0, half * 32, lane, none);
+          if constexpr (P == 3) {
+            if (__any_sync(0xffffffffu, bad))
+              repair_narrow_dx<ACT>(p, reinterpret_cast<const float*>(mine), row0 + lane,
+                                    half * 32, lane);
+            __syncwarp();
+          }
+        }
       }
     }
     if (want_dw && quad < 2) {
       const int n = quad * 32 + lane;
       float* out = p.partial + static_cast<int64_t>(blockIdx.x) * (p.n * p.k + p.n);
       if (n < p.n)
-        for (int i = 0; i < 32; ++i) {
-          const int k = half * 32 + i;
-          float v = 0.f;
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v = i == j ? dw[j] : v;
-          if (k >= p.k) break;
-          if constexpr (P == 3) {
-            if (!isfinite(v)) v = repair_narrow_dw<ACT>(p, n, k);
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const int k = half * 32 + i;
+            if (k < p.k) {
+              out[n * p.k + k] = dw[half][i];
+              if constexpr (P == 3) {
+                if (!isfinite(dw[half][i])) out[n * p.k + k] = repair_narrow_dw<ACT>(p, n, k);
+              }
+            }
           }
-          out[n * p.k + k] = v;
-        }
     }
   }
   tcgen05_fence_before();
@@ -712,8 +738,8 @@ __global__ void __launch_bounds__(kNarrowThreadsL, 1)
   // db: the 16 row lanes of each column, in order (the slices are free now)
   if (!want_dw) return;
   float* sums = reinterpret_cast<float*>(slices);
-  if (warp >= 8) {
-    const int tid = threadIdx.x - 256;
+  if (warp >= kBackwardEpilogue && warp < kNarrowMmaWarp) {
+    const int tid = threadIdx.x - kBackwardEpilogue * 32;
     *reinterpret_cast<float4*>(sums + (tid >> 4) * kNarrow + (tid & 15) * 4) =
         make_float4(db[0], db[1], db[2], db[3]);
   }

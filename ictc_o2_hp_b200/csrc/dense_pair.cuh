@@ -171,7 +171,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         const int n0 = static_cast<int>(pos.n0) + rank * (BN / 2);
         for (int c = pos.c0; c < pos.c1; ++c, ++it) {
           const int s = it % S;
-          ok = mbar_wait(&empty[s], ((it / S) & 1) ^ 1, kCodeProducer);
+          ok = mbar_wait_idle(&empty[s], ((it / S) & 1) ^ 1, kCodeProducer);
           if (!ok) break;
           unsigned char* stage = smem + s * kPairStageBytes<BN>;
           if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * kPairStageBytes<BN>);
@@ -182,7 +182,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       }
       // every stage's release by the MMAs has arrived before the CTA goes away
       for (int i = 0; ok && i < S; ++i, ++it)
-        ok = mbar_wait(&empty[it % S], ((it / S) & 1) ^ 1, kCodeProducer);
+        ok = mbar_wait_idle(&empty[it % S], ((it / S) & 1) ^ 1, kCodeProducer);
       if (!ok) {  // give copies in flight time to land before the CTA goes away
         const unsigned long long start = global_timer_ns();
         while (global_timer_ns() - start < kDrainLimitNs) {
@@ -198,13 +198,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       uint32_t it = 0, set = 0;
       for (int64_t t = first; ok && t < total; t += step, ++set) {
         const TilePos pos = tile_at<kPairRows>(p, t, BN);
-        ok = mbar_wait(&room[set & 1], ((set >> 1) & 1) ^ 1, kCodeMma);
+        ok = mbar_wait_idle(&room[set & 1], ((set >> 1) & 1) ^ 1, kCodeMma);
         if (!ok) break;
         tcgen05_fence_after();
         const uint32_t d = tmem + (set & 1) * BN;
         for (int c = pos.c0; c < pos.c1; ++c, ++it) {
           const int s = it % S;
-          ok = mbar_wait(&full[s], (it / S) & 1, kCodeMma);
+          ok = mbar_wait_idle(&full[s], (it / S) & 1, kCodeMma);
           if (!ok) break;
           tcgen05_fence_after();
           const uint32_t sa = smem_addr(smem + s * kPairStageBytes<BN>);

@@ -23,6 +23,22 @@ __device__ __forceinline__ uint32_t swizzled(uint32_t r, uint32_t c) {
   return r * 128 + ((c ^ (r & 7)) << 4);
 }
 
+// The bf16 parts of two float32 values, eight significant bits each by truncation (the
+// three add up to the value exactly), the first value in the low half.
+__device__ __forceinline__ void cut_pair(float x0, float x1, uint32_t (&part)[3]) {
+  const uint32_t u0 = __float_as_uint(x0), u1 = __float_as_uint(x1);
+  part[0] = __byte_perm(u0, u1, 0x7632);
+  // x - (leading part): the sign is flipped on the integer side, the pair added at once
+  const float2 r = __fadd2_rn(make_float2(x0, x1),
+                              make_float2(__uint_as_float((u0 & 0xffff0000u) ^ 0x80000000u),
+                                          __uint_as_float((u1 & 0xffff0000u) ^ 0x80000000u)));
+  const uint32_t v0 = __float_as_uint(r.x), v1 = __float_as_uint(r.y);
+  part[1] = __byte_perm(v0, v1, 0x7632);
+  const float2 s = __fadd2_rn(r, make_float2(__uint_as_float((v0 & 0xffff0000u) ^ 0x80000000u),
+                                             __uint_as_float((v1 & 0xffff0000u) ^ 0x80000000u)));
+  part[2] = __byte_perm(__float_as_uint(s.x), __float_as_uint(s.y), 0x7632);
+}
+
 // Shared-memory matrix descriptor, 128-byte swizzle.  Groups of eight 128-byte rows are
 // `stride` bytes apart; `leading` is the distance of the 64-element blocks of an
 // MN-major operand (unused for K-major ones).

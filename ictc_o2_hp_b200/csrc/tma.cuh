@@ -99,9 +99,32 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int co
   return false;
 }
 
+// The same with the thread suspended, up to a millisecond at a time, until the phase
+// completes: for warps whose neighbours need the issue slots that polling takes.
+__device__ __forceinline__ bool mbar_wait_idle(uint64_t* bar, uint32_t parity, int code) {
+  const auto suspended = [&] {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(smem_addr(bar)), "r"(parity), "r"(1000000u)
+        : "memory");
+    return done != 0;
+  };
+  if (suspended()) return true;
+  const unsigned long long start = global_timer_ns();
+  do {
+    if (suspended()) return true;
+  } while (global_timer_ns() - start < kWaitLimitNs);
+  atomicExch(&g_ictc_device_error, code);
+  return false;
+}
+
 // The same for a converged warp: one answer for all its lanes.
 __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, int code) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, code)) != 0;
+  return __all_sync(0xffffffffu, mbar_wait_idle(bar, parity, code)) != 0;
 }
 
 // Global -> shared bulk copy completing on `bar` (bytes counted by expect_tx).
