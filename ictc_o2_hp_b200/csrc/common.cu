@@ -96,12 +96,12 @@ int encode3(PFN_cuTensorMapEncodeTiled_v12000 fn, CUtensorMap* map, const float*
 
 }  // namespace
 
-int encode_matrix_map(const void* base, bool bf16, int64_t inner, int64_t outer, int64_t stride,
-                      int box_inner, int box_outer, CUtensorMap* map) {
+int encode_matrix_map(const void* base, int size, bool bf16, int64_t inner, int64_t outer,
+                      int64_t stride, int box_inner, int box_outer, CUtensorMap* map) {
   PFN_cuTensorMapEncodeTiled_v12000 fn = tensor_map_encoder();
   if (fn == nullptr || inner < 1 || outer < 1 || stride % 16 != 0 || stride >= (1ll << 40) ||
       inner >= (1ll << 31) || outer >= (1ll << 31) ||
-      stride < 2 * inner)  // rows that overlap or repeat are left to other kernels
+      stride < size * inner)  // rows that overlap or repeat are left to other kernels
     return -1;
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer)};
   const cuuint64_t strides[1] = {static_cast<cuuint64_t>(stride)};
@@ -109,9 +109,12 @@ int encode_matrix_map(const void* base, bool bf16, int64_t inner, int64_t outer,
                              static_cast<cuuint32_t>(box_outer)};
   const cuuint32_t estr[2] = {1, 1};
   const CUresult r =
-      fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
-         const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+      fn(map,
+         size == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                   : bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+         2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+         size == 4 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
+         CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? 0 : -1;
 }

@@ -134,7 +134,8 @@ __device__ __forceinline__ void stage_block(const float* acc, float4* mine, int 
   __syncwarp();
 }
 
-template <typename T, int ACT>
+// LATE: the residual is loaded here, half a block at a time, where registers are short.
+template <typename T, int ACT, bool LATE = false>
 __device__ __forceinline__ void write_staged(const ProductArgs& p, int split, const float4* mine,
                                              int64_t row0, int64_t col0, int lane,
                                              const ResidualBlock<T>& res) {
@@ -158,14 +159,26 @@ __device__ __forceinline__ void write_staged(const ProductArgs& p, int split, co
       float bias[4];
       load_bias4<T>(e, col, p.n, bias);
       const int64_t at = (row0 + (lane >> 3)) * p.n + col;
+      constexpr int kBatch = LATE ? 4 : 8;
+#pragma unroll 1
+      for (int i0 = 0; i0 < 8; i0 += kBatch) {
+        Pack<T, 4> late[4];
+        if constexpr (LATE) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int r = (lane >> 3) + 4 * i;
-        if (r < rows) {
-          const float4 f = mine[r * 8 + ((lane & 7) ^ (r & 7))];
-          float v[4] = {f.x, f.y, f.z, f.w};
-          Pack<T, 4> z{};
-          finish4<T, ACT>(e, at + 4 * i * p.n, v, bias, e.residual ? res.v[i] : z);
+          for (int i = 0; i < 4; ++i)
+            if (e.residual && (lane >> 3) + 4 * (i0 + i) < rows)
+              late[i] = residual4<T>(e, row0 + (lane >> 3) + 4 * (i0 + i), col);
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          const int r = (lane >> 3) + 4 * (i0 + i);
+          if (r < rows) {
+            const float4 f = mine[r * 8 + ((lane & 7) ^ (r & 7))];
+            float v[4] = {f.x, f.y, f.z, f.w};
+            Pack<T, 4> z{};
+            finish4<T, ACT>(e, at + 4 * (i0 + i) * p.n, v, bias,
+                            e.residual ? (LATE ? late[i & 3] : res.v[i]) : z);
+          }
         }
       }
     } else {

@@ -19,6 +19,7 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "dense_cut.cuh"
 #include "dense_epilogue.cuh"
 #include "dense_narrow.cuh"
 #include "dense_pair.cuh"
@@ -122,32 +123,6 @@ __device__ __forceinline__ void store_operand(unsigned char* dst, int tid,
     } else {
       *reinterpret_cast<uint4*>(dst + at) = *reinterpret_cast<const uint4*>(&h.v[i]);
     }
-  }
-}
-
-// The NaN and infinite elements of the block that write_block just wrote (lane = row;
-// the values are still in `mine`) again, by FMAs in K order: an infinity or NaN among a
-// float32 product's operands has no bf16 parts to speak of.  Rare, so kept out of line.
-template <bool A_MN, bool B_MN>
-__device__ __noinline__ void repair_block(const ProductArgs& p, int split, int c0, int c1,
-                                          const float* mine, int64_t row, int64_t col0, int lane) {
-  const float* a = static_cast<const float*>(p.a);
-  const float* b = static_cast<const float*>(p.b);
-  const int64_t k0 = static_cast<int64_t>(c0) * kBK;
-  const int64_t k1 = static_cast<int64_t>(c1) * kBK < p.k ? static_cast<int64_t>(c1) * kBK : p.k;
-  for (int c = 0; c < 32; ++c) {
-    const int64_t col = col0 + c;
-    const float v = mine[lane * 32 + (((c >> 2) ^ (lane & 7)) << 2) + (c & 3)];
-    if (row >= p.m || col >= p.n || isfinite(v)) continue;
-    float s = 0.f;
-    for (int64_t k = k0; k < k1; ++k)
-      s = fmaf(A_MN ? a[k * p.lda + row] : a[row * p.lda + k],
-               B_MN ? b[k * p.ldb + col] : b[col * p.ldb + k], s);
-    if (p.e.partial)
-      p.e.partial[(split * p.m + row) * p.n + col] = s;
-    else
-      finish1<float, kAnyActivation>(p.e, row, col, p.n, s,
-                     p.e.bias ? static_cast<const float*>(p.e.bias)[col] : 0.f);
   }
 }
 
@@ -340,8 +315,13 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
 #pragma unroll
           for (int i = 0; i < 32; ++i) zero = fmaf(acc[cb * 32 + i], 0.f, zero);
           if (__any_sync(0xffffffffu, zero != 0.f))
-            repair_block<A_MN, B_MN>(p, pos.split, pos.c0, pos.c1, reinterpret_cast<const float*>(mine), row0 + lane,
-                                     col0, lane);
+            {
+              const int64_t k0 = static_cast<int64_t>(pos.c0) * kBK;
+              const int64_t k1 = static_cast<int64_t>(pos.c1) * kBK;
+              repair_block<A_MN, B_MN>(p, pos.split, k0, k1 < p.k ? k1 : p.k,
+                                       reinterpret_cast<const float*>(mine), row0 + lane, col0,
+                                       lane);
+            }
           __syncwarp();
         }
       }
@@ -624,7 +604,7 @@ void for_epilogue(const ProductArgs& p, const F& f) {
 }
 
 template <typename T, bool A_MN, bool B_MN, int BN>
-int launch_pair(const PairMaps& maps, const ProductArgs& p, int device, cudaStream_t stream) {
+int launch_pair(const OperandMaps& maps, const ProductArgs& p, int device, cudaStream_t stream) {
   const int64_t total = static_cast<int64_t>(p.tiles_m) * p.tiles_n * p.splits;
   const int64_t pairs = sm_count(device) / 2;
   const unsigned grid = static_cast<unsigned>(2 * (total < pairs ? total : pairs));
@@ -639,6 +619,22 @@ int launch_pair(const PairMaps& maps, const ProductArgs& p, int device, cudaStre
   return e == cudaSuccess ? ICTC_OK : cuda_fail(e, "linear pair product launch");
 }
 
+template <bool A_MN, bool B_MN, int BN>
+int launch_cut(const OperandMaps& maps, const ProductArgs& p, int device, cudaStream_t stream) {
+  const int64_t total = static_cast<int64_t>(p.tiles_m) * p.tiles_n * p.splits;
+  const int64_t sms = sm_count(device);
+  const unsigned grid = static_cast<unsigned>(total < sms ? total : sms);
+  int st = ICTC_OK;
+  for_epilogue<!A_MN && !B_MN>(p, [&](auto act) {
+    const auto kernel = cut_product_kernel<A_MN, B_MN, BN, act.value>;
+    st = allow_smem(reinterpret_cast<const void*>(kernel), kCutSmem<BN>);
+    if (st == ICTC_OK) kernel<<<grid, kCutThreads, kCutSmem<BN>, stream>>>(maps, p);
+  });
+  if (st != ICTC_OK) return st;
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? ICTC_OK : cuda_fail(e, "linear float32 product launch");
+}
+
 template <typename T, bool A_MN, bool B_MN, int BN>
 int launch_product(const ProductArgs& p, int device, cudaStream_t stream) {
   const int64_t total = static_cast<int64_t>(p.tiles_m) * p.tiles_n * p.splits;
@@ -650,9 +646,8 @@ int launch_product(const ProductArgs& p, int device, cudaStream_t stream) {
     st = allow_smem(reinterpret_cast<const void*>(kernel), kProductSmem<T, BN>);
     if (st == ICTC_OK) kernel<<<grid, kProductThreads, kProductSmem<T, BN>, stream>>>(p);
   };
-  // 16-bit products come here only when small or unaligned: one kernel for every activation
-  if constexpr (sizeof(T) == 2) launch(std::integral_constant<int, kAnyActivation>{});
-  else for_epilogue<!A_MN && !B_MN>(p, launch);
+  // products come here only when small or unaligned: one kernel for every activation
+  launch(std::integral_constant<int, kAnyActivation>{});
   if (st != ICTC_OK) return st;
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? ICTC_OK : cuda_fail(e, "linear product launch");
@@ -682,13 +677,13 @@ int run_product(const T* a, int64_t lda, const T* b, int64_t ldb, int64_t m, int
   };
   if constexpr (sizeof(T) == 2) {
     const PairPlan q = plan_pair(m, n, k, device);
-    PairMaps maps;
+    OperandMaps maps;
     if (q.ok && use_pair(m, n, k) && chunk_aligned(a, lda, 2) && chunk_aligned(b, ldb, 2)) {
       constexpr bool kBf16 = std::is_same_v<T, __nv_bfloat16>;
       const bool mapped =
-          encode_matrix_map(a, kBf16, A_MN ? m : k, A_MN ? k : m, lda * 2, 64, A_MN ? 64 : 128,
+          encode_matrix_map(a, 2, kBf16, A_MN ? m : k, A_MN ? k : m, lda * 2, 64, A_MN ? 64 : 128,
                             &maps.a) == 0 &&
-          encode_matrix_map(b, kBf16, B_MN ? n : k, B_MN ? k : n, ldb * 2, 64,
+          encode_matrix_map(b, 2, kBf16, B_MN ? n : k, B_MN ? k : n, ldb * 2, 64,
                             B_MN ? 64 : q.bn / 2, &maps.b) == 0;
       if (mapped) {
         ProductArgs p{};
@@ -715,6 +710,18 @@ int run_product(const T* a, int64_t lda, const T* b, int64_t ldb, int64_t m, int
   p.vec_b = chunk_aligned(b, ldb, sizeof(T));
   e.partial = s.splits > 1 ? partial : nullptr;
   p.e = e;
+  if constexpr (sizeof(T) == 4) {
+    OperandMaps maps;
+    if (p.vec_a && p.vec_b && m < (1ll << 31) && n < (1ll << 31) && k < (1ll << 31) &&
+        encode_matrix_map(a, 4, false, A_MN ? m : k, A_MN ? k : m, lda * 4, A_MN ? 128 : kCutK,
+                          A_MN ? kCutK : 128, &maps.a) == 0 &&
+        encode_matrix_map(b, 4, false, B_MN ? n : k, B_MN ? k : n, ldb * 4, B_MN ? s.bn : kCutK,
+                          B_MN ? kCutK : s.bn, &maps.b) == 0) {
+      const int st = s.bn == 64 ? launch_cut<A_MN, B_MN, 64>(maps, p, device, stream)
+                                : launch_cut<A_MN, B_MN, 128>(maps, p, device, stream);
+      return st != ICTC_OK || s.splits == 1 ? st : join(s.splits);
+    }
+  }
   const int st = s.bn == 64 ? launch_product<T, A_MN, B_MN, 64>(p, device, stream)
                             : launch_product<T, A_MN, B_MN, 128>(p, device, stream);
   return st != ICTC_OK || s.splits == 1 ? st : join(s.splits);

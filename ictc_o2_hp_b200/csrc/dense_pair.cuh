@@ -106,7 +106,7 @@ constexpr size_t kPairSmem =
     1024 + kPairStages<BN> * kPairStageBytes<BN> + kPairEpilogueWarps * 4096 + 256;
 
 // Box of an operand's tensor map: K-major {64 k, rows}, MN-major {64 rows, 64 k}.
-struct alignas(64) PairMaps {
+struct alignas(64) OperandMaps {
   CUtensorMap a, b;
 };
 
@@ -123,7 +123,7 @@ __device__ __forceinline__ void load_tile(unsigned char* dst, const CUtensorMap*
 
 template <typename T, bool A_MN, bool B_MN, int BN, int ACT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
-    pair_product_kernel(const __grid_constant__ PairMaps maps, const __grid_constant__ ProductArgs p) {
+    pair_product_kernel(const __grid_constant__ OperandMaps maps, const __grid_constant__ ProductArgs p) {
   constexpr int S = kPairStages<BN>;
   constexpr uint32_t kABytes = 128 * 128;
   constexpr uint32_t kColumns = 2 * BN;  // two accumulator sets

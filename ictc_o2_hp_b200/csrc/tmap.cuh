@@ -32,12 +32,25 @@ struct alignas(64) RowTileMaps {
 int encode_row_tile_maps(const float* base, int64_t rows, int C, int M, bool full, bool cm,
                          int64_t width, int Ct, CUtensorMap* maps);
 
-// Host: a row-major matrix of 16-bit elements, `outer` rows of `inner` elements `stride`
-// bytes apart, read in boxes of box_inner x box_outer (box_inner = 64: one 128-byte
-// swizzled row), zeros outside.  Returns 0, or -1 when the driver entry point is
-// unavailable or the encoding is rejected.
-int encode_matrix_map(const void* base, bool bf16, int64_t inner, int64_t outer, int64_t stride,
-                      int box_inner, int box_outer, CUtensorMap* map);
+// Host: a row-major matrix of `size`-byte elements (2: bf16 or f16, 4: float32), `outer`
+// rows of `inner` elements `stride` bytes apart, read in boxes of box_inner x box_outer,
+// zeros outside.  16-bit boxes (box_inner = 64) land as 128-byte swizzled rows, float32
+// ones as plain rows.  Returns 0, or -1 when the driver entry point is unavailable or the
+// encoding is rejected.
+int encode_matrix_map(const void* base, int size, bool bf16, int64_t inner, int64_t outer,
+                      int64_t stride, int box_inner, int box_outer, CUtensorMap* map);
+
+// 2-D tile load of box coordinates (x, y) into shared memory, completing on `bar`.
+__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int x, int y,
+                                            uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3}], [%4];"
+      ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst))),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y),
+        "r"(static_cast<uint32_t>(__cvta_generic_to_shared(bar)))
+      : "memory");
+}
 
 // 3-D tile load of box coordinates (x, y, z) into shared memory, completing on `bar`.
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z,
