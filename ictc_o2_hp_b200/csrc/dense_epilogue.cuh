@@ -99,27 +99,44 @@ __device__ __forceinline__ void finish4(const Epilogue& e, int64_t at, float (&v
   *reinterpret_cast<Pack<T, 4>*>(static_cast<T*>(e.out) + at) = o;
 }
 
-// The residual's part of a 32 x 32 block: rows lane / 8 + 4 i, four columns each.  Loaded
-// well before write_block needs it (ahead of the wait for the accumulators): its latency,
-// exposed, had been half of the epilogue of a tile with little K.
+// The residual's part of a 32 x 32 block: with a vec epilogue rows lane / 8 + 4 i, four
+// columns each; otherwise column `lane`, element j of v[i] row 4 i + j.  Loaded well before
+// write_staged needs it (ahead of the wait for the accumulators): loads behind the stores,
+// which they might alias, had exposed their latency row by row.
 template <typename T>
 struct ResidualBlock {
   Pack<T, 4> v[8];
 };
 
+template <typename T, int COUNT>
+__device__ __forceinline__ void load_residual_part(const ProductArgs& p, int64_t row0,
+                                                   int64_t col0, int lane, int first,
+                                                   Pack<T, 4>* v) {
+  const Epilogue& e = p.e;
+  if (!e.residual || e.partial) return;
+  const int64_t col = col0 + (e.vec ? (lane & 7) * 4 : lane);
+  if (col >= p.n) return;
+  const T* base = static_cast<const T*>(e.residual) + col;
+  if (e.vec) {
+    const int64_t row = row0 + (lane >> 3) + 4 * first;
+    const T* at = base + row * e.residual_stride;
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i)
+      if (row + 4 * i < p.m)
+        v[i] = *reinterpret_cast<const Pack<T, 4>*>(at + 4 * i * e.residual_stride);
+  } else {
+    const int64_t row = row0 + 4 * first;
+    const T* at = base + row * e.residual_stride;
+#pragma unroll
+    for (int i = 0; i < 4 * COUNT; ++i)
+      if (row + i < p.m) v[i / 4].v[i % 4] = at[i * e.residual_stride];
+  }
+}
+
 template <typename T>
 __device__ __forceinline__ void load_residual(const ProductArgs& p, int64_t row0, int64_t col0,
                                               int lane, ResidualBlock<T>& res) {
-  const Epilogue& e = p.e;
-  if (!e.residual || !e.vec || e.partial) return;
-  const int64_t col = col0 + (lane & 7) * 4;
-  if (col >= p.n) return;
-  const T* at = static_cast<const T*>(e.residual) + (row0 + (lane >> 3)) * e.residual_stride + col;
-  const int64_t left = p.m - row0 - (lane >> 3);
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (4 * i < left)
-      res.v[i] = *reinterpret_cast<const Pack<T, 4>*>(at + 4 * i * e.residual_stride);
+  load_residual_part<T, 8>(p, row0, col0, lane, 0, res.v);
 }
 
 // One 32 x 32 block of an output tile, row-per-lane in `acc`, to memory: through the
@@ -163,12 +180,7 @@ __device__ __forceinline__ void write_staged(const ProductArgs& p, int split, co
 #pragma unroll 1
       for (int i0 = 0; i0 < 8; i0 += kBatch) {
         Pack<T, 4> late[4];
-        if constexpr (LATE) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (e.residual && (lane >> 3) + 4 * (i0 + i) < rows)
-              late[i] = residual4<T>(e, row0 + (lane >> 3) + 4 * (i0 + i), col);
-        }
+        if constexpr (LATE) load_residual_part<T, 4>(p, row0, col0, lane, i0, late);
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
           const int r = (lane >> 3) + 4 * (i0 + i);
@@ -184,10 +196,26 @@ __device__ __forceinline__ void write_staged(const ProductArgs& p, int split, co
     } else {
       const float bias = e.bias ? to_float(static_cast<const T*>(e.bias)[col]) : 0.f;
       const float* flat = reinterpret_cast<const float*>(mine);
-#pragma unroll 4
-      for (int r = 0; r < rows; ++r)
-        finish1<T, ACT>(e, row0 + r, col, p.n,
-                        flat[r * 32 + (((lane >> 2) ^ (r & 7)) << 2) + (lane & 3)], bias);
+      float* preact = e.preact ? e.preact + row0 * p.n + col : nullptr;
+      T* out = static_cast<T*>(e.out) + row0 * p.n + col;
+      constexpr int kBatch = LATE ? 16 : 32;
+#pragma unroll 1
+      for (int i0 = 0; i0 < 32; i0 += kBatch) {
+        Pack<T, 4> late[4];
+        if constexpr (LATE) load_residual_part<T, 4>(p, row0, col0, lane, i0 / 4, late);
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          const int r = i0 + i;
+          if (r < rows) {
+            const float v = flat[r * 32 + (((lane >> 2) ^ (r & 7)) << 2) + (lane & 3)] + bias;
+            if (preact) preact[r * p.n] = v;
+            float y = activate<ACT>(v, e.activation);
+            if (e.residual)
+              y += to_float(LATE ? late[(i / 4) & 3].v[i % 4] : res.v[i / 4].v[i % 4]);
+            out[r * p.n] = from_float<T>(y);
+          }
+        }
+      }
     }
   }
   __syncwarp();
