@@ -276,59 +276,6 @@ def radial_backward(left, angular, hidden, alpha, bias, grad_output, gx, gy, gh,
         ptr(workspace), workspace.numel(), stream_of(left.device)), "radial_backward")
 
 
-# ---------------------------------------------------------------------- dense
-# dtype and activation arguments are the C ABI's integer codes; `rows`-like tensors are
-# two-dimensional with unit stride inside a row.
-
-
-def layer_norm_workspace(rows: int, width: int, dtype: int, device: int) -> int:
-    out = _size()
-    check(load().ictc_o2_layer_norm_workspace(rows, width, dtype, device, ctypes.byref(out)),
-          "layer_norm_workspace")
-    return int(out.value)
-
-
-def layer_norm_forward(x, weight, bias, y, mean, rstd, eps, dtype, param_dtype):
-    check(load().ictc_o2_layer_norm_forward(
-        x.data_ptr(), x.stride(0), ptr(weight), ptr(bias), y.data_ptr(), ptr(mean), ptr(rstd),
-        x.shape[0], x.shape[1], eps, dtype, param_dtype, stream_of(x.device)),
-        "layer_norm_forward")
-
-
-def layer_norm_backward(x, weight, mean, rstd, grad, gx, gw, gb, workspace, dtype, param_dtype):
-    check(load().ictc_o2_layer_norm_backward(
-        x.data_ptr(), x.stride(0), ptr(weight), mean.data_ptr(), rstd.data_ptr(),
-        grad.data_ptr(), grad.stride(0), ptr(gx), ptr(gw), ptr(gb), ptr(workspace),
-        workspace.numel() if workspace is not None else 0, x.shape[0], x.shape[1], dtype,
-        param_dtype, stream_of(x.device)), "layer_norm_backward")
-
-
-def linear_workspace(rows: int, inner: int, outer: int, dtype: int, activation: int, layout: int,
-                     device: int) -> tuple[int, int]:
-    fwd, bwd = _size(), _size()
-    check(load().ictc_o2_linear_workspace(rows, inner, outer, dtype, activation, layout, device,
-                                          ctypes.byref(fwd), ctypes.byref(bwd)),
-          "linear_workspace")
-    return int(fwd.value), int(bwd.value)
-
-
-def linear_forward(x, weight, bias, residual, y, preact, workspace, outer, dtype, activation):
-    check(load().ictc_o2_linear_forward(
-        x.data_ptr(), x.stride(0), weight.data_ptr(), weight.stride(0), ptr(bias), ptr(residual),
-        residual.stride(0) if residual is not None else 0, y.data_ptr(), ptr(preact),
-        ptr(workspace), workspace.numel() if workspace is not None else 0, x.shape[0], x.shape[1],
-        outer, dtype, activation, stream_of(x.device)), "linear_forward")
-
-
-def linear_backward(x, weight, preact, grad, gx, gw, gb, workspace, rows, inner, outer, dtype,
-                    activation):
-    check(load().ictc_o2_linear_backward(
-        x.data_ptr(), x.stride(0), weight.data_ptr(), weight.stride(0), ptr(preact),
-        grad.data_ptr(), grad.stride(0), ptr(gx), ptr(gw), ptr(gb), ptr(workspace),
-        workspace.numel() if workspace is not None else 0, rows, inner, outer, dtype, activation,
-        stream_of(x.device)), "linear_backward")
-
-
 # ---------------------------------------------------------------------- graph
 
 
