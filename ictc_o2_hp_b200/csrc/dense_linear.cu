@@ -434,6 +434,66 @@ __global__ void __launch_bounds__(kRowThreads) few_rows_kernel(
   }
 }
 
+// --------------------------------------------------------------- few columns: no tiles
+// Up to eight columns over many rows that TMA cannot address: reading A once as it lies is
+// cheaper than copying it to aligned rows first.  A warp owns four rows; lanes run along K;
+// B's columns are staged in shared memory once per CTA, and each value read from there
+// serves four rows.  Sums: FMAs per lane, then a butterfly.
+constexpr int kThinColumns = 8, kThinRows = 4;
+constexpr size_t kThinBytes = 192 * 1024;  // of B's columns, at most
+
+template <typename T, bool B_MN, int NC>
+__global__ void __launch_bounds__(256) few_columns_kernel(const __grid_constant__ ProductArgs p) {
+  extern __shared__ float columns[];  // [NC][k]
+  const T* a = static_cast<const T*>(p.a);
+  const T* b = static_cast<const T*>(p.b);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n = static_cast<int>(p.n), len = static_cast<int>(p.k);
+#pragma unroll
+  for (int c = 0; c < NC; ++c)
+    for (int k = threadIdx.x; k < len; k += 256)
+      columns[c * len + k] = c < n ? to_float(B_MN ? b[k * p.ldb + c] : b[c * p.ldb + k]) : 0.f;
+  __syncthreads();
+  const int64_t step = static_cast<int64_t>(gridDim.x) * 8 * kThinRows;
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * 8 * kThinRows; base < p.m; base += step) {
+    const int64_t row0 = base + warp * kThinRows;
+    const T* rows[kThinRows];  // past the end: the last row again, its sums dropped
+#pragma unroll
+    for (int r = 0; r < kThinRows; ++r)
+      rows[r] = a + (row0 + r < p.m ? row0 + r : p.m - 1) * p.lda;
+    float acc[kThinRows][NC];
+#pragma unroll
+    for (int r = 0; r < kThinRows; ++r)
+#pragma unroll
+      for (int c = 0; c < NC; ++c) acc[r][c] = 0.f;
+    // unrolled for the loads: a warp has sixteen in flight
+#pragma unroll 4
+    for (int k = lane; k < len; k += 32) {
+      float x[kThinRows];
+#pragma unroll
+      for (int r = 0; r < kThinRows; ++r) x[r] = to_float(rows[r][k]);
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const float w = columns[c * len + k];
+#pragma unroll
+        for (int r = 0; r < kThinRows; ++r) acc[r][c] = fmaf(x[r], w, acc[r][c]);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < kThinRows; ++r)
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        float v = acc[r][c];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        if (lane == c && c < n && row0 + r < p.m)
+          finish1<T, kAnyActivation>(
+              p.e, row0 + r, c, p.n, v,
+              p.e.bias ? to_float(static_cast<const T*>(p.e.bias)[c]) : 0.f);
+      }
+  }
+}
+
 // ------------------------------------------------------- d = g act'(p) and sums of d
 // Bound by HBM.  A CTA owns a strip of columns and every gridDim.y-th block of rows; each
 // thread keeps its columns' sums in registers, and the CTA's partial row of db is joined
@@ -442,8 +502,9 @@ template <typename T, int V, int ACT>
 __global__ void __launch_bounds__(256) slope_kernel(const T* __restrict__ g, int64_t ldg,
                                                     const float* __restrict__ preact,
                                                     T* __restrict__ d, int64_t ldd,
-                                                    float* __restrict__ partial, int64_t m,
-                                                    int64_t n, int lanes) {
+                                                    float* __restrict__ partial,
+                                                    T* __restrict__ db, int64_t m, int64_t n,
+                                                    int lanes) {
   __shared__ float sums[256 * V];
   const int tx = threadIdx.x % lanes, ty = threadIdx.x / lanes, rows = 256 / lanes;
   const int64_t col = (static_cast<int64_t>(blockIdx.x) * lanes + tx) * V;
@@ -492,7 +553,8 @@ __global__ void __launch_bounds__(256) slope_kernel(const T* __restrict__ g, int
     if (at >= n) break;
     float total = 0.f;
     for (int q = 0; q < rows; ++q) total += sums[q * lanes * V + c];
-    partial[blockIdx.y * n + at] = total;
+    if (db != nullptr) db[at] = from_float<T>(total);
+    else partial[blockIdx.y * n + at] = total;
   }
 }
 
@@ -653,6 +715,14 @@ int launch_product(const ProductArgs& p, int device, cudaStream_t stream) {
   return e == cudaSuccess ? ICTC_OK : cuda_fail(e, "linear product launch");
 }
 
+int thin_columns(int64_t n) { return n == 1 ? 1 : n <= 4 ? 4 : kThinColumns; }
+
+// Few columns, held in shared memory, and enough rows to fill the SMs without splitting K.
+bool few_columns(int64_t m, int64_t n, int64_t k) {
+  return n <= kThinColumns && m >= 4096 &&
+         k <= static_cast<int64_t>(kThinBytes / sizeof(float)) / thin_columns(n);
+}
+
 template <typename T>
 bool vec_epilogue(const Epilogue& e, int64_t n) {
   return n % 4 == 0 && aligned(e.out, 4 * sizeof(T)) &&
@@ -675,6 +745,27 @@ int run_product(const T* a, int64_t lda, const T* b, int64_t ldb, int64_t m, int
     const cudaError_t err = cudaGetLastError();
     return err == cudaSuccess ? ICTC_OK : cuda_fail(err, "linear split join launch");
   };
+  if constexpr (!A_MN) {
+    if (few_columns(m, n, k) && !chunk_aligned(a, lda, sizeof(T))) {
+      ProductArgs p{};
+      p.a = a; p.b = b;
+      p.m = m; p.n = n; p.k = k;
+      p.lda = lda; p.ldb = ldb;
+      p.e = e;
+      const size_t bytes = static_cast<size_t>(thin_columns(n)) * k * sizeof(float);
+      const int64_t resident = bytes <= 48 * 1024 ? 4 : bytes <= 96 * 1024 ? 2 : 1;
+      const int64_t want = ceil_div(m, 8 * kThinRows), cap = sm_count(device) * resident;
+      const unsigned grid = static_cast<unsigned>(want < cap ? want : cap);
+      const auto kernel = n == 1   ? few_columns_kernel<T, B_MN, 1>
+                          : n <= 4 ? few_columns_kernel<T, B_MN, 4>
+                                   : few_columns_kernel<T, B_MN, kThinColumns>;
+      const int st = allow_smem(reinterpret_cast<const void*>(kernel), bytes);
+      if (st != ICTC_OK) return st;
+      kernel<<<grid, 256, bytes, stream>>>(p);
+      const cudaError_t err = cudaGetLastError();
+      return err == cudaSuccess ? ICTC_OK : cuda_fail(err, "linear few-column launch");
+    }
+  }
   if constexpr (sizeof(T) == 2) {
     const PairPlan q = plan_pair(m, n, k, device);
     OperandMaps maps;
@@ -822,7 +913,8 @@ LinearPlan plan_linear(int64_t m, int64_t n, int64_t k, int dtype, int activatio
   b.few = !backward && m <= kFewRows;
   b.narrow = !b.few && (layout & ICTC_LINEAR_PACKED) && n <= kNarrow && k <= kNarrow &&
              m <= (1ll << 36);
-  b.align = !(layout & ICTC_LINEAR_ALIGNED) && worth_aligning(m, n, k);
+  b.align = !(layout & ICTC_LINEAR_ALIGNED) && worth_aligning(m, n, k) &&
+            (backward || !few_columns(m, n, k));
   size_t at = 0;
   const auto take = [&](size_t bytes) {
     const size_t here = at;
@@ -929,7 +1021,7 @@ int run_linear_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, E
     return launch_few_rows<T, 1>(xt, ldx, wt, ldw, m, n, k, e, stream);
   }
   if (plan.narrow) return run_narrow_forward<T>(xt, wt, ldw, e, m, n, k, stream);
-  if (plan.align) {
+  if (plan.align) {  // never with few columns
     int st = align_operand(&xt, &ldx, m, k, workspace + plan.x, stream);
     if (st == ICTC_OK) st = align_operand(&wt, &ldw, n, k, workspace + plan.w, stream);
     if (st != ICTC_OK) return st;
@@ -955,6 +1047,7 @@ SlopePlan plan_slope(int64_t m, int64_t n, int vec) {
   int64_t y = ceil_div(148 * 8, s.blocks_x);
   if (y > kSlopeParts) y = kSlopeParts;
   if (y > row_blocks) y = row_blocks;
+  if (m <= 1024) y = 1;  // short sums are finished where they are formed
   s.blocks_y = static_cast<unsigned>(y < 1 ? 1 : y);
   return s;
 }
@@ -982,17 +1075,18 @@ int run_linear_backward(const void* x, int64_t ldx, const void* w, int64_t ldw,
     const bool vec = n % kFull == 0 && chunk_aligned(g, ldg, sizeof(T)) && aligned(preact, 16);
     const SlopePlan s = plan_slope(m, n, vec ? kFull : 1);
     const dim3 grid(s.blocks_x, s.blocks_y);
+    T* db_out = s.blocks_y == 1 ? static_cast<T*>(db) : nullptr;  // no partial rows to join
     for_activation(activation, [&](auto act) {
       if (vec)
         slope_kernel<T, kFull, act.value><<<grid, 256, 0, stream>>>(d, ldg, preact, d_out, d_pitch,
-                                                                    columns, m, n, s.lanes);
+                                                                    columns, db_out, m, n, s.lanes);
       else
         slope_kernel<T, 1, act.value><<<grid, 256, 0, stream>>>(d, ldg, preact, d_out, d_pitch,
-                                                                columns, m, n, s.lanes);
+                                                                columns, db_out, m, n, s.lanes);
     });
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return cuda_fail(e, "linear slope launch");
-    if (db) {
+    if (db && !db_out) {
       column_total_kernel<T><<<dim3(static_cast<unsigned>(ceil_div(n, 32))),
                                dim3(32, kColumnLanes), 0, stream>>>(
           columns, columns, static_cast<T*>(db), static_cast<T*>(db), s.blocks_y, n);

@@ -111,7 +111,8 @@ LINEAR_SHAPES = [
     (1, 1, 1), (1, 64, 64), (3, 7, 5), (4, 129, 1), (5, 8, 64), (37, 8, 64), (127, 63, 65),
     (128, 64, 128), (129, 65, 127), (200, 257, 3), (255, 16, 130), (300, 1000, 72), (64, 2049, 33),
     (1000, 33, 200), (2500, 64, 64), (5000, 7, 3), (3000, 64, 1), (129, 1, 64), (513, 61, 59),
-    (6, 16, 16), (700, 1025, 769), (2053, 211, 333),
+    (6, 16, 16), (700, 1025, 769), (2053, 211, 333), (4097, 702, 6), (5000, 1536, 8), (4100, 1030, 1),
+    (4500, 3, 130), (4099, 8, 520),
 ]
 
 
