@@ -1,7 +1,8 @@
 """ctypes binding of libictc_o2_b200.so, the C-ABI declared in include/ictc_o2_b200.h.
 
-This is the only place Python touches the native library.  A missing library is a
-hard error: the package has no CPU or PyTorch fallback for the kernels.
+This is the only place the package loads the native library (``dense`` hands the
+addresses of its entry points to the dense operators' C++ autograd module).  A missing
+library is a hard error: the package has no CPU or PyTorch fallback for the kernels.
 """
 
 from __future__ import annotations

@@ -8,11 +8,22 @@
 // eight significant bits each (x = x1 + x2 + x3, by truncation), and six of the nine
 // partial products are summed:
 //   a b ~ a1 b1 + (a1 b2 + a2 b1 + a2 b2 + a1 b3 + a3 b1)
-// the three left out are below 2^-22 of |a b|, 2^-24 on average.  The tensor core truncates when it adds
-// to an accumulator, so the large first term and the small others have accumulators of
-// their own, and both are moved into registers and added there, rounded to nearest,
-// every 256 elements of K.  An infinity or NaN in an operand cannot be cut; it makes the
-// element NaN or infinite, and such elements are summed again one FMA at a time.
+// The three left out are each below 2^-22 of |a b|, and mostly far below.  The tensor core
+// truncates when it adds to an accumulator, so the large first term and the small others
+// have accumulators of their own, and both are moved into registers and added there,
+// rounded to nearest, every 256 elements of K: errors against 64 bits are those of a
+// float32 product or smaller (2e-7 to 4e-7 in the 2-norm over the measured sizes).  An
+// infinity or NaN in an operand cannot be cut; it makes the element NaN or infinite, and
+// such elements are summed again one FMA at a time.
+//
+// Which kernel a product takes:
+//   up to 64 inputs and outputs, contiguous     one kernel per direction (dense_narrow.cuh)
+//   up to 4 rows (forward)                      FMAs, W read once (few_rows_kernel)
+//   up to 8 columns over unaligned rows         FMAs, A read once (few_columns_kernel)
+//   16-bit, aligned rows                        SM pairs fed by TMA (dense_pair.cuh)
+//   float32, aligned rows                       cut on the way in (dense_cut.cuh)
+//   anything else: small or unaligned           register-staged operands (product_kernel);
+//                                               large ones are copied to aligned rows first
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -153,6 +164,7 @@ __device__ __forceinline__ void issue_stage(uint32_t sa, uint32_t d, int steps, 
 }
 
 // ---------------------------------------------------------------------- the product
+// For operands that TMA cannot address (and 16-bit products below a tile of work).
 // One persistent CTA per SM, warps specialised: 8 producer warps load operand chunks
 // into registers, cut float32 values and store the swizzled tiles; one of their threads
 // issues the MMAs of a stage; 8 epilogue warps move finished accumulators out of TMEM, which holds

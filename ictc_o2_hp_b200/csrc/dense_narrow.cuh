@@ -155,9 +155,13 @@ __device__ __forceinline__ void read_unit(const Slice<T>& s, int r, int u, float
       if constexpr (sizeof(T) == 4)
         asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
                      : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3])
-                     : "r"(at));
+                     : "r"(at)
+                     : "memory");
       else
-        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(q[0]), "=r"(q[1]) : "r"(at));
+        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];"
+                     : "=r"(q[0]), "=r"(q[1])
+                     : "r"(at)
+                     : "memory");
     }
     const Pack<T, 4>& pk = *reinterpret_cast<const Pack<T, 4>*>(q);
 #pragma unroll
@@ -240,6 +244,16 @@ struct SliceWalk {
     }
   }
 };
+
+// A producer warp is done with a slot.  `seen` holds bits of every value that the lane read
+// from it, and the arrival depends on it: the assembler had moved reads whose values were
+// used later behind a plain arrival, where the next copy overwrote the slot first (one row
+// in some hundred thousand of the forward was another slice's).  The pattern is that of no
+// finite value, and lanes agree on it only if all 32 hold it.
+__device__ __forceinline__ void release_slot(uint64_t* bar, uint32_t seen, int lane) {
+  const uint32_t alike = __ballot_sync(0xffffffffu, seen == 0xffedcba9u);
+  if (lane == (alike == 0xffffffffu ? 1 : 0)) mbar_arrive(bar);
+}
 
 // Copies in flight land before the CTA goes away (after a wait ran out).
 __device__ __forceinline__ void settle_copies() {
@@ -377,17 +391,20 @@ __global__ void __launch_bounds__(kNarrowThreadsL, 1)
           slice.copied = static_cast<int>(slice_bytes<T>(p.k, slice.rows) / sizeof(T));
         }
         float v[4][4];
+        uint32_t seen = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) read_unit<PLAIN>(slice, r0 + 8 * j, unit, v[j]);
-        if (some) {
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&raw_empty[slot]);
-          ++n;
+        for (int j = 0; j < 4; ++j) {
+          read_unit<PLAIN>(slice, r0 + 8 * j, unit, v[j]);
+          seen |= __float_as_uint(v[j][0]);
         }
         if (unit < 4 * steps)
 #pragma unroll
           for (int j = 0; j < 4; ++j)
             store_unit<T>(tile, kPiece, q * kSliceRows + r0 + 8 * j, unit, v[j]);
+        if (some) {
+          release_slot(&raw_empty[slot], seen, lane);
+          ++n;
+        }
       }
       if (!ok) break;
       fence_proxy_async();
@@ -623,6 +640,7 @@ __global__ void __launch_bounds__(kNarrowThreadsL, 1)
           sp = {reinterpret_cast<const float*>(from + 2 * kSliceX<T>), p.preact + at.row() * p.n,
                 p.n, rows, static_cast<int>(slice_bytes<float>(p.n, rows) / sizeof(float))};
         }
+        uint32_t seen = 0;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           read_unit<PLAIN>(sx, r0 + 16 * j, unit, xv[2 * q + j]);
@@ -636,10 +654,10 @@ __global__ void __launch_bounds__(kNarrowThreadsL, 1)
           }
 #pragma unroll
           for (int i = 0; i < 4; ++i) db[i] += d[i];
+          seen |= __float_as_uint(xv[2 * q + j][0]) | __float_as_uint(d[0]);
         }
         if (some) {
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&raw_empty[slot]);
+          release_slot(&raw_empty[slot], seen, lane);
           ++n;
         }
       }

@@ -8,7 +8,7 @@
 // Both passes are bound by HBM: 2 (forward) or 3 (backward) values of the operand type
 // move per element.  A row is read once and kept in registers, so the centred sum of
 // squares is a second pass over registers and not over memory (no cancellation between
-// sum x^2 and mean^2).  Narrow rows belong to 4 to 32 lanes of a warp that load them
+// sum x^2 and mean^2).  Narrow rows belong to up to 32 lanes of a warp that load them
 // directly; wider rows to a whole CTA that takes them from a ring of shared-memory
 // stages filled by bulk copies several rows ahead, because a CTA that loads, reduces and
 // stores in turn leaves too few bytes in flight.  CTAs are persistent over rows: weights

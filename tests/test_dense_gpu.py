@@ -174,6 +174,27 @@ def test_linear_larger(shape, dtype, cuda_device):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+def test_linear_narrow_many_tiles(dtype, cuda_device):
+    """Many tiles per CTA: a stage that is written again while it is still read shows as
+    another tile's rows, in a few rows of a million."""
+    from ictc_o2_hp_b200 import dense
+    m, k, n = 700001, 64, 64
+    x = rand((m, k), dtype, cuda_device, 71)
+    w = rand((n, k), dtype, cuda_device, 72, 0.2)
+    g = rand((m, n), dtype, cuda_device, 73)
+    p = x.double() @ w.double().t()
+    bound = sum_error(k) * (x.double().abs() @ w.double().abs().t())
+    within("y", dense.linear(x, w), p, bound + (UNIT[dtype] + 2 * U) * p.abs() + TINY[dtype])
+    leaves = [t.clone().requires_grad_(True) for t in (x, w)]
+    first = None
+    for _ in range(8):
+        y = dense.linear(*leaves, activation="silu", residual=g)
+        out = (y.detach(), *torch.autograd.grad(y, leaves, g))
+        first = out if first is None else first
+        assert all(torch.equal(a, b) for a, b in zip(out, first))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_linear_strides_and_batches(dtype, cuda_device):
     """Column slices (rows off every vector boundary), transposed weights, expanded
     gradients and leading batch dimensions."""
