@@ -14,7 +14,15 @@ from __future__ import annotations
 import torch
 
 from . import ops
+from .dense import Linear
 from .uvu import UvuTensorProduct
+
+
+def _check_affine(radial_out: torch.nn.Linear) -> None:
+    """The kernels read only weight and bias: an activation would be left out."""
+    if isinstance(radial_out, Linear) and radial_out.activation != "none":
+        raise ValueError("radial_out must be affine: its activation "
+                         f"{radial_out.activation!r} would not be applied")
 
 
 class RadialUvuTensorProduct(torch.nn.Module):
@@ -32,10 +40,12 @@ class RadialUvuTensorProduct(torch.nn.Module):
             raise ValueError("radial_out.out_features must equal tp.weight_numel")
         if radial_out.in_features < 1:
             raise ValueError("radial_out must have at least one input feature")
+        _check_affine(radial_out)
         self.tp = tp
         self.radial_out = radial_out
 
     def _rconfig(self):
+        _check_affine(self.radial_out)  # the module may have been changed or replaced
         c = self.tp._config
         return [c[0], c[2], c[3], c[4], c[5], c[6], c[7], self.radial_out.in_features]
 

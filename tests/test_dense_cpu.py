@@ -98,3 +98,32 @@ def test_linear_status_codes():
         assert backward(**bad) == _lib.ERR_INVALID, bad
     for bad in ({"space": None}, {"size": 16}, {"space": ctypes.c_void_p(264)}):
         assert backward(**bad) == _lib.ERR_WORKSPACE, bad
+
+
+def test_radial_product_refuses_an_activation():
+    """The radial product reads weight and bias of its affine layer and nothing else."""
+    from ictc_o2_hp_b200 import RadialUvuTensorProduct, UvuTensorProduct
+    tp = UvuTensorProduct(4, 1, 2, parity="full", parity_in2="canonical", shared_weights=False)
+    with pytest.raises(ValueError, match="activation"):
+        RadialUvuTensorProduct(tp, Linear(8, tp.weight_numel, activation="silu"))
+    model = RadialUvuTensorProduct(tp, Linear(8, tp.weight_numel))
+    args = [torch.randn(3, d) for d in (tp.input1_dimension, tp.input2_dimension, 8)]
+    model.radial_out.activation = "relu"
+    with pytest.raises(ValueError, match="activation"):
+        model(*args)
+    model.radial_out = torch.nn.Linear(8, tp.weight_numel)
+    with pytest.raises(TypeError):  # accepted; CPU tensors are refused by the kernels
+        model(*args)
+
+
+def test_radial_messages_refuse_an_activation():
+    from types import SimpleNamespace
+
+    from ictc_o2_hp_b200 import RadialUvuTensorProduct, UvuTensorProduct, graph
+    tp = UvuTensorProduct(4, 1, 2, parity="full", parity_in2="canonical", shared_weights=False)
+    model = RadialUvuTensorProduct(tp, Linear(8, tp.weight_numel))
+    model.radial_out.activation = "gelu"
+    edges = SimpleNamespace(num_nodes=2, num_edges=3, csr=lambda which: (None, None, None))
+    with pytest.raises(ValueError, match="activation"):
+        graph.radial_messages(model, torch.randn(2, tp.input1_dimension), edges,
+                              torch.randn(3, tp.input2_dimension), torch.randn(3, 8))
