@@ -176,6 +176,15 @@ __device__ __forceinline__ void read_unit(const Slice<T>& s, int r, int u, float
   }
 }
 
+// Bits of every value of a unit, for release_slot: a PLAIN unit is one access, whose first
+// value arrives with the other three; elsewhere each value has a load of its own.
+template <bool PLAIN>
+__device__ __forceinline__ uint32_t unit_bits(const float (&v)[4]) {
+  const uint32_t first = __float_as_uint(v[0]);
+  if constexpr (PLAIN) return first;
+  return first | __float_as_uint(v[1]) | __float_as_uint(v[2]) | __float_as_uint(v[3]);
+}
+
 // The `steps` K steps of one product with 64 columns; strides in the descriptors' units of
 // 16 bytes.  The parts of B lie behind one another as 192 columns, so that a part of A
 // meets all the parts of B that it needs in one MMA (an MMA is bound by its operands'
@@ -249,8 +258,8 @@ struct SliceWalk {
   }
 };
 
-// A producer warp is done with a slot.  `seen` holds bits of every value that the lane read
-// from it, and the arrival depends on it: the assembler had moved reads whose values were
+// A producer warp is done with a slot.  `seen` holds bits of every load that the lane made
+// from it (unit_bits), and the arrival depends on it: the assembler had moved reads whose values were
 // used later behind a plain arrival, where the next copy overwrote the slot first (one row
 // in some hundred thousand of the forward was another slice's).  The pattern is that of no
 // finite value, and lanes agree on it only if all 32 hold it.
@@ -399,7 +408,7 @@ __global__ void __launch_bounds__(kNarrowThreadsL, 1)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           read_unit<PLAIN>(slice, r0 + 8 * j, unit, v[j]);
-          seen |= __float_as_uint(v[j][0]);
+          seen |= unit_bits<PLAIN>(v[j]);
         }
         if (unit < 4 * steps)
 #pragma unroll
@@ -658,7 +667,7 @@ __global__ void __launch_bounds__(kNarrowThreadsL, 1)
           }
 #pragma unroll
           for (int i = 0; i < 4; ++i) db[i] += d[i];
-          seen |= __float_as_uint(xv[2 * q + j][0]) | __float_as_uint(d[0]);
+          seen |= unit_bits<PLAIN>(xv[2 * q + j]) | unit_bits<PLAIN>(d);  // d from g and p
         }
         if (some) {
           release_slot(&raw_empty[slot], seen, lane);

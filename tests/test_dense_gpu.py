@@ -195,6 +195,29 @@ def test_linear_narrow_many_tiles(dtype, cuda_device):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+def test_linear_narrow_many_odd_tiles(dtype, cuda_device):
+    """The same over rows that are not whole 16-byte blocks, whose values are read one by
+    one: every slot of the ring is written again many times."""
+    from ictc_o2_hp_b200 import dense
+    m, k, n = 700001, 61, 59
+    x = rand((m, k), dtype, cuda_device, 75)
+    w = rand((n, k), dtype, cuda_device, 76, 0.2)
+    g = rand((m, n), dtype, cuda_device, 77)
+    p = x.double() @ w.double().t()
+    bound = sum_error(k) * (x.double().abs() @ w.double().abs().t())
+    within("y", dense.linear(x, w), p, bound + (UNIT[dtype] + 2 * U) * p.abs() + TINY[dtype])
+    leaves = [t.clone().requires_grad_(True) for t in (x, w)]
+    first = None
+    for _ in range(8):
+        y = dense.linear(*leaves, activation="silu", residual=g)
+        out = (y.detach(), *torch.autograd.grad(y, leaves, g))
+        if first is None:
+            first = out
+            check_linear(x, w, None, g, "silu", g, out[0], out[1:], dtype)
+        assert all(torch.equal(a, b) for a, b in zip(out, first))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_linear_strides_and_batches(dtype, cuda_device):
     """Column slices (rows off every vector boundary), transposed weights, expanded
     gradients and leading batch dimensions."""
