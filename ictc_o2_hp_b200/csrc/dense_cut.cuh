@@ -104,30 +104,6 @@ __device__ __forceinline__ void load_raw(unsigned char* dst, const CUtensorMap* 
   else tma_load_2d(dst, map, k0, static_cast<int>(mn0), bar);
 }
 
-// The NaN and infinite elements of the block that write_block just wrote (lane = row;
-// the values are still in `mine`) again, by FMAs in K order: an infinity or NaN among a
-// float32 product's operands has no bf16 parts to speak of.  Rare, so kept out of line.
-template <bool A_MN, bool B_MN>
-__device__ __noinline__ void repair_block(const ProductArgs& p, int split, int64_t k0, int64_t k1,
-                                          const float* mine, int64_t row, int64_t col0, int lane) {
-  const float* a = static_cast<const float*>(p.a);
-  const float* b = static_cast<const float*>(p.b);
-  for (int c = 0; c < 32; ++c) {
-    const int64_t col = col0 + c;
-    const float v = mine[lane * 32 + (((c >> 2) ^ (lane & 7)) << 2) + (c & 3)];
-    if (row >= p.m || col >= p.n || isfinite(v)) continue;
-    float s = 0.f;
-    for (int64_t k = k0; k < k1; ++k)
-      s = fmaf(A_MN ? a[k * p.lda + row] : a[row * p.lda + k],
-               B_MN ? b[k * p.ldb + col] : b[col * p.ldb + k], s);
-    if (p.e.partial)
-      p.e.partial[(split * p.m + row) * p.n + col] = s;
-    else
-      finish1<float, kAnyActivation>(p.e, row, col, p.n, s,
-                                     p.e.bias ? static_cast<const float*>(p.e.bias)[col] : 0.f);
-  }
-}
-
 template <bool A_MN, bool B_MN, int BN, int ACT>
 __global__ void __launch_bounds__(kCutThreads, 1)
     cut_product_kernel(const __grid_constant__ OperandMaps maps,
@@ -301,17 +277,17 @@ __global__ void __launch_bounds__(kCutThreads, 1)
 #pragma unroll
         for (int j = 0; j < kHalf; j += 16) {
           float w[16], y[16];
-          tmem_load16(at + j, w);
           tmem_load16(at + BN + j, y);
-          tmem_load_wait();
-#pragma unroll
-          for (int i = 0; i < 16; ++i) w[i] += y[i];
           if constexpr (BN == 64) {
-            tmem_load16(at + 2 * BN + j, y);
+            tmem_load16(at + 2 * BN + j, w);
             tmem_load_wait();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) w[i] += y[i];
+            for (int i = 0; i < 16; ++i) y[i] += w[i];
           }
+          tmem_load16(at + j, w);
+          tmem_load_wait();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) w[i] = join_parts(w[i], y[i]);
 #pragma unroll
           for (int i = 0; i < 16; ++i) acc[j + i] = gi == 0 ? w[i] : acc[j + i] + w[i];
         }
@@ -323,15 +299,8 @@ __global__ void __launch_bounds__(kCutThreads, 1)
 #pragma unroll
       for (int cb = 0; cb < kHalf / 32; ++cb) {
         const int64_t col0 = pos.n0 + half * kHalf + cb * 32;
-        float zero = 0.f;  // stays 0 unless an element is not finite
-#pragma unroll
-        for (int i = 0; i < 32; ++i) zero = fmaf(acc[cb * 32 + i], 0.f, zero);
         stage_block(acc + cb * 32, mine, lane);
         write_staged<float, ACT, BN == 128>(p, pos.split, mine, row0, col0, lane, res);
-        if (__any_sync(0xffffffffu, zero != 0.f))
-          repair_block<A_MN, B_MN>(p, pos.split, h0 * kCutK, h1 * kCutK < p.k ? h1 * kCutK : p.k,
-                                   reinterpret_cast<const float*>(mine), row0 + lane, col0, lane);
-        __syncwarp();
       }
     }
   }

@@ -13,8 +13,11 @@
 // have accumulators of their own, and both are moved into registers and added there,
 // rounded to nearest, every 256 elements of K: errors against 64 bits are those of a
 // float32 product or smaller (2e-7 to 4e-7 in the 2-norm over the measured sizes).  An
-// infinity or NaN in an operand cannot be cut; it makes the element NaN or infinite, and
-// such elements are summed again one FMA at a time.
+// infinity or NaN in an operand is its own leading part, and decides an element through
+// the sum of a1 b1 alone (join_parts).  Two things are given up for that: an infinity that
+// meets a subnormal below 2^-133, whose leading part is zero, gives NaN; and a signalling
+// NaN with nothing in its upper seven bits of payload, which no arithmetic produces, counts
+// as an infinity.
 //
 // Which kernel a product takes:
 //   up to 64 inputs and outputs, contiguous     one kernel per direction (dense_narrow.cuh)
@@ -302,15 +305,17 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
         for (int j = 0; j < kHalf; j += 16) {
           float v[16];
           tmem_load16(at + j, v);
-          tmem_load_wait();
-#pragma unroll
-          for (int i = 0; i < 16; ++i) acc[j + i] = gi == 0 ? v[i] : acc[j + i] + v[i];
           if constexpr (P == 3) {
-            tmem_load16(at + BN + j, v);
+            float y[16];
+            tmem_load16(at + BN + j, y);
             tmem_load_wait();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) acc[j + i] += v[i];
+            for (int i = 0; i < 16; ++i) v[i] = join_parts(v[i], y[i]);
+          } else {
+            tmem_load_wait();
           }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[j + i] = gi == 0 ? v[i] : acc[j + i] + v[i];
         }
         tcgen05_fence_before();
         __syncwarp();
@@ -322,20 +327,6 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
         const int64_t col0 = pos.n0 + half * kHalf + cb * 32;
         write_block<T, ACT>(p, pos.split, acc + cb * 32, mine, row0, col0, lane, res);
         if (cb + 1 < kHalf / 32) load_residual(p, row0, col0 + 32, lane, res);
-        if constexpr (P == 3) {
-          float zero = 0.f;  // stays 0 unless an element is not finite
-#pragma unroll
-          for (int i = 0; i < 32; ++i) zero = fmaf(acc[cb * 32 + i], 0.f, zero);
-          if (__any_sync(0xffffffffu, zero != 0.f))
-            {
-              const int64_t k0 = static_cast<int64_t>(pos.c0) * kBK;
-              const int64_t k1 = static_cast<int64_t>(pos.c1) * kBK;
-              repair_block<A_MN, B_MN>(p, pos.split, k0, k1 < p.k ? k1 : p.k,
-                                       reinterpret_cast<const float*>(mine), row0 + lane, col0,
-                                       lane);
-            }
-          __syncwarp();
-        }
       }
     }
   }

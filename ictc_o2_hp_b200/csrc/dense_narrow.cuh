@@ -210,7 +210,7 @@ __device__ __forceinline__ void issue_cut(uint32_t d, uint64_t a, uint64_t a_ste
   }
 }
 
-// 32 columns of the warp's TMEM lanes, the sums of all orders together, smallest first.
+// 32 columns of the warp's TMEM lanes, the sums of all orders together.
 template <int P>
 __device__ __forceinline__ void take_sums(uint32_t at, float (&v)[32], bool add) {
 #pragma unroll
@@ -224,17 +224,10 @@ __device__ __forceinline__ void take_sums(uint32_t at, float (&v)[32], bool add)
     tmem_load_wait();
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const float sum = P == 3 ? w[i] + (y[i] + z[i]) : w[i];
+      const float sum = P == 3 ? join_parts(w[i], y[i] + z[i]) : w[i];
       v[j + i] = add ? v[j + i] + sum : sum;
     }
   }
-}
-
-__device__ __forceinline__ bool any_nonfinite(const float (&v)[32]) {
-  float zero = 0.f;  // stays 0 unless an element is not finite
-#pragma unroll
-  for (int i = 0; i < 32; ++i) zero = fmaf(v[i], 0.f, zero);
-  return zero != 0.f;
 }
 
 // The CTA's slices in order, for the thread that issues copies and for those that wait.
@@ -276,22 +269,6 @@ __device__ __forceinline__ void settle_copies() {
 }
 
 // ------------------------------------------------------------------------- forward
-
-// Elements of y that came out NaN or infinite, by FMAs in order (the values are in `mine`).
-__device__ __noinline__ void repair_narrow_forward(const NarrowArgs& p, const float* mine,
-                                                   int64_t row, int col0, int lane) {
-  const float* x = static_cast<const float*>(p.x);
-  const float* w = static_cast<const float*>(p.w);
-  for (int c = 0; c < 32; ++c) {
-    const int col = col0 + c;
-    const float v = mine[lane * 32 + (((c >> 2) ^ (lane & 7)) << 2) + (c & 3)];
-    if (row >= p.m || col >= p.n || isfinite(v)) continue;
-    float s = 0.f;
-    for (int k = 0; k < p.k; ++k) s = fmaf(x[row * p.k + k], w[col * p.ldw + k], s);
-    finish1<float, kAnyActivation>(p.e, row, col, p.n, s,
-                                   p.e.bias ? static_cast<const float*>(p.e.bias)[col] : 0.f);
-  }
-}
 
 template <typename T, int ACT, bool PLAIN>
 __global__ void __launch_bounds__(kNarrowThreadsL, 1)
@@ -447,17 +424,10 @@ __global__ void __launch_bounds__(kNarrowThreadsL, 1)
       tcgen05_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&room[s]);
-      const bool bad = P == 3 && any_nonfinite(acc);
       stage_block(acc, mine, lane);
       res = next;
       load_residual(o, row0 + static_cast<int64_t>(gridDim.x) * kNarrowTile, half * 32, lane, next);
       write_staged<T, ACT>(o, 0, mine, row0, half * 32, lane, res);
-      if constexpr (P == 3) {
-        if (__any_sync(0xffffffffu, bad))
-          repair_narrow_forward(p, reinterpret_cast<const float*>(mine), row0 + lane, half * 32,
-                                lane);
-        __syncwarp();
-      }
     }
   }
   tcgen05_fence_before();
@@ -469,41 +439,6 @@ __global__ void __launch_bounds__(kNarrowThreadsL, 1)
 }
 
 // ------------------------------------------------------------------------ backward
-
-template <int ACT>
-__device__ __forceinline__ float narrow_d(const NarrowArgs& p, int64_t at) {
-  const float g = static_cast<const float*>(p.g)[at];
-  return ACT == ICTC_ACT_NONE ? g : g * activation_slope<ACT>(p.preact[at]);
-}
-
-// As above for dx = d W.
-template <int ACT>
-__device__ __noinline__ void repair_narrow_dx(const NarrowArgs& p, const float* mine, int64_t row,
-                                              int col0, int lane) {
-  const float* w = static_cast<const float*>(p.w);
-  for (int c = 0; c < 32; ++c) {
-    const int col = col0 + c;
-    const float v = mine[lane * 32 + (((c >> 2) ^ (lane & 7)) << 2) + (c & 3)];
-    if (row >= p.m || col >= p.k || isfinite(v)) continue;
-    float s = 0.f;
-    for (int n = 0; n < p.n; ++n) s = fmaf(narrow_d<ACT>(p, row * p.n + n), w[n * p.ldw + col], s);
-    static_cast<float*>(p.e.out)[row * p.k + col] = s;
-  }
-}
-
-// One element of the CTA's d^T x, by FMAs over its rows in order.
-template <int ACT>
-__device__ __noinline__ float repair_narrow_dw(const NarrowArgs& p, int n, int k) {
-  const float* x = static_cast<const float*>(p.x);
-  float s = 0.f;
-  for (int t = blockIdx.x; t < p.tiles; t += gridDim.x)
-    for (int r = 0; r < kNarrowTile; ++r) {
-      const int64_t row = static_cast<int64_t>(t) * kNarrowTile + r;
-      if (row >= p.m) break;
-      s = fmaf(narrow_d<ACT>(p, row * p.n + n), x[row * p.k + k], s);
-    }
-  return s;
-}
 
 template <typename T, int ACT, bool PLAIN>
 __global__ void __launch_bounds__(kNarrowThreadsL, 1)
@@ -730,15 +665,8 @@ __global__ void __launch_bounds__(kNarrowThreadsL, 1)
             if (lane == 0) mbar_arrive(room);
           }
           if (half * 32 >= p.k) continue;
-          const bool bad = P == 3 && any_nonfinite(acc);
           stage_block(acc, mine, lane);
           write_staged<T, ICTC_ACT_NONE>(o, 0, mine, row0, half * 32, lane, none);
-          if constexpr (P == 3) {
-            if (__any_sync(0xffffffffu, bad))
-              repair_narrow_dx<ACT>(p, reinterpret_cast<const float*>(mine), row0 + lane,
-                                    half * 32, lane);
-            __syncwarp();
-          }
         }
       }
     }
@@ -751,12 +679,7 @@ __global__ void __launch_bounds__(kNarrowThreadsL, 1)
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
             const int k = half * 32 + i;
-            if (k < p.k) {
-              out[n * p.k + k] = dw[half][i];
-              if constexpr (P == 3) {
-                if (!isfinite(dw[half][i])) out[n * p.k + k] = repair_narrow_dw<ACT>(p, n, k);
-              }
-            }
+            if (k < p.k) out[n * p.k + k] = dw[half][i];
           }
     }
   }

@@ -24,7 +24,7 @@ __device__ __forceinline__ uint32_t swizzled(uint32_t r, uint32_t c) {
 }
 
 // The bf16 parts of two float32 values, eight significant bits each by truncation (the
-// three add up to the value exactly), the first value in the low half.
+// three add up to a finite value exactly), the first value in the low half.
 __device__ __forceinline__ void cut_pair(float x0, float x1, uint32_t (&part)[3]) {
   const uint32_t u0 = __float_as_uint(x0), u1 = __float_as_uint(x1);
   part[0] = __byte_perm(u0, u1, 0x7632);
@@ -37,6 +37,13 @@ __device__ __forceinline__ void cut_pair(float x0, float x1, uint32_t (&part)[3]
   const float2 s = __fadd2_rn(r, make_float2(__uint_as_float((v0 & 0xffff0000u) ^ 0x80000000u),
                                              __uint_as_float((v1 & 0xffff0000u) ^ 0x80000000u)));
   part[2] = __byte_perm(__float_as_uint(s.x), __float_as_uint(s.y), 0x7632);
+}
+
+// An element of a float32 product from its sums of leading parts (a1 b1) and of the others.
+// An infinity is its own leading part (a NaN too), its other parts are NaN: the first sum
+// alone has what a product in order gives, with its sign, and takes no others.
+__device__ __forceinline__ float join_parts(float leading, float others) {
+  return fabsf(leading) <= 3.402823466e38f ? leading + others : leading;
 }
 
 // Shared-memory matrix descriptor, 128-byte swizzle.  Groups of eight 128-byte rows are

@@ -309,6 +309,55 @@ def test_linear_nonfinite_gradients(shape, cuda_device):
         assert keep.any() and torch.equal(p[keep], r[keep])
 
 
+@pytest.mark.parametrize("shape", [(1048576, 64, 64), (262147, 61, 59), (65536, 128, 512),
+                                   (300000, 96, 72), (40000, 65, 30)])
+def test_linear_nonfinite_rows_of_many(shape, cuda_device):
+    """A row of NaN, an infinity: every weight gradient that they reach, over long sums, for
+    the cost of a clean step (the extra time allowed is that of launching it)."""
+    from ictc_o2_hp_b200 import _lib, dense
+    m, k, n = shape
+    x = rand((m, k), torch.float32, cuda_device, 58)
+    w = rand((n, k), torch.float32, cuda_device, 59, 1.5 / math.sqrt(k))
+    g = rand((m, n), torch.float32, cuda_device, 60)
+
+    def step(x, w, g):
+        leaves = [t.clone().requires_grad_(True) for t in (x, w)]
+        y = dense.linear(*leaves, activation="silu")
+        return y.detach(), *torch.autograd.grad(y, leaves, g)
+
+    def cost(*args):
+        start, stop = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        for i in range(6):
+            if i == 2:
+                start.record()
+            out = step(*args)
+        stop.record()
+        torch.cuda.synchronize()
+        return out, start.elapsed_time(stop) / 4
+
+    base, clean = cost(x, w, g)
+    x2 = x.clone()
+    x2[m // 2] = math.nan
+    (y, dx, dw), spent = cost(x2, w, g)
+    keep = torch.ones(m, dtype=torch.bool, device=cuda_device)
+    keep[m // 2] = False
+    assert y[m // 2].isnan().all() and dx[m // 2].isnan().all() and dw.isnan().all()
+    assert torch.equal(y[keep], base[0][keep]) and torch.equal(dx[keep], base[1][keep])
+    assert spent <= 2 * clean + 0.5, f"{spent:.2f} ms with a NaN row, {clean:.2f} without"
+    g2 = g.clone()
+    g2[m // 3, 5] = math.inf
+    (y, dx, dw), spent = cost(x, w, g2)
+    slope = torch.autograd.functional.jvp(
+        lambda p: p * torch.sigmoid(p), x[m // 3].double() @ w[5].double(),
+        torch.ones((), dtype=torch.float64, device=cuda_device))[1].sign()
+    assert torch.equal(dw[5], x[m // 3].sign() * math.inf * slope.float())
+    assert torch.equal(y, base[0])
+    assert dw[torch.arange(n, device=cuda_device) != 5].isfinite().all()
+    assert torch.equal(dx[m // 3], w[5].sign() * math.inf * slope.float())
+    assert spent <= 2 * clean + 0.5, f"{spent:.2f} ms with an infinity, {clean:.2f} without"
+    assert _lib.device_error() == 0
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_linear_empty_and_partial_gradients(dtype, cuda_device):
     from ictc_o2_hp_b200 import dense
