@@ -8,7 +8,8 @@
 // Both passes are bound by HBM: 2 (forward) or 3 (backward) values of the operand type
 // move per element.  A row is read once and kept in registers, so the centred sum of
 // squares is a second pass over registers and not over memory (no cancellation between
-// sum x^2 and mean^2).  Narrow rows belong to up to 32 lanes of a warp that load them
+// sum x^2 and mean^2); it also sums the deviations themselves, which corrects the mean by
+// what the first sum and 1 / C rounded away.  Narrow rows belong to up to 32 lanes of a warp that load them
 // directly; wider rows to a whole CTA that takes them from a ring of shared-memory
 // stages filled by bulk copies several rows ahead, because a CTA that loads, reduces and
 // stores in turn leaves too few bytes in flight.  CTAs are persistent over rows: weights
@@ -17,9 +18,10 @@
 // fixed order by column_total_kernel.  Rows wider than a CTA's registers hold take the
 // streaming kernels at the end, which read the row again for each pass.
 //
-// Measured: float32 1,048,576 x 64 forward 90 us (6.0 TB/s), backward 124 us (6.5 TB/s); bf16
-// 16,384 x 4,096 forward 62 us (4.3 TB/s), backward 77 us (5.3 TB/s); float32 65,536 x 896
-// forward 91 us (5.2 TB/s); f16 9,973 x 1,337 (no row on a 16-byte boundary) 37 and 38 us.
+// Measured: float32 1,048,576 x 64 forward 91 us (5.9 TB/s), backward 123 us (6.5 TB/s); bf16
+// 16,384 x 4,096 forward 69 us (3.9 TB/s), backward 75 us (5.4 TB/s); float32 65,536 x 896
+// forward 89 us (5.3 TB/s); f16 9,973 x 1,337 (no row on a 16-byte boundary) 50 and 38 us.
+// The mean's correction is 7 of the 69 us.
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -59,13 +61,20 @@ __device__ __forceinline__ float group_sum(float v, int group, float* scratch) {
 }
 
 __device__ __forceinline__ float2 group_sum(float2 v, int group, float2* scratch) {
-  const int width = scratch ? 32 : group;
-  for (int o = width / 2; o > 0; o >>= 1) {
-    v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
-    v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
-  }
-  if (scratch) {
-    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
+  if (!scratch) {
+    for (int o = group / 2; o > 0; o >>= 1) {
+      v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+      v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+    }
+  } else {
+    // after one exchange the lower half warp adds x and the upper half y: five shuffles
+    // instead of ten, the same pairs
+    const int lane = threadIdx.x & 31;
+    const bool upper = lane >= 16;
+    float one = upper ? v.y : v.x;
+    one += __shfl_xor_sync(0xffffffffu, upper ? v.x : v.y, 16);
+    for (int o = 8; o > 0; o >>= 1) one += __shfl_xor_sync(0xffffffffu, one, o);
+    if ((lane & 15) == 0) reinterpret_cast<float*>(scratch)[threadIdx.x >> 4] = one;
     __syncthreads();
     v = make_float2(0.f, 0.f);
     for (int w = 0; w < group / 32; w += 2) {
@@ -152,17 +161,38 @@ __device__ __forceinline__ float2 centred(float2 v, float2 minus_mean, int q, in
   return d;
 }
 
-// (mean, 1 / standard deviation) of a row, whoever loaded it.
+// This thread's share of (sum d, sum d^2), d = v - mean.
 template <int V, int PAIRS>
-__device__ __forceinline__ float variance_sum(const float2 (&v)[PAIRS], float mean, int t,
-                                              int group, int width) {
-  float2 sq = both(0.f);
+__device__ __forceinline__ float2 deviation_sums(const float2 (&v)[PAIRS], float mean, int t,
+                                                 int group, int width) {
+  float2 sum = both(0.f), sq = both(0.f);
 #pragma unroll
   for (int q = 0; q < PAIRS; ++q) {
     const float2 d = centred<V>(v[q], both(-mean), q, t, group, width);
+    sum = add2(sum, d);
     sq = fma2(d, d, sq);
   }
-  return sq.x + sq.y;
+  return make_float2(sum.x + sum.y, sq.x + sq.y);
+}
+
+// A row's statistics: u = (x - mean) rstd + shift.
+struct Moments {
+  float mean, rstd, shift;
+};
+
+// From a first mean and the row's sums about it.  A mean that is off by delta = sum d / C
+// (1 / C is rounded, and so is the sum) would shift u by delta rstd: 0.9 for a constant row
+// of 896 values of 1e5.  What mean + delta rounds away stays in `shift`.
+__device__ __forceinline__ Moments moments_of(float first, float2 sums, float width, float inv,
+                                              float eps) {
+  const float delta = sums.x / width;
+  float var = sums.y * inv - delta * delta;
+  var = var < 0.f ? 0.f : var;  // a NaN stays
+  Moments m;
+  m.mean = first + delta;
+  m.rstd = 1.f / sqrtf(var + eps);
+  m.shift = ((m.mean - first) - delta) * m.rstd;
+  return m;
 }
 
 template <typename T, int V, int N>
@@ -200,10 +230,10 @@ __device__ __forceinline__ void store_row(T* row, int t, int group, int width, c
 template <typename T, int V, int N>
 __device__ __forceinline__ void store_normed(T* row, const float2 (&v)[kPairs<V, N>],
                                              const float2 (&w)[kPairs<V, N>],
-                                             const float2 (&b)[kPairs<V, N>], float mean,
-                                             float rstd, int t, int group, int width) {
+                                             const float2 (&b)[kPairs<V, N>],
+                                             const Moments& m, int t, int group, int width) {
   store_row<T, V, N>(row, t, group, width, [&](int q) {
-    return fma2(mul2(add2(v[q], both(-mean)), both(rstd)), w[q], b[q]);
+    return fma2(fma2(add2(v[q], both(-m.mean)), both(m.rstd), both(m.shift)), w[q], b[q]);
   });
 }
 
@@ -296,15 +326,17 @@ __global__ void __launch_bounds__(kNarrowThreads, 8) norm_forward(
     Held<T, V, N> row;
     load_row<T, V, N>(x, s.x_stride, r, r < s.rows, t, group, width, row);
     float2 v[kPairs<V, N>];
-    const float mean = group_sum(take_pairs(row, v), group, nullptr) * inv;
-    const float var =
-        group_sum(variance_sum<V>(v, mean, t, group, width), group, nullptr) * inv;
-    const float rstd = 1.f / sqrtf(var + s.eps);
+    const float first = group_sum(take_pairs(row, v), group, nullptr) * inv;
+    const Moments m =
+        moments_of(first,
+                   group_sum(deviation_sums<V>(v, first, t, group, width), group,
+                             static_cast<float2*>(nullptr)),
+                   static_cast<float>(width), inv, s.eps);
     if (r < s.rows) {
-      store_normed<T, V, N>(y + r * width, v, w, b, mean, rstd, t, group, width);
+      store_normed<T, V, N>(y + r * width, v, w, b, m, t, group, width);
       if (t == 0 && mean_out != nullptr) {
-        mean_out[r] = mean;
-        rstd_out[r] = rstd;
+        mean_out[r] = m.mean;
+        rstd_out[r] = m.rstd;
       }
     }
   }
@@ -496,7 +528,8 @@ __global__ void __launch_bounds__(kForwardThreads) norm_forward_ring(
     T* __restrict__ y, float* __restrict__ mean_out, float* __restrict__ rstd_out, NormShape s,
     Ring ring) {
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ __align__(16) float scratch[2][32];
+  __shared__ __align__(16) float sums[32];
+  __shared__ __align__(16) float2 deviations[32];
   __shared__ int failed[2];  // by the row's parity: a fast thread may be a row ahead
   const int group = blockDim.x, width = static_cast<int>(s.width), t = threadIdx.x;
   const float inv = 1.f / static_cast<float>(width);
@@ -505,7 +538,10 @@ __global__ void __launch_bounds__(kForwardThreads) norm_forward_ring(
   q.stride[0] = s.x_stride;
   q.rows = s.rows;
   q.width = width;
-  if (t < 64) (&scratch[0][0])[t] = 0.f;
+  if (t < 32) {
+    sums[t] = 0.f;
+    deviations[t] = both(0.f);
+  }
   ring_start(q, smem, ring, failed);
   float2 w[kPairs<V, N>], b[kPairs<V, N>];
   load_params<P, V, N>(weight, 1.f, t, group, width, w);
@@ -518,17 +554,17 @@ __global__ void __launch_bounds__(kForwardThreads) norm_forward_ring(
     Held<T, V, N> row;
     take_row<T, V, N>(q.stage(q.at), x, s.x_stride, r, s.rows, t, group, width, row);
     float2 v[kPairs<V, N>];
-    const float mean = group_sum(take_pairs(row, v), group, scratch[0]) * inv;
+    const float first = group_sum(take_pairs(row, v), group, sums) * inv;
     gone = failed[k] != 0;  // written before the barrier in group_sum: all threads agree
     if (gone) break;
     if (t == 0) q.fill(q.at, r + ahead);
-    const float var =
-        group_sum(variance_sum<V>(v, mean, t, group, width), group, scratch[1]) * inv;
-    const float rstd = 1.f / sqrtf(var + s.eps);
-    store_normed<T, V, N>(y + r * width, v, w, b, mean, rstd, t, group, width);
+    const Moments m = moments_of(
+        first, group_sum(deviation_sums<V>(v, first, t, group, width), group, deviations),
+        static_cast<float>(width), inv, s.eps);
+    store_normed<T, V, N>(y + r * width, v, w, b, m, t, group, width);
     if (t == 0 && mean_out != nullptr) {
-      mean_out[r] = mean;
-      rstd_out[r] = rstd;
+      mean_out[r] = m.mean;
+      rstd_out[r] = m.rstd;
     }
   }
   if (gone && t == 0) q.settle();
@@ -598,27 +634,30 @@ template <typename T, typename P>
 __global__ void __launch_bounds__(kStreamThreads) norm_forward_stream(
     const T* __restrict__ x, const P* __restrict__ weight, const P* __restrict__ bias,
     T* __restrict__ y, float* __restrict__ mean_out, float* __restrict__ rstd_out, NormShape s) {
-  __shared__ __align__(16) float scratch[2][32];
+  __shared__ __align__(16) float sums[32];
+  __shared__ __align__(16) float2 deviations[32];
   const float inv = 1.f / static_cast<float>(s.width);
   for (int64_t r = blockIdx.x; r < s.rows; r += gridDim.x) {
     const T* xr = x + r * s.x_stride;
     float sum = 0.f;
     for (int64_t c = threadIdx.x; c < s.width; c += kStreamThreads) sum += to_float(xr[c]);
-    const float mean = group_sum(sum, kStreamThreads, scratch[0]) * inv;
-    float sq = 0.f;
+    const float first = group_sum(sum, kStreamThreads, sums) * inv;
+    float2 about = both(0.f);
     for (int64_t c = threadIdx.x; c < s.width; c += kStreamThreads) {
-      const float d = to_float(xr[c]) - mean;
-      sq += d * d;
+      const float d = to_float(xr[c]) - first;
+      about.x += d;
+      about.y += d * d;
     }
-    const float var = group_sum(sq, kStreamThreads, scratch[1]) * inv;
-    const float rstd = 1.f / sqrtf(var + s.eps);
+    const Moments m = moments_of(first, group_sum(about, kStreamThreads, deviations),
+                                 static_cast<float>(s.width), inv, s.eps);
     for (int64_t c = threadIdx.x; c < s.width; c += kStreamThreads) {
       const float w = weight ? to_float(weight[c]) : 1.f, b = bias ? to_float(bias[c]) : 0.f;
-      y[r * s.width + c] = from_float<T>((to_float(xr[c]) - mean) * rstd * w + b);
+      const float u = fmaf(to_float(xr[c]) - m.mean, m.rstd, m.shift);
+      y[r * s.width + c] = from_float<T>(fmaf(u, w, b));
     }
     if (threadIdx.x == 0 && mean_out != nullptr) {
-      mean_out[r] = mean;
-      rstd_out[r] = rstd;
+      mean_out[r] = m.mean;
+      rstd_out[r] = m.rstd;
     }
   }
 }

@@ -490,6 +490,28 @@ def test_layer_norm_large_mean_and_constant_rows(cuda_device):
     assert torch.equal(dense.layer_norm(flat, None, b), b.expand(10, 64))
 
 
+@pytest.mark.parametrize("width", [3, 41, 300, 896, 1337, 5000, 20000])
+def test_layer_norm_mean_correction(width, cuda_device):
+    """The mean is that of the row, not a rounded sum times a rounded 1 / width: constant
+    rows give the bias, and rows far from zero are centred to the last bit that they hold.
+    The mean kept for the backward is off by at most its own rounding (U |mean|) and that of
+    sums over deviations, which stay below 2 sigma + 0.3 |mean| 2^-18 on average."""
+    from ictc_o2_hp_b200 import dense
+    b = rand((width,), torch.float32, cuda_device, 104)
+    for value in (0.1, 1000.0, 1e5, -12345.678):
+        flat = torch.full((7, width), value, device=cuda_device)
+        assert torch.equal(dense.layer_norm(flat, None, b), b.expand(7, width))
+    chain = (40 + width / 256) * U
+    for mean in (1000.0, 1e5):
+        x = rand((9, width), torch.float32, cuda_device, 105, 1.0, mean)
+        y, got_mean, got_rstd = dense._load().norm_forward(x, None, None, 1e-5)
+        want_mean, rstd, u = norm64(x, None, None, 1e-5, x)[:3]
+        spread = 2 / rstd.squeeze(-1) + 0.3 * mean * 2.0 ** -18
+        within("mean", got_mean, want_mean.squeeze(-1), 1.01 * U * mean + chain * spread)
+        within("rstd", got_rstd, rstd.squeeze(-1), 3 * chain * rstd.squeeze(-1))
+        within("y", y, u, chain * (2 + 0.3 * mean * 2.0 ** -18 * rstd + 4 * u.abs()))
+
+
 def test_layer_norm_empty_and_nonfinite(cuda_device):
     from ictc_o2_hp_b200 import dense
     w = torch.ones(8, device=cuda_device, requires_grad=True)
