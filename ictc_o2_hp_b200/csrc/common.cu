@@ -3,6 +3,7 @@
 
 #include <mutex>
 
+#include "smem_grants.h"
 #include "tmap.cuh"
 
 namespace ictc {
@@ -39,28 +40,16 @@ int sm_count(int device) {
 
 int allow_smem(const void* kernel, size_t bytes) {
   static std::mutex mu;
-  static const void* seen[256] = {};
-  static size_t granted[256] = {};
+  static SmemGrants grants;
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
   std::lock_guard<std::mutex> lock(mu);
-  int slot = -1;
-  for (int i = 0; i < 256; ++i) {
-    if (seen[i] == kernel) {
-      if (granted[i] >= bytes) return ICTC_OK;
-      slot = i;
-      break;
-    }
-    if (seen[i] == nullptr) {
-      slot = i;
-      break;
-    }
-  }
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             static_cast<int>(bytes));
+  if (grants.covers(device, kernel, bytes)) return ICTC_OK;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           static_cast<int>(bytes));
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(max dynamic smem)");
-  if (slot >= 0) {
-    seen[slot] = kernel;
-    granted[slot] = bytes;
-  }
+  grants.record(device, kernel, bytes);
   return ICTC_OK;
 }
 

@@ -31,7 +31,8 @@ int probe_take_device_error(int* code);
 int dense_take_device_error(int* code);
 int norm_take_device_error(int* code);
 
-// Opts a kernel into `bytes` of dynamic shared memory (cached per kernel).
+// Opts a kernel into `bytes` of dynamic shared memory on the current device (remembered
+// per device and kernel).
 int allow_smem(const void* kernel, size_t bytes);
 
 inline bool aligned(const void* p, uintptr_t bytes) {
