@@ -5,6 +5,11 @@
 // autograd.Function in Python over ctypes took 58 us a training call beside the engine's
 // own 65 us, more than the arithmetic of every call below about 10^9 operations.  The
 // kernel library is loaded by the Python package, which hands its entry points to bind().
+//
+// The functions work on the tensors' memory, past PyTorch's dispatcher.  Where something
+// watches the dispatcher (a trace, fake tensors, a functional transform) they go through
+// the registered custom operators instead, as under torch.compile.
+#include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
@@ -33,6 +38,32 @@ struct Api {
 };
 
 Api api{};
+
+// The custom operators in Python, which run the raw directions at the end of this file.
+struct Ops {
+  PyObject *norm_forward, *norm_backward, *linear_forward, *linear_backward;
+};
+
+Ops ops{};
+
+template <typename Result, typename... Args>
+Result through_dispatcher(PyObject* op, const Args&... args) {
+  const py::gil_scoped_acquire gil;
+  return py::reinterpret_borrow<py::object>(op)(args...).template cast<Result>();
+}
+
+// Whether a call on these tensors has to be seen by the dispatcher.
+bool watched(std::initializer_list<const Tensor*> tensors) {
+  using K = c10::DispatchKey;
+  constexpr c10::DispatchKeySet kWatchers(
+      {K::Python, K::Tracer, K::Functionalize, K::FuncTorchDynamicLayerFrontMode,
+       K::FuncTorchBatched, K::FuncTorchGradWrapper});
+  const auto local = c10::impl::tls_local_dispatch_key_set();
+  c10::DispatchKeySet keys = local.included_;
+  for (const Tensor* t : tensors)
+    if (t->defined()) keys = keys | t->key_set();
+  return !((keys - local.excluded_) & kWatchers).empty();
+}
 
 void check(int32_t status, const char* what) {
   if (status == ICTC_OK) return;
@@ -211,6 +242,11 @@ class LayerNormFunction : public torch::autograd::Function<LayerNormFunction> {
     const bool nb = ctx->saved_data["has_bias"].toBool() &&
                     ctx->needs_input_grad(weight.defined() ? 2 : 1);
     if (!at::GradMode::is_enabled()) {
+      if (watched({&grad, &x, &weight})) {
+        const auto [dx, dw, db] = through_dispatcher<std::tuple<Tensor, Tensor, Tensor>>(
+            ops.norm_backward, x, weight, saved[2], saved[3], grad, params == at::kFloat);
+        return {nx ? dx : Tensor(), nw ? dw : Tensor(), nb ? db : Tensor(), Tensor()};
+      }
       auto [dx, dw, db] =
           norm_backward(x, weight, saved[2], saved[3], grad, params, nx, nw, nb);
       return {dx, dw, db, Tensor()};
@@ -242,6 +278,9 @@ Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight_in,
                   const std::optional<Tensor>& bias_in, double eps) {
   const Tensor weight = wanted(weight_in), bias = wanted(bias_in);
   check_norm(x, weight, bias, eps);
+  if (watched({&x, &weight, &bias}))
+    return std::get<0>(through_dispatcher<std::tuple<Tensor, Tensor, Tensor>>(
+        ops.norm_forward, x, weight, bias, eps));
   if (any_grad({&x, &weight, &bias})) return LayerNormFunction::apply(x, given(weight), given(bias), eps);
   return std::get<0>(norm_forward(x, weight, bias, eps, false));
 }
@@ -357,6 +396,13 @@ class LinearFunction : public torch::autograd::Function<LinearFunction> {
     const Tensor dr = nr ? grad : Tensor();
     if (!nx && !nw && !nb) return {Tensor(), Tensor(), Tensor(), dr, Tensor()};
     if (!at::GradMode::is_enabled()) {
+      if (watched({&grad, &x, &weight})) {
+        const Tensor preact =
+            saved[3].defined() ? saved[3] : at::empty({0}, x.options().dtype(at::kFloat));
+        const auto [dx, dw, db] = through_dispatcher<std::tuple<Tensor, Tensor, Tensor>>(
+            ops.linear_backward, x, weight, preact, grad, code);
+        return {nx ? dx : Tensor(), nw ? dw : Tensor(), nb ? db : Tensor(), dr, Tensor()};
+      }
       auto [dx, dw, db] = linear_backward(x, weight, saved[3], grad, code, nx, nw, nb);
       return {dx, dw, db, dr, Tensor()};
     }
@@ -381,7 +427,11 @@ Tensor linear(const Tensor& x, const Tensor& weight, const std::optional<Tensor>
               const std::optional<Tensor>& residual_in, int64_t code) {
   const Tensor bias = wanted(bias_in), residual = wanted(residual_in);
   check_linear(x, weight, bias, residual, code);
-  if (any_grad({&x, &weight, &bias, &residual}))
+  const bool grad = any_grad({&x, &weight, &bias, &residual});
+  if (watched({&x, &weight, &bias, &residual}))
+    return std::get<0>(through_dispatcher<std::tuple<Tensor, Tensor>>(
+        ops.linear_forward, x, weight, bias, residual, code, grad && code != ICTC_ACT_NONE));
+  if (grad)
     return LinearFunction::apply(x, weight, given(bias), given(residual), code);
   return std::get<0>(linear_forward(x, weight, bias, residual, code, false));
 }
@@ -420,6 +470,13 @@ std::tuple<Tensor, Tensor, Tensor> linear_backward_op(const Tensor& x, const Ten
                          true, true);
 }
 
+// The custom operators, held for the life of the process.
+void bind_operators(py::object norm_fwd, py::object norm_bwd, py::object linear_fwd,
+                    py::object linear_bwd) {
+  ops = {norm_fwd.release().ptr(), norm_bwd.release().ptr(), linear_fwd.release().ptr(),
+         linear_bwd.release().ptr()};
+}
+
 // Entry points of the loaded kernel library, by address.
 void bind(uintptr_t last_error, uintptr_t norm_fwd, uintptr_t norm_ws, uintptr_t norm_bwd,
           uintptr_t linear_ws, uintptr_t linear_fwd, uintptr_t linear_bwd) {
@@ -437,6 +494,7 @@ void bind(uintptr_t last_error, uintptr_t norm_fwd, uintptr_t norm_ws, uintptr_t
 
 PYBIND11_MODULE(_dense_autograd, m) {
   m.def("bind", &bind);
+  m.def("bind_operators", &bind_operators);
   m.def("layer_norm", &layer_norm);
   m.def("linear", &linear);
   m.def("norm_forward", &norm_forward_op);

@@ -54,11 +54,12 @@ def _load():
                  "ictc_o2_layer_norm_backward", "ictc_o2_linear_workspace",
                  "ictc_o2_linear_forward", "ictc_o2_linear_backward")
         module.bind(*(ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in names))
+        module.bind_operators(_norm_op, _norm_grad_op, _linear_op, _linear_grad_op)
         _native = module
     return _native
 
 
-# ------------------------------------------------- custom operators, for torch.compile
+# ------------------- custom operators, for torch.compile and whatever watches the dispatcher
 
 
 @torch.library.custom_op(f"{NAMESPACE}::layer_norm_forward", mutates_args=())

@@ -127,3 +127,17 @@ def test_radial_messages_refuse_an_activation():
     with pytest.raises(ValueError, match="activation"):
         graph.radial_messages(model, torch.randn(2, tp.input1_dimension), edges,
                               torch.randn(3, tp.input2_dimension), torch.randn(3, 8))
+
+
+def test_fake_tensors_go_through_the_custom_operators():
+    """Shapes and types propagate without memory (the forward; autograd's engine wants a
+    device of the tensors' type)."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        x = torch.empty(3, 7, 16, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+        w = torch.empty(24, 16, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+        scale = torch.empty(24, device="cuda", requires_grad=True)
+        y = dense.layer_norm(dense.linear(x, w, activation="silu"), scale)
+        assert y.shape == (3, 7, 24) and y.dtype == torch.bfloat16 and y.device.type == "cuda"
+        with pytest.raises(ValueError):
+            dense.linear(x, w[:, :5])

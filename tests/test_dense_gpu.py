@@ -692,6 +692,58 @@ def test_compile_fullgraph(cuda_device):
     assert all(torch.equal(p, q) for p, q in zip(got, want))
 
 
+def test_traces_record_the_operators(cuda_device):
+    """torch.jit.trace and make_fx see the operators: a replay on other inputs computes with
+    those."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    from ictc_o2_hp_b200 import dense
+    w = rand((32, 32), torch.float32, cuda_device, 2, 0.2)
+    b = rand((32,), torch.float32, cuda_device, 3)
+    first, second = (rand((50, 32), torch.float32, cuda_device, s) for s in (4, 5))
+    g = rand((50, 32), torch.float32, cuda_device, 6)
+
+    def block(x):
+        return dense.linear(dense.layer_norm(x, None, b), w, b, "silu", x)
+
+    def step(x):
+        y = block(x)
+        return y, torch.autograd.grad(y, x, g)[0]
+
+    want = step(second.clone().requires_grad_(True))
+    traced = torch.jit.trace(block, (first.clone().requires_grad_(True),), check_trace=False)
+    leaf = second.clone().requires_grad_(True)
+    y = traced(leaf)
+    assert torch.equal(y, want[0])
+    assert torch.equal(torch.autograd.grad(y, leaf, g)[0], want[1])
+    recorded = make_fx(step)(first.clone().requires_grad_(True))
+    got = recorded(second.clone().requires_grad_(True))
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+    # the backward alone is watched: its nodes were made outside
+    leaf = second.clone().requires_grad_(True)
+    y = block(leaf)
+    back = make_fx(lambda g: torch.autograd.grad(y, leaf, g, retain_graph=True)[0])(g.clone())
+    twice = torch.autograd.grad(y, leaf, 2 * g)[0]
+    assert torch.equal(back(2 * g), twice) and not torch.equal(twice, want[1])
+    with pytest.raises(RuntimeError):  # custom operators have no rules for these transforms
+        torch.func.grad(lambda x: (block(x) * g).sum())(second)
+    batches = second.reshape(5, 10, 32)
+    assert torch.equal(torch.func.vmap(block)(batches), torch.stack([block(t) for t in batches]))
+
+
+def test_fake_tensors_forward_and_backward(cuda_device):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    from ictc_o2_hp_b200 import dense
+    with FakeTensorMode():
+        x = torch.empty(3, 7, 16, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+        w = torch.empty(24, 16, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+        scale = torch.empty(24, device="cuda", requires_grad=True)
+        y = dense.layer_norm(dense.linear(x, w, activation="silu"), scale)
+        grads = torch.autograd.grad(y, (x, w, scale), torch.empty_like(y))
+        assert [(g.shape, g.dtype) for g in grads] == [(t.shape, t.dtype) for t in (x, w, scale)]
+
+
 def test_refusals(cuda_device):
     from ictc_o2_hp_b200 import dense
     x = torch.randn(4, 6, device=cuda_device)
