@@ -418,7 +418,8 @@ class LinearFunction : public torch::autograd::Function<LinearFunction> {
       return linear(a, b, std::nullopt, std::nullopt, ICTC_ACT_NONE);
     };
     return {nx ? product(d, weight.t()).reshape(x.sizes()) : Tensor(),
-            nw ? product(d.t(), rows.t()) : Tensor(),
+            // a sum over no rows is no linear layer, but has its (zero) value and graph
+            nw ? (rows.size(0) > 0 ? product(d.t(), rows.t()) : at::matmul(d.t(), rows)) : Tensor(),
             nb ? d.to(at::kFloat).sum(0).to(x.scalar_type()) : Tensor(), dr, Tensor()};
   }
 };

@@ -377,6 +377,25 @@ def test_linear_empty_and_partial_gradients(dtype, cuda_device):
         assert torch.equal(alone, full[i])
 
 
+@pytest.mark.parametrize("act", ["none", "silu"])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_empty_batch_with_create_graph(dtype, act, cuda_device):
+    """No rows, gradients that are differentiated again: zeros, as without create_graph."""
+    from ictc_o2_hp_b200 import dense
+    w = rand((6, 5), dtype, cuda_device, 65).requires_grad_(True)
+    b = rand((6,), dtype, cuda_device, 66).requires_grad_(True)
+    scale = rand((6,), dtype, cuda_device, 67).requires_grad_(True)
+    x = torch.empty(0, 5, dtype=dtype, device=cuda_device, requires_grad=True)
+    leaves = (x, w, b, scale)
+    y = dense.layer_norm(dense.linear(x, w, b, act), scale)
+    first = torch.autograd.grad(y, leaves, torch.empty_like(y), create_graph=True)
+    assert [g.shape for g in first] == [t.shape for t in leaves]
+    assert not any(g.any() for g in first)
+    total = sum((g.float() ** 2).sum() for g in first)
+    second = torch.autograd.grad(total, leaves, allow_unused=True)
+    assert all(g is None or (g.shape == t.shape and not g.any()) for g, t in zip(second, leaves))
+
+
 # -------------------------------------------------------------------- layer norm
 
 
