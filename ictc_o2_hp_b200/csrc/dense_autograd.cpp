@@ -368,6 +368,18 @@ Tensor slope_formula(const Tensor& p, int64_t code) {
 Tensor linear(const Tensor& x, const Tensor& weight, const std::optional<Tensor>& bias_in,
               const std::optional<Tensor>& residual_in, int64_t code);
 
+// `value` with the derivatives of p, which has the same value but for its rounding.
+class ValueOf : public torch::autograd::Function<ValueOf> {
+ public:
+  static Tensor forward(AutogradContext*, const Tensor&, const Tensor& value) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    return at::alias(value);
+  }
+  static variable_list backward(AutogradContext*, variable_list grads) {
+    return {grads[0], Tensor()};
+  }
+};
+
 class LinearFunction : public torch::autograd::Function<LinearFunction> {
  public:
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight,
@@ -409,10 +421,13 @@ class LinearFunction : public torch::autograd::Function<LinearFunction> {
     // second derivatives: a differentiable composition whose products are linear layers
     // again, on the same kernels
     const Tensor rows = rows_of(x);
-    Tensor d = rows_of(grad);
+    Tensor d = rows_of(grad), wide = d.to(at::kFloat);
     if (code != ICTC_ACT_NONE) {
-      const Tensor p = linear(rows, weight, given(saved[2]), std::nullopt, ICTC_ACT_NONE).to(at::kFloat);
-      d = (d.to(at::kFloat) * slope_formula(p, code)).to(x.scalar_type());
+      // p again, for its graph; in 16-bit types it is rounded, so the float32 p that the
+      // forward kept is where the slope is taken, as in the kernels
+      const Tensor p = linear(rows, weight, given(saved[2]), std::nullopt, ICTC_ACT_NONE);
+      wide = wide * slope_formula(ValueOf::apply(p.to(at::kFloat), saved[3]), code);
+      d = wide.to(x.scalar_type());
     }
     const auto product = [](const Tensor& a, const Tensor& b) {
       return linear(a, b, std::nullopt, std::nullopt, ICTC_ACT_NONE);
@@ -420,7 +435,7 @@ class LinearFunction : public torch::autograd::Function<LinearFunction> {
     return {nx ? product(d, weight.t()).reshape(x.sizes()) : Tensor(),
             // a sum over no rows is no linear layer, but has its (zero) value and graph
             nw ? (rows.size(0) > 0 ? product(d.t(), rows.t()) : at::matmul(d.t(), rows)) : Tensor(),
-            nb ? d.to(at::kFloat).sum(0).to(x.scalar_type()) : Tensor(), dr, Tensor()};
+            nb ? wide.sum(0).to(x.scalar_type()) : Tensor(), dr, Tensor()};
   }
 };
 

@@ -618,6 +618,53 @@ def test_second_derivatives(act, cuda_device):
         assert (p.double() - q).norm() <= 1e-5 * q.norm()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", ACTS)
+def test_create_graph_keeps_first_gradients(act, dtype, cuda_device):
+    """The gradients that are differentiated again keep the error bounds of those that are
+    not; p far from zero, where rounding it to 16 bits would move the slope."""
+    from ictc_o2_hp_b200 import dense
+    m, k, n = 150, 40, 72
+    x = rand((m, k), dtype, cuda_device, 16, 2.0).requires_grad_(True)
+    w = rand((n, k), dtype, cuda_device, 17, 0.3).requires_grad_(True)
+    b = rand((n,), dtype, cuda_device, 18).requires_grad_(True)
+    g = rand((m, n), dtype, cuda_device, 19)
+    y = dense.linear(x, w, b, act)
+    grads = torch.autograd.grad(y, (x, w, b), g, create_graph=True)
+    assert all(t.requires_grad for t in grads[:2])
+    check_linear(x.detach(), w.detach(), b.detach(), None, act, g, y.detach(),
+                 [t.detach() for t in grads], dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES[1:])
+@pytest.mark.parametrize("act", ACTS)
+def test_second_derivatives_16_bit(act, dtype, cuda_device):
+    """As above in 16-bit types: some six tensors between the operands and a second
+    derivative are rounded, and the squares double what is off: 16 u in the 2-norm."""
+    from ictc_o2_hp_b200 import dense
+    m, k, n = 50, 24, 40
+    base = [rand((m, k), dtype, cuda_device, 1), rand((n, k), dtype, cuda_device, 2, 0.3),
+            rand((n,), dtype, cuda_device, 3)]
+    g = rand((m, n), dtype, cuda_device, 6)
+
+    def loss(x, w, b, g, lin):
+        f = torch.autograd.grad((lin(x, w, b) * g).sum(), x, create_graph=True)[0]
+        return (f.float() ** 2).sum() if f.dtype != torch.float64 else (f ** 2).sum()
+
+    ours = [t.clone().requires_grad_(True) for t in base]
+    got = torch.autograd.grad(loss(*ours, g, lambda x, w, b: dense.linear(x, w, b, act)), ours,
+                              allow_unused=True)
+    wide = [t.double().requires_grad_(True) for t in base]
+    want = torch.autograd.grad(
+        loss(*wide, g.double(), lambda x, w, b: act64(x @ w.t() + b, act)), wide,
+        allow_unused=True)
+    for p, q in zip(got, want):
+        if q is None or not q.any():
+            assert p is None or not p.any()
+            continue
+        assert (p.double() - q).norm() <= 16 * UNIT[dtype] * q.norm()
+
+
 # ----------------------------------------------------------- modules, streams, compile
 
 
