@@ -95,6 +95,13 @@ void check_like(const char* what, const char* name, const Tensor& t, const Tenso
                     what, ": ", name, " is ", t.scalar_type(), ", the input ", x.scalar_type());
 }
 
+// A dual tensor's tangent would be left out without a word.
+void check_tangents(const char* what, std::initializer_list<const Tensor*> tensors) {
+  for (const Tensor* t : tensors)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), what,
+                                " has no forward-mode derivative");
+}
+
 void check_norm(const Tensor& x, const Tensor& weight, const Tensor& bias, double eps) {
   check_input("layer_norm", x);
   TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1,
@@ -278,6 +285,7 @@ Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight_in,
                   const std::optional<Tensor>& bias_in, double eps) {
   const Tensor weight = wanted(weight_in), bias = wanted(bias_in);
   check_norm(x, weight, bias, eps);
+  check_tangents("layer_norm", {&x, &weight, &bias});
   if (watched({&x, &weight, &bias}))
     return std::get<0>(through_dispatcher<std::tuple<Tensor, Tensor, Tensor>>(
         ops.norm_forward, x, weight, bias, eps));
@@ -443,6 +451,7 @@ Tensor linear(const Tensor& x, const Tensor& weight, const std::optional<Tensor>
               const std::optional<Tensor>& residual_in, int64_t code) {
   const Tensor bias = wanted(bias_in), residual = wanted(residual_in);
   check_linear(x, weight, bias, residual, code);
+  check_tangents("linear", {&x, &weight, &bias, &residual});
   const bool grad = any_grad({&x, &weight, &bias, &residual});
   if (watched({&x, &weight, &bias, &residual}))
     return std::get<0>(through_dispatcher<std::tuple<Tensor, Tensor>>(

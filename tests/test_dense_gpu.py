@@ -797,6 +797,29 @@ def test_traces_record_the_operators(cuda_device):
     assert torch.equal(torch.func.vmap(block)(batches), torch.stack([block(t) for t in batches]))
 
 
+def test_dual_tensors_are_refused(cuda_device):
+    """A tangent is not dropped silently, whichever operand carries it."""
+    from torch.autograd import forward_ad
+
+    from ictc_o2_hp_b200 import dense
+    x, w, r = (rand((6, 6), torch.float32, cuda_device, s) for s in (1, 2, 3))
+    b = rand((6,), torch.float32, cuda_device, 4)
+    linear = [x, w, b, "none", r]
+    for leaf in (False, True):
+        with forward_ad.dual_level():
+            for i in (0, 1, 2, 4):
+                args = list(linear)
+                args[i] = forward_ad.make_dual(args[i].clone().requires_grad_(leaf),
+                                               torch.ones_like(args[i]))
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    dense.linear(*args)
+            for i in range(3):
+                args = [x, b, b]
+                args[i] = forward_ad.make_dual(args[i].clone(), torch.ones_like(args[i]))
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    dense.layer_norm(*args)
+
+
 def test_fake_tensors_forward_and_backward(cuda_device):
     from torch._subclasses.fake_tensor import FakeTensorMode
 
