@@ -9,6 +9,7 @@
 // The functions work on the tensors' memory, past PyTorch's dispatcher.  Where something
 // watches the dispatcher (a trace, fake tensors, a functional transform) they go through
 // the registered custom operators instead, as under torch.compile.
+#include <ATen/autocast_mode.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -447,9 +448,30 @@ class LinearFunction : public torch::autograd::Function<LinearFunction> {
   }
 };
 
+// Under autocast, operands of different types take autocast's; equal ones are left alone.
+bool cast_mixed(std::initializer_list<Tensor*> tensors) {
+  const auto first = (*tensors.begin())->scalar_type();
+  bool mixed = false;
+  for (const Tensor* t : tensors) mixed |= t->defined() && t->scalar_type() != first;
+  if (!mixed || !at::autocast::is_autocast_enabled(at::kCUDA)) return false;
+  for (const Tensor* t : tensors) {
+    if (!t->defined()) continue;
+    const auto type = t->scalar_type();
+    if (!t->is_cuda() || (type != at::kFloat && type != at::kBFloat16 && type != at::kHalf))
+      return false;
+  }
+  const auto type = at::autocast::get_autocast_dtype(at::kCUDA);
+  for (Tensor* t : tensors)
+    if (t->defined()) *t = t->to(type);
+  return true;
+}
+
 Tensor linear(const Tensor& x, const Tensor& weight, const std::optional<Tensor>& bias_in,
               const std::optional<Tensor>& residual_in, int64_t code) {
   const Tensor bias = wanted(bias_in), residual = wanted(residual_in);
+  Tensor cast[4] = {x, weight, bias, residual};
+  if (cast_mixed({&cast[0], &cast[1], &cast[2], &cast[3]}))
+    return linear(cast[0], cast[1], given(cast[2]), given(cast[3]), code);
   check_linear(x, weight, bias, residual, code);
   check_tangents("linear", {&x, &weight, &bias, &residual});
   const bool grad = any_grad({&x, &weight, &bias, &residual});

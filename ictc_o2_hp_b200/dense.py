@@ -159,14 +159,27 @@ def layer_norm(x: Tensor, weight: Tensor | None = None, bias: Tensor | None = No
     return (_native or _load()).layer_norm(x, weight, bias, eps)
 
 
+def _cast_mixed(tensors: list) -> list:
+    """What csrc/dense_autograd.cpp does under autocast, where a compiler traces."""
+    given = [t for t in tensors if t is not None]
+    if torch.is_autocast_enabled("cuda") and len({t.dtype for t in given}) > 1 and all(
+            t.is_cuda and t.dtype in (torch.float32, torch.bfloat16, torch.float16)
+            for t in given):
+        dtype = torch.get_autocast_dtype("cuda")
+        return [t if t is None else t.to(dtype) for t in tensors]
+    return tensors
+
+
 def linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, activation: str = "none",
            residual: Tensor | None = None) -> Tensor:
     """act(x weight^T + bias) + residual: x [..., in], weight [out, in], bias [out],
-    residual [..., out]; activation one of ACTIVATIONS."""
+    residual [..., out]; activation one of ACTIVATIONS.  Under ``torch.autocast`` operands
+    of different types are cast to its type (equal ones are computed in their own)."""
     code = ACTIVATIONS.get(activation)
     if code is None:
         raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}, got {activation!r}")
     if torch.compiler.is_compiling():
+        x, weight, bias, residual = _cast_mixed([x, weight, bias, residual])
         save = code != 0 and torch.is_grad_enabled() and any(
             t is not None and t.requires_grad for t in (x, weight, bias, residual))
         return _linear_op(x, weight, bias, residual, code, save)[0]

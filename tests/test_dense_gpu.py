@@ -797,6 +797,32 @@ def test_traces_record_the_operators(cuda_device):
     assert torch.equal(torch.func.vmap(block)(batches), torch.stack([block(t) for t in batches]))
 
 
+def test_autocast_casts_operands_of_different_types(cuda_device):
+    """float32 parameters beside 16-bit activations, as torch.nn.Linear takes them under
+    autocast; without it, and for operands of one type, nothing changes."""
+    from ictc_o2_hp_b200 import Linear, dense
+    layer = Linear(24, 40, activation="silu").to(cuda_device)
+    x = rand((30, 24), torch.float16, cuda_device, 1).requires_grad_(True)
+    r = rand((30, 40), torch.float32, cuda_device, 2)
+    g = rand((30, 40), torch.bfloat16, cuda_device, 3)
+    with pytest.raises(ValueError):
+        layer(x, r)
+    args = [t.detach().bfloat16().requires_grad_(True) for t in (x, layer.weight, layer.bias)]
+    want = dense.linear(*args, "silu", r.bfloat16())
+    grads = torch.autograd.grad(want, args, g)
+    for run in (layer, torch.compile(layer, fullgraph=True, backend="aot_eager")):
+        with torch.autocast("cuda", torch.bfloat16):
+            y = run(x, r)
+        got = torch.autograd.grad(y, (x, layer.weight, layer.bias), g)
+        assert torch.equal(y, want)
+        assert [t.dtype for t in got] == [torch.float16, torch.float32, torch.float32]
+        assert all(torch.equal(p, q.to(p.dtype)) for p, q in zip(got, grads))
+    with torch.autocast("cuda", torch.bfloat16):
+        assert layer(x.float(), r).dtype == torch.float32
+        with pytest.raises(TypeError):
+            dense.linear(x.double(), layer.weight)
+
+
 def test_dual_tensors_are_refused(cuda_device):
     """A tangent is not dropped silently, whichever operand carries it."""
     from torch.autograd import forward_ad
