@@ -155,6 +155,29 @@ def test_linear_activations(act, dtype, cuda_device):
     check_linear(x.detach(), w.detach(), b.detach(), r, act, g, y.detach(), grads, dtype)
 
 
+@pytest.mark.parametrize("rows", [4, 5000])
+def test_gelu_to_float32_rounding(rows, cuda_device):
+    """gelu and its slope by themselves (one input and a weight of 1: p is exact), also in
+    the tail, where the normal tail Q is all there is: its exponential is off by 1.5 p^2 U
+    (the rounded argument) and 4 U, what multiplies it by some 12 U."""
+    from ictc_o2_hp_b200 import dense
+    p = torch.linspace(-8, 8, rows * 13, device=cuda_device).reshape(rows, 13)
+    x = p.reshape(-1, 1).clone().requires_grad_(True)
+    w = torch.ones(1, 1, device=cuda_device)
+    y = dense.linear(x, w, None, "gelu")
+    slope = torch.autograd.grad(y, x, torch.ones_like(y))[0]
+    q = x.detach().double()
+    tail = 0.5 * torch.special.erfc(q.abs() * math.sqrt(0.5))
+    off = tail * (16 + 3 * q * q) * U
+    below = 0.5 * torch.special.erfc(-q * math.sqrt(0.5))  # the distribution function
+    want = q * below
+    within("y", y.detach(), want, q.abs() * (off + U * (q > 0)) + 2 * U * want.abs())
+    density = torch.exp(-0.5 * q * q) / math.sqrt(2 * math.pi)
+    want = below + q * density
+    within("slope", slope, want, off + U * (q > 0) + q.abs() * density * (8 + 1.5 * q * q) * U +
+           2 * U * want.abs())
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("shape", [(16, 4096, 520), (700, 1024, 768), (4096, 256, 256),
                                    (20000, 64, 64), (33, 8200, 24), (40000, 24, 8)])
