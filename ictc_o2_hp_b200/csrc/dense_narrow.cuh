@@ -16,8 +16,8 @@
 // time (the tensor core truncates when it adds), and the CTAs' partial results are
 // summed in CTA order.
 //
-// float32, 1,048,576 x 64 x 64 with SiLU and residual: forward 201 us (x, r, y, p: 1.07 GB,
-// 5.3 TB/s), backward 270 us (x, g, p, dx: 1.07 GB, 4.0 TB/s), where the cutting of x and d by
+// float32, 1,048,576 x 64 x 64 with SiLU and residual: forward 194 us (x, r, y, p: 1.07 GB,
+// 5.5 TB/s), backward 270 us (x, g, p, dx: 1.07 GB, 4.0 TB/s), where the cutting of x and d by
 // the producer warps is what is left over HBM.
 #pragma once
 
@@ -215,16 +215,19 @@ template <int P>
 __device__ __forceinline__ void take_sums(uint32_t at, float (&v)[32], bool add) {
 #pragma unroll
   for (int j = 0; j < 32; j += 16) {
-    float w[16], y[16], z[16];
-    tmem_load16(at + j, w);
+    float w[16], y[16];
     if constexpr (P == 3) {
       tmem_load16(at + kNarrow + j, y);
-      tmem_load16(at + 2 * kNarrow + j, z);
+      tmem_load16(at + 2 * kNarrow + j, w);
+      tmem_load_wait();
+#pragma unroll
+      for (int i = 0; i < 16; ++i) y[i] += w[i];
     }
+    tmem_load16(at + j, w);
     tmem_load_wait();
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const float sum = P == 3 ? join_parts(w[i], y[i] + z[i]) : w[i];
+      const float sum = P == 3 ? join_parts(w[i], y[i]) : w[i];
       v[j + i] = add ? v[j + i] + sum : sum;
     }
   }
@@ -409,10 +412,11 @@ __global__ void __launch_bounds__(kNarrowThreadsL, 1)
     o.n = p.n;
     o.e = p.e;
     uint32_t it = 0;
-    // a tile's residual is loaded while the tile before it is finished
-    ResidualBlock<T> res, next;
+    // a tile's residual is loaded as soon as the tile before it is written, ahead of the wait
+    // for its products (earlier still, the registers of two residuals spill: 225 us)
+    ResidualBlock<T> res;
     load_residual(o, static_cast<int64_t>(blockIdx.x) * kNarrowTile + quad * 32, half * 32, lane,
-                  next);
+                  res);
     for (int t = blockIdx.x; t < p.tiles; t += gridDim.x, ++it) {
       const int s = it & 1;
       const int64_t row0 = static_cast<int64_t>(t) * kNarrowTile + quad * 32;
@@ -425,9 +429,8 @@ __global__ void __launch_bounds__(kNarrowThreadsL, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&room[s]);
       stage_block(acc, mine, lane);
-      res = next;
-      load_residual(o, row0 + static_cast<int64_t>(gridDim.x) * kNarrowTile, half * 32, lane, next);
       write_staged<T, ACT>(o, 0, mine, row0, half * 32, lane, res);
+      load_residual(o, row0 + static_cast<int64_t>(gridDim.x) * kNarrowTile, half * 32, lane, res);
     }
   }
   tcgen05_fence_before();

@@ -41,9 +41,10 @@ __device__ __forceinline__ void cut_pair(float x0, float x1, uint32_t (&part)[3]
 
 // An element of a float32 product from its sums of leading parts (a1 b1) and of the others.
 // An infinity is its own leading part (a NaN too), its other parts are NaN: the first sum
-// alone has what a product in order gives, with its sign, and takes no others.
+// alone has what a product in order gives, with its sign, and the NaN of the others is
+// replaced by a finite value.
 __device__ __forceinline__ float join_parts(float leading, float others) {
-  return fabsf(leading) <= 3.402823466e38f ? leading + others : leading;
+  return leading + fmaxf(others, -3.402823466e38f);
 }
 
 // Shared-memory matrix descriptor, 128-byte swizzle.  Groups of eight 128-byte rows are
