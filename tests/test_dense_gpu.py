@@ -517,6 +517,27 @@ def test_layer_norm_strides(width, dtype, cuda_device):
                    norm64(x, w, None, 1e-5, g)[6].to(dtype)), dtype, dtype)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("width", [24, 64, 1000, 8200])
+def test_layer_norm_parameter_gradients_over_strides(width, dtype, cuda_device):
+    """The column sums over row slices at every offset, an expanded row, expanded and sliced
+    gradients: blocks at the tensors' ends, strides of 0, rows wider than a CTA holds."""
+    from ictc_o2_hp_b200 import dense
+    big = rand((60, width + 9), dtype, cuda_device, 94, 1.0, 0.3)
+    wide = rand((60, width + 9), dtype, cuda_device, 95)
+    w = rand((width,), dtype, cuda_device, 96)
+    b = rand((width,), dtype, cuda_device, 97)
+    rows = [big[:, o:o + width] for o in (0, 1, 8)] + [big[:1, :width].expand(60, width)]
+    grads = [wide[:, o:o + width] for o in (0, 3, 8)] + [
+        wide[:1, 1:width + 1].expand(60, width), wide[:, :1].expand(60, width)]
+    for x in rows:
+        for g in grads:
+            leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]
+            y = dense.layer_norm(*leaves)
+            got = torch.autograd.grad(y, leaves, g)
+            check_norm(x, w, b, 1e-5, g, y.detach(), got, dtype, dtype)
+
+
 def test_layer_norm_large_mean_and_constant_rows(cuda_device):
     """A mean far above the spread loses only what float32 inputs lose; constant rows
     give the bias."""
