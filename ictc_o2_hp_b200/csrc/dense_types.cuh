@@ -119,7 +119,9 @@ __device__ __forceinline__ float activation_slope(float p, int any = ICTC_ACT_NO
     }
     case ICTC_ACT_GELU_TANH: {
       const float s = sigmoid(1.5957691216057308f * (p + 0.044715f * p * p * p));
-      return s + p * s * (1.f - s) * 1.5957691216057308f * (1.f + 0.134145f * p * p);
+      // s (1 - s) is 0 long before p^2 overflows, which would make a NaN of it
+      const float p2 = fminf(p * p, 1e30f);
+      return s + p * s * (1.f - s) * 1.5957691216057308f * fmaf(0.134145f, p2, 1.f);
     }
     default:
       return 1.f;

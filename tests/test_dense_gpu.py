@@ -178,6 +178,22 @@ def test_gelu_to_float32_rounding(rows, cuda_device):
            2 * U * want.abs())
 
 
+@pytest.mark.parametrize("rows", [3, 40, 700])
+@pytest.mark.parametrize("act", ACTS)
+def test_activations_far_from_zero(act, rows, cuda_device):
+    """Finite p up to the end of float32: the activation is p or 0, its slope 1 or 0."""
+    from ictc_o2_hp_b200 import dense
+    p = torch.tensor([200.0, 3e3, 1e10, 1e19, 5e19, 1e25, 1e38, 3.4e38], device=cuda_device)
+    p = torch.cat([p, -p]).repeat(rows, 1)
+    x = p.reshape(-1, 1).clone().requires_grad_(True)
+    w = torch.ones(1, 1, device=cuda_device)
+    y = dense.linear(x, w, None, act)
+    slope = torch.autograd.grad(y, x, torch.ones_like(y))[0]
+    full = torch.ones_like(x, dtype=torch.bool) if act == "none" else x.detach() > 0
+    assert torch.equal(y.detach(), torch.where(full, x.detach(), torch.zeros_like(y)))
+    assert torch.equal(slope, full.float())
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("shape", [(16, 4096, 520), (700, 1024, 768), (4096, 256, 256),
                                    (20000, 64, 64), (33, 8200, 24), (40000, 24, 8)])
