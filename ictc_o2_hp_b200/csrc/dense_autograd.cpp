@@ -145,8 +145,11 @@ void check_linear(const Tensor& x, const Tensor& weight, const Tensor& bias,
   }
 }
 
-// [rows, width] with unit stride inside a row; copies only when it must.
+// [rows, width] with unit stride inside a row; copies only when it must.  (A view whose
+// sign is flipped by a bit on the tensor, such as the imaginary part of a conjugate, has
+// other values than its memory.)
 Tensor rows_of(const Tensor& t) {
+  if (t.is_neg()) return rows_of(t.resolve_neg());
   const int64_t width = t.size(-1);
   if (t.dim() == 2 && (width == 1 || t.stride(1) == 1)) return t;
   int64_t rows = 1;
@@ -155,7 +158,7 @@ Tensor rows_of(const Tensor& t) {
   return width == 1 || flat.stride(1) == 1 ? flat : flat.contiguous();
 }
 
-Tensor packed(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
+Tensor packed(const Tensor& t) { return t.defined() ? t.resolve_neg().contiguous() : t; }
 
 void* data(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 

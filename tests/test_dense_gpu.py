@@ -278,6 +278,28 @@ def test_linear_strides_and_batches(dtype, cuda_device):
                          y.detach().reshape(-1, n), (grads[0].reshape(-1, 40), grads[1]), dtype)
 
 
+def test_views_with_a_negative_bit(cuda_device):
+    """The imaginary part of a conjugate is the memory's negative: as rows of one column and
+    one bias it is read where it lies."""
+    from ictc_o2_hp_b200 import dense
+    z = torch.complex(*(rand((40, 1), torch.float32, cuda_device, s) for s in (36, 37)))
+    x = z.conj().imag
+    assert x.is_neg()
+    plain = x.resolve_neg()
+    w = rand((3, 1), torch.float32, cuda_device, 38)
+    one = torch.complex(*(rand((1,), torch.float32, cuda_device, s) for s in (39, 40))).conj().imag
+    assert torch.equal(dense.linear(x, w), dense.linear(plain, w))
+    assert torch.equal(dense.linear(plain, x[:5]), dense.linear(plain, plain[:5]))
+    assert torch.equal(dense.linear(plain, w[:1], one), dense.linear(plain, w[:1],
+                                                                    one.resolve_neg()))
+    assert torch.equal(dense.layer_norm(x, one, one),
+                       dense.layer_norm(plain, one.resolve_neg(), one.resolve_neg()))
+    leaf = plain.clone().requires_grad_(True)
+    y = dense.linear(leaf, w[:1], None, "silu")
+    assert torch.equal(*(torch.autograd.grad(y, leaf, g, retain_graph=True)[0]
+                         for g in (x, plain)))
+
+
 @pytest.mark.parametrize("rows", [2, 64])
 def test_linear_float32_range(rows, cuda_device):
     """Magnitudes from 1e-30 to 1e30: the cut into bf16 parts keeps every bit."""
