@@ -20,9 +20,11 @@
 // as an infinity.
 //
 // Which kernel a product takes:
+//   up to 4 rows, aligned (forward)             FMAs, W read once (few_rows_kernel)
+//   a dimension of at most 8                    FMAs, the large operand read once, in any
+//                                               layout (dense_thin.cuh; thin_form and
+//                                               plan_linear have the exceptions)
 //   up to 64 inputs and outputs, contiguous     one kernel per direction (dense_narrow.cuh)
-//   up to 4 rows (forward)                      FMAs, W read once (few_rows_kernel)
-//   up to 8 columns over unaligned rows         FMAs, A read once (few_columns_kernel)
 //   16-bit, aligned rows                        SM pairs fed by TMA (dense_pair.cuh)
 //   float32, aligned rows                       cut on the way in (dense_cut.cuh)
 //   anything else: small or unaligned           register-staged operands (product_kernel);
@@ -37,6 +39,7 @@
 #include "dense_epilogue.cuh"
 #include "dense_narrow.cuh"
 #include "dense_pair.cuh"
+#include "dense_thin.cuh"
 #include "dense_types.cuh"
 #include "tcgen05.cuh"
 #include "tmap.cuh"
@@ -438,67 +441,6 @@ __global__ void __launch_bounds__(kRowThreads) few_rows_kernel(
   }
 }
 
-// --------------------------------------------------------------- few columns: no tiles
-// Up to eight columns over many rows that TMA cannot address: reading A once as it lies is
-// cheaper than copying it to aligned rows first.  A warp owns four rows; lanes run along K;
-// B's columns are staged in shared memory once per CTA, and each value read from there
-// serves four rows.  Sums: FMAs per lane, then a butterfly.  float32 59,714 x 2,186 x 6: 197
-// us (2.7 TB/s), against 392 us with the copy.
-constexpr int kThinColumns = 8, kThinRows = 4;
-constexpr size_t kThinBytes = 192 * 1024;  // of B's columns, at most
-
-template <typename T, bool B_MN, int NC>
-__global__ void __launch_bounds__(256) few_columns_kernel(const __grid_constant__ ProductArgs p) {
-  extern __shared__ float columns[];  // [NC][k]
-  const T* a = static_cast<const T*>(p.a);
-  const T* b = static_cast<const T*>(p.b);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n = static_cast<int>(p.n), len = static_cast<int>(p.k);
-#pragma unroll
-  for (int c = 0; c < NC; ++c)
-    for (int k = threadIdx.x; k < len; k += 256)
-      columns[c * len + k] = c < n ? to_float(B_MN ? b[k * p.ldb + c] : b[c * p.ldb + k]) : 0.f;
-  __syncthreads();
-  const int64_t step = static_cast<int64_t>(gridDim.x) * 8 * kThinRows;
-  for (int64_t base = static_cast<int64_t>(blockIdx.x) * 8 * kThinRows; base < p.m; base += step) {
-    const int64_t row0 = base + warp * kThinRows;
-    const T* rows[kThinRows];  // past the end: the last row again, its sums dropped
-#pragma unroll
-    for (int r = 0; r < kThinRows; ++r)
-      rows[r] = a + (row0 + r < p.m ? row0 + r : p.m - 1) * p.lda;
-    float acc[kThinRows][NC];
-#pragma unroll
-    for (int r = 0; r < kThinRows; ++r)
-#pragma unroll
-      for (int c = 0; c < NC; ++c) acc[r][c] = 0.f;
-    // unrolled for the loads: a warp has sixteen in flight
-#pragma unroll 4
-    for (int k = lane; k < len; k += 32) {
-      float x[kThinRows];
-#pragma unroll
-      for (int r = 0; r < kThinRows; ++r) x[r] = to_float(rows[r][k]);
-#pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        const float w = columns[c * len + k];
-#pragma unroll
-        for (int r = 0; r < kThinRows; ++r) acc[r][c] = fmaf(x[r], w, acc[r][c]);
-      }
-    }
-#pragma unroll
-    for (int r = 0; r < kThinRows; ++r)
-#pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        float v = acc[r][c];
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        if (lane == c && c < n && row0 + r < p.m)
-          finish1<T, kAnyActivation>(
-              p.e, row0 + r, c, p.n, v,
-              p.e.bias ? to_float(static_cast<const T*>(p.e.bias)[c]) : 0.f);
-      }
-  }
-}
-
 // ------------------------------------------------------- d = g act'(p) and sums of d
 // Bound by HBM (bf16 16,384 x 4,096: 120 us, 4.5 TB/s; float32 65,536 x 512: 68 us, 5.9 TB/s).
 // A CTA owns a strip of columns and every gridDim.y-th block of rows; each
@@ -721,12 +663,85 @@ int launch_product(const ProductArgs& p, int device, cudaStream_t stream) {
   return e == cudaSuccess ? ICTC_OK : cuda_fail(e, "linear product launch");
 }
 
-int thin_columns(int64_t n) { return n == 1 ? 1 : n <= 4 ? 4 : kThinColumns; }
+// --------------------------------------------------------------- thin forms: host side
 
-// Few columns, held in shared memory, and enough rows to fill the SMs without splitting K.
-bool few_columns(int64_t m, int64_t n, int64_t k) {
-  return n <= kThinColumns && m >= 4096 &&
-         k <= static_cast<int64_t>(kThinBytes / sizeof(float)) / thin_columns(n);
+enum class Thin { none, dot, dot_swapped, outer, gram, gram_swapped };
+
+int thin_columns(int64_t count) { return count <= 2 ? static_cast<int>(count) : count <= 4 ? 4 : 8; }
+
+// The staged operand fits, and there are rows enough to fill the SMs without splitting the
+// sum (or it is short).
+bool dot_fits(int64_t rows, int64_t len, int64_t count) {
+  return len <= static_cast<int64_t>(kThinBytes / sizeof(float)) / thin_columns(count) - 3 &&
+         (rows >= 1024 || len <= 8192);
+}
+
+// The form of a product with a dimension of at most kThin.  A few rows over a weight whose
+// rows run along the sum (the forward's) are decided by the caller.
+Thin thin_form(bool a_mn, bool b_mn, int64_t m, int64_t n, int64_t k) {
+  if (k <= kThin) return Thin::outer;
+  if (n <= kThin && a_mn) return Thin::gram_swapped;
+  if (n <= kThin && dot_fits(m, k, n)) return Thin::dot;
+  if (m <= kThin && b_mn) return Thin::gram;
+  return Thin::none;
+}
+
+struct StripPlan {
+  int lanes;
+  unsigned blocks_x, blocks_y;
+};
+
+// Strips of 32 lanes of `vec` (or, strided, four) columns, and as many blocks of rows as fill the SMs, each
+// thread's at least four rows (the loads that it has in flight).
+StripPlan plan_strips(int64_t rows, int64_t width, int vec, int device) {
+  StripPlan s{};
+  const int64_t units = ceil_div(width, vec > 1 ? vec : kStrided);
+  s.lanes = 1;
+  while (s.lanes < 32 && s.lanes < units) s.lanes *= 2;
+  s.blocks_x = static_cast<unsigned>(ceil_div(units, s.lanes));
+  const int64_t most = ceil_div(rows, 4 * (kStripThreads / s.lanes));
+  int64_t y = ceil_div(static_cast<int64_t>(sm_count(device)) * 8, s.blocks_x);
+  if (y > 296) y = 296;
+  if (y > most) y = most;
+  s.blocks_y = static_cast<unsigned>(y < 1 ? 1 : y);
+  return s;
+}
+
+// Bytes of a gram form's partial sums, whichever access width the pointers allow.
+size_t gram_bytes(int64_t rows, int64_t width, int64_t count, size_t size, int device) {
+  size_t parts = 1;
+  for (const int vec : {static_cast<int>(16 / size), 1}) {
+    const size_t y = plan_strips(rows, width, vec, device).blocks_y;
+    if (y > parts) parts = y;
+  }
+  return parts * static_cast<size_t>(width) * count * sizeof(float);
+}
+
+// Workspace of a product, whichever kernel it takes.
+size_t product_bytes(bool a_mn, bool b_mn, int64_t m, int64_t n, int64_t k, int dtype,
+                     int device) {
+  const size_t size = dtype_size(dtype);
+  switch (thin_form(a_mn, b_mn, m, n, k)) {
+    case Thin::none: return split_bytes(m, n, k, dtype, device);
+    case Thin::gram: return gram_bytes(k, n, m, size, device);
+    case Thin::gram_swapped: return gram_bytes(k, m, n, size, device);
+    default: return 0;
+  }
+}
+
+// Calls f with the small dimension as a compile-time constant.
+template <typename F>
+void for_thin(int count, const F& f) {
+  switch (count) {
+    case 1: return f(std::integral_constant<int, 1>{});
+    case 2: return f(std::integral_constant<int, 2>{});
+    case 3: return f(std::integral_constant<int, 3>{});
+    case 4: return f(std::integral_constant<int, 4>{});
+    case 5: return f(std::integral_constant<int, 5>{});
+    case 6: return f(std::integral_constant<int, 6>{});
+    case 7: return f(std::integral_constant<int, 7>{});
+    default: return f(std::integral_constant<int, kThin>{});
+  }
 }
 
 template <typename T>
@@ -736,7 +751,115 @@ bool vec_epilogue(const Epilogue& e, int64_t n) {
          aligned(e.preact, 16);
 }
 
-// C = epilogue(A B^T); `partial` holds split_bytes() when the plan splits K.
+// Rows that a group of lanes holds at a time: several share every read of the staged operand,
+// as long as that leaves work for all warps of the SMs.
+template <typename T, int V, int NC, int L>
+int launch_dot(const ThinArgs& p, int64_t sms, cudaStream_t stream) {
+  constexpr int kMany = NC <= 2 ? 4 : 2, kWarps = kDotThreads / 32;
+  const size_t bytes = static_cast<size_t>(NC) * ((p.len + 3) & ~3) * sizeof(float);
+  const bool many = p.rows >= sms * kWarps * (32 / L) * kMany;
+  const int64_t want = ceil_div(p.rows, kWarps * (32 / L) * (many ? kMany : 1));
+  const int64_t cap = sms * (bytes <= 96 * 1024 ? 2 : 1);
+  const auto kernel =
+      many ? thin_dot_kernel<T, V, NC, L, kMany> : thin_dot_kernel<T, V, NC, L, 1>;
+  const int st = allow_smem(reinterpret_cast<const void*>(kernel), bytes);
+  if (st == ICTC_OK)
+    kernel<<<static_cast<unsigned>(want < cap ? want : cap), kDotThreads, bytes, stream>>>(p);
+  return st;
+}
+
+template <typename T, int V, int L>
+int launch_dot_columns(const ThinArgs& p, int64_t sms, cudaStream_t stream) {
+  switch (thin_columns(p.count)) {
+    case 1: return launch_dot<T, V, 1, L>(p, sms, stream);
+    case 2: return launch_dot<T, V, 2, L>(p, sms, stream);
+    case 4: return launch_dot<T, V, 4, L>(p, sms, stream);
+    default: return launch_dot<T, V, kThin, L>(p, sms, stream);
+  }
+}
+
+// Lanes of a row: enough that consecutive lanes read whole sectors, and no more than leave
+// each a few accesses, because every row's sums are joined over them (float32 343,990 x 65
+// x 7: 51 us with 4 lanes of 33 accesses; 136,107 x 175 x 6, as many values: 89 with 32 of 6).
+template <typename T, int V>
+int launch_dot_lanes(const ThinArgs& p, int64_t sms, cudaStream_t stream) {
+  const int accesses = p.len / V;
+  if (accesses <= 8) return launch_dot_columns<T, V, 1>(p, sms, stream);
+  if (accesses < 128 || (accesses < 1024 && p.rows >= sms * 256))
+    return launch_dot_columns<T, V, 4>(p, sms, stream);
+  return launch_dot_columns<T, V, 32>(p, sms, stream);
+}
+
+template <typename T, bool A_MN, bool B_MN>
+int run_thin(Thin form, const T* a, int64_t lda, const T* b, int64_t ldb, int64_t m, int64_t n,
+             int64_t k, const Epilogue& e, float* partial, cudaStream_t stream) {
+  constexpr int kFull = 16 / sizeof(T);
+  const int device = current_device();
+  const int64_t sms = sm_count(device);
+  // strides of A and B along their own index and along the sum
+  const int64_t a_i = A_MN ? 1 : lda, a_k = A_MN ? lda : 1;
+  const int64_t b_i = B_MN ? 1 : ldb, b_k = B_MN ? ldb : 1;
+  ThinArgs p{};
+  p.e = e;
+  p.e.vec = vec_epilogue<T>(e, n);
+  int st = ICTC_OK;
+  if (form == Thin::outer) {
+    p.small = a; p.small_i = a_i; p.small_c = a_k;
+    p.wide = b; p.wide_c = b_k; p.wide_j = b_i;
+    p.rows = m; p.width = n;
+    p.count = static_cast<int>(k);
+    const StripPlan s = plan_strips(m, n, p.e.vec ? 4 : 1, device);
+    p.lanes = s.lanes;
+    for_thin(p.count, [&](auto nc) {
+      const auto kernel =
+          p.e.vec ? thin_outer_kernel<T, 4, nc.value> : thin_outer_kernel<T, 1, nc.value>;
+      kernel<<<dim3(s.blocks_x, s.blocks_y), kStripThreads, 0, stream>>>(p);
+    });
+  } else if (form == Thin::dot || form == Thin::dot_swapped) {
+    p.swapped = form == Thin::dot_swapped;
+    p.big = p.swapped ? b : a;
+    p.big_ld = p.swapped ? ldb : lda;
+    p.small = p.swapped ? a : b;
+    p.small_i = p.swapped ? a_k : b_k;
+    p.small_c = p.swapped ? a_i : b_i;
+    p.rows = p.swapped ? n : m;
+    p.len = static_cast<int>(k);
+    p.count = static_cast<int>(p.swapped ? m : n);
+    const bool vec =
+        k % kFull == 0 && chunk_aligned(p.big, p.big_ld, sizeof(T));
+    st = vec ? launch_dot_lanes<T, kFull>(p, sms, stream) : launch_dot_lanes<T, 1>(p, sms, stream);
+    if (st != ICTC_OK) return st;
+  } else {
+    // the operand whose rows the sum runs over, and the few columns of the other
+    p.swapped = form == Thin::gram_swapped;
+    p.big = p.swapped ? a : b;
+    p.big_ld = p.swapped ? lda : ldb;
+    p.small = p.swapped ? b : a;
+    p.small_i = p.swapped ? b_k : a_k;
+    p.small_c = p.swapped ? b_i : a_i;
+    p.rows = k;
+    p.width = p.swapped ? m : n;
+    p.count = static_cast<int>(p.swapped ? n : m);
+    p.partial = partial;
+    const bool vec = p.width % kFull == 0 && chunk_aligned(p.big, p.big_ld, sizeof(T));
+    const StripPlan s = plan_strips(p.rows, p.width, vec ? kFull : 1, device);
+    p.lanes = s.lanes;
+    for_thin(p.count, [&](auto nc) {
+      const auto kernel = vec ? thin_gram_kernel<T, kFull, nc.value> : thin_gram_kernel<T, 1, nc.value>;
+      kernel<<<dim3(s.blocks_x, s.blocks_y), kStripThreads, 0, stream>>>(p);
+    });
+    const cudaError_t err = cudaGetLastError();
+    if (err != cudaSuccess) return cuda_fail(err, "thin linear product launch");
+    T* out = static_cast<T*>(e.out);
+    column_total_kernel<T><<<dim3(static_cast<unsigned>(ceil_div(m * n, 32))),
+                             dim3(32, kColumnLanes), 0, stream>>>(partial, partial, out, out,
+                                                                  s.blocks_y, m * n);
+  }
+  const cudaError_t err = cudaGetLastError();
+  return err == cudaSuccess ? ICTC_OK : cuda_fail(err, "thin linear product launch");
+}
+
+// C = epilogue(A B^T); `partial` holds product_bytes().
 template <typename T, bool A_MN, bool B_MN>
 int run_product(const T* a, int64_t lda, const T* b, int64_t ldb, int64_t m, int64_t n, int64_t k,
                 Epilogue e, float* partial, cudaStream_t stream) {
@@ -751,26 +874,9 @@ int run_product(const T* a, int64_t lda, const T* b, int64_t ldb, int64_t m, int
     const cudaError_t err = cudaGetLastError();
     return err == cudaSuccess ? ICTC_OK : cuda_fail(err, "linear split join launch");
   };
-  if constexpr (!A_MN) {
-    if (few_columns(m, n, k) && !chunk_aligned(a, lda, sizeof(T))) {
-      ProductArgs p{};
-      p.a = a; p.b = b;
-      p.m = m; p.n = n; p.k = k;
-      p.lda = lda; p.ldb = ldb;
-      p.e = e;
-      const size_t bytes = static_cast<size_t>(thin_columns(n)) * k * sizeof(float);
-      const int64_t resident = bytes <= 48 * 1024 ? 4 : bytes <= 96 * 1024 ? 2 : 1;
-      const int64_t want = ceil_div(m, 8 * kThinRows), cap = sm_count(device) * resident;
-      const unsigned grid = static_cast<unsigned>(want < cap ? want : cap);
-      const auto kernel = n == 1   ? few_columns_kernel<T, B_MN, 1>
-                          : n <= 4 ? few_columns_kernel<T, B_MN, 4>
-                                   : few_columns_kernel<T, B_MN, kThinColumns>;
-      const int st = allow_smem(reinterpret_cast<const void*>(kernel), bytes);
-      if (st != ICTC_OK) return st;
-      kernel<<<grid, 256, bytes, stream>>>(p);
-      const cudaError_t err = cudaGetLastError();
-      return err == cudaSuccess ? ICTC_OK : cuda_fail(err, "linear few-column launch");
-    }
+  if constexpr (B_MN) {  // a gradient (the forward's form is in its plan)
+    if (const Thin form = thin_form(A_MN, B_MN, m, n, k); form != Thin::none)
+      return run_thin<T, A_MN, B_MN>(form, a, lda, b, ldb, m, n, k, e, partial, stream);
   }
   if constexpr (sizeof(T) == 2) {
     const PairPlan q = plan_pair(m, n, k, device);
@@ -907,6 +1013,7 @@ int32_t layout_of(const void* x, int64_t ldx, const void* w, int64_t ldw, const 
 // Byte offsets of the workspace's parts, and its size.
 struct LinearPlan {
   bool few, narrow, align;
+  Thin thin;  // the forward's
   size_t d, x, w, g, columns, partial, total;
 };
 
@@ -916,11 +1023,27 @@ LinearPlan plan_linear(int64_t m, int64_t n, int64_t k, int dtype, int activatio
                        bool backward, int device) {
   LinearPlan b{};
   const size_t size = dtype_size(dtype);
-  b.few = !backward && m <= kFewRows;
-  b.narrow = !b.few && (layout & ICTC_LINEAR_PACKED) && n <= kNarrow && k <= kNarrow &&
-             m <= (1ll << 36);
-  b.align = !(layout & ICTC_LINEAR_ALIGNED) && worth_aligning(m, n, k) &&
-            (backward || !few_columns(m, n, k));
+  const int64_t full = static_cast<int64_t>(16 / size);
+  const bool rows_aligned = layout & ICTC_LINEAR_ALIGNED;
+  // both products of the backward are thin: no operand is copied to aligned rows
+  const bool thin = backward && (n <= kThin || m <= kThin || (k <= kThin && dot_fits(m, n, k)));
+  b.narrow = (layout & ICTC_LINEAR_PACKED) && n <= kNarrow && k <= kNarrow && m <= (1ll << 36);
+  if (!backward) {
+    b.few = m <= kFewRows && rows_aligned && k % full == 0;
+    if (!b.few) b.thin = thin_form(false, false, m, n, k);
+    // a few rows over a weight that few_rows_kernel and TMA would read by elements
+    if (!b.few && b.thin == Thin::none && m <= kThin && (m <= kFewRows || !rows_aligned) &&
+        dot_fits(n, k, m))
+      b.thin = Thin::dot_swapped;
+    if (b.thin == Thin::none) b.few = m <= kFewRows;
+    b.narrow = b.narrow && !b.few && b.thin == Thin::none;
+  } else if (thin && (n * size % 16 != 0 || k * size % 16 != 0) &&
+             m > 2 * kNarrowTile * static_cast<int64_t>(sm_count(device))) {
+    // rows that are not whole blocks: the narrow kernel reads them value by value, which
+    // more than a few tiles an SM cannot hide
+    b.narrow = false;
+  }
+  b.align = !rows_aligned && b.thin == Thin::none && !thin && worth_aligning(m, n, k);
   size_t at = 0;
   const auto take = [&](size_t bytes) {
     const size_t here = at;
@@ -930,7 +1053,7 @@ LinearPlan plan_linear(int64_t m, int64_t n, int64_t k, int dtype, int activatio
   const auto rows = [&](int64_t r, int64_t width) {
     return static_cast<size_t>(r) * aligned_pitch(width, size) * size;
   };
-  if (b.few) return b;
+  if (b.few || b.thin != Thin::none) return b;
   if (b.narrow) {
     if (backward)
       b.partial = take(static_cast<size_t>(sm_count(device)) * (n * k + n) * sizeof(float));
@@ -946,8 +1069,8 @@ LinearPlan plan_linear(int64_t m, int64_t n, int64_t k, int dtype, int activatio
   }
   if (backward) {
     b.columns = take(static_cast<size_t>(m < kSlopeParts ? m : kSlopeParts) * n * sizeof(float));
-    const size_t one = split_bytes(m, k, n, dtype, device);
-    const size_t other = split_bytes(n, k, m, dtype, device);
+    const size_t one = product_bytes(false, true, m, k, n, dtype, device);
+    const size_t other = product_bytes(true, true, n, k, m, dtype, device);
     b.partial = take(one > other ? one : other);
   } else {
     b.partial = take(split_bytes(m, n, k, dtype, device));
@@ -1027,7 +1150,9 @@ int run_linear_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, E
     return launch_few_rows<T, 1>(xt, ldx, wt, ldw, m, n, k, e, stream);
   }
   if (plan.narrow) return run_narrow_forward<T>(xt, wt, ldw, e, m, n, k, stream);
-  if (plan.align) {  // never with few columns
+  if (plan.thin != Thin::none)
+    return run_thin<T, false, false>(plan.thin, xt, ldx, wt, ldw, m, n, k, e, nullptr, stream);
+  if (plan.align) {
     int st = align_operand(&xt, &ldx, m, k, workspace + plan.x, stream);
     if (st == ICTC_OK) st = align_operand(&wt, &ldw, n, k, workspace + plan.w, stream);
     if (st != ICTC_OK) return st;
@@ -1050,7 +1175,7 @@ SlopePlan plan_slope(int64_t m, int64_t n, int vec) {
   s.lanes = lanes;
   s.blocks_x = static_cast<unsigned>(ceil_div(units, lanes));
   const int64_t row_blocks = ceil_div(m, 256 / lanes);
-  int64_t y = ceil_div(148 * 8, s.blocks_x);
+  int64_t y = ceil_div(static_cast<int64_t>(sm_count(current_device())) * 8, s.blocks_x);
   if (y > kSlopeParts) y = kSlopeParts;
   if (y > row_blocks) y = row_blocks;
   if (m <= 1024) y = 1;  // short sums are finished where they are formed

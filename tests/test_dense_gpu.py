@@ -278,6 +278,76 @@ def test_linear_strides_and_batches(dtype, cuda_device):
                          y.detach().reshape(-1, n), (grads[0].reshape(-1, 40), grads[1]), dtype)
 
 
+THIN = [1, 2, 3, 5, 7, 8]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("small", THIN)
+@pytest.mark.parametrize("side", ["rows", "in", "out"])
+def test_linear_thin(side, small, dtype, cuda_device):
+    """A dimension of at most eight: every form, with rows on and off the 16-byte boundaries
+    and lengths that no lane, strip or unrolled step divides."""
+    from ictc_o2_hp_b200 import _lib, dense
+    sizes = [(9, 9), (37, 64), (128, 33), (301, 1029), (1026, 2056), (40001, 24), (6001, 70)]
+    for i, (one, two) in enumerate(sizes):
+        if side == "rows":
+            m, k, n = small, one % 5000 + 8, two
+        elif side == "in":
+            m, k, n = one, small, two
+        else:
+            m, k, n = one, two, small
+        act = ACTS[(i + small) % len(ACTS)]
+        x = rand((m, k), dtype, cuda_device, 1).requires_grad_(True)
+        w = rand((n, k), dtype, cuda_device, 2, 1.5 / math.sqrt(k)).requires_grad_(True)
+        b = rand((n,), dtype, cuda_device, 3).requires_grad_(True)
+        r = rand((m, n), dtype, cuda_device, 4) if i % 2 else None
+        g = rand((m, n), dtype, cuda_device, 5)
+        y = dense.linear(x, w, b, act, r)
+        grads = torch.autograd.grad(y, (x, w, b), g)
+        check_linear(x.detach(), w.detach(), b.detach(), r, act, g, y.detach(), grads, dtype)
+        again = torch.autograd.grad(dense.linear(x, w, b, act, r), (x, w, b), g)
+        assert all(torch.equal(p, q) for p, q in zip(grads, again)), "not the same bits twice"
+    assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(6, 90, 70), (500, 90, 6), (500, 6, 90), (3, 6, 5), (500, 64, 8)])
+def test_linear_thin_strides(shape, dtype, cuda_device):
+    """Slices, transposed weights, repeated rows and expanded gradients in the thin forms."""
+    from ictc_o2_hp_b200 import dense
+    m, k, n = shape
+    big = rand((m + 3, 2 * k + 9), dtype, cuda_device, 31)
+    wide = rand((2 * n + 9, 2 * k + 9), dtype, cuda_device, 32, 0.2)
+    res = rand((m, n + 9), dtype, cuda_device, 33)
+    b = rand((n,), dtype, cuda_device, 35)
+    for x in (big[:m, :k], big[3:, 1:k + 1], big[:m, :2 * k:2], big[:1, :k].expand(m, k)):
+        for w in (wide[:n, 8:k + 8], wide[n:2 * n, 3:k + 3], wide.t()[:n, :k]):
+            if w.shape != (n, k):
+                continue
+            for r, g in ((res[:, 1:n + 1], rand((m, n), dtype, cuda_device, 36)),
+                         (res[:, :n], rand((1,), dtype, cuda_device, 37).expand(m, n)),
+                         (None, rand((m, n + 3), dtype, cuda_device, 38)[:, 3:])):
+                leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]
+                y = dense.linear(*leaves, "silu", r)
+                grads = torch.autograd.grad(y, leaves, g)
+                check_linear(x, w, b, r, "silu", g, y.detach(), grads, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(300007, 21, 2), (300007, 2, 21), (2, 300, 4001), (4100, 9000, 1)])
+def test_linear_thin_large(shape, dtype, cuda_device):
+    """Many blocks of rows: sums joined over CTAs, rows off the boundaries."""
+    from ictc_o2_hp_b200 import dense
+    m, k, n = shape
+    x = rand((m, k), dtype, cuda_device, 41).requires_grad_(True)
+    w = rand((n, k), dtype, cuda_device, 42, 1.5 / math.sqrt(k)).requires_grad_(True)
+    b = rand((n,), dtype, cuda_device, 43).requires_grad_(True)
+    g = rand((m, n), dtype, cuda_device, 45)
+    y = dense.linear(x, w, b, "gelu")
+    grads = torch.autograd.grad(y, (x, w, b), g)
+    check_linear(x.detach(), w.detach(), b.detach(), None, "gelu", g, y.detach(), grads, dtype)
+
+
 def test_views_with_a_negative_bit(cuda_device):
     """The imaginary part of a conjugate is the memory's negative: as rows of one column and
     one bias it is read where it lies."""
