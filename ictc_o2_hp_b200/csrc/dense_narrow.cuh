@@ -147,9 +147,25 @@ __device__ __noinline__ float4 read_unit_edge(const T* raw, const T* global, int
   return make_float4(v[0], v[1], v[2], v[3]);
 }
 
+// One value out of shared memory.
+template <typename T>
+__device__ __forceinline__ float read_shared(uint32_t at) {
+  if constexpr (sizeof(T) == 4) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+  } else {
+    uint16_t bits;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(bits) : "r"(at) : "memory");
+    return to_float(*reinterpret_cast<const T*>(&bits));
+  }
+}
+
 // Columns 4 u .. of row r, zeros outside the operand.  PLAIN: rows are whole 16-byte
-// blocks, so that all of a slice is copied and a unit is one access; a kernel of its own,
-// because the general read's code between the others' cost a third of the time.
+// blocks, and a unit is one access; a kernel of its own, because the general read's code
+// between the others' cost a third of the time.  Otherwise its values are read one by one;
+// 32 rows of any width are whole blocks, so only a tensor's last slice can have values that
+// were not copied.
 template <bool PLAIN, typename T>
 __device__ __forceinline__ void read_unit(const Slice<T>& s, int r, int u, float (&v)[4]) {
   if constexpr (PLAIN) {
@@ -170,6 +186,13 @@ __device__ __forceinline__ void read_unit(const Slice<T>& s, int r, int u, float
     const Pack<T, 4>& pk = *reinterpret_cast<const Pack<T, 4>*>(q);
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] = to_float(pk.v[j]);
+  } else if (s.copied == s.rows * s.width) {
+    const uint32_t at = smem_addr(s.raw) + (r * s.width + 4 * u) * sizeof(T);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[j] = 0.f;
+      if (r < s.rows && 4 * u + j < s.width) v[j] = read_shared<T>(at + j * sizeof(T));
+    }
   } else {
     const float4 f = read_unit_edge(s.raw, s.global, s.width, s.rows, s.copied, r, u);
     v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
