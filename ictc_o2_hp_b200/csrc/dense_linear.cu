@@ -524,9 +524,9 @@ struct Split {
 
 // The K axis is split when the output has too few tiles to fill the SMs: at least four
 // stages of K per split (the pipeline's depth), and no more splits than fill one wave.
-Split plan_product(int64_t m, int64_t n, int64_t k, int device) {
+Split plan_product(int64_t m, int64_t n, int64_t k, int device, int most_columns = 128) {
   Split s{};
-  s.bn = n <= 64 ? 64 : 128;
+  s.bn = n <= 64 || most_columns == 64 ? 64 : 128;
   const int64_t tm = ceil_div(m, kBM), tn = ceil_div(n, s.bn), chunks = ceil_div(k, kBK);
   s.fits = tm < (1ll << 31) && tn < (1ll << 31) && chunks < (1ll << 31);
   if (!s.fits) return s;
@@ -901,19 +901,22 @@ int run_product(const T* a, int64_t lda, const T* b, int64_t ldb, int64_t m, int
       }
     }
   }
-  const Split s = plan_product(m, n, k, device);
-  if (!s.fits) return fail(ICTC_ERR_UNSUPPORTED, "linear: a dimension is too large");
   ProductArgs p{};
   p.a = a; p.b = b;
   p.m = m; p.n = n; p.k = k;
   p.lda = lda; p.ldb = ldb;
-  p.tiles_m = s.tiles_m; p.tiles_n = s.tiles_n;
-  p.splits = s.splits; p.chunks = s.chunks; p.chunks_per_split = s.chunks_per_split;
   p.vec_a = chunk_aligned(a, lda, sizeof(T));
   p.vec_b = chunk_aligned(b, ldb, sizeof(T));
-  e.partial = s.splits > 1 ? partial : nullptr;
-  p.e = e;
+  const auto take = [&](const Split& s) {
+    p.tiles_m = s.tiles_m; p.tiles_n = s.tiles_n;
+    p.splits = s.splits; p.chunks = s.chunks; p.chunks_per_split = s.chunks_per_split;
+    e.partial = s.splits > 1 ? partial : nullptr;
+    p.e = e;
+  };
   if constexpr (sizeof(T) == 4) {
+    const Split s = plan_product(m, n, k, device);
+    if (!s.fits) return fail(ICTC_ERR_UNSUPPORTED, "linear: a dimension is too large");
+    take(s);
     OperandMaps maps;
     if (p.vec_a && p.vec_b && m < (1ll << 31) && n < (1ll << 31) && k < (1ll << 31) &&
         encode_matrix_map(a, 4, false, A_MN ? m : k, A_MN ? k : m, lda * 4, A_MN ? 128 : kCutK,
@@ -925,8 +928,17 @@ int run_product(const T* a, int64_t lda, const T* b, int64_t ldb, int64_t m, int
       return st != ICTC_OK || s.splits == 1 ? st : join(s.splits);
     }
   }
-  const int st = s.bn == 64 ? launch_product<T, A_MN, B_MN, 64>(p, device, stream)
-                            : launch_product<T, A_MN, B_MN, 128>(p, device, stream);
+  // A float32 tile is 64 columns wide: the cut parts of a wider one do not fit a producer's
+  // registers.  (More tiles are never more splits, for which `partial` has room.)
+  const Split s = plan_product(m, n, k, device, sizeof(T) == 4 ? 64 : 128);
+  if (!s.fits) return fail(ICTC_ERR_UNSUPPORTED, "linear: a dimension is too large");
+  take(s);
+  int st;
+  if constexpr (sizeof(T) == 4)
+    st = launch_product<T, A_MN, B_MN, 64>(p, device, stream);
+  else
+    st = s.bn == 64 ? launch_product<T, A_MN, B_MN, 64>(p, device, stream)
+                    : launch_product<T, A_MN, B_MN, 128>(p, device, stream);
   return st != ICTC_OK || s.splits == 1 ? st : join(s.splits);
 }
 
