@@ -341,34 +341,57 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
   }
 }
 
-// out = epilogue(sum of the splits' partial products), the splits added in order.
+// out = epilogue(sum of the splits' partial products), the splits added in order.  Rows of
+// whole quads lie behind one another: their quads are numbered through, four to a thread so
+// that their loads are in flight together.
 template <typename T>
 __global__ void __launch_bounds__(256) join_splits_kernel(const Epilogue e, int64_t m, int64_t n,
                                                           int splits) {
-  const int64_t quads = (n + 3) / 4;
+  constexpr int kAhead = 4;
+  const int64_t quads = (n + 3) / 4, total = m * quads;
   const int64_t step = static_cast<int64_t>(gridDim.x) * 256;
-  for (int64_t q = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; q < m * quads; q += step) {
+  int64_t q = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (e.vec) {
+    const float4* parts = reinterpret_cast<const float4*>(e.partial);
+    const bool placed = e.bias || e.residual;
+    for (; q < total; q += kAhead * step) {
+      float4 sum[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (q + u * step < total) sum[u] = parts[q + u * step];
+      for (int s = 1; s < splits; ++s) {
+        const float4* part = parts + s * total + q;
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+          if (q + u * step < total) {
+            const float4 f = part[u * step];
+            sum[u].x += f.x; sum[u].y += f.y; sum[u].z += f.z; sum[u].w += f.w;
+          }
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int64_t at = q + u * step;
+        if (at >= total) break;
+        float v[4] = {sum[u].x, sum[u].y, sum[u].z, sum[u].w}, bias[4] = {0.f, 0.f, 0.f, 0.f};
+        Pack<T, 4> r{};
+        if (placed) {
+          const int64_t row = at / quads, col = (at - row * quads) * 4;
+          load_bias4<T>(e, col, n, bias);
+          if (e.residual) r = residual4<T>(e, row, col);
+        }
+        finish4<T, kAnyActivation>(e, at * 4, v, bias, r);
+      }
+    }
+    return;
+  }
+  for (; q < total; q += step) {
     const int64_t row = q / quads, col = (q - row * quads) * 4;
     const float* at = e.partial + row * n + col;
-    if (e.vec) {
-      float v[4] = {0.f, 0.f, 0.f, 0.f}, bias[4];
-      load_bias4<T>(e, col, n, bias);
-      Pack<T, 4> r{};
-      if (e.residual) r = residual4<T>(e, row, col);
-#pragma unroll 4
-      for (int s = 0; s < splits; ++s, at += m * n) {
-        const float4 f = *reinterpret_cast<const float4*>(at);
-        v[0] += f.x; v[1] += f.y; v[2] += f.z; v[3] += f.w;
-      }
-      finish4<T, kAnyActivation>(e, row * n + col, v, bias, r);
-    } else {
-      for (int j = 0; j < 4 && col + j < n; ++j) {
-        float v = 0.f;
-        for (int s = 0; s < splits; ++s) v += at[s * m * n + j];
-        finish1<T, kAnyActivation>(
-            e, row, col + j, n, v,
-            e.bias ? to_float(static_cast<const T*>(e.bias)[col + j]) : 0.f);
-      }
+    for (int j = 0; j < 4 && col + j < n; ++j) {
+      float v = 0.f;
+      for (int s = 0; s < splits; ++s) v += at[s * m * n + j];
+      finish1<T, kAnyActivation>(e, row, col + j, n, v,
+                                 e.bias ? to_float(static_cast<const T*>(e.bias)[col + j]) : 0.f);
     }
   }
 }
@@ -522,9 +545,19 @@ struct Split {
   bool fits;  // tile counts fit the kernel's integers
 };
 
+// K stages of 64 that a 16-bit product adds up in one TMEM accumulator.  The tensor core
+// truncates when it adds 16 products to it, always to the same side of a sum of one sign:
+// measured, 7e-5 of such a sum over 16,384 elements (2.3 2^-24 of the sum so far a step), and
+// growing with their number, where rounding to float16 may be off by 2.4e-4.  Sums over more
+// than 8,192 elements are split, and the parts joined in float32.  (float32 products move
+// theirs out every 256 elements.)
+constexpr int64_t kMostChunks = 128;
+
 // The K axis is split when the output has too few tiles to fill the SMs: at least four
-// stages of K per split (the pipeline's depth), and no more splits than fill one wave.
-Split plan_product(int64_t m, int64_t n, int64_t k, int device, int most_columns = 128) {
+// stages of K per split (the pipeline's depth), and no more splits than fill one wave unless
+// kMostChunks asks for them.
+Split plan_product(int64_t m, int64_t n, int64_t k, bool f32, int device,
+                   int most_columns = 128) {
   Split s{};
   s.bn = n <= 64 || most_columns == 64 ? 64 : 128;
   const int64_t tm = ceil_div(m, kBM), tn = ceil_div(n, s.bn), chunks = ceil_div(k, kBK);
@@ -536,6 +569,7 @@ Split plan_product(int64_t m, int64_t n, int64_t k, int device, int most_columns
   const int64_t sms = sm_count(device);
   int64_t splits = tm * tn >= sms ? 1 : sms / (tm * tn);
   if (splits > chunks / 4) splits = chunks / 4;
+  if (!f32 && splits < ceil_div(chunks, kMostChunks)) splits = ceil_div(chunks, kMostChunks);
   if (splits < 1) splits = 1;
   s.chunks_per_split = static_cast<int>(ceil_div(chunks, splits));
   s.splits = static_cast<int>(ceil_div(chunks, s.chunks_per_split));
@@ -570,6 +604,7 @@ PairPlan plan_pair(int64_t m, int64_t n, int64_t k, int device) {
   s.chunks = static_cast<int>(chunks);
   int64_t splits = tm * tn >= pairs ? 1 : pairs / (tm * tn);
   if (splits > chunks / 8) splits = chunks / 8;
+  if (splits < ceil_div(chunks, kMostChunks)) splits = ceil_div(chunks, kMostChunks);
   if (splits < 1) splits = 1;
   s.chunks_per_split = static_cast<int>(ceil_div(chunks, splits));
   s.splits = static_cast<int>(ceil_div(chunks, s.chunks_per_split));
@@ -584,7 +619,7 @@ bool use_pair(int64_t m, int64_t n, int64_t k) {
 
 // Bytes of partial products, whichever kernel a call's pointers let it take.
 size_t split_bytes(int64_t m, int64_t n, int64_t k, int dtype, int device) {
-  int64_t splits = plan_product(m, n, k, device).splits;
+  int64_t splits = plan_product(m, n, k, dtype == ICTC_DTYPE_F32, device).splits;
   if (dtype != ICTC_DTYPE_F32) {
     const int64_t q = plan_pair(m, n, k, device).splits;
     if (q > splits) splits = q;
@@ -914,7 +949,7 @@ int run_product(const T* a, int64_t lda, const T* b, int64_t ldb, int64_t m, int
     p.e = e;
   };
   if constexpr (sizeof(T) == 4) {
-    const Split s = plan_product(m, n, k, device);
+    const Split s = plan_product(m, n, k, true, device);
     if (!s.fits) return fail(ICTC_ERR_UNSUPPORTED, "linear: a dimension is too large");
     take(s);
     OperandMaps maps;
@@ -930,7 +965,7 @@ int run_product(const T* a, int64_t lda, const T* b, int64_t ldb, int64_t m, int
   }
   // A float32 tile is 64 columns wide: the cut parts of a wider one do not fit a producer's
   // registers.  (More tiles are never more splits, for which `partial` has room.)
-  const Split s = plan_product(m, n, k, device, sizeof(T) == 4 ? 64 : 128);
+  const Split s = plan_product(m, n, k, sizeof(T) == 4, device, sizeof(T) == 4 ? 64 : 128);
   if (!s.fits) return fail(ICTC_ERR_UNSUPPORTED, "linear: a dimension is too large");
   take(s);
   int st;

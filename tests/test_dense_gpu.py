@@ -278,6 +278,22 @@ def test_linear_strides_and_batches(dtype, cuda_device):
                          y.detach().reshape(-1, n), (grads[0].reshape(-1, 40), grads[1]), dtype)
 
 
+@pytest.mark.parametrize("dtype", DTYPES[1:])
+@pytest.mark.parametrize("shape", [(1100, 100000, 1100), (96, 60000, 520), (70, 40001, 40)])
+def test_linear_long_sums_of_one_sign(shape, dtype, cuda_device):
+    """The tensor core truncates each time it adds 16 products to an accumulator (by up to
+    2 U of it, which grows to the sum), always to the same side of a sum of one sign.  No
+    accumulator takes more than 8,192 elements; seen in the float32 value before the
+    activation, which is not rounded to 16 bits."""
+    from ictc_o2_hp_b200 import dense
+    m, k, n = shape
+    x = rand((m, k), dtype, cuda_device, 46).abs()
+    w = rand((n, k), dtype, cuda_device, 47, 0.01).abs()
+    p = dense._load().linear_forward(x, w, None, None, dense.ACTIVATIONS["silu"], True)[1]
+    want = x.double() @ w.double().t()
+    within("p", p, want, (1024 + 64) * U * want)
+
+
 THIN = [1, 2, 3, 5, 7, 8]
 
 
