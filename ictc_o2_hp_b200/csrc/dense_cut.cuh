@@ -6,10 +6,11 @@
 // order that the MMA reads; one thread issues the MMAs; eight epilogue warps move sums out
 // of TMEM, which holds two sets, every 256 elements of K.
 //
-// What bounds it: an MMA reads its operands from shared memory at 64 bytes a cycle.  A
-// 128 x 128 tile's step of 16 takes 6 x 8 KB (768 cycles, the arithmetic 384); meeting
-// b1 | b2 in one MMA with a1 saves one reading of A (704).  A 64-column tile meets b1 | b2
-// | b3 at once and needs three MMAs (384).  65,536 x 128 x 512: forward with gelu and p 118
+// What bounds it, as far as the timings tell (they fit an MMA that reads its operands from
+// shared memory at 64 bytes a cycle; no counter was read): a 128 x 128 tile's step of 16 takes
+// 6 x 8 KB (768 cycles, the arithmetic 384); meeting b1 | b2 in one MMA with a1 saves one
+// reading of A (704).  A 64-column tile meets b1 | b2 | b3 at once and needs three MMAs (384).
+//  65,536 x 128 x 512: forward with gelu and p 118
 // us (73 TFLOP/s of float32 products), d W 84 us, d^T x 67 us (128 TFLOP/s); with operands
 // staged through registers 182, 109 and 95.
 #pragma once

@@ -351,7 +351,8 @@ ICTC_API int32_t ictc_o2_linear_workspace(int64_t rows, int64_t in, int64_t out,
  * [out] or null, residual [rows, out] or null, y [rows, out].  preact receives p in
  * float32 for the backward (needed there unless the activation is none), or is null.
  * float32 products run on the tensor cores with each operand cut exactly into three
- * bf16 parts; errors are those of a float32 product. */
+ * bf16 parts, of whose nine products the six largest are summed: errors of 1e-7 to 5e-7
+ * in the 2-norm.  An infinity times a subnormal below 2^-133 is NaN there. */
 ICTC_API int32_t ictc_o2_linear_forward(const void* x, int64_t x_stride, const void* weight,
                                         int64_t weight_stride, const void* bias,
                                         const void* residual, int64_t residual_stride, void* y,
@@ -361,7 +362,8 @@ ICTC_API int32_t ictc_o2_linear_forward(const void* x, int64_t x_stride, const v
 
 /* d = grad_output act'(p); grad_x = d weight, grad_weight = d^T x, grad_bias = sum of
  * d's rows (the residual's gradient is grad_output itself).  16-bit types round d to
- * their type before the products, as they would a tensor.  Any output may be null.
+ * their type before the products, as they would a tensor (errors 1.4 times those of
+ * rounding the results alone).  Any output may be null.
  * rows = 0 clears grad_weight and grad_bias. */
 ICTC_API int32_t ictc_o2_linear_backward(
     const void* x, int64_t x_stride, const void* weight, int64_t weight_stride,
