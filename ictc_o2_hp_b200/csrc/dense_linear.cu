@@ -673,6 +673,19 @@ int launch_cut(const OperandMaps& maps, const ProductArgs& p, int device, cudaSt
   int st = ICTC_OK;
   for_epilogue<!A_MN && !B_MN>(p, [&](auto act) {
     const auto kernel = cut_product_kernel<A_MN, B_MN, BN, act.value>;
+    // the warpgroups' shares are drawn from what the block is launched with: a build that
+    // gives its threads fewer registers would wait for them for good
+    static const bool shares_fit = [&] {
+      cudaFuncAttributes a{};
+      return cudaFuncGetAttributes(&a, kernel) == cudaSuccess &&
+             a.numRegs >= kCutLaunchRegisters;
+    }();
+    if (!shares_fit) {
+      st = fail(ICTC_ERR_UNSUPPORTED,
+                "float32 product: built with fewer than %d registers a thread",
+                kCutLaunchRegisters);
+      return;
+    }
     st = allow_smem(reinterpret_cast<const void*>(kernel), kCutSmem<BN>);
     if (st == ICTC_OK) kernel<<<grid, kCutThreads, kCutSmem<BN>, stream>>>(maps, p);
   });
