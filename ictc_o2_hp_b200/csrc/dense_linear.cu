@@ -546,17 +546,18 @@ struct Split {
   bool fits;  // tile counts fit the kernel's integers
 };
 
-// K stages of 64 that a 16-bit product adds up in one TMEM accumulator.  The tensor core
-// truncates when it adds 16 products to it, always to the same side of a sum of one sign:
-// measured, 7e-5 of such a sum over 16,384 elements (2.3 2^-24 of the sum so far a step), and
-// growing with their number, where rounding to float16 may be off by 2.4e-4.  Sums over more
-// than 8,192 elements are split, and the parts joined in float32.  (float32 products move
-// theirs out every 256 elements.)
-constexpr int64_t kMostChunks = 128;
+// Parts of K that a 16-bit product needs for its sums' sake.  The tensor core truncates when
+// it adds 16 products to an accumulator, always to the same side of a sum of one sign:
+// measured, 2.3 2^-24 of the sum so far a step, 7e-5 of the whole after 16,384 elements and
+// growing with their number, where rounding to float16 may be off by 2.4e-4.  Longer sums are
+// taken in parts of at most 8,192 elements, joined in float32 (a limit of 8,192 for all would
+// cost the training step of 16,384 x 4,096 x 4,096 44 us in 1,470).  float32 products move
+// theirs out every 256 elements.
+int64_t long_sum_parts(int64_t chunks) { return chunks <= 256 ? 1 : ceil_div(chunks, 128); }
 
 // The K axis is split when the output has too few tiles to fill the SMs: at least four
 // stages of K per split (the pipeline's depth), and no more splits than fill one wave unless
-// kMostChunks asks for them.
+// long_sum_parts asks for them.
 Split plan_product(int64_t m, int64_t n, int64_t k, bool f32, int device,
                    int most_columns = 128) {
   Split s{};
@@ -570,7 +571,7 @@ Split plan_product(int64_t m, int64_t n, int64_t k, bool f32, int device,
   const int64_t sms = sm_count(device);
   int64_t splits = tm * tn >= sms ? 1 : sms / (tm * tn);
   if (splits > chunks / 4) splits = chunks / 4;
-  if (!f32 && splits < ceil_div(chunks, kMostChunks)) splits = ceil_div(chunks, kMostChunks);
+  if (!f32 && splits < long_sum_parts(chunks)) splits = long_sum_parts(chunks);
   if (splits < 1) splits = 1;
   s.chunks_per_split = static_cast<int>(ceil_div(chunks, splits));
   s.splits = static_cast<int>(ceil_div(chunks, s.chunks_per_split));
@@ -605,7 +606,7 @@ PairPlan plan_pair(int64_t m, int64_t n, int64_t k, int device) {
   s.chunks = static_cast<int>(chunks);
   int64_t splits = tm * tn >= pairs ? 1 : pairs / (tm * tn);
   if (splits > chunks / 8) splits = chunks / 8;
-  if (splits < ceil_div(chunks, kMostChunks)) splits = ceil_div(chunks, kMostChunks);
+  if (splits < long_sum_parts(chunks)) splits = long_sum_parts(chunks);
   if (splits < 1) splits = 1;
   s.chunks_per_split = static_cast<int>(ceil_div(chunks, splits));
   s.splits = static_cast<int>(ceil_div(chunks, s.chunks_per_split));

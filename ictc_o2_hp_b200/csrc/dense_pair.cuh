@@ -9,8 +9,7 @@
 //
 // Bound by the tensor cores.  bf16, 16,384 x 4,096 x 4,096 (550 GFLOP a product): d W 345 us
 // (1.59 PFLOP/s, 0.95 of the measured burst rate), x W^T with SiLU, residual and p 385 us, d^T x
-// 365 us and 44 us that join its two parts (in one part 390 us: 256 tiles are 3.5 waves of 74
-// pairs).  Kernel times of short bursts; a long run of whole calls is some 15% slower.
+// 390 us (256 tiles are 3.5 waves of 74 pairs).  Kernel times of short bursts; a long run of whole calls is some 15% slower.
 #pragma once
 
 #include <cuda_runtime.h>
