@@ -1081,6 +1081,13 @@ struct LinearPlan {
 
 constexpr int64_t kSlopeParts = 296;
 
+// Most outputs for which the backward of a thin layer leaves the narrow kernel.  That has two
+// launches and a fixed time a tile (with SiLU, kernel times of 1,048,576 rows: 223 us float32,
+// 150 bf16; 370 and 297 of a million rows that are not whole blocks); the thin forms have five
+// and read d for each product: 8 x 8 66 and 59 us, 22 x 1 93 and 84, 61 x 8 294 (narrow 486),
+// 8 x 64 348 and 250 (narrow 237 and 148), 7 x 61 450 (narrow 369).
+constexpr int64_t kThinOutputs = 24;
+
 LinearPlan plan_linear(int64_t m, int64_t n, int64_t k, int dtype, int activation, int32_t layout,
                        bool backward, int device) {
   LinearPlan b{};
@@ -1099,10 +1106,8 @@ LinearPlan plan_linear(int64_t m, int64_t n, int64_t k, int dtype, int activatio
       b.thin = Thin::dot_swapped;
     if (b.thin == Thin::none) b.few = m <= kFewRows;
     b.narrow = b.narrow && !b.few && b.thin == Thin::none;
-  } else if (thin && (n * size % 16 != 0 || k * size % 16 != 0) &&
+  } else if (thin && n <= kThinOutputs &&
              m > 2 * kNarrowTile * static_cast<int64_t>(sm_count(device))) {
-    // rows that are not whole blocks: the narrow kernel reads them value by value, which
-    // more than a few tiles an SM cannot hide
     b.narrow = false;
   }
   b.align = !rows_aligned && b.thin == Thin::none && !thin && worth_aligning(m, n, k);
