@@ -726,13 +726,25 @@ bool dot_fits(int64_t rows, int64_t len, int64_t count) {
          (rows >= 1024 || len <= 8192);
 }
 
+// Whether a large 16-bit product goes to the SM pairs all the same: with TMA (`tiles`) their
+// mostly empty tiles still read it at up to 4.6 TB/s, where from three (dot) or five (outer,
+// gram) numbers a value on the FMAs and conversions take longer.  bf16 16,384 x 4,096 x 8
+// forward 29 us (dot 83), x 1 30 (26); 65,536 x 1,024 x 4 forward 30 (dot 38), dx 77 (outer 65),
+// dW 55 (gram 54); 8 x 4,096 x 16,384 dx 47 (gram 79), dW 77 (outer 89).  float32 tiles do not
+// (16,384 x 4,096 x 8 forward 111 us, dot 61).
+bool pairs_read_faster(bool tiles, int64_t one, int64_t two, int64_t count, int64_t most) {
+  return tiles && count > most && one > kNarrow && two > kNarrow && one * two >= (1 << 21);
+}
+
 // The form of a product with a dimension of at most kThin.  A few rows over a weight whose
 // rows run along the sum (the forward's) are decided by the caller.
-Thin thin_form(bool a_mn, bool b_mn, int64_t m, int64_t n, int64_t k) {
-  if (k <= kThin) return Thin::outer;
-  if (n <= kThin && a_mn) return Thin::gram_swapped;
-  if (n <= kThin && dot_fits(m, k, n)) return Thin::dot;
-  if (m <= kThin && b_mn) return Thin::gram;
+Thin thin_form(bool a_mn, bool b_mn, int64_t m, int64_t n, int64_t k, bool tiles) {
+  if (k <= kThin) return pairs_read_faster(tiles, m, n, k, 4) ? Thin::none : Thin::outer;
+  if (n <= kThin && a_mn)
+    return pairs_read_faster(tiles, m, k, n, 4) ? Thin::none : Thin::gram_swapped;
+  if (n <= kThin && dot_fits(m, k, n))
+    return pairs_read_faster(tiles, m, k, n, 2) ? Thin::none : Thin::dot;
+  if (m <= kThin && b_mn) return pairs_read_faster(tiles, n, k, m, 4) ? Thin::none : Thin::gram;
   return Thin::none;
 }
 
@@ -770,13 +782,12 @@ size_t gram_bytes(int64_t rows, int64_t width, int64_t count, size_t size, int d
 // Workspace of a product, whichever kernel it takes.
 size_t product_bytes(bool a_mn, bool b_mn, int64_t m, int64_t n, int64_t k, int dtype,
                      int device) {
-  const size_t size = dtype_size(dtype);
-  switch (thin_form(a_mn, b_mn, m, n, k)) {
-    case Thin::none: return split_bytes(m, n, k, dtype, device);
-    case Thin::gram: return gram_bytes(k, n, m, size, device);
-    case Thin::gram_swapped: return gram_bytes(k, m, n, size, device);
-    default: return 0;
-  }
+  const size_t size = dtype_size(dtype), tiles = split_bytes(m, n, k, dtype, device);
+  size_t thin = 0;
+  const Thin form = thin_form(a_mn, b_mn, m, n, k, false);
+  if (form == Thin::gram) thin = gram_bytes(k, n, m, size, device);
+  if (form == Thin::gram_swapped) thin = gram_bytes(k, m, n, size, device);
+  return tiles > thin ? tiles : thin;
 }
 
 // Calls f with the small dimension as a compile-time constant.
@@ -829,13 +840,14 @@ int launch_dot_columns(const ThinArgs& p, int64_t sms, cudaStream_t stream) {
 }
 
 // Lanes of a row: enough that consecutive lanes read whole sectors, and no more than leave
-// each a few accesses, because every row's sums are joined over them (float32 343,990 x 65
-// x 7: 51 us with 4 lanes of 33 accesses; 136,107 x 175 x 6, as many values: 89 with 32 of 6).
+// each a few accesses, because every row's sums are joined over them (float32 136,107 x 175 x
+// 6: 41 us with 4 lanes of 44 accesses, 89 with 32 of 6), unless rows are few (bf16 1,000 x 512
+// x 8: 14 us with 4 lanes, on 8 SMs).
 template <typename T, int V>
 int launch_dot_lanes(const ThinArgs& p, int64_t sms, cudaStream_t stream) {
   const int accesses = p.len / V;
   if (accesses <= 8) return launch_dot_columns<T, V, 1>(p, sms, stream);
-  if (accesses < 128 || (accesses < 1024 && p.rows >= sms * 256))
+  if (accesses < 16 || (accesses < 1024 && p.rows >= sms * 256))
     return launch_dot_columns<T, V, 4>(p, sms, stream);
   return launch_dot_columns<T, V, 32>(p, sms, stream);
 }
@@ -912,7 +924,7 @@ int run_thin(Thin form, const T* a, int64_t lda, const T* b, int64_t ldb, int64_
 // C = epilogue(A B^T); `partial` holds product_bytes().
 template <typename T, bool A_MN, bool B_MN>
 int run_product(const T* a, int64_t lda, const T* b, int64_t ldb, int64_t m, int64_t n, int64_t k,
-                Epilogue e, float* partial, cudaStream_t stream) {
+                Epilogue e, float* partial, bool tiles, cudaStream_t stream) {
   const int device = current_device();
   e.vec = vec_epilogue<T>(e, n);
   const auto join = [&](int splits) {
@@ -925,7 +937,7 @@ int run_product(const T* a, int64_t lda, const T* b, int64_t ldb, int64_t m, int
     return err == cudaSuccess ? ICTC_OK : cuda_fail(err, "linear split join launch");
   };
   if constexpr (B_MN) {  // a gradient (the forward's form is in its plan)
-    if (const Thin form = thin_form(A_MN, B_MN, m, n, k); form != Thin::none)
+    if (const Thin form = thin_form(A_MN, B_MN, m, n, k, tiles); form != Thin::none)
       return run_thin<T, A_MN, B_MN>(form, a, lda, b, ldb, m, n, k, e, partial, stream);
   }
   if constexpr (sizeof(T) == 2) {
@@ -1075,7 +1087,8 @@ int32_t layout_of(const void* x, int64_t ldx, const void* w, int64_t ldw, const 
 // Byte offsets of the workspace's parts, and its size.
 struct LinearPlan {
   bool few, narrow, align;
-  Thin thin;  // the forward's
+  bool tiles;  // 16-bit operands that TMA can address
+  Thin thin;   // the forward's
   size_t d, x, w, g, columns, partial, total;
 };
 
@@ -1094,12 +1107,13 @@ LinearPlan plan_linear(int64_t m, int64_t n, int64_t k, int dtype, int activatio
   const size_t size = dtype_size(dtype);
   const int64_t full = static_cast<int64_t>(16 / size);
   const bool rows_aligned = layout & ICTC_LINEAR_ALIGNED;
+  b.tiles = size == 2 && rows_aligned;
   // both products of the backward are thin: no operand is copied to aligned rows
   const bool thin = backward && (n <= kThin || m <= kThin || (k <= kThin && dot_fits(m, n, k)));
   b.narrow = (layout & ICTC_LINEAR_PACKED) && n <= kNarrow && k <= kNarrow && m <= (1ll << 36);
   if (!backward) {
     b.few = m <= kFewRows && rows_aligned && k % full == 0;
-    if (!b.few) b.thin = thin_form(false, false, m, n, k);
+    if (!b.few) b.thin = thin_form(false, false, m, n, k, b.tiles);
     // a few rows over a weight that few_rows_kernel and TMA would read by elements
     if (!b.few && b.thin == Thin::none && m <= kThin && (m <= kFewRows || !rows_aligned) &&
         dot_fits(n, k, m))
@@ -1225,7 +1239,8 @@ int run_linear_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, E
     if (st != ICTC_OK) return st;
   }
   return run_product<T, false, false>(xt, ldx, wt, ldw, m, n, k, e,
-                                      reinterpret_cast<float*>(workspace + plan.partial), stream);
+                                      reinterpret_cast<float*>(workspace + plan.partial),
+                                      plan.tiles, stream);
 }
 
 struct SlopePlan {
@@ -1309,12 +1324,12 @@ int run_linear_backward(const void* x, int64_t ldx, const void* w, int64_t ldw,
   if (dx) {
     e.out = dx;
     const int st =
-        run_product<T, false, true>(d, ldd, wt, ldw, m, k, n, e, partial, stream);
+        run_product<T, false, true>(d, ldd, wt, ldw, m, k, n, e, partial, plan.tiles, stream);
     if (st != ICTC_OK) return st;
   }
   if (dw) {
     e.out = dw;
-    return run_product<T, true, true>(d, ldd, xt, ldx, n, k, m, e, partial, stream);
+    return run_product<T, true, true>(d, ldd, xt, ldx, n, k, m, e, partial, plan.tiles, stream);
   }
   return ICTC_OK;
 }
