@@ -12,13 +12,14 @@
 //
 // Bound by HBM where few numbers meet each value of the large operand (dot, float32 7,245 x
 // 14,302 x 1: 85 us, 4.9 TB/s), by the reads of the small operand beside it towards eight
-// (dot, float32 136,107 x 175 x 6: 41 us; outer, float32 1,048,576 x 8 x 64 with SiLU: 102 us,
-// 2.9 TB/s; the three products of a float16 training step of 7 x 4,826 x 9,305, rows off the
-// boundaries: 53, 68 and 99 us for 90 MB each).  Calls that took tiles before: float32 937,427 x 89 x 6 forward 1,139 us (149 here), 343,990 x 65 x
-// 7 407 us (52), 1 x 14,793 x 3,978 164 us (54).  Against the narrow kernel, which takes
-// widths up to 64 otherwise (kernel times, SiLU, float32 and bf16): 37 x 8 x 64 4.5 and 3.6 us
-// (narrow 6.8 and 6.0), 1,048,576 x 8 x 64 101 and 100 (151 and 114), x 64 x 8 90 and 87 (140 and
-// 98), x 32 x 1 49 and 16 (176 and 176).
+// (dot, float32 136,107 x 175 x 6: 41 us; outer, float32 1,048,576 x 8 x 64 with SiLU: 101 us,
+// 3.0 TB/s; the three products of a float16 training step of 7 x 4,826 x 9,305, rows off the
+// boundaries: 53, 68 and 99 us for 90 MB each).  Calls that took tiles before: float32
+// 937,427 x 89 x 6 forward 1,139 us (148 here), 343,990 x 65 x 7 407 us (52), 1 x 14,793 x
+// 3,978 164 us (54).  Against the narrow kernel, which takes widths up to 64 otherwise (kernel
+// times, SiLU, float32 and bf16): 37 x 8 x 64 4.5 and 3.6 us (narrow 6.8 and 6.0),
+// 1,048,576 x 8 x 64 101 and 100 (151 and 114), x 64 x 8 90 and 87 (140 and 98), x 32 x 1 49
+// and 16 (176 and 176).
 #pragma once
 
 #include <cuda_runtime.h>
