@@ -6,10 +6,11 @@
 // order that the MMA reads; one thread issues the MMAs; eight epilogue warps move sums out
 // of TMEM, which holds two sets, every 256 elements of K.
 //
-// What bounds it, as far as the timings tell (they fit an MMA that reads its operands from
-// shared memory at 64 bytes a cycle; no counter was read): a 128 x 128 tile's step of 16 takes
-// 6 x 8 KB (768 cycles, the arithmetic 384); meeting b1 | b2 in one MMA with a1 saves one
-// reading of A (704).  A 64-column tile meets b1 | b2 | b3 at once and needs three MMAs (384).
+// What bounds it: no single unit (65,536 x 128 x 512: the tensor pipe is busy 19% to 34% of
+// the time, LSU wavefronts 40% to 48%, issue slots 37% to 54%, DRAM 20% to 28%), so the chain
+// raw tile, cut, MMA, accumulator.  An MMA fetches its operands from shared memory every time:
+// six of a 128 x 128 tile's step of 16 read 6 x 8 KB; meeting b1 | b2 in one MMA with a1 saves
+// one reading of A.  A 64-column tile meets b1 | b2 | b3 at once and needs three MMAs.
 //  65,536 x 128 x 512: forward with gelu and p 118
 // us (73 TFLOP/s of float32 products), d W 84 us, d^T x 67 us (128 TFLOP/s); with operands
 // staged through registers 182, 109 and 95.

@@ -210,8 +210,7 @@ __device__ __forceinline__ uint32_t unit_bits(const float (&v)[4]) {
 
 // The `steps` K steps of one product with 64 columns; strides in the descriptors' units of
 // 16 bytes.  The parts of B lie behind one another as 192 columns, so that a part of A
-// meets all the parts of B that it needs in one MMA, which fetches A again every time (the
-// timings fit 64 bytes of operands a cycle out of shared memory):
+// meets all the parts of B that it needs in one MMA, which fetches A again every time:
 //   a1 (b1 | b2 | b3), a2 (b1 | b2), a3 b1   into sums of order 0, 1 and 2, 64 columns each.
 template <int P>
 __device__ __forceinline__ void issue_cut(uint32_t d, uint64_t a, uint64_t a_step, uint64_t a_part,
