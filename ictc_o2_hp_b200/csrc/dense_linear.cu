@@ -717,7 +717,9 @@ int launch_product(const ProductArgs& p, int device, cudaStream_t stream) {
 
 enum class Thin { none, dot, dot_swapped, outer, gram, gram_swapped };
 
-int thin_columns(int64_t count) { return count <= 2 ? static_cast<int>(count) : count <= 4 ? 4 : 8; }
+int thin_columns(int64_t count) {
+  return count <= 2 ? static_cast<int>(count) : count <= 4 ? 4 : kThin;
+}
 
 // The staged operand fits, and there are rows enough to fill the SMs without splitting the
 // sum (or it is short).
@@ -753,8 +755,8 @@ struct StripPlan {
   unsigned blocks_x, blocks_y;
 };
 
-// Strips of 32 lanes of `vec` (or, strided, four) columns, and as many blocks of rows as fill the SMs, each
-// thread's at least four rows (the loads that it has in flight).
+// Strips of 32 lanes of `vec` (or, strided, four) columns, and as many blocks of rows as fill
+// the SMs, each thread's at least four rows (the loads that it has in flight).
 StripPlan plan_strips(int64_t rows, int64_t width, int vec, int device) {
   StripPlan s{};
   const int64_t units = ceil_div(width, vec > 1 ? vec : kStrided);
@@ -907,7 +909,8 @@ int run_thin(Thin form, const T* a, int64_t lda, const T* b, int64_t ldb, int64_
     const StripPlan s = plan_strips(p.rows, p.width, vec ? kFull : 1, device);
     p.lanes = s.lanes;
     for_thin(p.count, [&](auto nc) {
-      const auto kernel = vec ? thin_gram_kernel<T, kFull, nc.value> : thin_gram_kernel<T, 1, nc.value>;
+      const auto kernel =
+          vec ? thin_gram_kernel<T, kFull, nc.value> : thin_gram_kernel<T, 1, nc.value>;
       kernel<<<dim3(s.blocks_x, s.blocks_y), kStripThreads, 0, stream>>>(p);
     });
     const cudaError_t err = cudaGetLastError();
