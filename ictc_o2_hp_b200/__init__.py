@@ -3,15 +3,18 @@
 Public names mirror the reference package ``ictc_o2_hp`` (src/ictc_o2_hp/__init__.py):
 ``TensorProduct``, ``TupleTensorProduct``, ``ComponentMajorTensorProduct``,
 ``UvuTensorProduct`` and ``RadialUvuTensorProduct``.  ``LayerNorm``, ``Linear``,
-``ResidualBlock`` and ``RadialTrunk`` (module ``dense``) are the networks around them.
+``GatedLinear``, ``ResidualBlock``, ``GatedBlock`` and ``RadialTrunk`` (module ``dense``) are
+the networks around them, ``grad_norm``, ``clip_grad_norm_`` and ``clip_grads`` (module
+``gradients``) what a training step does with their gradients.
 Imports are lazy so that the package imports without a GPU.
 """
 
 __version__ = "0.1.0"
 __all__ = [
     "TensorProduct", "TupleTensorProduct", "ComponentMajorTensorProduct",
-    "UvuTensorProduct", "RadialUvuTensorProduct", "LayerNorm", "Linear", "ResidualBlock",
-    "RadialTrunk", "__version__",
+    "UvuTensorProduct", "RadialUvuTensorProduct", "LayerNorm", "Linear", "GatedLinear",
+    "ResidualBlock", "GatedBlock", "RadialTrunk", "grad_norm", "clip_grad_norm_", "clip_grads",
+    "__version__",
 ]
 
 
@@ -25,7 +28,11 @@ def __getattr__(name):
     if name == "RadialUvuTensorProduct":
         from .radial import RadialUvuTensorProduct
         return RadialUvuTensorProduct
-    if name in {"LayerNorm", "Linear", "ResidualBlock", "RadialTrunk"}:
+    if name in {"LayerNorm", "Linear", "GatedLinear", "ResidualBlock", "GatedBlock",
+                "RadialTrunk"}:
         from . import dense
         return getattr(dense, name)
+    if name in {"grad_norm", "clip_grad_norm_", "clip_grads"}:
+        from . import gradients
+        return getattr(gradients, name)
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

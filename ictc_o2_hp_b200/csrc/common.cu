@@ -152,4 +152,4 @@ extern "C" int32_t ictc_o2_device_error(int32_t* code) {
   return ICTC_OK;
 }
 
-extern "C" int32_t ictc_o2_abi_version(void) { return 102; }
+extern "C" int32_t ictc_o2_abi_version(void) { return 103; }

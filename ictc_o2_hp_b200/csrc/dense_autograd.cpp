@@ -1,5 +1,5 @@
 // The dense operators' autograd layer: argument checks, allocation, and the autograd nodes
-// of layer norm and the linear layer, over the C ABI in ictc_o2_b200.h.
+// of layer norm and the linear layers, over the C ABI in ictc_o2_b200.h.
 //
 // In C++ because these operators are called on a few rows as often as on millions: an
 // autograd.Function in Python over ctypes took 58 us a training call beside the engine's
@@ -36,13 +36,17 @@ struct Api {
   decltype(&ictc_o2_linear_workspace) linear_workspace;
   decltype(&ictc_o2_linear_forward) linear_forward;
   decltype(&ictc_o2_linear_backward) linear_backward;
+  decltype(&ictc_o2_gated_linear_workspace) gated_workspace;
+  decltype(&ictc_o2_gated_linear_forward) gated_forward;
+  decltype(&ictc_o2_gated_linear_backward) gated_backward;
 };
 
 Api api{};
 
 // The custom operators in Python, which run the raw directions at the end of this file.
 struct Ops {
-  PyObject *norm_forward, *norm_backward, *linear_forward, *linear_backward;
+  PyObject *norm_forward, *norm_backward, *linear_forward, *linear_backward, *gated_forward,
+      *gated_backward;
 };
 
 Ops ops{};
@@ -142,6 +146,24 @@ void check_linear(const Tensor& x, const Tensor& weight, const Tensor& bias,
     for (int64_t i = 0; same && i + 1 < x.dim(); ++i) same = residual.size(i) == x.size(i);
     TORCH_CHECK_VALUE(same, "linear: residual must have the output's shape, got ",
                       residual.sizes());
+  }
+}
+
+void check_gated(const Tensor& x, const Tensor& weight, const Tensor& bias, int64_t code) {
+  check_input("gated_linear", x);
+  TORCH_CHECK_VALUE(code >= ICTC_ACT_NONE && code <= ICTC_ACT_GELU_TANH, "unknown activation");
+  TORCH_CHECK_VALUE(weight.dim() == 2 && x.dim() >= 1 && x.size(-1) == weight.size(1),
+                    "gated_linear: x [..., in] and weight [2 hidden, in] do not match: ",
+                    x.sizes(), " and ", weight.sizes());
+  TORCH_CHECK_VALUE(weight.size(0) >= 2 && weight.size(0) % 2 == 0 && weight.size(1) >= 1,
+                    "gated_linear: weight must have an even number of rows (gate, then up) and "
+                    "at least one column, got ", weight.sizes());
+  check_like("gated_linear", "weight", weight, x);
+  if (bias.defined()) {
+    check_like("gated_linear", "bias", bias, x);
+    TORCH_CHECK_VALUE(bias.dim() == 1 && bias.size(0) == weight.size(0),
+                      "gated_linear: bias must have shape [", weight.size(0), "], got ",
+                      bias.sizes());
   }
 }
 
@@ -486,6 +508,127 @@ Tensor linear(const Tensor& x, const Tensor& weight, const std::optional<Tensor>
   return std::get<0>(linear_forward(x, weight, bias, residual, code, false));
 }
 
+// ---------------------------------------------------------------------- gated linear
+
+std::tuple<Tensor, Tensor> gated_forward(const Tensor& x, const Tensor& weight,
+                                         const Tensor& bias_in, int64_t code, bool save) {
+  const c10::cuda::CUDAGuard guard(x.device());
+  const Tensor rows = rows_of(x), w = rows_of(weight), bias = packed(bias_in);
+  const int64_t m = rows.size(0), k = rows.size(1), n = w.size(0) / 2;
+  c10::SmallVector<int64_t, 6> shape(x.sizes().begin(), x.sizes().end());
+  shape.back() = n;
+  const Tensor y = at::empty(shape, x.options());
+  Tensor preact;
+  if (save) preact = at::empty({m, 2 * n}, x.options().dtype(at::kFloat));
+  const int32_t dtype = code_of(x.scalar_type()), act = static_cast<int32_t>(code);
+  size_t bytes = 0, other = 0;
+  check(api.gated_workspace(m, k, n, dtype, act, layout_of(rows, w, nullptr), save,
+                            x.device().index(), &bytes, &other),
+        "gated_linear_workspace");
+  const Tensor space = scratch(bytes, x);
+  check(api.gated_forward(rows.data_ptr(), rows.stride(0), w.data_ptr(), w.stride(0), data(bias),
+                          y.data_ptr(), floats(preact), data(space), bytes, m, k, n, dtype, act,
+                          stream_of(x)),
+        "gated_linear_forward");
+  return {y, preact};
+}
+
+std::tuple<Tensor, Tensor, Tensor> gated_backward(const Tensor& x, const Tensor& weight,
+                                                  const Tensor& preact, const Tensor& grad,
+                                                  int64_t code, bool need_x, bool need_w,
+                                                  bool need_b) {
+  const c10::cuda::CUDAGuard guard(x.device());
+  const Tensor rows = rows_of(x), w = rows_of(weight), g = rows_of(grad);
+  const int64_t m = rows.size(0), k = rows.size(1), n = w.size(0) / 2;
+  Tensor dx, dw, db;
+  if (need_x) dx = at::empty(x.sizes(), x.options());
+  if (need_w) dw = at::empty({2 * n, k}, x.options());
+  if (need_b) db = at::empty({2 * n}, x.options());
+  const int32_t dtype = code_of(x.scalar_type()), act = static_cast<int32_t>(code);
+  size_t bytes = 0, other = 0;
+  check(api.gated_workspace(m, k, n, dtype, act, layout_of(rows, w, nullptr), true,
+                            x.device().index(), &other, &bytes),
+        "gated_linear_workspace");
+  const Tensor space = scratch(bytes, x);
+  check(api.gated_backward(rows.data_ptr(), rows.stride(0), w.data_ptr(), w.stride(0),
+                           floats(preact), g.data_ptr(), g.stride(0), data(dx), data(dw),
+                           data(db), data(space), bytes, m, k, n, dtype, act, stream_of(x)),
+        "gated_linear_backward");
+  return {dx, dw, db};
+}
+
+// act(p) in differentiable operations.
+Tensor activation_formula(const Tensor& p, int64_t code) {
+  if (code == ICTC_ACT_RELU) return p.relu();
+  if (code == ICTC_ACT_SILU) return p * p.sigmoid();
+  if (code == ICTC_ACT_GELU) return 0.5 * p * (1 + (p * M_SQRT1_2).erf());
+  if (code == ICTC_ACT_GELU_TANH)
+    return 0.5 * p * (1 + (M_2_SQRTPI * M_SQRT1_2 * (p + 0.044715 * p * p * p)).tanh());
+  return p;
+}
+
+class GatedLinearFunction : public torch::autograd::Function<GatedLinearFunction> {
+ public:
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight,
+                        const std::optional<Tensor>& bias_in, int64_t code) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const Tensor bias = wanted(bias_in);
+    auto [y, preact] = gated_forward(x, weight, bias, code, true);
+    ctx->save_for_backward({x, weight, bias, preact});
+    ctx->saved_data["code"] = code;
+    return y;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const Tensor& grad = grads[0];
+    if (!grad.defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &weight = saved[1], &preact = saved[3];
+    const int64_t code = ctx->saved_data["code"].toInt();
+    const bool nx = ctx->needs_input_grad(0), nw = ctx->needs_input_grad(1);
+    const bool nb = saved[2].defined() && ctx->needs_input_grad(2);
+    if (!nx && !nw && !nb) return {Tensor(), Tensor(), Tensor(), Tensor()};
+    if (!at::GradMode::is_enabled()) {
+      if (watched({&grad, &x, &weight})) {
+        const auto [dx, dw, db] = through_dispatcher<std::tuple<Tensor, Tensor, Tensor>>(
+            ops.gated_backward, x, weight, preact, grad, code);
+        return {nx ? dx : Tensor(), nw ? dw : Tensor(), nb ? db : Tensor(), Tensor()};
+      }
+      auto [dx, dw, db] = gated_backward(x, weight, preact, grad, code, nx, nw, nb);
+      return {dx, dw, db, Tensor()};
+    }
+    // second derivatives: as in the linear layer
+    const Tensor rows = rows_of(x), g = rows_of(grad).to(at::kFloat);
+    const Tensor p = linear(rows, weight, given(saved[2]), std::nullopt, ICTC_ACT_NONE);
+    const auto halves = ValueOf::apply(p.to(at::kFloat), preact).chunk(2, 1);
+    const Tensor slope = code == ICTC_ACT_NONE ? halves[1] : halves[1] * slope_formula(halves[0], code);
+    const Tensor wide = at::cat({g * slope, g * activation_formula(halves[0], code)}, 1);
+    const Tensor d = wide.to(x.scalar_type());
+    const auto product = [](const Tensor& a, const Tensor& b) {
+      return linear(a, b, std::nullopt, std::nullopt, ICTC_ACT_NONE);
+    };
+    return {nx ? product(d, weight.t()).reshape(x.sizes()) : Tensor(),
+            nw ? (rows.size(0) > 0 ? product(d.t(), rows.t()) : at::matmul(d.t(), rows)) : Tensor(),
+            nb ? wide.sum(0).to(x.scalar_type()) : Tensor(), Tensor()};
+  }
+};
+
+Tensor gated_linear(const Tensor& x, const Tensor& weight, const std::optional<Tensor>& bias_in,
+                    int64_t code) {
+  const Tensor bias = wanted(bias_in);
+  Tensor cast[3] = {x, weight, bias};
+  if (cast_mixed({&cast[0], &cast[1], &cast[2]}))
+    return gated_linear(cast[0], cast[1], given(cast[2]), code);
+  check_gated(x, weight, bias, code);
+  check_tangents("gated_linear", {&x, &weight, &bias});
+  const bool grad = any_grad({&x, &weight, &bias});
+  if (watched({&x, &weight, &bias}))
+    return std::get<0>(through_dispatcher<std::tuple<Tensor, Tensor>>(ops.gated_forward, x, weight,
+                                                                      bias, code, grad));
+  if (grad) return GatedLinearFunction::apply(x, weight, given(bias), code);
+  return std::get<0>(gated_forward(x, weight, bias, code, false));
+}
+
 // ---------------------------------------------- raw directions, for the custom operators
 
 std::tuple<Tensor, Tensor, Tensor> norm_forward_op(const Tensor& x,
@@ -520,16 +663,32 @@ std::tuple<Tensor, Tensor, Tensor> linear_backward_op(const Tensor& x, const Ten
                          true, true);
 }
 
+std::tuple<Tensor, Tensor> gated_forward_op(const Tensor& x, const Tensor& weight,
+                                            const std::optional<Tensor>& bias, int64_t code,
+                                            bool save) {
+  check_gated(x, weight, wanted(bias), code);
+  auto [y, preact] = gated_forward(x, weight, wanted(bias), code, save);
+  if (!save) preact = at::empty({0}, x.options().dtype(at::kFloat));
+  return {y, preact};
+}
+
+std::tuple<Tensor, Tensor, Tensor> gated_backward_op(const Tensor& x, const Tensor& weight,
+                                                     const Tensor& preact, const Tensor& grad,
+                                                     int64_t code) {
+  return gated_backward(x, weight, preact, grad, code, true, true, true);
+}
+
 // The custom operators, held for the life of the process.
 void bind_operators(py::object norm_fwd, py::object norm_bwd, py::object linear_fwd,
-                    py::object linear_bwd) {
-  ops = {norm_fwd.release().ptr(), norm_bwd.release().ptr(), linear_fwd.release().ptr(),
-         linear_bwd.release().ptr()};
+                    py::object linear_bwd, py::object gated_fwd, py::object gated_bwd) {
+  ops = {norm_fwd.release().ptr(),   norm_bwd.release().ptr(),  linear_fwd.release().ptr(),
+         linear_bwd.release().ptr(), gated_fwd.release().ptr(), gated_bwd.release().ptr()};
 }
 
 // Entry points of the loaded kernel library, by address.
 void bind(uintptr_t last_error, uintptr_t norm_fwd, uintptr_t norm_ws, uintptr_t norm_bwd,
-          uintptr_t linear_ws, uintptr_t linear_fwd, uintptr_t linear_bwd) {
+          uintptr_t linear_ws, uintptr_t linear_fwd, uintptr_t linear_bwd, uintptr_t gated_ws,
+          uintptr_t gated_fwd, uintptr_t gated_bwd) {
   const auto set = [](auto& fn, uintptr_t at) { fn = reinterpret_cast<std::decay_t<decltype(fn)>>(at); };
   set(api.last_error, last_error);
   set(api.norm_forward, norm_fwd);
@@ -538,6 +697,9 @@ void bind(uintptr_t last_error, uintptr_t norm_fwd, uintptr_t norm_ws, uintptr_t
   set(api.linear_workspace, linear_ws);
   set(api.linear_forward, linear_fwd);
   set(api.linear_backward, linear_bwd);
+  set(api.gated_workspace, gated_ws);
+  set(api.gated_forward, gated_fwd);
+  set(api.gated_backward, gated_bwd);
 }
 
 }  // namespace
@@ -547,8 +709,11 @@ PYBIND11_MODULE(_dense_autograd, m) {
   m.def("bind_operators", &bind_operators);
   m.def("layer_norm", &layer_norm);
   m.def("linear", &linear);
+  m.def("gated_linear", &gated_linear);
   m.def("norm_forward", &norm_forward_op);
   m.def("norm_backward", &norm_backward_op);
   m.def("linear_forward", &linear_forward_op);
   m.def("linear_backward", &linear_backward_op);
+  m.def("gated_forward", &gated_forward_op);
+  m.def("gated_backward", &gated_backward_op);
 }

@@ -1,0 +1,440 @@
+// The global norm of many tensors, and clipping by it.
+//
+//   norm = sqrt(sum over all tensors of g^2), or max |g|
+//   c = min(1, max_norm / (norm + 1e-6)),  out = c g
+//
+// Bound by HBM: every value is read for the norm, and where c < 1 (or the result goes
+// elsewhere) read again and written.  A launch takes up to 1,024 tensors of mixed types,
+// their addresses and sizes among its arguments, so nothing is copied to the device and a
+// captured call holds all it needs.  Work is cut into chunks of 32 KB that are dealt out to
+// the CTAs in order; a CTA's sum goes to its place in the workspace and every CTA of the
+// second pass adds those up in the same order, so that results do not depend on scheduling.
+// The second pass takes a CTA's chunks from the last to the first: the last ones are still in
+// L2.
+//
+// Squares are added in float32 over the 16 bytes of a load and in float64 beyond.  Where
+// such a short sum leaves float32's safe range it is taken again in float64, so the norm is
+// finite wherever float32 holds it, and small gradients do not vanish.
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <type_traits>
+
+#include "common.cuh"
+#include "dense_types.cuh"
+
+namespace ictc {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kUnits = 8;  // 16-byte units of a chunk per thread
+constexpr int kChunkBytes = kThreads * kUnits * 16;
+constexpr int kBlocksPerSm = 8;
+constexpr int kMostTensors = 1024;  // of a launch: 29 bytes each of its 32,764 of arguments
+
+enum Kind { kTwoNorm = ICTC_GRAD_NORM_2, kMaxNorm = ICTC_GRAD_NORM_MAX };
+
+// Chunk c of a tensor is the c-th whole chunk counted from the 16-byte boundary at or below
+// its first element (its first `shift` elements are not the tensor's).
+template <int N>
+struct Tensors {
+  const void* in[N];
+  void* out[N];
+  int64_t count[N];
+  int first[N + 1];  // chunks before each tensor
+  uint8_t dtype[N];
+  int tensors;
+};
+
+struct Place {
+  int tensor;
+  int64_t chunk;  // in the tensor
+};
+
+template <int N>
+__device__ __forceinline__ Place place_of(const Tensors<N>& list, int chunk) {
+  int low = 0, high = list.tensors;  // first[low] <= chunk < first[high]
+  while (high - low > 1) {
+    const int mid = (low + high) >> 1;
+    if (list.first[mid] <= chunk) low = mid;
+    else high = mid;
+  }
+  return {low, chunk - list.first[low]};
+}
+
+// What a chunk's elements are: the tensor's are [begin, end) of the chunk's.
+template <typename T>
+struct Chunk {
+  const T* in;  // of the chunk's first element, which may not be the tensor's
+  int64_t offset;
+  int begin, end;
+};
+
+template <typename T, int N>
+__device__ __forceinline__ Chunk<T> chunk_at(const Tensors<N>& list, const Place& at) {
+  constexpr int kElements = kChunkBytes / sizeof(T);
+  const T* base = static_cast<const T*>(list.in[at.tensor]);
+  const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(base) % 16 / sizeof(T));
+  Chunk<T> c;
+  c.offset = at.chunk * kElements - shift;
+  c.in = base + c.offset;
+  c.begin = at.chunk == 0 ? shift : 0;
+  const int64_t left = list.count[at.tensor] - c.offset;
+  c.end = left < kElements ? static_cast<int>(left) : kElements;
+  return c;
+}
+
+// The values of unit `u`, zeros outside the tensor.
+template <typename T>
+__device__ __forceinline__ Pack<T, 16 / sizeof(T)> load_unit(const Chunk<T>& c, int u) {
+  constexpr int V = 16 / sizeof(T);
+  const int at = u * V;
+  Pack<T, V> v{};
+  if (at >= c.begin && at + V <= c.end) {
+    v = *reinterpret_cast<const Pack<T, V>*>(c.in + at);
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (at + j >= c.begin && at + j < c.end) v.v[j] = c.in[at + j];
+  }
+  return v;
+}
+
+// A thread's running value: a sum of squares, or the largest |g| as the bits of a
+// non-negative float32 (whose order is that of integers, with NaN above infinity).
+template <int KIND>
+struct Running;
+
+template <>
+struct Running<kTwoNorm> {
+  double value = 0.0;
+  template <typename T, int V>
+  __device__ __forceinline__ void add(const Pack<T, V>& p) {
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float f = to_float(p.v[j]);
+      s = fmaf(f, f, s);
+    }
+    if constexpr (!std::is_same_v<T, __half>) {
+      if (!(s >= 1e-30f && s <= 1e38f)) {  // zeros, too small, too large, infinite or NaN
+        double d = 0.0;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const double f = to_float(p.v[j]);
+          d = fma(f, f, d);
+        }
+        value += d;
+        return;
+      }
+    }
+    value += s;
+  }
+  __device__ __forceinline__ void join(double other) { value += other; }
+  __device__ __forceinline__ double get() const { return value; }
+  __device__ __forceinline__ double norm() const { return sqrt(value); }
+};
+
+template <>
+struct Running<kMaxNorm> {
+  uint32_t bits = 0;
+  template <typename T, int V>
+  __device__ __forceinline__ void add(const Pack<T, V>& p) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const uint32_t b = __float_as_uint(to_float(p.v[j])) & 0x7fffffffu;
+      bits = b > bits ? b : bits;
+    }
+  }
+  __device__ __forceinline__ void join(double other) {
+    const uint32_t b = __float_as_uint(static_cast<float>(other)) & 0x7fffffffu;
+    bits = b > bits ? b : bits;
+  }
+  __device__ __forceinline__ double get() const { return __uint_as_float(bits); }
+  __device__ __forceinline__ double norm() const { return __uint_as_float(bits); }
+};
+
+// The running value over all threads of the CTA, in a fixed order; every thread gets it.
+template <int KIND>
+__device__ __forceinline__ Running<KIND> over_block(Running<KIND> r) {
+  __shared__ double parts[kThreads / 32];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) r.join(__shfl_xor_sync(0xffffffffu, r.get(), o));
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) parts[threadIdx.x >> 5] = r.get();
+  __syncthreads();
+  Running<KIND> all;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) all.join(parts[w]);
+  return all;
+}
+
+template <int KIND, typename T, int N>
+__device__ __forceinline__ void add_chunk(const Tensors<N>& list, const Place& at,
+                                          Running<KIND>& r) {
+  const Chunk<T> c = chunk_at<T>(list, at);
+  Pack<T, 16 / sizeof(T)> v[kUnits];
+#pragma unroll
+  for (int i = 0; i < kUnits; ++i) v[i] = load_unit(c, i * kThreads + threadIdx.x);
+#pragma unroll
+  for (int i = 0; i < kUnits; ++i) r.add(v[i]);
+}
+
+template <int KIND, int N>
+__device__ __forceinline__ Running<KIND> block_value(const Tensors<N>& list) {
+  Running<KIND> r;
+  const int chunks = list.first[list.tensors];
+  for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
+    const Place at = place_of(list, c);
+    switch (list.dtype[at.tensor]) {
+      case ICTC_DTYPE_F32: add_chunk<KIND, float>(list, at, r); break;
+      case ICTC_DTYPE_BF16: add_chunk<KIND, __nv_bfloat16>(list, at, r); break;
+      default: add_chunk<KIND, __half>(list, at, r);
+    }
+  }
+  return over_block(r);
+}
+
+template <int KIND, int N>
+__global__ void __launch_bounds__(kThreads)
+    partial_kernel(const __grid_constant__ Tensors<N> list, double* __restrict__ partial) {
+  const Running<KIND> r = block_value<KIND>(list);
+  if (threadIdx.x == 0) partial[blockIdx.x] = r.get();
+}
+
+template <int KIND>
+__device__ __forceinline__ double norm_of(const double* __restrict__ partial, int parts) {
+  Running<KIND> r;
+  for (int i = threadIdx.x; i < parts; i += kThreads) r.join(partial[i]);
+  return over_block(r).norm();
+}
+
+template <int KIND>
+__global__ void __launch_bounds__(kThreads)
+    norm_kernel(const double* __restrict__ partial, int parts, float* __restrict__ norm) {
+  const double n = norm_of<KIND>(partial, parts);
+  if (threadIdx.x == 0) *norm = static_cast<float>(n);
+}
+
+// min(1, max_norm / (norm + 1e-6)), rounded once; NaN stays NaN.
+__device__ __forceinline__ float factor_of(double norm, double max_norm) {
+  const double q = max_norm / (norm + 1e-6);
+  return static_cast<float>(q > 1.0 ? 1.0 : q);
+}
+
+template <typename T, int N>
+__device__ __forceinline__ void scale_chunk(const Tensors<N>& list, const Place& at,
+                                            float factor) {
+  constexpr int V = 16 / sizeof(T), kElements = kChunkBytes / sizeof(T);
+  const Chunk<T> c = chunk_at<T>(list, at);
+  T* out = static_cast<T*>(list.out[at.tensor]) + c.offset;
+  if (reinterpret_cast<uintptr_t>(out) % 16 == 0) {
+    Pack<T, V> v[kUnits];
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) v[i] = load_unit(c, i * kThreads + threadIdx.x);
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) {
+      const int e = (i * kThreads + threadIdx.x) * V;
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[i].v[j] = from_float<T>(to_float(v[i].v[j]) * factor);
+      if (e >= c.begin && e + V <= c.end) {
+        *reinterpret_cast<Pack<T, V>*>(out + e) = v[i];
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (e + j >= c.begin && e + j < c.end) out[e + j] = v[i].v[j];
+      }
+    }
+  } else {  // boundaries apart: element by element
+    constexpr int kAhead = 8;
+    for (int e0 = threadIdx.x; e0 < kElements; e0 += kAhead * kThreads) {
+      T v[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int e = e0 + i * kThreads;
+        if (e >= c.begin && e < c.end) v[i] = c.in[e];
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int e = e0 + i * kThreads;
+        if (e >= c.begin && e < c.end) out[e] = from_float<T>(to_float(v[i]) * factor);
+      }
+    }
+  }
+}
+
+template <int N>
+__device__ __forceinline__ void scale_chunks(const Tensors<N>& list, float factor) {
+  const int chunks = list.first[list.tensors];
+  if (static_cast<int>(blockIdx.x) >= chunks) return;
+  const int step = static_cast<int>(gridDim.x);
+  for (int c = blockIdx.x + (chunks - 1 - blockIdx.x) / step * step; c >= 0; c -= step) {
+    const Place at = place_of(list, c);
+    if (factor == 1.f && list.in[at.tensor] == list.out[at.tensor]) continue;  // as they are
+    switch (list.dtype[at.tensor]) {
+      case ICTC_DTYPE_F32: scale_chunk<float>(list, at, factor); break;
+      case ICTC_DTYPE_BF16: scale_chunk<__nv_bfloat16>(list, at, factor); break;
+      default: scale_chunk<__half>(list, at, factor);
+    }
+  }
+}
+
+template <int KIND, int N>
+__global__ void __launch_bounds__(kThreads)
+    scale_kernel(const __grid_constant__ Tensors<N> list, const double* __restrict__ partial,
+                 int parts, double max_norm, float* __restrict__ norm) {
+  const double n = norm_of<KIND>(partial, parts);
+  if (norm != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *norm = static_cast<float>(n);
+  scale_chunks(list, factor_of(n, max_norm));
+}
+
+// ----------------------------------------------------------------------- host side
+
+struct Request {
+  const void* const* in;
+  void* const* out;  // null: the norm alone
+  const int64_t* counts;
+  const int32_t* dtypes;
+  int64_t tensors;
+  double max_norm;
+  float* norm;
+  double* partial;
+  cudaStream_t stream;
+};
+
+// The tensors from `at` on that one launch takes, without empty ones.
+template <int N>
+int64_t fill(const Request& q, int64_t at, Tensors<N>& list) {
+  list.tensors = 0;
+  list.first[0] = 0;
+  for (; at < q.tensors && list.tensors < N; ++at) {
+    if (q.counts[at] == 0) continue;
+    const int64_t size = static_cast<int64_t>(dtype_size(q.dtypes[at]));
+    const int64_t shift = static_cast<int64_t>(reinterpret_cast<uintptr_t>(q.in[at]) % 16);
+    const int64_t chunks = ceil_div(q.counts[at] * size + shift, kChunkBytes);
+    if (list.first[list.tensors] + chunks >= (1ll << 31)) break;
+    const int i = list.tensors++;
+    list.in[i] = q.in[at];
+    list.out[i] = q.out ? q.out[at] : nullptr;
+    list.count[i] = q.counts[at];
+    list.dtype[i] = static_cast<uint8_t>(q.dtypes[at]);
+    list.first[i + 1] = list.first[i] + static_cast<int>(chunks);
+  }
+  return at;
+}
+
+int device_sms() {
+  int device = 0;
+  return sm_count(cudaGetDevice(&device) == cudaSuccess ? device : 0);
+}
+
+template <int N>
+unsigned grid_of(const Tensors<N>& list) {
+  const int most = device_sms() * kBlocksPerSm, chunks = list.first[list.tensors];
+  return static_cast<unsigned>(chunks < 1 ? 1 : chunks < most ? chunks : most);
+}
+
+template <int KIND, int N>
+int run(const Request& q) {
+  static thread_local Tensors<N> list;
+  int parts = 0;
+  int64_t at = 0;
+  bool whole = false;  // one launch holds all tensors
+  do {
+    const int64_t next = fill(q, at, list);
+    whole = at == 0 && next == q.tensors;
+    at = next;
+    const unsigned grid = grid_of(list);
+    partial_kernel<KIND, N><<<grid, kThreads, 0, q.stream>>>(list, q.partial + parts);
+    parts += static_cast<int>(grid);
+  } while (at < q.tensors);
+  if (!q.out) {
+    norm_kernel<KIND><<<1, kThreads, 0, q.stream>>>(q.partial, parts, q.norm);
+  } else {
+    at = 0;
+    do {
+      float* norm = at == 0 ? q.norm : nullptr;
+      at = whole ? q.tensors : fill(q, at, list);
+      scale_kernel<KIND, N><<<grid_of(list), kThreads, 0, q.stream>>>(list, q.partial, parts,
+                                                                     q.max_norm, norm);
+    } while (at < q.tensors);
+  }
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? ICTC_OK : cuda_fail(e, "gradient norm launch");
+}
+
+template <int KIND>
+int run_sized(const Request& q) {
+  return q.tensors <= 64 ? run<KIND, 64>(q) : run<KIND, kMostTensors>(q);
+}
+
+// A tensor has at most 2^36 elements, so that a launch takes at least 255 of them before its
+// count of chunks leaves its integers.
+constexpr int64_t kMostElements = 1ll << 36;
+
+int64_t most_launches(int64_t tensors) { return tensors / 255 + 1; }
+
+size_t workspace_bytes_of(int64_t tensors, int device) {
+  return static_cast<size_t>(most_launches(tensors)) * sm_count(device) * kBlocksPerSm *
+         sizeof(double);
+}
+
+int run_request(const Request& q, int32_t kind, const void* workspace, size_t bytes) {
+  if (q.tensors < 0) return fail(ICTC_ERR_INVALID, "negative number of tensors");
+  if (kind != kTwoNorm && kind != kMaxNorm) return fail(ICTC_ERR_INVALID, "unknown norm %d", kind);
+  if (!q.norm || (q.tensors > 0 && (!q.in || !q.counts || !q.dtypes)))
+    return fail(ICTC_ERR_INVALID, "null pointer");
+  for (int64_t i = 0; i < q.tensors; ++i) {
+    if (q.counts[i] < 0 || q.counts[i] > kMostElements)
+      return fail(ICTC_ERR_INVALID, "tensor %lld has %lld elements", static_cast<long long>(i),
+                  static_cast<long long>(q.counts[i]));
+    if (!known_dtype(q.dtypes[i]))
+      return fail(ICTC_ERR_INVALID, "unknown dtype code %d", q.dtypes[i]);
+    const uintptr_t size = dtype_size(q.dtypes[i]);
+    if (q.counts[i] > 0 &&
+        (!q.in[i] || !aligned(q.in[i], size) || (q.out && (!q.out[i] || !aligned(q.out[i], size)))))
+      return fail(ICTC_ERR_INVALID, "tensor %lld has a null or misaligned pointer",
+                  static_cast<long long>(i));
+  }
+  int device = 0;
+  const cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
+  const size_t needed = workspace_bytes_of(q.tensors, device);
+  if (!workspace || bytes < needed || !aligned(workspace, 16))
+    return fail(ICTC_ERR_WORKSPACE, "workspace has %zu bytes, needs %zu (16-byte aligned)",
+                workspace ? bytes : 0, needed);
+  return kind == kTwoNorm ? run_sized<kTwoNorm>(q) : run_sized<kMaxNorm>(q);
+}
+
+}  // namespace
+}  // namespace ictc
+
+using namespace ictc;
+
+extern "C" int32_t ictc_o2_grad_norm_workspace(int64_t tensors, int32_t device, size_t* bytes) {
+  if (tensors < 0) return fail(ICTC_ERR_INVALID, "negative number of tensors");
+  if (!bytes) return fail(ICTC_ERR_INVALID, "null output");
+  *bytes = workspace_bytes_of(tensors, device);
+  return ICTC_OK;
+}
+
+extern "C" int32_t ictc_o2_grad_norm(const void* const* grads, const int64_t* counts,
+                                     const int32_t* dtypes, int64_t tensors, int32_t kind,
+                                     float* norm, void* workspace, size_t workspace_bytes,
+                                     void* stream) {
+  const Request q{grads, nullptr, counts, dtypes, tensors, 0.0, norm,
+                  static_cast<double*>(workspace), static_cast<cudaStream_t>(stream)};
+  return run_request(q, kind, workspace, workspace_bytes);
+}
+
+extern "C" int32_t ictc_o2_clip_grads(const void* const* grads, void* const* out,
+                                      const int64_t* counts, const int32_t* dtypes,
+                                      int64_t tensors, int32_t kind, double max_norm, float* norm,
+                                      void* workspace, size_t workspace_bytes, void* stream) {
+  if (!(max_norm >= 0.0)) return fail(ICTC_ERR_INVALID, "max_norm must be >= 0");
+  if (tensors > 0 && !out) return fail(ICTC_ERR_INVALID, "null pointer");
+  static void* const kNone[1] = {nullptr};
+  const Request q{grads, out ? out : kNone, counts, dtypes, tensors, max_norm, norm,
+                  static_cast<double*>(workspace), static_cast<cudaStream_t>(stream)};
+  return run_request(q, kind, workspace, workspace_bytes);
+}

@@ -371,6 +371,58 @@ ICTC_API int32_t ictc_o2_linear_backward(
     void* grad_weight, void* grad_bias, void* workspace, size_t workspace_bytes, int64_t rows,
     int64_t in, int64_t out, int32_t dtype, int32_t activation, void* stream);
 
+/* The gated linear layer: (pg | pu) = x weight^T + bias, y = act(pg) pu with weight
+ * [2 hidden, in] and bias [2 hidden] or null (the gate's rows first), y [rows, hidden].
+ * preact [rows, 2 hidden] receives pg and pu in float32 for the backward, or is null.
+ * `keep` of the workspace query: whether the forward is given preact.  The layout flags
+ * are those of x and weight. */
+ICTC_API int32_t ictc_o2_gated_linear_workspace(int64_t rows, int64_t in, int64_t hidden,
+                                                int32_t dtype, int32_t activation,
+                                                int32_t layout, int32_t keep, int32_t device,
+                                                size_t* forward_bytes, size_t* backward_bytes);
+
+ICTC_API int32_t ictc_o2_gated_linear_forward(const void* x, int64_t x_stride,
+                                              const void* weight, int64_t weight_stride,
+                                              const void* bias, void* y, float* preact,
+                                              void* workspace, size_t workspace_bytes,
+                                              int64_t rows, int64_t in, int64_t hidden,
+                                              int32_t dtype, int32_t activation, void* stream);
+
+/* D = (grad_output pu act'(pg) | grad_output act(pg)), rounded to the operand type;
+ * grad_x = D weight, grad_weight = D^T x, grad_bias = sum of D's rows before rounding.
+ * Any output may be null.  rows = 0 clears grad_weight and grad_bias. */
+ICTC_API int32_t ictc_o2_gated_linear_backward(
+    const void* x, int64_t x_stride, const void* weight, int64_t weight_stride,
+    const float* preact, const void* grad_output, int64_t grad_stride, void* grad_x,
+    void* grad_weight, void* grad_bias, void* workspace, size_t workspace_bytes, int64_t rows,
+    int64_t in, int64_t hidden, int32_t dtype, int32_t activation, void* stream);
+
+/* ------------------------------------------------------------------------------
+ * The global norm of many tensors (a training step's gradients) and clipping by it.
+ * Host arrays of `tensors` entries: device addresses (aligned to their type), element
+ * counts (at most 2^36; 0 is skipped) and type codes, which may differ.  `kind`: the
+ * 2-norm (squares added in float32 over 16 bytes, in float64 beyond) or the largest
+ * magnitude; NaN counts as the largest.  Results do not depend on scheduling.
+ * ------------------------------------------------------------------------------ */
+
+enum { ICTC_GRAD_NORM_2 = 0, ICTC_GRAD_NORM_MAX = 1 };
+
+/* Bytes of workspace (16-byte aligned) that a call on so many tensors needs. */
+ICTC_API int32_t ictc_o2_grad_norm_workspace(int64_t tensors, int32_t device, size_t* bytes);
+
+/* *norm (device) = the norm of all tensors together. */
+ICTC_API int32_t ictc_o2_grad_norm(const void* const* grads, const int64_t* counts,
+                                   const int32_t* dtypes, int64_t tensors, int32_t kind,
+                                   float* norm, void* workspace, size_t workspace_bytes,
+                                   void* stream);
+
+/* The same, and out = grads min(1, max_norm / (norm + 1e-6)).  out[i] is grads[i] (scaled in
+ * place; left untouched where the factor is 1) or overlaps none of the tensors. */
+ICTC_API int32_t ictc_o2_clip_grads(const void* const* grads, void* const* out,
+                                    const int64_t* counts, const int32_t* dtypes,
+                                    int64_t tensors, int32_t kind, double max_norm, float* norm,
+                                    void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,460 @@
+"""The gated linear layer on the GPU against plain float64 formulas.
+
+Tolerances are error bounds of the arithmetic, element by element, with U the unit roundoff
+of float32 and u that of the operand type (test_dense_gpu.py has those of sums and
+activations).  With e(t) the error of t, a = act(pg), s = act'(pg), pg and pu sums over k:
+- e(a) <= 1.2 e(pg) + 16 U (|pg| + 1) and e(s) <= 1.1 e(pg) + 16 U (for relu: |s| <= 1 where pg
+  is within its error of 0);
+- y = a pu: e(a) (|pu| + e(pu)) + |a| e(pu), its rounding u |y|, one product in float32;
+- dg = g pu s and du = g a: |g| times the same, a 16-bit backward rounds them (u |d|);
+- dx, dW and db are sums over those.
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from test_dense_gpu import ACTS, DTYPES, TINY, U, UNIT, act64, rand, slope64, sum_error, within
+
+pytestmark = pytest.mark.gpu
+
+
+def gated64(x, w, b, act, g):
+    x, w, g = x.double(), w.double(), g.double()
+    pg, pu = (x @ w.t() + (0 if b is None else b.double())).chunk(2, -1)
+    a, s = act64(pg, act), slope64(pg, act)
+    d = torch.cat([g * pu * s, g * a], -1)
+    return pg, pu, a, s, a * pu, d, d @ w, d.t() @ x, d.sum(0)
+
+
+def check_gated(x, w, b, act, g, y, grads, dtype):
+    u, (m, k), n2 = UNIT[dtype], x.shape, w.shape[0]
+    pg, pu, a, s, y64, d, dx, dw, db = gated64(x, w, b, act, g)
+    ax, aw, ag = x.double().abs(), w.double().abs(), g.double().abs()
+    ep = sum_error(k) * (ax @ aw.t() + (0 if b is None else b.double().abs()))
+    epg, epu = ep.chunk(2, -1)
+    own = 16 * U * (pg.abs() + 1) * (act != "none")
+    ea = 1.2 * epg + own
+    es = (1.1 * epg + 16 * U) * (act != "none")
+    if act == "relu":
+        es = (pg.abs() <= epg).double()
+    tiny = TINY[dtype]
+    ey = ea * (pu.abs() + epu) + a.abs() * epu
+    within("y", y, y64, ey + (u + 2 * U) * (y64.abs() + ey) + tiny)
+    if grads is None:
+        return
+    ed = torch.cat([ag * (es * (pu.abs() + epu) + s.abs() * epu), ag * ea], -1) + 4 * U * d.abs()
+    eds = ed
+    if dtype != torch.float32:
+        ed = ed + u * (d.abs() + ed) + tiny
+    ad = d.abs() + ed
+    if grads[0] is not None:
+        within("dx", grads[0], dx, ed @ aw + sum_error(n2) * (ad @ aw) + (u + 2 * U) * (
+            dx.abs() + ed @ aw) + tiny)
+    if grads[1] is not None:
+        within("dweight", grads[1], dw, ed.t() @ ax + sum_error(m) * (ad.t() @ ax) +
+               (u + 2 * U) * (dw.abs() + ed.t() @ ax) + tiny)
+    if b is not None and grads[2] is not None:
+        within("dbias", grads[2], db, eds.sum(0) + (m + 64) * U * ad.sum(0) + (u + 2 * U) * (
+            db.abs() + eds.sum(0)) + tiny)
+
+
+def operands(m, k, n, dtype, device, seed=0, bias=True):
+    x = rand((m, k), dtype, device, seed + 1)
+    w = rand((2 * n, k), dtype, device, seed + 2, 1.5 / math.sqrt(k))
+    b = rand((2 * n,), dtype, device, seed + 3) if bias else None
+    return x, w, b, rand((m, n), dtype, device, seed + 5)
+
+
+def step(x, w, b, act, g):
+    """Output and gradients, b's left out with b."""
+    from ictc_o2_hp_b200 import dense
+    leaves = [t.detach().requires_grad_(True) for t in (x, w, b) if t is not None]
+    y = dense.gated_linear(*leaves, activation=act)
+    return y.detach(), torch.autograd.grad(y, leaves, g)
+
+
+SHAPES = [
+    (1, 1, 1), (1, 64, 64), (3, 7, 5), (4, 129, 1), (5, 8, 64), (37, 8, 64), (37, 64, 64),
+    (127, 63, 65), (128, 64, 128), (129, 65, 127), (200, 257, 3), (255, 16, 130), (300, 1000, 72),
+    (64, 2049, 33), (1000, 33, 200), (2500, 64, 64), (2500, 64, 32), (5000, 7, 3), (3000, 64, 1),
+    (129, 1, 64), (513, 61, 59), (6, 16, 16), (16, 512, 96), (31, 520, 264), (700, 1025, 769),
+    (2053, 211, 333), (4097, 702, 6), (5000, 1536, 8), (4500, 3, 130), (4099, 8, 520), (2, 4096, 40),
+    (4, 8192, 513), (1, 1000, 2048), (700, 1024, 768), (4096, 256, 256), (16, 4096, 520),
+    (20000, 64, 64), (33, 8200, 24), (40000, 24, 8), (260, 96, 4100), (9001, 64, 48), (64, 24, 3000),
+]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+def test_against_float64(shape, dtype, cuda_device):
+    from ictc_o2_hp_b200 import _lib, dense
+    m, k, n = shape
+    act = ACTS[(m + k + n) % len(ACTS)]
+    x, w, b, g = operands(m, k, n, dtype, cuda_device, bias=(m + n) % 3 > 0)
+    y, grads = step(x, w, b, act, g)
+    check_gated(x, w, b, act, g, y, (*grads, None), dtype)
+    plain = dense.gated_linear(x, w, b, act)
+    check_gated(x, w, b, act, g, plain, None, dtype)
+    y2, again = step(x, w, b, act, g)
+    assert torch.equal(y, y2) and all(torch.equal(p, q) for p, q in zip(grads, again)), \
+        "not the same bits twice"
+    assert torch.equal(dense.gated_linear(x, w, b, act), plain)
+    assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("shape", [(150, 40, 72), (3, 40, 72), (1300, 48, 24), (20, 512, 200)])
+def test_activations(shape, act, dtype, cuda_device):
+    """Every activation on p over a wide range."""
+    x, w, b, g = operands(*shape, dtype, cuda_device, 10)
+    w = w * 2.0
+    y, grads = step(x, w, b, act, g)
+    check_gated(x, w, b, act, g, y, grads, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("k,n", [(40, 24), (64, 64), (264, 40)])
+def test_strides_and_batches(k, n, dtype, cuda_device):
+    """Column slices (rows off every vector boundary), repeated rows, transposed weights,
+    expanded gradients and leading batch dimensions."""
+    from ictc_o2_hp_b200 import dense
+    big = rand((70, 3, 2 * k + 9), dtype, cuda_device, 31)
+    wide = rand((2 * n + 9, 2 * k + 9), dtype, cuda_device, 32, 0.2)
+    gw = rand((70, 3, n + 9), dtype, cuda_device, 33)
+    b = rand((2 * n,), dtype, cuda_device, 35)
+    for x in (big[..., 1:k + 1], big[:, :, :k], big[:, 1, 3:k + 3], big[..., ::2][..., :k],
+              big[:1, :1, 8:k + 8].expand(70, 3, k), big[0, 0, :k]):
+        for w in (wide[:2 * n, 8:k + 8], wide[3:2 * n + 3, 5:k + 5],
+                  wide[:2 * n, :k].t().contiguous().t()):
+            lead = x.shape[:-1]
+            full = gw[..., :n] if x.dim() == 3 else gw[:, 1, 5:n + 5] if x.dim() == 2 else gw[0, 0, 1:n + 1]
+            for g in (full, rand((1,), dtype, cuda_device, 34).expand(*lead, n)):
+                xx, ww = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+                y = dense.gated_linear(xx, ww, b, "gelu")
+                assert y.shape == (*lead, n) and y.is_contiguous()
+                grads = torch.autograd.grad(y, (xx, ww), g)
+                check_gated(x.reshape(-1, k), w, b, "gelu", g.reshape(-1, n),
+                            y.detach().reshape(-1, n),
+                            (grads[0].reshape(-1, k), grads[1], None), dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(700001, 64, 64), (300007, 61, 59), (400003, 24, 40)])
+def test_many_tiles(shape, dtype, cuda_device):
+    """Many tiles per CTA, run after run: a buffer that is written again while it is still
+    read shows as another tile's rows, in a few rows of a million."""
+    from ictc_o2_hp_b200 import dense
+    x, w, b, g = operands(*shape, dtype, cuda_device, 70)
+    first = None
+    for _ in range(6):
+        y, grads = step(x, w, b, "silu", g)
+        out = (y, *grads, dense.gated_linear(x, w, b, "silu"))
+        if first is None:
+            first = out
+            check_gated(x, w, b, "silu", g, y, grads, dtype)
+            check_gated(x, w, b, "silu", g, out[-1], None, dtype)
+        assert all(torch.equal(p, q) for p, q in zip(out, first))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(5, 9), (30, 64), (30, 5), (300, 70), (2000, 48)])
+def test_partial_gradients(shape, dtype, cuda_device):
+    """Each gradient alone is the one of all together."""
+    from ictc_o2_hp_b200 import dense
+    m, k = shape
+    x, w, b, g = operands(m, k, 24, dtype, cuda_device, 60)
+    full = step(x, w, b, "gelu", g)[1]
+    for i in range(3):
+        leaves = [t.detach().requires_grad_(i == j) for j, t in enumerate((x, w, b))]
+        y = dense.gated_linear(*leaves, "gelu")
+        assert torch.equal(torch.autograd.grad(y, leaves[i], g)[0], full[i])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_empty(dtype, cuda_device):
+    from ictc_o2_hp_b200 import dense
+    w = rand((12, 5), dtype, cuda_device, 61).requires_grad_(True)
+    b = rand((12,), dtype, cuda_device, 62).requires_grad_(True)
+    x = torch.empty(0, 3, 5, dtype=dtype, device=cuda_device, requires_grad=True)
+    y = dense.gated_linear(x, w, b)
+    assert y.shape == (0, 3, 6)
+    for graph in (False, True):
+        gx, gw, gb = torch.autograd.grad(y, (x, w, b), torch.empty_like(y), retain_graph=True,
+                                         create_graph=graph)
+        assert gx.shape == x.shape and gw.shape == w.shape and gb.shape == b.shape
+        assert not gw.any() and not gb.any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(3, 72, 140), (150, 72, 140), (12, 520, 64), (200, 48, 40)])
+def test_nonfinite(shape, dtype, cuda_device):
+    """An infinity or NaN reaches exactly the outputs that the formula gives it, with its
+    sign (act none: products of infinities alone); the others keep their values."""
+    from ictc_o2_hp_b200 import dense
+    m, k, n = shape
+    x, w, _, _ = operands(m, k, n, dtype, cuda_device, 50, bias=False)
+    w[:, 7] = 1.0
+    w[5, 7] = -2.0
+    w[n + 9, 7] = -1.0
+    base = dense.gated_linear(x, w, None, "none")
+    x[1, 7] = math.inf
+    x[2, 3] = math.nan
+    w[20, 30] = -math.inf
+    y = dense.gated_linear(x, w, None, "none")
+    pg, pu = (x.double() @ w.double().t()).chunk(2, -1)
+    want = pg * pu
+    assert torch.equal(y.isnan(), want.isnan()) and torch.equal(y.isinf(), want.isinf())
+    assert torch.equal(y[y.isinf()].double(), want[want.isinf()])
+    keep = want.isfinite()
+    assert keep.any() and torch.equal(y[keep], base[keep])
+
+
+@pytest.mark.parametrize("shape", [(3, 40, 48), (700, 48, 40), (700, 48, 140)])
+def test_nonfinite_gradients(shape, cuda_device):
+    """Infinities and NaN in the gradient and in x reach the sums they belong to, and no
+    others."""
+    m, k, n = shape
+    x, w, _, g = operands(m, k, n, torch.float32, cuda_device, 55, bias=False)
+    base = step(x, w, None, "none", g)[1]
+    g = g.clone()
+    g[m - 1, 7] = math.nan
+    dx, dw = step(x, w, None, "none", g)[1]
+    rows = torch.arange(m, device=cuda_device) != m - 1
+    cols = torch.arange(2 * n, device=cuda_device) % n != 7
+    assert dx[m - 1].isnan().all() and torch.equal(dx[rows], base[0][rows])
+    assert dw[~cols].isnan().all() and torch.equal(dw[cols], base[1][cols])
+
+
+def test_gradients_against_differences(cuda_device):
+    """Directional derivatives against central differences of the float64 formula."""
+    m, k, n, h = 40, 24, 32, 1e-5
+    x, w, b, g = operands(m, k, n, torch.float32, cuda_device, 80)
+
+    def total(x, w, b, act):
+        pg, pu = (x @ w.t() + b).chunk(2, -1)
+        return (act64(pg, act) * pu * g.double()).sum()
+
+    for act in ("none", "silu", "gelu", "gelu_tanh"):
+        grads = step(x, w, b, act, g)[1]
+        point = [t.double() for t in (x, w, b)]
+        for i, grad in enumerate(grads):
+            v = rand(grad.shape, torch.float32, cuda_device, 20 + i).double()
+            ends = [total(*(t + sign * h * v if j == i else t for j, t in enumerate(point)), act)
+                    for sign in (1, -1)]
+            slope = (ends[0] - ends[1]).item() / (2 * h)
+            size = (grad.double().abs() * v.abs()).sum().item()
+            assert abs((grad.double() * v).sum().item() - slope) <= 1e-5 * size
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_second_derivatives(act, dtype, cuda_device):
+    """A force-like loss: squared input gradients, differentiated by every operand.  In
+    16-bit types some eight tensors between the operands and a second derivative are rounded,
+    and the squares double what is off: 24 u in the 2-norm."""
+    from ictc_o2_hp_b200 import dense
+    x, w, b, g = operands(50, 24, 40, dtype, cuda_device, 90)
+
+    def loss(x, w, b, g, layer):
+        f = torch.autograd.grad((layer(x, w, b) * g).sum(), x, create_graph=True)[0]
+        return (f.double() ** 2).sum() if f.dtype == torch.float64 else (f.float() ** 2).sum()
+
+    def plain(x, w, b):
+        pg, pu = (x @ w.t() + b).chunk(2, -1)
+        return act64(pg, act) * pu
+
+    ours = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    got = torch.autograd.grad(loss(*ours, g, lambda *t: dense.gated_linear(*t, act)), ours)
+    wide = [t.double().requires_grad_(True) for t in (x, w, b)]
+    want = torch.autograd.grad(loss(*wide, g.double(), plain), wide)
+    limit = 1e-5 if dtype == torch.float32 else 24 * UNIT[dtype]
+    for p, q in zip(got, want):
+        assert (p.double() - q).norm() <= limit * q.norm()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", ACTS)
+def test_create_graph_keeps_first_gradients(act, dtype, cuda_device):
+    """The gradients that are differentiated again keep the error bounds of those that are
+    not."""
+    from ictc_o2_hp_b200 import dense
+    x, w, b, g = operands(150, 40, 72, dtype, cuda_device, 16)
+    x = x * 2.0
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    y = dense.gated_linear(*leaves, act)
+    grads = torch.autograd.grad(y, leaves, g, create_graph=True)
+    assert all(t.requires_grad for t in grads)
+    check_gated(x, w, b, act, g, y.detach(), [t.detach() for t in grads], dtype)
+
+
+# ----------------------------------------------------------- modules, streams, compile
+
+
+def test_modules(cuda_device):
+    from ictc_o2_hp_b200 import GatedBlock, GatedLinear, RadialTrunk
+    torch.manual_seed(3)
+    ours = GatedLinear(20, 30).to(cuda_device)
+    torch.manual_seed(3)
+    theirs = torch.nn.Linear(20, 60).to(cuda_device)
+    theirs.load_state_dict(ours.state_dict())
+    assert torch.equal(ours.weight, theirs.weight)
+    x = rand((9, 20), torch.float32, cuda_device, 1)
+    f = torch.nn.functional
+
+    def gated(layer, x):
+        pg, pu = f.linear(x, layer.weight.double(), layer.bias.double()).chunk(2, -1)
+        return f.silu(pg) * pu
+
+    want = gated(ours, x.double())
+    assert (ours(x).double() - want).norm() <= 1e-6 * want.norm()
+    block = GatedBlock(20, 48).to(cuda_device)
+    h = gated(block.gated, f.layer_norm(x.double(), (20,)))
+    want = x.double() + f.linear(h, block.down.weight.double(), block.down.bias.double())
+    assert (block(x).double() - want).norm() <= 1e-6 * want.norm()
+    trunk = RadialTrunk(8, 64, blocks=2, gated=True).to(cuda_device)
+    assert all(isinstance(b, GatedBlock) for b in trunk.blocks)
+    out = trunk(rand((5, 11, 8), torch.float32, cuda_device, 2))
+    assert out.shape == (5, 11, 64) and out.mean(-1).abs().max() <= 1e-5
+
+
+def test_gated_trunk_feeds_the_radial_product(cuda_device):
+    """Gated trunk, final affine layer and per-edge product together, against the same
+    network of torch modules in front of the product."""
+    from ictc_o2_hp_b200 import Linear, RadialTrunk, RadialUvuTensorProduct, UvuTensorProduct
+    torch.manual_seed(0)
+    tp = UvuTensorProduct(16, 1, 2, parity="full", parity_in2="canonical", shared_weights=False)
+    product = RadialUvuTensorProduct(tp, Linear(32, tp.weight_numel)).to(cuda_device)
+    trunk = RadialTrunk(8, 32, gated=True).to(cuda_device)
+    basis = rand((300, 8), torch.float32, cuda_device, 1)
+    x = rand((300, tp.input1_dimension), torch.float32, cuda_device, 2)
+    y = rand((300, tp.input2_dimension), torch.float32, cuda_device, 3)
+    out = product(x, y, trunk(basis))
+    f = torch.nn.functional
+
+    def torch_trunk(b):
+        h = f.silu(f.linear(b, trunk.embed.weight, trunk.embed.bias))
+        for q in trunk.blocks:
+            z = f.layer_norm(h, (32,), q.norm.weight, q.norm.bias)
+            pg, pu = f.linear(z, q.gated.weight, q.gated.bias).chunk(2, -1)
+            h = h + f.linear(f.silu(pg) * pu, q.down.weight, q.down.bias)
+        return f.layer_norm(h, (32,), trunk.norm.weight, trunk.norm.bias)
+
+    want = product(x, y, torch_trunk(basis))
+    assert (out - want).norm() <= 1e-5 * want.norm()
+    params = list(trunk.parameters())
+    g = rand(out.shape, torch.float32, cuda_device, 4)
+    for p, q in zip(torch.autograd.grad(out, params, g), torch.autograd.grad(want, params, g)):
+        assert (p - q).norm() <= 1e-4 * q.norm()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(3, 96, 64), (20, 512, 64), (200, 96, 64), (2000, 64, 64)])
+def test_other_stream_and_graph_capture(shape, dtype, cuda_device):
+    """Work goes to the caller's stream; a captured step replays on new inputs, two captured
+    steps do not touch each other's buffers."""
+    from ictc_o2_hp_b200 import dense
+    x, w, b, g = operands(*shape, dtype, cuda_device, 120)
+    want = step(x, w, b, "gelu", g)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step(x, w, b, "gelu", g)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got[0], want[0]) and all(map(torch.equal, got[1], want[1]))
+    leaves = [torch.zeros_like(t).requires_grad_(True) for t in (x, w, b)]
+    held = torch.zeros_like(g)
+    graphs, outs = [], []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = dense.gated_linear(*leaves, "gelu")
+            outs.append((y, *torch.autograd.grad(y, leaves, held)))
+        graphs.append(graph)
+    with torch.no_grad():
+        for t, source in zip((*leaves, held), (x, w, b, g)):
+            t.copy_(source)
+    graphs[0].replay()
+    graphs[1].replay()
+    for out in outs:
+        assert torch.equal(out[0], want[0]) and all(map(torch.equal, out[1:], want[1]))
+
+
+def test_compile_and_traces(cuda_device):
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    from ictc_o2_hp_b200 import GatedBlock
+    torch.manual_seed(1)
+    block = GatedBlock(32).to(cuda_device)
+    x, other = (rand((64, 32), torch.float32, cuda_device, s).requires_grad_(True) for s in (1, 3))
+    g = rand((64, 32), torch.float32, cuda_device, 2)
+    params = list(block.parameters())
+    want = torch.autograd.grad(block(x), (x, *params), g)
+    run = torch.compile(block, fullgraph=True, backend="aot_eager")
+    assert all(map(torch.equal, torch.autograd.grad(run(x), (x, *params), g), want))
+
+    def whole(x):
+        y = block(x)
+        return y, torch.autograd.grad(y, x, g)[0]
+
+    recorded = make_fx(whole)(other.detach().clone().requires_grad_(True))
+    got = recorded(x.detach().clone().requires_grad_(True))
+    assert torch.equal(got[0], block(x)) and torch.equal(got[1], want[0])
+
+
+def test_autocast(cuda_device):
+    from ictc_o2_hp_b200 import GatedLinear, dense
+    layer = GatedLinear(24, 40).to(cuda_device)
+    x = rand((30, 24), torch.float16, cuda_device, 1).requires_grad_(True)
+    g = rand((30, 40), torch.bfloat16, cuda_device, 3)
+    with pytest.raises(ValueError):
+        layer(x)
+    args = [t.detach().bfloat16().requires_grad_(True) for t in (x, layer.weight, layer.bias)]
+    want = dense.gated_linear(*args)
+    grads = torch.autograd.grad(want, args, g)
+    for run in (layer, torch.compile(layer, fullgraph=True, backend="aot_eager")):
+        with torch.autocast("cuda", torch.bfloat16):
+            y = run(x)
+        got = torch.autograd.grad(y, (x, layer.weight, layer.bias), g)
+        assert torch.equal(y, want)
+        assert all(torch.equal(p, q.to(p.dtype)) for p, q in zip(got, grads))
+
+
+def test_views_with_a_negative_bit(cuda_device):
+    from ictc_o2_hp_b200 import dense
+    z = torch.complex(*(rand((40, 1), torch.float32, cuda_device, s) for s in (36, 37)))
+    x = z.conj().imag
+    assert x.is_neg()
+    w = rand((6, 1), torch.float32, cuda_device, 38)
+    assert torch.equal(dense.gated_linear(x, w), dense.gated_linear(x.resolve_neg(), w))
+
+
+def test_refusals(cuda_device):
+    from torch.autograd import forward_ad
+
+    from ictc_o2_hp_b200 import dense
+    x = torch.randn(4, 6, device=cuda_device)
+    w = torch.randn(10, 6, device=cuda_device)
+    with pytest.raises(TypeError):
+        dense.gated_linear(x.double(), w.double())
+    for call in (
+        lambda: dense.gated_linear(x, w.half()),
+        lambda: dense.gated_linear(x, w[:, :5]),
+        lambda: dense.gated_linear(x, w[:9]),
+        lambda: dense.gated_linear(x, w[:0]),
+        lambda: dense.gated_linear(x, w[0]),
+        lambda: dense.gated_linear(x, w, w[:5, 0]),
+        lambda: dense.gated_linear(x, w, w[:, 0].cpu()),
+        lambda: dense.gated_linear(x, w, activation="swish"),
+        lambda: dense.gated_linear(x[:, :0], w[:, :0]),
+    ):
+        with pytest.raises(ValueError):
+            call()
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x.clone(), torch.ones_like(x))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            dense.gated_linear(dual, w)
