@@ -510,10 +510,31 @@ Tensor linear(const Tensor& x, const Tensor& weight, const std::optional<Tensor>
 
 // ---------------------------------------------------------------------- gated linear
 
+// rows_of, whose rows do not overlap (a repeated row is copied out).
+Tensor apart(const Tensor& t) {
+  const Tensor rows = rows_of(t);
+  return rows.size(0) > 1 && rows.stride(0) < rows.size(1) ? rows.contiguous() : rows;
+}
+
+// The distance of rows; that of a single row says nothing.
+int64_t row_stride(const Tensor& rows) {
+  return rows.size(0) > 1 ? rows.stride(0) : rows.size(1);
+}
+
+int32_t gated_layout(const Tensor& x, const Tensor& w) {
+  const int64_t block = 16 / x.element_size();
+  const auto start = [](const Tensor& t) {
+    return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  };
+  const bool rows = start(x) && start(w) && row_stride(x) % block == 0 && row_stride(w) % block == 0;
+  return (rows ? ICTC_LINEAR_ALIGNED : 0) |
+         (start(x) && row_stride(x) == x.size(1) ? ICTC_LINEAR_PACKED : 0);
+}
+
 std::tuple<Tensor, Tensor> gated_forward(const Tensor& x, const Tensor& weight,
                                          const Tensor& bias_in, int64_t code, bool save) {
   const c10::cuda::CUDAGuard guard(x.device());
-  const Tensor rows = rows_of(x), w = rows_of(weight), bias = packed(bias_in);
+  const Tensor rows = apart(x), w = apart(weight), bias = packed(bias_in);
   const int64_t m = rows.size(0), k = rows.size(1), n = w.size(0) / 2;
   c10::SmallVector<int64_t, 6> shape(x.sizes().begin(), x.sizes().end());
   shape.back() = n;
@@ -522,11 +543,11 @@ std::tuple<Tensor, Tensor> gated_forward(const Tensor& x, const Tensor& weight,
   if (save) preact = at::empty({m, 2 * n}, x.options().dtype(at::kFloat));
   const int32_t dtype = code_of(x.scalar_type()), act = static_cast<int32_t>(code);
   size_t bytes = 0, other = 0;
-  check(api.gated_workspace(m, k, n, dtype, act, layout_of(rows, w, nullptr), save,
+  check(api.gated_workspace(m, k, n, dtype, act, gated_layout(rows, w), save,
                             x.device().index(), &bytes, &other),
         "gated_linear_workspace");
   const Tensor space = scratch(bytes, x);
-  check(api.gated_forward(rows.data_ptr(), rows.stride(0), w.data_ptr(), w.stride(0), data(bias),
+  check(api.gated_forward(rows.data_ptr(), row_stride(rows), w.data_ptr(), row_stride(w), data(bias),
                           y.data_ptr(), floats(preact), data(space), bytes, m, k, n, dtype, act,
                           stream_of(x)),
         "gated_linear_forward");
@@ -538,7 +559,7 @@ std::tuple<Tensor, Tensor, Tensor> gated_backward(const Tensor& x, const Tensor&
                                                   int64_t code, bool need_x, bool need_w,
                                                   bool need_b) {
   const c10::cuda::CUDAGuard guard(x.device());
-  const Tensor rows = rows_of(x), w = rows_of(weight), g = rows_of(grad);
+  const Tensor rows = apart(x), w = apart(weight), g = rows_of(grad);
   const int64_t m = rows.size(0), k = rows.size(1), n = w.size(0) / 2;
   Tensor dx, dw, db;
   if (need_x) dx = at::empty(x.sizes(), x.options());
@@ -546,11 +567,11 @@ std::tuple<Tensor, Tensor, Tensor> gated_backward(const Tensor& x, const Tensor&
   if (need_b) db = at::empty({2 * n}, x.options());
   const int32_t dtype = code_of(x.scalar_type()), act = static_cast<int32_t>(code);
   size_t bytes = 0, other = 0;
-  check(api.gated_workspace(m, k, n, dtype, act, layout_of(rows, w, nullptr), true,
+  check(api.gated_workspace(m, k, n, dtype, act, gated_layout(rows, w), true,
                             x.device().index(), &other, &bytes),
         "gated_linear_workspace");
   const Tensor space = scratch(bytes, x);
-  check(api.gated_backward(rows.data_ptr(), rows.stride(0), w.data_ptr(), w.stride(0),
+  check(api.gated_backward(rows.data_ptr(), row_stride(rows), w.data_ptr(), row_stride(w),
                            floats(preact), g.data_ptr(), g.stride(0), data(dx), data(dw),
                            data(db), data(space), bytes, m, k, n, dtype, act, stream_of(x)),
         "gated_linear_backward");

@@ -106,13 +106,16 @@ __device__ __forceinline__ void load_raw(unsigned char* dst, const CUtensorMap* 
   else tma_load_2d(dst, map, k0, static_cast<int>(mn0), bar);
 }
 
-template <bool A_MN, bool B_MN, int BN, int ACT>
+// GATED: the forward of the gated layer (as in dense_pair.cuh; 64 columns of each half).
+template <bool A_MN, bool B_MN, int BN, int ACT, bool GATED = false>
 __global__ void __launch_bounds__(kCutThreads, 1)
     cut_product_kernel(const __grid_constant__ OperandMaps maps,
                        const __grid_constant__ ProductArgs p) {
   constexpr int R = kCutSlots<BN>;
   constexpr uint32_t kA = 3 * 128 * 128;  // bytes of A's parts
   constexpr uint32_t kSet = BN == 128 ? 256 : 192;
+  constexpr int kTile = GATED ? BN / 2 : BN;  // columns of the output
+  static_assert(!GATED || (BN == 128 && !B_MN));
   extern __shared__ unsigned char smem_raw[];
   unsigned char* tile = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t{1023});
@@ -160,7 +163,7 @@ __global__ void __launch_bounds__(kCutThreads, 1)
       bool ok = true;
       uint32_t n = 0;
       for (int64_t t = blockIdx.x; ok && t < total; t += gridDim.x) {
-        const TilePos pos = tile_at<128>(p, t, BN);
+        const TilePos pos = tile_at<128>(p, t, kTile);
         const int64_t h1 = halves_end(pos);
         for (int64_t h = 2ll * pos.c0; h < h1; ++h, ++n) {
           const int s = n % R;
@@ -171,6 +174,9 @@ __global__ void __launch_bounds__(kCutThreads, 1)
           load_raw<A_MN, 128>(slot, &maps.a, pos.m0, static_cast<int>(h * kCutK), &raw_full[s]);
           load_raw<B_MN, BN>(slot + 128 * kCutK * 4, &maps.b, pos.n0,
                              static_cast<int>(h * kCutK), &raw_full[s]);
+          if constexpr (GATED)  // a box has half of the rows
+            load_raw<B_MN, BN>(slot + (128 + BN / 2) * kCutK * 4, &maps.b, p.n + pos.n0,
+                               static_cast<int>(h * kCutK), &raw_full[s]);
         }
       }
       if (!ok) {  // copies in flight land before the CTA goes away
@@ -191,7 +197,7 @@ __global__ void __launch_bounds__(kCutThreads, 1)
       bool ok = true;
       uint32_t n = 0, set = 0;
       for (int64_t t = blockIdx.x; ok && t < total; t += gridDim.x) {
-        const TilePos pos = tile_at<128>(p, t, BN);
+        const TilePos pos = tile_at<128>(p, t, kTile);
         const int64_t h0 = 2ll * pos.c0, h1 = halves_end(pos);
         for (int64_t h = h0; h < h1; ++h, ++n) {
           const bool first = (h - h0) % kCutGroupHalves == 0;
@@ -237,7 +243,7 @@ __global__ void __launch_bounds__(kCutThreads, 1)
     bool ok = true;
     uint32_t n = 0;
     for (int64_t t = blockIdx.x; ok && t < total; t += gridDim.x) {
-      const TilePos pos = tile_at<128>(p, t, BN);
+      const TilePos pos = tile_at<128>(p, t, kTile);
       const int64_t h1 = halves_end(pos);
       for (int64_t h = 2ll * pos.c0; h < h1; ++h, ++n) {
         const int s = n % R, half = n & 1;
@@ -263,7 +269,7 @@ __global__ void __launch_bounds__(kCutThreads, 1)
     bool ok = true;
     uint32_t set = 0;
     for (int64_t t = blockIdx.x; ok && t < total; t += gridDim.x) {
-      const TilePos pos = tile_at<128>(p, t, BN);
+      const TilePos pos = tile_at<128>(p, t, kTile);
       const int64_t h0 = 2ll * pos.c0, h1 = halves_end(pos);
       const int groups = static_cast<int>((h1 - h0 + kCutGroupHalves - 1) / kCutGroupHalves);
       const int64_t row0 = pos.m0 + quad * 32;
@@ -274,10 +280,11 @@ __global__ void __launch_bounds__(kCutThreads, 1)
         ok = mbar_wait_warp(&done[set & 1], (set >> 1) & 1, kCodeEpilogue);
         if (!ok) break;
         tcgen05_fence_after();
-        const uint32_t at =
-            tmem + (set & 1) * kSet + (static_cast<uint32_t>(quad * 32) << 16) + half * kHalf;
+        const uint32_t first = tmem + (set & 1) * kSet + (static_cast<uint32_t>(quad * 32) << 16) +
+                               half * (GATED ? 32 : kHalf);
 #pragma unroll
         for (int j = 0; j < kHalf; j += 16) {
+          const uint32_t at = first + (GATED && j >= 32 ? BN / 2 - 32 : 0);
           float w[16], y[16];
           tmem_load16(at + BN + j, y);
           if constexpr (BN == 64) {
@@ -298,11 +305,16 @@ __global__ void __launch_bounds__(kCutThreads, 1)
         if (lane == 0) mbar_arrive(&room[set & 1]);
       }
       if (!ok) break;
+      if constexpr (GATED) {
+        write_gated_block<float, ACT>(p, pos.split, acc, acc + 32, mine, row0, pos.n0 + half * 32,
+                                      lane);
+      } else {
 #pragma unroll
-      for (int cb = 0; cb < kHalf / 32; ++cb) {
-        const int64_t col0 = pos.n0 + half * kHalf + cb * 32;
-        stage_block(acc + cb * 32, mine, lane);
-        write_staged<float, ACT, BN == 128>(p, pos.split, mine, row0, col0, lane, res);
+        for (int cb = 0; cb < kHalf / 32; ++cb) {
+          const int64_t col0 = pos.n0 + half * kHalf + cb * 32;
+          stage_block(acc + cb * 32, mine, lane);
+          write_staged<float, ACT, BN == 128>(p, pos.split, mine, row0, col0, lane, res);
+        }
       }
     }
   }
@@ -312,6 +324,19 @@ __global__ void __launch_bounds__(kCutThreads, 1)
     tcgen05_fence_after();
     tmem_free(tmem, 512);
   }
+}
+
+// Host: the warpgroups' shares are drawn from what the block is launched with: a build that
+// gives its threads fewer registers would wait for them for good.
+template <bool A_MN, bool B_MN, int BN, int ACT, bool GATED = false>
+bool cut_shares_fit() {
+  static const bool fit = [] {
+    cudaFuncAttributes a{};
+    return cudaFuncGetAttributes(&a, cut_product_kernel<A_MN, B_MN, BN, ACT, GATED>) ==
+               cudaSuccess &&
+           a.numRegs >= kCutLaunchRegisters;
+  }();
+  return fit;
 }
 
 }  // namespace ictc

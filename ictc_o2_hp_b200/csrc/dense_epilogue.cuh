@@ -229,4 +229,89 @@ __device__ __forceinline__ void write_block(const ProductArgs& p, int split, con
   write_staged<T, ACT>(p, split, mine, row0, col0, lane, res);
 }
 
+// The same for the gated layer, whose tile has 32 columns of the gate's sums and the 32 of the
+// other half beside them: y = act(pg) pu at columns col0 .. of `n`, p = (pg | pu) and partial
+// sums in rows of 2 n.  Both blocks pass through the warp's 4 KB one after the other.
+template <typename T, int ACT>
+__device__ __forceinline__ void write_gated_block(const ProductArgs& p, int split,
+                                                  const float* gate, const float* up,
+                                                  float4* mine, int64_t row0, int64_t col0,
+                                                  int lane) {
+  const Epilogue& e = p.e;
+  const int64_t col = col0 + (e.vec ? (lane & 7) * 4 : lane), wide = 2 * p.n;
+  const int rows = p.m - row0 < 32 ? static_cast<int>(p.m - row0) : 32;  // <= 0: none
+  float* sums = e.partial ? e.partial + (split * p.m + row0) * wide + col
+                          : e.preact ? e.preact + row0 * wide + col : nullptr;
+  T* out = static_cast<T*>(e.out) + row0 * p.n + col;
+  if (e.vec) {
+    const int r0 = lane >> 3;
+    float4 g[8];
+    stage_block(gate, mine, lane);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = r0 + 4 * i;
+      g[i] = mine[r * 8 + ((lane & 7) ^ (r & 7))];
+    }
+    __syncwarp();
+    stage_block(up, mine, lane);
+    if (col < p.n) {
+      float bg[4] = {0.f, 0.f, 0.f, 0.f}, bu[4] = {0.f, 0.f, 0.f, 0.f};
+      if (e.bias && !e.partial) {
+        const T* bias = static_cast<const T*>(e.bias) + col;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          bg[j] = to_float(bias[j]);
+          bu[j] = to_float(bias[p.n + j]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = r0 + 4 * i;
+        if (r >= rows) break;
+        const float4 u = mine[r * 8 + ((lane & 7) ^ (r & 7))];
+        const float pg[4] = {g[i].x + bg[0], g[i].y + bg[1], g[i].z + bg[2], g[i].w + bg[3]};
+        const float pu[4] = {u.x + bu[0], u.y + bu[1], u.z + bu[2], u.w + bu[3]};
+        if (sums) {
+          *reinterpret_cast<float4*>(sums + r * wide) = make_float4(pg[0], pg[1], pg[2], pg[3]);
+          *reinterpret_cast<float4*>(sums + r * wide + p.n) =
+              make_float4(pu[0], pu[1], pu[2], pu[3]);
+        }
+        if (e.partial) continue;
+        Pack<T, 4> o;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o.v[j] = from_float<T>(activate<ACT>(pg[j], e.activation) * pu[j]);
+        *reinterpret_cast<Pack<T, 4>*>(out + r * p.n) = o;
+      }
+    }
+  } else {
+    const float* flat = reinterpret_cast<const float*>(mine);
+    const auto at = [&](int r) { return r * 32 + (((lane >> 2) ^ (r & 7)) << 2) + (lane & 3); };
+    float g[32];
+    stage_block(gate, mine, lane);
+#pragma unroll
+    for (int r = 0; r < 32; ++r) g[r] = flat[at(r)];
+    __syncwarp();
+    stage_block(up, mine, lane);
+    if (col < p.n) {
+      float bg = 0.f, bu = 0.f;
+      if (e.bias && !e.partial) {
+        const T* bias = static_cast<const T*>(e.bias) + col;
+        bg = to_float(bias[0]);
+        bu = to_float(bias[p.n]);
+      }
+#pragma unroll
+      for (int r = 0; r < 32; ++r) {
+        if (r >= rows) break;
+        const float pg = g[r] + bg, pu = flat[at(r)] + bu;
+        if (sums) {
+          sums[r * wide] = pg;
+          sums[r * wide + p.n] = pu;
+        }
+        if (!e.partial) out[r * p.n] = from_float<T>(activate<ACT>(pg, e.activation) * pu);
+      }
+    }
+  }
+  __syncwarp();
+}
+
 }  // namespace ictc

@@ -6,55 +6,146 @@
 //   dx = D W,  dW = D^T x,  db = sum_rows D
 //
 // With both halves of W in one tensor the backward's products are those of a linear layer of
-// 2 H outputs without activation (dense_linear.cu), and so are the forward's sums here; the
-// activation and the product of the halves are a pass over p = (pg | pu) in float32.
+// 2 H outputs without activation (dense_linear.cu).
+//
+// Which kernel a forward takes:
+//   up to 4 rows, aligned or small   FMAs, W read once (few_kernel)
+//   16-bit, aligned rows             SM pairs fed by TMA (dense_pair.cuh, GATED)
+//   float32, aligned rows            cut on the way in (dense_cut.cuh, GATED)
+//   unaligned rows                   large products are copied to aligned rows first; for
+//                                    small ones the linear layer leaves p in memory, and
+//                                    gate_kernel makes y of it
+// A tile of these kernels has the sums of both halves for the same columns of y, so that the
+// epilogue needs nothing from another tile, and p is written only where a backward wants it.
 #include <cuda_runtime.h>
 
 #include <cstdint>
 #include <type_traits>
 
 #include "common.cuh"
+#include "dense_cut.cuh"
+#include "dense_epilogue.cuh"
+#include "dense_pair.cuh"
+#include "dense_plan.cuh"
 #include "dense_types.cuh"
+#include "tmap.cuh"
 
 namespace ictc {
 namespace {
 
-int current_device() {
-  int device = 0;
-  return cudaGetDevice(&device) == cudaSuccess ? device : 0;
-}
-
-bool chunk_aligned(const void* p, int64_t ld, size_t size) {
-  return aligned(p, 16) && (ld * static_cast<int64_t>(size)) % 16 == 0;
-}
-
-// Calls f with the activation code as a compile-time constant.
-template <typename F>
-void for_activation(int activation, const F& f) {
-  switch (activation) {
-    case ICTC_ACT_RELU: return f(std::integral_constant<int, ICTC_ACT_RELU>{});
-    case ICTC_ACT_SILU: return f(std::integral_constant<int, ICTC_ACT_SILU>{});
-    case ICTC_ACT_GELU: return f(std::integral_constant<int, ICTC_ACT_GELU>{});
-    case ICTC_ACT_GELU_TANH: return f(std::integral_constant<int, ICTC_ACT_GELU_TANH>{});
-    default: return f(std::integral_constant<int, ICTC_ACT_NONE>{});
-  }
-}
-
 // --------------------------------------------------------------------- y = act(pg) pu
-// One pass over p, bound by HBM.  V columns of each half a thread.
+// p is the sum of `splits` parts [m, 2 n], in order, and the bias; kept in `preact` where that is
+// given.  One pass, bound by HBM.  V columns of each half a thread.
 template <typename T, int V, int ACT>
-__global__ void __launch_bounds__(256) gate_kernel(const float* __restrict__ p, T* __restrict__ y,
-                                                   int64_t m, int64_t n) {
-  const int64_t units = n / V, total = m * units;
+__global__ void __launch_bounds__(256) gate_kernel(const float* parts, int splits,
+                                                   const T* __restrict__ bias, float* preact,
+                                                   T* __restrict__ y, int64_t m, int64_t n) {
+  using Floats = Pack<float, V>;
+  const int64_t units = n / V, total = m * units, part = m * 2 * n;
   const int64_t step = static_cast<int64_t>(gridDim.x) * 256;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total; i += step) {
-    const int64_t row = i / units, col = (i - row * units) * V;
-    const Pack<float, V> g = *reinterpret_cast<const Pack<float, V>*>(p + row * 2 * n + col);
-    const Pack<float, V> u = *reinterpret_cast<const Pack<float, V>*>(p + row * 2 * n + n + col);
+    const int64_t row = i / units, col = (i - row * units) * V, at = row * 2 * n + col;
+    Floats g = *reinterpret_cast<const Floats*>(parts + at);
+    Floats u = *reinterpret_cast<const Floats*>(parts + at + n);
+    for (int s = 1; s < splits; ++s) {
+      const Floats a = *reinterpret_cast<const Floats*>(parts + s * part + at);
+      const Floats b = *reinterpret_cast<const Floats*>(parts + s * part + at + n);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        g.v[j] += a.v[j];
+        u.v[j] += b.v[j];
+      }
+    }
+    if (bias) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        g.v[j] += to_float(bias[col + j]);
+        u.v[j] += to_float(bias[n + col + j]);
+      }
+    }
+    if (preact) {
+      *reinterpret_cast<Floats*>(preact + at) = g;
+      *reinterpret_cast<Floats*>(preact + at + n) = u;
+    }
     Pack<T, V> o;
 #pragma unroll
     for (int j = 0; j < V; ++j) o.v[j] = from_float<T>(activate<ACT>(g.v[j]) * u.v[j]);
     *reinterpret_cast<Pack<T, V>*>(y + row * n + col) = o;
+  }
+}
+
+// ---------------------------------------------------------------- few rows: no tiles
+// Up to four rows: W is read once and the products run on the FMA pipes.  `share` warps have
+// one column of y, each a part of K; a lane reads V consecutive elements of both rows of W, and
+// the warps' sums are added in warp order.
+constexpr int kFewThreads = 256, kFewWarps = kFewThreads / 32;
+constexpr int64_t kFewRows = 4;
+
+template <typename T, int ROWS, int V>
+__global__ void __launch_bounds__(kFewThreads) few_kernel(
+    const T* __restrict__ x, int64_t ldx, const T* __restrict__ w, int64_t ldw, int64_t rows,
+    int64_t n, int64_t k, int share, const Epilogue e) {
+  __shared__ float sums[kFewWarps][2 * ROWS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int per_cta = kFewWarps / share, part = warp % share;
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * per_cta; base < n;
+       base += static_cast<int64_t>(gridDim.x) * per_cta) {
+    const int64_t col = base + warp / share;
+    float acc[2 * ROWS];
+#pragma unroll
+    for (int r = 0; r < 2 * ROWS; ++r) acc[r] = 0.f;
+    if (col < n) {
+      const T* wg = w + col * ldw;
+      const T* wu = wg + n * ldw;
+#pragma unroll 4
+      for (int64_t c = (part * 32 + lane) * V; c < k; c += share * 32 * V) {
+        const Pack<T, V> pg = *reinterpret_cast<const Pack<T, V>*>(wg + c);
+        const Pack<T, V> pu = *reinterpret_cast<const Pack<T, V>*>(wu + c);
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+          if (r >= rows) break;
+          const Pack<T, V> px = *reinterpret_cast<const Pack<T, V>*>(x + r * ldx + c);
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            const float v = to_float(px.v[j]);
+            acc[2 * r] = fmaf(v, to_float(pg.v[j]), acc[2 * r]);
+            acc[2 * r + 1] = fmaf(v, to_float(pu.v[j]), acc[2 * r + 1]);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < 2 * ROWS; ++r)
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) acc[r] += __shfl_xor_sync(0xffffffffu, acc[r], o);
+    if (share > 1) {
+      if (lane == 0)
+#pragma unroll
+        for (int r = 0; r < 2 * ROWS; ++r) sums[warp][r] = acc[r];
+      __syncthreads();
+      if (part == 0)
+#pragma unroll
+        for (int r = 0; r < 2 * ROWS; ++r) {
+          acc[r] = 0.f;
+          for (int q = 0; q < share; ++q) acc[r] += sums[warp + q][r];
+        }
+      __syncthreads();
+    }
+    if (part == 0 && lane == 0 && col < n) {
+      const T* bias = static_cast<const T*>(e.bias);
+      const float bg = bias ? to_float(bias[col]) : 0.f, bu = bias ? to_float(bias[n + col]) : 0.f;
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) {
+        if (r >= rows) break;
+        const float pg = acc[2 * r] + bg, pu = acc[2 * r + 1] + bu;
+        if (e.preact) {
+          e.preact[r * 2 * n + col] = pg;
+          e.preact[r * 2 * n + n + col] = pu;
+        }
+        static_cast<T*>(e.out)[r * n + col] =
+            from_float<T>(activate<kAnyActivation>(pg, e.activation) * pu);
+      }
+    }
   }
 }
 
@@ -127,79 +218,120 @@ __global__ void __launch_bounds__(256) gated_slope_kernel(
 
 // ------------------------------------------------------------------- plan of a call
 
-int64_t aligned_pitch(int64_t width, size_t size) {
-  const int64_t v = static_cast<int64_t>(16 / size);
-  return ceil_div(width, v) * v;
-}
-
-int32_t layout_of(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t m, int64_t k,
-                  size_t size) {
+// What a call's pointers and strides allow.  (A single row may have any stride: the entry
+// points take it as packed.)
+int32_t layout_of(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t k, size_t size) {
   int32_t flags = 0;
   if (chunk_aligned(x, ldx, size) && chunk_aligned(w, ldw, size)) flags |= ICTC_LINEAR_ALIGNED;
-  if (aligned(x, 16) && (ldx == k || m <= 1)) flags |= ICTC_LINEAR_PACKED;
+  if (aligned(x, 16) && ldx == k) flags |= ICTC_LINEAR_PACKED;
   return flags;
 }
 
+enum class Way { few, pair, cut, general };
+
 // Byte offsets of the workspace's parts, and its size.
 struct GatedPlan {
-  size_t p, y, d, columns, product, product_bytes, total;
+  Way way;
+  bool align;  // operands are copied to aligned rows
+  PairPlan pair;
+  Split cut;
+  size_t x, w, partial;                  // forward
+  size_t p, y;                           // forward, general
+  size_t d, columns;                     // backward
+  size_t product, product_bytes, total;  // the linear layer's
+};
+
+struct Layout {
+  size_t at = 0;
+  size_t take(size_t bytes) {
+    const size_t here = at;
+    at += align_up(bytes, 256);
+    return here;
+  }
 };
 
 constexpr int64_t kSlopeParts = 296;
 
-// The forward's sums are a linear layer of 2 n outputs: p, and in 16-bit types the layer's
-// own output, which nobody reads.
 int plan_forward(int64_t m, int64_t n, int64_t k, int dtype, int32_t layout, bool keep, int device,
                  GatedPlan* b) {
   const size_t size = dtype_size(dtype);
-  size_t at = 0;
-  const auto take = [&](size_t bytes) {
-    const size_t here = at;
-    at += align_up(bytes, 256);
-    return here;
-  };
-  if (!keep) b->p = take(static_cast<size_t>(m) * 2 * n * sizeof(float));
-  if (dtype != ICTC_DTYPE_F32) b->y = take(static_cast<size_t>(m) * 2 * n * size);
+  const bool rows_aligned = layout & ICTC_LINEAR_ALIGNED;
+  const bool wide = dtype == ICTC_DTYPE_F32;
+  Layout space;
+  b->way = Way::general;
+  if (m <= kFewRows && ((rows_aligned && k % static_cast<int64_t>(16 / size) == 0) ||
+                        2 * n * k <= (1 << 18))) {
+    b->way = Way::few;
+    return ICTC_OK;
+  }
+  b->align = !rows_aligned && worth_aligning(m, 2 * n, k);
+  if (rows_aligned || b->align) {
+    int splits = 0;
+    if (wide) {
+      b->cut = plan_product(m, 2 * n, k, true, device, 128, 128);
+      if (b->cut.fits && m < (1ll << 30) && n < (1ll << 30) && k < (1ll << 30)) {
+        b->way = Way::cut;
+        splits = b->cut.splits;
+      }
+    } else {
+      b->pair = plan_pair(m, 2 * n, k, device);
+      if (b->pair.ok) {
+        b->way = Way::pair;
+        splits = b->pair.splits;
+      }
+    }
+    if (b->way != Way::general) {
+      if (b->align) {
+        b->x = space.take(static_cast<size_t>(m) * aligned_pitch(k, size) * size);
+        b->w = space.take(static_cast<size_t>(2 * n) * aligned_pitch(k, size) * size);
+      }
+      if (splits > 1) b->partial = space.take(static_cast<size_t>(splits) * m * 2 * n * sizeof(float));
+      b->total = space.at;
+      return ICTC_OK;
+    }
+  }
+  // the sums by the linear layer of 2 n outputs: p, and in 16-bit types the layer's own
+  // output, which nobody reads
+  if (!keep) b->p = space.take(static_cast<size_t>(m) * 2 * n * sizeof(float));
+  if (!wide) b->y = space.take(static_cast<size_t>(m) * 2 * n * size);
   size_t other;
   const int st = ictc_o2_linear_workspace(m, k, 2 * n, dtype, ICTC_ACT_NONE, layout, device,
                                           &b->product_bytes, &other);
   if (st != ICTC_OK) return st;
-  b->product = take(b->product_bytes);
-  b->total = at;
+  b->product = space.take(b->product_bytes);
+  b->total = space.at;
   return ICTC_OK;
 }
 
 int plan_backward(int64_t m, int64_t n, int64_t k, int dtype, int32_t layout, int device,
                   GatedPlan* b) {
   const size_t size = dtype_size(dtype);
-  size_t at = 0;
-  const auto take = [&](size_t bytes) {
-    const size_t here = at;
-    at += align_up(bytes, 256);
-    return here;
-  };
+  Layout space;
   const int64_t pitch = aligned_pitch(2 * n, size);
-  b->d = take(static_cast<size_t>(m) * pitch * size);
-  b->columns = take(static_cast<size_t>(m < kSlopeParts ? m : kSlopeParts) * 2 * n * sizeof(float));
+  b->d = space.take(static_cast<size_t>(m) * pitch * size);
+  b->columns =
+      space.take(static_cast<size_t>(m < kSlopeParts ? m : kSlopeParts) * 2 * n * sizeof(float));
   const int32_t flags = layout & (pitch == 2 * n || m <= 1 ? ~0 : ~ICTC_LINEAR_PACKED);
   size_t other;
   const int st = ictc_o2_linear_workspace(m, k, 2 * n, dtype, ICTC_ACT_NONE, flags, device,
                                           &other, &b->product_bytes);
   if (st != ICTC_OK) return st;
-  b->product = take(b->product_bytes);
-  b->total = at;
+  b->product = space.take(b->product_bytes);
+  b->total = space.at;
   return ICTC_OK;
 }
 
 template <typename T>
-int run_gate(const float* p, T* y, int64_t m, int64_t n, int activation, cudaStream_t stream) {
-  const bool vec = n % 4 == 0 && aligned(y, 4 * sizeof(T)) && aligned(p, 16);
+int run_gate(const float* parts, int splits, const T* bias, float* preact, T* y, int64_t m,
+             int64_t n, int activation, cudaStream_t stream) {
+  const bool vec = n % 4 == 0 && aligned(y, 4 * sizeof(T)) && aligned(parts, 16) &&
+                   aligned(preact, 16);
   const int64_t blocks = ceil_div(m * (vec ? n / 4 : n), 256);
   const int64_t cap = static_cast<int64_t>(sm_count(current_device())) * 8;
   const unsigned grid = static_cast<unsigned>(blocks < cap ? blocks : cap);
   for_activation(activation, [&](auto act) {
-    if (vec) gate_kernel<T, 4, act.value><<<grid, 256, 0, stream>>>(p, y, m, n);
-    else gate_kernel<T, 1, act.value><<<grid, 256, 0, stream>>>(p, y, m, n);
+    const auto kernel = vec ? gate_kernel<T, 4, act.value> : gate_kernel<T, 1, act.value>;
+    kernel<<<grid, 256, 0, stream>>>(parts, splits, bias, preact, y, m, n);
   });
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? ICTC_OK : cuda_fail(e, "gated linear gate launch");
@@ -238,17 +370,128 @@ int run_slope(const T* g, int64_t ldg, const float* p, T* d, int64_t ldd, float*
   return ICTC_OK;
 }
 
+// Calls f with the activation that a launch's epilogue needs: partial sums have none.
+template <typename F>
+void for_epilogue(const ProductArgs& p, const F& f) {
+  for_activation(p.e.partial ? ICTC_ACT_NONE : p.e.activation, f);
+}
+
+template <typename T, int V>
+int run_few(const T* x, int64_t ldx, const T* w, int64_t ldw, const Epilogue& e, int64_t m,
+            int64_t n, int64_t k, cudaStream_t stream) {
+  const int64_t sms = sm_count(current_device());
+  // all eight warps of a CTA share a column while that still gives every SM work
+  const int share = n <= sms * 8 ? kFewWarps : 1;
+  const int64_t want = ceil_div(n, kFewWarps / share);
+  const unsigned grid = static_cast<unsigned>(want < sms * 8 ? want : sms * 8);
+  const auto kernel = m == 1 ? few_kernel<T, 1, V> : few_kernel<T, kFewRows, V>;
+  kernel<<<grid, kFewThreads, 0, stream>>>(x, ldx, w, ldw, m, n, k, share, e);
+  const cudaError_t err = cudaGetLastError();
+  return err == cudaSuccess ? ICTC_OK : cuda_fail(err, "gated linear few-row launch");
+}
+
+template <typename T, int BN>
+int launch_pair(const OperandMaps& maps, const ProductArgs& p, cudaStream_t stream) {
+  const int64_t total = static_cast<int64_t>(p.tiles_m) * p.tiles_n * p.splits;
+  const int64_t pairs = sm_count(current_device()) / 2;
+  const unsigned grid = static_cast<unsigned>(2 * (total < pairs ? total : pairs));
+  int st = ICTC_OK;
+  for_epilogue(p, [&](auto act) {
+    const auto kernel = pair_product_kernel<T, false, false, BN, act.value, true>;
+    st = allow_smem(reinterpret_cast<const void*>(kernel), kPairSmem<BN>);
+    if (st == ICTC_OK) kernel<<<grid, kPairThreads, kPairSmem<BN>, stream>>>(maps, p);
+  });
+  return st;
+}
+
+int launch_cut(const OperandMaps& maps, const ProductArgs& p, cudaStream_t stream) {
+  constexpr int BN = 128;
+  const int64_t total = static_cast<int64_t>(p.tiles_m) * p.tiles_n * p.splits;
+  const int64_t sms = sm_count(current_device());
+  const unsigned grid = static_cast<unsigned>(total < sms ? total : sms);
+  int st = ICTC_OK;
+  for_epilogue(p, [&](auto act) {
+    const auto kernel = cut_product_kernel<false, false, BN, act.value, true>;
+    if (!cut_shares_fit<false, false, BN, act.value, true>()) {
+      st = fail(ICTC_ERR_UNSUPPORTED,
+                "float32 product: built with fewer than %d registers a thread",
+                kCutLaunchRegisters);
+      return;
+    }
+    st = allow_smem(reinterpret_cast<const void*>(kernel), kCutSmem<BN>);
+    if (st == ICTC_OK) kernel<<<grid, kCutThreads, kCutSmem<BN>, stream>>>(maps, p);
+  });
+  return st;
+}
+
 template <typename T>
-int run_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, void* y,
-                float* preact, unsigned char* ws, const GatedPlan& plan, int64_t m, int64_t n,
-                int64_t k, int dtype, int activation, cudaStream_t stream) {
-  float* p = preact ? preact : reinterpret_cast<float*>(ws + plan.p);
+int run_tiles(const T* x, int64_t ldx, const T* w, int64_t ldw, Epilogue e, unsigned char* ws,
+              const GatedPlan& plan, int64_t m, int64_t n, int64_t k, cudaStream_t stream) {
+  int st = ICTC_OK;
+  if (plan.align) {
+    st = align_operand(&x, &ldx, m, k, ws + plan.x, stream);
+    if (st == ICTC_OK) st = align_operand(&w, &ldw, 2 * n, k, ws + plan.w, stream);
+    if (st != ICTC_OK) return st;
+  }
+  ProductArgs p{};
+  p.m = m; p.n = n; p.k = k;
+  OperandMaps maps;
+  constexpr int kSize = sizeof(T);
+  constexpr bool kBf16 = std::is_same_v<T, __nv_bfloat16>;
+  int bn;
+  if constexpr (kSize == 2) {
+    p.tiles_m = plan.pair.tiles_m; p.tiles_n = plan.pair.tiles_n;
+    p.splits = plan.pair.splits; p.chunks = plan.pair.chunks;
+    p.chunks_per_split = plan.pair.chunks_per_split;
+    bn = plan.pair.bn;
+  } else {
+    p.tiles_m = plan.cut.tiles_m; p.tiles_n = plan.cut.tiles_n;
+    p.splits = plan.cut.splits; p.chunks = plan.cut.chunks;
+    p.chunks_per_split = plan.cut.chunks_per_split;
+    bn = plan.cut.bn;
+  }
+  constexpr int kBoxK = kSize == 2 ? 64 : kCutK;
+  if (encode_matrix_map(x, kSize, kBf16, k, m, ldx * kSize, kBoxK, 128, &maps.a) != 0 ||
+      encode_matrix_map(w, kSize, kBf16, k, 2 * n, ldw * kSize, kBoxK, bn / 2, &maps.b) != 0)
+    return fail(ICTC_ERR_UNSUPPORTED, "gated linear: no tensor map for these operands");
+  float* partial = p.splits > 1 ? reinterpret_cast<float*>(ws + plan.partial) : nullptr;
+  e.vec = vec_epilogue<T>(e, n);
+  p.e = e;
+  p.e.partial = partial;
+  if (partial) p.e.vec = n % 4 == 0;
+  if constexpr (kSize == 2)
+    st = bn == 256 ? launch_pair<T, 256>(maps, p, stream) : launch_pair<T, 128>(maps, p, stream);
+  else
+    st = launch_cut(maps, p, stream);
+  if (st != ICTC_OK) return st;
+  const cudaError_t err = cudaGetLastError();
+  if (err != cudaSuccess) return cuda_fail(err, "gated linear product launch");
+  if (!partial) return ICTC_OK;
+  return run_gate<T>(partial, p.splits, static_cast<const T*>(e.bias), e.preact,
+                     static_cast<T*>(e.out), m, n, e.activation, stream);
+}
+
+template <typename T>
+int run_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const Epilogue& e,
+                unsigned char* ws, const GatedPlan& plan, int64_t m, int64_t n, int64_t k,
+                int dtype, cudaStream_t stream) {
+  const T* xt = static_cast<const T*>(x);
+  const T* wt = static_cast<const T*>(w);
+  if (plan.way == Way::few) {
+    constexpr int kFull = 16 / sizeof(T);
+    if (k % kFull == 0 && chunk_aligned(x, ldx, sizeof(T)) && chunk_aligned(w, ldw, sizeof(T)))
+      return run_few<T, kFull>(xt, ldx, wt, ldw, e, m, n, k, stream);
+    return run_few<T, 1>(xt, ldx, wt, ldw, e, m, n, k, stream);
+  }
+  if (plan.way != Way::general) return run_tiles(xt, ldx, wt, ldw, e, ws, plan, m, n, k, stream);
+  float* p = e.preact ? e.preact : reinterpret_cast<float*>(ws + plan.p);
   const bool wide = sizeof(T) == 4;
   const int st = ictc_o2_linear_forward(
-      x, ldx, w, ldw, bias, nullptr, 0, wide ? static_cast<void*>(p) : ws + plan.y,
+      x, ldx, w, ldw, e.bias, nullptr, 0, wide ? static_cast<void*>(p) : ws + plan.y,
       wide ? nullptr : p, ws + plan.product, plan.product_bytes, m, k, 2 * n, dtype, ICTC_ACT_NONE,
       stream);
-  return st != ICTC_OK ? st : run_gate<T>(p, static_cast<T*>(y), m, n, activation, stream);
+  if (st != ICTC_OK) return st;
+  return run_gate<T>(p, 1, nullptr, nullptr, static_cast<T*>(e.out), m, n, e.activation, stream);
 }
 
 template <typename T>
@@ -289,6 +532,13 @@ int check_workspace(const void* workspace, size_t bytes, size_t needed) {
 }
 
 }  // namespace
+
+int gated_take_device_error(int* code) {
+  cudaError_t e;
+  if (take_unit_device_error(code, &e) != 0) return cuda_fail(e, "gated linear device error flag");
+  return ICTC_OK;
+}
+
 }  // namespace ictc
 
 using namespace ictc;
@@ -320,18 +570,24 @@ extern "C" int32_t ictc_o2_gated_linear_forward(const void* x, int64_t x_stride,
   if (st != ICTC_OK) return st;
   if (rows == 0) return ICTC_OK;
   if (!x || !weight || !y) return fail(ICTC_ERR_INVALID, "null pointer");
-  if (x_stride < 0 || weight_stride < 0) return fail(ICTC_ERR_INVALID, "negative row stride");
-  const int32_t layout =
-      layout_of(x, x_stride, weight, weight_stride, rows, in, dtype_size(dtype));
+  if (rows == 1) x_stride = in;
+  if (x_stride < in || weight_stride < in)
+    return fail(ICTC_ERR_INVALID, "rows of x and weight must not overlap");
+  const int32_t layout = layout_of(x, x_stride, weight, weight_stride, in, dtype_size(dtype));
   GatedPlan plan{};
   st = plan_forward(rows, hidden, in, dtype, layout, preact != nullptr, current_device(), &plan);
   if (st == ICTC_OK) st = check_workspace(workspace, workspace_bytes, plan.total);
   if (st != ICTC_OK) return st;
+  Epilogue e{};
+  e.bias = bias;
+  e.preact = preact;
+  e.out = y;
+  e.activation = activation;
   unsigned char* ws = static_cast<unsigned char*>(workspace);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-#define ICTC_GATED_FORWARD(T)                                                                  \
-  return run_forward<T>(x, x_stride, weight, weight_stride, bias, y, preact, ws, plan, rows, \
-                        hidden, in, dtype, activation, s)
+#define ICTC_GATED_FORWARD(T)                                                                 \
+  return run_forward<T>(x, x_stride, weight, weight_stride, e, ws, plan, rows, hidden, in, dtype, \
+                        s)
   if (dtype == ICTC_DTYPE_F32) ICTC_GATED_FORWARD(float);
   if (dtype == ICTC_DTYPE_BF16) ICTC_GATED_FORWARD(__nv_bfloat16);
   ICTC_GATED_FORWARD(__half);
@@ -352,10 +608,11 @@ extern "C" int32_t ictc_o2_gated_linear_backward(
                                    ICTC_ACT_NONE, stream);
   if (!grad_x && !grad_weight && !grad_bias) return ICTC_OK;
   if (!x || !weight || !grad_output || !preact) return fail(ICTC_ERR_INVALID, "null pointer");
-  if (x_stride < 0 || weight_stride < 0 || grad_stride < 0)
-    return fail(ICTC_ERR_INVALID, "negative row stride");
-  const int32_t layout =
-      layout_of(x, x_stride, weight, weight_stride, rows, in, dtype_size(dtype));
+  if (rows == 1) x_stride = in;
+  if (x_stride < in || weight_stride < in)
+    return fail(ICTC_ERR_INVALID, "rows of x and weight must not overlap");
+  if (grad_stride < 0) return fail(ICTC_ERR_INVALID, "negative row stride");
+  const int32_t layout = layout_of(x, x_stride, weight, weight_stride, in, dtype_size(dtype));
   GatedPlan plan{};
   st = plan_backward(rows, hidden, in, dtype, layout, current_device(), &plan);
   if (st == ICTC_OK) st = check_workspace(workspace, workspace_bytes, plan.total);

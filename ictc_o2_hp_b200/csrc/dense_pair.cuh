@@ -125,7 +125,10 @@ __device__ __forceinline__ void load_tile(unsigned char* dst, const CUtensorMap*
   }
 }
 
-template <typename T, bool A_MN, bool B_MN, int BN, int ACT>
+// GATED: the forward of the gated layer.  p.n is the number of its outputs; a tile has BN / 2
+// columns of the gate's sums, whose rows of W the leading CTA brings, and after them the same
+// columns of the other half, whose rows its peer brings.
+template <typename T, bool A_MN, bool B_MN, int BN, int ACT, bool GATED = false>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     pair_product_kernel(const __grid_constant__ OperandMaps maps, const __grid_constant__ ProductArgs p) {
   constexpr int S = kPairStages<BN>;
@@ -164,15 +167,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   const uint32_t tmem = *tmem_at;
   const int64_t total = static_cast<int64_t>(p.tiles_m) * p.tiles_n * p.splits;
   const int64_t first = blockIdx.x >> 1, step = gridDim.x >> 1;
+  constexpr int kTile = GATED ? BN / 2 : BN;  // columns of the output
 
   if (warp == kPairLoadWarp) {
     if (lane == 0) {
       bool ok = true;
       uint32_t it = 0;
       for (int64_t t = first; ok && t < total; t += step) {
-        const TilePos pos = tile_at<kPairRows>(p, t, BN);
+        const TilePos pos = tile_at<kPairRows>(p, t, kTile);
         const int m0 = static_cast<int>(pos.m0) + rank * 128;
-        const int n0 = static_cast<int>(pos.n0) + rank * (BN / 2);
+        const int n0 =
+            static_cast<int>(pos.n0) + static_cast<int>(rank) * (GATED ? static_cast<int>(p.n) : BN / 2);
         for (int c = pos.c0; c < pos.c1; ++c, ++it) {
           const int s = it % S;
           ok = mbar_wait_idle(&empty[s], ((it / S) & 1) ^ 1, kCodeProducer);
@@ -201,7 +206,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       bool ok = true;
       uint32_t it = 0, set = 0;
       for (int64_t t = first; ok && t < total; t += step, ++set) {
-        const TilePos pos = tile_at<kPairRows>(p, t, BN);
+        const TilePos pos = tile_at<kPairRows>(p, t, kTile);
         ok = mbar_wait_idle(&room[set & 1], ((set >> 1) & 1) ^ 1, kCodeMma);
         if (!ok) break;
         tcgen05_fence_after();
@@ -231,15 +236,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     __syncwarp();
   } else {
     const int quad = warp & 3, half = warp >> 2;
-    constexpr int kHalf = BN / 2;
+    constexpr int kHalf = kTile / 2;
     float4* mine = reinterpret_cast<float4*>(staging + warp * 4096);
     bool ok = true;
     uint32_t set = 0;
     for (int64_t t = first; t < total; t += step, ++set) {
-      const TilePos pos = tile_at<kPairRows>(p, t, BN);
+      const TilePos pos = tile_at<kPairRows>(p, t, kTile);
       const int64_t row0 = pos.m0 + rank * 128 + quad * 32, col0 = pos.n0 + half * kHalf;
       ResidualBlock<T> res, next;
-      load_residual(p, row0, col0, lane, next);
+      if constexpr (!GATED) load_residual(p, row0, col0, lane, next);
       ok = mbar_wait_warp(&done[set & 1], (set >> 1) & 1, kCodeEpilogue);
       if (!ok) break;
       tcgen05_fence_after();
@@ -247,21 +252,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           tmem + (set & 1) * BN + (static_cast<uint32_t>(quad * 32) << 16) + half * kHalf;
 #pragma unroll 1
       for (int cb = 0; cb < kHalf / 32; ++cb) {
-        float acc[32];
-        float(&lo)[16] = *reinterpret_cast<float(*)[16]>(acc);
-        float(&hi)[16] = *reinterpret_cast<float(*)[16]>(acc + 16);
-        tmem_load16(at + cb * 32, lo);
-        tmem_load16(at + cb * 32 + 16, hi);
-        res = next;
+        float acc[GATED ? 64 : 32];
+#pragma unroll
+        for (int j = 0; j < (GATED ? 64 : 32); j += 16)
+          tmem_load16(at + cb * 32 + (j < 32 ? j : BN / 2 + j - 32),
+                      *reinterpret_cast<float(*)[16]>(acc + j));
         const bool last = cb == kHalf / 32 - 1;
-        if (!last) load_residual(p, row0, col0 + (cb + 1) * 32, lane, next);
+        if constexpr (!GATED) {
+          res = next;
+          if (!last) load_residual(p, row0, col0 + (cb + 1) * 32, lane, next);
+        }
         tmem_load_wait();
         if (last) {  // the set's last columns are in registers
           tcgen05_fence_before();
           __syncwarp();
           if (lane == 0) arrive_cluster(peer_addr(&room[set & 1], 0));
         }
-        write_block<T, ACT>(p, pos.split, acc, mine, row0, col0 + cb * 32, lane, res);
+        if constexpr (GATED)
+          write_gated_block<T, ACT>(p, pos.split, acc, acc + 32, mine, row0, col0 + cb * 32, lane);
+        else
+          write_block<T, ACT>(p, pos.split, acc, mine, row0, col0 + cb * 32, lane, res);
       }
     }
   }
