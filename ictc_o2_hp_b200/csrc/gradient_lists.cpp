@@ -5,13 +5,13 @@
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/extension.h>
 
 #include <algorithm>
 #include <cstdint>
-#include <optional>
 #include <string>
-#include <tuple>
+#include <utility>
 #include <vector>
 
 #include "ictc_o2_b200.h"
@@ -19,7 +19,6 @@
 namespace {
 
 using at::Tensor;
-using Tensors = std::vector<Tensor>;
 
 struct Api {
   decltype(&ictc_o2_last_error) last_error;
@@ -38,27 +37,55 @@ void check(int32_t status, const char* what) {
   TORCH_CHECK(false, message);
 }
 
+// A Python sequence of tensors (or one tensor), read where it lies.
+class Sequence {
+ public:
+  Sequence(const char* what, py::handle given) : what_(what) {
+    if (THPVariable_Check(given.ptr())) {
+      items_ = py::make_tuple(given);
+    } else {
+      items_ = py::reinterpret_steal<py::object>(PySequence_Fast(given.ptr(), "expected tensors"));
+      if (!items_) throw py::error_already_set();
+    }
+    size_ = static_cast<size_t>(PySequence_Fast_GET_SIZE(items_.ptr()));
+  }
+  size_t size() const { return size_; }
+  const Tensor& operator[](size_t i) const {
+    PyObject* item = PySequence_Fast_GET_ITEM(items_.ptr(), static_cast<Py_ssize_t>(i));
+    TORCH_CHECK_TYPE(THPVariable_Check(item), what_, " takes tensors, got ", Py_TYPE(item)->tp_name);
+    return THPVariable_Unpack(item);
+  }
+  const py::object& items() const { return items_; }
+
+ private:
+  const char* what_;
+  py::object items_;
+  size_t size_;
+};
+
 // Whether a call on these tensors has to be seen by the dispatcher (a trace, fake tensors).
-bool watched(const Tensors& tensors) {
+bool watched(const Sequence& tensors) {
   using K = c10::DispatchKey;
   constexpr c10::DispatchKeySet kWatchers(
       {K::Python, K::Tracer, K::Functionalize, K::FuncTorchDynamicLayerFrontMode,
        K::FuncTorchBatched, K::FuncTorchGradWrapper});
   const auto local = c10::impl::tls_local_dispatch_key_set();
   c10::DispatchKeySet keys = local.included_;
-  for (const Tensor& t : tensors) keys = keys | t.key_set();
+  for (size_t i = 0; i < tensors.size(); ++i) keys = keys | tensors[i].key_set();
   return !((keys - local.excluded_) & kWatchers).empty();
 }
 
-void check_inputs(const char* what, const Tensors& tensors) {
-  for (const Tensor& t : tensors) {
+void check_inputs(const char* what, const Sequence& tensors) {
+  const auto device = tensors[0].device();
+  for (size_t i = 0; i < tensors.size(); ++i) {
+    const Tensor& t = tensors[i];
     const auto type = t.scalar_type();
     TORCH_CHECK_TYPE(t.layout() == at::kStrided && t.is_cuda() &&
                          (type == at::kFloat || type == at::kBFloat16 || type == at::kHalf),
                      what, " takes dense CUDA float32, bfloat16 or float16 tensors; got ", type,
                      " (", t.layout(), ") on ", t.device());
-    TORCH_CHECK_VALUE(t.device() == tensors[0].device(), what, ": tensors are on ",
-                      tensors[0].device(), " and ", t.device());
+    TORCH_CHECK_VALUE(t.device() == device, what, ": tensors are on ", device, " and ",
+                      t.device());
   }
 }
 
@@ -70,55 +97,65 @@ struct Lists {
   std::vector<void*> out;
   std::vector<int64_t> counts;
   std::vector<int32_t> dtypes;
-  Tensors kept;  // copies that the call reads
+  std::vector<Tensor> kept;  // copies that the call reads
 
+  explicit Lists(size_t size) {
+    in.reserve(size);
+    out.reserve(size);
+    counts.reserve(size);
+    dtypes.reserve(size);
+  }
   void add(const Tensor& t) {
     const auto type = t.scalar_type();
-    in.push_back(t.numel() ? t.data_ptr() : nullptr);
+    in.push_back(t.numel() ? t.const_data_ptr() : nullptr);
     counts.push_back(t.numel());
     dtypes.push_back(type == at::kFloat ? ICTC_DTYPE_F32
                      : type == at::kBFloat16 ? ICTC_DTYPE_BF16 : ICTC_DTYPE_F16);
   }
-};
-
-Tensor plain_copy(const Tensor& t) { return t.resolve_neg().contiguous(); }
-
-struct Space {
-  Tensor norm, workspace;
-  size_t bytes = 0;
-};
-
-Space space_for(const Tensors& tensors) {
-  Space s;
-  const auto options = at::TensorOptions().device(tensors[0].device());
-  check(api.workspace(static_cast<int64_t>(tensors.size()), tensors[0].device().index(), &s.bytes),
-        "grad_norm_workspace");
-  s.norm = at::empty({}, options.dtype(at::kFloat));
-  s.workspace = at::empty({static_cast<int64_t>(s.bytes)}, options.dtype(at::kByte));
-  return s;
-}
-
-void* stream_of(const Tensor& t) {
-  return c10::cuda::getCurrentCUDAStream(t.device().index()).stream();
-}
-
-Tensor grad_norm(const Tensors& tensors, bool largest) {
-  check_inputs("grad_norm", tensors);
-  TORCH_CHECK_VALUE(!tensors.empty(), "grad_norm: no tensors");
-  const at::NoGradGuard no_grad;
-  const c10::cuda::CUDAGuard guard(tensors[0].device());
-  Lists lists;
-  for (const Tensor& t : tensors) {
-    lists.kept.push_back(dense(t) ? t : plain_copy(t));
-    lists.add(lists.kept.back());
+  void add_copy(const Tensor& t) {
+    kept.push_back(t.resolve_neg().contiguous());
+    add(kept.back());
   }
-  const Space s = space_for(tensors);
-  check(api.norm(lists.in.data(), lists.counts.data(), lists.dtypes.data(),
-                 static_cast<int64_t>(lists.in.size()),
+  int64_t size() const { return static_cast<int64_t>(in.size()); }
+};
+
+// The norm, and workspace that goes back to the current stream's pool with this.
+struct Space {
+  Tensor norm;
+  c10::DataPtr workspace;
+  size_t bytes = 0;
+
+  Space(int64_t tensors, c10::Device device) {
+    check(api.workspace(tensors, device.index(), &bytes), "grad_norm_workspace");
+    norm = at::empty({}, at::TensorOptions().device(device).dtype(at::kFloat));
+    workspace = c10::GetAllocator(c10::kCUDA)->allocate(bytes);
+  }
+};
+
+void* stream_of(c10::Device device) {
+  return c10::cuda::getCurrentCUDAStream(device.index()).stream();
+}
+
+// None where the dispatcher has to see the call.
+py::object grad_norm(py::handle given, bool largest) {
+  const Sequence tensors("grad_norm", given);
+  TORCH_CHECK_VALUE(tensors.size() > 0, "grad_norm: no tensors");
+  if (watched(tensors)) return py::none();
+  check_inputs("grad_norm", tensors);
+  const auto device = tensors[0].device();
+  const at::NoGradGuard no_grad;
+  const c10::cuda::CUDAGuard guard(device);
+  Lists lists(tensors.size());
+  for (size_t i = 0; i < tensors.size(); ++i) {
+    if (dense(tensors[i])) lists.add(tensors[i]);
+    else lists.add_copy(tensors[i]);
+  }
+  const Space s(lists.size(), device);
+  check(api.norm(lists.in.data(), lists.counts.data(), lists.dtypes.data(), lists.size(),
                  largest ? ICTC_GRAD_NORM_MAX : ICTC_GRAD_NORM_2, s.norm.data_ptr<float>(),
-                 s.workspace.data_ptr(), s.bytes, stream_of(tensors[0])),
+                 s.workspace.get(), s.bytes, stream_of(device)),
         "grad_norm");
-  return s.norm;
+  return py::cast(s.norm);
 }
 
 // Refuses outputs that share memory with one another or with another gradient: their
@@ -146,59 +183,81 @@ void check_apart(const Lists& lists) {
                       "clip_grads: gradients or outputs share memory; list each tensor once");
 }
 
-// out = grads scaled to at most max_norm; `fresh`: the outputs were made for this call.
-Tensor clip(const Tensors& grads, const Tensors& out, double max_norm, bool largest, bool fresh) {
-  check_inputs("clip_grads", grads);
-  TORCH_CHECK_VALUE(!grads.empty(), "clip_grads: no tensors");
-  TORCH_CHECK_VALUE(max_norm >= 0, "clip_grads: max_norm must be >= 0, got ", max_norm);
-  TORCH_CHECK_VALUE(out.size() == grads.size(), "clip_grads: ", grads.size(), " gradients and ",
-                    out.size(), " outputs");
-  const at::NoGradGuard no_grad;
-  const c10::cuda::CUDAGuard guard(grads[0].device());
-  for (size_t i = 0; !fresh && i < out.size(); ++i) {
-    TORCH_CHECK_VALUE(out[i].sizes() == grads[i].sizes() &&
-                          out[i].scalar_type() == grads[i].scalar_type() &&
-                          out[i].device() == grads[i].device() && out[i].layout() == at::kStrided,
-                      "clip_grads: output ", i, " must have its gradient's shape, type and "
-                      "device");
-    TORCH_CHECK_VALUE(at::has_internal_overlap(out[i]) != at::MemOverlap::Yes,
-                      "clip_grads: output ", i, " has elements that share memory");
-  }
-  Lists lists;
-  Tensors targets;  // what the kernels write, where it is not the output itself
-  for (size_t i = 0; i < grads.size(); ++i) {
-    const Tensor &g = grads[i], &o = out[i];
-    const bool same = dense(g) && dense(o) && g.strides() == o.strides();
-    const bool plain = !same && dense(o) && o.is_contiguous();
-    lists.kept.push_back(same ? g : plain_copy(g));
-    lists.add(lists.kept.back());
-    targets.push_back(same || plain ? o : at::empty(g.sizes(), g.options()));
-    lists.out.push_back(g.numel() ? targets.back().data_ptr() : nullptr);
-  }
-  if (!fresh) check_apart(lists);
-  const Space s = space_for(grads);
+Tensor launch(const Lists& lists, c10::Device device, double max_norm, bool largest) {
+  const Space s(lists.size(), device);
   check(api.clip(lists.in.data(), lists.out.data(), lists.counts.data(), lists.dtypes.data(),
-                 static_cast<int64_t>(lists.in.size()),
-                 largest ? ICTC_GRAD_NORM_MAX : ICTC_GRAD_NORM_2, max_norm,
-                 s.norm.data_ptr<float>(), s.workspace.data_ptr(), s.bytes, stream_of(grads[0])),
+                 lists.size(), largest ? ICTC_GRAD_NORM_MAX : ICTC_GRAD_NORM_2, max_norm,
+                 s.norm.data_ptr<float>(), s.workspace.get(), s.bytes, stream_of(device)),
         "clip_grads");
-  for (size_t i = 0; !fresh && i < out.size(); ++i) {
-    if (!targets[i].is_same(out[i])) out[i].copy_(targets[i]);
-    else if (!out[i].is_inference()) out[i].unsafeGetTensorImpl()->bump_version();
-  }
   return s.norm;
 }
 
-std::tuple<Tensors, Tensor> clip_grads(const Tensors& grads, double max_norm, bool largest,
-                                       const std::optional<Tensors>& out) {
-  if (out.has_value()) return {*out, clip(grads, *out, max_norm, largest, false)};
+// Into the tensors of `out`.
+Tensor clip_into(const Sequence& grads, const Sequence& out, double max_norm, bool largest) {
+  TORCH_CHECK_VALUE(out.size() == grads.size(), "clip_grads: ", grads.size(), " gradients and ",
+                    out.size(), " outputs");
+  Lists lists(grads.size());
+  std::vector<std::pair<size_t, Tensor>> apart;  // results that the kernels leave elsewhere
+  for (size_t i = 0; i < grads.size(); ++i) {
+    const Tensor &g = grads[i], &o = out[i];
+    const bool one = g.is_same(o);
+    if (!one) {
+      TORCH_CHECK_VALUE(o.sizes() == g.sizes() && o.scalar_type() == g.scalar_type() &&
+                            o.device() == g.device() && o.layout() == at::kStrided,
+                        "clip_grads: output ", i, " must have its gradient's shape, type and "
+                        "device");
+    }
+    if (dense(g) && (one || (dense(o) && g.strides() == o.strides()))) {
+      lists.add(g);
+      lists.out.push_back(g.numel() ? o.data_ptr() : nullptr);
+      continue;
+    }
+    TORCH_CHECK_VALUE(at::has_internal_overlap(o) != at::MemOverlap::Yes, "clip_grads: output ", i,
+                      " has elements that share memory");
+    lists.add_copy(g);
+    if (!dense(o) || !o.is_contiguous())
+      apart.emplace_back(i, at::empty(g.sizes(), g.options()));
+    const Tensor& to = !apart.empty() && apart.back().first == i ? apart.back().second : o;
+    lists.out.push_back(g.numel() ? to.data_ptr() : nullptr);
+  }
+  check_apart(lists);
+  const Tensor norm = launch(lists, grads[0].device(), max_norm, largest);
+  size_t next = 0;
+  for (size_t i = 0; i < out.size(); ++i) {
+    if (next < apart.size() && apart[next].first == i) out[i].copy_(apart[next++].second);
+    else if (!out[i].is_inference()) out[i].unsafeGetTensorImpl()->bump_version();
+  }
+  return norm;
+}
+
+// (outputs, norm); None where the dispatcher has to see the call.
+py::object clip_grads(py::handle given, double max_norm, bool largest, py::handle out) {
+  const Sequence grads("clip_grads", given);
+  TORCH_CHECK_VALUE(max_norm >= 0, "clip_grads: max_norm must be >= 0, got ", max_norm);
+  TORCH_CHECK_VALUE(grads.size() > 0, "clip_grads: no tensors");
+  if (watched(grads)) return py::none();
   check_inputs("clip_grads", grads);
+  const auto device = grads[0].device();
   const at::NoGradGuard no_grad;
-  Tensors made;
-  made.reserve(grads.size());
-  for (const Tensor& g : grads) made.push_back(at::empty_like(g));
-  const Tensor norm = clip(grads, made, max_norm, largest, true);
-  return {made, norm};
+  const c10::cuda::CUDAGuard guard(device);
+  if (!out.is_none()) {
+    const Sequence to("clip_grads", out);
+    if (watched(to)) return py::none();
+    const Tensor norm = clip_into(grads, to, max_norm, largest);
+    return py::make_tuple(py::list(to.items()), norm);
+  }
+  Lists lists(grads.size());
+  py::list made(grads.size());
+  for (size_t i = 0; i < grads.size(); ++i) {
+    const Tensor& g = grads[i];
+    const Tensor o = dense(g) ? at::empty_like(g) : at::empty(g.sizes(), g.options());
+    made[i] = py::cast(o);
+    if (dense(g)) lists.add(g);
+    else lists.add_copy(g);
+    lists.out.push_back(o.numel() ? o.data_ptr() : nullptr);
+  }
+  const Tensor norm = launch(lists, device, max_norm, largest);
+  return py::make_tuple(made, norm);
 }
 
 // Entry points of the loaded kernel library, by address.
@@ -214,7 +273,6 @@ void bind(uintptr_t last_error, uintptr_t workspace, uintptr_t norm, uintptr_t c
 
 PYBIND11_MODULE(_gradient_lists, m) {
   m.def("bind", &bind);
-  m.def("watched", &watched);
   m.def("grad_norm", &grad_norm);
   m.def("clip_grads", &clip_grads);
 }

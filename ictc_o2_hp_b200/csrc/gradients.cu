@@ -7,10 +7,13 @@
 // elsewhere) read again and written.  A launch takes up to 1,024 tensors of mixed types,
 // their addresses and sizes among its arguments, so nothing is copied to the device and a
 // captured call holds all it needs.  Work is cut into chunks of 32 KB that are dealt out to
-// the CTAs in order; a CTA's sum goes to its place in the workspace and every CTA of the
-// second pass adds those up in the same order, so that results do not depend on scheduling.
-// The second pass takes a CTA's chunks from the last to the first: the last ones are still in
-// L2.
+// groups of 256 threads in order, and sums are added up in that order, so that results do not
+// depend on scheduling.
+//
+// Two launches: every CTA leaves its sum in the workspace; every CTA of the second adds those
+// up and scales its chunks, from the last to the first, which are still in L2.  Up to
+// kClusterChunks chunks are one launch of a cluster, whose CTAs read each other's sums from
+// shared memory.
 //
 // Squares are added in float32 over the 16 bytes of a load and in float64 beyond.  Where
 // such a short sum leaves float32's safe range it is taken again in float64, so the norm is
@@ -21,15 +24,18 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "dense_pair.cuh"
 #include "dense_types.cuh"
 
 namespace ictc {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kUnits = 8;  // 16-byte units of a chunk per thread
+constexpr int kThreads = 256;  // of a group that takes a chunk
+constexpr int kUnits = 8;      // 16-byte units of a chunk per thread
 constexpr int kChunkBytes = kThreads * kUnits * 16;
 constexpr int kBlocksPerSm = 8;
+constexpr int kClusterCtas = 8, kClusterGroups = 2;  // groups of a CTA
+constexpr int kClusterChunks = 128;
 constexpr int kMostTensors = 1024;  // of a launch: 29 bytes each of its 32,764 of arguments
 
 enum Kind { kTwoNorm = ICTC_GRAD_NORM_2, kMaxNorm = ICTC_GRAD_NORM_MAX };
@@ -44,6 +50,7 @@ struct Tensors {
   int first[N + 1];  // chunks before each tensor
   uint8_t dtype[N];
   int tensors;
+  bool in_place;  // every out is its in
 };
 
 struct Place {
@@ -155,9 +162,10 @@ struct Running<kMaxNorm> {
 };
 
 // The running value over all threads of the CTA, in a fixed order; every thread gets it.
-template <int KIND>
+template <int KIND, int GROUPS = 1>
 __device__ __forceinline__ Running<KIND> over_block(Running<KIND> r) {
-  __shared__ double parts[kThreads / 32];
+  constexpr int kWarps = GROUPS * kThreads / 32;
+  __shared__ double parts[kWarps];
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) r.join(__shfl_xor_sync(0xffffffffu, r.get(), o));
   __syncthreads();
@@ -165,40 +173,50 @@ __device__ __forceinline__ Running<KIND> over_block(Running<KIND> r) {
   __syncthreads();
   Running<KIND> all;
 #pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) all.join(parts[w]);
+  for (int w = 0; w < kWarps; ++w) all.join(parts[w]);
   return all;
 }
 
-template <int KIND, typename T, int N>
-__device__ __forceinline__ void add_chunk(const Tensors<N>& list, const Place& at,
-                                          Running<KIND>& r) {
+// `meanwhile` runs between the loads and the arithmetic.
+template <int KIND, typename T, int N, typename F>
+__device__ __forceinline__ void add_chunk(const Tensors<N>& list, const Place& at, int thread,
+                                          Running<KIND>& r, const F& meanwhile) {
   const Chunk<T> c = chunk_at<T>(list, at);
   Pack<T, 16 / sizeof(T)> v[kUnits];
 #pragma unroll
-  for (int i = 0; i < kUnits; ++i) v[i] = load_unit(c, i * kThreads + threadIdx.x);
+  for (int i = 0; i < kUnits; ++i) v[i] = load_unit(c, i * kThreads + thread);
+  meanwhile();
 #pragma unroll
   for (int i = 0; i < kUnits; ++i) r.add(v[i]);
 }
 
+// The thread's part of chunks first, first + step, ...
 template <int KIND, int N>
-__device__ __forceinline__ Running<KIND> block_value(const Tensors<N>& list) {
+__device__ __forceinline__ Running<KIND> add_chunks(const Tensors<N>& list, int first, int step,
+                                                    int thread) {
   Running<KIND> r;
   const int chunks = list.first[list.tensors];
-  for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
-    const Place at = place_of(list, c);
+  Place next{};
+  if (first < chunks) next = place_of(list, first);
+  for (int c = first; c < chunks; c += step) {
+    const Place at = next;
+    const auto meanwhile = [&] {
+      if (c + step < chunks) next = place_of(list, c + step);
+    };
     switch (list.dtype[at.tensor]) {
-      case ICTC_DTYPE_F32: add_chunk<KIND, float>(list, at, r); break;
-      case ICTC_DTYPE_BF16: add_chunk<KIND, __nv_bfloat16>(list, at, r); break;
-      default: add_chunk<KIND, __half>(list, at, r);
+      case ICTC_DTYPE_F32: add_chunk<KIND, float>(list, at, thread, r, meanwhile); break;
+      case ICTC_DTYPE_BF16: add_chunk<KIND, __nv_bfloat16>(list, at, thread, r, meanwhile); break;
+      default: add_chunk<KIND, __half>(list, at, thread, r, meanwhile);
     }
   }
-  return over_block(r);
+  return r;
 }
 
 template <int KIND, int N>
 __global__ void __launch_bounds__(kThreads)
     partial_kernel(const __grid_constant__ Tensors<N> list, double* __restrict__ partial) {
-  const Running<KIND> r = block_value<KIND>(list);
+  const Running<KIND> r = over_block(
+      add_chunks<KIND>(list, static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x), threadIdx.x));
   if (threadIdx.x == 0) partial[blockIdx.x] = r.get();
 }
 
@@ -224,17 +242,17 @@ __device__ __forceinline__ float factor_of(double norm, double max_norm) {
 
 template <typename T, int N>
 __device__ __forceinline__ void scale_chunk(const Tensors<N>& list, const Place& at,
-                                            float factor) {
+                                            int thread, float factor) {
   constexpr int V = 16 / sizeof(T), kElements = kChunkBytes / sizeof(T);
   const Chunk<T> c = chunk_at<T>(list, at);
   T* out = static_cast<T*>(list.out[at.tensor]) + c.offset;
   if (reinterpret_cast<uintptr_t>(out) % 16 == 0) {
     Pack<T, V> v[kUnits];
 #pragma unroll
-    for (int i = 0; i < kUnits; ++i) v[i] = load_unit(c, i * kThreads + threadIdx.x);
+    for (int i = 0; i < kUnits; ++i) v[i] = load_unit(c, i * kThreads + thread);
 #pragma unroll
     for (int i = 0; i < kUnits; ++i) {
-      const int e = (i * kThreads + threadIdx.x) * V;
+      const int e = (i * kThreads + thread) * V;
 #pragma unroll
       for (int j = 0; j < V; ++j) v[i].v[j] = from_float<T>(to_float(v[i].v[j]) * factor);
       if (e >= c.begin && e + V <= c.end) {
@@ -247,7 +265,7 @@ __device__ __forceinline__ void scale_chunk(const Tensors<N>& list, const Place&
     }
   } else {  // boundaries apart: element by element
     constexpr int kAhead = 8;
-    for (int e0 = threadIdx.x; e0 < kElements; e0 += kAhead * kThreads) {
+    for (int e0 = thread; e0 < kElements; e0 += kAhead * kThreads) {
       T v[kAhead];
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
@@ -264,17 +282,16 @@ __device__ __forceinline__ void scale_chunk(const Tensors<N>& list, const Place&
 }
 
 template <int N>
-__device__ __forceinline__ void scale_chunks(const Tensors<N>& list, float factor) {
+__device__ __forceinline__ void scale_chunks(const Tensors<N>& list, int first, int step,
+                                             int thread, float factor) {
   const int chunks = list.first[list.tensors];
-  if (static_cast<int>(blockIdx.x) >= chunks) return;
-  const int step = static_cast<int>(gridDim.x);
-  for (int c = blockIdx.x + (chunks - 1 - blockIdx.x) / step * step; c >= 0; c -= step) {
+  if (first >= chunks || (factor == 1.f && list.in_place)) return;  // they are as they should be
+  for (int c = first + (chunks - 1 - first) / step * step; c >= 0; c -= step) {
     const Place at = place_of(list, c);
-    if (factor == 1.f && list.in[at.tensor] == list.out[at.tensor]) continue;  // as they are
     switch (list.dtype[at.tensor]) {
-      case ICTC_DTYPE_F32: scale_chunk<float>(list, at, factor); break;
-      case ICTC_DTYPE_BF16: scale_chunk<__nv_bfloat16>(list, at, factor); break;
-      default: scale_chunk<__half>(list, at, factor);
+      case ICTC_DTYPE_F32: scale_chunk<float>(list, at, thread, factor); break;
+      case ICTC_DTYPE_BF16: scale_chunk<__nv_bfloat16>(list, at, thread, factor); break;
+      default: scale_chunk<__half>(list, at, thread, factor);
     }
   }
 }
@@ -285,7 +302,35 @@ __global__ void __launch_bounds__(kThreads)
                  int parts, double max_norm, float* __restrict__ norm) {
   const double n = norm_of<KIND>(partial, parts);
   if (norm != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *norm = static_cast<float>(n);
-  scale_chunks(list, factor_of(n, max_norm));
+  scale_chunks(list, static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x), threadIdx.x,
+               factor_of(n, max_norm));
+}
+
+// All of it in one cluster.
+template <int KIND, int N>
+__global__ void __cluster_dims__(kClusterCtas, 1, 1)
+    __launch_bounds__(kThreads* kClusterGroups)
+        cluster_kernel(const __grid_constant__ Tensors<N> list, bool scale, double max_norm,
+                       float* __restrict__ norm) {
+  __shared__ double sum;
+  constexpr int kStep = kClusterCtas * kClusterGroups;
+  const int thread = threadIdx.x % kThreads;
+  const int first = static_cast<int>(blockIdx.x) * kClusterGroups + threadIdx.x / kThreads;
+  const Running<KIND> own =
+      over_block<KIND, kClusterGroups>(add_chunks<KIND>(list, first, kStep, thread));
+  if (threadIdx.x == 0) sum = own.get();
+  cluster_sync();
+  Running<KIND> all;
+#pragma unroll
+  for (int c = 0; c < kClusterCtas; ++c) {
+    double part;
+    asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(part) : "r"(peer_addr(&sum, c)) : "memory");
+    all.join(part);
+  }
+  const double n = all.norm();
+  if (blockIdx.x == 0 && threadIdx.x == 0) *norm = static_cast<float>(n);
+  if (scale) scale_chunks(list, first, kStep, thread, factor_of(n, max_norm));
+  cluster_sync();  // no CTA leaves while another may read its sum
 }
 
 // ----------------------------------------------------------------------- host side
@@ -307,6 +352,7 @@ template <int N>
 int64_t fill(const Request& q, int64_t at, Tensors<N>& list) {
   list.tensors = 0;
   list.first[0] = 0;
+  list.in_place = q.out != nullptr;
   for (; at < q.tensors && list.tensors < N; ++at) {
     if (q.counts[at] == 0) continue;
     const int64_t size = static_cast<int64_t>(dtype_size(q.dtypes[at]));
@@ -316,6 +362,7 @@ int64_t fill(const Request& q, int64_t at, Tensors<N>& list) {
     const int i = list.tensors++;
     list.in[i] = q.in[at];
     list.out[i] = q.out ? q.out[at] : nullptr;
+    list.in_place = list.in_place && q.out[at] == q.in[at];
     list.count[i] = q.counts[at];
     list.dtype[i] = static_cast<uint8_t>(q.dtypes[at]);
     list.first[i + 1] = list.first[i] + static_cast<int>(chunks);
@@ -334,38 +381,48 @@ unsigned grid_of(const Tensors<N>& list) {
   return static_cast<unsigned>(chunks < 1 ? 1 : chunks < most ? chunks : most);
 }
 
-template <int KIND, int N>
-int run(const Request& q) {
-  static thread_local Tensors<N> list;
-  int parts = 0;
-  int64_t at = 0;
-  bool whole = false;  // one launch holds all tensors
-  do {
-    const int64_t next = fill(q, at, list);
-    whole = at == 0 && next == q.tensors;
-    at = next;
-    const unsigned grid = grid_of(list);
-    partial_kernel<KIND, N><<<grid, kThreads, 0, q.stream>>>(list, q.partial + parts);
-    parts += static_cast<int>(grid);
-  } while (at < q.tensors);
-  if (!q.out) {
-    norm_kernel<KIND><<<1, kThreads, 0, q.stream>>>(q.partial, parts, q.norm);
-  } else {
-    at = 0;
-    do {
-      float* norm = at == 0 ? q.norm : nullptr;
-      at = whole ? q.tensors : fill(q, at, list);
-      scale_kernel<KIND, N><<<grid_of(list), kThreads, 0, q.stream>>>(list, q.partial, parts,
-                                                                     q.max_norm, norm);
-    } while (at < q.tensors);
-  }
+int launched() {
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? ICTC_OK : cuda_fail(e, "gradient norm launch");
 }
 
+template <int KIND, int N>
+int run(const Request& q) {
+  static thread_local Tensors<N> list;
+  int64_t at = fill(q, 0, list);
+  const bool whole = at == q.tensors;  // one launch holds all tensors
+  if (whole && list.first[list.tensors] <= kClusterChunks) {
+    cluster_kernel<KIND, N><<<kClusterCtas, kThreads * kClusterGroups, 0, q.stream>>>(
+        list, q.out != nullptr, q.max_norm, q.norm);
+    return launched();
+  }
+  int parts = 0;
+  for (;;) {
+    const unsigned grid = grid_of(list);
+    partial_kernel<KIND, N><<<grid, kThreads, 0, q.stream>>>(list, q.partial + parts);
+    parts += static_cast<int>(grid);
+    if (at == q.tensors) break;
+    at = fill(q, at, list);
+  }
+  if (!q.out) {
+    norm_kernel<KIND><<<1, kThreads, 0, q.stream>>>(q.partial, parts, q.norm);
+    return launched();
+  }
+  float* norm = q.norm;
+  at = whole ? q.tensors : fill(q, 0, list);
+  for (;;) {
+    scale_kernel<KIND, N><<<grid_of(list), kThreads, 0, q.stream>>>(list, q.partial, parts,
+                                                                   q.max_norm, norm);
+    if (at == q.tensors) return launched();
+    norm = nullptr;
+    at = fill(q, at, list);
+  }
+}
+
 template <int KIND>
 int run_sized(const Request& q) {
-  return q.tensors <= 64 ? run<KIND, 64>(q) : run<KIND, kMostTensors>(q);
+  return q.tensors <= 16 ? run<KIND, 16>(q) : q.tensors <= 128 ? run<KIND, 128>(q)
+                                                              : run<KIND, kMostTensors>(q);
 }
 
 // A tensor has at most 2^36 elements, so that a launch takes at least 255 of them before its

@@ -95,24 +95,23 @@ def _is_largest(norm_type: float) -> bool:
     return kind == math.inf
 
 
-def _is_watched(tensors: list[Tensor]) -> bool:
-    return torch.compiler.is_compiling() or _load().watched(tensors)
-
-
-@torch.no_grad()
 def grad_norm(tensors: Tensor | Iterable[Tensor], norm_type: float = 2.0) -> Tensor:
     """The norm of all tensors together, as if they were one vector: a float32 scalar on
     their device (0 on the CPU for no tensors)."""
-    grads = [tensors] if isinstance(tensors, Tensor) else list(tensors)
+    if not isinstance(tensors, (list, tuple)):
+        tensors = [tensors] if isinstance(tensors, Tensor) else list(tensors)
     largest = _is_largest(norm_type)
-    if not grads:
+    if not tensors:
         return torch.zeros(())
-    if _is_watched(grads):
-        return _norm_op(grads, largest)
-    return _native.grad_norm(grads, largest)
+    norm = None
+    if not torch.compiler.is_compiling():
+        norm = (_native or _load()).grad_norm(tensors, largest)
+    if norm is None:
+        with torch.no_grad():
+            norm = _norm_op(list(tensors), largest)
+    return norm
 
 
-@torch.no_grad()
 def clip_grads(grads: Sequence[Tensor], max_norm: float, norm_type: float = 2.0,
                out: Sequence[Tensor] | None = None) -> tuple[list[Tensor], Tensor]:
     """The gradients times min(1, max_norm / (norm + 1e-6)), and their norm.
@@ -120,8 +119,10 @@ def clip_grads(grads: Sequence[Tensor], max_norm: float, norm_type: float = 2.0,
     ``out``: tensors of the same shapes and types to write (flat buckets' views, say);
     ``out=grads`` scales in place.  Without it new tensors are made.  An output may be its own
     gradient, but share no memory with any other."""
-    grads = list(grads)
-    out = None if out is None else list(out)
+    if not isinstance(grads, (list, tuple)):
+        grads = list(grads)
+    if out is not None and not isinstance(out, (list, tuple)):
+        out = list(out)
     largest, max_norm = _is_largest(norm_type), float(max_norm)
     if not max_norm >= 0:
         raise ValueError(f"max_norm must be >= 0, got {max_norm}")
@@ -129,13 +130,20 @@ def clip_grads(grads: Sequence[Tensor], max_norm: float, norm_type: float = 2.0,
         if out:
             raise ValueError(f"0 gradients and {len(out)} outputs")
         return [], torch.zeros(())
-    if _is_watched(grads):
-        if out is not None and len(out) == len(grads) and all(
-                o is g for o, g in zip(out, grads)):
-            return out, _clip_in_place_op(grads, max_norm, largest)
-        made = [torch.empty_like(g) for g in grads] if out is None else out
-        return made, _clip_op(grads, made, max_norm, largest)
-    return _native.clip_grads(grads, max_norm, largest, out)
+    result = None
+    if not torch.compiler.is_compiling():
+        result = (_native or _load()).clip_grads(grads, max_norm, largest, out)
+    if result is None:
+        result = _clip_watched(list(grads), max_norm, largest, out)
+    return result
+
+
+@torch.no_grad()
+def _clip_watched(grads, max_norm, largest, out):
+    if out is not None and len(out) == len(grads) and all(o is g for o, g in zip(out, grads)):
+        return list(out), _clip_in_place_op(grads, max_norm, largest)
+    out = [torch.empty_like(g) for g in grads] if out is None else list(out)
+    return out, _clip_op(grads, out, max_norm, largest)
 
 
 def clip_grad_norm_(parameters: Tensor | Iterable[Tensor], max_norm: float,
