@@ -76,8 +76,9 @@ SIGNATURES = {
                                               ctypes.POINTER(_size), ctypes.POINTER(_size)]),
     "ictc_o2_gated_linear_forward": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _size,
                                             _i64, _i64, _i64, _i32, _i32, _vp]),
-    "ictc_o2_gated_linear_backward": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _i64] + [_vp] * 4 +
-                                      [_size, _i64, _i64, _i64, _i32, _i32, _vp]),
+    "ictc_o2_gated_linear_keeps": (_i32, [_i64, _i64, _i64, _i32, _i32]),
+    "ictc_o2_gated_linear_backward": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64] +
+                                      [_vp] * 4 + [_size, _i64, _i64, _i64, _i32, _i32, _vp]),
     "ictc_o2_grad_norm_workspace": (_i32, [_i64, _i32, ctypes.POINTER(_size)]),
     "ictc_o2_grad_norm": (_i32, [_vp, _vp, _vp, _i64, _i32, _vp, _vp, _size, _vp]),
     "ictc_o2_clip_grads": (_i32, [_vp, _vp, _vp, _vp, _i64, _i32, ctypes.c_double, _vp, _vp,

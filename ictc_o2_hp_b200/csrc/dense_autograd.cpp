@@ -39,6 +39,7 @@ struct Api {
   decltype(&ictc_o2_gated_linear_workspace) gated_workspace;
   decltype(&ictc_o2_gated_linear_forward) gated_forward;
   decltype(&ictc_o2_gated_linear_backward) gated_backward;
+  decltype(&ictc_o2_gated_linear_keeps) gated_keeps;
 };
 
 Api api{};
@@ -531,49 +532,61 @@ int32_t gated_layout(const Tensor& x, const Tensor& w) {
          (start(x) && row_stride(x) == x.size(1) ? ICTC_LINEAR_PACKED : 0);
 }
 
+// What the training forward keeps beside its inputs.
+enum class Keep { nothing, preact, if_useful };
+
 std::tuple<Tensor, Tensor> gated_forward(const Tensor& x, const Tensor& weight,
-                                         const Tensor& bias_in, int64_t code, bool save) {
+                                         const Tensor& bias_in, int64_t code, Keep keep) {
   const c10::cuda::CUDAGuard guard(x.device());
   const Tensor rows = apart(x), w = apart(weight), bias = packed(bias_in);
   const int64_t m = rows.size(0), k = rows.size(1), n = w.size(0) / 2;
+  const int32_t dtype = code_of(x.scalar_type()), act = static_cast<int32_t>(code);
+  const int32_t layout = gated_layout(rows, w);
   c10::SmallVector<int64_t, 6> shape(x.sizes().begin(), x.sizes().end());
   shape.back() = n;
   const Tensor y = at::empty(shape, x.options());
   Tensor preact;
-  if (save) preact = at::empty({m, 2 * n}, x.options().dtype(at::kFloat));
-  const int32_t dtype = code_of(x.scalar_type()), act = static_cast<int32_t>(code);
+  if (keep == Keep::preact ||
+      (keep == Keep::if_useful && api.gated_keeps(m, k, n, dtype, layout)))
+    preact = at::empty({m, 2 * n}, x.options().dtype(at::kFloat));
   size_t bytes = 0, other = 0;
-  check(api.gated_workspace(m, k, n, dtype, act, gated_layout(rows, w), save,
-                            x.device().index(), &bytes, &other),
+  check(api.gated_workspace(m, k, n, dtype, act, layout, preact.defined(), x.device().index(),
+                            &bytes, &other),
         "gated_linear_workspace");
   const Tensor space = scratch(bytes, x);
-  check(api.gated_forward(rows.data_ptr(), row_stride(rows), w.data_ptr(), row_stride(w), data(bias),
-                          y.data_ptr(), floats(preact), data(space), bytes, m, k, n, dtype, act,
-                          stream_of(x)),
+  check(api.gated_forward(rows.data_ptr(), row_stride(rows), w.data_ptr(), row_stride(w),
+                          data(bias), y.data_ptr(), floats(preact), data(space), bytes, m, k, n,
+                          dtype, act, stream_of(x)),
         "gated_linear_forward");
   return {y, preact};
 }
 
 std::tuple<Tensor, Tensor, Tensor> gated_backward(const Tensor& x, const Tensor& weight,
-                                                  const Tensor& preact, const Tensor& grad,
-                                                  int64_t code, bool need_x, bool need_w,
-                                                  bool need_b) {
+                                                  const Tensor& bias_in, const Tensor& preact,
+                                                  const Tensor& grad, int64_t code, bool need_x,
+                                                  bool need_w, bool need_b) {
   const c10::cuda::CUDAGuard guard(x.device());
-  const Tensor rows = apart(x), w = apart(weight), g = rows_of(grad);
+  const Tensor rows = apart(x), w = apart(weight), bias = packed(bias_in);
+  Tensor g = rows_of(grad);
   const int64_t m = rows.size(0), k = rows.size(1), n = w.size(0) / 2;
+  const int32_t dtype = code_of(x.scalar_type()), act = static_cast<int32_t>(code);
+  const int32_t layout = gated_layout(rows, w);
+  if (!preact.defined() && !api.gated_keeps(m, k, n, dtype, layout) &&
+      (!g.is_contiguous() || reinterpret_cast<uintptr_t>(g.data_ptr()) % 16))
+    g = g.clone(at::MemoryFormat::Contiguous);
   Tensor dx, dw, db;
   if (need_x) dx = at::empty(x.sizes(), x.options());
   if (need_w) dw = at::empty({2 * n, k}, x.options());
   if (need_b) db = at::empty({2 * n}, x.options());
-  const int32_t dtype = code_of(x.scalar_type()), act = static_cast<int32_t>(code);
   size_t bytes = 0, other = 0;
-  check(api.gated_workspace(m, k, n, dtype, act, gated_layout(rows, w), true,
-                            x.device().index(), &other, &bytes),
+  check(api.gated_workspace(m, k, n, dtype, act, layout, preact.defined(), x.device().index(),
+                            &other, &bytes),
         "gated_linear_workspace");
   const Tensor space = scratch(bytes, x);
   check(api.gated_backward(rows.data_ptr(), row_stride(rows), w.data_ptr(), row_stride(w),
-                           floats(preact), g.data_ptr(), g.stride(0), data(dx), data(dw),
-                           data(db), data(space), bytes, m, k, n, dtype, act, stream_of(x)),
+                           data(bias), floats(preact), g.data_ptr(), g.stride(0), data(dx),
+                           data(dw), data(db), data(space), bytes, m, k, n, dtype, act,
+                           stream_of(x)),
         "gated_linear_backward");
   return {dx, dw, db};
 }
@@ -594,7 +607,7 @@ class GatedLinearFunction : public torch::autograd::Function<GatedLinearFunction
                         const std::optional<Tensor>& bias_in, int64_t code) {
     at::AutoDispatchBelowADInplaceOrView below;
     const Tensor bias = wanted(bias_in);
-    auto [y, preact] = gated_forward(x, weight, bias, code, true);
+    auto [y, preact] = gated_forward(x, weight, bias, code, Keep::if_useful);
     ctx->save_for_backward({x, weight, bias, preact});
     ctx->saved_data["code"] = code;
     return y;
@@ -612,16 +625,24 @@ class GatedLinearFunction : public torch::autograd::Function<GatedLinearFunction
     if (!at::GradMode::is_enabled()) {
       if (watched({&grad, &x, &weight})) {
         const auto [dx, dw, db] = through_dispatcher<std::tuple<Tensor, Tensor, Tensor>>(
-            ops.gated_backward, x, weight, preact, grad, code);
+            ops.gated_backward, x, weight, given(saved[2]),
+            preact.defined() ? preact : at::empty({0}, x.options().dtype(at::kFloat)), grad, code);
         return {nx ? dx : Tensor(), nw ? dw : Tensor(), nb ? db : Tensor(), Tensor()};
       }
-      auto [dx, dw, db] = gated_backward(x, weight, preact, grad, code, nx, nw, nb);
+      auto [dx, dw, db] = gated_backward(x, weight, saved[2], preact, grad, code, nx, nw, nb);
       return {dx, dw, db, Tensor()};
     }
     // second derivatives: as in the linear layer
     const Tensor rows = rows_of(x), g = rows_of(grad).to(at::kFloat);
     const Tensor p = linear(rows, weight, given(saved[2]), std::nullopt, ICTC_ACT_NONE);
-    const auto halves = ValueOf::apply(p.to(at::kFloat), preact).chunk(2, 1);
+    const Tensor exact = preact.defined() || rows.size(0) == 0
+                             ? preact
+                             : std::get<1>(gated_forward(rows.detach(), weight.detach(),
+                                                         saved[2].defined() ? saved[2].detach()
+                                                                            : Tensor(),
+                                                         code, Keep::preact));
+    const Tensor wide_p = p.to(at::kFloat);
+    const auto halves = (exact.defined() ? ValueOf::apply(wide_p, exact) : wide_p).chunk(2, 1);
     const Tensor slope = code == ICTC_ACT_NONE ? halves[1] : halves[1] * slope_formula(halves[0], code);
     const Tensor wide = at::cat({g * slope, g * activation_formula(halves[0], code)}, 1);
     const Tensor d = wide.to(x.scalar_type());
@@ -643,11 +664,15 @@ Tensor gated_linear(const Tensor& x, const Tensor& weight, const std::optional<T
   check_gated(x, weight, bias, code);
   check_tangents("gated_linear", {&x, &weight, &bias});
   const bool grad = any_grad({&x, &weight, &bias});
-  if (watched({&x, &weight, &bias}))
+  if (watched({&x, &weight, &bias})) {
+    // by the sizes alone: there may be no memory whose layout could be asked
+    const bool keep = grad && api.gated_keeps(x.numel() / x.size(-1), x.size(-1), weight.size(0) / 2,
+                                              code_of(x.scalar_type()), ICTC_LINEAR_PACKED);
     return std::get<0>(through_dispatcher<std::tuple<Tensor, Tensor>>(ops.gated_forward, x, weight,
-                                                                      bias, code, grad));
+                                                                      given(bias), code, keep));
+  }
   if (grad) return GatedLinearFunction::apply(x, weight, given(bias), code);
-  return std::get<0>(gated_forward(x, weight, bias, code, false));
+  return std::get<0>(gated_forward(x, weight, bias, code, Keep::nothing));
 }
 
 // ---------------------------------------------- raw directions, for the custom operators
@@ -688,15 +713,18 @@ std::tuple<Tensor, Tensor> gated_forward_op(const Tensor& x, const Tensor& weigh
                                             const std::optional<Tensor>& bias, int64_t code,
                                             bool save) {
   check_gated(x, weight, wanted(bias), code);
-  auto [y, preact] = gated_forward(x, weight, wanted(bias), code, save);
+  auto [y, preact] =
+      gated_forward(x, weight, wanted(bias), code, save ? Keep::preact : Keep::nothing);
   if (!save) preact = at::empty({0}, x.options().dtype(at::kFloat));
   return {y, preact};
 }
 
 std::tuple<Tensor, Tensor, Tensor> gated_backward_op(const Tensor& x, const Tensor& weight,
+                                                     const std::optional<Tensor>& bias,
                                                      const Tensor& preact, const Tensor& grad,
                                                      int64_t code) {
-  return gated_backward(x, weight, preact, grad, code, true, true, true);
+  return gated_backward(x, weight, wanted(bias), preact.dim() == 2 ? preact : Tensor(), grad, code,
+                        true, true, true);
 }
 
 // The custom operators, held for the life of the process.
@@ -709,7 +737,7 @@ void bind_operators(py::object norm_fwd, py::object norm_bwd, py::object linear_
 // Entry points of the loaded kernel library, by address.
 void bind(uintptr_t last_error, uintptr_t norm_fwd, uintptr_t norm_ws, uintptr_t norm_bwd,
           uintptr_t linear_ws, uintptr_t linear_fwd, uintptr_t linear_bwd, uintptr_t gated_ws,
-          uintptr_t gated_fwd, uintptr_t gated_bwd) {
+          uintptr_t gated_fwd, uintptr_t gated_bwd, uintptr_t gated_keeps) {
   const auto set = [](auto& fn, uintptr_t at) { fn = reinterpret_cast<std::decay_t<decltype(fn)>>(at); };
   set(api.last_error, last_error);
   set(api.norm_forward, norm_fwd);
@@ -721,6 +749,7 @@ void bind(uintptr_t last_error, uintptr_t norm_fwd, uintptr_t norm_ws, uintptr_t
   set(api.gated_workspace, gated_ws);
   set(api.gated_forward, gated_fwd);
   set(api.gated_backward, gated_bwd);
+  set(api.gated_keeps, gated_keeps);
 }
 
 }  // namespace

@@ -10,11 +10,14 @@
 //
 // Which kernel a forward takes:
 //   up to 4 rows, aligned or small   FMAs, W read once (few_kernel)
+//   up to 64 inputs and outputs,     one kernel per direction (dense_gated_narrow.cuh), which
+//   contiguous 16-byte rows          keeps no p: the backward computes it again
 //   16-bit, aligned rows             SM pairs fed by TMA (dense_pair.cuh, GATED)
 //   float32, aligned rows            cut on the way in (dense_cut.cuh, GATED)
 //   unaligned rows                   large products are copied to aligned rows first; for
 //                                    small ones the linear layer leaves p in memory, and
 //                                    gate_kernel makes y of it
+// The backward forms D in a pass over p and g (gated_slope_kernel) but for the narrow layers.
 // A tile of these kernels has the sums of both halves for the same columns of y, so that the
 // epilogue needs nothing from another tile, and p is written only where a backward wants it.
 #include <cuda_runtime.h>
@@ -25,6 +28,7 @@
 #include "common.cuh"
 #include "dense_cut.cuh"
 #include "dense_epilogue.cuh"
+#include "dense_gated_narrow.cuh"
 #include "dense_pair.cuh"
 #include "dense_plan.cuh"
 #include "dense_types.cuh"
@@ -227,7 +231,14 @@ int32_t layout_of(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_
   return flags;
 }
 
-enum class Way { few, pair, cut, general };
+// Layers whose backward computes p again at no cost of a pass (their g is contiguous too).
+bool is_narrow(int64_t m, int64_t n, int64_t k, int dtype, int32_t layout) {
+  const int64_t full = static_cast<int64_t>(16 / dtype_size(dtype));
+  return (layout & ICTC_LINEAR_PACKED) && n <= kNarrow && k <= kNarrow && n % full == 0 &&
+         k % full == 0 && m <= (1ll << 36);
+}
+
+enum class Way { few, narrow, pair, cut, general };
 
 // Byte offsets of the workspace's parts, and its size.
 struct GatedPlan {
@@ -237,7 +248,7 @@ struct GatedPlan {
   Split cut;
   size_t x, w, partial;                  // forward
   size_t p, y;                           // forward, general
-  size_t d, columns;                     // backward
+  size_t d, columns, forward;            // backward
   size_t product, product_bytes, total;  // the linear layer's
 };
 
@@ -262,6 +273,10 @@ int plan_forward(int64_t m, int64_t n, int64_t k, int dtype, int32_t layout, boo
   if (m <= kFewRows && ((rows_aligned && k % static_cast<int64_t>(16 / size) == 0) ||
                         2 * n * k <= (1 << 18))) {
     b->way = Way::few;
+    return ICTC_OK;
+  }
+  if (!keep && is_narrow(m, n, k, dtype, layout)) {
+    b->way = Way::narrow;
     return ICTC_OK;
   }
   b->align = !rows_aligned && worth_aligning(m, 2 * n, k);
@@ -303,10 +318,27 @@ int plan_forward(int64_t m, int64_t n, int64_t k, int dtype, int32_t layout, boo
   return ICTC_OK;
 }
 
-int plan_backward(int64_t m, int64_t n, int64_t k, int dtype, int32_t layout, int device,
+// keep: the forward kept p.  Otherwise it is computed again, by the forward kernels where the
+// layer is not narrow.
+int plan_backward(int64_t m, int64_t n, int64_t k, int dtype, int32_t layout, bool keep, int device,
                   GatedPlan* b) {
   const size_t size = dtype_size(dtype);
   Layout space;
+  if (!keep && is_narrow(m, n, k, dtype, layout)) {
+    b->way = Way::narrow;
+    b->partial = space.take(static_cast<size_t>(sm_count(device)) * 2 * n * (k + 1) * sizeof(float));
+    b->total = space.at;
+    return ICTC_OK;
+  }
+  if (!keep) {
+    GatedPlan forward{};
+    const int st = plan_forward(m, n, k, dtype, layout, true, device, &forward);
+    if (st != ICTC_OK) return st;
+    b->p = space.take(static_cast<size_t>(m) * 2 * n * sizeof(float));
+    b->y = space.take(static_cast<size_t>(m) * n * size);
+    b->forward = space.take(forward.total);
+  }
+  b->way = Way::general;
   const int64_t pitch = aligned_pitch(2 * n, size);
   b->d = space.take(static_cast<size_t>(m) * pitch * size);
   b->columns =
@@ -425,6 +457,74 @@ int launch_cut(const OperandMaps& maps, const ProductArgs& p, cudaStream_t strea
 }
 
 template <typename T>
+GatedNarrowArgs narrow_args(const T* x, const T* w, int64_t ldw, const void* bias, int64_t m,
+                            int64_t n, int64_t k) {
+  GatedNarrowArgs p{};
+  p.x = x; p.w = w; p.bias = bias;
+  p.m = m; p.ldw = ldw;
+  p.n = static_cast<int>(n); p.k = static_cast<int>(k);
+  p.tiles = static_cast<int>(ceil_div(m, kNarrowTile));
+  return p;
+}
+
+template <typename T>
+int run_narrow_forward(const T* x, const T* w, int64_t ldw, Epilogue e, int64_t m, int64_t n,
+                       int64_t k, cudaStream_t stream) {
+  GatedNarrowArgs p = narrow_args(x, w, ldw, e.bias, m, n, k);
+  e.vec = aligned(e.out, 16);
+  p.e = e;
+  const int sms = sm_count(current_device());
+  int st = ICTC_OK;
+  for_activation(e.activation, [&](auto act) {
+    const auto kernel = gated_narrow_forward_kernel<T, act.value>;
+    st = allow_smem(reinterpret_cast<const void*>(kernel), kGatedForwardSmem<T>);
+    if (st == ICTC_OK)
+      kernel<<<p.tiles < sms ? p.tiles : sms, kGatedThreads, kGatedForwardSmem<T>, stream>>>(p);
+  });
+  if (st != ICTC_OK) return st;
+  const cudaError_t err = cudaGetLastError();
+  return err == cudaSuccess ? ICTC_OK : cuda_fail(err, "narrow gated forward launch");
+}
+
+template <typename T>
+int run_narrow_backward(const T* x, const T* w, int64_t ldw, const void* bias, const T* g, T* dx,
+                        T* dw, T* db, float* partial, int64_t m, int64_t n, int64_t k,
+                        int activation, cudaStream_t stream) {
+  GatedNarrowArgs p = narrow_args(x, w, ldw, bias, m, n, k);
+  p.g = g;
+  p.partial = dw || db ? partial : nullptr;
+  p.e.out = dx;
+  p.e.vec = aligned(dx, 16);
+  const int sms = sm_count(current_device());
+  const int grid = p.tiles < sms ? p.tiles : sms;
+  int st = ICTC_OK;
+  for_activation(activation, [&](auto act) {
+    const auto kernel = gated_narrow_backward_kernel<T, act.value>;
+    static const bool shares_fit = [&] {
+      cudaFuncAttributes a{};
+      return cudaFuncGetAttributes(&a, kernel) == cudaSuccess &&
+             a.numRegs >= kGatedLaunchRegisters;
+    }();
+    if (!shares_fit) {
+      st = fail(ICTC_ERR_UNSUPPORTED, "gated linear: built with fewer than %d registers a thread",
+                kGatedLaunchRegisters);
+      return;
+    }
+    st = allow_smem(reinterpret_cast<const void*>(kernel), kGatedBackwardSmem<T>);
+    if (st == ICTC_OK) kernel<<<grid, kGatedThreads, kGatedBackwardSmem<T>, stream>>>(p);
+  });
+  if (st != ICTC_OK) return st;
+  cudaError_t err = cudaGetLastError();
+  if (err != cudaSuccess) return cuda_fail(err, "narrow gated backward launch");
+  if (!p.partial) return ICTC_OK;
+  const int wide = 2 * p.n, nk = wide * p.k;
+  narrow_total_kernel<T><<<static_cast<unsigned>(ceil_div(nk + wide, 32)), dim3(32, kColumnLanes),
+                           0, stream>>>(partial, dw, db, grid, nk, wide);
+  err = cudaGetLastError();
+  return err == cudaSuccess ? ICTC_OK : cuda_fail(err, "narrow gated column sum launch");
+}
+
+template <typename T>
 int run_tiles(const T* x, int64_t ldx, const T* w, int64_t ldw, Epilogue e, unsigned char* ws,
               const GatedPlan& plan, int64_t m, int64_t n, int64_t k, cudaStream_t stream) {
   int st = ICTC_OK;
@@ -483,6 +583,7 @@ int run_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const Ep
       return run_few<T, kFull>(xt, ldx, wt, ldw, e, m, n, k, stream);
     return run_few<T, 1>(xt, ldx, wt, ldw, e, m, n, k, stream);
   }
+  if (plan.way == Way::narrow) return run_narrow_forward(xt, wt, ldw, e, m, n, k, stream);
   if (plan.way != Way::general) return run_tiles(xt, ldx, wt, ldw, e, ws, plan, m, n, k, stream);
   float* p = e.preact ? e.preact : reinterpret_cast<float*>(ws + plan.p);
   const bool wide = sizeof(T) == 4;
@@ -494,18 +595,47 @@ int run_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const Ep
   return run_gate<T>(p, 1, nullptr, nullptr, static_cast<T*>(e.out), m, n, e.activation, stream);
 }
 
+struct Backward {
+  const void *x, *w, *bias;
+  int64_t ldx, ldw;
+  const float* preact;
+  const void* g;
+  int64_t ldg;
+  void *dx, *dw, *db;
+};
+
 template <typename T>
-int run_backward(const void* x, int64_t ldx, const void* w, int64_t ldw, const float* p,
-                 const void* g, int64_t ldg, void* dx, void* dw, void* db, unsigned char* ws,
-                 const GatedPlan& plan, int64_t m, int64_t n, int64_t k, int dtype, int activation,
-                 cudaStream_t stream) {
-  T* d = dx || dw ? reinterpret_cast<T*>(ws + plan.d) : nullptr;
+int run_backward(const Backward& q, unsigned char* ws, const GatedPlan& plan, int64_t m, int64_t n,
+                 int64_t k, int dtype, int activation, int32_t layout, cudaStream_t stream) {
+  const T* g = static_cast<const T*>(q.g);
+  T* db = static_cast<T*>(q.db);
+  if (plan.way == Way::narrow)
+    return run_narrow_backward(static_cast<const T*>(q.x), static_cast<const T*>(q.w), q.ldw, q.bias,
+                               g, static_cast<T*>(q.dx), static_cast<T*>(q.dw), db,
+                               reinterpret_cast<float*>(ws + plan.partial), m, n, k, activation,
+                               stream);
+  const float* p = q.preact;
+  int st = ICTC_OK;
+  if (!p) {
+    GatedPlan forward{};
+    st = plan_forward(m, n, k, dtype, layout, true, current_device(), &forward);
+    if (st != ICTC_OK) return st;
+    Epilogue e{};
+    e.bias = q.bias;
+    e.preact = reinterpret_cast<float*>(ws + plan.p);
+    e.out = ws + plan.y;
+    e.activation = activation;
+    p = e.preact;
+    st = run_forward<T>(q.x, q.ldx, q.w, q.ldw, e, ws + plan.forward, forward, m, n, k, dtype,
+                        stream);
+    if (st != ICTC_OK) return st;
+  }
+  T* d = q.dx || q.dw ? reinterpret_cast<T*>(ws + plan.d) : nullptr;
   const int64_t pitch = aligned_pitch(2 * n, sizeof(T));
-  const int st = run_slope<T>(static_cast<const T*>(g), ldg, p, d, pitch,
-                              reinterpret_cast<float*>(ws + plan.columns), static_cast<T*>(db), m,
-                              n, activation, stream);
+  st = run_slope<T>(g, q.ldg, p, d, pitch, reinterpret_cast<float*>(ws + plan.columns), db, m, n,
+                    activation, stream);
   if (st != ICTC_OK || !d) return st;
-  return ictc_o2_linear_backward(x, ldx, w, ldw, nullptr, d, pitch, dx, dw, nullptr,
+  return ictc_o2_linear_backward(q.x, q.ldx, q.w, q.ldw, nullptr, d, pitch, q.dx, q.dw, nullptr,
                                  ws + plan.product, plan.product_bytes, m, k, 2 * n, dtype,
                                  ICTC_ACT_NONE, stream);
 }
@@ -554,7 +684,8 @@ extern "C" int32_t ictc_o2_gated_linear_workspace(int64_t rows, int64_t in, int6
   if (rows == 0) return ICTC_OK;
   GatedPlan forward{}, backward{};
   st = plan_forward(rows, hidden, in, dtype, layout, keep != 0, device, &forward);
-  if (st == ICTC_OK) st = plan_backward(rows, hidden, in, dtype, layout, device, &backward);
+  if (st == ICTC_OK)
+    st = plan_backward(rows, hidden, in, dtype, layout, keep != 0, device, &backward);
   *forward_bytes = forward.total;
   *backward_bytes = backward.total;
   return st;
@@ -595,7 +726,7 @@ extern "C" int32_t ictc_o2_gated_linear_forward(const void* x, int64_t x_stride,
 }
 
 extern "C" int32_t ictc_o2_gated_linear_backward(
-    const void* x, int64_t x_stride, const void* weight, int64_t weight_stride,
+    const void* x, int64_t x_stride, const void* weight, int64_t weight_stride, const void* bias,
     const float* preact, const void* grad_output, int64_t grad_stride, void* grad_x,
     void* grad_weight, void* grad_bias, void* workspace, size_t workspace_bytes, int64_t rows,
     int64_t in, int64_t hidden, int32_t dtype, int32_t activation, void* stream) {
@@ -607,23 +738,36 @@ extern "C" int32_t ictc_o2_gated_linear_backward(
                                    grad_weight, grad_bias, nullptr, 0, 0, in, 2 * hidden, dtype,
                                    ICTC_ACT_NONE, stream);
   if (!grad_x && !grad_weight && !grad_bias) return ICTC_OK;
-  if (!x || !weight || !grad_output || !preact) return fail(ICTC_ERR_INVALID, "null pointer");
-  if (rows == 1) x_stride = in;
+  if (!x || !weight || !grad_output) return fail(ICTC_ERR_INVALID, "null pointer");
+  if (rows == 1) {
+    x_stride = in;
+    grad_stride = hidden;
+  }
   if (x_stride < in || weight_stride < in)
     return fail(ICTC_ERR_INVALID, "rows of x and weight must not overlap");
   if (grad_stride < 0) return fail(ICTC_ERR_INVALID, "negative row stride");
-  const int32_t layout = layout_of(x, x_stride, weight, weight_stride, in, dtype_size(dtype));
+  const size_t size = dtype_size(dtype);
+  const int32_t layout = layout_of(x, x_stride, weight, weight_stride, in, size);
+  if (!preact && is_narrow(rows, hidden, in, dtype, layout) &&
+      (grad_stride != hidden || !aligned(grad_output, 16)))
+    return fail(ICTC_ERR_INVALID,
+                "without preact a narrow layer needs a contiguous, 16-byte aligned grad_output");
   GatedPlan plan{};
-  st = plan_backward(rows, hidden, in, dtype, layout, current_device(), &plan);
+  st = plan_backward(rows, hidden, in, dtype, layout, preact != nullptr, current_device(), &plan);
   if (st == ICTC_OK) st = check_workspace(workspace, workspace_bytes, plan.total);
   if (st != ICTC_OK) return st;
+  const Backward q{x, weight, bias, x_stride, weight_stride, preact, grad_output,
+                   grad_stride, grad_x, grad_weight, grad_bias};
   unsigned char* ws = static_cast<unsigned char*>(workspace);
-#define ICTC_GATED_BACKWARD(T)                                                              \
-  return run_backward<T>(x, x_stride, weight, weight_stride, preact, grad_output, grad_stride, \
-                         grad_x, grad_weight, grad_bias, ws, plan, rows, hidden, in, dtype, \
-                         activation, s)
+#define ICTC_GATED_BACKWARD(T) \
+  return run_backward<T>(q, ws, plan, rows, hidden, in, dtype, activation, layout, s)
   if (dtype == ICTC_DTYPE_F32) ICTC_GATED_BACKWARD(float);
   if (dtype == ICTC_DTYPE_BF16) ICTC_GATED_BACKWARD(__nv_bfloat16);
   ICTC_GATED_BACKWARD(__half);
 #undef ICTC_GATED_BACKWARD
+}
+
+extern "C" int32_t ictc_o2_gated_linear_keeps(int64_t rows, int64_t in, int64_t hidden,
+                                              int32_t dtype, int32_t layout) {
+  return known_dtype(dtype) && !is_narrow(rows, hidden, in, dtype, layout);
 }

@@ -57,7 +57,7 @@ def _load():
                  "ictc_o2_layer_norm_backward", "ictc_o2_linear_workspace",
                  "ictc_o2_linear_forward", "ictc_o2_linear_backward",
                  "ictc_o2_gated_linear_workspace", "ictc_o2_gated_linear_forward",
-                 "ictc_o2_gated_linear_backward")
+                 "ictc_o2_gated_linear_backward", "ictc_o2_gated_linear_keeps")
         module.bind(*(ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in names))
         module.bind_operators(_norm_op, _norm_grad_op, _linear_op, _linear_grad_op, _gated_op,
                               _gated_grad_op)
@@ -167,26 +167,26 @@ def _gated_op_fake(x, weight, bias, code, save):
 
 
 @torch.library.custom_op(f"{NAMESPACE}::gated_linear_backward", mutates_args=())
-def _gated_grad_op(x: Tensor, weight: Tensor, preact: Tensor, grad: Tensor, code: int
-                   ) -> tuple[Tensor, Tensor, Tensor]:
-    return _load().gated_backward(x, weight, preact, grad, code)
+def _gated_grad_op(x: Tensor, weight: Tensor, bias: Tensor | None, preact: Tensor, grad: Tensor,
+                   code: int) -> tuple[Tensor, Tensor, Tensor]:
+    return _load().gated_backward(x, weight, bias, preact, grad, code)
 
 
 @_gated_grad_op.register_fake
-def _gated_grad_op_fake(x, weight, preact, grad, code):
+def _gated_grad_op_fake(x, weight, bias, preact, grad, code):
     return _linear_grad_op_fake(x, weight, preact, grad, code)
 
 
 def _gated_op_setup(ctx, inputs, output):
-    x, weight, _, code, _ = inputs
-    ctx.save_for_backward(x, weight, output[1])
+    x, weight, bias, code, _ = inputs
+    ctx.save_for_backward(x, weight, bias, output[1])
     ctx.code = code
 
 
 def _gated_op_backward(ctx, grad, _preact_grad):
-    x, weight, preact = ctx.saved_tensors
+    x, weight, bias, preact = ctx.saved_tensors
     need = ctx.needs_input_grad
-    dx, dw, db = _gated_grad_op(x, weight, preact, grad, ctx.code)
+    dx, dw, db = _gated_grad_op(x, weight, bias, preact, grad, ctx.code)
     return (dx if need[0] else None, dw if need[1] else None, db if need[2] else None, None, None)
 
 
@@ -247,6 +247,9 @@ def gated_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None,
         x, weight, bias = _cast_mixed([x, weight, bias])
         save = torch.is_grad_enabled() and any(
             t is not None and t.requires_grad for t in (x, weight, bias))
+        if save and weight.dim() == 2:  # as ictc_o2_gated_linear_keeps, by the sizes
+            sizes, block = (weight.shape[0] // 2, weight.shape[1]), 16 // x.element_size()
+            save = any(s > 64 or s % block for s in sizes)
         return _gated_op(x, weight, bias, code, save)[0]
     return (_native or _load()).gated_linear(x, weight, bias, code)
 

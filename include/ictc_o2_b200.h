@@ -373,13 +373,20 @@ ICTC_API int32_t ictc_o2_linear_backward(
 
 /* The gated linear layer: (pg | pu) = x weight^T + bias, y = act(pg) pu with weight
  * [2 hidden, in] and bias [2 hidden] or null (the gate's rows first), y [rows, hidden].
- * preact [rows, 2 hidden] receives pg and pu in float32 for the backward, or is null.
- * `keep` of the workspace query: whether the forward is given preact.  The layout flags
- * are those of x and weight. */
+ * Rows of x and of weight do not overlap.  preact [rows, 2 hidden] receives pg and pu in
+ * float32 for the backward, or is null: the backward then computes them again.
+ * `keep` of the workspace query: whether both directions are given preact.  The layout
+ * flags are those of x and weight. */
 ICTC_API int32_t ictc_o2_gated_linear_workspace(int64_t rows, int64_t in, int64_t hidden,
                                                 int32_t dtype, int32_t activation,
                                                 int32_t layout, int32_t keep, int32_t device,
                                                 size_t* forward_bytes, size_t* backward_bytes);
+
+/* Whether preact saves the backward anything: 0 for contiguous layers of at most 64 inputs
+ * and 64 outputs in whole 16-byte blocks, whose backward is faster without it (and needs a
+ * contiguous, 16-byte aligned grad_output then), 1 otherwise. */
+ICTC_API int32_t ictc_o2_gated_linear_keeps(int64_t rows, int64_t in, int64_t hidden,
+                                            int32_t dtype, int32_t layout);
 
 ICTC_API int32_t ictc_o2_gated_linear_forward(const void* x, int64_t x_stride,
                                               const void* weight, int64_t weight_stride,
@@ -390,9 +397,10 @@ ICTC_API int32_t ictc_o2_gated_linear_forward(const void* x, int64_t x_stride,
 
 /* D = (grad_output pu act'(pg) | grad_output act(pg)), rounded to the operand type;
  * grad_x = D weight, grad_weight = D^T x, grad_bias = sum of D's rows before rounding.
- * Any output may be null.  rows = 0 clears grad_weight and grad_bias. */
+ * Any output may be null.  bias is read where preact is null.  rows = 0 clears grad_weight
+ * and grad_bias. */
 ICTC_API int32_t ictc_o2_gated_linear_backward(
-    const void* x, int64_t x_stride, const void* weight, int64_t weight_stride,
+    const void* x, int64_t x_stride, const void* weight, int64_t weight_stride, const void* bias,
     const float* preact, const void* grad_output, int64_t grad_stride, void* grad_x,
     void* grad_weight, void* grad_bias, void* workspace, size_t workspace_bytes, int64_t rows,
     int64_t in, int64_t hidden, int32_t dtype, int32_t activation, void* stream);

@@ -67,7 +67,7 @@ def test_status_codes():
 
     def backward(preact=some, g=some, x=some, w=some, dw=some, space=some, size=1 << 30, rows=300,
                  stride=80):
-        return lib.ictc_o2_gated_linear_backward(x, 200, w, 200, preact, g, stride, some, dw, some,
+        return lib.ictc_o2_gated_linear_backward(x, 200, w, 200, None, preact, g, stride, some, dw, some,
                                                  space, size, rows, 200, 80, 0, 2, None)
 
     for bad in ({"g": None}, {"x": None}, {"w": None}, {"rows": -1}, {"stride": -1}):

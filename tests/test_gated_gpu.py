@@ -85,6 +85,7 @@ SHAPES = [
     (2053, 211, 333), (4097, 702, 6), (5000, 1536, 8), (4500, 3, 130), (4099, 8, 520), (2, 4096, 40),
     (4, 8192, 513), (1, 1000, 2048), (700, 1024, 768), (4096, 256, 256), (16, 4096, 520),
     (20000, 64, 64), (33, 8200, 24), (40000, 24, 8), (260, 96, 4100), (9001, 64, 48), (64, 24, 3000),
+    (777, 8, 8), (130, 16, 24), (5000, 56, 40), (1, 40, 24), (300, 48, 16), (641, 4, 12),
 ]
 
 
@@ -173,6 +174,40 @@ def test_partial_gradients(shape, dtype, cuda_device):
         leaves = [t.detach().requires_grad_(i == j) for j, t in enumerate((x, w, b))]
         y = dense.gated_linear(*leaves, "gelu")
         assert torch.equal(torch.autograd.grad(y, leaves[i], g)[0], full[i])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(3, 40, 24), (700, 64, 64), (700, 24, 56), (1000, 63, 61),
+                                   (300, 264, 200)])
+def test_recomputed_p(shape, dtype, cuda_device):
+    """A backward that is given no p computes it again, whichever kernels the layer takes; a
+    gradient off the boundaries is copied first."""
+    from ictc_o2_hp_b200 import dense
+    x, w, b, g = operands(*shape, dtype, cuda_device, 65)
+    native, code = dense._load(), dense.ACTIVATIONS["silu"]
+    y, p = native.gated_forward(x, w, b, code, True)
+    assert p.shape == (shape[0], 2 * shape[2]) and p.dtype == torch.float32
+    none = torch.empty(0, device=cuda_device)
+    odd = rand((shape[0] * shape[2] + 1,), dtype, cuda_device, 66)[1:].view(*g.shape)
+    for grad in (g, odd, g[:1].expand_as(g)):
+        for kept in (p, none):
+            grads = native.gated_backward(x, w, b, kept, grad, code)
+            check_gated(x, w, b, "silu", grad, y, grads, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(300, 64, 64), (700, 24, 40), (129, 16, 8)])
+def test_infinite_bias(shape, dtype, cuda_device):
+    """Rows past the last of a tile have a bias too: it must not reach the sums."""
+    m, k, n = shape
+    x, w, b, g = operands(m, k, n, dtype, cuda_device, 67)
+    base = step(x, w, b, "none", g)
+    b[n + 2] = math.inf
+    y, (dx, dw, db) = step(x, w, b, "none", g)
+    keep = torch.arange(2 * n, device=cuda_device) != 2
+    assert torch.equal(y[:, keep[:n]], base[0][:, keep[:n]]) and not y[:, 2].isfinite().any()
+    assert torch.equal(dw[keep], base[1][1][keep]) and torch.equal(db[keep], base[1][2][keep])
+    assert not dw[2].isfinite().any() and not dx.isfinite().any()
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
