@@ -83,10 +83,9 @@ int encode3(PFN_cuTensorMapEncodeTiled_v12000 fn, CUtensorMap* map, const float*
   return r == CUDA_SUCCESS ? 0 : -1;
 }
 
-}  // namespace
-
-int encode_matrix_map(const void* base, int size, bool bf16, int64_t inner, int64_t outer,
-                      int64_t stride, int box_inner, int box_outer, CUtensorMap* map) {
+int encode_matrix(const void* base, int size, bool bf16, int64_t inner, int64_t outer,
+                  int64_t stride, int box_inner, int box_outer, CUtensorMapSwizzle swizzle,
+                  CUtensorMap* map) {
   PFN_cuTensorMapEncodeTiled_v12000 fn = tensor_map_encoder();
   if (fn == nullptr || inner < 1 || outer < 1 || stride % 16 != 0 || stride >= (1ll << 40) ||
       inner >= (1ll << 31) || outer >= (1ll << 31) ||
@@ -102,10 +101,22 @@ int encode_matrix_map(const void* base, int size, bool bf16, int64_t inner, int6
          size == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                    : bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
          2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-         size == 4 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
-         CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+         swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? 0 : -1;
+}
+
+}  // namespace
+
+int encode_matrix_map(const void* base, int size, bool bf16, int64_t inner, int64_t outer,
+                      int64_t stride, int box_inner, int box_outer, CUtensorMap* map) {
+  return encode_matrix(base, size, bf16, inner, outer, stride, box_inner, box_outer,
+                       size == 4 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, map);
+}
+
+int encode_swizzled_map(const void* base, int size, bool bf16, int64_t inner, int64_t outer,
+                        int64_t stride, int box_outer, CUtensorMap* map) {
+  return encode_matrix(base, size, bf16, inner, outer, stride, 128 / size, box_outer,
+                       CU_TENSOR_MAP_SWIZZLE_128B, map);
 }
 
 int encode_row_tile_maps(const float* base, int64_t rows, int C, int M, bool full, bool cm,

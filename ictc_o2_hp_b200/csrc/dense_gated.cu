@@ -235,7 +235,7 @@ int32_t layout_of(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_
 bool is_narrow(int64_t m, int64_t n, int64_t k, int dtype, int32_t layout) {
   const int64_t full = static_cast<int64_t>(16 / dtype_size(dtype));
   return (layout & ICTC_LINEAR_PACKED) && n <= kNarrow && k <= kNarrow && n % full == 0 &&
-         k % full == 0 && m <= (1ll << 36);
+         k % full == 0 && m <= (1ll << 30);
 }
 
 enum class Way { few, narrow, pair, cut, general };
@@ -494,7 +494,15 @@ int run_narrow_backward(const T* x, const T* w, int64_t ldw, const void* bias, c
   p.g = g;
   p.partial = dw || db ? partial : nullptr;
   p.e.out = dx;
-  p.e.vec = aligned(dx, 16);
+  GatedNarrowMaps maps{};
+  constexpr int kSize = sizeof(T);
+  constexpr bool kBf16 = std::is_same_v<T, __nv_bfloat16>;
+  const auto encode = [&](const void* base, int64_t width, CUtensorMap* map) {
+    return encode_swizzled_map(base, kSize, kBf16, width, m, width * kSize, kNarrowTile, map);
+  };
+  if (encode(x, k, &maps.x) != 0 || encode(g, n, &maps.g) != 0 ||
+      (dx && encode(dx, k, &maps.dx) != 0))
+    return fail(ICTC_ERR_UNSUPPORTED, "gated linear: no tensor map for these operands");
   const int sms = sm_count(current_device());
   const int grid = p.tiles < sms ? p.tiles : sms;
   int st = ICTC_OK;
@@ -503,15 +511,15 @@ int run_narrow_backward(const T* x, const T* w, int64_t ldw, const void* bias, c
     static const bool shares_fit = [&] {
       cudaFuncAttributes a{};
       return cudaFuncGetAttributes(&a, kernel) == cudaSuccess &&
-             a.numRegs >= kGatedLaunchRegisters;
+             a.numRegs >= kBackLaunchRegisters;
     }();
     if (!shares_fit) {
       st = fail(ICTC_ERR_UNSUPPORTED, "gated linear: built with fewer than %d registers a thread",
-                kGatedLaunchRegisters);
+                kBackLaunchRegisters);
       return;
     }
     st = allow_smem(reinterpret_cast<const void*>(kernel), kGatedBackwardSmem<T>);
-    if (st == ICTC_OK) kernel<<<grid, kGatedThreads, kGatedBackwardSmem<T>, stream>>>(p);
+    if (st == ICTC_OK) kernel<<<grid, kBackThreads, kGatedBackwardSmem<T>, stream>>>(maps, p);
   });
   if (st != ICTC_OK) return st;
   cudaError_t err = cudaGetLastError();
@@ -749,9 +757,10 @@ extern "C" int32_t ictc_o2_gated_linear_backward(
   const size_t size = dtype_size(dtype);
   const int32_t layout = layout_of(x, x_stride, weight, weight_stride, in, size);
   if (!preact && is_narrow(rows, hidden, in, dtype, layout) &&
-      (grad_stride != hidden || !aligned(grad_output, 16)))
+      (grad_stride != hidden || !aligned(grad_output, 16) || !aligned(grad_x, 16)))
     return fail(ICTC_ERR_INVALID,
-                "without preact a narrow layer needs a contiguous, 16-byte aligned grad_output");
+                "without preact a narrow layer needs a contiguous grad_output, and it and grad_x "
+                "16-byte aligned");
   GatedPlan plan{};
   st = plan_backward(rows, hidden, in, dtype, layout, preact != nullptr, current_device(), &plan);
   if (st == ICTC_OK) st = check_workspace(workspace, workspace_bytes, plan.total);

@@ -119,21 +119,6 @@ __device__ __forceinline__ void take_p(uint32_t at, float (&gate)[8], float (&up
   }
 }
 
-// 16 columns of a 64-column product.
-template <int P>
-__device__ __forceinline__ void take_product(uint32_t at, float (&v)[16]) {
-  tmem_load16(at, v);
-  if constexpr (P == 3) {
-    float y[16];
-    tmem_load16(at + kNarrow, y);
-    tmem_load_wait();
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = join_parts(v[i], y[i]);
-  } else {
-    tmem_load_wait();
-  }
-}
-
 // N columns of a row, of which `left` exist.  A thread owns a row, so lanes write rows apart:
 // 16 bytes each, whose sectors L2 puts together.  (Through shared memory, with lanes along
 // the columns, forward and backward took the same time and 32 KB that the slices need.)
@@ -225,9 +210,9 @@ template <typename T>
 constexpr size_t kGatedForwardSmem =
     1024 + 3 * kGatedOperand<T> + kGatedForwardSlices * kSliceX<T> + kGatedRows * 4 + 256;
 
-template <typename T>
+template <typename T, int THREADS>
 __device__ __forceinline__ void stage_bias(float* to, const GatedNarrowArgs& p) {
-  for (int i = threadIdx.x; i < kGatedRows; i += kGatedThreads) {
+  for (int i = threadIdx.x; i < kGatedRows; i += THREADS) {
     const int c = i & (kNarrow - 1);
     to[i] = p.bias && c < p.n
                 ? to_float(static_cast<const T*>(p.bias)[(i >= kNarrow ? p.n : 0) + c])
@@ -281,7 +266,7 @@ __global__ void __launch_bounds__(kGatedThreads, 1)
   }
   if (warp == 0) tmem_alloc(tmem_at, 2 * kSet);
   load_gated_weights<T, kGatedThreads>(weights, p);
-  stage_bias<T>(bias, p);
+  stage_bias<T, kGatedThreads>(bias, p);
   fence_proxy_async();
   tcgen05_fence_before();
   __syncthreads();
@@ -362,18 +347,35 @@ __global__ void __launch_bounds__(kGatedThreads, 1)
 }
 
 // ------------------------------------------------------------------------ backward
+//
+// A tile's chain is p, D, then dW and dx (their MMAs in turn: two that add to the same sums
+// take 110 to 160 cycles each, to different ones 76), then dx out.  16-bit types have room to
+// overlap two tiles of it: p of the next is formed while D of one waits for its products.  In
+// float32 one tile fills shared memory and TMEM: g lands where D's third parts will be, dx
+// leaves from where its first parts were, dx's sums lie where p's were, and the row warps cut
+// the next x while the tensor cores work on D.
 
-// Registers move to the row warps, which hold the sums of db.
-constexpr int kGatedLaunchRegisters = 80;  // 65,536 / 768, in steps of 8
-constexpr int kRowRegisters = 96, kGatedProducerRegisters = 56, kGatedIssueRegisters = 40;
-static_assert(kRowWarps * kRowRegisters + kGatedProducerWarps * kGatedProducerRegisters +
-                  4 * kGatedIssueRegisters <=
-              24 * kGatedLaunchRegisters);
-constexpr int kGatedBackwardSlices = 4;  // a tile
+constexpr int kRowThreads = kRowWarps * 32;
+constexpr int kBackMmaWarp = kRowWarps, kBackLoadWarp = kRowWarps + 1,
+              kBackStoreWarp = kRowWarps + 2;
+constexpr int kBackThreads = 20 * 32;
+// Registers move to the row warps, which hold sums of dW and db.
+constexpr int kBackLaunchRegisters = 96;  // 65,536 / 640, in steps of 8
+constexpr int kRowRegisters = 104, kIssueRegisters = 64;
+static_assert(kRowWarps * kRowRegisters + 4 * kIssueRegisters <= 20 * kBackLaunchRegisters);
+
+struct alignas(64) GatedNarrowMaps {
+  CUtensorMap x, g, dx;  // boxes of 128 bytes x 128 rows, swizzled; x in 16-bit types only
+};
 
 template <typename T>
-constexpr size_t kGatedBackwardSmem = 1024 + 4 * kGatedOperand<T> +
-                                      kGatedBackwardSlices * kSliceX<T> + kGatedRows * 4 + 512;
+constexpr int kBackBuffers = kCut<T> == 3 ? 1 : 2;  // of x, D, and (16-bit) g and p
+// Bytes of the raw x tile, or of two g tiles and the dx that leaves
+template <typename T>
+constexpr uint32_t kBackMore = kCut<T> == 3 ? kNarrowTile * kNarrow * 4 : 3 * kGatedBlock;
+template <typename T>
+constexpr size_t kGatedBackwardSmem =
+    1024 + (1 + 3 * kBackBuffers<T>)*kGatedOperand<T> + kBackMore<T> + kGatedRows * 4 + 512;
 
 // Eight columns of D to their tile, part by part.
 template <typename T>
@@ -394,201 +396,368 @@ __device__ __forceinline__ void store_d(unsigned char* at, const float (&v)[8]) 
   }
 }
 
+// One K step of a 64-column product: with three parts a1 (b1 | b2 | b3), a2 (b1 | b2), a3 b1
+// into sums of order 0, 1 and 2.
+template <int P>
+__device__ __forceinline__ void issue_orders(uint32_t d, uint64_t a, uint64_t a_part, uint64_t b,
+                                             bool bf16, bool a_mn, bool b_mn, bool add) {
+  const uint32_t one = mma_descriptor(bf16, a_mn, b_mn, kNarrowTile, kNarrow);
+  if constexpr (P == 3) {
+    mma_f16(d, a, b, mma_descriptor(bf16, a_mn, b_mn, kNarrowTile, 3 * kNarrow), add);
+    mma_f16(d + kNarrow, a + a_part, b,
+            mma_descriptor(bf16, a_mn, b_mn, kNarrowTile, 2 * kNarrow), true);
+    mma_f16(d + 2 * kNarrow, a + 2 * a_part, b, one, true);
+  } else {
+    mma_f16(d, a, b, one, add);
+  }
+}
+
+// 16 columns of such a product.
+template <int P>
+__device__ __forceinline__ void take_orders(uint32_t at, float (&v)[16]) {
+  tmem_load16(at, v);
+  if constexpr (P == 3) {
+    float y[16], z[16];
+    tmem_load16(at + kNarrow, y);
+    tmem_load16(at + 2 * kNarrow, z);
+    tmem_load_wait();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = join_parts(v[i], y[i] + z[i]);
+  } else {
+    tmem_load_wait();
+  }
+}
+
+// Where 16 bytes of column `col` of a row lie in swizzled boxes of 128 bytes x 128 rows.
+template <typename T>
+__device__ __forceinline__ uint32_t boxed(int row, int col) {
+  constexpr int kWidth = 128 / sizeof(T), V = 16 / sizeof(T);
+  return (col / kWidth) * kGatedBlock + swizzled(row, (col % kWidth) / V);
+}
+
 template <typename T, int ACT>
-__global__ void __launch_bounds__(kGatedThreads, 1)
-    gated_narrow_backward_kernel(const __grid_constant__ GatedNarrowArgs p) {
-  constexpr int P = kCut<T>, R = kGatedBackwardSlices;
-  constexpr uint32_t kOrders = P == 3 ? 2 : 1;
-  constexpr uint32_t kDx = kOrders * kGatedRows, kDw = kDx + kOrders * kNarrow;
-  constexpr uint32_t kColumns = kOrders * 256;
+__global__ void __launch_bounds__(kBackThreads, 1)
+    gated_narrow_backward_kernel(const __grid_constant__ GatedNarrowMaps maps,
+                                 const __grid_constant__ GatedNarrowArgs p) {
+  constexpr int P = kCut<T>, B = kBackBuffers<T>, kLag = B - 1;
+  constexpr bool kWide = P == 3;
+  constexpr uint32_t kPset = kWide ? 0 : kGatedRows;  // TMEM columns from one p to the next
+  constexpr uint32_t kDx = kWide ? 0 : 2 * kGatedRows, kDxSet = kWide ? 0 : kNarrow;
+  constexpr uint32_t kDw = kWide ? 2 * kGatedRows : 2 * kGatedRows + 2 * kNarrow;
   extern __shared__ unsigned char raw_smem[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t{1023});
   unsigned char* weights = smem;
-  unsigned char* x_tile = weights + kGatedOperand<T>;
-  unsigned char* d_tile = x_tile + kGatedOperand<T>;  // [parts][gate, up][128 rows][64]
-  unsigned char* slices = d_tile + 2 * kGatedOperand<T>;
-  float* bias = reinterpret_cast<float*>(slices + R * kSliceX<T>);
+  unsigned char* x_tiles = weights + kGatedOperand<T>;
+  unsigned char* d_tiles = x_tiles + B * kGatedOperand<T>;  // [parts][gate, up][128 rows][64]
+  unsigned char* more = d_tiles + 2 * B * kGatedOperand<T>;
+  unsigned char* g_tiles = kWide ? d_tiles + 4 * kGatedBlock : more;
+  unsigned char* leaving = kWide ? d_tiles : more + 2 * kGatedBlock;
+  float* bias = reinterpret_cast<float*>(more + kBackMore<T>);
   uint64_t* raw_full = reinterpret_cast<uint64_t*>(bias + kGatedRows);
-  uint64_t* raw_empty = raw_full + R;
-  uint64_t* x_full = raw_empty + R;
-  uint64_t* x_empty = x_full + 1;
-  uint64_t* p_done = x_empty + 1;
-  uint64_t* p_room = p_done + 1;
-  uint64_t* d_full = p_room + 1;
-  uint64_t* d_empty = d_full + 1;
-  uint64_t* dx_done = d_empty + 1;
-  uint64_t* dx_room = dx_done + 1;
-  uint64_t* dw_done = dx_room + 1;
+  uint64_t* raw_empty = raw_full + 1;
+  uint64_t* x_full = raw_empty + 1;
+  uint64_t* x_empty = x_full + B;
+  uint64_t* g_full = x_empty + B;
+  uint64_t* g_read = g_full + B;
+  uint64_t* p_done = g_read + B;
+  uint64_t* p_room = p_done + B;
+  uint64_t* d_full = p_room + B;
+  uint64_t* d_empty = d_full + B;
+  uint64_t* dx_done = d_empty + B;
+  uint64_t* dx_room = dx_done + B;
+  uint64_t* dw_done = dx_room + B;
   uint64_t* dw_room = dw_done + 1;
-  uint64_t* drain = dw_room + 1;
+  uint64_t* staged = dw_room + 1;
+  uint64_t* stage_free = staged + 1;
+  uint64_t* drain = stage_free + 1;
   uint32_t* tmem_at = reinterpret_cast<uint32_t*>(drain + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < R; ++i) {
-      mbar_init(&raw_full[i], 1);
-      mbar_init(&raw_empty[i], kGatedProducerWarps);
+    mbar_init(raw_full, 1);
+    mbar_init(raw_empty, kRowWarps);
+    for (int i = 0; i < B; ++i) {
+      mbar_init(&x_full[i], kWide ? kRowWarps : 1);
+      mbar_init(&x_empty[i], 1);
+      mbar_init(&g_full[i], 1);
+      mbar_init(&g_read[i], kRowWarps);
+      mbar_init(&p_done[i], 1);
+      mbar_init(&p_room[i], kRowWarps);
+      mbar_init(&d_full[i], kRowWarps);
+      mbar_init(&d_empty[i], 1);
+      mbar_init(&dx_done[i], 1);
+      mbar_init(&dx_room[i], kRowWarps);
     }
-    mbar_init(x_full, kGatedProducerWarps);
-    mbar_init(x_empty, 1);
-    mbar_init(p_done, 1);
-    mbar_init(p_room, kRowWarps);
-    mbar_init(d_full, kRowWarps);
-    mbar_init(d_empty, 1);
-    mbar_init(dx_done, 1);
-    mbar_init(dx_room, kRowWarps);
     mbar_init(dw_done, 1);
     mbar_init(dw_room, kRowWarps);
+    mbar_init(staged, kRowWarps);
+    mbar_init(stage_free, 1);
     mbar_init(drain, 1);
     fence_mbarrier_init();
   }
-  if (warp == 0) tmem_alloc(tmem_at, kColumns);
-  load_gated_weights<T, kGatedThreads>(weights, p);
-  stage_bias<T>(bias, p);
-  // columns of x past k and of D past n are never written, but the MMAs read them
-  for (uint32_t i = threadIdx.x; i < 3 * kGatedOperand<T> / 16; i += kGatedThreads)
-    reinterpret_cast<uint4*>(x_tile)[i] = make_uint4(0, 0, 0, 0);
+  if (warp == 0) tmem_alloc(tmem_at, 512);
+  load_gated_weights<T, kBackThreads>(weights, p);
+  stage_bias<T, kBackThreads>(bias, p);
+  // columns of x past k and of D past n may never be written, but the MMAs read them
+  for (uint32_t i = threadIdx.x; i < 3 * B * kGatedOperand<T> / 16; i += kBackThreads)
+    reinterpret_cast<uint4*>(x_tiles)[i] = make_uint4(0, 0, 0, 0);
   fence_proxy_async();
   tcgen05_fence_before();
   __syncthreads();
   tcgen05_fence_after();
   const uint32_t tmem = *tmem_at;
   const bool want_dx = p.e.out != nullptr, want_dw = p.partial != nullptr;
+  const int step = static_cast<int>(gridDim.x), first = static_cast<int>(blockIdx.x);
   const auto closes_group = [&](int t, uint32_t it) {
-    return it % kDwTiles == kDwTiles - 1 || t + static_cast<int>(gridDim.x) >= p.tiles;
+    return it % kDwTiles == kDwTiles - 1 || t + step >= p.tiles;
   };
   const int wide = 2 * p.n;
-  float* partial = want_dw ? p.partial + static_cast<int64_t>(blockIdx.x) * (wide * p.k + wide)
-                           : nullptr;
+  float* partial =
+      want_dw ? p.partial + static_cast<int64_t>(first) * (wide * p.k + wide) : nullptr;
 
-  if (warp >= kGatedMmaWarp) {
-    give_registers<kGatedIssueRegisters>();
-    if (warp == kGatedCopyWarp && lane == 0) copy_slices<T, R>(slices, raw_full, raw_empty, p);
-    if (warp == kGatedMmaWarp && lane == 0) {
-      constexpr bool kBf16 = !std::is_same_v<T, __half>;
-      const uint32_t xa = smem_addr(x_tile), da = smem_addr(d_tile), wa = smem_addr(weights);
-      const uint64_t d_rows = matrix_descriptor(da, 0, 1024);            // K-major
-      const uint64_t d_columns = matrix_descriptor(da, kGatedBlock, 1024);  // MN-major, two blocks
-      // MN-major with the parts behind one another as further columns
-      const uint64_t x_columns = matrix_descriptor(xa, kGatedBlock, 1024);
-      const uint64_t w_columns = matrix_descriptor(wa, kGatedRows * 128, 1024);
-      constexpr uint64_t kXp = kGatedBlock / 16, kDp = 2 * kXp, kWp = kGatedRows * 8;
+  if (warp >= kRowWarps) {
+    give_registers<kIssueRegisters>();
+    if (warp == kBackLoadWarp && lane == 0) {
       bool ok = true;
       uint32_t it = 0;
-      for (int t = blockIdx.x; t < p.tiles; t += gridDim.x, ++it) {
-        ok = mbar_wait_idle(x_full, it & 1, kCodeMma) &&
-             mbar_wait_idle(p_room, (it & 1) ^ 1, kCodeMma);
+      for (int t = first; t < p.tiles; t += step, ++it) {
+        const uint32_t b = it & kLag, phase = (it >> kLag) & 1;
+        const int64_t row0 = static_cast<int64_t>(t) * kNarrowTile;
+        if constexpr (kWide) {
+          ok = mbar_wait_idle(raw_empty, phase ^ 1, kCodeProducer);
+          if (!ok) break;
+          const int64_t left = p.m - row0;
+          const uint32_t bytes =
+              static_cast<uint32_t>(left < kNarrowTile ? left : kNarrowTile) * p.k * 4;
+          mbar_arrive_expect_tx(raw_full, bytes);
+          bulk_g2s(more, static_cast<const float*>(p.x) + row0 * p.k, bytes, raw_full);
+          ok = mbar_wait_idle(&d_empty[0], phase ^ 1, kCodeProducer);
+        } else {
+          ok = mbar_wait_idle(&x_empty[b], phase ^ 1, kCodeProducer);
+          if (!ok) break;
+          mbar_arrive_expect_tx(&x_full[b], kGatedBlock);
+          tma_load_2d(x_tiles + b * kGatedBlock, &maps.x, 0, static_cast<int>(row0), &x_full[b]);
+          ok = mbar_wait_idle(&g_read[b], phase ^ 1, kCodeProducer);
+        }
+        if (!ok) break;
+        mbar_arrive_expect_tx(&g_full[b], kNarrowTile * kNarrow * sizeof(T));
+        for (int c = 0; c < kNarrow; c += 128 / static_cast<int>(sizeof(T)))
+          tma_load_2d(g_tiles + b * kGatedBlock + boxed<T>(0, c), &maps.g, c,
+                      static_cast<int>(row0), &g_full[b]);
+      }
+      if (!ok) settle_copies();
+    }
+    if (warp == kBackStoreWarp && lane == 0 && want_dx) {
+      uint32_t it = 0;
+      for (int t = first; t < p.tiles; t += step, ++it) {
+        if (!mbar_wait_idle(staged, it & 1, kCodeProducer)) break;
+        for (int c = 0; c < p.k; c += 128 / static_cast<int>(sizeof(T)))
+          tma_store_2d(leaving + boxed<T>(0, c), &maps.dx, c, t * kNarrowTile);
+        tma_store_wait_read();
+        mbar_arrive(stage_free);
+      }
+    }
+    if (warp == kBackMmaWarp && lane == 0) {
+      constexpr bool kBf16 = !std::is_same_v<T, __half>;
+      const uint32_t wa = smem_addr(weights);
+      // MN-major with the parts behind one another as further columns
+      const uint64_t w_columns = matrix_descriptor(wa, kGatedRows * 128, 1024);
+      constexpr uint64_t kXp = kGatedBlock / 16, kDp = 2 * kXp;
+      const int steps = (p.n + 15) / 16, dx_steps = want_dx ? 2 * steps : 0;
+      const int dw_steps = want_dw ? kNarrowTile / 16 : 0;
+      const int most = dx_steps > dw_steps ? dx_steps : dw_steps;
+      bool ok = true;
+      uint32_t it = 0;
+      const auto form_p = [&](uint32_t i) {
+        const uint32_t b = i & kLag, phase = (i >> kLag) & 1;
+        ok = mbar_wait_idle(&x_full[b], phase, kCodeMma);
+        if (ok && (!kWide || want_dx))  // in float32 dx's sums lie where p will be
+          ok = mbar_wait_idle(kWide ? &dx_room[b] : &p_room[b], phase ^ 1, kCodeMma);
+        if (!ok) return;
+        tcgen05_fence_after();
+        issue_p<T>(tmem + b * kPset, smem_addr(x_tiles + b * kGatedOperand<T>), wa, p.k);
+        mma_commit(&p_done[b]);
+      };
+      if (kLag && first < p.tiles) form_p(0);
+      for (int t = first; ok && t < p.tiles; t += step, ++it) {
+        const uint32_t b = it & kLag, phase = (it >> kLag) & 1;
+        if (!kLag) form_p(it);
+        else if (t + step < p.tiles) form_p(it + 1);
+        if (ok) ok = mbar_wait_idle(&d_full[b], phase, kCodeMma);
+        if (!ok) break;
+        const bool opens = it % kDwTiles == 0;
+        if (want_dw && opens)
+          ok = mbar_wait_idle(dw_room, ((it / kDwTiles) & 1) ^ 1, kCodeMma);
+        if (ok && !kWide && want_dx) ok = mbar_wait_idle(&dx_room[b], phase ^ 1, kCodeMma);
         if (!ok) break;
         tcgen05_fence_after();
-        issue_p<T>(tmem, xa, wa, p.k);
-        mma_commit(p_done);
-        ok = mbar_wait_idle(d_full, it & 1, kCodeMma);
-        if (!ok) break;
-        tcgen05_fence_after();
-        // dW first: x's tile is free again while the MMAs of dx still read D's
-        if (want_dw) {
-          const bool first = it % kDwTiles == 0;
-          if (first) ok = mbar_wait_idle(dw_room, ((it / kDwTiles) & 1) ^ 1, kCodeMma);
-          if (!ok) break;
-          tcgen05_fence_after();
+        const uint32_t xa = smem_addr(x_tiles + b * kGatedOperand<T>);
+        const uint32_t da = smem_addr(d_tiles + b * 2 * kGatedOperand<T>);
+        const uint64_t x_columns = matrix_descriptor(xa, kGatedBlock, 1024);
+        const uint64_t d_rows = matrix_descriptor(da, 0, 1024);               // K-major
+        const uint64_t d_columns = matrix_descriptor(da, kGatedBlock, 1024);  // two blocks
 #pragma unroll 1
-          for (int s = 0; s < kNarrowTile / 16; ++s)
-            issue_gated<P, kNarrow>(tmem + kDw, d_columns + 128 * s, kDp, x_columns + 128 * s, kXp,
-                                    kBf16, true, true, !first || s > 0);
-          if (closes_group(t, it)) mma_commit(dw_done);
+        for (int s = 0; s < most; ++s) {
+          if (s < dw_steps)
+            issue_orders<P>(tmem + kDw, d_columns + 128 * s, kDp, x_columns + 128 * s, kBf16, true,
+                            true, !opens || s > 0);
+          if (s < dx_steps) {  // 64 columns of D and rows of W a half
+            const int h = s >= steps, q = s - h * steps;
+            issue_orders<P>(tmem + kDx + b * kDxSet, d_rows + h * kXp + 2 * q, kDp,
+                            w_columns + h * 512 + 128 * q, kBf16, false, true, s > 0);
+          }
         }
-        mma_commit(x_empty);
-        if (want_dx) {
-          ok = mbar_wait_idle(dx_room, (it & 1) ^ 1, kCodeMma);
-          if (!ok) break;
-          tcgen05_fence_after();
-#pragma unroll 1
-          for (int h = 0; h < 2; ++h)
-#pragma unroll 1
-            for (int s = 0; 16 * s < p.n; ++s)  // 64 rows of W and columns of D a half
-              issue_gated<P, kNarrow>(tmem + kDx, d_rows + h * kXp + 2 * s, kDp,
-                                      w_columns + h * 512 + 128 * s, kWp, kBf16, false, true,
-                                      h > 0 || s > 0);
-          mma_commit(dx_done);
-        }
-        mma_commit(d_empty);
+        if (want_dw && closes_group(t, it)) mma_commit(dw_done);
+        mma_commit(&x_empty[b]);
+        if (want_dx) mma_commit(&dx_done[b]);
+        mma_commit(&d_empty[b]);
       }
       // the last arrival lands before the CTA goes away
-      if (ok && it > 0) ok = mbar_wait_idle(d_empty, (it - 1) & 1, kCodeMma);
+      if (ok && it > 0)
+        ok = mbar_wait_idle(&d_empty[(it - 1) & kLag], ((it - 1) >> kLag) & 1, kCodeMma);
       if (!ok) {  // MMAs in flight finish
         mma_commit(drain);
         mbar_wait(drain, 0, kCodeDrain, kDrainLimitNs);
       }
     }
     __syncwarp();
-  } else if (warp >= kRowWarps) {
-    give_registers<kGatedProducerRegisters>();
-    const int tid = threadIdx.x - kRowWarps * 32;
-    uint32_t it = 0, n = 0;
-    for (int t = blockIdx.x; t < p.tiles; t += gridDim.x, ++it) {
-      if (!mbar_wait_warp(x_empty, (it & 1) ^ 1, kCodeProducer) ||
-          !fill_x_tile<T, R>(x_tile, slices, raw_full, raw_empty, t, p, tid, lane, n))
-        break;
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(x_full);
-    }
   } else {
     take_registers<kRowRegisters>();
     // a thread has a row of p and dx and a row of dW (TMEM lanes 0-63 the gate's, 64-127 the
     // other's), 16 columns of each
+    constexpr int V = 16 / sizeof(T);
     const int quad = warp & 3, c0 = (warp >> 2) * 16, in_tile = quad * 32 + lane;
     const uint32_t at = tmem + (static_cast<uint32_t>(quad * 32) << 16) + c0;
-    unsigned char* d_row = d_tile + in_tile * 128;
-    constexpr int V = 16 / sizeof(T);
-    const T* g = static_cast<const T*>(p.g) + c0;
-    T* dx = static_cast<T*>(p.e.out) + c0;
-    const int dw_row = (in_tile & (kNarrow - 1)) + (in_tile >= kNarrow ? p.n : 0);
-    float* dw = partial + dw_row * p.k + c0;
-    const bool dw_some = want_dw && (in_tile & (kNarrow - 1)) < p.n;
-    float db[2][16];
+    // sums of db over the rows of lanes l and l + 16: the gate's in the one, the other's in
+    // the other
+    float db[16], dw[16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) db[0][i] = db[1][i] = 0.f;
-    Pack<T, V> gv[16 / V];
-    const auto load_g = [&](int64_t row) {
+    for (int i = 0; i < 16; ++i) db[i] = dw[i] = 0.f;
+    bool ok = true;
+
+    // float32: the next tile's x, cut
+    const auto fill_x = [&](int t, uint32_t it) {
+      if constexpr (kWide) {
+        ok = mbar_wait_warp(raw_full, it & 1, kCodeProducer) &&
+             mbar_wait_warp(&x_empty[0], (it & 1) ^ 1, kCodeProducer);
+        if (!ok) return;
+        const int unit = threadIdx.x & 15, r0 = threadIdx.x >> 4;
+        const int64_t left = p.m - static_cast<int64_t>(t) * kNarrowTile;
+        const Slice<T> raw{reinterpret_cast<const T*>(more), nullptr, p.k,
+                           left < kNarrowTile ? static_cast<int>(left) : kNarrowTile, 0};
+        float v[4][4];
+        uint32_t seen = 0;
 #pragma unroll
-      for (int i = 0; i < 16 / V; ++i) {
-        gv[i] = Pack<T, V>{};
-        if (row < p.m && c0 + i * V < p.n)
-          gv[i] = *reinterpret_cast<const Pack<T, V>*>(g + row * p.n + i * V);
+        for (int j = 0; j < 4; ++j) {
+          read_unit<true>(raw, r0 + 32 * j, unit, v[j]);
+          seen |= unit_bits<true>(v[j]);
+        }
+        release_slot(raw_empty, seen, lane);
+        if (4 * unit < p.k)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) store_unit<T>(x_tiles, kGatedBlock, r0 + 32 * j, unit, v[j]);
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&x_full[0]);
       }
     };
-    load_g(static_cast<int64_t>(blockIdx.x) * kNarrowTile + in_tile);
-    bool ok = true;
+
+    // what the products of a tile left
+    const auto take_tile = [&](int t, uint32_t it) {
+      const uint32_t b = it & kLag, phase = (it >> kLag) & 1;
+      if (want_dw && closes_group(t, it)) {
+        ok = mbar_wait_warp(dw_done, (it / kDwTiles) & 1, kCodeEpilogue);
+        if (!ok) return;
+        tcgen05_fence_after();
+        float sum[16];
+        take_orders<P>(at + kDw, sum);
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(dw_room);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) dw[i] += sum[i];
+      }
+      float sum[16];
+      if (want_dx) {
+        ok = mbar_wait_warp(&dx_done[b], phase, kCodeEpilogue);
+        if (!ok) return;
+        tcgen05_fence_after();
+        take_orders<P>(at + kDx + b * kDxSet, sum);
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&dx_room[b]);
+      }
+      if (kWide && t + step < p.tiles) fill_x(t + step, it + 1);
+      if (!ok || !want_dx) return;
+      if (!kWide) {
+        ok = mbar_wait_warp(stage_free, (it & 1) ^ 1, kCodeEpilogue);
+        if (!ok) return;
+      }
+#pragma unroll
+      for (int i = 0; i < 16; i += V) {
+        Pack<T, V> o;
+#pragma unroll
+        for (int j = 0; j < V; ++j) o.v[j] = from_float<T>(sum[i + j]);
+        *reinterpret_cast<Pack<T, V>*>(leaving + boxed<T>(in_tile, c0 + i)) = o;
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(staged);
+    };
+
+    if (kWide && first < p.tiles) fill_x(first, 0);
     uint32_t it = 0;
-    for (int t = blockIdx.x; ok && t < p.tiles; t += gridDim.x, ++it) {
-      const int64_t row = static_cast<int64_t>(t) * kNarrowTile + in_tile;
-      ok = mbar_wait_warp(p_done, it & 1, kCodeEpilogue) &&
-           mbar_wait_warp(d_empty, (it & 1) ^ 1, kCodeEpilogue);
+    for (int t = first; ok && t < p.tiles; t += step, ++it) {
+      const uint32_t b = it & kLag, phase = (it >> kLag) & 1;
+      const bool in = static_cast<int64_t>(t) * kNarrowTile + in_tile < p.m;
+      ok = mbar_wait_warp(&g_full[b], phase, kCodeEpilogue);
+      if (!ok) break;
+      float g[16];
+      uint32_t seen = 0;
+#pragma unroll
+      for (int i = 0; i < 16; i += V) {
+        uint32_t q[4];
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3])
+                     : "r"(smem_addr(g_tiles + b * kGatedBlock + boxed<T>(in_tile, c0 + i)))
+                     : "memory");
+        const Pack<T, V>& pk = *reinterpret_cast<const Pack<T, V>*>(q);
+#pragma unroll
+        for (int j = 0; j < V; ++j) g[i + j] = to_float(pk.v[j]);
+        seen |= q[0];
+      }
+      release_slot(&g_read[b], seen, lane);
+      ok = mbar_wait_warp(&p_done[b], phase, kCodeEpilogue);
+      // where D goes: g has been read and dx has left, or the products before last are done
+      if (ok && kWide) ok = mbar_wait_warp(&g_read[0], phase, kCodeEpilogue);
+      if (ok && kWide && want_dx) ok = mbar_wait_warp(stage_free, phase ^ 1, kCodeEpilogue);
+      if (ok && !kWide) ok = mbar_wait_warp(&d_empty[b], phase ^ 1, kCodeEpilogue);
       if (!ok) break;
       tcgen05_fence_after();
+      unsigned char* d_row = d_tiles + b * 2 * kGatedOperand<T> + in_tile * 128;
 #pragma unroll
       for (int j = 0; j < 16; j += 8) {
         float gate[8], up[8];
-        take_p<P>(at + j, gate, up);
+        take_p<P>(at + b * kPset + j, gate, up);
         if (j == 8) {
           tcgen05_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(p_room);
+          if (lane == 0) mbar_arrive(&p_room[b]);
         }
-        if (c0 + j >= p.n) continue;
+        // up to the last K step of dx: zeros past n, over what dx left there
+        if (c0 + j >= ((p.n + 15) & ~15)) continue;
         add_bias(gate, bias + c0 + j);
         add_bias(up, bias + kNarrow + c0 + j);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float v = to_float(gv[(j + i) / V].v[(j + i) % V]);
-          const float pg = gate[i], pu = up[i];
+          const float v = g[j + i], pg = gate[i], pu = up[i];
           // rows past the last have no gradient, but a bias that may be infinite
-          gate[i] = row < p.m ? v * pu * activation_slope<ACT>(pg) : 0.f;
-          up[i] = row < p.m ? v * activate<ACT>(pg) : 0.f;
-          db[0][j + i] += gate[i];
-          db[1][j + i] += up[i];
+          gate[i] = in ? v * pu * activation_slope<ACT>(pg) : 0.f;
+          up[i] = in ? v * activate<ACT>(pg) : 0.f;
+          const bool low = lane < 16;
+          const float other = __shfl_xor_sync(0xffffffffu, low ? up[i] : gate[i], 16);
+          db[j + i] += (low ? gate[i] : up[i]) + other;
         }
         unsigned char* to = d_row + ((((c0 + j) / 8) ^ (in_tile & 7)) << 4);
         store_d<T>(to, gate);
@@ -596,68 +765,41 @@ __global__ void __launch_bounds__(kGatedThreads, 1)
       }
       fence_proxy_async();
       __syncwarp();
-      if (lane == 0) mbar_arrive(d_full);
-      // on their way while the MMAs run: the next tile's g, and what dW is so far
-      load_g(row + static_cast<int64_t>(gridDim.x) * kNarrowTile);
-      if (want_dw && closes_group(t, it)) {
-        float4 old[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          old[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (dw_some && it >= kDwTiles && c0 + 4 * i < p.k)
-            old[i] = *reinterpret_cast<const float4*>(dw + 4 * i);
-        }
-        ok = mbar_wait_warp(dw_done, (it / kDwTiles) & 1, kCodeEpilogue);
-        if (!ok) break;
-        tcgen05_fence_after();
-        float sum[16];
-        take_product<P>(at + kDw, sum);
-        tcgen05_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(dw_room);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (dw_some && c0 + 4 * i < p.k)
-            *reinterpret_cast<float4*>(dw + 4 * i) =
-                make_float4(old[i].x + sum[4 * i], old[i].y + sum[4 * i + 1],
-                            old[i].z + sum[4 * i + 2], old[i].w + sum[4 * i + 3]);
-      }
-      if (want_dx) {
-        ok = mbar_wait_warp(dx_done, it & 1, kCodeEpilogue);
-        if (!ok) break;
-        tcgen05_fence_after();
-        float sum[16];
-        take_product<P>(at + kDx, sum);
-        tcgen05_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(dx_room);
-        if (row < p.m && c0 < p.k) store_columns(dx + row * p.k, sum, p.k - c0, p.e.vec);
-      }
+      if (lane == 0) mbar_arrive(&d_full[b]);
+      if (!kLag) take_tile(t, it);
+      else if (it > 0) take_tile(t - step, it - 1);
     }
-    // db: over the lanes, then (below) over the four quads in order.  Every slice was read
-    // long ago where all went well; elsewhere nothing is used.
-    if (ok) {
-      float* sums = reinterpret_cast<float*>(slices) + warp * 32;
+    if (kLag && ok && it > 0)
+      take_tile(first + static_cast<int>(it - 1) * step, it - 1);
+    if (ok && want_dw) {
+      // every product is done: x's tile has room for the sums of db
+      float* sums = reinterpret_cast<float*>(x_tiles) + warp * 32;
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int i = 0; i < 16; ++i) {
+        float v = db[i];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          float v = db[h][i];
+        for (int s = 8; s > 0; s >>= 1) v += __shfl_xor_sync(0xffffffffu, v, s);
+        if ((lane & 15) == 0) sums[lane + i] = v;
+      }
+      const int column = in_tile & (kNarrow - 1);  // of D, in its half
+      float* to = partial + ((in_tile >= kNarrow ? p.n : 0) + column) * p.k + c0;
+      if (column < p.n)
 #pragma unroll
-          for (int s = 16; s > 0; s >>= 1) v += __shfl_xor_sync(0xffffffffu, v, s);
-          if (lane == 0) sums[h * 16 + i] = v;
-        }
+        for (int i = 0; i < 16; i += 4)
+          if (c0 + i < p.k)
+            *reinterpret_cast<float4*>(to + i) =
+                make_float4(dw[i], dw[i + 1], dw[i + 2], dw[i + 3]);
     }
   }
   tcgen05_fence_before();
   __syncthreads();
   if (warp == 0) {
     tcgen05_fence_after();
-    tmem_free(tmem, kColumns);
+    tmem_free(tmem, 512);
   }
-  if (want_dw && threadIdx.x < kGatedRows) {
+  if (want_dw && threadIdx.x < kGatedRows) {  // db over the four quads, in order
     const int h = threadIdx.x >> 6, c = threadIdx.x & (kNarrow - 1);
-    const float* sums = reinterpret_cast<const float*>(slices);
+    const float* sums = reinterpret_cast<const float*>(x_tiles);
     if (c < p.n) {
       float total = 0.f;
       for (int q = 0; q < 4; ++q) total += sums[((c >> 4) * 4 + q) * 32 + h * 16 + (c & 15)];

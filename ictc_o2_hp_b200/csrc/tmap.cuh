@@ -40,6 +40,10 @@ int encode_row_tile_maps(const float* base, int64_t rows, int C, int M, bool ful
 int encode_matrix_map(const void* base, int size, bool bf16, int64_t inner, int64_t outer,
                       int64_t stride, int box_inner, int box_outer, CUtensorMap* map);
 
+// The same in boxes of 128 bytes x box_outer, swizzled rows for either size.
+int encode_swizzled_map(const void* base, int size, bool bf16, int64_t inner, int64_t outer,
+                        int64_t stride, int box_outer, CUtensorMap* map);
+
 // 2-D tile load of box coordinates (x, y) into shared memory, completing on `bar`.
 __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int x, int y,
                                             uint64_t* bar) {
@@ -50,6 +54,20 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, i
         "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y),
         "r"(static_cast<uint32_t>(__cvta_generic_to_shared(bar)))
       : "memory");
+}
+
+// One thread: 2-D tile store of shared memory to box coordinates (x, y), clipped to the
+// tensor, and the wait until every such store of the thread has read its shared memory.
+__device__ __forceinline__ void tma_store_2d(const void* src, const CUtensorMap* map, int x,
+                                             int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];"
+               ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y),
+               "r"(static_cast<uint32_t>(__cvta_generic_to_shared(src)))
+               : "memory");
+}
+__device__ __forceinline__ void tma_store_wait_read() {
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+  asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
 }
 
 // 3-D tile load of box coordinates (x, y, z) into shared memory, completing on `bar`.
