@@ -467,19 +467,35 @@ GatedNarrowArgs narrow_args(const T* x, const T* w, int64_t ldw, const void* bia
   return p;
 }
 
+// `out` [m, wide_out] is y or dx.
 template <typename T>
-int run_narrow_forward(const T* x, const T* w, int64_t ldw, Epilogue e, int64_t m, int64_t n,
+int narrow_maps(const T* x, const T* g, const T* out, int64_t m, int64_t n, int64_t k,
+                int64_t wide_out, GatedNarrowMaps* maps) {
+  constexpr int kSize = sizeof(T);
+  constexpr bool kBf16 = std::is_same_v<T, __nv_bfloat16>;
+  const auto encode = [&](const T* base, int64_t width, CUtensorMap* map) {
+    return base == nullptr ||
+           encode_swizzled_map(base, kSize, kBf16, width, m, width * kSize, kNarrowTile, map) == 0;
+  };
+  if (encode(x, k, &maps->x) && encode(g, n, &maps->g) && encode(out, wide_out, &maps->out))
+    return ICTC_OK;
+  return fail(ICTC_ERR_UNSUPPORTED, "gated linear: no tensor map for these operands");
+}
+
+template <typename T>
+int run_narrow_forward(const T* x, const T* w, int64_t ldw, const Epilogue& e, int64_t m, int64_t n,
                        int64_t k, cudaStream_t stream) {
-  GatedNarrowArgs p = narrow_args(x, w, ldw, e.bias, m, n, k);
-  e.vec = aligned(e.out, 16);
-  p.e = e;
+  const GatedNarrowArgs p = narrow_args(x, w, ldw, e.bias, m, n, k);
+  GatedNarrowMaps maps{};
+  int st = narrow_maps<T>(x, nullptr, static_cast<const T*>(e.out), m, n, k, n, &maps);
+  if (st != ICTC_OK) return st;
   const int sms = sm_count(current_device());
-  int st = ICTC_OK;
   for_activation(e.activation, [&](auto act) {
     const auto kernel = gated_narrow_forward_kernel<T, act.value>;
     st = allow_smem(reinterpret_cast<const void*>(kernel), kGatedForwardSmem<T>);
     if (st == ICTC_OK)
-      kernel<<<p.tiles < sms ? p.tiles : sms, kGatedThreads, kGatedForwardSmem<T>, stream>>>(p);
+      kernel<<<p.tiles < sms ? p.tiles : sms, kGatedForwardThreads, kGatedForwardSmem<T>, stream>>>(
+          maps, p);
   });
   if (st != ICTC_OK) return st;
   const cudaError_t err = cudaGetLastError();
@@ -495,17 +511,10 @@ int run_narrow_backward(const T* x, const T* w, int64_t ldw, const void* bias, c
   p.partial = dw || db ? partial : nullptr;
   p.e.out = dx;
   GatedNarrowMaps maps{};
-  constexpr int kSize = sizeof(T);
-  constexpr bool kBf16 = std::is_same_v<T, __nv_bfloat16>;
-  const auto encode = [&](const void* base, int64_t width, CUtensorMap* map) {
-    return encode_swizzled_map(base, kSize, kBf16, width, m, width * kSize, kNarrowTile, map);
-  };
-  if (encode(x, k, &maps.x) != 0 || encode(g, n, &maps.g) != 0 ||
-      (dx && encode(dx, k, &maps.dx) != 0))
-    return fail(ICTC_ERR_UNSUPPORTED, "gated linear: no tensor map for these operands");
+  int st = narrow_maps<T>(x, g, dx, m, n, k, k, &maps);
+  if (st != ICTC_OK) return st;
   const int sms = sm_count(current_device());
   const int grid = p.tiles < sms ? p.tiles : sms;
-  int st = ICTC_OK;
   for_activation(activation, [&](auto act) {
     const auto kernel = gated_narrow_backward_kernel<T, act.value>;
     static const bool shares_fit = [&] {
@@ -715,6 +724,8 @@ extern "C" int32_t ictc_o2_gated_linear_forward(const void* x, int64_t x_stride,
   const int32_t layout = layout_of(x, x_stride, weight, weight_stride, in, dtype_size(dtype));
   GatedPlan plan{};
   st = plan_forward(rows, hidden, in, dtype, layout, preact != nullptr, current_device(), &plan);
+  if (st == ICTC_OK && plan.way == Way::narrow && !aligned(y, 16))
+    st = fail(ICTC_ERR_INVALID, "without preact a narrow layer needs a 16-byte aligned y");
   if (st == ICTC_OK) st = check_workspace(workspace, workspace_bytes, plan.total);
   if (st != ICTC_OK) return st;
   Epilogue e{};

@@ -97,118 +97,77 @@ __device__ __forceinline__ void issue_p(uint32_t d, uint32_t x_tile, uint32_t we
                                      !std::is_same_v<T, __half>, false, false, s > 0);
 }
 
-// Eight columns of p, of the gate's half and of the other.
+// Eight columns, with three parts the leading sums and, `others` columns on, the others.
 template <int P>
-__device__ __forceinline__ void take_p(uint32_t at, float (&gate)[8], float (&up)[8]) {
+__device__ __forceinline__ void take8(uint32_t at, uint32_t others, float2 (&v)[4]) {
+  float w[8];
+  tmem_load8(at, w);
   if constexpr (P == 3) {
-    float y[8], z[8];
-    tmem_load8(at, gate);
-    tmem_load8(at + kNarrow, up);
-    tmem_load8(at + kGatedRows, y);
-    tmem_load8(at + kGatedRows + kNarrow, z);
+    float y[8];
+    tmem_load8(at + others, y);
     tmem_load_wait();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      gate[i] = join_parts(gate[i], y[i]);
-      up[i] = join_parts(up[i], z[i]);
-    }
+    for (int i = 0; i < 4; ++i)  // join_parts
+      v[i] = __fadd2_rn(make_float2(w[2 * i], w[2 * i + 1]),
+                        make_float2(fmaxf(y[2 * i], -3.402823466e38f),
+                                    fmaxf(y[2 * i + 1], -3.402823466e38f)));
   } else {
-    tmem_load8(at, gate);
-    tmem_load8(at + kNarrow, up);
     tmem_load_wait();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = make_float2(w[2 * i], w[2 * i + 1]);
   }
 }
 
-// N columns of a row, of which `left` exist.  A thread owns a row, so lanes write rows apart:
-// 16 bytes each, whose sectors L2 puts together.  (Through shared memory, with lanes along
-// the columns, forward and backward took the same time and 32 KB that the slices need.)
-template <typename T, int N>
-__device__ __forceinline__ void store_columns(T* to, const float (&v)[N], int left, bool vec) {
-  constexpr int V = 16 / sizeof(T);
-  if (vec) {
-#pragma unroll
-    for (int i = 0; i < N; i += V) {
-      Pack<T, V> o;
-#pragma unroll
-      for (int j = 0; j < V; ++j) o.v[j] = from_float<T>(v[i + j]);
-      if (i < left) *reinterpret_cast<Pack<T, V>*>(to + i) = o;
-    }
+// act and act' of two values.  f32x2 arithmetic: the row warps are bound by their issue slots.
+template <int ACT>
+__device__ __forceinline__ void gate_pair(float2 p, float2* a, float2* slope) {
+  if constexpr (ACT == ICTC_ACT_SILU) {
+    const float2 e = __fmul2_rn(p, make_float2(-1.4426950408889634f, -1.4426950408889634f));
+    float2 s;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(s.x) : "f"(e.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(s.y) : "f"(e.y));
+    s = __fadd2_rn(s, make_float2(1.f, 1.f));
+    s = make_float2(fast_reciprocal(s.x), fast_reciprocal(s.y));
+    *a = __fmul2_rn(p, s);
+    // s (1 + p (1 - s)) = s + p s (1 - s)
+    *slope = __ffma2_rn(*a, __ffma2_rn(s, make_float2(-1.f, -1.f), make_float2(1.f, 1.f)), s);
   } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (i < left) to[i] = from_float<T>(v[i]);
+    *a = make_float2(activate<ACT>(p.x), activate<ACT>(p.y));
+    *slope = make_float2(activation_slope<ACT>(p.x), activation_slope<ACT>(p.y));
   }
 }
 
-// The producers' four warps: the tile's x from the ring of slices, cut, into `tile`.
-template <typename T, int R>
-__device__ __forceinline__ bool fill_x_tile(unsigned char* tile, const unsigned char* slices,
-                                            uint64_t* raw_full, uint64_t* raw_empty, int t,
-                                            const GatedNarrowArgs& p, int tid, int lane,
-                                            uint32_t& n) {
-  const int unit = tid & 15, r0 = tid >> 4;
-  const int columns = (p.k + 15) & ~15;  // that the MMAs read
-  SliceWalk at{t, 0, p.tiles, static_cast<int>(gridDim.x), p.m};
-#pragma unroll 1
-  for (int q = 0; q < kNarrowTile / kSliceRows; ++q, ++at.slice) {
-    Slice<T> slice{nullptr, nullptr, p.k, 0, 0};
-    const bool some = at.row() < p.m;
-    const int slot = n % R;
-    if (some) {
-      if (!mbar_wait_warp(&raw_full[slot], (n / R) & 1, kCodeProducer)) return false;
-      slice.raw = reinterpret_cast<const T*>(slices + slot * kSliceX<T>);
-      slice.rows = at.rows();
-    }
-    float v[4][4];
-    uint32_t seen = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      read_unit<true>(slice, r0 + 8 * j, unit, v[j]);
-      seen |= unit_bits<true>(v[j]);
-    }
-    if (4 * unit < columns)
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        store_unit<T>(tile, kGatedBlock, q * kSliceRows + r0 + 8 * j, unit, v[j]);
-    if (some) {
-      release_slot(&raw_empty[slot], seen, lane);
-      ++n;
-    }
-  }
-  return true;
-}
-
-// One thread: x's slices into the ring.
-template <typename T, int R>
-__device__ __forceinline__ void copy_slices(unsigned char* slices, uint64_t* raw_full,
-                                            uint64_t* raw_empty, const GatedNarrowArgs& p) {
-  const T* x = static_cast<const T*>(p.x);
-  SliceWalk at{static_cast<int>(blockIdx.x), 0, p.tiles, static_cast<int>(gridDim.x), p.m};
-  bool ok = true;
-  for (uint32_t n = 0; !at.done(); at.next(), ++n) {
-    const int slot = n % R;
-    ok = mbar_wait_idle(&raw_empty[slot], ((n / R) & 1) ^ 1, kCodeProducer);
-    if (!ok) break;
-    const uint32_t bytes = slice_bytes<T>(p.k, at.rows());
-    mbar_arrive_expect_tx(&raw_full[slot], bytes);
-    bulk_g2s(slices + slot * kSliceX<T>, x + at.row() * p.k, bytes, &raw_full[slot]);
-  }
-  if (!ok) settle_copies();
-}
-
-// Warps of both kernels: 16 that take rows out of TMEM, four producers, MMA and copy warp.
-// More of the first hide the latencies of TMEM and of the exponentials (with eight, bf16
-// 1,048,576 x 64 x 64 forward 127 us, backward 482).
-constexpr int kRowWarps = 16, kGatedProducerWarps = 4;
-constexpr int kGatedMmaWarp = kRowWarps + kGatedProducerWarps, kGatedCopyWarp = kGatedMmaWarp + 1;
-constexpr int kGatedThreads = 24 * 32;
-
-// ------------------------------------------------------------------------- forward
-
-constexpr int kGatedForwardSlices = 8;
+// Where 16 bytes of column `col` of a row lie in swizzled boxes of 128 bytes x 128 rows.
 template <typename T>
-constexpr size_t kGatedForwardSmem =
-    1024 + 3 * kGatedOperand<T> + kGatedForwardSlices * kSliceX<T> + kGatedRows * 4 + 256;
+__device__ __forceinline__ uint32_t boxed(int row, int col) {
+  constexpr int kWidth = 128 / sizeof(T), V = 16 / sizeof(T);
+  return (col / kWidth) * kGatedBlock + swizzled(row, (col % kWidth) / V);
+}
+
+// Eight columns of a row to such boxes.
+template <typename T>
+__device__ __forceinline__ void store_boxed(unsigned char* boxes, int row, int col,
+                                            const float2 (&v)[4]) {
+  constexpr int V = 16 / sizeof(T);
+#pragma unroll
+  for (int i = 0; i < 8; i += V) {
+    Pack<T, V> o;
+#pragma unroll
+    for (int j = 0; j < V; j += 2) {
+      o.v[j] = from_float<T>(v[(i + j) / 2].x);
+      o.v[j + 1] = from_float<T>(v[(i + j) / 2].y);
+    }
+    *reinterpret_cast<Pack<T, V>*>(boxes + boxed<T>(row, col + i)) = o;
+  }
+}
+
+struct alignas(64) GatedNarrowMaps {
+  CUtensorMap x, g, out;  // boxes of 128 bytes x 128 rows, swizzled; out is y or dx
+};
+
+// Warps that take rows out of TMEM.  So many hide its latency and that of the exponentials
+// (with eight, bf16 1,048,576 x 64 x 64 forward 127 us, backward 482).
+constexpr int kRowWarps = 16;
 
 template <typename T, int THREADS>
 __device__ __forceinline__ void stage_bias(float* to, const GatedNarrowArgs& p) {
@@ -221,32 +180,72 @@ __device__ __forceinline__ void stage_bias(float* to, const GatedNarrowArgs& p) 
 }
 
 // Eight values of the staged bias.
-__device__ __forceinline__ void add_bias(float (&v)[8], const float* bias) {
+__device__ __forceinline__ void add_bias(float2 (&v)[4], const float* bias) {
   const float4 a = *reinterpret_cast<const float4*>(bias);
   const float4 b = *reinterpret_cast<const float4*>(bias + 4);
-  v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
-  v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+  v[0] = __fadd2_rn(v[0], make_float2(a.x, a.y));
+  v[1] = __fadd2_rn(v[1], make_float2(a.z, a.w));
+  v[2] = __fadd2_rn(v[2], make_float2(b.x, b.y));
+  v[3] = __fadd2_rn(v[3], make_float2(b.z, b.w));
 }
 
+// One thread: what the row warps staged leaves for memory, tile after tile.  `groups` of them
+// take tiles in turn, and each has a barrier that tells when its tile's boxes were read.
+template <typename T, int BUFFERS, int GROUPS>
+__device__ __forceinline__ void send_tiles(const unsigned char* boxes, const CUtensorMap* map,
+                                           int width, uint64_t* staged, uint64_t* stage_free,
+                                           int tiles) {
+  uint32_t it = 0;
+  for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++it) {
+    const uint32_t b = it % BUFFERS;
+    if (!mbar_wait_idle(&staged[b], (it / BUFFERS) & 1, kCodeProducer)) break;
+    for (int c = 0; c < width; c += 128 / static_cast<int>(sizeof(T)))
+      tma_store_2d(boxes + b * kGatedBlock + boxed<T>(0, c), map, c, t * kNarrowTile);
+    tma_store_wait_read();
+    mbar_arrive(&stage_free[it % GROUPS]);
+  }
+}
+
+// ------------------------------------------------------------------------- forward
+
+// Row warps, eight producers that cut float32 x (16-bit x arrives as the MMA reads it), and
+// the MMA, load and store warps.
+constexpr int kGatedProducerWarps = 8;
+constexpr int kForwardMmaWarp = kRowWarps + kGatedProducerWarps, kForwardLoadWarp = kForwardMmaWarp + 1,
+              kForwardStoreWarp = kForwardMmaWarp + 2;
+constexpr int kGatedForwardThreads = 28 * 32;
+constexpr int kGatedForwardSlices = 6;
+template <typename T>
+constexpr int kLeaving = kCut<T> == 3 ? 1 : 2;  // buffers of y
+template <typename T>
+constexpr size_t kGatedForwardSmem =
+    1024 + 3 * kGatedOperand<T> + 2 * kGatedBlock +
+    (kCut<T> == 3 ? kGatedForwardSlices * kSliceX<T> : 0) + kGatedRows * 4 + 256;
+
 template <typename T, int ACT>
-__global__ void __launch_bounds__(kGatedThreads, 1)
-    gated_narrow_forward_kernel(const __grid_constant__ GatedNarrowArgs p) {
+__global__ void __launch_bounds__(kGatedForwardThreads, 1)
+    gated_narrow_forward_kernel(const __grid_constant__ GatedNarrowMaps maps,
+                                const __grid_constant__ GatedNarrowArgs p) {
   constexpr int P = kCut<T>, R = kGatedForwardSlices;
-  constexpr uint32_t kSet = (P == 3 ? 2 : 1) * kGatedRows;
+  constexpr bool kWide = P == 3;
+  constexpr uint32_t kSet = (kWide ? 2 : 1) * kGatedRows;
   extern __shared__ unsigned char raw_smem[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t{1023});
   unsigned char* weights = smem;
   unsigned char* tiles = weights + kGatedOperand<T>;
-  unsigned char* slices = tiles + 2 * kGatedOperand<T>;
-  float* bias = reinterpret_cast<float*>(slices + R * kSliceX<T>);
+  unsigned char* leaving = tiles + 2 * kGatedOperand<T>;
+  unsigned char* slices = leaving + 2 * kGatedBlock;  // float32
+  float* bias = reinterpret_cast<float*>(slices + (kWide ? R * kSliceX<T> : 0));
   uint64_t* raw_full = reinterpret_cast<uint64_t*>(bias + kGatedRows);
   uint64_t* raw_empty = raw_full + R;
   uint64_t* full = raw_empty + R;
   uint64_t* empty = full + 2;
   uint64_t* done = empty + 2;
   uint64_t* room = done + 2;
-  uint64_t* drain = room + 2;
+  uint64_t* staged = room + 2;
+  uint64_t* stage_free = staged + 2;
+  uint64_t* drain = stage_free + 2;
   uint32_t* tmem_at = reinterpret_cast<uint32_t*>(drain + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -256,31 +255,62 @@ __global__ void __launch_bounds__(kGatedThreads, 1)
       mbar_init(&raw_empty[i], kGatedProducerWarps);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&full[i], kGatedProducerWarps);
+      mbar_init(&full[i], kWide ? kGatedProducerWarps : 1);
       mbar_init(&empty[i], 1);
       mbar_init(&done[i], 1);
       mbar_init(&room[i], kRowWarps / 2);
+      mbar_init(&staged[i], kRowWarps / 2);
+      mbar_init(&stage_free[i], 1);
     }
     mbar_init(drain, 1);
     fence_mbarrier_init();
   }
   if (warp == 0) tmem_alloc(tmem_at, 2 * kSet);
-  load_gated_weights<T, kGatedThreads>(weights, p);
-  stage_bias<T, kGatedThreads>(bias, p);
+  load_gated_weights<T, kGatedForwardThreads>(weights, p);
+  stage_bias<T, kGatedForwardThreads>(bias, p);
   fence_proxy_async();
   tcgen05_fence_before();
   __syncthreads();
   tcgen05_fence_after();
   const uint32_t tmem = *tmem_at;
+  const int first = static_cast<int>(blockIdx.x), step = static_cast<int>(gridDim.x);
 
-  if (warp == kGatedCopyWarp) {
-    if (lane == 0) copy_slices<T, R>(slices, raw_full, raw_empty, p);
+  if (warp == kForwardLoadWarp) {
+    if (lane == 0) {
+      bool ok = true;
+      if constexpr (kWide) {
+        const T* x = static_cast<const T*>(p.x);
+        SliceWalk at{first, 0, p.tiles, step, p.m};
+        for (uint32_t n = 0; !at.done(); at.next(), ++n) {
+          const int slot = n % R;
+          ok = mbar_wait_idle(&raw_empty[slot], ((n / R) & 1) ^ 1, kCodeProducer);
+          if (!ok) break;
+          const uint32_t bytes = slice_bytes<T>(p.k, at.rows());
+          mbar_arrive_expect_tx(&raw_full[slot], bytes);
+          bulk_g2s(slices + slot * kSliceX<T>, x + at.row() * p.k, bytes, &raw_full[slot]);
+        }
+      } else {
+        uint32_t it = 0;
+        for (int t = first; t < p.tiles; t += step, ++it) {
+          const int s = it & 1;
+          ok = mbar_wait_idle(&empty[s], ((it >> 1) & 1) ^ 1, kCodeProducer);
+          if (!ok) break;
+          mbar_arrive_expect_tx(&full[s], kGatedBlock);
+          tma_load_2d(tiles + s * kGatedBlock, &maps.x, 0, t * kNarrowTile, &full[s]);
+        }
+      }
+      if (!ok) settle_copies();
+    }
     __syncwarp();
-  } else if (warp == kGatedMmaWarp) {
+  } else if (warp == kForwardStoreWarp) {
+    if (lane == 0)
+      send_tiles<T, kLeaving<T>, 2>(leaving, &maps.out, p.n, staged, stage_free, p.tiles);
+    __syncwarp();
+  } else if (warp == kForwardMmaWarp) {
     if (lane == 0) {
       bool ok = true;
       uint32_t it = 0;
-      for (int t = blockIdx.x; t < p.tiles; t += gridDim.x, ++it) {
+      for (int t = first; t < p.tiles; t += step, ++it) {
         const int s = it & 1;
         ok = mbar_wait_idle(&room[s], ((it >> 1) & 1) ^ 1, kCodeMma) &&
              mbar_wait_idle(&full[s], (it >> 1) & 1, kCodeMma);
@@ -297,15 +327,44 @@ __global__ void __launch_bounds__(kGatedThreads, 1)
       }
     }
     __syncwarp();
-  } else if (warp >= kRowWarps && warp < kGatedMmaWarp) {
-    const int tid = threadIdx.x - kRowWarps * 32;
-    uint32_t it = 0, n = 0;  // tiles and slices so far
-    for (int t = blockIdx.x; t < p.tiles; t += gridDim.x, ++it) {
+  } else if (kWide && warp >= kRowWarps && warp < kForwardMmaWarp) {
+    const int tid = threadIdx.x - kRowWarps * 32, unit = tid & 15, r0 = tid >> 4;
+    const int columns = (p.k + 15) & ~15;  // that the MMAs read
+    uint32_t it = 0, n = 0;                // tiles and slices so far
+    bool ok = true;
+    for (int t = first; ok && t < p.tiles; t += step, ++it) {
       const int s = it & 1;
-      if (!mbar_wait_warp(&empty[s], ((it >> 1) & 1) ^ 1, kCodeProducer) ||
-          !fill_x_tile<T, R>(tiles + s * kGatedOperand<T>, slices, raw_full, raw_empty, t, p, tid,
-                             lane, n))
-        break;
+      ok = mbar_wait_warp(&empty[s], ((it >> 1) & 1) ^ 1, kCodeProducer);
+      unsigned char* tile = tiles + s * kGatedOperand<T>;
+      SliceWalk at{t, 0, p.tiles, step, p.m};
+#pragma unroll 1
+      for (int q = 0; ok && q < kNarrowTile / kSliceRows; ++q, ++at.slice) {
+        Slice<T> slice{nullptr, nullptr, p.k, 0, 0};
+        const bool some = at.row() < p.m;
+        const int slot = n % R;
+        if (some) {
+          ok = mbar_wait_warp(&raw_full[slot], (n / R) & 1, kCodeProducer);
+          if (!ok) break;
+          slice.raw = reinterpret_cast<const T*>(slices + slot * kSliceX<T>);
+          slice.rows = at.rows();
+        }
+        float v[2][4];
+        uint32_t seen = 0;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          read_unit<true>(slice, r0 + 16 * j, unit, v[j]);
+          seen |= unit_bits<true>(v[j]);
+        }
+        if (4 * unit < columns)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            store_unit<T>(tile, kGatedBlock, q * kSliceRows + r0 + 16 * j, unit, v[j]);
+        if (some) {
+          release_slot(&raw_empty[slot], seen, lane);
+          ++n;
+        }
+      }
+      if (!ok) break;
       fence_proxy_async();
       __syncwarp();
       if (lane == 0) mbar_arrive(&full[s]);
@@ -313,18 +372,25 @@ __global__ void __launch_bounds__(kGatedThreads, 1)
   } else if (warp < kRowWarps) {
     // eight warps for each of the two sets, every other tile: rows of a quad, half the columns
     const int quad = warp & 3, half = (warp >> 2) & 1, s = warp >> 3;
-    T* y = static_cast<T*>(p.e.out);
+    constexpr int L = kLeaving<T>;
     uint32_t it = 0;
-    for (int t = blockIdx.x + s * gridDim.x; t < p.tiles; t += 2 * gridDim.x, ++it) {
-      const int64_t row = static_cast<int64_t>(t) * kNarrowTile + quad * 32 + lane;
-      if (!mbar_wait_warp(&done[s], it & 1, kCodeEpilogue)) break;
+    for (int t = first + s * step; t < p.tiles; t += 2 * step, ++it) {
+      const uint32_t tile = 2 * it + s;  // of the CTA's
+      unsigned char* boxes = leaving + (tile % L) * kGatedBlock;
+      // the boxes were last those of tile - L.  One barrier for both groups would not do: a
+      // group can come back two tiles later, when its phase looks like the one before.
+      const uint32_t last = tile + 2 - L;  // + 2, which keeps parities
+      if (!mbar_wait_warp(&done[s], it & 1, kCodeEpilogue) ||
+          !mbar_wait_warp(&stage_free[last & 1], ((last >> 1) & 1) ^ 1, kCodeEpilogue))
+        break;
       tcgen05_fence_after();
       const uint32_t at = tmem + s * kSet + (static_cast<uint32_t>(quad * 32) << 16) + half * 32;
 #pragma unroll
       for (int j = 0; j < 32; j += 8) {
         const int col = half * 32 + j;
-        float gate[8], up[8];
-        take_p<P>(at + j, gate, up);
+        float2 gate[4], up[4];
+        take8<P>(at + j, kGatedRows, gate);
+        take8<P>(at + kNarrow + j, kGatedRows, up);
         if (j == 24) {
           tcgen05_fence_before();
           __syncwarp();
@@ -333,9 +399,16 @@ __global__ void __launch_bounds__(kGatedThreads, 1)
         add_bias(gate, bias + col);
         add_bias(up, bias + kNarrow + col);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) up[i] *= activate<ACT>(gate[i]);
-        if (row < p.m && col < p.n) store_columns(y + row * p.n + col, up, p.n - col, p.e.vec);
+        for (int i = 0; i < 4; ++i) {
+          float2 a, slope;
+          gate_pair<ACT>(gate[i], &a, &slope);
+          up[i] = __fmul2_rn(up[i], a);
+        }
+        store_boxed<T>(boxes, quad * 32 + lane, col, up);
       }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&staged[tile % L]);
     }
   }
   tcgen05_fence_before();
@@ -364,10 +437,6 @@ constexpr int kBackLaunchRegisters = 96;  // 65,536 / 640, in steps of 8
 constexpr int kRowRegisters = 104, kIssueRegisters = 64;
 static_assert(kRowWarps * kRowRegisters + 4 * kIssueRegisters <= 20 * kBackLaunchRegisters);
 
-struct alignas(64) GatedNarrowMaps {
-  CUtensorMap x, g, dx;  // boxes of 128 bytes x 128 rows, swizzled; x in 16-bit types only
-};
-
 template <typename T>
 constexpr int kBackBuffers = kCut<T> == 3 ? 1 : 2;  // of x, D, and (16-bit) g and p
 // Bytes of the raw x tile, or of two g tiles and the dx that leaves
@@ -379,11 +448,11 @@ constexpr size_t kGatedBackwardSmem =
 
 // Eight columns of D to their tile, part by part.
 template <typename T>
-__device__ __forceinline__ void store_d(unsigned char* at, const float (&v)[8]) {
+__device__ __forceinline__ void store_d(unsigned char* at, const float2 (&v)[4]) {
   if constexpr (kCut<T> == 3) {
     uint32_t part[4][3];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) cut_pair(v[2 * j], v[2 * j + 1], part[j]);
+    for (int j = 0; j < 4; ++j) cut_pair(v[j].x, v[j].y, part[j]);
 #pragma unroll
     for (int q = 0; q < 3; ++q)
       *reinterpret_cast<uint4*>(at + q * 2 * kGatedBlock) =
@@ -391,7 +460,10 @@ __device__ __forceinline__ void store_d(unsigned char* at, const float (&v)[8]) 
   } else {
     Pack<T, 8> o;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) o.v[j] = from_float<T>(v[j]);
+    for (int j = 0; j < 4; ++j) {
+      o.v[2 * j] = from_float<T>(v[j].x);
+      o.v[2 * j + 1] = from_float<T>(v[j].y);
+    }
     *reinterpret_cast<Pack<T, 8>*>(at) = o;
   }
 }
@@ -412,27 +484,23 @@ __device__ __forceinline__ void issue_orders(uint32_t d, uint64_t a, uint64_t a_
   }
 }
 
-// 16 columns of such a product.
+// Eight columns of such a product.
 template <int P>
-__device__ __forceinline__ void take_orders(uint32_t at, float (&v)[16]) {
-  tmem_load16(at, v);
+__device__ __forceinline__ void take_orders(uint32_t at, float2 (&v)[4]) {
+  float w[8];
+  tmem_load8(at, w);
   if constexpr (P == 3) {
-    float y[16], z[16];
-    tmem_load16(at + kNarrow, y);
-    tmem_load16(at + 2 * kNarrow, z);
+    float y[8], z[8];
+    tmem_load8(at + kNarrow, y);
+    tmem_load8(at + 2 * kNarrow, z);
     tmem_load_wait();
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = join_parts(v[i], y[i] + z[i]);
+    for (int i = 0; i < 8; ++i) w[i] = join_parts(w[i], y[i] + z[i]);
   } else {
     tmem_load_wait();
   }
-}
-
-// Where 16 bytes of column `col` of a row lie in swizzled boxes of 128 bytes x 128 rows.
-template <typename T>
-__device__ __forceinline__ uint32_t boxed(int row, int col) {
-  constexpr int kWidth = 128 / sizeof(T), V = 16 / sizeof(T);
-  return (col / kWidth) * kGatedBlock + swizzled(row, (col % kWidth) / V);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = make_float2(w[2 * i], w[2 * i + 1]);
 }
 
 template <typename T, int ACT>
@@ -548,16 +616,8 @@ __global__ void __launch_bounds__(kBackThreads, 1)
       }
       if (!ok) settle_copies();
     }
-    if (warp == kBackStoreWarp && lane == 0 && want_dx) {
-      uint32_t it = 0;
-      for (int t = first; t < p.tiles; t += step, ++it) {
-        if (!mbar_wait_idle(staged, it & 1, kCodeProducer)) break;
-        for (int c = 0; c < p.k; c += 128 / static_cast<int>(sizeof(T)))
-          tma_store_2d(leaving + boxed<T>(0, c), &maps.dx, c, t * kNarrowTile);
-        tma_store_wait_read();
-        mbar_arrive(stage_free);
-      }
-    }
+    if (warp == kBackStoreWarp && lane == 0 && want_dx)
+      send_tiles<T, 1, 1>(leaving, &maps.out, p.k, staged, stage_free, p.tiles);
     if (warp == kBackMmaWarp && lane == 0) {
       constexpr bool kBf16 = !std::is_same_v<T, __half>;
       const uint32_t wa = smem_addr(weights);
@@ -566,7 +626,6 @@ __global__ void __launch_bounds__(kBackThreads, 1)
       constexpr uint64_t kXp = kGatedBlock / 16, kDp = 2 * kXp;
       const int steps = (p.n + 15) / 16, dx_steps = want_dx ? 2 * steps : 0;
       const int dw_steps = want_dw ? kNarrowTile / 16 : 0;
-      const int most = dx_steps > dw_steps ? dx_steps : dw_steps;
       bool ok = true;
       uint32_t it = 0;
       const auto form_p = [&](uint32_t i) {
@@ -597,19 +656,23 @@ __global__ void __launch_bounds__(kBackThreads, 1)
         const uint64_t x_columns = matrix_descriptor(xa, kGatedBlock, 1024);
         const uint64_t d_rows = matrix_descriptor(da, 0, 1024);               // K-major
         const uint64_t d_columns = matrix_descriptor(da, kGatedBlock, 1024);  // two blocks
+        const auto add_dx = [&](int s) {  // 64 columns of D and rows of W a half
+          const int h = s >= steps, q = s - h * steps;
+          issue_orders<P>(tmem + kDx + b * kDxSet, d_rows + h * kXp + 2 * q, kDp,
+                          w_columns + h * 512 + 128 * q, kBf16, false, true, s > 0);
+        };
+        // x is free after dW: the last steps of dx run while it is filled again
+        int s = 0;
 #pragma unroll 1
-        for (int s = 0; s < most; ++s) {
-          if (s < dw_steps)
-            issue_orders<P>(tmem + kDw, d_columns + 128 * s, kDp, x_columns + 128 * s, kBf16, true,
-                            true, !opens || s > 0);
-          if (s < dx_steps) {  // 64 columns of D and rows of W a half
-            const int h = s >= steps, q = s - h * steps;
-            issue_orders<P>(tmem + kDx + b * kDxSet, d_rows + h * kXp + 2 * q, kDp,
-                            w_columns + h * 512 + 128 * q, kBf16, false, true, s > 0);
-          }
+        for (int i = 0; i < dw_steps; ++i) {
+          issue_orders<P>(tmem + kDw, d_columns + 128 * i, kDp, x_columns + 128 * i, kBf16, true,
+                          true, !opens || i > 0);
+          if ((!kWide || i % 2 == 1) && s < dx_steps) add_dx(s++);
         }
-        if (want_dw && closes_group(t, it)) mma_commit(dw_done);
         mma_commit(&x_empty[b]);
+#pragma unroll 1
+        for (; s < dx_steps; ++s) add_dx(s);
+        if (want_dw && closes_group(t, it)) mma_commit(dw_done);
         if (want_dx) mma_commit(&dx_done[b]);
         mma_commit(&d_empty[b]);
       }
@@ -629,11 +692,9 @@ __global__ void __launch_bounds__(kBackThreads, 1)
     constexpr int V = 16 / sizeof(T);
     const int quad = warp & 3, c0 = (warp >> 2) * 16, in_tile = quad * 32 + lane;
     const uint32_t at = tmem + (static_cast<uint32_t>(quad * 32) << 16) + c0;
-    // sums of db over the rows of lanes l and l + 16: the gate's in the one, the other's in
-    // the other
-    float db[16], dw[16];
+    float2 db[2][8], dw[8];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) db[i] = dw[i] = 0.f;
+    for (int i = 0; i < 8; ++i) db[0][i] = db[1][i] = dw[i] = make_float2(0.f, 0.f);
     bool ok = true;
 
     // float32: the next tile's x, cut
@@ -670,36 +731,32 @@ __global__ void __launch_bounds__(kBackThreads, 1)
         ok = mbar_wait_warp(dw_done, (it / kDwTiles) & 1, kCodeEpilogue);
         if (!ok) return;
         tcgen05_fence_after();
-        float sum[16];
-        take_orders<P>(at + kDw, sum);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float2 sum[4];
+          take_orders<P>(at + kDw + 8 * j, sum);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) dw[4 * j + i] = __fadd2_rn(dw[4 * j + i], sum[i]);
+        }
         tcgen05_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(dw_room);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) dw[i] += sum[i];
       }
-      float sum[16];
-      if (want_dx) {
-        ok = mbar_wait_warp(&dx_done[b], phase, kCodeEpilogue);
-        if (!ok) return;
-        tcgen05_fence_after();
-        take_orders<P>(at + kDx + b * kDxSet, sum);
-        tcgen05_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&dx_room[b]);
-      }
-      if (kWide && t + step < p.tiles) fill_x(t + step, it + 1);
-      if (!ok || !want_dx) return;
-      if (!kWide) {
-        ok = mbar_wait_warp(stage_free, (it & 1) ^ 1, kCodeEpilogue);
-        if (!ok) return;
-      }
+      if (!want_dx) return;
+      ok = mbar_wait_warp(&dx_done[b], phase, kCodeEpilogue);
+      if (ok && !kWide) ok = mbar_wait_warp(stage_free, (it & 1) ^ 1, kCodeEpilogue);
+      if (!ok) return;
+      tcgen05_fence_after();
 #pragma unroll
-      for (int i = 0; i < 16; i += V) {
-        Pack<T, V> o;
-#pragma unroll
-        for (int j = 0; j < V; ++j) o.v[j] = from_float<T>(sum[i + j]);
-        *reinterpret_cast<Pack<T, V>*>(leaving + boxed<T>(in_tile, c0 + i)) = o;
+      for (int j = 0; j < 16; j += 8) {
+        float2 sum[4];
+        take_orders<P>(at + kDx + b * kDxSet + j, sum);
+        if (j == 8) {
+          tcgen05_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&dx_room[b]);
+        }
+        store_boxed<T>(leaving, in_tile, c0 + j, sum);
       }
       fence_proxy_async();
       __syncwarp();
@@ -713,7 +770,7 @@ __global__ void __launch_bounds__(kBackThreads, 1)
       const bool in = static_cast<int64_t>(t) * kNarrowTile + in_tile < p.m;
       ok = mbar_wait_warp(&g_full[b], phase, kCodeEpilogue);
       if (!ok) break;
-      float g[16];
+      Pack<T, V> g[16 / V];
       uint32_t seen = 0;
 #pragma unroll
       for (int i = 0; i < 16; i += V) {
@@ -722,9 +779,7 @@ __global__ void __launch_bounds__(kBackThreads, 1)
                      : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3])
                      : "r"(smem_addr(g_tiles + b * kGatedBlock + boxed<T>(in_tile, c0 + i)))
                      : "memory");
-        const Pack<T, V>& pk = *reinterpret_cast<const Pack<T, V>*>(q);
-#pragma unroll
-        for (int j = 0; j < V; ++j) g[i + j] = to_float(pk.v[j]);
+        g[i / V] = *reinterpret_cast<const Pack<T, V>*>(q);
         seen |= q[0];
       }
       release_slot(&g_read[b], seen, lane);
@@ -736,10 +791,12 @@ __global__ void __launch_bounds__(kBackThreads, 1)
       if (!ok) break;
       tcgen05_fence_after();
       unsigned char* d_row = d_tiles + b * 2 * kGatedOperand<T> + in_tile * 128;
+      const bool whole = static_cast<int64_t>(t + 1) * kNarrowTile <= p.m;
 #pragma unroll
       for (int j = 0; j < 16; j += 8) {
-        float gate[8], up[8];
-        take_p<P>(at + b * kPset + j, gate, up);
+        float2 gate[4], up[4];
+        take8<P>(at + b * kPset + j, kGatedRows, gate);
+        take8<P>(at + b * kPset + kNarrow + j, kGatedRows, up);
         if (j == 8) {
           tcgen05_fence_before();
           __syncwarp();
@@ -749,15 +806,21 @@ __global__ void __launch_bounds__(kBackThreads, 1)
         if (c0 + j >= ((p.n + 15) & ~15)) continue;
         add_bias(gate, bias + c0 + j);
         add_bias(up, bias + kNarrow + c0 + j);
+        if (!whole && !in) {  // no gradient past the last row, but a bias that may be infinite
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float v = g[j + i], pg = gate[i], pu = up[i];
-          // rows past the last have no gradient, but a bias that may be infinite
-          gate[i] = in ? v * pu * activation_slope<ACT>(pg) : 0.f;
-          up[i] = in ? v * activate<ACT>(pg) : 0.f;
-          const bool low = lane < 16;
-          const float other = __shfl_xor_sync(0xffffffffu, low ? up[i] : gate[i], 16);
-          db[j + i] += (low ? gate[i] : up[i]) + other;
+          for (int i = 0; i < 4; ++i) gate[i] = up[i] = make_float2(0.f, 0.f);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int at_g = j + 2 * i;
+          const float2 v = make_float2(to_float(g[at_g / V].v[at_g % V]),
+                                       to_float(g[(at_g + 1) / V].v[(at_g + 1) % V]));
+          float2 a, slope;
+          gate_pair<ACT>(gate[i], &a, &slope);
+          gate[i] = __fmul2_rn(__fmul2_rn(v, up[i]), slope);
+          up[i] = __fmul2_rn(v, a);
+          db[0][j / 2 + i] = __fadd2_rn(db[0][j / 2 + i], gate[i]);
+          db[1][j / 2 + i] = __fadd2_rn(db[1][j / 2 + i], up[i]);
         }
         unsigned char* to = d_row + ((((c0 + j) / 8) ^ (in_tile & 7)) << 4);
         store_d<T>(to, gate);
@@ -766,8 +829,12 @@ __global__ void __launch_bounds__(kBackThreads, 1)
       fence_proxy_async();
       __syncwarp();
       if (lane == 0) mbar_arrive(&d_full[b]);
-      if (!kLag) take_tile(t, it);
-      else if (it > 0) take_tile(t - step, it - 1);
+      if (kLag) {
+        if (it > 0) take_tile(t - step, it - 1);
+      } else {
+        if (t + step < p.tiles) fill_x(t + step, it + 1);
+        if (ok) take_tile(t, it);
+      }
     }
     if (kLag && ok && it > 0)
       take_tile(first + static_cast<int>(it - 1) * step, it - 1);
@@ -775,20 +842,22 @@ __global__ void __launch_bounds__(kBackThreads, 1)
       // every product is done: x's tile has room for the sums of db
       float* sums = reinterpret_cast<float*>(x_tiles) + warp * 32;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float v = db[i];
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int s = 8; s > 0; s >>= 1) v += __shfl_xor_sync(0xffffffffu, v, s);
-        if ((lane & 15) == 0) sums[lane + i] = v;
-      }
+        for (int i = 0; i < 16; ++i) {
+          float v = i % 2 ? db[h][i / 2].y : db[h][i / 2].x;
+#pragma unroll
+          for (int s = 16; s > 0; s >>= 1) v += __shfl_xor_sync(0xffffffffu, v, s);
+          if (lane == 0) sums[h * 16 + i] = v;
+        }
       const int column = in_tile & (kNarrow - 1);  // of D, in its half
       float* to = partial + ((in_tile >= kNarrow ? p.n : 0) + column) * p.k + c0;
       if (column < p.n)
 #pragma unroll
-        for (int i = 0; i < 16; i += 4)
-          if (c0 + i < p.k)
-            *reinterpret_cast<float4*>(to + i) =
-                make_float4(dw[i], dw[i + 1], dw[i + 2], dw[i + 3]);
+        for (int i = 0; i < 4; ++i)
+          if (c0 + 4 * i < p.k)
+            *reinterpret_cast<float4*>(to + 4 * i) =
+                make_float4(dw[2 * i].x, dw[2 * i].y, dw[2 * i + 1].x, dw[2 * i + 1].y);
     }
   }
   tcgen05_fence_before();

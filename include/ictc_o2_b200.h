@@ -383,8 +383,9 @@ ICTC_API int32_t ictc_o2_gated_linear_workspace(int64_t rows, int64_t in, int64_
                                                 size_t* forward_bytes, size_t* backward_bytes);
 
 /* Whether preact saves the backward anything: 0 for contiguous layers of at most 64 inputs
- * and 64 outputs in whole 16-byte blocks, whose backward is faster without it (and then needs
- * a contiguous grad_output, and it and grad_x 16-byte aligned), 1 otherwise. */
+ * and 64 outputs in whole 16-byte blocks, whose backward is faster without it, 1 otherwise.
+ * Calls of the former without preact need y, grad_output (contiguous) and grad_x aligned to 16
+ * bytes. */
 ICTC_API int32_t ictc_o2_gated_linear_keeps(int64_t rows, int64_t in, int64_t hidden,
                                             int32_t dtype, int32_t layout);
 
