@@ -79,19 +79,24 @@ __global__ void __launch_bounds__(256) gate_kernel(const float* parts, int split
 }
 
 // ---------------------------------------------------------------- few rows: no tiles
-// Up to four rows: W is read once and the products run on the FMA pipes.  `share` warps have
-// one column of y, each a part of K; a lane reads V consecutive elements of both rows of W, and
-// the warps' sums are added in warp order.
+// Blocks of up to four rows (blockIdx.y): W is read once a block and the products run on the
+// FMA pipes.  `share` warps have one column of y, each a part of K; a lane reads V consecutive
+// elements of both rows of W, and the warps' sums are added in warp order.
 constexpr int kFewThreads = 256, kFewWarps = kFewThreads / 32;
 constexpr int64_t kFewRows = 4;
 
 template <typename T, int ROWS, int V>
 __global__ void __launch_bounds__(kFewThreads) few_kernel(
     const T* __restrict__ x, int64_t ldx, const T* __restrict__ w, int64_t ldw, int64_t rows,
-    int64_t n, int64_t k, int share, const Epilogue e) {
+    int64_t n, int64_t k, int share, Epilogue e) {
   __shared__ float sums[kFewWarps][2 * ROWS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int per_cta = kFewWarps / share, part = warp % share;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.y) * ROWS;
+  x += row0 * ldx;
+  rows -= row0;
+  if (e.preact) e.preact += row0 * 2 * n;
+  T* y = static_cast<T*>(e.out) + row0 * n;
   for (int64_t base = static_cast<int64_t>(blockIdx.x) * per_cta; base < n;
        base += static_cast<int64_t>(gridDim.x) * per_cta) {
     const int64_t col = base + warp / share;
@@ -101,7 +106,7 @@ __global__ void __launch_bounds__(kFewThreads) few_kernel(
     if (col < n) {
       const T* wg = w + col * ldw;
       const T* wu = wg + n * ldw;
-#pragma unroll 4
+#pragma unroll 8
       for (int64_t c = (part * 32 + lane) * V; c < k; c += share * 32 * V) {
         const Pack<T, V> pg = *reinterpret_cast<const Pack<T, V>*>(wg + c);
         const Pack<T, V> pu = *reinterpret_cast<const Pack<T, V>*>(wu + c);
@@ -146,8 +151,7 @@ __global__ void __launch_bounds__(kFewThreads) few_kernel(
           e.preact[r * 2 * n + col] = pg;
           e.preact[r * 2 * n + n + col] = pu;
         }
-        static_cast<T*>(e.out)[r * n + col] =
-            from_float<T>(activate<kAnyActivation>(pg, e.activation) * pu);
+        y[r * n + col] = from_float<T>(activate<kAnyActivation>(pg, e.activation) * pu);
       }
     }
   }
@@ -231,6 +235,19 @@ int32_t layout_of(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_
   return flags;
 }
 
+// Products that the FMA pipes are through with before a tile's barriers, TMEM and tensor maps
+// are set up: a warp for each column of four rows, and few rounds of them.  Float32 37 x 64 x
+// 64 takes 3.6 us (narrow kernel 8.3), 256 x 64 x 64 6.1 (8.8), 512 x 64 x 64 8.8 (8.8), bf16 128
+// x 64 x 64 3.9 (5.8), 256 x 64 x 64 6.6 (5.8), 16 x 512 x 512 4.9 (7.9), unaligned 300 x 33 x 77
+// 6.1 (19.6 with the linear layer's kernels).
+bool is_small(int64_t m, int64_t n, int64_t k, size_t size, bool whole) {
+  const int64_t elements = whole ? 16 / static_cast<int64_t>(size) : 1;  // a lane's
+  const int64_t warps = ceil_div(m, kFewRows) * n;
+  return m <= 4096 && n <= 4096 && k <= 65536 &&
+         warps <= (!whole ? 8192 : size == 4 ? 4096 : 2048) &&
+         warps * ceil_div(k, 32 * elements) <= (whole ? 8192 : 16384);
+}
+
 // Layers whose backward computes p again at no cost of a pass (their g is contiguous too).
 bool is_narrow(int64_t m, int64_t n, int64_t k, int dtype, int32_t layout) {
   const int64_t full = static_cast<int64_t>(16 / dtype_size(dtype));
@@ -270,8 +287,12 @@ int plan_forward(int64_t m, int64_t n, int64_t k, int dtype, int32_t layout, boo
   const bool wide = dtype == ICTC_DTYPE_F32;
   Layout space;
   b->way = Way::general;
-  if (m <= kFewRows && ((rows_aligned && k % static_cast<int64_t>(16 / size) == 0) ||
-                        2 * n * k <= (1 << 18))) {
+  const bool whole = rows_aligned && k % static_cast<int64_t>(16 / size) == 0;
+  // three or four rows of 16 bits make more FMAs and conversions than the SM pairs' mostly empty
+  // tiles cost (4 x 4,096 x 16,384 90 us, pairs 64; 4 x 2,048 x 2,048 10, pairs 13)
+  const bool slow = size == 2 && m > 2 && n * k >= (1 << 24);
+  if ((m <= kFewRows && (whole ? !slow : 2 * n * k <= (1 << 18))) ||
+      is_small(m, n, k, size, whole)) {
     b->way = Way::few;
     return ICTC_OK;
   }
@@ -412,11 +433,16 @@ template <typename T, int V>
 int run_few(const T* x, int64_t ldx, const T* w, int64_t ldw, const Epilogue& e, int64_t m,
             int64_t n, int64_t k, cudaStream_t stream) {
   const int64_t sms = sm_count(current_device());
-  // all eight warps of a CTA share a column while that still gives every SM work
-  const int share = n <= sms * 8 ? kFewWarps : 1;
+  const int64_t blocks = ceil_div(m, kFewRows);
+  // warps of a CTA share a column where there are few, each with work for all of its lanes
+  int share = 1;
+  while (share < kFewWarps && n * blocks * share < sms * 8 && 2 * share * 32 * V <= k) share *= 2;
   const int64_t want = ceil_div(n, kFewWarps / share);
-  const unsigned grid = static_cast<unsigned>(want < sms * 8 ? want : sms * 8);
-  const auto kernel = m == 1 ? few_kernel<T, 1, V> : few_kernel<T, kFewRows, V>;
+  const dim3 grid(static_cast<unsigned>(want < sms * 8 ? want : sms * 8),
+                  static_cast<unsigned>(blocks));
+  const auto kernel = m == 1   ? few_kernel<T, 1, V>
+                      : m == 2 ? few_kernel<T, 2, V>
+                               : few_kernel<T, kFewRows, V>;
   kernel<<<grid, kFewThreads, 0, stream>>>(x, ldx, w, ldw, m, n, k, share, e);
   const cudaError_t err = cudaGetLastError();
   return err == cudaSuccess ? ICTC_OK : cuda_fail(err, "gated linear few-row launch");
