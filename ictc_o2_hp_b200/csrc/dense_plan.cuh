@@ -141,8 +141,8 @@ static __global__ void __launch_bounds__(256)
   }
 }
 
-inline int64_t aligned_pitch(int64_t width, size_t size) {
-  const int64_t v = static_cast<int64_t>(16 / size);
+inline int64_t aligned_pitch(int64_t width, size_t size, int64_t unit = 16) {
+  const int64_t v = unit / static_cast<int64_t>(size);
   return ceil_div(width, v) * v;
 }
 
@@ -152,12 +152,13 @@ inline bool worth_aligning(int64_t m, int64_t n, int64_t k) {
   return static_cast<double>(m) * n * k >= static_cast<double>(1 << 26);
 }
 
-// An operand with aligned rows: itself, or its copy in `space`.
+// An operand with aligned rows: itself, or its copy in `space`, whose rows are whole blocks of
+// `unit` bytes.
 template <typename T>
 static int align_operand(const T** p, int64_t* ld, int64_t rows, int64_t width,
-                         unsigned char* space, cudaStream_t stream) {
+                         unsigned char* space, cudaStream_t stream, int64_t unit = 16) {
   if (chunk_aligned(*p, *ld, sizeof(T))) return ICTC_OK;
-  const int64_t pitch = aligned_pitch(width, sizeof(T));
+  const int64_t pitch = aligned_pitch(width, sizeof(T), unit);
   T* to = reinterpret_cast<T*>(space);
   const int64_t blocks = ceil_div(rows * pitch * static_cast<int64_t>(sizeof(T)), 256 * 16);
   const int64_t cap = static_cast<int64_t>(sm_count(current_device())) * 8;
