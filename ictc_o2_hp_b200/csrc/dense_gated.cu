@@ -310,8 +310,10 @@ int plan_forward(int64_t m, int64_t n, int64_t k, int dtype, int32_t layout, boo
   }
   // a few columns of both halves together: the linear layer's FMA kernels read x once, in any
   // layout, where tiles would be mostly empty (float32 40,000 x 732 x 4 64 us, tiles 74; x 733
-  // 82, copied 110; aligned 16-bit tiles are as fast)
-  const bool thin = 2 * n <= kThin && k > kThin && (wide || !rows_aligned);
+  // 82, copied 110; aligned 16-bit tiles are as fast).  Likewise a few rows against weights off
+  // the boundaries, which are not worth a copy.
+  const bool thin =
+      (2 * n <= kThin && k > kThin && (wide || !rows_aligned)) || (m <= kThin && !rows_aligned);
   b->align = !thin && !rows_aligned && worth_aligning(m, 2 * n, k);
   if (!thin && (rows_aligned || b->align)) {
     int splits = 0;
