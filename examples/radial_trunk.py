@@ -2,10 +2,12 @@
 for a few steps on synthetic edges.
 
     python examples/radial_trunk.py [--edges N] [--hidden H] [--blocks B] [--steps S]
+                                    [--gated] [--clip M]
 
 Basis values go through ``RadialTrunk`` (linear layers with bias, SiLU and residual in
-their epilogues, layer norms between them) to the hidden features of
-``RadialUvuTensorProduct``, whose last affine layer is a ``Linear`` too.
+their epilogues, layer norms between them; with --gated blocks of ``GatedLinear``) to the
+hidden features of ``RadialUvuTensorProduct``, whose last affine layer is a ``Linear`` too.
+With --clip every step scales its gradients to a norm of at most M.
 """
 
 import argparse
@@ -16,7 +18,8 @@ import torch
 
 sys.path.insert(0, str(Path(__file__).resolve().parents[1]))
 
-from ictc_o2_hp_b200 import Linear, RadialTrunk, RadialUvuTensorProduct, UvuTensorProduct
+from ictc_o2_hp_b200 import (Linear, RadialTrunk, RadialUvuTensorProduct, UvuTensorProduct,
+                             clip_grad_norm_)
 
 
 def main() -> int:
@@ -25,6 +28,8 @@ def main() -> int:
     parser.add_argument("--hidden", type=int, default=64)
     parser.add_argument("--blocks", type=int, default=2)
     parser.add_argument("--steps", type=int, default=20)
+    parser.add_argument("--gated", action="store_true", help="gated blocks in the trunk")
+    parser.add_argument("--clip", type=float, default=None, help="largest norm of the gradients")
     args = parser.parse_args()
     if not torch.cuda.is_available():
         print("needs a CUDA device")
@@ -32,7 +37,7 @@ def main() -> int:
     device = torch.device("cuda")
     torch.manual_seed(0)
     tp = UvuTensorProduct(32, 1, 2, parity="full", parity_in2="canonical", shared_weights=False)
-    trunk = RadialTrunk(8, args.hidden, blocks=args.blocks).to(device)
+    trunk = RadialTrunk(8, args.hidden, blocks=args.blocks, gated=args.gated).to(device)
     product = RadialUvuTensorProduct(tp, Linear(args.hidden, tp.weight_numel)).to(device)
     basis = torch.randn(args.edges, 8, device=device)
     left = torch.randn(args.edges, tp.input1_dimension, device=device)
@@ -47,6 +52,8 @@ def main() -> int:
         loss = (product(left, angular, trunk(basis)) - target).square().mean()
         optimizer.zero_grad(set_to_none=True)
         loss.backward()
+        if args.clip is not None:
+            clip_grad_norm_(params, args.clip)
         optimizer.step()
         if step % 5 == 0:
             print(f"step {step:3d}  loss {loss.item():.6f}")

@@ -145,7 +145,9 @@ def test_strides_and_batches(k, n, dtype, cuda_device):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("shape", [(700001, 64, 64), (300007, 61, 59), (400003, 24, 40)])
+@pytest.mark.parametrize("shape", [(700001, 64, 64), (300007, 61, 59), (400003, 24, 40),
+                                   (900001, 8, 8), (500001, 64, 24), (500001, 40, 64),
+                                   (60001, 72, 136)])
 def test_many_tiles(shape, dtype, cuda_device):
     """Many tiles per CTA, run after run: a buffer that is written again while it is still
     read shows as another tile's rows, in a few rows of a million."""
@@ -160,6 +162,28 @@ def test_many_tiles(shape, dtype, cuda_device):
             check_gated(x, w, b, "silu", g, y, grads, dtype)
             check_gated(x, w, b, "silu", g, out[-1], None, dtype)
         assert all(torch.equal(p, q) for p, q in zip(out, first))
+
+
+def test_offsets_past_32_bits(cuda_device):
+    """p and D of more than 2^31 elements, y of more than 2^30: rows on both sides of such
+    offsets, the last ones, and the bias gradient over all."""
+    from ictc_o2_hp_b200 import dense
+    m, k, n = 140001, 16, 8192
+    x, w, b, _ = operands(1, k, n, torch.bfloat16, cuda_device, 75)
+    x = rand((m, k), torch.bfloat16, cuda_device, 76)
+    g = rand((1,), torch.bfloat16, cuda_device, 77).expand(m, n)
+    y, (dx, dw, db) = step(x, w, b, "silu", g)
+    for at in (0, 2 ** 31 // n - 150, 2 ** 31 // (2 * n) - 150, 2 ** 30 // n - 150, m - 300):
+        q = slice(at, at + 300)
+        check_gated(x[q], w, b, "silu", g[q], y[q], (dx[q], None, None), torch.bfloat16)
+    total = torch.zeros(2 * n, dtype=torch.float64, device=cuda_device)
+    size = torch.zeros_like(total)
+    for rows in x.split(10000):
+        d = gated64(rows, w, b, "silu", g[:len(rows)])[5]
+        total += d.sum(0)
+        size += d.abs().sum(0)
+    within("dbias", db, total, 1.01 * (m + 200) * U * size + 2 * UNIT[torch.bfloat16] * total.abs())
+    assert dw.isfinite().all()
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -387,6 +411,18 @@ def test_gated_trunk_feeds_the_radial_product(cuda_device):
         assert (p - q).norm() <= 1e-4 * q.norm()
 
 
+def test_example_runs(cuda_device):
+    import subprocess
+    import sys
+    from pathlib import Path
+    example = Path(__file__).resolve().parents[1] / "examples" / "radial_trunk.py"
+    run = subprocess.run([sys.executable, str(example), "--edges", "700", "--hidden", "32",
+                          "--steps", "3", "--gated", "--clip", "0.5"], capture_output=True,
+                         text=True, timeout=300)
+    assert run.returncode == 0, run.stderr
+    assert "700 edges" in run.stdout
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("shape", [(3, 96, 64), (20, 512, 64), (200, 96, 64), (2000, 64, 64)])
 def test_other_stream_and_graph_capture(shape, dtype, cuda_device):
@@ -466,6 +502,19 @@ def test_views_with_a_negative_bit(cuda_device):
     assert x.is_neg()
     w = rand((6, 1), torch.float32, cuda_device, 38)
     assert torch.equal(dense.gated_linear(x, w), dense.gated_linear(x.resolve_neg(), w))
+
+
+def test_changed_operands_are_noticed(cuda_device):
+    """A backward that would compute p again from other values refuses."""
+    from ictc_o2_hp_b200 import dense
+    x, w, b, g = operands(300, 64, 64, torch.float32, cuda_device, 130)
+    for i in range(3):
+        leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+        y = dense.gated_linear(*leaves)
+        with torch.no_grad():
+            leaves[i].add_(1)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(y, leaves, g)
 
 
 def test_refusals(cuda_device):

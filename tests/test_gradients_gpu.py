@@ -121,6 +121,27 @@ def test_range(scale, dtype, cuda_device):
         check_clipped(clipped, grads, want / 8)
 
 
+def test_offsets_past_32_bits(cuda_device):
+    """One tensor of more than 2^31 elements, a value past the end of 32 bits that decides."""
+    from ictc_o2_hp_b200 import gradients
+    n = 2 ** 31 + 100_003
+    big = torch.zeros(n, dtype=torch.bfloat16, device=cuda_device)
+    big[-3], big[5] = 3.0, 4.0
+    assert gradients.grad_norm([big]).item() == 5.0
+    assert gradients.grad_norm([big], math.inf).item() == 4.0
+    _, norm = gradients.clip_grads([big], 2.5, out=[big])
+    assert norm.item() == 5.0 and abs(big[-3].item() - 1.5) <= 1.5 * 2.0 ** -8
+    assert abs(big[5].item() - 2.0) <= 2.0 * 2.0 ** -8 and big.count_nonzero().item() == 2
+
+
+def test_a_single_tensor(cuda_device):
+    from ictc_o2_hp_b200 import gradients
+    g = rand((3, 50), torch.float32, cuda_device, 25)
+    check_norm(gradients.grad_norm(g), norm64([g]))
+    clipped, norm = gradients.clip_grads((t for t in [g]), 0.1)
+    check_clipped(clipped, [g], 0.1)
+
+
 def test_zeros(cuda_device):
     from ictc_o2_hp_b200 import gradients
     grads = [torch.zeros(100_000, dtype=t, device=cuda_device) for t in DTYPES]
