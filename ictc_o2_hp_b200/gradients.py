@@ -117,8 +117,9 @@ def clip_grads(grads: Sequence[Tensor], max_norm: float, norm_type: float = 2.0,
     """The gradients times min(1, max_norm / (norm + 1e-6)), and their norm.
 
     ``out``: tensors of the same shapes and types to write (flat buckets' views, say);
-    ``out=grads`` scales in place.  Without it new tensors are made.  An output may be its own
-    gradient, but share no memory with any other."""
+    ``out=grads`` scales in place.  Without it new tensors are made, parts of one allocation
+    (which lives as long as any of them).  An output may be its own gradient, but share no
+    memory with any other."""
     if not isinstance(grads, (list, tuple)):
         grads = list(grads)
     if out is not None and not isinstance(out, (list, tuple)):

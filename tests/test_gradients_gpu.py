@@ -134,6 +134,27 @@ def test_offsets_past_32_bits(cuda_device):
     assert abs(big[5].item() - 2.0) <= 2.0 * 2.0 ** -8 and big.count_nonzero().item() == 2
 
 
+def test_new_outputs_are_tensors_of_their_own(cuda_device):
+    """Parts of one allocation: aligned, apart, usable as leaves and in place."""
+    from ictc_o2_hp_b200 import gradients
+    grads = [rand((n,), t, cuda_device, 26) for n in (1, 7, 100, 0) for t in DTYPES]
+    grads.append(rand((5, 9), torch.float32, cuda_device, 27).t())
+    clipped, _ = gradients.clip_grads(grads, 0.1)
+    check_clipped(clipped, grads, 0.1)
+    assert clipped[-1].stride() == grads[-1].stride()
+    assert all(t.data_ptr() % 64 == 0 for t in clipped if t.numel())
+    before = [t.clone() for t in clipped]
+    clipped[2].add_(1)
+    clipped[2].requires_grad_(True)
+    (clipped[2].float() * 3).sum().backward()
+    assert torch.equal(clipped[2].grad, torch.full_like(before[2], 3.0))
+    assert all(torch.equal(a, b) for i, (a, b) in enumerate(zip(clipped, before)) if i != 2)
+    held = clipped[5]
+    del clipped
+    torch.empty(1 << 20, device=cuda_device).fill_(7.0)
+    assert torch.equal(held, before[5])
+
+
 def test_a_single_tensor(cuda_device):
     from ictc_o2_hp_b200 import gradients
     g = rand((3, 50), torch.float32, cuda_device, 25)
