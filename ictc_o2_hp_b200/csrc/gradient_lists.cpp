@@ -10,6 +10,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <optional>
 #include <string>
 #include <utility>
 #include <vector>
@@ -63,30 +64,35 @@ class Sequence {
   size_t size_;
 };
 
-// Whether a call on these tensors has to be seen by the dispatcher (a trace, fake tensors).
-bool watched(const Sequence& tensors) {
-  using K = c10::DispatchKey;
-  constexpr c10::DispatchKeySet kWatchers(
-      {K::Python, K::Tracer, K::Functionalize, K::FuncTorchDynamicLayerFrontMode,
-       K::FuncTorchBatched, K::FuncTorchGradWrapper});
-  const auto local = c10::impl::tls_local_dispatch_key_set();
-  c10::DispatchKeySet keys = local.included_;
-  for (size_t i = 0; i < tensors.size(); ++i) keys = keys | tensors[i].key_set();
-  return !((keys - local.excluded_) & kWatchers).empty();
-}
-
-void check_inputs(const char* what, const Sequence& tensors) {
-  const auto device = tensors[0].device();
-  for (size_t i = 0; i < tensors.size(); ++i) {
-    const Tensor& t = tensors[i];
-    const auto type = t.scalar_type();
-    TORCH_CHECK_TYPE(t.layout() == at::kStrided && t.is_cuda() &&
-                         (type == at::kFloat || type == at::kBFloat16 || type == at::kHalf),
-                     what, " takes dense CUDA float32, bfloat16 or float16 tensors; got ", type,
-                     " (", t.layout(), ") on ", t.device());
-    TORCH_CHECK_VALUE(t.device() == device, what, ": tensors are on ", device, " and ",
-                      t.device());
+// Which calls the dispatcher has to see (a trace, fake tensors).  Asked of each tensor just
+// before it is read, in the one pass over a list: a list of thousands does not stay in the
+// CPU's caches for a second.
+class Watch {
+ public:
+  Watch() {
+    const auto local = c10::impl::tls_local_dispatch_key_set();
+    watchers_ = c10::DispatchKeySet({K::Python, K::Tracer, K::Functionalize,
+                                     K::FuncTorchDynamicLayerFrontMode, K::FuncTorchBatched,
+                                     K::FuncTorchGradWrapper}) - local.excluded_;
+    everything_ = !(local.included_ & watchers_).empty();
   }
+  bool sees(const Tensor& t) const {
+    return everything_ || !(t.key_set() & watchers_).empty();
+  }
+
+ private:
+  using K = c10::DispatchKey;
+  c10::DispatchKeySet watchers_;
+  bool everything_;
+};
+
+void check_input(const char* what, const Tensor& t, c10::Device device) {
+  const auto type = t.scalar_type();
+  TORCH_CHECK_TYPE(t.layout() == at::kStrided && t.is_cuda() &&
+                       (type == at::kFloat || type == at::kBFloat16 || type == at::kHalf),
+                   what, " takes dense CUDA float32, bfloat16 or float16 tensors; got ", type,
+                   " (", t.layout(), ") on ", t.device());
+  TORCH_CHECK_VALUE(t.device() == device, what, ": tensors are on ", device, " and ", t.device());
 }
 
 // Whether the tensor's elements fill its memory, in whatever order of dimensions.
@@ -132,6 +138,10 @@ struct Space {
   }
 };
 
+std::optional<c10::Device> cuda_or_none(c10::Device device) {
+  return device.is_cuda() ? std::optional<c10::Device>(device) : std::nullopt;
+}
+
 void* stream_of(c10::Device device) {
   return c10::cuda::getCurrentCUDAStream(device.index()).stream();
 }
@@ -140,15 +150,18 @@ void* stream_of(c10::Device device) {
 py::object grad_norm(py::handle given, bool largest) {
   const Sequence tensors("grad_norm", given);
   TORCH_CHECK_VALUE(tensors.size() > 0, "grad_norm: no tensors");
-  if (watched(tensors)) return py::none();
-  check_inputs("grad_norm", tensors);
+  const Watch watch;
+  if (watch.sees(tensors[0])) return py::none();  // before its device is made current
   const auto device = tensors[0].device();
   const at::NoGradGuard no_grad;
-  const c10::cuda::CUDAGuard guard(device);
+  const c10::cuda::OptionalCUDAGuard guard(cuda_or_none(device));
   Lists lists(tensors.size());
   for (size_t i = 0; i < tensors.size(); ++i) {
-    if (dense(tensors[i])) lists.add(tensors[i]);
-    else lists.add_copy(tensors[i]);
+    const Tensor& t = tensors[i];
+    if (watch.sees(t)) return py::none();
+    check_input("grad_norm", t, device);
+    if (dense(t)) lists.add(t);
+    else lists.add_copy(t);
   }
   const Space s(lists.size(), device);
   check(api.norm(lists.in.data(), lists.counts.data(), lists.dtypes.data(), lists.size(),
@@ -164,23 +177,31 @@ void check_apart(const Lists& lists) {
   struct Range {
     uintptr_t begin, end;
   };
-  std::vector<Range> ranges;
-  ranges.reserve(2 * lists.in.size());
+  // outputs, and gradients that are none; lists come in the order of their memory as a rule
+  std::vector<Range> ranges[2];
+  for (auto& r : ranges) r.reserve(lists.in.size());
   for (size_t i = 0; i < lists.in.size(); ++i) {
     const uintptr_t bytes = static_cast<uintptr_t>(lists.counts[i]) *
                             (lists.dtypes[i] == ICTC_DTYPE_F32 ? 4 : 2);
     if (!bytes) continue;
     const auto out = reinterpret_cast<uintptr_t>(lists.out[i]);
     const auto in = reinterpret_cast<uintptr_t>(lists.in[i]);
-    ranges.push_back({out, out + bytes});
-    if (in != out) ranges.push_back({in, in + bytes});
+    ranges[0].push_back({out, out + bytes});
+    if (in != out) ranges[1].push_back({in, in + bytes});
   }
   const auto before = [](const Range& a, const Range& b) { return a.begin < b.begin; };
-  if (!std::is_sorted(ranges.begin(), ranges.end(), before))
-    std::sort(ranges.begin(), ranges.end(), before);
-  for (size_t i = 1; i < ranges.size(); ++i)
-    TORCH_CHECK_VALUE(ranges[i - 1].end <= ranges[i].begin,
+  for (auto& r : ranges)
+    if (!std::is_sorted(r.begin(), r.end(), before)) std::sort(r.begin(), r.end(), before);
+  // a gradient may share memory with another gradient, but an output with neither
+  uintptr_t out_end = 0, any_end = 0;
+  for (auto o = ranges[0].begin(), g = ranges[1].begin(); o != ranges[0].end() || g != ranges[1].end();) {
+    const bool is_out = g == ranges[1].end() || (o != ranges[0].end() && o->begin <= g->begin);
+    const Range r = is_out ? *o++ : *g++;
+    TORCH_CHECK_VALUE(r.begin >= (is_out ? any_end : out_end),
                       "clip_grads: gradients or outputs share memory; list each tensor once");
+    if (is_out) out_end = std::max(out_end, r.end);
+    any_end = std::max(any_end, r.end);
+  }
 }
 
 Tensor launch(const Lists& lists, c10::Device device, double max_norm, bool largest) {
@@ -192,14 +213,19 @@ Tensor launch(const Lists& lists, c10::Device device, double max_norm, bool larg
   return s.norm;
 }
 
-// Into the tensors of `out`.
-Tensor clip_into(const Sequence& grads, const Sequence& out, double max_norm, bool largest) {
+// Into the tensors of `out`; nothing where the dispatcher has to see the call.
+std::optional<Tensor> clip_into(const Sequence& grads, const Sequence& out, double max_norm,
+                                bool largest) {
   TORCH_CHECK_VALUE(out.size() == grads.size(), "clip_grads: ", grads.size(), " gradients and ",
                     out.size(), " outputs");
+  const auto device = grads[0].device();
+  const Watch watch;
   Lists lists(grads.size());
   std::vector<std::pair<size_t, Tensor>> apart;  // results that the kernels leave elsewhere
   for (size_t i = 0; i < grads.size(); ++i) {
     const Tensor &g = grads[i], &o = out[i];
+    if (watch.sees(g) || watch.sees(o)) return std::nullopt;
+    check_input("clip_grads", g, device);
     const bool one = g.is_same(o);
     if (!one) {
       TORCH_CHECK_VALUE(o.sizes() == g.sizes() && o.scalar_type() == g.scalar_type() &&
@@ -221,7 +247,7 @@ Tensor clip_into(const Sequence& grads, const Sequence& out, double max_norm, bo
     lists.out.push_back(g.numel() ? to.data_ptr() : nullptr);
   }
   check_apart(lists);
-  const Tensor norm = launch(lists, grads[0].device(), max_norm, largest);
+  const Tensor norm = launch(lists, device, max_norm, largest);
   size_t next = 0;
   for (size_t i = 0; i < out.size(); ++i) {
     if (next < apart.size() && apart[next].first == i) out[i].copy_(apart[next++].second);
@@ -261,16 +287,19 @@ py::object clip_grads(py::handle given, double max_norm, bool largest, py::handl
   const Sequence grads("clip_grads", given);
   TORCH_CHECK_VALUE(max_norm >= 0, "clip_grads: max_norm must be >= 0, got ", max_norm);
   TORCH_CHECK_VALUE(grads.size() > 0, "clip_grads: no tensors");
-  if (watched(grads)) return py::none();
-  check_inputs("clip_grads", grads);
+  const Watch watch;
+  if (watch.sees(grads[0])) return py::none();  // before its device is made current
   const auto device = grads[0].device();
   const at::NoGradGuard no_grad;
-  const c10::cuda::CUDAGuard guard(device);
+  const c10::cuda::OptionalCUDAGuard guard(cuda_or_none(device));
   if (!out.is_none()) {
     const Sequence to("clip_grads", out);
-    if (watched(to)) return py::none();
-    const Tensor norm = clip_into(grads, to, max_norm, largest);
-    return py::make_tuple(py::list(to.items()), norm);
+    const auto norm = clip_into(grads, to, max_norm, largest);
+    return norm ? py::object(py::make_tuple(py::list(to.items()), *norm)) : py::none();
+  }
+  for (size_t i = 0; i < grads.size(); ++i) {
+    if (watch.sees(grads[i])) return py::none();
+    check_input("clip_grads", grads[i], device);
   }
   Lists lists(grads.size());
   py::list made(grads.size());

@@ -372,6 +372,17 @@ def test_refusals(cuda_device):
         with pytest.raises(ValueError):
             call()
     assert (a == 1).all() and (b == 1).all()
+    # gradients that share memory with each other are read, and may
+    both, norm = gradients.clip_grads([a, a, a[2:5]], 1.0, out=[b, torch.empty_like(b), b.new_empty(3)])
+    assert abs(norm.item() - math.sqrt(19)) <= 1e-6 and torch.equal(both[0], both[1])
+    b.fill_(1)
+    whole = torch.ones(64, device=cuda_device)
+    for grads, outs in (([whole[:8], whole[40:48]], [whole[8:16], whole[44:52]]),
+                        ([whole[40:48], whole[:8]], [whole[16:24], whole[20:28]]),
+                        ([whole[:32], whole[32:]], [whole[32:], whole[:32]])):
+        with pytest.raises(ValueError, match="share memory"):
+            gradients.clip_grads(grads, 1.0, out=outs)
+    assert (whole == 1).all()
     p = torch.nn.Parameter(a)
     p.grad = b
     with pytest.raises(ValueError, match="once"):
