@@ -13,8 +13,8 @@
 // Two launches: every CTA leaves its sum in the workspace; every CTA of the second adds those
 // up and scales its chunks, from the last to the first, which are still in L2.  Up to
 // kClusterChunks chunks are one launch of a cluster, whose CTAs read each other's sums from
-// shared memory.  268,435,456 float32 values: norm 167 us (6.4 TB/s), scaling 329 us (6.5); bf16
-// norm 95 us (5.6).  300 tensors of 40 million values: 37 and 44 us.  16 tensors of 24,768: 5.8
+// shared memory.  268,435,456 float32 values: norm 170 us (6.3 TB/s), scaling 337 us (6.4); bf16
+// norm 83 us (6.5).  300 tensors of 40 million values: 31 and 35 us.  16 tensors of 24,768: 5.8
 // us in all.
 //
 // Squares are added in float32 over the 16 bytes of a load and in float64 beyond.  Where
@@ -35,7 +35,7 @@ namespace {
 constexpr int kThreads = 256;  // of a group that takes a chunk
 constexpr int kUnits = 8;      // 16-byte units of a chunk per thread
 constexpr int kChunkBytes = kThreads * kUnits * 16;
-constexpr int kBlocksPerSm = 8;
+constexpr int kBlocksPerSm = 2;  // as many as run at a time, by their registers
 constexpr int kClusterCtas = 8, kClusterGroups = 2;  // groups of a CTA
 constexpr int kClusterChunks = 128;
 constexpr int kMostTensors = 1024;  // of a launch: 29 bytes each of its 32,764 of arguments
@@ -55,20 +55,23 @@ struct Tensors {
   bool in_place;  // every out is its in
 };
 
-struct Place {
-  int tensor;
-  int64_t chunk;  // in the tensor
+// A chunk of a launch: chunk number `chunk` of a tensor.
+struct Item {
+  const void* in;
+  void* out;
+  int64_t count, chunk;
+  int dtype;
 };
 
 template <int N>
-__device__ __forceinline__ Place place_of(const Tensors<N>& list, int chunk) {
+__device__ __forceinline__ Item item_at(const Tensors<N>& list, int chunk) {
   int low = 0, high = list.tensors;  // first[low] <= chunk < first[high]
   while (high - low > 1) {
     const int mid = (low + high) >> 1;
     if (list.first[mid] <= chunk) low = mid;
     else high = mid;
   }
-  return {low, chunk - list.first[low]};
+  return {list.in[low], list.out[low], list.count[low], chunk - list.first[low], list.dtype[low]};
 }
 
 // What a chunk's elements are: the tensor's are [begin, end) of the chunk's.
@@ -79,18 +82,51 @@ struct Chunk {
   int begin, end;
 };
 
-template <typename T, int N>
-__device__ __forceinline__ Chunk<T> chunk_at(const Tensors<N>& list, const Place& at) {
+template <typename T>
+__device__ __forceinline__ Chunk<T> chunk_of(const Item& at) {
   constexpr int kElements = kChunkBytes / sizeof(T);
-  const T* base = static_cast<const T*>(list.in[at.tensor]);
+  const T* base = static_cast<const T*>(at.in);
   const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(base) % 16 / sizeof(T));
   Chunk<T> c;
   c.offset = at.chunk * kElements - shift;
   c.in = base + c.offset;
   c.begin = at.chunk == 0 ? shift : 0;
-  const int64_t left = list.count[at.tensor] - c.offset;
+  const int64_t left = at.count - c.offset;
   c.end = left < kElements ? static_cast<int>(left) : kElements;
   return c;
+}
+
+// Calls f(item) for the chunks of the CTA, from the first to the last, or back.  They are found
+// ahead, kItems at a time, by a thread each: a search through the arguments costs a miss of the
+// constant cache a step, which the chunks would wait for one after the other (300 mixed tensors,
+// norm and scaling: 81 us, found ahead 67).
+constexpr int kItems = 64;
+
+template <int N, typename F>
+__device__ __forceinline__ void for_chunks(const Tensors<N>& list, bool back, const F& f) {
+  __shared__ Item items[kItems];
+  const int chunks = list.first[list.tensors], step = static_cast<int>(gridDim.x);
+  const int first = static_cast<int>(blockIdx.x);
+  const int rounds = first < chunks ? (chunks - 1 - first) / step + 1 : 0;
+  const int batches = (rounds + kItems - 1) / kItems;
+  for (int i = 0; i < batches; ++i) {
+    const int base = (back ? batches - 1 - i : i) * kItems;
+    const int here = rounds - base < kItems ? rounds - base : kItems;
+    __syncthreads();
+    if (static_cast<int>(threadIdx.x) < here)
+      items[threadIdx.x] = item_at(list, first + (base + static_cast<int>(threadIdx.x)) * step);
+    __syncthreads();
+    for (int j = 0; j < here; ++j) f(items[back ? here - 1 - j : j]);
+  }
+}
+
+// The same for a group of a cluster's CTA, which has a few chunks at most: each found as it comes.
+template <int N, typename F>
+__device__ __forceinline__ void for_chunks_of_group(const Tensors<N>& list, const F& f) {
+  const int chunks = list.first[list.tensors];
+  for (int c = static_cast<int>(blockIdx.x) * kClusterGroups + threadIdx.x / kThreads; c < chunks;
+       c += kClusterCtas * kClusterGroups)
+    f(item_at(list, c));
 }
 
 template <typename T>
@@ -113,18 +149,21 @@ __device__ __forceinline__ void load_units(const Chunk<T>& c, int thread, Held<T
       h.unit[i] = *reinterpret_cast<const Unit*>(c.in + (i * kThreads + thread) * V);
     return;
   }
+  // whole units first, their loads together, then the one at either end
 #pragma unroll
   for (int i = 0; i < kUnits; ++i) {
     const int at = (i * kThreads + thread) * V;
-    Unit v{};
-    if (at >= c.begin && at + V <= c.end) {
-      v = *reinterpret_cast<const Unit*>(c.in + at);
-    } else if (at + V > c.begin && at < c.end) {
+    h.unit[i] = Unit{};
+    if (at >= c.begin && at + V <= c.end) h.unit[i] = *reinterpret_cast<const Unit*>(c.in + at);
+  }
+#pragma unroll
+  for (int i = 0; i < kUnits; ++i) {
+    const int at = (i * kThreads + thread) * V;
+    const bool cut = (at < c.begin && at + V > c.begin) || (at < c.end && at + V > c.end);
+    if (cut)
 #pragma unroll
       for (int j = 0; j < V; ++j)
-        if (at + j >= c.begin && at + j < c.end) v.v[j] = c.in[at + j];
-    }
-    h.unit[i] = v;
+        if (at + j >= c.begin && at + j < c.end) h.unit[i].v[j] = c.in[at + j];
   }
 }
 
@@ -214,44 +253,28 @@ __device__ __forceinline__ Running<KIND> over_block(Running<KIND> r) {
   return all;
 }
 
-// `meanwhile` runs between the loads and the arithmetic.
-template <int KIND, typename T, int N, typename F>
-__device__ __forceinline__ void add_chunk(const Tensors<N>& list, const Place& at, int thread,
-                                          Running<KIND>& r, const F& meanwhile) {
-  const Chunk<T> c = chunk_at<T>(list, at);
+template <int KIND, typename T>
+__device__ __forceinline__ void add_chunk(const Item& at, int thread, Running<KIND>& r) {
   Held<T> h;
-  load_units(c, thread, h);
-  meanwhile();
+  load_units(chunk_of<T>(at), thread, h);
   r.add(h);
 }
 
-// The thread's part of chunks first, first + step, ...
-template <int KIND, int N>
-__device__ __forceinline__ Running<KIND> add_chunks(const Tensors<N>& list, int first, int step,
-                                                    int thread) {
-  Running<KIND> r;
-  const int chunks = list.first[list.tensors];
-  Place next{};
-  if (first < chunks) next = place_of(list, first);
-  for (int c = first; c < chunks; c += step) {
-    const Place at = next;
-    const auto meanwhile = [&] {
-      if (c + step < chunks) next = place_of(list, c + step);
-    };
-    switch (list.dtype[at.tensor]) {
-      case ICTC_DTYPE_F32: add_chunk<KIND, float>(list, at, thread, r, meanwhile); break;
-      case ICTC_DTYPE_BF16: add_chunk<KIND, __nv_bfloat16>(list, at, thread, r, meanwhile); break;
-      default: add_chunk<KIND, __half>(list, at, thread, r, meanwhile);
-    }
+template <int KIND>
+__device__ __forceinline__ void add_item(const Item& at, int thread, Running<KIND>& r) {
+  switch (at.dtype) {
+    case ICTC_DTYPE_F32: return add_chunk<KIND, float>(at, thread, r);
+    case ICTC_DTYPE_BF16: return add_chunk<KIND, __nv_bfloat16>(at, thread, r);
+    default: add_chunk<KIND, __half>(at, thread, r);
   }
-  return r;
 }
 
 template <int KIND, int N>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 2)
     partial_kernel(const __grid_constant__ Tensors<N> list, double* __restrict__ partial) {
-  const Running<KIND> r = over_block(
-      add_chunks<KIND>(list, static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x), threadIdx.x));
+  Running<KIND> r;
+  for_chunks(list, false, [&](const Item& at) { add_item(at, threadIdx.x, r); });
+  r = over_block(r);
   if (threadIdx.x == 0) partial[blockIdx.x] = r.get();
 }
 
@@ -263,7 +286,7 @@ __device__ __forceinline__ double norm_of(const double* __restrict__ partial, in
 }
 
 template <int KIND>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 2)
     norm_kernel(const double* __restrict__ partial, int parts, float* __restrict__ norm) {
   const double n = norm_of<KIND>(partial, parts);
   if (threadIdx.x == 0) *norm = static_cast<float>(n);
@@ -275,12 +298,11 @@ __device__ __forceinline__ float factor_of(double norm, double max_norm) {
   return static_cast<float>(q > 1.0 ? 1.0 : q);
 }
 
-template <typename T, int N>
-__device__ __forceinline__ void scale_chunk(const Tensors<N>& list, const Place& at,
-                                            int thread, float factor) {
+template <typename T>
+__device__ __forceinline__ void scale_chunk(const Item& at, int thread, float factor) {
   constexpr int V = kPerUnit<T>, kElements = kChunkBytes / sizeof(T);
-  const Chunk<T> c = chunk_at<T>(list, at);
-  T* out = static_cast<T*>(list.out[at.tensor]) + c.offset;
+  const Chunk<T> c = chunk_of<T>(at);
+  T* out = static_cast<T*>(at.out) + c.offset;
   if (reinterpret_cast<uintptr_t>(out) % 16 == 0) {
     Held<T> h;
     load_units(c, thread, h);
@@ -324,29 +346,23 @@ __device__ __forceinline__ void scale_chunk(const Tensors<N>& list, const Place&
   }
 }
 
-template <int N>
-__device__ __forceinline__ void scale_chunks(const Tensors<N>& list, int first, int step,
-                                             int thread, float factor) {
-  const int chunks = list.first[list.tensors];
-  if (first >= chunks || (factor == 1.f && list.in_place)) return;  // they are as they should be
-  for (int c = first + (chunks - 1 - first) / step * step; c >= 0; c -= step) {
-    const Place at = place_of(list, c);
-    switch (list.dtype[at.tensor]) {
-      case ICTC_DTYPE_F32: scale_chunk<float>(list, at, thread, factor); break;
-      case ICTC_DTYPE_BF16: scale_chunk<__nv_bfloat16>(list, at, thread, factor); break;
-      default: scale_chunk<__half>(list, at, thread, factor);
-    }
+__device__ __forceinline__ void scale_item(const Item& at, int thread, float factor) {
+  switch (at.dtype) {
+    case ICTC_DTYPE_F32: return scale_chunk<float>(at, thread, factor);
+    case ICTC_DTYPE_BF16: return scale_chunk<__nv_bfloat16>(at, thread, factor);
+    default: scale_chunk<__half>(at, thread, factor);
   }
 }
 
 template <int KIND, int N>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 2)
     scale_kernel(const __grid_constant__ Tensors<N> list, const double* __restrict__ partial,
                  int parts, double max_norm, float* __restrict__ norm) {
   const double n = norm_of<KIND>(partial, parts);
   if (norm != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *norm = static_cast<float>(n);
-  scale_chunks(list, static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x), threadIdx.x,
-               factor_of(n, max_norm));
+  const float factor = factor_of(n, max_norm);
+  if (factor == 1.f && list.in_place) return;  // they are as they should be
+  for_chunks(list, true, [&](const Item& at) { scale_item(at, threadIdx.x, factor); });
 }
 
 // All of it in one cluster.
@@ -356,11 +372,10 @@ __global__ void __cluster_dims__(kClusterCtas, 1, 1)
         cluster_kernel(const __grid_constant__ Tensors<N> list, bool scale, double max_norm,
                        float* __restrict__ norm) {
   __shared__ double sum;
-  constexpr int kStep = kClusterCtas * kClusterGroups;
   const int thread = threadIdx.x % kThreads;
-  const int first = static_cast<int>(blockIdx.x) * kClusterGroups + threadIdx.x / kThreads;
-  const Running<KIND> own =
-      over_block<KIND, kClusterGroups>(add_chunks<KIND>(list, first, kStep, thread));
+  Running<KIND> own;
+  for_chunks_of_group(list, [&](const Item& at) { add_item(at, thread, own); });
+  own = over_block<KIND, kClusterGroups>(own);
   if (threadIdx.x == 0) sum = own.get();
   cluster_sync();
   Running<KIND> all;
@@ -372,7 +387,9 @@ __global__ void __cluster_dims__(kClusterCtas, 1, 1)
   }
   const double n = all.norm();
   if (blockIdx.x == 0 && threadIdx.x == 0) *norm = static_cast<float>(n);
-  if (scale) scale_chunks(list, first, kStep, thread, factor_of(n, max_norm));
+  const float factor = factor_of(n, max_norm);
+  if (scale && !(factor == 1.f && list.in_place))
+    for_chunks_of_group(list, [&](const Item& at) { scale_item(at, thread, factor); });
   cluster_sync();  // no CTA leaves while another may read its sum
 }
 
