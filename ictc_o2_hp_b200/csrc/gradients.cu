@@ -13,8 +13,8 @@
 // Two launches: every CTA leaves its sum in the workspace; every CTA of the second adds those
 // up and scales its chunks, from the last to the first, which are still in L2.  Up to
 // kClusterChunks chunks are one launch of a cluster, whose CTAs read each other's sums from
-// shared memory.  268,435,456 float32 values: norm 170 us (6.3 TB/s), scaling 337 us (6.4); bf16
-// norm 83 us (6.5).  300 tensors of 40 million values: 31 and 35 us.  16 tensors of 24,768: 5.8
+// shared memory.  268,435,456 float32 values: norm 170 us (6.3 TB/s), scaling 340 us (6.3); bf16
+// norm 83 us (6.5).  300 tensors of 40 million values: 31 and 34 us.  16 tensors of 24,768: 5.8
 // us in all.
 //
 // Squares are added in float32 over the 16 bytes of a load and in float64 beyond.  Where
@@ -99,7 +99,7 @@ __device__ __forceinline__ Chunk<T> chunk_of(const Item& at) {
 // Calls f(item) for the chunks of the CTA, from the first to the last, or back.  They are found
 // ahead, kItems at a time, by a thread each: a search through the arguments costs a miss of the
 // constant cache a step, which the chunks would wait for one after the other (300 mixed tensors,
-// norm and scaling: 81 us, found ahead 67).
+// norm and scaling: 81 us, found ahead 65).
 constexpr int kItems = 64;
 
 template <int N, typename F>
