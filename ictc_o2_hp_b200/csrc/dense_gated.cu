@@ -20,6 +20,13 @@
 // The backward forms D in a pass over p and g (gated_slope_kernel) but for the narrow layers.
 // A tile of these kernels has the sums of both halves for the same columns of y, so that the
 // epilogue needs nothing from another tile, and p is written only where a backward wants it.
+//
+// Relu's slope jumps at 0, where a p within its own rounding may have either sign.  In float32
+// one such element among 10^8 moves dx and dW by 10^-4 of their norms, a thousand times what
+// rounding does, so the sign is not left to the order in which a kernel happens to sum: p within
+// the bounds of its error is computed again by fused multiply-adds in the order of k, bias last
+// (settle_kernel; gated_narrow_backward_kernel for its own p), and every path has the same
+// slopes.  (16-bit gradients are rounded by more than that.)
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -160,6 +167,152 @@ __global__ void __launch_bounds__(kFewThreads) few_kernel(
   }
 }
 
+// ------------------------------------------------- relu: p near 0, in the order of k
+// A product's p and the sum in order differ by at most near_zero(k) |x|_2 |w|_2: the products
+// that the cut parts drop, the tensor core's truncation (2.3 2^-24 of the sum so far a step of 16
+// elements; sums are moved out every 256) and k rounding errors, seven standard deviations of
+// them where that is less than all of one sign.
+inline float near_zero(int64_t k) {
+  const float elements = static_cast<float>(k);
+  return 5.9604645e-8f * (6.f + 0.15f * fminf(elements, 256.f) + fminf(elements, 4.f * sqrtf(elements)));
+}
+
+// |w_c|_2 of the n gate rows of W, then |x_r|_2 of the m rows of x; `lanes` of a warp a row,
+// kNormRows rows in flight.  Squares that leave float32's range are taken again in float64.
+constexpr int kNormThreads = 256, kNormRows = 4;
+
+template <int V>
+__global__ void __launch_bounds__(kNormThreads)
+    row_norm_kernel(const float* __restrict__ x, int64_t ldx, const float* __restrict__ w,
+                    int64_t ldw, float* __restrict__ norms, int64_t m, int64_t n, int64_t k,
+                    int lanes) {
+  const int part = threadIdx.x % lanes, rows = kNormThreads / lanes;
+  const int64_t total = m + n, step = static_cast<int64_t>(gridDim.x) * rows * kNormRows;
+  const auto row_at = [&](int64_t r) { return r < n ? w + r * ldw : x + (r - n) * ldx; };
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * rows * kNormRows; base < total;
+       base += step) {
+    const int64_t r0 = base + threadIdx.x / lanes;
+    const float* row[kNormRows];
+    float sum[kNormRows];
+#pragma unroll
+    for (int q = 0; q < kNormRows; ++q) {
+      row[q] = row_at(r0 + q * rows < total ? r0 + q * rows : 0);
+      sum[q] = 0.f;
+    }
+#pragma unroll 2
+    for (int64_t c = part * V; c < k; c += lanes * V) {
+      Pack<float, V> v[kNormRows];
+#pragma unroll
+      for (int q = 0; q < kNormRows; ++q) v[q] = *reinterpret_cast<const Pack<float, V>*>(row[q] + c);
+#pragma unroll
+      for (int q = 0; q < kNormRows; ++q)
+#pragma unroll
+        for (int j = 0; j < V; ++j) sum[q] = fmaf(v[q].v[j], v[q].v[j], sum[q]);
+    }
+#pragma unroll
+    for (int q = 0; q < kNormRows; ++q)
+      for (int o = lanes / 2; o > 0; o >>= 1) sum[q] += __shfl_xor_sync(0xffffffffu, sum[q], o);
+#pragma unroll
+    for (int q = 0; q < kNormRows; ++q) {
+      if (part != 0 || r0 + q * rows >= total) continue;
+      float norm = sqrtf(sum[q]);
+      if (!(sum[q] >= 1e-30f && sum[q] <= 1e38f)) {
+        double wide = 0.0;
+        for (int64_t c = 0; c < k; ++c) {
+          const double v = row[q][c];
+          wide = fma(v, v, wide);
+        }
+        norm = static_cast<float>(sqrt(wide));
+      }
+      norms[r0 + q * rows] = 1.01f * norm;
+    }
+  }
+}
+
+// Gate columns of preact that lie near 0 by fused multiply-adds in the order of k, bias last.
+// One pass over the gate half, a run of segments a warp; what is near 0 in them then goes to a lane
+// each.  float32 65,536 x 128 x 512, where that is 4 elements in 10^5: 11 us for the norms and 66;
+// 4,096 x 16,384 x 2,048, 35 in 10^4 and long sums: 138 and 1,840 of a step's 13,000.
+constexpr int kSettleWarps = 8, kSettleLoads = 8, kSettleRun = 32;
+
+// V: elements of a load of preact, whose row lengths are whole ones; U: of x and W.  `run`
+// segments a warp, kSettleRun at most.
+template <int V, int U>
+__global__ void __launch_bounds__(kSettleWarps * 32)
+    settle_kernel(const float* __restrict__ x, int64_t ldx, const float* __restrict__ w,
+                  int64_t ldw, const float* __restrict__ bias, const float* __restrict__ norms,
+                  float* preact, int64_t m, int64_t n, int64_t k, float near, int run) {
+  constexpr int kSegment = 32 * V * kSettleLoads, kRoom = 2 * kSegment;
+  constexpr int kAhead = U == 4 ? 8 : 32;  // loads of x and of W in flight
+  static_assert(kSegment * kSettleRun <= 65536);
+  __shared__ uint16_t found[kSettleWarps][kRoom];
+  __shared__ int counts[kSettleWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t total = m * n, length = static_cast<int64_t>(run) * kSegment;
+  const int64_t next_row = 32 * V / n, next_col = 32 * V % n;  // a load of the warp on
+  for (int64_t base = (static_cast<int64_t>(blockIdx.x) * kSettleWarps + warp) * length;
+       base < total; base += static_cast<int64_t>(gridDim.x) * kSettleWarps * length) {
+    if (lane == 0) counts[warp] = 0;
+    __syncwarp();
+    int64_t row = (base + lane * V) / n, col = base + lane * V - row * n;
+#pragma unroll 1
+    for (int segment = 0; segment < run; ++segment) {
+      Pack<float, V> p[kSettleLoads];
+      float size[kSettleLoads];
+      int64_t cols[kSettleLoads];
+#pragma unroll
+      for (int i = 0; i < kSettleLoads; ++i) {
+        size[i] = -1.f;
+        cols[i] = col;
+        if (row < m) {
+          p[i] = *reinterpret_cast<const Pack<float, V>*>(preact + row * 2 * n + col);
+          size[i] = near * norms[n + row];
+        }
+        row += next_row;
+        col += next_col;
+        if (col >= n) {
+          col -= n;
+          ++row;
+        }
+      }
+      uint32_t mine = 0;
+#pragma unroll
+      for (int i = 0; i < kSettleLoads; ++i) {
+        if (size[i] < 0.f) continue;
+        const Pack<float, V> most = *reinterpret_cast<const Pack<float, V>*>(norms + cols[i]);
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (fabsf(p[i].v[j]) <= fmaf(size[i], most.v[j], 1.1754944e-38f)) mine |= 1u << (i * V + j);
+      }
+      for (; mine != 0; mine &= mine - 1) {
+        const int bit = __ffs(mine) - 1;
+        found[warp][atomicAdd(&counts[warp], 1)] =
+            static_cast<uint16_t>(segment * kSegment + (bit / V * 32 + lane) * V + bit % V);
+      }
+      __syncwarp();
+      const int count = counts[warp];
+      if (count <= kRoom - kSegment && segment + 1 < run) continue;
+      for (int i = lane; i < count; i += 32) {
+        const int64_t e = base + found[warp][i], r = e / n, c = e - r * n;
+        const float* xr = x + r * ldx;
+        const float* wr = w + c * ldw;
+        float sum = 0.f;
+#pragma unroll kAhead
+        for (int64_t q = 0; q < k; q += U) {
+          const Pack<float, U> a = *reinterpret_cast<const Pack<float, U>*>(xr + q);
+          const Pack<float, U> b = *reinterpret_cast<const Pack<float, U>*>(wr + q);
+#pragma unroll
+          for (int j = 0; j < U; ++j) sum = fmaf(a.v[j], b.v[j], sum);
+        }
+        preact[r * 2 * n + c] = bias ? sum + bias[c] : sum;
+      }
+      __syncwarp();
+      if (lane == 0) counts[warp] = 0;
+      __syncwarp();
+    }
+  }
+}
+
 // ------------------------------------------------------- D = (dg | du) and its column sums
 // Bound by HBM (bf16 16,384 x 4,096: 159 us, 5.9 TB/s; float32 65,536 x 512: 110 us, 6.1 TB/s;
 // odd rows, f16 4,999 x 777, 18 us: issue).  A CTA owns a strip of columns of both halves and every gridDim.y-th block
@@ -269,6 +422,7 @@ struct GatedPlan {
   Split cut;
   size_t x, w, partial;                  // forward
   size_t p, y;                           // forward, general
+  size_t norms;                          // forward, where p is settled
   size_t d, columns, forward;            // backward
   size_t product, product_bytes, total;  // the linear layer's
 };
@@ -291,12 +445,20 @@ constexpr int64_t kPitchUnit = 64;
 
 int64_t row_pitch(int64_t width, size_t size) { return aligned_pitch(width, size, kPitchUnit); }
 
-int plan_forward(int64_t m, int64_t n, int64_t k, int dtype, int32_t layout, bool keep, int device,
-                 GatedPlan* b) {
+// Whether the p that a forward leaves for the backward is settled.
+bool settles(int dtype, int activation) {
+  return dtype == ICTC_DTYPE_F32 && activation == ICTC_ACT_RELU;
+}
+
+int plan_forward(int64_t m, int64_t n, int64_t k, int dtype, int activation, int32_t layout,
+                 bool keep, int device, GatedPlan* b) {
   const size_t size = dtype_size(dtype);
   const bool rows_aligned = layout & ICTC_LINEAR_ALIGNED;
   const bool wide = dtype == ICTC_DTYPE_F32;
   Layout space;
+  if (keep && settles(dtype, activation))
+    b->norms = space.take(static_cast<size_t>(m + n) * sizeof(float));
+  b->total = space.at;
   b->way = Way::general;
   const bool whole = rows_aligned && k % static_cast<int64_t>(16 / size) == 0;
   // three or four rows of 16 bits make more FMAs and conversions than the SM pairs' mostly empty
@@ -358,8 +520,8 @@ int plan_forward(int64_t m, int64_t n, int64_t k, int dtype, int32_t layout, boo
 
 // keep: the forward kept p.  Otherwise it is computed again, by the forward kernels where the
 // layer is not narrow.
-int plan_backward(int64_t m, int64_t n, int64_t k, int dtype, int32_t layout, bool keep, int device,
-                  GatedPlan* b) {
+int plan_backward(int64_t m, int64_t n, int64_t k, int dtype, int activation, int32_t layout,
+                  bool keep, int device, GatedPlan* b) {
   const size_t size = dtype_size(dtype);
   Layout space;
   if (!keep && is_narrow(m, n, k, dtype, layout)) {
@@ -370,7 +532,7 @@ int plan_backward(int64_t m, int64_t n, int64_t k, int dtype, int32_t layout, bo
   }
   if (!keep) {
     GatedPlan forward{};
-    const int st = plan_forward(m, n, k, dtype, layout, true, device, &forward);
+    const int st = plan_forward(m, n, k, dtype, activation, layout, true, device, &forward);
     if (st != ICTC_OK) return st;
     b->p = space.take(static_cast<size_t>(m) * 2 * n * sizeof(float));
     b->y = space.take(static_cast<size_t>(m) * n * size);
@@ -564,6 +726,7 @@ int run_narrow_backward(const T* x, const T* w, int64_t ldw, const void* bias, c
                         int activation, cudaStream_t stream) {
   GatedNarrowArgs p = narrow_args(x, w, ldw, bias, m, n, k);
   p.g = g;
+  p.near = near_zero(k);
   p.partial = dw || db ? partial : nullptr;
   p.e.out = dx;
   GatedNarrowMaps maps{};
@@ -645,9 +808,9 @@ int run_tiles(const T* x, int64_t ldx, const T* w, int64_t ldw, Epilogue e, unsi
 }
 
 template <typename T>
-int run_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const Epilogue& e,
-                unsigned char* ws, const GatedPlan& plan, int64_t m, int64_t n, int64_t k,
-                int dtype, cudaStream_t stream) {
+int run_products(const void* x, int64_t ldx, const void* w, int64_t ldw, const Epilogue& e,
+                 unsigned char* ws, const GatedPlan& plan, int64_t m, int64_t n, int64_t k,
+                 int dtype, cudaStream_t stream) {
   const T* xt = static_cast<const T*>(x);
   const T* wt = static_cast<const T*>(w);
   if (plan.way == Way::few) {
@@ -666,6 +829,48 @@ int run_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const Ep
       stream);
   if (st != ICTC_OK) return st;
   return run_gate<T>(p, 1, nullptr, nullptr, static_cast<T*>(e.out), m, n, e.activation, stream);
+}
+
+int run_settle(const float* x, int64_t ldx, const float* w, int64_t ldw, const Epilogue& e,
+               float* norms, int64_t m, int64_t n, int64_t k, cudaStream_t stream) {
+  const int64_t sms = sm_count(current_device());
+  const auto grid = [&](int64_t blocks) {
+    return static_cast<unsigned>(blocks < sms * 8 ? blocks : sms * 8);
+  };
+  const bool whole = k % 4 == 0 && chunk_aligned(x, ldx, 4) && chunk_aligned(w, ldw, 4);
+  int lanes = 1;
+  while (lanes < 32 && 4 * lanes * (whole ? 4 : 1) < k) lanes *= 2;  // four loads a lane
+  const int64_t rows = kNormThreads / lanes * kNormRows;
+  const auto norm = whole ? row_norm_kernel<4> : row_norm_kernel<1>;
+  norm<<<grid(ceil_div(m + n, rows)), kNormThreads, 0, stream>>>(x, ldx, w, ldw, norms, m, n, k,
+                                                                 lanes);
+  cudaError_t err = cudaGetLastError();
+  if (err != cudaSuccess) return cuda_fail(err, "gated linear row norm launch");
+  const bool vec = n % 4 == 0 && aligned(e.preact, 16);
+  const auto settle = vec ? (whole ? settle_kernel<4, 4> : settle_kernel<4, 1>)
+                          : (whole ? settle_kernel<1, 4> : settle_kernel<1, 1>);
+  // one wave, if runs of kSettleRun segments make one
+  const int64_t segments = ceil_div(m * n, 32 * kSettleLoads * (vec ? 4 : 1));
+  const int64_t warps = sms * 3 * kSettleWarps;
+  int64_t run = ceil_div(segments, warps);
+  if (run > kSettleRun) run = kSettleRun;
+  const int64_t blocks = ceil_div(segments, run * kSettleWarps);
+  settle<<<grid(blocks), kSettleWarps * 32, 0, stream>>>(x, ldx, w, ldw,
+                                                         static_cast<const float*>(e.bias), norms,
+                                                         e.preact, m, n, k, near_zero(k),
+                                                         static_cast<int>(run));
+  err = cudaGetLastError();
+  return err == cudaSuccess ? ICTC_OK : cuda_fail(err, "gated linear settle launch");
+}
+
+template <typename T>
+int run_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const Epilogue& e,
+                unsigned char* ws, const GatedPlan& plan, int64_t m, int64_t n, int64_t k,
+                int dtype, cudaStream_t stream) {
+  const int st = run_products<T>(x, ldx, w, ldw, e, ws, plan, m, n, k, dtype, stream);
+  if (st != ICTC_OK || !e.preact || !settles(dtype, e.activation)) return st;
+  return run_settle(static_cast<const float*>(x), ldx, static_cast<const float*>(w), ldw, e,
+                    reinterpret_cast<float*>(ws + plan.norms), m, n, k, stream);
 }
 
 struct Backward {
@@ -691,7 +896,7 @@ int run_backward(const Backward& q, unsigned char* ws, const GatedPlan& plan, in
   int st = ICTC_OK;
   if (!p) {
     GatedPlan forward{};
-    st = plan_forward(m, n, k, dtype, layout, true, current_device(), &forward);
+    st = plan_forward(m, n, k, dtype, activation, layout, true, current_device(), &forward);
     if (st != ICTC_OK) return st;
     Epilogue e{};
     e.bias = q.bias;
@@ -774,9 +979,9 @@ extern "C" int32_t ictc_o2_gated_linear_workspace(int64_t rows, int64_t in, int6
   *forward_bytes = *backward_bytes = 0;
   if (rows == 0) return ICTC_OK;
   GatedPlan forward{}, backward{};
-  st = plan_forward(rows, hidden, in, dtype, layout, keep != 0, device, &forward);
+  st = plan_forward(rows, hidden, in, dtype, activation, layout, keep != 0, device, &forward);
   if (st == ICTC_OK)
-    st = plan_backward(rows, hidden, in, dtype, layout, keep != 0, device, &backward);
+    st = plan_backward(rows, hidden, in, dtype, activation, layout, keep != 0, device, &backward);
   *forward_bytes = forward.total;
   *backward_bytes = backward.total;
   return st;
@@ -797,7 +1002,8 @@ extern "C" int32_t ictc_o2_gated_linear_forward(const void* x, int64_t x_stride,
     return fail(ICTC_ERR_INVALID, "rows of x and weight must not overlap");
   const int32_t layout = layout_of(x, x_stride, weight, weight_stride, in, dtype_size(dtype));
   GatedPlan plan{};
-  st = plan_forward(rows, hidden, in, dtype, layout, preact != nullptr, current_device(), &plan);
+  st = plan_forward(rows, hidden, in, dtype, activation, layout, preact != nullptr,
+                    current_device(), &plan);
   if (st == ICTC_OK && plan.way == Way::narrow && !aligned(y, 16))
     st = fail(ICTC_ERR_INVALID, "without preact a narrow layer needs a 16-byte aligned y");
   if (st == ICTC_OK) st = check_workspace(workspace, workspace_bytes, plan.total);
@@ -847,7 +1053,8 @@ extern "C" int32_t ictc_o2_gated_linear_backward(
                 "without preact a narrow layer needs a contiguous grad_output, and it and grad_x "
                 "16-byte aligned");
   GatedPlan plan{};
-  st = plan_backward(rows, hidden, in, dtype, layout, preact != nullptr, current_device(), &plan);
+  st = plan_backward(rows, hidden, in, dtype, activation, layout, preact != nullptr,
+                     current_device(), &plan);
   if (st == ICTC_OK) st = check_workspace(workspace, workspace_bytes, plan.total);
   if (st != ICTC_OK) return st;
   const Backward q{x, weight, bias, x_stride, weight_stride, preact, grad_output,

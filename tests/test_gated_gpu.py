@@ -234,6 +234,78 @@ def test_infinite_bias(shape, dtype, cuda_device):
     assert not dw[2].isfinite().any() and not dx.isfinite().any()
 
 
+def in_order(x, w):
+    """x w^T by float32 fused multiply-adds in the order of k.  Products are exact in float64;
+    a sum there is rounded to odd, so that rounding it again to float32 rounds once."""
+    acc = torch.zeros(x.shape[0], w.shape[0], dtype=torch.float64, device=x.device)
+    for i in range(x.shape[1]):
+        p = x[:, i:i + 1].double() * w[:, i].double()
+        s = p + acc
+        back = s - p
+        lost = (p - (s - back)) + (acc - back)
+        bits = s.view(torch.int64)
+        away = torch.where((lost > 0) == (s > 0), 1, -1)
+        bits = torch.where((lost != 0) & (bits % 2 == 0), bits + away, bits)
+        acc = bits.view(torch.float64).float().double()
+    return acc.float()
+
+
+@pytest.mark.parametrize("bias", [True, False])
+@pytest.mark.parametrize("shape", [
+    (1, 64, 64), (5, 8, 4), (37, 64, 64), (3, 700, 9), (3000, 64, 64), (20001, 40, 64), (9001, 64, 12),
+    (2000, 16, 48), (300, 33, 77), (5000, 63, 61), (2000, 8, 3), (300, 264, 200), (2053, 211, 333),
+    (4097, 702, 6), (5000, 1536, 8), (4500, 3, 130), (260, 96, 1100), (64, 2049, 33), (20, 8200, 24)])
+def test_relu_slopes_are_those_of_the_sum_in_order(shape, bias, cuda_device):
+    """The slope of a projection within its rounding of 0 does not depend on the kernel: it is
+    that of float32 multiply-adds in the order of k, the bias last.  One row of every column is
+    given a bias that leaves one ulp of it, 0 or minus one ulp; the gradients' bounds then have
+    no room for a slope of the other side."""
+    from ictc_o2_hp_b200 import dense
+    m, k, n = shape
+    x, w, b, g = operands(m, k, n, torch.float32, cuda_device, 140)
+    p = in_order(x, w[:n])
+    if bias:
+        cols = torch.arange(n, device=cuda_device)
+        at = p[cols * 37 % m, cols]
+        step_to = torch.tensor([math.inf, 0.0, -math.inf], device=cuda_device)[cols % 3]
+        b[:n] = -torch.where(cols % 3 == 1, at, torch.nextafter(at, step_to))
+        p = p + b[:n]
+        assert (p == 0).any() or n < 2
+    else:
+        b = None
+    slope = (p > 0).double()
+    native, code = dense._load(), dense.ACTIVATIONS["relu"]
+    y, kept = native.gated_forward(x, w, b, code, True)
+    assert torch.equal(kept[:, :n] > 0, p > 0)
+    none = torch.empty(0, device=cuda_device)
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, b) if t is not None]
+    y = dense.gated_linear(*leaves, activation="relu")
+    ways = [torch.autograd.grad(y, leaves, g, retain_graph=True),
+            [t.detach() for t in torch.autograd.grad(y, leaves, g, create_graph=True)],
+            native.gated_backward(x, w, b, kept, g, code),
+            native.gated_backward(x, w, b, none, g, code)]
+
+    pg, pu, a, _, _, _, _, _, _ = gated64(x, w, b, "relu", g)
+    a = a * slope
+    ax, aw, ag = x.double().abs(), w.double().abs(), g.double().abs()
+    ep = sum_error(k) * (ax @ aw.t() + (0 if b is None else b.double().abs()))
+    epg, epu = ep.chunk(2, -1)
+    d = torch.cat([g * pu * slope, g * a], -1)
+    ed = torch.cat([ag * slope * epu, ag * epg], -1) + 4 * U * d.abs()
+    ad = d.abs() + ed
+    for grads in ways:
+        for name, got, left, right, count in (
+                ("dx", grads[0], d, w.double(), 2 * n), ("dweight", grads[1], d.t(), x.double(), m),
+                ("dbias", grads[2] if b is not None else None, d.t(), torch.ones(m, 1, device=cuda_device).double(), m)):
+            if got is None:
+                continue
+            wide = left @ right
+            e, size = (ed, ad) if name == "dx" else (ed.t(), ad.t())
+            bound = e @ right.abs() + max(sum_error(count), (count + 64) * U * (name == "dbias")) * (
+                size @ right.abs()) + 3 * U * (wide.abs() + e @ right.abs())
+            within(name, got.reshape(wide.shape), wide, bound)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_empty(dtype, cuda_device):
     from ictc_o2_hp_b200 import dense
