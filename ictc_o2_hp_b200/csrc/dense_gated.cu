@@ -551,15 +551,23 @@ int plan_backward(int64_t m, int64_t n, int64_t k, int dtype, int activation, in
     b->x = space.take(static_cast<size_t>(m) * row_pitch(k, size) * size);
     b->w = space.take(static_cast<size_t>(2 * n) * row_pitch(k, size) * size);
   }
-  int32_t flags = layout & (pitch == 2 * n || m <= 1 ? ~0 : ~ICTC_LINEAR_PACKED);
+  const bool packed = pitch == 2 * n || m <= 1;  // D
+  const auto add_product = [&](int32_t flags) {
+    size_t other, bytes = 0;
+    const int st = ictc_o2_linear_workspace(m, k, 2 * n, dtype, ICTC_ACT_NONE, flags, device,
+                                            &other, &bytes);
+    if (bytes > b->product_bytes) b->product_bytes = bytes;
+    return st;
+  };
+  int st;
   if (b->align) {
-    const bool kept = (layout & ICTC_LINEAR_PACKED) && k * size % 16 == 0;  // x is not copied
-    const bool packed = pitch == 2 * n && (kept || row_pitch(k, size) == k);
-    flags = ICTC_LINEAR_ALIGNED | (packed ? ICTC_LINEAR_PACKED : 0);
+    // the flags do not say which operand is off the boundaries: x may stay in rows of its own
+    // distance or be copied to packed ones, which take other products
+    st = add_product(ICTC_LINEAR_ALIGNED);
+    if (st == ICTC_OK && packed) st = add_product(ICTC_LINEAR_ALIGNED | ICTC_LINEAR_PACKED);
+  } else {
+    st = add_product(layout & (packed ? ~0 : ~ICTC_LINEAR_PACKED));
   }
-  size_t other;
-  const int st = ictc_o2_linear_workspace(m, k, 2 * n, dtype, ICTC_ACT_NONE, flags, device,
-                                          &other, &b->product_bytes);
   if (st != ICTC_OK) return st;
   b->product = space.take(b->product_bytes);
   b->total = space.at;

@@ -76,6 +76,31 @@ def test_status_codes():
         assert backward(**bad) == _lib.ERR_WORKSPACE, bad
 
 
+@pytest.mark.parametrize("dtype,size", [(0, 4), (1, 2), (2, 2)])
+@pytest.mark.parametrize("rows,inner,hidden", [(40000, 64, 32), (2000000, 64, 32), (1000000, 32, 16),
+                                               (40000, 96, 64)])
+def test_backward_workspace_holds_either_inner_product(rows, inner, hidden, dtype, size):
+    """Operands off the 16-byte boundaries are copied where they are, one by one: x may stay in
+    rows of its own distance, whose product needs other room than packed rows."""
+    lib = _lib.load()
+    fwd, bwd, inner_bytes = ctypes.c_size_t(), ctypes.c_size_t(), ctypes.c_size_t()
+    assert lib.ictc_o2_gated_linear_workspace(rows, inner, hidden, dtype, 2, 0, 1, 0,
+                                              ctypes.byref(fwd), ctypes.byref(bwd)) == _lib.OK
+
+    def padded(n):
+        return -(-n // 256) * 256
+
+    def pitch(width):
+        return -(-width * size // 64) * 64
+
+    held = padded(rows * pitch(2 * hidden)) + padded(min(rows, 296) * 2 * hidden * 4)
+    held += padded(rows * pitch(inner)) + padded(2 * hidden * pitch(inner))
+    for layout in (1, 3):  # aligned rows; aligned and packed
+        assert lib.ictc_o2_linear_workspace(rows, inner, 2 * hidden, dtype, 0, layout, 0,
+                                            ctypes.byref(fwd), ctypes.byref(inner_bytes)) == _lib.OK
+        assert bwd.value >= held + inner_bytes.value, layout
+
+
 def test_fake_tensors():
     from torch._subclasses.fake_tensor import FakeTensorMode
     with FakeTensorMode():

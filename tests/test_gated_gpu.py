@@ -307,6 +307,24 @@ def test_relu_slopes_are_those_of_the_sum_in_order(shape, bias, cuda_device):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("which", ["x strided", "x odd", "both"])
+@pytest.mark.parametrize("shape", [(40000, 64, 32), (2000000, 64, 32), (50000, 96, 40)])
+def test_one_operand_off_the_boundaries(shape, which, dtype, cuda_device):
+    """Sizes whose operands are copied to aligned rows, with an x that is aligned but not
+    contiguous beside a W off the boundaries, the other way round, and both off."""
+    m, k, n = shape
+    x, w, b, g = operands(m, k, n, dtype, cuda_device, 145)
+    if which == "x strided":
+        x = torch.cat([x, x], 1)[:, :k]
+    else:
+        x = torch.cat([x.reshape(-1)[:1], x.reshape(-1)])[1:].view(m, k)
+    if which != "x odd":
+        w = torch.cat([w.reshape(-1)[:1], w.reshape(-1)])[1:].view(2 * n, k)
+    y, grads = step(x, w, b, "silu", g)
+    check_gated(x, w, b, "silu", g, y, grads, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_empty(dtype, cuda_device):
     from ictc_o2_hp_b200 import dense
     w = rand((12, 5), dtype, cuda_device, 61).requires_grad_(True)
