@@ -171,37 +171,125 @@ py::object grad_norm(py::handle given, bool largest) {
   return py::cast(s.norm);
 }
 
-// Refuses outputs that share memory with one another or with another gradient: their
-// elements would be scaled twice, or be read by some CTAs after others wrote them.
-void check_apart(const Lists& lists) {
-  struct Range {
-    uintptr_t begin, end;
-  };
-  // outputs, and gradients that are none; lists come in the order of their memory as a rule
-  std::vector<Range> ranges[2];
-  for (auto& r : ranges) r.reserve(lists.in.size());
-  for (size_t i = 0; i < lists.in.size(); ++i) {
-    const uintptr_t bytes = static_cast<uintptr_t>(lists.counts[i]) *
-                            (lists.dtypes[i] == ICTC_DTYPE_F32 ? 4 : 2);
-    if (!bytes) continue;
-    const auto out = reinterpret_cast<uintptr_t>(lists.out[i]);
-    const auto in = reinterpret_cast<uintptr_t>(lists.in[i]);
-    ranges[0].push_back({out, out + bytes});
-    if (in != out) ranges[1].push_back({in, in + bytes});
+struct Range {
+  uintptr_t begin, end;
+};
+
+// From the first to the last element.
+Range extent(const Tensor& t) {
+  const auto begin = reinterpret_cast<uintptr_t>(t.const_data_ptr());
+  int64_t last = 0;
+  for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+  return {begin, begin + static_cast<uintptr_t>((last + 1) * static_cast<int64_t>(t.element_size()))};
+}
+
+// Stride and size of the dimensions, the smallest stride first; expanded ones left out.
+std::vector<std::pair<int64_t, int64_t>> by_stride(const Tensor& t) {
+  std::vector<std::pair<int64_t, int64_t>> dims;
+  for (int64_t d = 0; d < t.dim(); ++d)
+    if (t.size(d) > 1 && t.stride(d) != 0) dims.emplace_back(t.stride(d), t.size(d));
+  std::sort(dims.begin(), dims.end());
+  return dims;
+}
+
+// Whether every stride steps over all that smaller ones reach, as in slices of a dense tensor;
+// then no two elements are one.
+bool is_nested(const Tensor& t) {
+  int64_t reach = 0;
+  for (const auto& [stride, size] : by_stride(t)) {
+    if (stride <= reach) return false;
+    reach += stride * (size - 1);
   }
+  return true;
+}
+
+// Every run of elements that follow one another in memory.
+void add_runs(const Tensor& t, std::vector<Range>& runs) {
+  const auto dims = by_stride(t);
+  int64_t run = 1;
+  size_t outer = 0;
+  for (; outer < dims.size() && dims[outer].first == run; ++outer) run *= dims[outer].second;
+  const auto size = static_cast<int64_t>(t.element_size());
+  const auto start = reinterpret_cast<uintptr_t>(t.const_data_ptr());
+  std::vector<int64_t> at(dims.size(), 0);
+  int64_t offset = 0;
+  for (;;) {
+    const uintptr_t begin = start + static_cast<uintptr_t>(offset * size);
+    runs.push_back({begin, begin + static_cast<uintptr_t>(run * size)});
+    size_t d = outer;
+    for (; d < dims.size(); ++d) {
+      offset += dims[d].first;
+      if (++at[d] < dims[d].second) break;
+      offset -= dims[d].first * dims[d].second;
+      at[d] = 0;
+    }
+    if (d == dims.size()) return;
+  }
+}
+
+// Whether no output shares memory with another or with a gradient.  (A gradient may share
+// memory with another gradient.)  Outputs and gradients come apart, each in the order of their
+// memory as a rule.
+bool are_apart(std::vector<Range>& outs, std::vector<Range>& grads) {
   const auto before = [](const Range& a, const Range& b) { return a.begin < b.begin; };
-  for (auto& r : ranges)
-    if (!std::is_sorted(r.begin(), r.end(), before)) std::sort(r.begin(), r.end(), before);
-  // a gradient may share memory with another gradient, but an output with neither
+  for (auto* r : {&outs, &grads})
+    if (!std::is_sorted(r->begin(), r->end(), before)) std::sort(r->begin(), r->end(), before);
   uintptr_t out_end = 0, any_end = 0;
-  for (auto o = ranges[0].begin(), g = ranges[1].begin(); o != ranges[0].end() || g != ranges[1].end();) {
-    const bool is_out = g == ranges[1].end() || (o != ranges[0].end() && o->begin <= g->begin);
+  for (auto o = outs.begin(), g = grads.begin(); o != outs.end() || g != grads.end();) {
+    const bool is_out = g == grads.end() || (o != outs.end() && o->begin <= g->begin);
     const Range r = is_out ? *o++ : *g++;
-    TORCH_CHECK_VALUE(r.begin >= (is_out ? any_end : out_end),
-                      "clip_grads: gradients or outputs share memory; list each tensor once");
+    if (r.begin < (is_out ? any_end : out_end)) return false;
     if (is_out) out_end = std::max(out_end, r.end);
     any_end = std::max(any_end, r.end);
   }
+  return true;
+}
+
+// Refuses outputs that share memory with one another or with another gradient: their elements
+// would be scaled twice, be read by some CTAs after others wrote them, or be overwritten by a
+// later copy.  `copied`: the entries whose gradient the kernels read a copy of, whose memory may
+// have gaps; that of the others is the list's.
+void check_apart(const Lists& lists, const Sequence& given, const Sequence& to,
+                 const std::vector<size_t>& copied) {
+  std::vector<Range> outs, grads;
+  outs.reserve(lists.in.size());
+  grads.reserve(lists.in.size());
+  auto next = copied.begin();
+  bool nested = true;
+  const auto same_view = [](const Tensor& a, const Tensor& b) {
+    if (a.is_same(b)) return true;
+    bool same = a.const_data_ptr() == b.const_data_ptr();
+    for (int64_t d = 0; same && d < a.dim(); ++d) same = a.size(d) == 1 || a.stride(d) == b.stride(d);
+    return same;
+  };
+  for (size_t i = 0; i < lists.in.size(); ++i) {
+    const uintptr_t bytes = static_cast<uintptr_t>(lists.counts[i]) *
+                            (lists.dtypes[i] == ICTC_DTYPE_F32 ? 4 : 2);
+    const bool apart = next != copied.end() && *next == i;
+    if (apart) ++next;
+    if (!bytes) continue;
+    if (apart) {
+      outs.push_back(extent(to[i]));
+      nested = nested && is_nested(to[i]);
+      if (!same_view(given[i], to[i])) grads.push_back(extent(given[i]));
+      continue;
+    }
+    const auto out = reinterpret_cast<uintptr_t>(lists.out[i]);
+    const auto in = reinterpret_cast<uintptr_t>(lists.in[i]);
+    outs.push_back({out, out + bytes});
+    if (in != out) grads.push_back({in, in + bytes});
+  }
+  bool fine = are_apart(outs, grads) && nested;
+  if (!fine && !copied.empty()) {  // extents cross; slices of one tensor may do so without sharing
+    std::vector<Range> runs[2];
+    for (size_t i = 0; i < lists.in.size(); ++i) {
+      if (!lists.counts[i]) continue;
+      add_runs(to[i], runs[0]);
+      if (!same_view(given[i], to[i])) add_runs(given[i], runs[1]);
+    }
+    fine = are_apart(runs[0], runs[1]);
+  }
+  TORCH_CHECK_VALUE(fine, "clip_grads: gradients or outputs share memory; list each tensor once");
 }
 
 Tensor launch(const Lists& lists, c10::Device device, double max_norm, bool largest) {
@@ -222,6 +310,7 @@ std::optional<Tensor> clip_into(const Sequence& grads, const Sequence& out, doub
   const Watch watch;
   Lists lists(grads.size());
   std::vector<std::pair<size_t, Tensor>> apart;  // results that the kernels leave elsewhere
+  std::vector<size_t> copied;                    // gradients that they read a copy of
   for (size_t i = 0; i < grads.size(); ++i) {
     const Tensor &g = grads[i], &o = out[i];
     if (watch.sees(g) || watch.sees(o)) return std::nullopt;
@@ -241,12 +330,13 @@ std::optional<Tensor> clip_into(const Sequence& grads, const Sequence& out, doub
     TORCH_CHECK_VALUE(at::has_internal_overlap(o) != at::MemOverlap::Yes, "clip_grads: output ", i,
                       " has elements that share memory");
     lists.add_copy(g);
+    copied.push_back(i);
     if (!dense(o) || !o.is_contiguous())
       apart.emplace_back(i, at::empty(g.sizes(), g.options()));
     const Tensor& to = !apart.empty() && apart.back().first == i ? apart.back().second : o;
     lists.out.push_back(g.numel() ? to.data_ptr() : nullptr);
   }
-  check_apart(lists);
+  check_apart(lists, grads, out, copied);
   const Tensor norm = launch(lists, device, max_norm, largest);
   size_t next = 0;
   for (size_t i = 0; i < out.size(); ++i) {

@@ -387,3 +387,52 @@ def test_refusals(cuda_device):
     p.grad = b
     with pytest.raises(ValueError, match="once"):
         gradients.clip_grad_norm_([p, p], 1.0)
+
+
+def test_outputs_with_gaps_that_share_memory(cuda_device):
+    """Slices are refused where they share elements with another output or gradient, and only
+    there: slices of one tensor may lie in each other's gaps."""
+    from ictc_o2_hp_b200 import gradients
+    wide = torch.ones(30, 24, device=cuda_device)
+    like = torch.ones(30, 8, device=cuda_device)
+    cube = torch.ones(6, 4, 10, device=cuda_device)
+    v = wide[:, 5:20]
+    for grads, outs in (
+        ([v, v], [v, v]),
+        ([v, wide[:, 5:20]], [v, wide[:, 5:20]]),
+        ([like, like], [wide[:, :8], wide[:, 7:15]]),
+        ([like, wide.view(-1)[24:48]], [wide[:, :8], wide.view(-1)[24:48]]),
+        ([like, torch.ones(24, device=cuda_device)], [wide[:, :8], wide[7]]),
+        ([like, wide[3]], [wide[:, 16:24], torch.ones(24, device=cuda_device)]),
+        ([wide[:, :8]], [wide[:, 4:12]]),
+        ([wide[:, ::2], wide[:, ::3]], [wide[:, ::2], wide[:, ::3]]),
+        ([cube[:, 1:3], cube[:, :, 3:5]], [cube[:, 1:3], cube[:, :, 3:5]]),
+        ([torch.ones(8, 3, device=cuda_device)], [wide.view(-1).as_strided((8, 3), (2, 3))]),
+    ):
+        with pytest.raises(ValueError, match="share memory"):
+            gradients.clip_grads(grads, 0.5, out=outs)
+    assert (wide == 1).all() and (cube == 1).all()
+    p = torch.nn.Parameter(v.clone())
+    p.grad = v
+    with pytest.raises(ValueError, match="once"):
+        gradients.clip_grad_norm_([p, p], 0.5)
+    assert (wide == 1).all()
+
+    for lists in ([wide[:, :8], wide[:, 8:16], wide[:, 16:]], [wide[:, ::2], wide[:, 1::2]],
+                  [wide[::2], wide[1::2]], [cube[:, ::2], cube[:, 1::2]],
+                  [cube[:, :, :5], cube[:, 1:3, 5:], wide.t()[:, :30]],
+                  [wide[:15, :20].t(), wide[15:, :20], wide[:15, 20:]]):
+        before = [t.clone() for t in lists]
+        gradients.clip_grads(lists, 0.5, out=lists)
+        check_clipped(lists, before, 0.5)
+        wide.fill_(1)
+        cube.fill_(1)
+    # a gradient by two views of it, the distance of a single row being nobody's
+    one = wide[:, 3:4]
+    gradients.clip_grads([one], 0.5, out=[wide.as_strided((30, 1), (24, 5), 3)])
+    check_clipped([one], [torch.ones(30, 1, device=cuda_device)], 0.5)
+    wide.fill_(1)
+    # gradients that share memory with each other are read, and may
+    clipped, _ = gradients.clip_grads([wide[:, :8], wide[:, 4:12]], 0.5,
+                                      out=[torch.empty_like(like), torch.empty(8, 30, device=cuda_device).t()])
+    assert torch.equal(clipped[0], clipped[1])
