@@ -5,6 +5,7 @@
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/extension.h>
 
@@ -86,6 +87,19 @@ class Watch {
   bool everything_;
 };
 
+// A dual tensor's tangent would be left out, or left as it was beside a scaled value.
+class Tangents {
+ public:
+  Tangents() : some_(torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr) {}
+  void refuse(const char* what, const Tensor& t) const {
+    TORCH_CHECK_NOT_IMPLEMENTED(!some_ || !t._fw_grad(0).defined(), what,
+                                " has no forward-mode derivative");
+  }
+
+ private:
+  bool some_;  // no tensor has one outside of a level
+};
+
 void check_input(const char* what, const Tensor& t, c10::Device device) {
   const auto type = t.scalar_type();
   TORCH_CHECK_TYPE(t.layout() == at::kStrided && t.is_cuda() &&
@@ -155,11 +169,13 @@ py::object grad_norm(py::handle given, bool largest) {
   const auto device = tensors[0].device();
   const at::NoGradGuard no_grad;
   const c10::cuda::OptionalCUDAGuard guard(cuda_or_none(device));
+  const Tangents tangents;
   Lists lists(tensors.size());
   for (size_t i = 0; i < tensors.size(); ++i) {
     const Tensor& t = tensors[i];
     if (watch.sees(t)) return py::none();
     check_input("grad_norm", t, device);
+    tangents.refuse("grad_norm", t);
     if (dense(t)) lists.add(t);
     else lists.add_copy(t);
   }
@@ -308,6 +324,7 @@ std::optional<Tensor> clip_into(const Sequence& grads, const Sequence& out, doub
                     out.size(), " outputs");
   const auto device = grads[0].device();
   const Watch watch;
+  const Tangents tangents;
   Lists lists(grads.size());
   std::vector<std::pair<size_t, Tensor>> apart;  // results that the kernels leave elsewhere
   std::vector<size_t> copied;                    // gradients that they read a copy of
@@ -315,8 +332,10 @@ std::optional<Tensor> clip_into(const Sequence& grads, const Sequence& out, doub
     const Tensor &g = grads[i], &o = out[i];
     if (watch.sees(g) || watch.sees(o)) return std::nullopt;
     check_input("clip_grads", g, device);
+    tangents.refuse("clip_grads", g);
     const bool one = g.is_same(o);
     if (!one) {
+      tangents.refuse("clip_grads", o);
       TORCH_CHECK_VALUE(o.sizes() == g.sizes() && o.scalar_type() == g.scalar_type() &&
                             o.device() == g.device() && o.layout() == at::kStrided,
                         "clip_grads: output ", i, " must have its gradient's shape, type and "
@@ -387,9 +406,11 @@ py::object clip_grads(py::handle given, double max_norm, bool largest, py::handl
     const auto norm = clip_into(grads, to, max_norm, largest);
     return norm ? py::object(py::make_tuple(py::list(to.items()), *norm)) : py::none();
   }
+  const Tangents tangents;
   for (size_t i = 0; i < grads.size(); ++i) {
     if (watch.sees(grads[i])) return py::none();
     check_input("clip_grads", grads[i], device);
+    tangents.refuse("clip_grads", grads[i]);
   }
   Lists lists(grads.size());
   py::list made(grads.size());

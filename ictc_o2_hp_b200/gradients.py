@@ -11,8 +11,8 @@ and nothing waits for it.  2-norms (sums of squares in float64) and the largest 
 (``norm_type=math.inf``).  Non-finite gradients scale as in PyTorch: a NaN norm makes
 every gradient NaN, an infinite one makes finite gradients 0.
 
-Nothing here is differentiable: results carry no graph.  Other devices and types raise
-TypeError instead of falling back.
+Nothing here is differentiable: results carry no graph, and tensors with forward-mode tangents
+raise NotImplementedError.  Other devices and types raise TypeError instead of falling back.
 """
 
 from __future__ import annotations

@@ -436,3 +436,24 @@ def test_outputs_with_gaps_that_share_memory(cuda_device):
     clipped, _ = gradients.clip_grads([wide[:, :8], wide[:, 4:12]], 0.5,
                                       out=[torch.empty_like(like), torch.empty(8, 30, device=cuda_device).t()])
     assert torch.equal(clipped[0], clipped[1])
+
+
+def test_dual_tensors_are_refused(cuda_device):
+    """Scaling a dual tensor's value alone would leave it a tangent of another function."""
+    from torch.autograd import forward_ad
+
+    from ictc_o2_hp_b200 import gradients
+    a, b = (torch.ones(8, device=cuda_device) for _ in range(2))
+    p = torch.nn.Parameter(torch.ones(8, device=cuda_device))
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(a, torch.ones_like(a))
+        p.grad = dual
+        for call in (lambda: gradients.grad_norm([b, dual]), lambda: gradients.clip_grads([dual], 0.5),
+                     lambda: gradients.clip_grads([dual], 0.5, out=[dual]),
+                     lambda: gradients.clip_grads([dual[::2]], 0.5, out=[dual[::2]]),
+                     lambda: gradients.clip_grads([b], 0.5, out=[dual]),
+                     lambda: gradients.clip_grad_norm_([p], 0.5)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+        gradients.clip_grads([b], 0.5, out=[b])  # others go on
+    assert (a == 1).all() and abs(b.norm().item() - 0.5) <= 1e-5
