@@ -69,6 +69,18 @@ PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
   return fn;
 }
 
+// The driver's encoder wants a current context, which a thread has only after its first call of
+// the runtime: the encoding may be that call (an autograd or a worker thread whose memory comes
+// from the allocator's cache).
+template <typename... Args>
+CUresult encode_tiled(PFN_cuTensorMapEncodeTiled_v12000 fn, Args... args) {
+  const CUresult r = fn(args...);
+  if (r != CUDA_ERROR_INVALID_CONTEXT && r != CUDA_ERROR_NOT_INITIALIZED) return r;
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || cudaSetDevice(device) != cudaSuccess) return r;
+  return fn(args...);
+}
+
 int encode3(PFN_cuTensorMapEncodeTiled_v12000 fn, CUtensorMap* map, const float* base,
             uint64_t d0, uint64_t d1, uint64_t d2, uint64_t s1, uint64_t s2, uint32_t b0,
             uint32_t b1) {
@@ -76,10 +88,10 @@ int encode3(PFN_cuTensorMapEncodeTiled_v12000 fn, CUtensorMap* map, const float*
   const cuuint64_t strides[2] = {s1, s2};  // bytes, dims 1 and 2
   const cuuint32_t box[3] = {b0, b1, 1};
   const cuuint32_t estr[3] = {1, 1, 1};
-  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<float*>(base), dims,
-                        strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const CUresult r = encode_tiled(
+      fn, map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<float*>(base), dims, strides, box,
+      estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? 0 : -1;
 }
 
@@ -96,12 +108,12 @@ int encode_matrix(const void* base, int size, bool bf16, int64_t inner, int64_t 
   const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_inner),
                              static_cast<cuuint32_t>(box_outer)};
   const cuuint32_t estr[2] = {1, 1};
-  const CUresult r =
-      fn(map,
-         size == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
-                   : bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
-         2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-         swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const CUresult r = encode_tiled(
+      fn, map,
+      size == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                : bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+      2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+      swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? 0 : -1;
 }
 

@@ -514,6 +514,40 @@ def test_example_runs(cuda_device):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(3000, 64, 64), (700, 512, 256), (700, 511, 255), (300, 72, 40)])
+def test_first_call_of_a_thread(shape, dtype, cuda_device):
+    """A thread that has no context yet, because its memory comes from the allocator's cache."""
+    import threading
+
+    from ictc_o2_hp_b200 import dense
+    x, w, b, g = operands(*shape, dtype, cuda_device, 125)
+    native, code = dense._load(), dense.ACTIVATIONS["silu"]
+    _, p = native.gated_forward(x, w, b, code, True)
+    none = torch.empty(0, device=cuda_device)
+    for call in (lambda: (dense.gated_linear(x, w, b),), lambda: native.gated_forward(x, w, b, code, True),
+                 lambda: native.gated_backward(x, w, b, p, g, code),
+                 lambda: native.gated_backward(x, w, b, none, g, code),
+                 lambda: (dense.linear(x, w, b),)):
+        want = [t.clone() for t in call()]
+        held = call()
+        torch.cuda.synchronize()
+        del held
+        got, failed = [], []
+
+        def run():
+            try:
+                got.extend(call())
+            except Exception as e:  # noqa: BLE001
+                failed.append(e)
+
+        thread = threading.Thread(target=run)
+        thread.start()
+        thread.join()
+        assert not failed, failed
+        assert all(map(torch.equal, got, want))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("shape", [(3, 96, 64), (20, 512, 64), (200, 96, 64), (2000, 64, 64)])
 def test_other_stream_and_graph_capture(shape, dtype, cuda_device):
     """Work goes to the caller's stream; a captured step replays on new inputs, two captured
