@@ -164,6 +164,74 @@ def test_many_tiles(shape, dtype, cuda_device):
         assert all(torch.equal(p, q) for p, q in zip(out, first))
 
 
+def whole_operands(m, k, n, dtype, device, seed):
+    """Operands of -1, 0 and 1: with an activation of slope 0 or 1 every product and sum is a
+    whole number below 2^24, exact in float32 in any order, and D is exact in every type."""
+    gen = torch.Generator(device=device).manual_seed(seed)
+
+    def draw(*shape):
+        return torch.randint(-1, 2, shape, generator=gen, device=device).to(dtype)
+
+    return draw(m, k), draw(2 * n, k), draw(2 * n), draw(m, n)
+
+
+def exact_step(x, w, b, act, g):
+    """y, dx, dW and db in float64, in blocks of rows; and the largest partial sum there is."""
+    n = w.shape[0] // 2
+    wide, outs, dxs = w.double(), [], []
+    dw = torch.zeros(w.shape, dtype=torch.float64, device=w.device)
+    db = torch.zeros(w.shape[0], dtype=torch.float64, device=w.device)
+    most = 0.0
+    for rows, grad in zip(x.split(50000), g.split(50000)):
+        rows, grad = rows.double(), grad.double()
+        pg, pu = (rows @ wide.t() + b.double()).split(n, 1)
+        a, slope = (pg.clamp(min=0), (pg > 0).double()) if act == "relu" else (pg, torch.ones_like(pg))
+        d = torch.cat([grad * pu * slope, grad * a], 1)
+        outs.append(a * pu)
+        dxs.append(d @ wide)
+        dw += d.t() @ rows
+        db += d.sum(0)
+        most = max(most, dw.abs().max().item(), db.abs().max().item(), d.abs().max().item())
+    return torch.cat(outs), torch.cat(dxs), dw, db, most
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", ["none", "relu"])
+@pytest.mark.parametrize("shape", [(700001, 64, 64), (300007, 61, 59), (400003, 24, 40),
+                                   (900001, 8, 8), (500001, 64, 24), (300001, 40, 64),
+                                   (200001, 72, 136), (38000, 200, 72)])
+def test_every_row_counts_once(shape, act, dtype, cuda_device):
+    """Whole numbers, whose sums over many tiles are exact: a tile that is left out, taken twice
+    or read too early shows whatever the bounds of rounding.  Each set of gradients that a
+    caller can ask for, in rows of W of their own distance too."""
+    m, k, n = shape
+    x, w, b, g = whole_operands(m, k, n, dtype, cuda_device, 150)
+    y, *grads, most = exact_step(x, w, b, act, g)
+    assert most < 2 ** 22  # far from where float32 stops holding whole numbers, on the way too
+    want = [t.to(dtype) for t in grads]
+    from ictc_o2_hp_b200 import dense
+    apart = torch.cat([w, w.new_zeros(2 * n, 16)], 1)[:, :k]
+    for needs in ((1, 1, 1), (1, 0, 0), (0, 1, 0), (0, 0, 1), (1, 1, 0), (0, 1, 1), (1, 0, 1)):
+        for weight in (w, apart) if all(needs) else (w,):
+            leaves = [t.detach().requires_grad_(bool(q)) for t, q in zip((x, weight, b), needs)]
+            out = dense.gated_linear(*leaves, activation=act)
+            assert torch.equal(out, y.to(dtype))
+            asked = [t for t in leaves if t.requires_grad]
+            got = torch.autograd.grad(out, asked, g)
+            assert all(map(torch.equal, got, [t for t, q in zip(want, needs) if q])), needs
+
+
+def test_weight_gradients_past_32_bits(cuda_device):
+    """D of more than 2^31 elements: every row's part of dW and db, exactly."""
+    x, w, b, _ = whole_operands(140001, 16, 8192, torch.bfloat16, cuda_device, 151)
+    g = x.new_ones(1).expand(140001, 8192)
+    y, (dx, dw, db) = step(x, w, b, "none", g)
+    y64, dx64, dw64, db64, most = exact_step(x, w, b, "none", g)
+    assert most < 2 ** 22
+    for got, want in ((y, y64), (dx, dx64), (dw, dw64), (db, db64)):
+        assert torch.equal(got, want.to(got.dtype))
+
+
 def test_offsets_past_32_bits(cuda_device):
     """p and D of more than 2^31 elements, y of more than 2^30: rows on both sides of such
     offsets, the last ones, and the bias gradient over all."""
