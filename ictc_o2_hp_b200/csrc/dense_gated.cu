@@ -231,8 +231,8 @@ __global__ void __launch_bounds__(kNormThreads)
 
 // Gate columns of preact that lie near 0 by fused multiply-adds in the order of k, bias last.
 // One pass over the gate half, a run of segments a warp; what is near 0 in them then goes to a lane
-// each.  float32 65,536 x 128 x 512, where that is 4 elements in 10^5: 11 us for the norms and 66;
-// 4,096 x 16,384 x 2,048, 35 in 10^4 and long sums: 138 and 1,840 of a step's 13,000.
+// each.  float32 65,536 x 128 x 512, where that is 4 elements in 10^5: 11 us for the norms and 43;
+// 4,096 x 16,384 x 2,048, 35 in 10^4 and long sums: 138 and 1,480 of a step's 12,600.
 constexpr int kSettleWarps = 8, kSettleLoads = 8, kSettleRun = 32;
 
 // V: elements of a load of preact, whose row lengths are whole ones; U: of x and W.  `run`
@@ -282,7 +282,7 @@ __global__ void __launch_bounds__(kSettleWarps * 32)
         const Pack<float, V> most = *reinterpret_cast<const Pack<float, V>*>(norms + cols[i]);
 #pragma unroll
         for (int j = 0; j < V; ++j)
-          if (fabsf(p[i].v[j]) <= fmaf(size[i], most.v[j], 1.1754944e-38f)) mine |= 1u << (i * V + j);
+          if (is_near(p[i].v[j], size[i] * most.v[j])) mine |= 1u << (i * V + j);
       }
       for (; mine != 0; mine &= mine - 1) {
         const int bit = __ffs(mine) - 1;

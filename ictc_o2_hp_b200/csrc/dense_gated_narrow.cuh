@@ -509,8 +509,15 @@ __device__ __forceinline__ void take_orders(uint32_t at, float2 (&v)[4]) {
 
 // Relu in float32: gate projections within the bounds of their error are computed again, in the
 // order of k and the bias last, so that the slope is that of every other path.  |x|_2 |w|_2
-// bounds a row's sums; a warp takes the few such elements (2 in 10^5) together, a lane its part
-// of x and W.  1,048,576 x 64 x 64 backward: 453 us, without it 404.
+// bounds a row's sums; a lane adds up those of its row (2 elements in 10^5 as a rule) from the
+// parts in shared memory.  1,048,576 x 64 x 64 backward: 445 us, without it 404; with whole
+// numbers for operands, where one in 14 is 0, some 2.4 times that.
+
+// Whether a p that may be off by `error` may have another sign.  Rows and columns of zeros have
+// no error, those with an infinity no p of a finite value.
+__device__ __forceinline__ bool is_near(float p, float error) {
+  return error > 0.f && error <= 3.402823466e38f && fabsf(p) <= error;
+}
 
 // At least |x_r|_2 of a row of the x tile, from its leading parts: bf16 sums of 32 squares each
 // of the two halves, low by less than the fifth that is added.  Where squares leave the range,
@@ -558,56 +565,60 @@ __device__ __forceinline__ void stage_gate_sizes(float* to, const GatedNarrowArg
   }
 }
 
+// Four values of a row from the parts of an operand, exactly.
+__device__ __forceinline__ void join_unit(const unsigned char* operand, int row, int unit,
+                                          float (&v)[4]) {
+  const unsigned char* at = operand + swizzled(row, unit >> 1) + (unit & 1) * 8;
+  float part[3][4];
+#pragma unroll
+  for (int q = 0; q < 3; ++q) {
+    const uint2 u = *reinterpret_cast<const uint2*>(at + q * kGatedBlock);
+    part[q][0] = __uint_as_float(u.x << 16);
+    part[q][1] = __uint_as_float(u.x & 0xffff0000u);
+    part[q][2] = __uint_as_float(u.y << 16);
+    part[q][3] = __uint_as_float(u.y & 0xffff0000u);
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = part[0][j] + (part[1][j] + part[2][j]);
+}
+
 // Whole warp: the gate projections of the columns `col` to col + 7 of a row a lane; those of a
-// row may be off by `near` times a column's size (negative: no row).
+// row may be off by `near` times a column's size (0: no row).
 __device__ __forceinline__ void settle_gate(float2 (&gate)[4], float near, float most,
                                             const float* sizes, const float* bias,
-                                            const GatedNarrowArgs& p, int64_t row0, int col,
-                                            int lane) {
-  constexpr float kLeast = 1.1754944e-38f;
-  if (col >= p.n) return;
+                                            const unsigned char* x, const unsigned char* w, int n,
+                                            int k, int row, int col) {
+  if (col >= n) return;
   const auto least = [](float2 a, float2 b) {
     return fminf(fminf(fabsf(a.x), fabsf(a.y)), fminf(fabsf(b.x), fabsf(b.y)));
   };
   float low = least(gate[0], gate[1]);
-  if (col + 4 < p.n) low = fminf(low, least(gate[2], gate[3]));  // n is a multiple of 4
-  const bool some = near >= 0.f && low <= fmaf(near, most, kLeast);
-  if (!__any_sync(0xffffffffu, some)) return;
+  if (col + 4 < n) low = fminf(low, least(gate[2], gate[3]));  // n is a multiple of 4
+  if (!__any_sync(0xffffffffu, is_near(low, near * most))) return;
   uint32_t mine = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float v = i % 2 ? gate[i / 2].y : gate[i / 2].x;
-    if (near >= 0.f && col + i < p.n && fabsf(v) <= fmaf(near, sizes[col + i], kLeast))
-      mine |= 1u << i;
+    if (col + i < n && is_near(v, near * sizes[col + i])) mine |= 1u << i;
   }
 #pragma unroll 1
-  for (uint32_t lanes = __ballot_sync(0xffffffffu, mine != 0); lanes != 0;
-       lanes = __ballot_sync(0xffffffffu, mine != 0)) {
-    const int from = __ffs(lanes) - 1;
-    const int i = __ffs(__shfl_sync(0xffffffffu, mine, from)) - 1;
-    const float* x = static_cast<const float*>(p.x) + (row0 + from) * p.k;
-    const float* w = static_cast<const float*>(p.w) + (col + i) * p.ldw;
-    float xs[2], ws[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int at = h * 32 + lane;
-      xs[h] = at < p.k ? x[at] : 0.f;
-      ws[h] = at < p.k ? w[at] : 0.f;
-    }
+  for (; mine != 0; mine &= mine - 1) {
+    const int i = __ffs(mine) - 1;
     float sum = 0.f;
+#pragma unroll 1
+    for (int u = 0; 4 * u < k; ++u) {
+      float a[4], b[4];
+      join_unit(x, row, u, a);
+      join_unit(w, col + i, u, b);
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll 8
-      for (int s = 0; s < 32 && h * 32 + s < p.k; ++s)
-        sum = fmaf(__shfl_sync(0xffffffffu, xs[h], s), __shfl_sync(0xffffffffu, ws[h], s), sum);
-    sum += bias[col + i];
-    if (lane == from) {
-      mine &= mine - 1;
-#pragma unroll
-      for (int q = 0; q < 8; ++q)
-        if (q == i) (q % 2 ? gate[q / 2].y : gate[q / 2].x) = sum;
+      for (int j = 0; j < 4; ++j) sum = fmaf(a[j], b[j], sum);
     }
+    sum += bias[col + i];
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      if (q == i) (q % 2 ? gate[q / 2].y : gate[q / 2].x) = sum;
   }
+  __syncwarp();
 }
 
 template <typename T, int ACT>
@@ -896,7 +907,7 @@ __global__ void __launch_bounds__(kBackThreads, 1)
         seen |= q[0];
       }
       release_slot(&g_read[b], seen, lane);
-      float near = -1.f;
+      float near = 0.f;
       if constexpr (kSettles) {  // while the tensor cores form p
         ok = mbar_wait_warp(&x_full[b], phase, kCodeEpilogue);
         if (!ok) break;
@@ -926,8 +937,7 @@ __global__ void __launch_bounds__(kBackThreads, 1)
         add_bias(gate, bias + c0 + j);
         add_bias(up, bias + kNarrow + c0 + j);
         if constexpr (kSettles)
-          settle_gate(gate, near, most, sizes, bias, p,
-                      static_cast<int64_t>(t) * kNarrowTile + quad * 32, c0 + j, lane);
+          settle_gate(gate, near, most, sizes, bias, x_tiles, weights, p.n, p.k, in_tile, c0 + j);
         if (!whole && !in) {  // no gradient past the last row, but a bias that may be infinite
 #pragma unroll
           for (int i = 0; i < 4; ++i) gate[i] = up[i] = make_float2(0.f, 0.f);

@@ -164,6 +164,33 @@ def test_many_tiles(shape, dtype, cuda_device):
         assert all(torch.equal(p, q) for p, q in zip(out, first))
 
 
+@pytest.mark.parametrize("shape", [(300, 64, 64), (5, 8, 4), (300, 72, 40), (300, 33, 77), (40, 2048, 24)])
+def test_relu_of_zero_and_infinite_rows(shape, cuda_device):
+    """Rows and columns of zeros have a p of exactly 0 and relu's slope there, which is 0;
+    infinities have the slope of their sign, and NaN has none."""
+    m, k, n = shape
+    x, w, _, g = operands(m, k, n, torch.float32, cuda_device, 142, bias=False)
+    x[1] = 0
+    x[m - 1] = 0
+    w[2] = 0
+    base = step(x, w, None, "relu", g)
+    for t in (base[1][0], base[1][1]):
+        assert t.isfinite().all()
+    assert not base[1][0][1].any() and not base[1][0][m - 1].any() and not base[1][1][2].any()
+    pg, pu, a, s, y64, d, dx, dw, _ = gated64(x, w, None, "relu", g)
+    check_gated(x, w, None, "relu", g, base[0], (*base[1], None), torch.float32)
+    x[3, 5] = math.inf
+    w[:, 5] = w[:, 5].abs() + 0.1
+    w[1, 5] = -1.0
+    w[n + 1, 5] = 1.0
+    y, (dx, dw) = step(x, w, None, "relu", g)
+    want = torch.full((n,), math.inf, device=cuda_device)
+    want[1] = math.nan  # relu(-inf) inf
+    assert torch.equal(y[3].isnan(), want.isnan()) and torch.equal(y[3].isinf(), want.isinf())
+    keep = torch.arange(m, device=cuda_device) != 3
+    assert dx[keep].isfinite().all() and not dx[3].isfinite().any()
+
+
 def whole_operands(m, k, n, dtype, device, seed):
     """Operands of -1, 0 and 1: with an activation of slope 0 or 1 every product and sum is a
     whole number below 2^24, exact in float32 in any order, and D is exact in every type."""
