@@ -374,7 +374,9 @@ ICTC_API int32_t ictc_o2_linear_backward(
 /* The gated linear layer: (pg | pu) = x weight^T + bias, y = act(pg) pu with weight
  * [2 hidden, in] and bias [2 hidden] or null (the gate's rows first), y [rows, hidden].
  * Rows of x and of weight do not overlap.  preact [rows, 2 hidden] receives pg and pu in
- * float32 for the backward, or is null: the backward then computes them again.
+ * float32 for the backward, or is null: the backward then computes them again.  In float32
+ * with relu a pg within its rounding of 0 is, for the backward, that of fused multiply-adds in the
+ * order of in, the bias last.
  * `keep` of the workspace query: whether both directions are given preact.  The layout
  * flags are those of x and weight. */
 ICTC_API int32_t ictc_o2_gated_linear_workspace(int64_t rows, int64_t in, int64_t hidden,

@@ -674,6 +674,42 @@ def test_other_stream_and_graph_capture(shape, dtype, cuda_device):
         assert torch.equal(out[0], want[0]) and all(map(torch.equal, out[1:], want[1]))
 
 
+@pytest.mark.parametrize("shape", [(5, 8, 4), (2000, 64, 64), (700, 200, 72), (300, 33, 77)])
+def test_relu_captured_and_traced(shape, cuda_device):
+    """The passes that decide relu's slopes in a captured step, beside another captured one, and
+    through the dispatcher."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    from ictc_o2_hp_b200 import dense
+    x, w, b, g = operands(*shape, torch.float32, cuda_device, 127)
+    want = step(x, w, b, "relu", g)
+    leaves = [torch.zeros_like(t).requires_grad_(True) for t in (x, w, b)]
+    held = torch.zeros_like(g)
+    graphs, outs = [], []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = dense.gated_linear(*leaves, activation="relu")
+            outs.append((y, *torch.autograd.grad(y, leaves, held)))
+        graphs.append(graph)
+    with torch.no_grad():
+        for t, source in zip((*leaves, held), (x, w, b, g)):
+            t.copy_(source)
+    for graph in graphs:
+        graph.replay()
+    for out in outs:
+        assert torch.equal(out[0], want[0]) and all(map(torch.equal, out[1:], want[1]))
+
+    def whole(x, w, b):
+        y = dense.gated_linear(x, w, b, "relu")
+        return (y, *torch.autograd.grad(y, (x, w, b), g))
+
+    leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]
+    got = make_fx(whole)(*leaves)(*leaves)
+    # the recorded step may keep p where the other computes it again: other kernels, same slopes
+    check_gated(x, w, b, "relu", g, got[0].detach(), got[1:], torch.float32)
+
+
 def test_compile_and_traces(cuda_device):
     from torch.fx.experimental.proxy_tensor import make_fx
 
