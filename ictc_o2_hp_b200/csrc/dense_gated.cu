@@ -178,7 +178,8 @@ inline float near_zero(int64_t k) {
 }
 
 // |w_c|_2 of the n gate rows of W, then |x_r|_2 of the m rows of x; `lanes` of a warp a row,
-// kNormRows rows in flight.  Squares that leave float32's range are taken again in float64.
+// kNormRows rows in flight.  Squares of finite values that leave float32's range are taken again
+// in float64.
 constexpr int kNormThreads = 256, kNormRows = 4;
 
 template <int V>
@@ -193,11 +194,11 @@ __global__ void __launch_bounds__(kNormThreads)
        base += step) {
     const int64_t r0 = base + threadIdx.x / lanes;
     const float* row[kNormRows];
-    float sum[kNormRows];
+    float sum[kNormRows], most[kNormRows];
 #pragma unroll
     for (int q = 0; q < kNormRows; ++q) {
       row[q] = row_at(r0 + q * rows < total ? r0 + q * rows : 0);
-      sum[q] = 0.f;
+      sum[q] = most[q] = 0.f;
     }
 #pragma unroll 2
     for (int64_t c = part * V; c < k; c += lanes * V) {
@@ -207,16 +208,22 @@ __global__ void __launch_bounds__(kNormThreads)
 #pragma unroll
       for (int q = 0; q < kNormRows; ++q)
 #pragma unroll
-        for (int j = 0; j < V; ++j) sum[q] = fmaf(v[q].v[j], v[q].v[j], sum[q]);
+        for (int j = 0; j < V; ++j) {
+          sum[q] = fmaf(v[q].v[j], v[q].v[j], sum[q]);
+          most[q] = fmaxf(most[q], fabsf(v[q].v[j]));
+        }
     }
 #pragma unroll
     for (int q = 0; q < kNormRows; ++q)
-      for (int o = lanes / 2; o > 0; o >>= 1) sum[q] += __shfl_xor_sync(0xffffffffu, sum[q], o);
+      for (int o = lanes / 2; o > 0; o >>= 1) {
+        sum[q] += __shfl_xor_sync(0xffffffffu, sum[q], o);
+        most[q] = fmaxf(most[q], __shfl_xor_sync(0xffffffffu, most[q], o));
+      }
 #pragma unroll
     for (int q = 0; q < kNormRows; ++q) {
       if (part != 0 || r0 + q * rows >= total) continue;
       float norm = sqrtf(sum[q]);
-      if (!(sum[q] >= 1e-30f && sum[q] <= 1e38f)) {
+      if ((sum[q] < 1e-30f || sum[q] > 1e38f) && most[q] > 0.f && most[q] <= 3.402823466e38f) {
         double wide = 0.0;
         for (int64_t c = 0; c < k; ++c) {
           const double v = row[q][c];

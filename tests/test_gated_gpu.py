@@ -164,6 +164,30 @@ def test_many_tiles(shape, dtype, cuda_device):
         assert all(torch.equal(p, q) for p, q in zip(out, first))
 
 
+@pytest.mark.parametrize("scale", [1e-18, 1e-13, 1e15, 1e17])
+@pytest.mark.parametrize("shape", [(300, 64, 64), (300, 72, 40), (300, 33, 77)])
+def test_relu_slopes_of_small_and_large_operands(shape, scale, cuda_device):
+    """Operands whose squares leave float32's range while their products do not."""
+    from ictc_o2_hp_b200 import dense
+    m, k, n = shape
+    x, w, _, g = operands(m, k, n, torch.float32, cuda_device, 143, bias=False)
+    x, w = x * scale, w * scale
+    at = torch.arange(n, device=cuda_device)
+    p = in_order(x, w[:n])
+    b = torch.zeros(2 * n, device=cuda_device)
+    b[:n] = -torch.nextafter(p[at * 37 % m, at], torch.full((n,), math.inf, device=cuda_device))
+    p = p + b[:n]
+    native, code = dense._load(), dense.ACTIVATIONS["relu"]
+    _, kept = native.gated_forward(x, w, b, code, True)
+    assert torch.equal(kept[:, :n] > 0, p > 0)
+    y, (dx, dw, db) = step(x, w, b, "relu", torch.ones_like(g))
+    pu = (x.double() @ w.double()[n:].t())
+    want = (pu * (p > 0)).sum(0)
+    size = (pu.abs() * (p > 0)).sum(0) + sum_error(k) * (x.double().abs() @ w.double()[n:].abs().t()).sum(0)
+    within("dbias", db[:n], want, sum_error(k) * (x.double().abs() @ w.double()[n:].abs().t()).sum(0) +
+           (m + 64) * U * size)
+
+
 @pytest.mark.parametrize("shape", [(300, 64, 64), (5, 8, 4), (300, 72, 40), (300, 33, 77), (40, 2048, 24)])
 def test_relu_of_zero_and_infinite_rows(shape, cuda_device):
     """Rows and columns of zeros have a p of exactly 0 and relu's slope there, which is 0;
